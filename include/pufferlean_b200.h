@@ -525,6 +525,58 @@ int pl_ckpt_read(const char* path, double* w, size_t cap, size_t* P);
 int pl_policy_save(size_t handle, size_t P, const char* path);
 int pl_policy_restore(const char* path, size_t* P, size_t* handle);
 
+/* ------------------------------------------------------------------ token policies ------------ */
+/* A policy whose actions are tokens of a large vocabulary: the layer norm in front of its head, the head with its
+ * cross entropy, and distillation of a teacher's top logits into it (no reference counterpart; the update paths
+ * above stop at heads of 128 outputs). All pointers are device pointers, all calls enqueue on `stream` and return
+ * without waiting. Matrices are row-major with a row stride in elements; bf16 rows that start at 16-byte boundaries
+ * with a stride that is a multiple of 8 go to the tensor cores as they lie, others are copied first. Workspaces are
+ * the caller's (256-byte aligned, no contents kept between calls): calls on several streams need one each.
+ *
+ * Gradients here are of sum_n scale_n loss_n (descent); Muon ascends, so pass negative scales for it. */
+
+/* Layer norm over the columns of x [rows x cols] (f32, or bf16 with bf16 = 1; y likewise): y = (x - mean) rstd w + b,
+ * rstd = 1 / sqrt(var + eps). w, b [cols] f32, each may be NULL; mean, rstd [rows] f32 are written for the gradient. */
+int pl_layernorm_dev(const void* x, size_t ldx, const float* w, const float* b, size_t rows, size_t cols, double eps,
+                     uint8_t bf16, void* y, size_t ldy, float* mean, float* rstd, void* stream);
+/* Its gradient: dx (x's type), and, where not NULL, dw[c] = sum_rows dy xhat and db[c] = sum_rows dy (f32, summed in a
+ * fixed order). ws: pl_layernorm_grad_ws(rows, cols) bytes when dw or db is wanted. */
+size_t pl_layernorm_grad_ws(size_t rows, size_t cols);
+int pl_layernorm_grad_dev(const void* dy, size_t lddy, const void* x, size_t ldx, const float* w, const float* mean,
+                          const float* rstd, size_t rows, size_t cols, uint8_t bf16, void* dx, size_t lddx, float* dw,
+                          float* db, void* ws, size_t ws_bytes, void* stream);
+
+/* The head's logits are u = (x w^T + bias) / temperature with x [N x D], w [V x D], bias [V] or NULL, all bf16
+ * (f32 accumulation); they are never written out. loss, lse [N] f32.
+ *
+ * Cross entropy: target [N] int32, loss_n = lse_n - u_n,target (minus the log-probability of the target). A negative
+ * target leaves the row out: loss = lse = 0, no gradient, and no work in the products. A target >= V makes the row's
+ * loss (and the gradients) NaN.
+ * Distillation: ids, teacher [N x K] (int32, f32 logits); a negative id or a teacher logit of -inf is an absent entry.
+ * p = softmax(teacher / temperature) over the present entries, loss_n = sum_k p_k (log p_k - u_n,id_k) + lse_n = KL(p | q).
+ * A row with no entry is left out like a negative target; entries that name the same id add up.
+ *
+ * ws: pl_vocab_ws bytes (K = 1 for the cross entropy; aligned = 1 when x, w and dx start at 16 bytes with row strides
+ * that are multiples of 8). The gradient forms keep one piece of rows' softmax terms there (2 bytes each): piece_bytes
+ * bounds that piece, 0 = 4 GiB; the results do not depend on it beyond the order of dw's f32 sums.
+ * dx [N x D] bf16; dw [V x D] and dbias [V] (given exactly when bias is) bf16, or f32 with dw_f32 = 1 (f32 sums of
+ * products of bf16-rounded gradients). row_scale [N] f32 or NULL (ones). */
+size_t pl_vocab_ws(size_t N, size_t V, size_t D, size_t K, uint8_t bias, uint8_t grad, uint8_t aligned,
+                   size_t piece_bytes);
+int pl_vocab_ce_dev(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, const int32_t* target,
+                    size_t N, size_t V, size_t D, float* loss, float* lse, void* ws, size_t ws_bytes, void* stream);
+int pl_vocab_ce_grad_dev(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, const int32_t* target,
+                         const float* row_scale, size_t N, size_t V, size_t D, float* loss, float* lse, void* dx,
+                         size_t lddx, void* dw, size_t lddw, void* dbias, uint8_t dw_f32, size_t piece_bytes, void* ws,
+                         size_t ws_bytes, void* stream);
+int pl_vocab_distill_dev(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, const int32_t* ids,
+                         const float* teacher, size_t K, double temperature, size_t N, size_t V, size_t D, float* loss,
+                         float* lse, void* ws, size_t ws_bytes, void* stream);
+int pl_vocab_distill_grad_dev(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, const int32_t* ids,
+                              const float* teacher, size_t K, double temperature, const float* row_scale, size_t N,
+                              size_t V, size_t D, float* loss, float* lse, void* dx, size_t lddx, void* dw, size_t lddw,
+                              void* dbias, uint8_t dw_f32, size_t piece_bytes, void* ws, size_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------ dashboard losses ----------- */
 /* The reference's 7-loss channel [policy, value, entropy, total, old_kl, kl, clipfrac]
  * (ffi/puffercuda.cu:251-262, 336-352). */

@@ -124,13 +124,14 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
   memset(&mc, 0, sizeof(mc));
   memset(&mc2, 0, sizeof(mc2));
   ep.tma_out = 0;
-  if (epi == EPI_FWD || epi == EPI_DGRAD || epi == EPI_BF16) {
+  if (epi == EPI_FWD || epi == EPI_DGRAD || epi == EPI_BF16 || (epi == EPI_VOCAB && ep.out)) {
     bool ok = gemm_store_map(&mc, ep.out, ep.out_rows, ep.out_cols, ep.ldo, batch, ep.out_bstride);
     if (ok && epi == EPI_FWD && ep.out2) ok = gemm_store_map(&mc2, ep.out2, ep.out_rows, ep.out_cols, ep.ldo2, 1, 0);
     // the staged epilogue reads its aux tile with aligned 16-byte loads
     if (ok && ep.aux && (((uintptr_t)ep.aux & 15) || (ep.ld_aux % 8) || (batch > 1 && (ep.aux_bstride % 8))))
       ok = false;
     ep.tma_out = ok ? 1 : 0;
+    PL_REQUIRE(ok || epi != EPI_VOCAB, PL_ERR_INVALID, "the head's exponentials need a TMA store map");
   }
   if (at) {
     // the aux operand map ({64, 128} boxes, 128-byte swizzle) rides in the second store map's slot

@@ -13,6 +13,8 @@
 // Tiles are BM=128 x BN, BK=64 (one 128-byte swizzle atom of bf16 per row); the kernel is
 // persistent, one CTA per SM.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "pl_common.cuh"
 #include "pl_tc.cuh"
 
@@ -24,6 +26,8 @@ enum EpiKind : int {
   EPI_FWD = 2,    // z = acc + bias; out(bf16) = act(z); out2(bf16) = z (GELU only)
   EPI_DGRAD = 3,  // out(bf16) = acc * act'(aux); column partial sums of it  [bias grads]
   EPI_PPO = 4,    // logits+value = acc + bias -> PPO objective gradient dOut(bf16) + column sums
+  EPI_VOCAB = 5,  // u = acc * scale2 + bias2 (log2 units) -> per row and BN/2 columns: max, sum of 2^(u - max);
+                  // optionally out(f16) = 2^(u - max + 15)  [large-vocabulary heads]
 };
 
 struct EpiArgs {
@@ -64,6 +68,18 @@ struct EpiArgs {
   // fold_scale[batch] for the next product. Every warp computes the same s.
   float* fold_scale;
   double fold_eps;
+  // EPI_VOCAB: u = acc * scale2 + bias2[col] (bias2 optional, f32, padded to whole tiles), and the segment
+  // statistics [rows][ld_stat] (max, sum) of every row
+  float scale2;
+  const float* bias2;
+  float2* stat;
+  long ld_stat;
+  // EPI_F32, optional: out += alpha*acc instead of out = alpha*acc
+  int accum;
+  // Rows that exist (optional): the extent M (dyn_k = 0) or K (dyn_k = 1) of this call is
+  // clamp(*dyn_rows - dyn_off, 0, extent given by the host).
+  const int* dyn_rows;
+  int dyn_off, dyn_k;
 };
 
 // s = 1 / (sqrt(sum_i diag_i) + eps) over the m bf16 diagonal entries of a matrix (leading dimension
@@ -142,6 +158,21 @@ __device__ __forceinline__ void store_row16_f32(float* p, const float (&v)[16], 
     for (int j = 0; j < 4; j++) reinterpret_cast<float4*>(p)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   } else {
     for (int j = 0; j < nvalid; j++) p[j] = v[j];
+  }
+}
+__device__ __forceinline__ void load_row16_f32(const float* p, float (&v)[16], int nvalid, bool vec) {
+  if (vec && nvalid == 16 && ((uintptr_t)p & 15) == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float4 f = reinterpret_cast<const float4*>(p)[j];
+      v[4 * j] = f.x;
+      v[4 * j + 1] = f.y;
+      v[4 * j + 2] = f.z;
+      v[4 * j + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] = (j < nvalid) ? p[j] : 0.f;
   }
 }
 __device__ __forceinline__ void load_row16_bf16(const __nv_bfloat16* p, float (&v)[16], int nvalid, bool vec) {
@@ -268,8 +299,8 @@ struct GemmSmem {
   static constexpr uint32_t A_BYTES = BM * BK * 2;
   static constexpr uint32_t B_BYTES = BN * BK * 2;
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int NOUT = EPI == EPI_FWD ? 2 : ((EPI == EPI_DGRAD || EPI == EPI_BF16) ? 1 : 0);
-  static constexpr int STG_BUFS = (EPI == EPI_BF16 || AT) ? 2 : 1;
+  static constexpr int NOUT = EPI == EPI_FWD ? 2 : ((EPI == EPI_DGRAD || EPI == EPI_BF16 || EPI == EPI_VOCAB) ? 1 : 0);
+  static constexpr int STG_BUFS = (EPI == EPI_BF16 || EPI == EPI_VOCAB || AT) ? 2 : 1;
   static constexpr uint32_t STG_ONE = NOUT * 32 * 32 * 2;
   static constexpr uint32_t STG_WARP = STG_BUFS * STG_ONE;
   static constexpr uint32_t STG_BYTES = 8 * STG_WARP;
@@ -296,6 +327,26 @@ __device__ __forceinline__ TileIdx tile_of(int t, int num_n, int num_m) {
   r.m = q % num_m;
   r.z = q / num_m;
   return r;
+}
+
+// Order of the head's logit tiles (EPI_VOCAB): the weight matrix is the large operand, so m is the fast
+// index inside groups of 32 row tiles: the CTAs that run at one time share a few column panels of the
+// weights (read once from HBM per group) and the group's 4,096 rows stay in L2.
+constexpr int kVocabGroupM = 32;
+template <int EPI>
+__device__ __forceinline__ TileIdx tile_at(int t, int num_n, int num_m) {
+  if constexpr (EPI == EPI_VOCAB) {
+    const int g = t / (kVocabGroupM * num_n), first = g * kVocabGroupM;
+    const int gm = min(kVocabGroupM, num_m - first);
+    const int q = t - g * (kVocabGroupM * num_n);
+    TileIdx r;
+    r.n = q / gm;
+    r.m = first + q - r.n * gm;
+    r.z = 0;
+    return r;
+  } else {
+    return tile_of(t, num_n, num_m);
+  }
 }
 
 // Epilogue of one 128 x BN accumulator tile held in TMEM columns [tcol, tcol + BN).
@@ -349,6 +400,104 @@ __device__ __forceinline__ void aux_smem32(const uint8_t* aux_sm, int rl, int c3
   const int q0 = (c32 & 63) >> 3;
 #pragma unroll
   for (int i = 0; i < 4; i++) o[i] = *reinterpret_cast<const uint4*>(base + (((q0 + i) ^ (rl & 7)) << 4));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// EPI_VOCAB: this warp's 32 rows x BN/2 columns of a logit tile, one row per lane, its BN/2 accumulators in
+// registers. In log2 units u = acc * scale2 + bias2, m = max u, s = sum 2^(u - m): the pair goes to
+// stat[row][2 n_tile + half]. With tma_out the terms leave as f16 scaled by 2^15, so the largest is 2^15
+// exactly and 11 bits of mantissa hold down to 2^-29 of it; bf16 would cost a second rounding of 2^-8 when
+// the gradient is formed from them. Columns past the vocabulary count as -inf.
+template <int BN>
+__device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, uint32_t t_row, int m_tile, int n_tile, int rows,
+                                               int sub, int half, int lane, uint8_t* stg, const CUtensorMap* tmC,
+                                               uint32_t& seq) {
+  constexpr int W = BN / 2, NQ = W / 16;
+  const int row0 = m_tile * 128 + sub * 32;
+  const int n0 = n_tile * BN + half * W;
+  const int left = ep.out_cols - n0;
+  if (row0 >= rows || left <= 0) {  // warp-uniform: nothing of this warp's part exists
+    if (row0 < rows && row0 + lane < rows)
+      ep.stat[(long)(row0 + lane) * ep.ld_stat + 2 * n_tile + half] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+  uint32_t r[NQ][16];
+#pragma unroll
+  for (int q = 0; q < NQ; q++) tc::tmem_ld16(t_row + half * W + 16 * q, r[q]);
+  tc::tmem_wait_ld();
+#pragma unroll
+  for (int q = 0; q < NQ; q++) tc::tmem_tie16(r[q]);
+  float v[W];
+#pragma unroll
+  for (int j = 0; j < W; j++) v[j] = __uint_as_float(r[j >> 4][j & 15]);
+  float scale = ep.scale2;
+  if (ep.bias2) {
+    const float4* b4 = reinterpret_cast<const float4*>(ep.bias2 + n0);
+#pragma unroll
+    for (int j = 0; j < W / 4; j++) {
+      const float4 b = __ldg(b4 + j);
+      v[4 * j] = __fmaf_rn(v[4 * j], scale, b.x);
+      v[4 * j + 1] = __fmaf_rn(v[4 * j + 1], scale, b.y);
+      v[4 * j + 2] = __fmaf_rn(v[4 * j + 2], scale, b.z);
+      v[4 * j + 3] = __fmaf_rn(v[4 * j + 3], scale, b.w);
+    }
+    scale = 1.f;
+  }
+  if (left < W) {
+#pragma unroll
+    for (int j = 0; j < W; j++) v[j] = j < left ? v[j] : -INFINITY;
+  }
+  float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int j = 4; j < W; j += 4) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) mx[i] = fmaxf(mx[i], v[j + i]);
+  }
+  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;  // scale > 0
+  const float ref = top == -INFINITY ? 0.f : top;  // a row with nothing but -inf here: every term 0
+  const float shift = 15.f - ref;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < W; j++) {
+    v[j] = ex2(__fmaf_rn(v[j], scale, shift));
+    sum[j & 3] += v[j];
+  }
+  const float total = ((sum[0] + sum[1]) + (sum[2] + sum[3])) * (1.f / 32768.f);
+  if (row0 + lane < rows)
+    ep.stat[(long)(row0 + lane) * ep.ld_stat + 2 * n_tile + half] = make_float2(top, total);
+  if (!ep.tma_out) return;
+  const int nch = min(W / 32, (left + 31) >> 5);
+#pragma unroll
+  for (int ch = 0; ch < W / 32; ch++) {
+    if (ch >= nch) break;  // warp-uniform
+    uint8_t* st = stg + (seq & 1u) * GemmSmem<BN, EPI_VOCAB>::STG_ONE;
+    seq++;
+    if (lane == 0) tc::bulk_wait_read<1>();  // the store that last read this tile is done with it
+    __syncwarp();
+    uint8_t* row = st + lane * 64;
+    const int x = (lane >> 1) & 3;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      uint32_t u[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const __half2 h = __floats2half2_rn(v[32 * ch + 8 * c + 2 * k], v[32 * ch + 8 * c + 2 * k + 1]);
+        u[k] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      *reinterpret_cast<uint4*>(row + ((c ^ x) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    tc::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tc::tma_store_3d(tmC, st, n0 + 32 * ch, row0, 0);
+      tc::bulk_commit();
+    }
+  }
 }
 
 template <int BN, int EPI, int NB_ = GemmSmem<BN, EPI>::STG_BUFS>
@@ -782,6 +931,14 @@ __device__ __forceinline__ void epilogue_tile(const EpiArgs& ep, uint32_t t_row,
             v[j] = row == n0 + j ? __fadd_rn(t, ep.diag) : t;
           }
           const long off = (long)bz * ep.out_bstride + (long)row * ep.ldo + n0;
+          if constexpr (EPI == EPI_F32) {
+            if (ep.accum) {
+              float o[16];
+              load_row16_f32((const float*)ep.out + off, o, nvalid, (ep.ldo % 4) == 0);
+#pragma unroll
+              for (int j = 0; j < 16; j++) v[j] += o[j];
+            }
+          }
           if constexpr (EPI == EPI_F32)
             store_row16_f32((float*)ep.out + off, v, nvalid, (ep.ldo % 4) == 0);
           else
@@ -864,6 +1021,13 @@ __global__ void __launch_bounds__(320, 1)
   uint32_t* tmem_slot = (uint32_t*)(aux_empty + 2);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
+  if (ep.dyn_rows) {  // the rows that exist, counted on the device by an earlier kernel of the stream
+    const int have = max(0, *ep.dyn_rows - ep.dyn_off);
+    if (ep.dyn_k)
+      K = min(K, have);
+    else
+      M = min(M, have);
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_n = (N + BN - 1) / BN, num_m = (M + BM - 1) / BM;
   const int num_z = ep.k_splits > 1 ? ep.k_splits : (ep.nbatch > 1 ? ep.nbatch : 1);
@@ -918,7 +1082,7 @@ __global__ void __launch_bounds__(320, 1)
       long it = 0;
       long ja = 0;  // aux tiles issued (AT)
       for (int t = blockIdx.x; t < total_tiles && !*abort_flag; t += gridDim.x) {
-        const TileIdx ti = tile_of(t, num_n, num_m);
+        const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
         const int batch = ep.k_splits > 1 ? 0 : ti.z;
         int b0, b1;
         kb_range(ti.z, b0, b1);
@@ -975,7 +1139,7 @@ __global__ void __launch_bounds__(320, 1)
       long it = 0;
       int j = 0;
       for (int t = blockIdx.x; t < total_tiles && !*abort_flag; t += gridDim.x, j++) {
-        const TileIdx ti = tile_of(t, num_n, num_m);
+        const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
         int b0, b1;
         kb_range(ti.z, b0, b1);
         const int buf = j & 1;
@@ -1020,7 +1184,7 @@ __global__ void __launch_bounds__(320, 1)
     uint32_t stg_seq = 0;  // chunks this warp has staged: picks the staging tile
     int j = 0;
     for (int t = blockIdx.x; t < total_tiles; t += gridDim.x, j++) {
-      const TileIdx ti = tile_of(t, num_n, num_m);
+      const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
       int b0, b1;
       kb_range(ti.z, b0, b1);
       const int buf = j & 1;
@@ -1033,9 +1197,13 @@ __global__ void __launch_bounds__(320, 1)
       }
       tc::tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t)(buf * BN) + ((uint32_t)(sub * 32) << 16);
-      epilogue_tile<BN, EPI, S::STG_BUFS>(ep, t_row, ti.m, ti.n, ti.z, ep.k_splits > 1 ? 0 : ti.z, b1 > b0, sub, half,
-                                          lane, red, rowscr, stg_base + (warp - 2) * S::STG_WARP, &tmC, &tmC2,
-                                          stg_seq, AT ? sAux + buf * S::AUX_TILE : nullptr);
+      if constexpr (EPI == EPI_VOCAB)
+        epilogue_vocab<BN>(ep, t_row, ti.m, ti.n, M, sub, half, lane, stg_base + (warp - 2) * S::STG_WARP, &tmC,
+                           stg_seq);
+      else
+        epilogue_tile<BN, EPI, S::STG_BUFS>(ep, t_row, ti.m, ti.n, ti.z, ep.k_splits > 1 ? 0 : ti.z, b1 > b0, sub,
+                                            half, lane, red, rowscr, stg_base + (warp - 2) * S::STG_WARP, &tmC, &tmC2,
+                                            stg_seq, AT ? sAux + buf * S::AUX_TILE : nullptr);
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -1109,6 +1277,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
+  if (ep.dyn_rows) {  // the rows that exist, counted on the device by an earlier kernel of the stream
+    const int have = max(0, *ep.dyn_rows - ep.dyn_off);
+    if (ep.dyn_k)
+      K = min(K, have);
+    else
+      M = min(M, have);
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_ctarank();
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
@@ -1159,7 +1334,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
       // ---------------- TMA producer of this CTA's halves; the even CTA arms full[s] for both
       long it = 0;
       for (int t = pair; t < total_tiles && !*abort_flag; t += npairs) {
-        const TileIdx ti = tile_of(t, num_n, num_m);
+        const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
         const int batch = ep.k_splits > 1 ? 0 : ti.z;
         const int arow = ti.m * 2 * BM + (int)rank * BM;
         const int brow = ti.n * BN + (int)rank * BNH;
@@ -1202,7 +1377,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
       long it = 0;
       int j = 0;
       for (int t = pair; t < total_tiles && !*abort_flag; t += npairs, j++) {
-        const TileIdx ti = tile_of(t, num_n, num_m);
+        const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
         int b0, b1;
         kb_range(ti.z, b0, b1);
         const int buf = j & 1;
@@ -1248,7 +1423,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
     uint32_t stg_seq = 0;  // chunks this warp has staged: picks the staging tile
     int j = 0;
     for (int t = pair; t < total_tiles; t += npairs, j++) {
-      const TileIdx ti = tile_of(t, num_n, num_m);
+      const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
       int b0, b1;
       kb_range(ti.z, b0, b1);
       const int buf = j & 1;

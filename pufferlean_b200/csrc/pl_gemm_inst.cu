@@ -35,6 +35,11 @@ GemmKernel gemm_instance(int bn, int epi, bool a_mn, bool b_mn, uint32_t* smem) 
   PL_INST(128, false, true, EPI_BF16)
   PL_INST(256, false, false, EPI_BF16)
   PL_INST(256, false, true, EPI_BF16)
+  // the large-vocabulary head: logits, and the weight gradient in bf16
+  PL_INST(128, false, false, EPI_VOCAB)
+  PL_INST(256, false, false, EPI_VOCAB)
+  PL_INST(128, true, true, EPI_BF16)
+  PL_INST(256, true, true, EPI_BF16)
   // MLP forward / data-gradient / PPO head
   PL_INST(64, false, false, EPI_FWD)
   PL_INST(128, false, false, EPI_FWD)
