@@ -83,6 +83,14 @@ bool gemm_store_map(CUtensorMap* map, const void* ptr, long rows, long cols, lon
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int gemm_sms() {
+  static int num_sms[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && num_sms[dev] == 0) cudaDeviceGetAttribute(&num_sms[dev], cudaDevAttrMultiProcessorCount, dev);
+  return (dev >= 0 && dev < 64 && num_sms[dev] > 0) ? num_sms[dev] : 148;
+}
+
 int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const Operand& B, int M, int N, int K,
                 int batch, const EpiArgs& ep_in, cudaStream_t st) {
   const int bn_in = bn;
@@ -94,7 +102,7 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
              "GEMM B storage %ldx%ld too small for N=%d K=%d", B.rows, B.cols, N, K);
   uint32_t smem = 0;
   GemmKernel k = nullptr;
-  const bool pair = (g_pair_mode == 1 || (g_pair_mode == 2 && a_mn && b_mn)) && bn == 256 && epi != EPI_PPO && M > 128 &&
+  const bool pair = (g_pair_mode == 1 || (g_pair_mode == 2 && a_mn && b_mn)) && bn == 256 && epi != EPI_PPO && epi != EPI_SLICE && M > 128 &&
                     (k = gemm_pair_instance(bn, epi, a_mn, b_mn, &smem)) != nullptr;
   // the data gradient of a short-K product (the head's, K <= 128) is a memory-bound epilogue: 128-wide
   // tiles whose aux comes through TMA into shared memory (needs the staged stores, checked below)
@@ -124,15 +132,21 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
   memset(&mc, 0, sizeof(mc));
   memset(&mc2, 0, sizeof(mc2));
   ep.tma_out = 0;
-  if (epi == EPI_FWD || epi == EPI_DGRAD || epi == EPI_BF16 || (epi == EPI_VOCAB && ep.out)) {
+  if (epi == EPI_FWD || epi == EPI_DGRAD || epi == EPI_BF16) {
     bool ok = gemm_store_map(&mc, ep.out, ep.out_rows, ep.out_cols, ep.ldo, batch, ep.out_bstride);
     if (ok && epi == EPI_FWD && ep.out2) ok = gemm_store_map(&mc2, ep.out2, ep.out_rows, ep.out_cols, ep.ldo2, 1, 0);
     // the staged epilogue reads its aux tile with aligned 16-byte loads
     if (ok && ep.aux && (((uintptr_t)ep.aux & 15) || (ep.ld_aux % 8) || (batch > 1 && (ep.aux_bstride % 8))))
       ok = false;
     ep.tma_out = ok ? 1 : 0;
-    PL_REQUIRE(ok || epi != EPI_VOCAB, PL_ERR_INVALID, "the head's exponentials need a TMA store map");
   }
+  if (epi == EPI_SLICE)
+    PL_REQUIRE(batch == 1 && ep.k_splits <= 1 && ep.slabs && (((uintptr_t)ep.out | (uintptr_t)ep.slabs) & 31) == 0 &&
+                   ep.ldo % 8 == 0 && ep.ldo >= ep.out_cols,
+               PL_ERR_INVALID, "a sliced product needs slabs and 32-byte rows (ldo = %ld)", ep.ldo);
+  if (epi == EPI_VOCAB && ep.out)
+    PL_REQUIRE(((uintptr_t)ep.out & 31) == 0 && ep.ldo % 64 == 0 && ep.ldo >= ep.out_cols, PL_ERR_INVALID,
+               "the head's terms need 32-byte rows (ldo = %ld)", ep.ldo);
   if (at) {
     // the aux operand map ({64, 128} boxes, 128-byte swizzle) rides in the second store map's slot
     Operand aux{ep.aux, ep.out_rows, ep.out_cols, ep.ld_aux, 1, 0};
@@ -147,11 +161,7 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
   int splits = ep.k_splits > 1 ? ep.k_splits : 1;
   PL_REQUIRE(splits == 1 || batch == 1, PL_ERR_INVALID, "split-K and batching are exclusive");
   ep.nbatch = batch;
-  static int num_sms[64] = {0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && num_sms[dev] == 0) cudaDeviceGetAttribute(&num_sms[dev], cudaDevAttrMultiProcessorCount, dev);
-  const int sms = (dev >= 0 && dev < 64 && num_sms[dev] > 0) ? num_sms[dev] : 148;
+  const int sms = gemm_sms();
   dim3 grid;
   if (pair) {
     // one cluster of two CTAs per pair tile of 256 rows, at most one CTA per SM
@@ -160,7 +170,7 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
     grid = dim3((unsigned)(2 * pairs), 1, 1);
   } else {
     const long tiles = ceil_div(N, bn) * ceil_div(M, 128) * (long)(splits > 1 ? splits : batch);
-    grid = dim3((unsigned)(tiles < sms ? tiles : sms), 1, 1);
+    grid = dim3((unsigned)(tiles < sms && epi != EPI_SLICE ? tiles : sms), 1, 1);
   }
   static std::mutex mu;
   {

@@ -28,7 +28,32 @@ enum EpiKind : int {
   EPI_PPO = 4,    // logits+value = acc + bias -> PPO objective gradient dOut(bf16) + column sums
   EPI_VOCAB = 5,  // u = acc * scale2 + bias2 (log2 units) -> per row and BN/2 columns: max, sum of 2^(u - max);
                   // optionally out(f16) = 2^(u - max + 15)  [large-vocabulary heads]
+  EPI_SLICE = 6,  // out(f32) = acc; the tiles of an incomplete last wave are split along K (SliceShape)
 };
+
+// EPI_SLICE: tiles go to the CTAs in whole waves; the `rem` tiles of the last, incomplete one are cut along K into q
+// slices each, as many as keep every CTA busy, and the CTAs of one slice walk the same k-blocks at the same time (so
+// they still share what they read of the operands through L2; dealing the k-blocks out in one line, every CTA at
+// another place of the long axis, made the product of 4,096 x 1,024 x 65,537 take 520 instead of 396 us). Slices go
+// to slabs of [128][BN] f32, slice z of the i-th of these tiles to slab z rem + i, and whoever reads the result adds
+// them in order (slice_sum8). The extents may be known on the device only, so the shape is worked out there.
+struct SliceShape {
+  int num_n, num_m, kb, rem, q;
+  long full;  // tiles of the whole waves
+};
+__host__ __device__ inline SliceShape slice_shape(int M, int N, int K, int bn, int grid) {
+  SliceShape s;
+  s.num_n = (N + bn - 1) / bn;
+  s.num_m = (M + 127) / 128;
+  s.kb = (K + 63) / 64;
+  const long tiles = (long)s.num_n * s.num_m;
+  s.full = tiles / grid * grid;
+  s.rem = (int)(tiles - s.full);
+  s.q = s.rem ? grid / s.rem : 1;
+  if (s.q > s.kb / 4) s.q = s.kb / 4;  // a slice costs a slab's write and read: at least four k-blocks each
+  if (s.q < 1) s.q = 1;
+  return s;
+}
 
 struct EpiArgs {
   void* out;
@@ -68,12 +93,16 @@ struct EpiArgs {
   // fold_scale[batch] for the next product. Every warp computes the same s.
   float* fold_scale;
   double fold_eps;
-  // EPI_VOCAB: u = acc * scale2 + bias2[col] (bias2 optional, f32, padded to whole tiles), and the segment
-  // statistics [rows][ld_stat] (max, sum) of every row
+  // EPI_VOCAB: u = acc * scale2 + vbias[col] * scale2 (vbias optional), the segment statistics [rows][ld_stat]
+  // (max, sum) of every row, and optionally ut[row] = u at column target[row_ids ? row_ids[row] : row]
   float scale2;
-  const float* bias2;
+  const __nv_bfloat16* vbias;
   float2* stat;
   long ld_stat;
+  const int* target;
+  const int* row_ids;
+  float* ut;
+  float* slabs;  // EPI_SLICE: [gridDim.x][128][BN]
   // EPI_F32, optional: out += alpha*acc instead of out = alpha*acc
   int accum;
   // Rows that exist (optional): the extent M (dyn_k = 0) or K (dyn_k = 1) of this call is
@@ -299,13 +328,13 @@ struct GemmSmem {
   static constexpr uint32_t A_BYTES = BM * BK * 2;
   static constexpr uint32_t B_BYTES = BN * BK * 2;
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int NOUT = EPI == EPI_FWD ? 2 : ((EPI == EPI_DGRAD || EPI == EPI_BF16 || EPI == EPI_VOCAB) ? 1 : 0);
-  static constexpr int STG_BUFS = (EPI == EPI_BF16 || EPI == EPI_VOCAB || AT) ? 2 : 1;
+  static constexpr int NOUT = EPI == EPI_FWD ? 2 : ((EPI == EPI_DGRAD || EPI == EPI_BF16) ? 1 : 0);
+  static constexpr int STG_BUFS = (EPI == EPI_BF16 || AT) ? 2 : 1;
   static constexpr uint32_t STG_ONE = NOUT * 32 * 32 * 2;
   static constexpr uint32_t STG_WARP = STG_BUFS * STG_ONE;
   static constexpr uint32_t STG_BYTES = 8 * STG_WARP;
   static constexpr uint32_t RED_BYTES =
-      (EPI == EPI_DGRAD || EPI == EPI_PPO) ? (4 * BN * 4 + 4 * 8 * 4 + (EPI == EPI_PPO ? 128 * 8 * 4 : 0)) : 0;
+      EPI == EPI_VOCAB ? 8 * (BN / 2) * 4 : (EPI == EPI_DGRAD || EPI == EPI_PPO) ? (4 * BN * 4 + 4 * 8 * 4 + (EPI == EPI_PPO ? 128 * 8 * 4 : 0)) : 0;
   static constexpr uint32_t AUX_TILE = AT ? 128u * BN * 2u : 0u;
   static constexpr uint32_t AUX_BYTES = 2 * AUX_TILE;
   static constexpr uint32_t FIXED = 1024 + 256 + STG_BYTES + RED_BYTES + AUX_BYTES;
@@ -348,6 +377,54 @@ __device__ __forceinline__ TileIdx tile_at(int t, int num_n, int num_m) {
     return tile_of(t, num_n, num_m);
   }
 }
+
+// The tiles (and their ranges of k-blocks) that a CTA works on, in order: every gridDim.x-th tile, whole or one
+// split-K slice of it; with EPI_SLICE the whole waves and then one slice of the rest.
+template <int EPI>
+struct TileWalk {
+  int num_n, num_m, kb, per_split, k_splits;
+  long t, total;
+  SliceShape s;
+  long slab;  // EPI_SLICE: where the part goes (-1: out)
+  __device__ __forceinline__ TileWalk(int num_n_, int num_m_, int total_, int kb_, int per_split_, int k_splits_,
+                                      const SliceShape& s_)
+      : num_n(num_n_), num_m(num_m_), kb(kb_), per_split(per_split_), k_splits(k_splits_), t(blockIdx.x), total(total_),
+        s(s_), slab(-1) {}
+  __device__ __forceinline__ bool next(TileIdx& ti, int& b0, int& b1) {
+    if constexpr (EPI == EPI_SLICE) {
+      b0 = 0;
+      b1 = kb;
+      if (t < s.full) {
+        ti = tile_of((int)t, num_n, num_m);
+      } else {
+        const int i = (int)(t - s.full);
+        if (i >= s.rem * s.q) return false;
+        const int z = i / s.rem;
+        ti = tile_of((int)s.full + i - z * s.rem, num_n, num_m);
+        if (s.q > 1) {
+          b0 = (int)((long)kb * z / s.q);
+          b1 = (int)((long)kb * (z + 1) / s.q);
+          slab = i;
+        }
+      }
+      t += gridDim.x;
+      return true;
+    } else {
+      if (t >= total) return false;
+      ti = tile_at<EPI>((int)t, num_n, num_m);
+      t += gridDim.x;
+      if (k_splits > 1) {
+        b0 = ti.z * per_split;
+        b1 = min(kb, b0 + per_split);
+        if (b1 < b0) b1 = b0;
+      } else {
+        b0 = 0;
+        b1 = kb;
+      }
+      return true;
+    }
+  }
+};
 
 // Epilogue of one 128 x BN accumulator tile held in TMEM columns [tcol, tcol + BN).
 // Runs on the 4 epilogue warps; warp `sub` owns TMEM lanes / tile rows [32 sub, 32 sub + 32).
@@ -402,45 +479,87 @@ __device__ __forceinline__ void aux_smem32(const uint8_t* aux_sm, int rl, int c3
   for (int i = 0; i < 4; i++) o[i] = *reinterpret_cast<const uint4*>(base + (((q0 + i) ^ (rl & 7)) << 4));
 }
 
+// A head's bias in log2 units; finite values stay finite (the type's lowest may stand for a mask).
+__device__ __forceinline__ float vocab_bias2(float b, float scale2) {
+  return isfinite(b) ? fminf(fmaxf(b * scale2, -1e38f), 1e38f) : b;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// EPI_VOCAB: this warp's 32 rows x BN/2 columns of a logit tile, one row per lane, its BN/2 accumulators in
-// registers. In log2 units u = acc * scale2 + bias2, m = max u, s = sum 2^(u - m): the pair goes to
-// stat[row][2 n_tile + half]. With tma_out the terms leave as f16 scaled by 2^15, so the largest is 2^15
-// exactly and 11 bits of mantissa hold down to 2^-29 of it; bf16 would cost a second rounding of 2^-8 when
-// the gradient is formed from them. Columns past the vocabulary count as -inf.
+// What EPI_VOCAB reads beside the accumulators, loaded before the wait for them: this lane's four columns of the
+// bias (bf16), and the target column of its row.
+struct VocabPre {
+  uint2 bias;
+  int target;
+};
 template <int BN>
-__device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, uint32_t t_row, int m_tile, int n_tile, int rows,
-                                               int sub, int half, int lane, uint8_t* stg, const CUtensorMap* tmC,
-                                               uint32_t& seq) {
+__device__ __forceinline__ VocabPre vocab_prefetch(const EpiArgs& ep, int m_tile, int n_tile, int rows, int sub, int half,
+                                                   int lane) {
+  VocabPre p;
+  p.bias = make_uint2(0u, 0u);
+  p.target = -1;
+  const int c = n_tile * BN + half * (BN / 2) + 4 * lane;
+  if (ep.vbias && 4 * lane < BN / 2) {
+    if (c + 4 <= ep.out_cols && (reinterpret_cast<uintptr_t>(ep.vbias) & 7) == 0) {
+      p.bias = __ldg(reinterpret_cast<const uint2*>(ep.vbias + c));
+    } else {
+      uint32_t h[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        h[j] = c + j < ep.out_cols ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(ep.vbias) + c + j) : 0u;
+      p.bias = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    }
+  }
+  const int row = m_tile * 128 + sub * 32 + lane;
+  if (ep.target && row < rows) p.target = __ldg(ep.target + (ep.row_ids ? __ldg(ep.row_ids + row) : row));
+  return p;
+}
+
+// EPI_VOCAB: this warp's 32 rows x BN/2 columns of a logit tile, one row per lane, its BN/2 accumulators in
+// registers. In log2 units u = acc * scale2 + bias * scale2, m = max u, s = sum 2^(u - m): the pair goes to
+// stat[row][2 n_tile + half], u of the row's target column to ut[row]. With `out` the terms leave as f16 scaled by
+// 2^15, so the largest is 2^15 exactly and 11 bits of mantissa hold down to 2^-29 of it; bf16 would cost a second
+// rounding of 2^-8 when the gradient is formed from them. A lane's terms are one row's, 32 bytes to a store: whole
+// sectors, without the shared memory that the products' operands need. Columns past the vocabulary count as -inf.
+template <int BN>
+__device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, const VocabPre& pre, uint32_t t_row, int m_tile,
+                                               int n_tile, int rows, int sub, int half, int lane, float* bias_sm) {
   constexpr int W = BN / 2, NQ = W / 16;
-  const int row0 = m_tile * 128 + sub * 32;
+  const int row0 = m_tile * 128 + sub * 32, row = row0 + lane;
   const int n0 = n_tile * BN + half * W;
   const int left = ep.out_cols - n0;
   if (row0 >= rows || left <= 0) {  // warp-uniform: nothing of this warp's part exists
-    if (row0 < rows && row0 + lane < rows)
-      ep.stat[(long)(row0 + lane) * ep.ld_stat + 2 * n_tile + half] = make_float2(-INFINITY, 0.f);
+    if (row < rows) ep.stat[(long)row * ep.ld_stat + 2 * n_tile + half] = make_float2(-INFINITY, 0.f);
     return;
   }
   uint32_t r[NQ][16];
 #pragma unroll
   for (int q = 0; q < NQ; q++) tc::tmem_ld16(t_row + half * W + 16 * q, r[q]);
+  float scale = ep.scale2;
+  if (ep.vbias) {  // to shared memory once per warp, finite values kept finite (the lowest value may stand for a mask)
+    __syncwarp();
+    if (4 * lane < W) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&pre.bias);
+      float b[4] = {__low2float(h[0]), __high2float(h[0]), __low2float(h[1]), __high2float(h[1])};
+#pragma unroll
+      for (int j = 0; j < 4; j++) b[j] = vocab_bias2(b[j], scale);
+      reinterpret_cast<float4*>(bias_sm)[lane] = make_float4(b[0], b[1], b[2], b[3]);
+    }
+    __syncwarp();
+  }
   tc::tmem_wait_ld();
 #pragma unroll
   for (int q = 0; q < NQ; q++) tc::tmem_tie16(r[q]);
   float v[W];
 #pragma unroll
   for (int j = 0; j < W; j++) v[j] = __uint_as_float(r[j >> 4][j & 15]);
-  float scale = ep.scale2;
-  if (ep.bias2) {
-    const float4* b4 = reinterpret_cast<const float4*>(ep.bias2 + n0);
+  if (ep.vbias) {
 #pragma unroll
     for (int j = 0; j < W / 4; j++) {
-      const float4 b = __ldg(b4 + j);
+      const float4 b = reinterpret_cast<const float4*>(bias_sm)[j];
       v[4 * j] = __fmaf_rn(v[4 * j], scale, b.x);
       v[4 * j + 1] = __fmaf_rn(v[4 * j + 1], scale, b.y);
       v[4 * j + 2] = __fmaf_rn(v[4 * j + 2], scale, b.z);
@@ -452,6 +571,14 @@ __device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, uint32_t t_row
 #pragma unroll
     for (int j = 0; j < W; j++) v[j] = j < left ? v[j] : -INFINITY;
   }
+  const int rel = pre.target - n0;
+  const bool here = pre.target >= 0 && rel >= 0 && rel < min(left, W);
+  if (__any_sync(0xffffffffu, here)) {
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; j++) t = j == rel ? v[j] : t;
+    if (here) ep.ut[row] = t * scale;
+  }
   float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
   for (int j = 4; j < W; j += 4) {
@@ -462,41 +589,77 @@ __device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, uint32_t t_row
   const float ref = top == -INFINITY ? 0.f : top;  // a row with nothing but -inf here: every term 0
   const float shift = 15.f - ref;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool ok = row < rows;
+  uint16_t* out = reinterpret_cast<uint16_t*>(ep.out) + (long)row * ep.ldo + n0;
 #pragma unroll
-  for (int j = 0; j < W; j++) {
-    v[j] = ex2(__fmaf_rn(v[j], scale, shift));
-    sum[j & 3] += v[j];
+  for (int c = 0; c < W; c += 16) {
+    uint32_t u[8];
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float a = ex2(__fmaf_rn(v[c + j], scale, shift)), b = ex2(__fmaf_rn(v[c + j + 1], scale, shift));
+      sum[j & 3] += a;
+      sum[(j & 3) + 1] += b;
+      const __half2 h = __floats2half2_rn(a, b);
+      u[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    if (ep.out && ok && c < left)  // a row's stride is a multiple of 64: the 16 columns that hold `left` exist
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c), "r"(u[0]), "r"(u[1]),
+                   "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                   : "memory");
   }
-  const float total = ((sum[0] + sum[1]) + (sum[2] + sum[3])) * (1.f / 32768.f);
-  if (row0 + lane < rows)
-    ep.stat[(long)(row0 + lane) * ep.ld_stat + 2 * n_tile + half] = make_float2(top, total);
-  if (!ep.tma_out) return;
-  const int nch = min(W / 32, (left + 31) >> 5);
+  if (ok)
+    ep.stat[(long)row * ep.ld_stat + 2 * n_tile + half] =
+        make_float2(top, ((sum[0] + sum[1]) + (sum[2] + sum[3])) * (1.f / 32768.f));
+}
+
+// EPI_SLICE: this warp's 32 rows x BN/2 columns to out, or to the slab of a slice; a lane writes its row in 32-byte
+// pieces (out's rows are padded to a multiple of 8 columns).
+template <int BN>
+__device__ __forceinline__ void epilogue_slice(const EpiArgs& ep, uint32_t t_row, int m_tile, int n_tile, int rows,
+                                               long slab, bool have_acc, int sub, int half, int lane) {
+  const int row = m_tile * 128 + sub * 32 + lane, n0 = n_tile * BN;
+  float* at = slab < 0 ? reinterpret_cast<float*>(ep.out) + (long)row * ep.ldo + n0
+                       : ep.slabs + (slab * 128 + sub * 32 + lane) * BN;
 #pragma unroll
-  for (int ch = 0; ch < W / 32; ch++) {
-    if (ch >= nch) break;  // warp-uniform
-    uint8_t* st = stg + (seq & 1u) * GemmSmem<BN, EPI_VOCAB>::STG_ONE;
-    seq++;
-    if (lane == 0) tc::bulk_wait_read<1>();  // the store that last read this tile is done with it
-    __syncwarp();
-    uint8_t* row = st + lane * 64;
-    const int x = (lane >> 1) & 3;
+  for (int c = 0; c < BN / 2; c += 32) {
+    const int c0 = half * (BN / 2) + c;
+    if (n0 + c0 >= ep.out_cols) break;  // warp-uniform
+    uint32_t r[2][16];
+    tc::tmem_ld16(t_row + c0, r[0]);
+    tc::tmem_ld16(t_row + c0 + 16, r[1]);
+    tc::tmem_wait_ld_tie(r[0], r[1]);
+    if (!have_acc) {  // no k-blocks at all: the accumulator was never written
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      uint32_t u[4];
+      for (int j = 0; j < 16; j++) r[0][j] = r[1][j] = 0u;
+    }
+    if (row < rows) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const __half2 h = __floats2half2_rn(v[32 * ch + 8 * c + 2 * k], v[32 * ch + 8 * c + 2 * k + 1]);
-        u[k] = *reinterpret_cast<const uint32_t*>(&h);
+      for (int q = 0; q < 4; q++) {
+        const uint32_t* u = &r[q >> 1][(q & 1) * 8];
+        if (n0 + c0 + 8 * q < ep.out_cols)
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at + c0 + 8 * q), "r"(u[0]),
+                       "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                       : "memory");
       }
-      *reinterpret_cast<uint4*>(row + ((c ^ x) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
     }
-    tc::fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      tc::tma_store_3d(tmC, st, n0 + 32 * ch, row0, 0);
-      tc::bulk_commit();
-    }
+  }
+}
+
+// Eight values of row `row` at columns [col, col + 8) of a product that EPI_SLICE left in out and slabs (bn: its
+// column tile).
+__device__ __forceinline__ void slice_sum8(const SliceShape& s, const float* out, long ldo, const float* slabs, int bn,
+                                           long row, int col, float (&v)[8]) {
+  const int nt = col / bn;
+  const long t = (row >> 7) * s.num_n + nt;
+  const bool whole = t < s.full || s.q == 1;
+  const float* p = whole ? out + row * ldo + col : slabs + ((t - s.full) * 128 + (row & 127)) * bn + (col - nt * bn);
+  const int parts = whole ? 1 : s.q;
+#pragma unroll
+  for (int j = 0; j < 8; j++) v[j] = 0.f;
+#pragma unroll 4
+  for (int z = 0; z < parts; z++, p += (long)s.rem * 128 * bn) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
   }
 }
 
@@ -1065,27 +1228,19 @@ __global__ void __launch_bounds__(320, 1)
   tc::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  auto kb_range = [&](int z, int& b0, int& b1) {
-    if (ep.k_splits > 1) {
-      b0 = z * per_split;
-      b1 = min(total_kb, b0 + per_split);
-      if (b1 < b0) b1 = b0;
-    } else {
-      b0 = 0;
-      b1 = total_kb;
-    }
-  };
+  SliceShape shape{};
+  if constexpr (EPI == EPI_SLICE) shape = slice_shape(M, N, K, BN, gridDim.x);
+  TileWalk<EPI> walk(num_n, num_m, total_tiles, total_kb, per_split, ep.k_splits, shape);
+  TileIdx ti;
+  int b0, b1;
 
   if (warp == 0) {
     if (lane == 0) {
       // ---------------- TMA producer: one ring across all tiles of this CTA
       long it = 0;
       long ja = 0;  // aux tiles issued (AT)
-      for (int t = blockIdx.x; t < total_tiles && !*abort_flag; t += gridDim.x) {
-        const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
+      while (!*abort_flag && walk.next(ti, b0, b1)) {
         const int batch = ep.k_splits > 1 ? 0 : ti.z;
-        int b0, b1;
-        kb_range(ti.z, b0, b1);
         if (AT) {  // this tile's aux, into the buffer the epilogue released two tiles ago
           const int ab = (int)(ja & 1);
           if (ja >= 2 &&
@@ -1138,10 +1293,7 @@ __global__ void __launch_bounds__(320, 1)
       // ---------------- MMA issuer (one thread)
       long it = 0;
       int j = 0;
-      for (int t = blockIdx.x; t < total_tiles && !*abort_flag; t += gridDim.x, j++) {
-        const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
-        int b0, b1;
-        kb_range(ti.z, b0, b1);
+      for (; !*abort_flag && walk.next(ti, b0, b1); j++) {
         const int buf = j & 1;
         if (j >= 2 &&
             !tc::mbar_wait(&acc_empty[buf], (uint32_t)(((j >> 1) - 1) & 1), ep.err, PL_ERR_MBAR_TIMEOUT | 3)) {
@@ -1183,11 +1335,10 @@ __global__ void __launch_bounds__(320, 1)
     const int half = (warp - 2) >> 2;
     uint32_t stg_seq = 0;  // chunks this warp has staged: picks the staging tile
     int j = 0;
-    for (int t = blockIdx.x; t < total_tiles; t += gridDim.x, j++) {
-      const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
-      int b0, b1;
-      kb_range(ti.z, b0, b1);
+    for (; walk.next(ti, b0, b1); j++) {
       const int buf = j & 1;
+      VocabPre pre;
+      if constexpr (EPI == EPI_VOCAB) pre = vocab_prefetch<BN>(ep, ti.m, ti.n, M, sub, half, lane);
       const bool ok = tc::mbar_wait(&acc_full[buf], (uint32_t)((j >> 1) & 1), ep.err, PL_ERR_MBAR_TIMEOUT | 6) &&
                       (!AT || tc::mbar_wait(&aux_full[buf], (uint32_t)((j >> 1) & 1), ep.err,
                                             PL_ERR_MBAR_TIMEOUT | 12));
@@ -1197,9 +1348,10 @@ __global__ void __launch_bounds__(320, 1)
       }
       tc::tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t)(buf * BN) + ((uint32_t)(sub * 32) << 16);
-      if constexpr (EPI == EPI_VOCAB)
-        epilogue_vocab<BN>(ep, t_row, ti.m, ti.n, M, sub, half, lane, stg_base + (warp - 2) * S::STG_WARP, &tmC,
-                           stg_seq);
+      if constexpr (EPI == EPI_SLICE)
+        epilogue_slice<BN>(ep, t_row, ti.m, ti.n, M, walk.slab, b1 > b0, sub, half, lane);
+      else if constexpr (EPI == EPI_VOCAB)
+        epilogue_vocab<BN>(ep, pre, t_row, ti.m, ti.n, M, sub, half, lane, red + (warp - 2) * (BN / 2));
       else
         epilogue_tile<BN, EPI, S::STG_BUFS>(ep, t_row, ti.m, ti.n, ti.z, ep.k_splits > 1 ? 0 : ti.z, b1 > b0, sub,
                                             half, lane, red, rowscr, stg_base + (warp - 2) * S::STG_WARP, &tmC, &tmC2,
@@ -1479,5 +1631,7 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
 // operands are MN-major (the weight gradients; the default); a negative mode only queries. Returns the
 // previous mode.
 int gemm_set_pair_mode(int mode);
+// CTAs of an EPI_SLICE launch (the current device's SMs): the `grid` of its slice_shape.
+int gemm_sms();
 
 }  // namespace pl

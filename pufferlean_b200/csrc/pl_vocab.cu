@@ -23,19 +23,87 @@ namespace pl {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// The answers of a call: one target per row (ids [N], teacher NULL, K = 1) or K entries per row.
+// Which rows count: a target that is not negative (cross entropy), or `has` (distillation).
 struct Answers {
-  const int* ids;
-  const float* teacher;  // NULL: every present entry has probability 1
-  long K;
+  const int* target;
+  const uint8_t* has;
 };
-
 __device__ __forceinline__ bool row_counts(const Answers& a, long row) {
-  for (long k = 0; k < a.K; k++) {
-    if (a.ids[row * a.K + k] < 0) continue;
-    if (!a.teacher || a.teacher[row * a.K + k] > -INFINITY || isnan(a.teacher[row * a.K + k])) return true;
+  return a.target ? __ldg(a.target + row) >= 0 : (a.has ? __ldg(a.has + row) != 0 : true);
+}
+__device__ __forceinline__ long rows_here(const int* count, long off, long n) {
+  return count ? min(n, max(0L, (long)*count - off)) : n;
+}
+__device__ __forceinline__ float warp_sum_f(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max_f(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// The teacher's side of every row, one warp each: p = softmax(teacher / T) over the present entries (f32), entries
+// that name one id added up in the first of them (the others become absent), and ent = sum_k p_k log2 p_k of the
+// single entries. ids2, p [N][K]; a row without entries gets has = 0.
+__global__ void __launch_bounds__(128)
+    vocab_teacher_kernel(const int* __restrict__ ids, const float* __restrict__ teacher, long N, int K, float tscale,
+                         int* __restrict__ ids2, float* __restrict__ p, float* __restrict__ ent,
+                         uint8_t* __restrict__ has) {
+  extern __shared__ uint8_t dyn_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long r = (long)blockIdx.x * 4 + warp;
+  if (r >= N) return;
+  int* id_s = reinterpret_cast<int*>(dyn_smem) + warp * 2 * K;
+  float* p_s = reinterpret_cast<float*>(id_s + K);
+  float top = -INFINITY;
+  bool any = false;
+  for (int k = lane; k < K; k += 32) {
+    int id = ids[r * K + k];
+    const float t = teacher[r * K + k];
+    if (t == -INFINITY) id = -1;
+    id_s[k] = id;
+    p_s[k] = t;
+    if (id >= 0) {
+      top = fmaxf(top, t);
+      any = true;
+    }
   }
-  return false;
+  any = __any_sync(0xffffffffu, any);
+  top = warp_max_f(top);
+  float tot = 0.f;
+  for (int k = lane; k < K; k += 32)
+    if (id_s[k] >= 0) tot += exp2f((p_s[k] - top) * tscale);
+  tot = warp_sum_f(tot);
+  const float log_tot = log2f(tot);
+  float e = 0.f;
+  for (int k = lane; k < K; k += 32) {
+    float q = 0.f;
+    if (id_s[k] >= 0) {
+      const float l = (p_s[k] - top) * tscale - log_tot;
+      q = exp2f(l);
+      if (!(q == 0.f)) e = __fmaf_rn(q, l, e);
+    }
+    p_s[k] = q;
+  }
+  e = warp_sum_f(e);
+  __syncwarp();
+  for (int k = lane; k < K; k += 32) {
+    const int id = id_s[k];
+    float q = p_s[k];
+    bool first = id >= 0;
+    for (int g = 0; first && g < k; g++) first = id_s[g] != id;
+    if (first)
+      for (int g = k + 1; g < K; g++) q += id_s[g] == id ? p_s[g] : 0.f;
+    ids2[r * K + k] = first ? id : -1;
+    p[r * K + k] = first ? q : 0.f;
+  }
+  if (lane == 0) {
+    ent[r] = e;
+    has[r] = any;
+  }
 }
 
 // rows[0 .. *count) = the rows that count, in order; loss = lse = 0 for the others. One block.
@@ -51,18 +119,20 @@ __global__ void __launch_bounds__(1024)
     const unsigned mask = __ballot_sync(0xffffffffu, in);
     if (lane == 0) warp_n[warp] = __popc(mask);
     __syncthreads();
-    int before = base, all = base;
-    for (int w = 0; w < 32; w++) {
-      if (w < warp) before += warp_n[w];
-      all += warp_n[w];
+    int n = warp_n[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += t;
     }
+    const int before = base + (warp ? __shfl_sync(0xffffffffu, n, warp - 1) : 0);
     if (in) {
       rows[before + __popc(mask & ((1u << lane) - 1u))] = (int)r;
     } else if (r < N) {
       loss[r] = 0.f;
       lse[r] = 0.f;
     }
-    base = all;
+    base += __shfl_sync(0xffffffffu, n, 31);
     __syncthreads();
   }
   if (threadIdx.x == 0) *count = base;
@@ -75,235 +145,310 @@ __global__ void __launch_bounds__(256)
                       const int* __restrict__ count, long off, long n, __nv_bfloat16* __restrict__ dst, long ldd) {
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  const long have = count ? min(n, max(0L, (long)*count - off)) : n;
+  const long have = rows_here(count, off, n);
   if (i >= (have + 63) / 64 * 64) return;
   bool in = i < have;
   long r = i;
   if (in) {
     if (rows)
       r = rows[off + i];
-    else if (a.ids)
+    else
       in = row_counts(a, r);
   }
   __nv_bfloat16* d = dst + i * ldd;
   const __nv_bfloat16* s = src + r * ld;
   if (((uintptr_t)src & 15) == 0 && ld % 8 == 0 && D % 8 == 0) {
+#pragma unroll 4
     for (long c = lane * 8; c < D; c += 256)
       *reinterpret_cast<uint4*>(d + c) = in ? *reinterpret_cast<const uint4*>(s + c) : make_uint4(0, 0, 0, 0);
   } else {
+#pragma unroll 4
     for (long c = lane; c < D; c += 32) d[c] = in ? s[c] : __float2bfloat16_rn(0.f);
   }
 }
 
-// bias2 = bias / T in log2 units, finite values kept finite (the type's lowest value may stand for a mask).
+// The row's lse in log2 units from its segments' (max, sum); a fixed order over the threads t of `threads`.
+__device__ __forceinline__ float2 seg_fold(const float2* __restrict__ sr, long segs, int t, int threads) {
+  float m = -INFINITY, s = 0.f;
+  for (long q = t; q < segs; q += threads) {
+    const float2 f = sr[q];
+    const float hi = fmaxf(m, f.x);
+    const float ref = hi == -INFINITY ? 0.f : hi;  // empty segments add their 0 (or NaN)
+    s = s * exp2f(m - ref) + f.y * (f.x == -INFINITY ? 1.f : exp2f(f.x - ref));
+    m = hi;
+  }
+  return make_float2(m, s);
+}
+__device__ __forceinline__ float2 seg_join(float2 a, float2 b) {
+  const float hi = fmaxf(a.x, b.x), ref = hi == -INFINITY ? 0.f : hi;
+  return make_float2(hi, a.y * (a.x == -INFINITY ? 1.f : exp2f(a.x - ref)) + b.y * (b.x == -INFINITY ? 1.f : exp2f(b.x - ref)));
+}
+__device__ __forceinline__ float2 warp_join(float2 v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    v = seg_join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+  return v;
+}
+__device__ __forceinline__ float seg_lse(float2 v) { return (v.x == -INFINITY ? 0.f : v.x) + log2f(v.y); }
+
+// What the gradient needs of a row of the piece: info[i] = (lse in log2 units, scale / T; 0 where it does not
+// count), and per answer entry the column (-1: absent) and the gradient there, in f32.
+struct RowOut {
+  float2* info;
+  int* col;
+  float* val;
+};
+
+// Cross entropy, one warp per row: the target's logit comes from the product itself (ut), so that loss = lse - u
+// carries no difference between two ways of summing.
 __global__ void __launch_bounds__(256)
-    vocab_bias_kernel(const __nv_bfloat16* __restrict__ bias, long V, long Vp, float scale2, float* __restrict__ out) {
-  const long v = (long)blockIdx.x * 256 + threadIdx.x;
-  if (v >= Vp) return;
-  float b = v < V ? __bfloat162float(bias[v]) : 0.f;
-  if (isfinite(b)) b = fminf(fmaxf(b * scale2, -1e38f), 1e38f);
-  out[v] = b;
-}
-
-__device__ __forceinline__ float block_max(float v, float* scr) {  // 128 threads
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if ((threadIdx.x & 31) == 0) scr[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = fmaxf(fmaxf(scr[0], scr[1]), fmaxf(scr[2], scr[3]));
-  __syncthreads();
-  return v;
-}
-__device__ __forceinline__ float block_sum(float v, float* scr) {  // 128 threads, a fixed order
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) scr[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = (scr[0] + scr[1]) + (scr[2] + scr[3]);
-  __syncthreads();
-  return v;
-}
-
-// One block per row of the piece: the answer's logits (K products of length D with gathered rows of W: exact to
-// f32, which the terms in f16 are not), the row's lse from its segments, the loss, and what the gradient needs:
-// info[i] = (lse in log2 units, scale / T), uk[i][k] = u of entry k in log2 units, pk[i][k] its probability.
-__global__ void __launch_bounds__(128)
-    vocab_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx, const __nv_bfloat16* __restrict__ w, long ldw,
-                      const float* __restrict__ bias2, long V, long D, Answers a, float scale2, float inv_t,
-                      const float* __restrict__ row_scale, const int* __restrict__ rows, const int* __restrict__ count,
-                      long off, const float2* __restrict__ stat, long ld_stat, float* __restrict__ loss,
-                      float* __restrict__ lse, float2* __restrict__ info, float* __restrict__ uk,
-                      float* __restrict__ pk) {
-  __shared__ float scr[4];
-  const long i = blockIdx.x;
-  if (count && off + i >= *count) return;
+    vocab_ce_rows_kernel(const int* __restrict__ target, long V, const float* __restrict__ row_scale,
+                         const int* __restrict__ rows, const int* __restrict__ count, long off, long n,
+                         const float2* __restrict__ stat, long ld_stat, const float* __restrict__ ut,
+                         float* __restrict__ loss, float* __restrict__ lse, RowOut o) {
+  const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (i >= rows_here(count, off, n)) return;
   const long r = rows ? rows[off + i] : off + i;
-  const long K = a.K;
-  const int* ids = a.ids + r * K;
-  if (!rows && !row_counts(a, r)) {
-    if (threadIdx.x == 0) {
-      loss[r] = 0.f;
-      lse[r] = 0.f;
-      if (info) info[i] = make_float2(0.f, 0.f);
+  const int t = target[r];
+  float lse2 = seg_lse(warp_join(seg_fold(stat + i * ld_stat, ld_stat, lane, 32)));
+  if (lane) return;
+  if (t < 0) {
+    loss[r] = 0.f;
+    lse[r] = 0.f;
+    if (o.info) {
+      o.info[i] = make_float2(0.f, 0.f);
+      o.col[i] = -1;
+      o.val[i] = 0.f;
     }
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // lse2 = max + log2 sum over the segments
-  const float2* sr = stat + i * ld_stat;
-  float mx = -INFINITY;
-  for (long q = threadIdx.x; q < ld_stat; q += 128) mx = fmaxf(mx, sr[q].x);
-  mx = block_max(mx, scr);
-  const float ref = mx == -INFINITY ? 0.f : mx;
-  float s = 0.f;
-  for (long q = threadIdx.x; q < ld_stat; q += 128) {
-    const float2 f = sr[q];
-    s += f.x == -INFINITY ? f.y : f.y * exp2f(f.x - ref);  // an empty segment's sum is 0 (or NaN)
-  }
-  s = block_sum(s, scr);
-  float lse2 = ref + log2f(s);
-  // the answer's distribution
-  float top = -INFINITY, tot = 1.f;
-  bool bad = false;
-  const float tscale = inv_t * kLog2e;
-  if (a.teacher) {
-    for (long k = threadIdx.x; k < K; k += 128)
-      if (ids[k] >= 0) top = fmaxf(top, a.teacher[r * K + k]);
-    top = block_max(top, scr);
-    tot = 0.f;
-    for (long k = threadIdx.x; k < K; k += 128)
-      if (ids[k] >= 0) tot += exp2f((a.teacher[r * K + k] - top) * tscale);
-    tot = block_sum(tot, scr);
-  }
-  const float log_tot = log2f(tot);
-  // sum_k p_k (log2 p_k - u_k), entry k on warp k mod 4
-  const __nv_bfloat16* xr = x + i * ldx;
-  const bool vec = ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && ldx % 8 == 0 && ldw % 8 == 0;
-  float acc = 0.f;
-  for (long k = warp; k < K; k += 4) {
-    const int id = ids[k];
-    float p = 0.f, u = 0.f, logp = 0.f;
-    if (id >= 0) {
-      p = 1.f;
-      if (a.teacher) {
-        logp = (a.teacher[r * K + k] - top) * tscale - log_tot;
-        p = exp2f(logp);
-      }
-      if (id >= V) {
-        bad = true;
-      } else {
-        const __nv_bfloat16* wr = w + (long)id * ldw;
-        float d = 0.f;
-        long c = 0;
-        if (vec) {
-          const long Dv = D / 8 * 8;
-#pragma unroll 4
-          for (c = lane * 8; c < Dv; c += 256) {
-            const uint4 xv = *reinterpret_cast<const uint4*>(xr + c), wv = __ldg(reinterpret_cast<const uint4*>(wr + c));
-            const __nv_bfloat162 *xh = reinterpret_cast<const __nv_bfloat162*>(&xv),
-                                 *wh = reinterpret_cast<const __nv_bfloat162*>(&wv);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const float2 f = __bfloat1622float2(xh[j]), g = __bfloat1622float2(wh[j]);
-              d = __fmaf_rn(f.x, g.x, d);
-              d = __fmaf_rn(f.y, g.y, d);
-            }
-          }
-          c = Dv;
-        }
-        for (c += lane; c < D; c += 32) d = __fmaf_rn(__bfloat162float(xr[c]), __bfloat162float(wr[c]), d);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        u = __fmaf_rn(d, scale2, bias2 ? bias2[id] : 0.f);
-        if (p > 0.f) acc = __fmaf_rn(p, logp - u, acc);
-        else if (isnan(p)) acc = p;
-      }
-    }
-    if (lane == 0 && info) {
-      uk[i * K + k] = u;
-      pk[i * K + k] = p;
-    }
-  }
-  acc = block_sum(lane == 0 ? acc : 0.f, scr);
-  if (block_sum(bad ? 1.f : 0.f, scr) > 0.f) acc = lse2 = NAN;  // an index past the vocabulary: seen in the loss
-  if (threadIdx.x == 0) {
-    loss[r] = (acc + lse2) * kLn2;
-    lse[r] = lse2 * kLn2;
-    if (info) info[i] = make_float2(lse2, (row_scale ? row_scale[r] : 1.f) * inv_t);
+  float u = 0.f;
+  if (t >= V)
+    lse2 = NAN;  // a target past the vocabulary: seen in the loss
+  else
+    u = ut[i];
+  loss[r] = (lse2 - u) * kLn2;
+  lse[r] = lse2 * kLn2;
+  if (o.info) {
+    const float scale = row_scale ? row_scale[r] : 1.f;
+    o.info[i] = make_float2(lse2, scale);
+    o.col[i] = t;
+    o.val[i] = (exp2f(u - lse2) - 1.f) * scale;
   }
 }
 
-// The f16 terms of a 64-row x 256-column tile become dz in place (bf16): t 2^(max - lse - 15) scale, and at the
-// answer's columns scale (2^(u - lse) - sum p) from the f32 logits. A warp walks the rows, a lane owns 8 columns;
-// which rows have an answer in the tile is found first, so that the others pay one flag. With `part` each lane's
-// column sums (of the unrounded values) go to part[row tile][V] for dbias. Rows from the count to the next
-// multiple of 64 are zeroed (the weight-gradient product reads whole k-blocks of rows).
-__global__ void __launch_bounds__(256)
-    vocab_dz_kernel(void* __restrict__ terms, long ld, long V, Answers a, const int* __restrict__ rows,
-                    const int* __restrict__ count, long off, long n, const float2* __restrict__ info,
-                    const float* __restrict__ uk, const float* __restrict__ pk, const float2* __restrict__ stat,
-                    long ld_stat, int seg, float* __restrict__ part) {
-  __shared__ int hit[64];
-  __shared__ float fold[8][256];
-  const long have = count ? min(n, max(0L, (long)*count - off)) : n;
-  const long r0 = (long)blockIdx.y * 64, c0 = (long)blockIdx.x * 256;
+// Distillation, one block per row: the logits of the entries are products of length D with gathered rows of W, four
+// entries at a time per warp.
+__global__ void __launch_bounds__(128)
+    vocab_distill_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx, const __nv_bfloat16* __restrict__ w,
+                              long ldw, const __nv_bfloat16* __restrict__ bias, long V, long D, int K,
+                              const int* __restrict__ ids2, const float* __restrict__ p, const float* __restrict__ ent,
+                              const uint8_t* __restrict__ has, float scale2, float inv_t,
+                              const float* __restrict__ row_scale, const int* __restrict__ rows,
+                              const int* __restrict__ count, long off, const float2* __restrict__ stat, long ld_stat,
+                              float* __restrict__ loss, float* __restrict__ lse, RowOut o) {
+  __shared__ float2 seg_s[4];
+  __shared__ float acc_s[4];
+  __shared__ int bad_s[4];
+  const long i = blockIdx.x;
+  if (count && off + i >= *count) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long c = c0 + lane * 8;
-  float sum[8];
+  const long r = rows ? rows[off + i] : off + i;
+  if (!rows && !has[r]) {
+    if (threadIdx.x == 0) {
+      loss[r] = 0.f;
+      lse[r] = 0.f;
+      if (o.info) o.info[i] = make_float2(0.f, 0.f);
+    }
+    if (o.info)
+      for (int k = threadIdx.x; k < K; k += 128) o.col[i * K + k] = -1;
+    return;
+  }
+  const float2 mine = warp_join(seg_fold(stat + i * ld_stat, ld_stat, threadIdx.x, 128));
+  if (lane == 0) seg_s[warp] = mine;
+  __syncthreads();
+  const float lse2 = seg_lse(seg_join(seg_join(seg_s[0], seg_s[1]), seg_join(seg_s[2], seg_s[3])));
+  const float scale = (row_scale ? row_scale[r] : 1.f) * inv_t;
+  const __nv_bfloat16* xr = x + i * ldx;
+  const bool vec = ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && ldx % 8 == 0 && ldw % 8 == 0;
+  const long Dv = vec ? D / 8 * 8 : 0;
+  float acc = 0.f;
+  bool bad = false;
+  for (int k0 = warp * 4; k0 < K; k0 += 16) {
+    const __nv_bfloat16* wr[4];
+    int id[4];
 #pragma unroll
-  for (int j = 0; j < 8; j++) sum[j] = 0.f;
-  if (r0 < have) {
-    const int nr = (int)min(64L, have - r0);
-    if (threadIdx.x < 64) hit[threadIdx.x] = 0;
+    for (int j = 0; j < 4; j++) {
+      id[j] = k0 + j < K ? ids2[r * K + k0 + j] : -1;
+      wr[j] = w + (id[j] >= 0 && id[j] < V ? (long)id[j] : 0L) * ldw;  // absent entries read row 0, to no effect
+    }
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (long c = lane * 8; c < Dv; c += 256) {
+      const uint4 xv = *reinterpret_cast<const uint4*>(xr + c);
+      uint4 wv[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) wv[j] = __ldg(reinterpret_cast<const uint4*>(wr[j] + c));
+      const __nv_bfloat162* xh = reinterpret_cast<const __nv_bfloat162*>(&xv);
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const float2 f = __bfloat1622float2(xh[q]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float2 g = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&wv[j])[q]);
+          d[j] = __fmaf_rn(f.x, g.x, d[j]);
+          d[j] = __fmaf_rn(f.y, g.y, d[j]);
+        }
+      }
+    }
+    for (long c = Dv + lane; c < D; c += 32) {
+      const float f = __bfloat162float(xr[c]);
+#pragma unroll
+      for (int j = 0; j < 4; j++) d[j] = __fmaf_rn(f, __bfloat162float(wr[j][c]), d[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) d[j] = warp_sum_f(d[j]);
+    // lane j finishes entry k0 + j
+    const float dot = lane == 0 ? d[0] : (lane == 1 ? d[1] : (lane == 2 ? d[2] : d[3]));
+    if (lane < 4 && k0 + lane < K) {
+      const int c = ids2[r * K + k0 + lane];
+      float val = 0.f;
+      if (c >= V) {
+        bad = true;
+      } else if (c >= 0) {
+        const float q = p[r * K + k0 + lane];
+        const float u = __fmaf_rn(dot, scale2, bias ? vocab_bias2(__bfloat162float(bias[c]), scale2) : 0.f);
+        if (!(q == 0.f)) acc = __fmaf_rn(-q, u, acc);
+        val = (exp2f(u - lse2) - q) * scale;
+      }
+      if (o.info) {
+        o.col[i * K + k0 + lane] = c;
+        o.val[i * K + k0 + lane] = val;
+      }
+    }
+  }
+  acc = warp_sum_f(acc);
+  bad = __any_sync(0xffffffffu, bad);
+  if (lane == 0) {
+    acc_s[warp] = acc;
+    bad_s[warp] = bad;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool any_bad = bad_s[0] | bad_s[1] | bad_s[2] | bad_s[3];  // an id past the vocabulary: seen in the loss
+    const float l2 = any_bad ? NAN : lse2;
+    loss[r] = (ent[r] + ((acc_s[0] + acc_s[1]) + (acc_s[2] + acc_s[3])) + l2) * kLn2;
+    lse[r] = l2 * kLn2;
+    if (o.info) o.info[i] = make_float2(l2, scale);
+  }
+}
+
+// The f16 terms of a tile of `rpb` rows x 256 NS columns become dz in place (bf16): t 2^(max - lse - 15) scale, and
+// at the answer's columns the f32 values of the rows kernels. A warp walks the rows, a lane owns 8 columns of every
+// 256. The block first lists the answer entries that fall into its tile (in an order that depends on nothing but the
+// entries) and marks them in a bit mask; the walk leaves marked columns out, and the listed values are written after
+// it. With `part` the column sums of the unrounded values go to part[row tile][V] for dbias. Rows from the count to
+// the next multiple of 64 are zeroed (the weight-gradient product reads whole k-blocks of rows).
+// Bound by HBM: 4 bytes per term.
+template <int NS>
+struct DzSmem {
+  static constexpr int COLS = 256 * NS;
+  static size_t bytes(int rpb, long K, bool part) {
+    return (size_t)rpb * COLS / 8 + (size_t)rpb * K * 8 + (part ? (size_t)8 * COLS * 4 : 0);
+  }
+};
+template <int NS>
+__global__ void __launch_bounds__(256)
+    vocab_dz_kernel(void* __restrict__ terms, long ld, long V, int K, const int* __restrict__ count, long off, long n,
+                    int rpb, RowOut in, const float2* __restrict__ stat, long ld_stat, int seg_shift,
+                    float* __restrict__ part) {
+  constexpr int COLS = 256 * NS;
+  extern __shared__ __align__(16) uint8_t dyn_smem[];
+  uint32_t* mask = reinterpret_cast<uint32_t*>(dyn_smem);                   // [rpb][COLS / 32]
+  uint32_t* hit_at = mask + rpb * (COLS / 32);                              // [rpb K]: row << 16 | column
+  float* hit_v = reinterpret_cast<float*>(hit_at + (long)rpb * K);          // [rpb K]
+  float* fold = hit_v + (long)rpb * K;                                      // [8][COLS] (part)
+  __shared__ int warp_n[8];
+  const long have = rows_here(count, off, n);
+  const long r0 = (long)blockIdx.y * rpb, c0 = (long)blockIdx.x * COLS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint16_t* base = reinterpret_cast<uint16_t*>(terms);
+  float sum[NS][8];
+#pragma unroll
+  for (int s = 0; s < NS; s++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) sum[s][j] = 0.f;
+  int hits = 0;
+  const int nr = (int)max(0L, min((long)rpb, have - r0));
+  if (nr > 0) {
+    for (int q = threadIdx.x; q < rpb * (COLS / 32); q += 256) mask[q] = 0u;
+    const int total = nr * K;
+    int mine = 0;
+    for (int q = threadIdx.x; q < total; q += 256) {
+      const long d = in.col[r0 * K + q] - c0;
+      mine += d >= 0 && d < COLS && d + c0 < V;
+    }
+    // exclusive prefix over the threads
+    int pre = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, pre, o);
+      if (lane >= o) pre += t;
+    }
+    if (lane == 31) warp_n[warp] = pre;
     __syncthreads();
-    for (long q = threadIdx.x; q < nr * a.K; q += 256) {
-      const long i = r0 + q / a.K, k = q - q / a.K * a.K;
-      const int id = a.ids[(rows ? (long)rows[off + i] : off + i) * a.K + k];
-      if (id >= c0 && id < c0 + 256) hit[i - r0] = 1;
+    int at = pre - mine;
+#pragma unroll
+    for (int q = 0; q < 8; q++) {
+      if (q < warp) at += warp_n[q];
+      hits += warp_n[q];
+    }
+    if (mine) {
+      for (int q = threadIdx.x; q < total; q += 256) {
+        const long d = in.col[r0 * K + q] - c0;
+        if (d >= 0 && d < COLS && d + c0 < V) {
+          const int row = q / K;
+          hit_at[at] = (uint32_t)row << 16 | (uint32_t)d;
+          hit_v[at] = in.val[r0 * K + q];
+          atomicOr(&mask[row * (COLS / 32) + (int)(d >> 5)], 1u << (d & 31));
+          at++;
+        }
+      }
     }
     __syncthreads();
-    if (c < V) {  // V's pad up to a multiple of 8 lies inside ld
-#pragma unroll 4
-      for (int q = warp; q < 64; q += 8) {
-        const long i = r0 + q;
-        uint4* at = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(terms) + i * ld + c);
+#pragma unroll 2
+    for (int q = warp; q < nr; q += 8) {
+      const long i = r0 + q;
+      const float2 f = in.info[i];  // (lse2, scale)
+      uint4 raw[NS];
+      float m[NS];
+#pragma unroll
+      for (int s = 0; s < NS; s++) {
+        const long c = c0 + 256 * s + lane * 8;
+        if (c < V) {  // V's pad up to a multiple of 8 lies inside ld
+          raw[s] = *reinterpret_cast<const uint4*>(base + i * ld + c);
+          m[s] = stat[i * ld_stat + (c >> seg_shift)].x;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < NS; s++) {
+        const long c = c0 + 256 * s + lane * 8;
+        if (c >= V) continue;
+        const uint32_t bits = mask[q * (COLS / 32) + 8 * s + (lane >> 2)] >> (8 * (lane & 3)) & 0xffu;
+        const float k = m[s] == -INFINITY ? 0.f : exp2f(m[s] - f.x - 15.f) * f.y;
+        const __half2* h = reinterpret_cast<const __half2*>(&raw[s]);
         float v[8];
-        if (q < nr) {
-          const float2 f = info[i];  // (lse2, scale)
-          const uint4 raw = *at;
-          const __half2* h = reinterpret_cast<const __half2*>(&raw);
-          if (f.y == 0.f) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = 0.f;
-          } else {
-            const float m = stat[i * ld_stat + c / seg].x;
-            const float k = m == -INFINITY ? 0.f : exp2f(m - f.x - 15.f) * f.y;
+        for (int j = 0; j < 4; j++) {
+          const float2 t = __half22float2(h[j]);
+          v[2 * j] = t.x * k;
+          v[2 * j + 1] = t.y * k;
+        }
+        if (f.y == 0.f || bits) {  // a row that does not count; columns whose values are listed
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const float2 t = __half22float2(h[j]);
-              v[2 * j] = t.x * k;
-              v[2 * j + 1] = t.y * k;
-            }
-            if (hit[q]) {
-              const int* ids = a.ids + (rows ? (long)rows[off + i] : off + i) * a.K;
-              for (long e = 0; e < a.K; e++) {
-                const long d = (long)ids[e] - c;
-                if (d < 0 || d >= 8) continue;
-                float p = 0.f;  // entries that name the same column add up
-                for (long g = 0; g < a.K; g++)
-                  if (ids[g] == ids[e]) p += pk[i * a.K + g];
-                const float val = (exp2f(uk[i * a.K + e] - f.x) - p) * f.y;
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = j == (int)d ? val : v[j];
-              }
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 8; j++) sum[j] += v[j];
-        } else {
-          if (i >= (have + 63) / 64 * 64) continue;
-#pragma unroll
-          for (int j = 0; j < 8; j++) v[j] = 0.f;
+          for (int j = 0; j < 8; j++)
+            if (f.y == 0.f || (bits >> j & 1u)) v[j] = 0.f;
         }
         uint4 o;
         uint32_t* u = reinterpret_cast<uint32_t*>(&o);
@@ -312,20 +457,38 @@ __global__ void __launch_bounds__(256)
           const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
           u[j] = *reinterpret_cast<const uint32_t*>(&b);
         }
-        *at = o;
+        *reinterpret_cast<uint4*>(base + i * ld + c) = o;
+#pragma unroll
+        for (int j = 0; j < 8; j++) sum[s][j] += v[j];
       }
     }
   }
-  if (!part) return;
+  for (long i = r0 + nr + warp; i < min(r0 + rpb, (have + 63) / 64 * 64); i += 8)
 #pragma unroll
-  for (int j = 0; j < 8; j++) fold[warp][lane * 8 + j] = sum[j];
+    for (int s = 0; s < NS; s++) {
+      const long c = c0 + 256 * s + lane * 8;
+      if (c < V) *reinterpret_cast<uint4*>(base + i * ld + c) = make_uint4(0u, 0u, 0u, 0u);
+    }
+  if (part) {
+#pragma unroll
+    for (int s = 0; s < NS; s++)
+#pragma unroll
+      for (int j = 0; j < 8; j += 4)
+        *reinterpret_cast<float4*>(fold + warp * COLS + 256 * s + lane * 8 + j) =
+            make_float4(sum[s][j], sum[s][j + 1], sum[s][j + 2], sum[s][j + 3]);
+  }
   __syncthreads();
-  const long cc = c0 + threadIdx.x;
-  if (cc < V) {
-    float t = fold[0][threadIdx.x];
+  for (int h = threadIdx.x; h < hits; h += 256)
+    base[(r0 + (hit_at[h] >> 16)) * ld + c0 + (hit_at[h] & 0xffffu)] =
+        __bfloat16_as_ushort(__float2bfloat16_rn(hit_v[h]));
+  if (!part) return;
+  for (int c = threadIdx.x; c < COLS && c0 + c < V; c += 256) {
+    float t = fold[c];
 #pragma unroll
-    for (int q = 1; q < 8; q++) t += fold[q][threadIdx.x];
-    part[(long)blockIdx.y * V + cc] = t;
+    for (int q = 1; q < 8; q++) t += fold[q * COLS + c];
+    for (int h = 0; h < hits; h++)
+      if ((hit_at[h] & 0xffffu) == (uint32_t)c) t += hit_v[h];
+    part[(long)blockIdx.y * V + c0 + c] = t;
   }
 }
 
@@ -336,7 +499,7 @@ __global__ void __launch_bounds__(256)
   const long v = (long)blockIdx.x * 256 + threadIdx.x;
   if (v >= V) return;
   float s = first ? 0.f : acc[v];
-#pragma unroll 4
+#pragma unroll 8
   for (int q = 0; q < tiles; q++) s += part[(long)q * V + v];
   if (!last)
     acc[v] = s;
@@ -346,72 +509,105 @@ __global__ void __launch_bounds__(256)
     reinterpret_cast<__nv_bfloat16*>(dbias)[v] = __float2bfloat16_rn(s);
 }
 
-// dx row rows[off + i] = row i of `src`, i < the rows that count: summed over `splits` f32 slices or copied from
-// bf16. One warp per row.
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  uint4 o;
+  uint32_t* u = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    u[j] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return o;
+}
+
+// dx row rows[off + i] = row i of the sliced product dz W, in bf16. With one answer per row (K = 1) its column of dz
+// carries most of the row, and what its rounding to bf16 took away (val - bf16(val)) W[target] is given back, so that
+// dx is rounded once; among many answers no single rounding stands out. One warp per row.
 __global__ void __launch_bounds__(256)
-    vocab_dx_kernel(const void* __restrict__ src, long lds, long slice, int splits, const int* __restrict__ rows,
-                    const int* __restrict__ count, long off, long n, long D, __nv_bfloat16* __restrict__ dx, long lddx) {
+    vocab_dx_kernel(const float* __restrict__ out, long ldo, const float* __restrict__ slabs, int bn, int grid,
+                    const int* __restrict__ rows, const int* __restrict__ count, long off, long n, long V, long D,
+                    int K, RowOut in, const __nv_bfloat16* __restrict__ w, long ldw, __nv_bfloat16* __restrict__ dx,
+                    long lddx) {
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  const long have = count ? min(n, max(0L, (long)*count - off)) : n;
-  const bool vec = ((uintptr_t)dx & 15) == 0 && lddx % 8 == 0 && D % 8 == 0;
+  const long have = rows_here(count, off, n);
   if (i >= have) return;
+  const SliceShape shape = slice_shape((int)have, (int)D, (int)V, bn, grid);
   const long r = rows ? rows[off + i] : off + i;
+  const bool vec = ((uintptr_t)dx & 15) == 0 && lddx % 8 == 0 && D % 8 == 0;
   __nv_bfloat16* d = dx + r * lddx;
-  if (splits > 0) {
-    const float* s = reinterpret_cast<const float*>(src) + i * lds;
-    if (vec) {
-      for (long c = lane * 8; c < D; c += 256) {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int z = 0; z < splits; z++) {
-          const float4 p = *reinterpret_cast<const float4*>(s + z * slice + c),
-                       q = *reinterpret_cast<const float4*>(s + z * slice + c + 4);
-          v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w, v[4] += q.x, v[5] += q.y, v[6] += q.z, v[7] += q.w;
-        }
-        uint4 o;
-        uint32_t* u = reinterpret_cast<uint32_t*>(&o);
+  float rest = 0.f;
+  const __nv_bfloat16* wr = w;
+  if (K == 1 && in.col[i] >= 0 && in.col[i] < V) {
+    rest = in.val[i] - __bfloat162float(__float2bfloat16_rn(in.val[i]));
+    wr = w + (long)in.col[i] * ldw;
+  }
+  const bool wvec = ((uintptr_t)w & 15) == 0 && ldw % 8 == 0;
+  for (long c = lane * 8; c < D; c += 256) {
+    float v[8];
+    slice_sum8(shape, out, ldo, slabs, bn, i, (int)c, v);
+    if (rest != 0.f) {
+      if (wvec && c + 8 <= D) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(wr + c));
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          u[j] = *reinterpret_cast<const uint32_t*>(&b);
+          const float2 f = __bfloat1622float2(h[j]);
+          v[2 * j] = __fmaf_rn(rest, f.x, v[2 * j]);
+          v[2 * j + 1] = __fmaf_rn(rest, f.y, v[2 * j + 1]);
         }
-        *reinterpret_cast<uint4*>(d + c) = o;
-      }
-    } else {
-      for (long c = lane; c < D; c += 32) {
-        float v = 0.f;
-        for (int z = 0; z < splits; z++) v += s[z * slice + c];
-        d[c] = __float2bfloat16_rn(v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (c + j < D) v[j] = __fmaf_rn(rest, __bfloat162float(wr[c + j]), v[j]);
       }
     }
-  } else {
-    const __nv_bfloat16* s = reinterpret_cast<const __nv_bfloat16*>(src) + i * lds;
     if (vec) {
-      for (long c = lane * 8; c < D; c += 256) *reinterpret_cast<uint4*>(d + c) = *reinterpret_cast<const uint4*>(s + c);
+      *reinterpret_cast<uint4*>(d + c) = pack8(v);
     } else {
-      for (long c = lane; c < D; c += 32) d[c] = s[c];
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (c + j < D) d[c + j] = __float2bfloat16_rn(v[j]);
     }
   }
 }
 
-// The weight gradient from `splits` f32 slices (and the pieces before, in `acc`): kept in acc, or after the last
-// piece written in the caller's type.
+// The weight gradient from f32: a sliced product's parts (slabs) or the sum of the pieces (slabs NULL, src = acc);
+// pieces before the last are kept in acc, the last goes to dw in the caller's type. One warp per row and 256 columns.
 __global__ void __launch_bounds__(256)
-    vocab_dw_kernel(const float* __restrict__ src, long lds, long slice, int splits, float* __restrict__ acc, int first,
-                    int last, long V, long D, int f32, void* __restrict__ dw, long lddw) {
-  for (long r = blockIdx.x; r < V; r += gridDim.x)
-    for (long c = threadIdx.x; c < D; c += 256) {
-      float v = first ? 0.f : acc[r * lds + c];
-#pragma unroll 4
-      for (int z = 0; z < splits; z++) v += src[z * slice + r * lds + c];
-      if (!last)
-        acc[r * lds + c] = v;
-      else if (f32)
-        reinterpret_cast<float*>(dw)[r * lddw + c] = v;
-      else
-        reinterpret_cast<__nv_bfloat16*>(dw)[r * lddw + c] = __float2bfloat16_rn(v);
+    vocab_dw_kernel(const float* __restrict__ src, long lds, const float* __restrict__ slabs, int bn, int grid,
+                    const int* __restrict__ count, long off, long n, float* __restrict__ acc, int add, int last, long V,
+                    long D, int f32, void* __restrict__ dw, long lddw) {
+  const long r = (long)blockIdx.x * 8 + (threadIdx.x >> 5), c = (long)blockIdx.y * 256 + (threadIdx.x & 31) * 8;
+  if (r >= V || c >= D) return;
+  float v[8];
+  if (slabs) {
+    slice_sum8(slice_shape((int)V, (int)D, (int)rows_here(count, off, n), bn, grid), src, lds, slabs, bn, r, (int)c, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = src[r * lds + c + j];
+  }
+  if (add) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] += acc[r * lds + c + j];
+  }
+  if (!last) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) acc[r * lds + c + j] = v[j];
+  } else if (f32) {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (c + j < D) reinterpret_cast<float*>(dw)[r * lddw + c + j] = v[j];
+  } else {
+    __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(dw) + r * lddw + c;
+    if (((uintptr_t)dw & 15) == 0 && lddw % 8 == 0 && c + 8 <= D) {
+      *reinterpret_cast<uint4*>(d) = pack8(v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (c + j < D) d[j] = __float2bfloat16_rn(v[j]);
     }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- host side
@@ -421,20 +617,23 @@ constexpr long kVocabOneTile = 128;
 // Bytes of terms that one piece may hold. Fewer pieces mean fewer passes over the f32 weight gradient (each piece
 // after the first adds to it: 8 V D bytes).
 constexpr size_t kVocabPieceBytes = (size_t)4 << 30;
+constexpr size_t kVocabMaxK = 512;  // entries of a row: its lists stay in shared memory
 
 struct VocabPlan {
-  bool grad, compact, pack_x, pack_w, dx_direct;
-  long N, V, D, K;
-  long Dp;       // row stride of the packed matrices and of dx's
-  long ldt;      // row stride of the terms
-  int bn;        // column tile of the logits product
+  bool compact, pack_x, pack_w;
+  bool dw_slice;   // dW by a sliced product
+  long Dp;         // row stride of the packed matrices and of the f32 products
+  long ldt;        // row stride of the terms
+  int bn;          // column tile of the logits product
+  int bd;          // column tile of the two products over D columns
   long ld_stat;
-  long R;        // rows of a piece
+  long R;          // rows of a piece
   int pieces;
-  int splits, dw_splits;  // slices of the long axes of dx (V) and dW (the rows); 0: one
+  int rpb;         // rows of a block that turns terms into gradients
+  int ns;          // its columns, in 256s
   size_t bytes;
   // offsets into the workspace
-  size_t rows, count, xp, wp, bias2, stat, terms, info, uk, pk, dxs, dws, dwacc, part, dbacc;
+  size_t ids2, p, ent, has, rows, count, xp, wp, stat, ut, terms, info, col, val, dxs, slabs, dws, dwacc, part, dbacc;
 };
 
 static size_t carve(size_t& at, size_t bytes) {
@@ -443,63 +642,64 @@ static size_t carve(size_t& at, size_t bytes) {
   return o;
 }
 
-// x_ok, w_ok, dx_ok: the matrix starts at 16 bytes and its row stride is a multiple of 8 (what TMA needs).
-static VocabPlan vocab_plan(long N, long V, long D, long K, bool bias, bool grad, bool x_ok, bool w_ok, bool dx_ok,
-                            bool dw_bf16, size_t piece_bytes) {
+// K = 0: cross entropy. x_ok, w_ok: the matrix starts at 16 bytes and its row stride is a multiple of 8 (what TMA
+// needs).
+static VocabPlan vocab_plan(long N, long V, long D, long K, bool bias, bool grad, bool x_ok, bool w_ok, size_t piece_bytes,
+                            int sms) {
   VocabPlan p{};
-  p.grad = grad;
-  p.N = N;
-  p.V = V;
-  p.D = D;
-  p.K = K;
+  const long k1 = K ? K : 1;
   p.compact = N > kVocabOneTile;
   p.pack_x = p.compact || grad || !x_ok;
   p.pack_w = !w_ok;
   p.Dp = round_up(D, 8);
   p.ldt = round_up(V, 64);
   p.bn = V > 148 * 128 ? 256 : 128;
+  p.bd = D > 128 ? 256 : 128;
   p.ld_stat = ceil_div(V, p.bn) * 2;
   if (!piece_bytes) piece_bytes = kVocabPieceBytes;
   long R = (long)(piece_bytes / ((size_t)p.ldt * 2)) / 128 * 128;
   if (R < 128) R = 128;
   if (R > round_up(N, 128)) R = round_up(N, 128);
-  if (R > (1 << 21)) R = 1 << 21;  // 64-row tiles on a grid's second axis
+  if (R > (1 << 18)) R = 1 << 18;  // 8-row tiles on a grid's second axis
   p.pieces = (int)ceil_div(N, R);
   p.R = round_up(ceil_div(N, p.pieces), 128);
   p.pieces = (int)ceil_div(N, p.R);
-  // Few tiles and a long inner axis are split along it, so that every SM has a part: at least 4 k-blocks of 64.
-  auto split = [](long tiles, long inner) {
-    long s = 148 / tiles;
-    if (s > inner / 256) s = inner / 256;
-    return s > 1 ? (int)s : 0;
-  };
-  if (grad) {
-    p.splits = split(ceil_div(p.R, 128) * ceil_div(D, 256), V);
-    p.dw_splits = split(ceil_div(V, 128) * ceil_div(D, 256), p.R);
-  }
-  p.dx_direct = !p.compact && p.splits == 0 && dx_ok;
+  // a weight gradient of fewer 256 x 256 tiles than there are pairs of SMs, over enough rows to be cut
+  p.dw_slice = ceil_div(V, 256) * ceil_div(D, 256) < sms / 2 && p.R >= 512;
+  // 64 x 1,024 terms to a block, fewer where that leaves SMs idle, lists more than 512 answers or has no room for
+  // all of its rows' entries (they may all name one tile)
+  p.ns = ceil_div(V, 1024) * ceil_div(N, 64) >= 2 * sms ? 4 : 1;
+  p.rpb = 64;
+  const long cols = 256L * p.ns;
+  while (p.rpb > 8 && (p.rpb * k1 > 4096 || ceil_div(V, cols) * ceil_div(N, p.rpb) < 2 * sms ||
+                       (double)p.rpb * k1 * (V < cols ? 1.0 : (double)cols / V) > 512.0))
+    p.rpb /= 2;
   size_t at = 0;
+  if (K) {
+    p.ids2 = carve(at, (size_t)N * K * 4);
+    p.p = carve(at, (size_t)N * K * 4);
+    p.ent = carve(at, (size_t)N * 4);
+    p.has = carve(at, (size_t)N);
+  }
   if (p.compact) {
     p.rows = carve(at, (size_t)N * 4);
     p.count = carve(at, 4);
   }
   if (p.pack_x) p.xp = carve(at, (size_t)p.R * p.Dp * 2);
   if (p.pack_w) p.wp = carve(at, (size_t)round_up(V, 64) * p.Dp * 2);
-  if (bias) p.bias2 = carve(at, (size_t)round_up(V, 256) * 4);
   p.stat = carve(at, (size_t)p.R * p.ld_stat * 8);
+  if (!K) p.ut = carve(at, (size_t)p.R * 4);
   if (grad) {
     p.terms = carve(at, (size_t)p.R * p.ldt * 2);
     p.info = carve(at, (size_t)p.R * 8);
-    p.uk = carve(at, (size_t)p.R * K * 4);
-    p.pk = carve(at, (size_t)p.R * K * 4);
-    if (p.splits)
-      p.dxs = carve(at, (size_t)p.splits * p.R * p.Dp * 4);
-    else if (!p.dx_direct)
-      p.dxs = carve(at, (size_t)p.R * p.Dp * 2);
-    if (p.dw_splits) p.dws = carve(at, (size_t)p.dw_splits * V * p.Dp * 4);
-    if (p.pieces > 1 && (dw_bf16 || p.dw_splits)) p.dwacc = carve(at, (size_t)V * p.Dp * 4);
+    p.col = carve(at, (size_t)p.R * k1 * 4);
+    p.val = carve(at, (size_t)p.R * k1 * 4);
+    p.dxs = carve(at, (size_t)p.R * p.Dp * 4);
+    p.slabs = carve(at, (size_t)sms * 128 * p.bd * 4);
+    if (p.dw_slice) p.dws = carve(at, (size_t)V * p.Dp * 4);
+    if (p.pieces > 1) p.dwacc = carve(at, (size_t)V * p.Dp * 4);
     if (bias) {
-      p.part = carve(at, (size_t)(p.R / 64) * V * 4);
+      p.part = carve(at, (size_t)(p.R / p.rpb) * V * 4);
       p.dbacc = carve(at, (size_t)V * 4);
     }
   }
@@ -514,7 +714,9 @@ struct VocabCall {
   const void* w;
   size_t ldw;
   const void* bias;
-  Answers a;
+  const int* ids;
+  const float* teacher;
+  size_t K;  // 0: cross entropy, ids holds one target per row
   double temperature;
   const float* row_scale;
   size_t N, V, D;
@@ -534,10 +736,25 @@ struct VocabCall {
 
 static bool rows16(const void* p, size_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 
+template <int NS>
+static int dz_launch(const VocabPlan& p, uint8_t* ws, long V, long K, const int* count, long off, long n, RowOut ro,
+                     float* part, cudaStream_t st) {
+  const size_t smem = DzSmem<NS>::bytes(p.rpb, K, part != nullptr);
+  if (smem > 48 * 1024)
+    PL_CUDA(cudaFuncSetAttribute(vocab_dz_kernel<NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  vocab_dz_kernel<NS><<<dim3((unsigned)ceil_div(V, 256 * NS), (unsigned)(round_up(n, 64) / p.rpb)), 256, smem, st>>>(
+      ws + p.terms, p.ldt, V, (int)K, count, off, n, p.rpb, ro, (const float2*)(ws + p.stat), p.ld_stat,
+      p.bn == 256 ? 7 : 6, part);
+  count_launch();
+  PL_LAUNCH("vocab_dz_kernel");
+  return PL_OK;
+}
+
 static int vocab_run(const VocabCall& c) {
-  PL_REQUIRE(c.V > 0 && c.D > 0 && c.a.K > 0, PL_ERR_INVALID, "%s: V = %zu, D = %zu, K = %ld", c.what, c.V, c.D, c.a.K);
-  PL_REQUIRE(c.N <= (1u << 30) && c.V <= (1u << 30) && c.D <= (1u << 24) && c.a.K <= (1 << 20), PL_ERR_INVALID,
-             "%s: N = %zu, V = %zu, D = %zu, K = %ld is too large", c.what, c.N, c.V, c.D, c.a.K);
+  PL_REQUIRE(c.V > 0 && c.D > 0, PL_ERR_INVALID, "%s: V = %zu, D = %zu", c.what, c.V, c.D);
+  PL_REQUIRE(c.N <= (1u << 30) && c.V <= (1u << 30) && c.D <= (1u << 24), PL_ERR_INVALID,
+             "%s: N = %zu, V = %zu, D = %zu is too large", c.what, c.N, c.V, c.D);
+  PL_REQUIRE(c.K <= kVocabMaxK, PL_ERR_INVALID, "%s: K = %zu entries, at most %zu", c.what, c.K, kVocabMaxK);
   PL_REQUIRE(c.ldx >= c.D && c.ldw >= c.D, PL_ERR_INVALID, "%s: row strides %zu, %zu below D = %zu", c.what, c.ldx, c.ldw,
              c.D);
   PL_REQUIRE(c.temperature > 0.0 && c.temperature < 1e30, PL_ERR_INVALID, "%s: temperature %g", c.what, c.temperature);
@@ -548,11 +765,11 @@ static int vocab_run(const VocabCall& c) {
                c.lddx, c.lddw, c.D);
     PL_REQUIRE(!c.bias == !c.dbias, PL_ERR_INVALID, "%s: bias and its gradient go together", c.what);
   }
-  PL_REQUIRE(c.N == 0 || (c.x && c.a.ids && c.loss && c.lse && (!c.grad || c.dx)), PL_ERR_INVALID, "%s: NULL matrix",
-             c.what);
+  PL_REQUIRE(c.N == 0 || (c.x && c.ids && (!c.K || c.teacher) && c.loss && c.lse && (!c.grad || c.dx)), PL_ERR_INVALID,
+             "%s: NULL matrix or answers", c.what);
   int rc = require_device();
   if (rc) return rc;
-  const long N = (long)c.N, V = (long)c.V, D = (long)c.D, K = c.a.K;
+  const long N = (long)c.N, V = (long)c.V, D = (long)c.D, K = (long)c.K, k1 = K ? K : 1;
   cudaStream_t st = c.st;
   const size_t wsize = c.dw_f32 ? 4 : 2;
   if (N == 0) {
@@ -562,8 +779,9 @@ static int vocab_run(const VocabCall& c) {
     }
     return PL_OK;
   }
+  const int sms = gemm_sms();
   const VocabPlan p = vocab_plan(N, V, D, K, c.bias != nullptr, c.grad, rows16(c.x, c.ldx), rows16(c.w, c.ldw),
-                                 c.grad && rows16(c.dx, c.lddx), !c.dw_f32, c.piece_bytes);
+                                 c.piece_bytes, sms);
   PL_REQUIRE(c.ws && c.ws_bytes >= p.bytes && ((uintptr_t)c.ws & 255) == 0, PL_ERR_INVALID,
              "%s: %zu bytes of workspace (256-byte aligned), %zu needed", c.what, c.ws ? c.ws_bytes : (size_t)0, p.bytes);
   uint8_t* ws = (uint8_t*)c.ws;
@@ -571,17 +789,19 @@ static int vocab_run(const VocabCall& c) {
   int* count = p.compact ? (int*)(ws + p.count) : nullptr;
   const float inv_t = (float)(1.0 / c.temperature);
   const float scale2 = (float)((double)kLog2e / c.temperature);
-  float* bias2 = nullptr;
-  if (c.bias) {
-    bias2 = (float*)(ws + p.bias2);
-    const long Vp = round_up(V, 256);
-    vocab_bias_kernel<<<(unsigned)(Vp / 256), 256, 0, st>>>((const __nv_bfloat16*)c.bias, V, Vp, scale2, bias2);
+  const __nv_bfloat16* bias = (const __nv_bfloat16*)c.bias;
+  Answers a{K ? nullptr : c.ids, K ? ws + p.has : nullptr};
+  if (K) {
+    const size_t smem = (size_t)4 * 2 * K * 4;
+    vocab_teacher_kernel<<<(unsigned)ceil_div(N, 4), 128, smem, st>>>(c.ids, c.teacher, N, (int)K, scale2,
+                                                                     (int*)(ws + p.ids2), (float*)(ws + p.p),
+                                                                     (float*)(ws + p.ent), ws + p.has);
     count_launch();
-    PL_LAUNCH("vocab_bias_kernel");
+    PL_LAUNCH("vocab_teacher_kernel");
   }
   if (p.compact) {
     if (c.grad) PL_CUDA(cudaMemset2DAsync(c.dx, c.lddx * 2, 0, c.D * 2, c.N, st));  // rows that do not count
-    vocab_plan_kernel<<<1, 1024, 0, st>>>(c.a, N, rows, count, c.loss, c.lse);
+    vocab_plan_kernel<<<1, 1024, 0, st>>>(a, N, rows, count, c.loss, c.lse);
     count_launch();
     PL_LAUNCH("vocab_plan_kernel");
   }
@@ -602,81 +822,82 @@ static int vocab_run(const VocabCall& c) {
     long ldx = (long)c.ldx;
     if (p.pack_x) {
       __nv_bfloat16* xp = (__nv_bfloat16*)(ws + p.xp);
-      vocab_pack_kernel<<<(unsigned)ceil_div(round_up(n, 64), 8), 256, 0, st>>>(x, ldx, D, c.a, rows, count, off, n, xp,
+      vocab_pack_kernel<<<(unsigned)ceil_div(round_up(n, 64), 8), 256, 0, st>>>(x, ldx, D, a, rows, count, off, n, xp,
                                                                                p.Dp);
       count_launch();
       PL_LAUNCH("vocab_pack_kernel");
       x = xp;
       ldx = p.Dp;
     }
-    // logits: statistics of every segment, and the terms
+    // logits: statistics of every segment, the targets' logits, and the terms
     const Operand X{x, p.pack_x ? p.R : n, D, ldx, 1, 0}, W{w, V, D, ldw, 1, 0};
-    EpiArgs e{};
-    e.out = c.grad ? ws + p.terms : nullptr;
-    e.ldo = p.ldt;
-    e.out_rows = (int)(c.grad ? p.R : n);
-    e.out_cols = (int)V;
-    e.scale2 = scale2;
-    e.bias2 = bias2;
-    e.stat = (float2*)(ws + p.stat);
-    e.ld_stat = p.ld_stat;
-    e.dyn_rows = count;
-    e.dyn_off = (int)off;
-    rc = gemm_launch(p.bn, EPI_VOCAB, false, false, X, W, (int)n, (int)V, (int)D, 1, e, st);
-    if (rc) return rc;
-    float2* info = c.grad ? (float2*)(ws + p.info) : nullptr;
-    float* uk = c.grad ? (float*)(ws + p.uk) : nullptr;
-    float* pk = c.grad ? (float*)(ws + p.pk) : nullptr;
-    vocab_rows_kernel<<<(unsigned)n, 128, 0, st>>>(x, ldx, w, ldw, bias2, V, D, c.a, scale2, inv_t, c.row_scale, rows,
-                                                   count, off, (const float2*)(ws + p.stat), p.ld_stat, c.loss, c.lse,
-                                                   info, uk, pk);
+    {
+      EpiArgs e{};
+      e.out = c.grad ? ws + p.terms : nullptr;
+      e.ldo = p.ldt;
+      e.out_rows = (int)n;
+      e.out_cols = (int)V;
+      e.scale2 = scale2;
+      e.vbias = bias;
+      e.stat = (float2*)(ws + p.stat);
+      e.ld_stat = p.ld_stat;
+      if (!K) {
+        e.target = c.ids;
+        e.row_ids = rows ? rows + off : nullptr;
+        e.ut = (float*)(ws + p.ut);
+      }
+      e.dyn_rows = count;
+      e.dyn_off = (int)off;
+      rc = gemm_launch(p.bn, EPI_VOCAB, false, false, X, W, (int)n, (int)V, (int)D, 1, e, st);
+      if (rc) return rc;
+    }
+    RowOut ro{};
+    if (c.grad) ro = RowOut{(float2*)(ws + p.info), (int*)(ws + p.col), (float*)(ws + p.val)};
+    if (K) {
+      vocab_distill_rows_kernel<<<(unsigned)n, 128, 0, st>>>(
+          x, ldx, w, ldw, bias, V, D, (int)K, (const int*)(ws + p.ids2), (const float*)(ws + p.p),
+          (const float*)(ws + p.ent), ws + p.has, scale2, inv_t, c.row_scale, rows, count, off,
+          (const float2*)(ws + p.stat), p.ld_stat, c.loss, c.lse, ro);
+    } else {
+      vocab_ce_rows_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(c.ids, V, c.row_scale, rows, count, off, n,
+                                                                    (const float2*)(ws + p.stat), p.ld_stat,
+                                                                    (const float*)(ws + p.ut), c.loss, c.lse, ro);
+    }
     count_launch();
     PL_LAUNCH("vocab_rows_kernel");
     if (!c.grad) continue;
-    float* part = c.bias ? (float*)(ws + p.part) : nullptr;
-    const long tiles = ceil_div(n, 64);
-    vocab_dz_kernel<<<dim3((unsigned)ceil_div(V, 256), (unsigned)tiles), 256, 0, st>>>(
-        ws + p.terms, p.ldt, V, c.a, rows, count, off, n, info, uk, pk, (const float2*)(ws + p.stat), p.ld_stat, p.bn / 2,
-        part);
-    count_launch();
-    PL_LAUNCH("vocab_dz_kernel");
     const bool last = q == p.pieces - 1;
-    if (c.bias) {
-      vocab_dbias_kernel<<<(unsigned)ceil_div(V, 256), 256, 0, st>>>(part, (int)tiles, V, (float*)(ws + p.dbacc), q == 0,
-                                                                    last, c.dw_f32, c.dbias);
+    float* part = bias ? (float*)(ws + p.part) : nullptr;
+    rc = p.ns == 4 ? dz_launch<4>(p, ws, V, k1, count, off, n, ro, part, st)
+                   : dz_launch<1>(p, ws, V, k1, count, off, n, ro, part, st);
+    if (rc) return rc;
+    if (bias) {
+      vocab_dbias_kernel<<<(unsigned)ceil_div(V, 256), 256, 0, st>>>(part, (int)(round_up(n, 64) / p.rpb), V,
+                                                                    (float*)(ws + p.dbacc), q == 0, last, c.dw_f32,
+                                                                    c.dbias);
       count_launch();
       PL_LAUNCH("vocab_dbias_kernel");
     }
-    // dx = dz W
-    const Operand Z{ws + p.terms, p.R, V, p.ldt, 1, 0};
-    {
+    float* slabs = (float*)(ws + p.slabs);
+    {  // dx = dz W
       EpiArgs g{};
-      g.alpha = 1.f;
+      g.out = ws + p.dxs;
+      g.ldo = p.Dp;
+      g.slabs = slabs;
       g.out_rows = (int)n;
       g.out_cols = (int)D;
       g.dyn_rows = count;
       g.dyn_off = (int)off;
-      if (p.dx_direct) {
-        g.out = c.dx;
-        g.ldo = (long)c.lddx;
-      } else {
-        g.out = ws + p.dxs;
-        g.ldo = p.Dp;
-        g.out_bstride = p.R * p.Dp;
-      }
-      g.k_splits = p.splits;
-      const int bn = D > 128 ? 256 : 128;
-      rc = gemm_launch(bn, p.splits ? EPI_F32 : EPI_BF16, false, true, Z, W, (int)n, (int)D, (int)V, 1, g, st);
+      const Operand Z{ws + p.terms, p.R, V, p.ldt, 1, 0};
+      rc = gemm_launch(p.bd, EPI_SLICE, false, true, Z, W, (int)n, (int)D, (int)V, 1, g, st);
       if (rc) return rc;
-    }
-    if (!p.dx_direct) {
-      vocab_dx_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(ws + p.dxs, p.Dp, p.R * p.Dp, p.splits, rows, count, off, n,
-                                                               D, (__nv_bfloat16*)c.dx, (long)c.lddx);
+      vocab_dx_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>((const float*)(ws + p.dxs), p.Dp, slabs, p.bd, sms, rows,
+                                                               count, off, n, V, D, (int)k1, ro, w, ldw,
+                                                               (__nv_bfloat16*)c.dx, (long)c.lddx);
       count_launch();
       PL_LAUNCH("vocab_dx_kernel");
     }
-    // dW (+)= dz^T x
-    {
+    {  // dW (+)= dz^T x: to the caller's matrix, to the f32 sum of the pieces, or sliced
       EpiArgs g{};
       g.alpha = 1.f;
       g.out_rows = (int)V;
@@ -684,24 +905,21 @@ static int vocab_run(const VocabCall& c) {
       g.dyn_rows = count;
       g.dyn_off = (int)off;
       g.dyn_k = 1;
-      // slices, the sum of the pieces so far, or the caller's matrix
-      const bool direct = !p.dw_splits && (p.pieces == 1 || c.dw_f32);
-      const bool f32 = !direct || c.dw_f32;
-      g.out = direct ? c.dw : (void*)(ws + (p.dw_splits ? p.dws : p.dwacc));
+      const bool direct = !p.dw_slice && (p.pieces == 1 || c.dw_f32);
+      float* acc = (float*)(ws + p.dwacc);
+      const int epi = p.dw_slice ? EPI_SLICE : (direct && !c.dw_f32 ? EPI_BF16 : EPI_F32);
+      g.out = p.dw_slice ? (void*)(ws + p.dws) : (direct ? c.dw : (void*)acc);
       g.ldo = direct ? (long)c.lddw : p.Dp;
-      g.out_bstride = V * p.Dp;
-      g.k_splits = p.dw_splits;
-      g.accum = !p.dw_splits && q > 0;
+      g.slabs = slabs;
+      g.accum = !p.dw_slice && q > 0;
       const Operand Xk{x, n, D, ldx, 1, 0};
       const Operand Zk{ws + p.terms, n, V, p.ldt, 1, 0};
-      const int bn = D > 128 ? 256 : 128;
-      rc = gemm_launch(bn, f32 ? EPI_F32 : EPI_BF16, true, true, Zk, Xk, (int)V, (int)D, (int)n, 1, g, st);
+      rc = gemm_launch(p.bd, epi, true, true, Zk, Xk, (int)V, (int)D, (int)n, 1, g, st);
       if (rc) return rc;
-      if (!direct && (p.dw_splits || last)) {
-        float* acc = (float*)(ws + p.dwacc);
-        vocab_dw_kernel<<<(unsigned)(V < 148 * 16 ? V : 148 * 16), 256, 0, st>>>(
-            p.dw_splits ? (const float*)(ws + p.dws) : acc, p.Dp, V * p.Dp, p.dw_splits ? p.dw_splits : 1, acc,
-            !p.dw_splits || q == 0, last, V, D, c.dw_f32, c.dw, (long)c.lddw);
+      if (!direct && (p.dw_slice || last)) {
+        vocab_dw_kernel<<<dim3((unsigned)ceil_div(V, 8), (unsigned)ceil_div(D, 256)), 256, 0, st>>>(
+            p.dw_slice ? (const float*)(ws + p.dws) : acc, p.Dp, p.dw_slice ? slabs : nullptr, p.bd, sms, count, off, n,
+            acc, p.dw_slice && q > 0, last, V, D, c.dw_f32, c.dw, (long)c.lddw);
         count_launch();
         PL_LAUNCH("vocab_dw_kernel");
       }
@@ -716,9 +934,11 @@ extern "C" {
 
 size_t pl_vocab_ws(size_t N, size_t V, size_t D, size_t K, uint8_t bias, uint8_t grad, uint8_t aligned,
                    size_t piece_bytes) {
-  if (N == 0 || V == 0 || D == 0 || K == 0) return 0;
+  if (N == 0 || V == 0 || D == 0) return 0;
   const bool ok = aligned != 0;
-  return pl::vocab_plan((long)N, (long)V, (long)D, (long)K, bias != 0, grad != 0, ok, ok, ok, true, piece_bytes).bytes;
+  return pl::vocab_plan((long)N, (long)V, (long)D, (long)K, bias != 0, grad != 0, ok, ok, piece_bytes,
+                        pl::gemm_sms())
+      .bytes;
 }
 
 int pl_vocab_ce_dev(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, const int32_t* target,
@@ -726,7 +946,7 @@ int pl_vocab_ce_dev(const void* x, size_t ldx, const void* w, size_t ldw, const 
   pl::VocabCall c{};
   c.what = "pl_vocab_ce_dev";
   c.x = x, c.ldx = ldx, c.w = w, c.ldw = ldw, c.bias = bias;
-  c.a = pl::Answers{target, nullptr, 1};
+  c.ids = target;
   c.temperature = 1.0;
   c.N = N, c.V = V, c.D = D, c.loss = loss, c.lse = lse, c.ws = ws, c.ws_bytes = ws_bytes;
   c.st = (cudaStream_t)stream;
@@ -740,7 +960,7 @@ int pl_vocab_ce_grad_dev(const void* x, size_t ldx, const void* w, size_t ldw, c
   pl::VocabCall c{};
   c.what = "pl_vocab_ce_grad_dev";
   c.x = x, c.ldx = ldx, c.w = w, c.ldw = ldw, c.bias = bias;
-  c.a = pl::Answers{target, nullptr, 1};
+  c.ids = target;
   c.temperature = 1.0;
   c.row_scale = row_scale;
   c.N = N, c.V = V, c.D = D, c.loss = loss, c.lse = lse, c.ws = ws, c.ws_bytes = ws_bytes;
@@ -756,11 +976,11 @@ int pl_vocab_distill_dev(const void* x, size_t ldx, const void* w, size_t ldw, c
   pl::VocabCall c{};
   c.what = "pl_vocab_distill_dev";
   c.x = x, c.ldx = ldx, c.w = w, c.ldw = ldw, c.bias = bias;
-  c.a = pl::Answers{ids, teacher, (long)K};
+  c.ids = ids, c.teacher = teacher, c.K = K;
   c.temperature = temperature;
   c.N = N, c.V = V, c.D = D, c.loss = loss, c.lse = lse, c.ws = ws, c.ws_bytes = ws_bytes;
   c.st = (cudaStream_t)stream;
-  if (N > 0 && !teacher) return pl::set_error(PL_ERR_INVALID, "pl_vocab_distill_dev: NULL teacher");
+  if (K == 0) return pl::set_error(PL_ERR_INVALID, "pl_vocab_distill_dev: K = 0");
   return pl::vocab_run(c);
 }
 
@@ -771,14 +991,14 @@ int pl_vocab_distill_grad_dev(const void* x, size_t ldx, const void* w, size_t l
   pl::VocabCall c{};
   c.what = "pl_vocab_distill_grad_dev";
   c.x = x, c.ldx = ldx, c.w = w, c.ldw = ldw, c.bias = bias;
-  c.a = pl::Answers{ids, teacher, (long)K};
+  c.ids = ids, c.teacher = teacher, c.K = K;
   c.temperature = temperature;
   c.row_scale = row_scale;
   c.N = N, c.V = V, c.D = D, c.loss = loss, c.lse = lse, c.ws = ws, c.ws_bytes = ws_bytes;
   c.dx = dx, c.lddx = lddx, c.dw = dw, c.lddw = lddw, c.dbias = dbias, c.dw_f32 = dw_f32, c.piece_bytes = piece_bytes;
   c.grad = true;
   c.st = (cudaStream_t)stream;
-  if (N > 0 && !teacher) return pl::set_error(PL_ERR_INVALID, "pl_vocab_distill_grad_dev: NULL teacher");
+  if (K == 0) return pl::set_error(PL_ERR_INVALID, "pl_vocab_distill_grad_dev: K = 0");
   return pl::vocab_run(c);
 }
 

@@ -137,13 +137,13 @@ def _head(what, x, w, bias, ids, teacher, temperature, row_scale, grad, dw_f32=F
         tp = _vector(teacher, what, "teacher", _F32, (n, k), dev)
         _need(temperature > 0.0, what, "temperature %g", temperature)
     else:
-        k = 1
+        k = 0
         _need(ids is not None, what, "target is needed")
         ip = _vector(ids, what, "target", _I32, (n,), dev)
     sp = _vector(row_scale, what, "row_scale", _F32, (n,), dev)
     with _On(dev) as st:
         L = lib()
-        aligned = ldx % 8 == 0 and ldw % 8 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0 and d % 8 == 0
+        aligned = ldx % 8 == 0 and ldw % 8 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0
         size = L.pl_vocab_ws(n, v, d, k, bias is not None, grad, aligned, piece_bytes)
         out = torch.empty((2, n), dtype=_F32, device=dev)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
