@@ -93,108 +93,10 @@ __device__ __forceinline__ float group_sum(float v, float* scr) {
   return warp_sum(lane < NW ? scr[w0 + lane] : 0.f);
 }
 
-template <typename T, int VEC, int TPR, int K>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
-    norm_fwd_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w, const float* __restrict__ b,
-                    long rows, int cols, float eps, T* __restrict__ y, long ldy, float* __restrict__ mean,
-                    float* __restrict__ rstd) {
-  constexpr int THREADS = TPR > 256 ? TPR : 256, G = THREADS / TPR;
-  __shared__ float scr[2][32];
-  const int t = threadIdx.x % TPR;
-  const long row = (long)blockIdx.x * G + threadIdx.x / TPR;
-  const bool ok = row < rows;
-  Pack<T, VEC> in[K];
-  const T* xr = x + row * ldx;
-#pragma unroll
-  for (int k = 0; k < K; k++) {
-    const int c = (k * TPR + t) * VEC;
-    if (ok && c < cols) in[k].load(xr + c);
-  }
-  float s = 0.f;
-#pragma unroll
-  for (int k = 0; k < K; k++) {
-    if (ok && (k * TPR + t) * VEC < cols) {
-#pragma unroll
-      for (int j = 0; j < VEC; j++) s += to_f(in[k].v[j]);
-    }
-  }
-  const float inv = 1.f / (float)cols;
-  const float m = group_sum<TPR>(s, scr[0]) * inv;
-  s = 0.f;
-#pragma unroll
-  for (int k = 0; k < K; k++) {
-    if (ok && (k * TPR + t) * VEC < cols) {
-#pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        const float d = to_f(in[k].v[j]) - m;
-        s = __fmaf_rn(d, d, s);
-      }
-    }
-  }
-  const float r = 1.f / sqrtf(group_sum<TPR>(s, scr[1]) * inv + eps);
-  if (!ok) return;
-  if (t == 0) {
-    mean[row] = m;
-    rstd[row] = r;
-  }
-  T* yr = y + row * ldy;
-#pragma unroll
-  for (int k = 0; k < K; k++) {
-    const int c = (k * TPR + t) * VEC;
-    if (c >= cols) break;
-    float wv[VEC], bv[VEC];
-    if (w) load_param<VEC>(w, c, wv);
-    if (b) load_param<VEC>(b, c, bv);
-    Pack<T, VEC> out;
-#pragma unroll
-    for (int j = 0; j < VEC; j++) {
-      float v = (to_f(in[k].v[j]) - m) * r;
-      if (w) v *= wv[j];
-      if (b) v += bv[j];
-      out.v[j] = from_f<T>(v);
-    }
-    out.store(yr + c);
-  }
-}
+// Threads of a block whose rows take TPR threads each, and the blocks that share an SM (`of256` of 256 threads).
+__host__ __device__ constexpr int norm_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+__host__ __device__ constexpr int norm_blocks(int tpr, int of256) { return tpr > 256 ? (tpr > 512 ? 1 : (of256 + 1) / 2) : of256; }
 
-// Rows too wide for the registers: one block per row, the row read three times (its second and third reads hit
-// L2).
-template <typename T>
-__global__ void __launch_bounds__(512)
-    norm_fwd_wide_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w, const float* __restrict__ b,
-                         long rows, long cols, float eps, T* __restrict__ y, long ldy, float* __restrict__ mean,
-                         float* __restrict__ rstd) {
-  __shared__ float scr[2][32];
-  const long row = blockIdx.x;
-  const T* xr = x + row * ldx;
-  const float inv = 1.f / (float)cols;
-  float s = 0.f;
-  for (long c = threadIdx.x; c < cols; c += 512) s += to_f(xr[c]);
-  const float m = group_sum<512>(s, scr[0]) * inv;
-  s = 0.f;
-  for (long c = threadIdx.x; c < cols; c += 512) {
-    const float d = to_f(xr[c]) - m;
-    s = __fmaf_rn(d, d, s);
-  }
-  const float r = 1.f / sqrtf(group_sum<512>(s, scr[1]) * inv + eps);
-  if (threadIdx.x == 0) {
-    mean[row] = m;
-    rstd[row] = r;
-  }
-  for (long c = threadIdx.x; c < cols; c += 512) {
-    float v = (to_f(xr[c]) - m) * r;
-    if (w) v *= w[c];
-    if (b) v += b[c];
-    y[row * ldy + c] = from_f<T>(v);
-  }
-}
-
-// ---------------------------------------------------------------------------------------------- backward
-// A block walks the rows with RB of them per group in flight: the two row sums of RB rows are folded in one
-// butterfly, and each thread adds its columns of dy xh and dy to registers over all of its block's rows. The
-// blocks' column sums go to `part` ([grid][2][cols]) and are added in block order by norm_param_kernel.
-// Wide rows leave few registers per thread: RB falls, and the weight is read again (from L1) for each row.
-//
 // Sums N values (a power of two up to 32) over the lanes with one exchange less per level than the values kept:
 // lane l returns the total of value l / (32 / N).
 template <int N>
@@ -238,12 +140,162 @@ __device__ __forceinline__ float warp_sum_n(const float (&v)[N], int lane) {
   }
 }
 
+// Totals over each row group of the N values a thread brings (a fixed order), the values spread over the lanes: lane l
+// of every warp of the group holds value l / (32 / N). `scr` is [N][32] floats that no thread still reads.
+template <int TPR, int N>
+__device__ __forceinline__ float group_sum_n(const float (&s)[N], float (*scr)[32], int lane, int warp) {
+  constexpr int NW = TPR / 32, LV = 32 / N;
+  float v = warp_sum_n<N>(s, lane);
+  if constexpr (NW > 1) {
+    if (lane % LV == 0) scr[lane / LV][warp] = v;
+    __syncthreads();
+    v = 0.f;
+    const int w0 = warp / NW * NW;
+#pragma unroll
+    for (int q = 0; q < (NW + LV - 1) / LV; q++)
+      if (lane % LV + LV * q < NW) v += scr[lane / LV][w0 + lane % LV + LV * q];
+#pragma unroll
+    for (int o = 1; o < LV; o *= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
+  return v;
+}
+
+// A block walks the rows, RB of them per group at a time: their loads are issued one step ahead, their sums folded in
+// one butterfly, and the weights stay in registers (read again per row they cost twice the row's own L1 traffic:
+// 65,536 x 2,048 bf16 took 135 us that way).
 template <typename T, int VEC, int TPR, int K, int RB>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+__global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR, 3))
+    norm_fwd_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w, const float* __restrict__ b,
+                    long rows, int cols, float eps, T* __restrict__ y, long ldy, float* __restrict__ mean,
+                    float* __restrict__ rstd) {
+  constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR, LV = 32 / RB;
+  __shared__ float scr[2][RB][32];
+  const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float inv = 1.f / (float)cols;
+  float wv[K][VEC], bv[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int c = (k * TPR + t) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+      wv[k][j] = 1.f;
+      bv[k][j] = 0.f;
+    }
+    if (w && c < cols) load_param<VEC>(w, c, wv[k]);
+    if (b && c < cols) load_param<VEC>(b, c, bv[k]);
+  }
+  Pack<T, VEC> in[RB][K], nx[RB][K];
+  auto load = [&](long r0, Pack<T, VEC> (&p)[RB][K]) {
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        const int c = (k * TPR + t) * VEC;
+        if (r0 + i < rows && c < cols) p[i][k].load(x + (r0 + i) * ldx + c);
+      }
+  };
+  const long step = (long)gridDim.x * G * RB;
+  load((long)blockIdx.x * G * RB + g * RB, in);
+  for (long base = (long)blockIdx.x * G * RB; base < rows; base += step) {
+    const long r0 = base + (long)g * RB;
+    if (base + step < rows) load(r0 + step, nx);
+    float s[RB], m[RB];
+#pragma unroll
+    for (int i = 0; i < RB; i++) {
+      s[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; k++)
+        if (r0 + i < rows && (k * TPR + t) * VEC < cols) {
+#pragma unroll
+          for (int j = 0; j < VEC; j++) s[i] += to_f(in[i][k].v[j]);
+        }
+    }
+    float v = group_sum_n<TPR, RB>(s, scr[0], lane, warp);
+#pragma unroll
+    for (int i = 0; i < RB; i++) {
+      m[i] = __shfl_sync(0xffffffffu, v, i * LV) * inv;
+      s[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; k++)
+        if (r0 + i < rows && (k * TPR + t) * VEC < cols) {
+#pragma unroll
+          for (int j = 0; j < VEC; j++) {
+            const float d = to_f(in[i][k].v[j]) - m[i];
+            s[i] = __fmaf_rn(d, d, s[i]);
+          }
+        }
+    }
+    v = group_sum_n<TPR, RB>(s, scr[1], lane, warp);  // its barrier also ends the reads of scr[0]
+#pragma unroll
+    for (int i = 0; i < RB; i++) {
+      const float r = 1.f / sqrtf(__shfl_sync(0xffffffffu, v, i * LV) * inv + eps);
+      if (r0 + i < rows) {
+        if (t == 0) {
+          mean[r0 + i] = m[i];
+          rstd[r0 + i] = r;
+        }
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+          const int c = (k * TPR + t) * VEC;
+          if (c >= cols) break;
+          Pack<T, VEC> out;
+#pragma unroll
+          for (int j = 0; j < VEC; j++) out.v[j] = from_f<T>((to_f(in[i][k].v[j]) - m[i]) * r * wv[k][j] + bv[k][j]);
+          out.store(y + (r0 + i) * ldy + c);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+      for (int k = 0; k < K; k++) in[i][k] = nx[i][k];
+  }
+}
+
+// Rows too wide for the registers: one block per row, the row read three times (its second and third reads hit
+// L2).
+template <typename T>
+__global__ void __launch_bounds__(512)
+    norm_fwd_wide_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w, const float* __restrict__ b,
+                         long rows, long cols, float eps, T* __restrict__ y, long ldy, float* __restrict__ mean,
+                         float* __restrict__ rstd) {
+  __shared__ float scr[2][32];
+  const long row = blockIdx.x;
+  const T* xr = x + row * ldx;
+  const float inv = 1.f / (float)cols;
+  float s = 0.f;
+  for (long c = threadIdx.x; c < cols; c += 512) s += to_f(xr[c]);
+  const float m = group_sum<512>(s, scr[0]) * inv;
+  s = 0.f;
+  for (long c = threadIdx.x; c < cols; c += 512) {
+    const float d = to_f(xr[c]) - m;
+    s = __fmaf_rn(d, d, s);
+  }
+  const float r = 1.f / sqrtf(group_sum<512>(s, scr[1]) * inv + eps);
+  if (threadIdx.x == 0) {
+    mean[row] = m;
+    rstd[row] = r;
+  }
+  for (long c = threadIdx.x; c < cols; c += 512) {
+    float v = (to_f(xr[c]) - m) * r;
+    if (w) v *= w[c];
+    if (b) v += b[c];
+    y[row * ldy + c] = from_f<T>(v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- backward
+// A block walks the rows with RB of them per group in flight: the two row sums of RB rows are folded in one
+// butterfly, and each thread adds its columns of dy xh and dy to registers over all of its block's rows. The
+// blocks' column sums go to `part` ([grid][2][cols]) and are added in block order by norm_param_kernel.
+// Wide rows leave few registers per thread: RB falls, and the weight is read again (from L1) for each row.
+template <typename T, int VEC, int TPR, int K, int RB>
+__global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR, 2))
     norm_bwd_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ x, long ldx,
                     const float* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
                     long rows, int cols, T* __restrict__ dx, long lddx, float* __restrict__ part) {
-  constexpr int THREADS = TPR > 256 ? TPR : 256, G = THREADS / TPR, E = VEC * K, NW = TPR / 32;
+  constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR, E = VEC * K;
   constexpr int NV = 2 * RB, LV = 32 / NV;  // values of an iteration, lanes that hold one of them
   constexpr bool KEEP_W = TPR < 1024;
   __shared__ float scr[2][NV][32];          // [iteration parity][value][warp]
@@ -265,11 +317,9 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
 #pragma unroll
   for (int e = 0; e < E; e++) dw[e] = db[e] = 0.f;
 
-  int parity = 0;
-  for (long base = (long)blockIdx.x * G * RB; base < rows; base += (long)gridDim.x * G * RB, parity ^= 1) {
-    const long r0 = base + (long)g * RB;
-    Pack<T, VEC> xi[RB][K], di[RB][K];
-    float m[RB], r[RB];
+  Pack<T, VEC> xi[RB][K], di[RB][K], xn[RB][K], dn[RB][K];
+  float m[RB], r[RB], mn[RB], rn[RB];
+  auto load = [&](long r0, Pack<T, VEC> (&px)[RB][K], Pack<T, VEC> (&pd)[RB][K], float (&pm)[RB], float (&pr)[RB]) {
 #pragma unroll
     for (int i = 0; i < RB; i++) {
       const bool ok = r0 + i < rows;
@@ -277,16 +327,23 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
       for (int k = 0; k < K; k++) {
         const int c = (k * TPR + t) * VEC;
         if (ok && c < cols) {
-          xi[i][k].load(x + (r0 + i) * ldx + c);
-          di[i][k].load(dy + (r0 + i) * lddy + c);
+          px[i][k].load(x + (r0 + i) * ldx + c);
+          pd[i][k].load(dy + (r0 + i) * lddy + c);
         } else {  // nothing there: dy = 0 keeps it out of every sum
 #pragma unroll
-          for (int j = 0; j < VEC; j++) xi[i][k].v[j] = di[i][k].v[j] = from_f<T>(0.f);
+          for (int j = 0; j < VEC; j++) px[i][k].v[j] = pd[i][k].v[j] = from_f<T>(0.f);
         }
       }
-      m[i] = ok ? __ldg(mean + r0 + i) : 0.f;
-      r[i] = ok ? __ldg(rstd + r0 + i) : 0.f;
+      pm[i] = ok ? __ldg(mean + r0 + i) : 0.f;
+      pr[i] = ok ? __ldg(rstd + r0 + i) : 0.f;
     }
+  };
+  int parity = 0;
+  const long step = (long)gridDim.x * G * RB;
+  load((long)blockIdx.x * G * RB + g * RB, xi, di, m, r);
+  for (long base = (long)blockIdx.x * G * RB; base < rows; base += step, parity ^= 1) {
+    const long r0 = base + (long)g * RB;
+    if (base + step < rows) load(r0 + step, xn, dn, mn, rn);
     float s[NV];
 #pragma unroll
     for (int i = 0; i < RB; i++) {
@@ -306,18 +363,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
       s[2 * i] = s1;
       s[2 * i + 1] = s2;
     }
-    float v = warp_sum_n<NV>(s, lane);
-    if constexpr (NW > 1) {
-      if (lane % LV == 0) scr[parity][lane / LV][warp] = v;
-      __syncthreads();  // the other parity's values were read before this barrier
-      v = 0.f;
-      const int w0 = g * NW;
-#pragma unroll
-      for (int q = 0; q < (NW + LV - 1) / LV; q++)
-        if (lane % LV + LV * q < NW) v += scr[parity][lane / LV][w0 + lane % LV + LV * q];
-#pragma unroll
-      for (int o = 1; o < LV; o *= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-    }
+    const float v = group_sum_n<TPR, NV>(s, scr[parity], lane, warp);  // the other parity's barrier ended its reads
 #pragma unroll
     for (int i = 0; i < RB; i++) {
       const float a1 = __shfl_sync(0xffffffffu, v, 2 * i * LV) * inv;        // mean of g
@@ -338,6 +384,16 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
           out.store(dx + (r0 + i) * lddx + c);
         }
       }
+    }
+#pragma unroll
+    for (int i = 0; i < RB; i++) {
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        xi[i][k] = xn[i][k];
+        di[i][k] = dn[i][k];
+      }
+      m[i] = mn[i];
+      r[i] = rn[i];
     }
   }
   if (!part) return;
@@ -377,29 +433,26 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
   }
 }
 
-// dw[c] = sum_p part[p][0][c], db[c] = sum_p part[p][1][c]: 32 columns per block, eight slices of the parts, both
+// dw[c] = sum_p part[p][0][c], db[c] = sum_p part[p][1][c]: 32 columns per block, 32 slices of the parts, both
 // folded in a fixed order.
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
     norm_param_kernel(const float* __restrict__ part, int parts, long cols, float* __restrict__ dw,
                       float* __restrict__ db) {
-  __shared__ float scr[8][32];
+  __shared__ float scr[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const long c = (long)blockIdx.x * 32 + lane;
   const float* p = part + (blockIdx.y ? cols : 0);
   float s = 0.f;
   if (c < cols) {
-#pragma unroll 4
-    for (int q = slice; q < parts; q += 8) s += __ldg(p + (long)q * 2 * cols + c);
+#pragma unroll 10
+    for (int q = slice; q < parts; q += 32) s += __ldg(p + (long)q * 2 * cols + c);
   }
   scr[slice][lane] = s;
   __syncthreads();
-  if (slice == 0 && c < cols) {
-    float t = scr[0][lane];
-#pragma unroll
-    for (int q = 1; q < 8; q++) t += scr[q][lane];
-    float* o = blockIdx.y ? db : dw;
-    if (o) o[c] = t;
-  }
+  s = warp_sum(scr[lane][slice]);  // warp `slice` folds column `slice` of the block
+  const long o = (long)blockIdx.x * 32 + slice;
+  float* out = blockIdx.y ? db : dw;
+  if (lane == 0 && o < cols && out) out[o] = s;
 }
 
 // Rows too wide for the registers. dx: one block per row, both inputs read twice.
@@ -444,18 +497,23 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-constexpr int kNormParts = 2 * 148;   // most blocks (and slices) whose column sums are kept
+constexpr int kNormSms = 148;             // SMs that the persistent grids are sized for
+constexpr int kNormParts = 2 * kNormSms;  // most blocks (and slices) whose column sums are kept
 
 static bool vec_ok(const void* p, size_t ld, size_t esz) {
   return ((uintptr_t)p & 15) == 0 && (ld * esz) % 16 == 0;
 }
 
-template <typename T, int VEC, int TPR, int K>
+template <typename T, int VEC, int TPR, int K, int RB>
 static int fwd_launch(const void* x, long ldx, const float* w, const float* b, long rows, int cols, float eps, void* y,
                       long ldy, float* mean, float* rstd, cudaStream_t st) {
-  constexpr int THREADS = TPR > 256 ? TPR : 256, G = THREADS / TPR;
-  norm_fwd_kernel<T, VEC, TPR, K><<<(unsigned)ceil_div(rows, G), THREADS, 0, st>>>((const T*)x, ldx, w, b, rows, cols,
-                                                                                   eps, (T*)y, ldy, mean, rstd);
+  constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR;
+  const long need = ceil_div(rows, (long)G * RB), most = (long)kNormSms * norm_blocks(TPR, 3);
+  // few rows: one per group, so that more SMs have some (latency); many: RB at a time
+  if constexpr (RB > 1)
+    if (need < most / 2) return fwd_launch<T, VEC, TPR, K, 1>(x, ldx, w, b, rows, cols, eps, y, ldy, mean, rstd, st);
+  norm_fwd_kernel<T, VEC, TPR, K, RB><<<(unsigned)(need < most ? need : most), THREADS, 0, st>>>(
+      (const T*)x, ldx, w, b, rows, cols, eps, (T*)y, ldy, mean, rstd);
   count_launch();
   PL_LAUNCH("norm_fwd_kernel");
   return PL_OK;
@@ -467,24 +525,26 @@ static int fwd_pick(const void* x, long ldx, const float* w, const float* b, lon
   constexpr int V = 16 / sizeof(T);
   const bool vec = vec_ok(x, ldx, sizeof(T)) && vec_ok(y, ldy, sizeof(T)) && cols % V == 0 &&
                    (!w || ((uintptr_t)w & 15) == 0) && (!b || ((uintptr_t)b & 15) == 0);
-#define PL_FWD(VEC, TPR, K) \
-  if (cols <= (long)VEC * TPR * K) return fwd_launch<T, VEC, TPR, K>(x, ldx, w, b, rows, (int)cols, eps, y, ldy, mean, rstd, st);
+#define PL_FWD(VEC, TPR, K, RB)    \
+  if (cols <= (long)VEC * TPR * K) \
+    return fwd_launch<T, VEC, TPR, K, RB>(x, ldx, w, b, rows, (int)cols, eps, y, ldy, mean, rstd, st);
   if (vec) {
-    PL_FWD(V, 32, 1)
-    PL_FWD(V, 32, 2)
-    PL_FWD(V, 32, 4)
-    PL_FWD(V, 128, 2)
-    PL_FWD(V, 128, 4)
-    PL_FWD(V, 512, 2)
-    PL_FWD(V, 512, 4)
-    PL_FWD(V, 512, 8)
+    PL_FWD(V, 32, 1, 4)
+    PL_FWD(V, 64, 1, 4)
+    PL_FWD(V, 128, 1, 4)
+    PL_FWD(V, 256, 1, 4)
+    PL_FWD(V, 512, 1, 2)
+    PL_FWD(V, 1024, 1, 2)
+    PL_FWD(V, 1024, 2, 1)
+    if constexpr (V == 4) PL_FWD(V, 1024, 4, 1)
   } else {
-    PL_FWD(1, 32, 4)
-    PL_FWD(1, 32, 16)
-    PL_FWD(1, 128, 8)
-    PL_FWD(1, 128, 16)
-    PL_FWD(1, 512, 16)
-    PL_FWD(1, 512, 32)
+    PL_FWD(1, 32, 4, 4)
+    PL_FWD(1, 64, 8, 2)
+    PL_FWD(1, 128, 8, 2)
+    PL_FWD(1, 256, 8, 2)
+    PL_FWD(1, 512, 8, 1)
+    PL_FWD(1, 1024, 8, 1)
+    PL_FWD(1, 1024, 16, 1)
   }
 #undef PL_FWD
   norm_fwd_wide_kernel<T><<<(unsigned)rows, 512, 0, st>>>((const T*)x, ldx, w, b, rows, cols, eps, (T*)y, ldy, mean, rstd);
@@ -494,7 +554,7 @@ static int fwd_pick(const void* x, long ldx, const float* w, const float* b, lon
 }
 
 static int param_launch(const float* part, int parts, long cols, float* dw, float* db, cudaStream_t st) {
-  norm_param_kernel<<<dim3((unsigned)ceil_div(cols, 32), 2), 256, 0, st>>>(part, parts, cols, dw, db);
+  norm_param_kernel<<<dim3((unsigned)ceil_div(cols, 32), 2), 1024, 0, st>>>(part, parts, cols, dw, db);
   count_launch();
   PL_LAUNCH("norm_param_kernel");
   return PL_OK;
@@ -504,11 +564,15 @@ template <typename T, int VEC, int TPR, int K, int RB>
 static int bwd_launch(const void* dy, long lddy, const void* x, long ldx, const float* w, const float* mean,
                       const float* rstd, long rows, int cols, void* dx, long lddx, float* dw, float* db, float* part,
                       cudaStream_t st) {
-  constexpr int THREADS = TPR > 256 ? TPR : 256, G = THREADS / TPR;
+  constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR;
   constexpr size_t SMEM = G > 1 ? (size_t)G * 2 * TPR * VEC * K * 4 : 0;
   static_assert(SMEM <= 48 * 1024, "column sums of the groups");
-  const long need = ceil_div(rows, (long)G * RB);
-  const int grid = (int)(need < kNormParts ? need : kNormParts);
+  const long need = ceil_div(rows, (long)G * RB), most = (long)kNormSms * norm_blocks(TPR, 2);
+  static_assert(kNormSms * norm_blocks(TPR, 2) <= kNormParts, "column sums of the blocks");
+  if constexpr (RB > 1)
+    if (need < most / 2)
+      return bwd_launch<T, VEC, TPR, K, 1>(dy, lddy, x, ldx, w, mean, rstd, rows, cols, dx, lddx, dw, db, part, st);
+  const int grid = (int)(need < most ? need : most);
   norm_bwd_kernel<T, VEC, TPR, K, RB><<<grid, THREADS, SMEM, st>>>((const T*)dy, lddy, (const T*)x, ldx, w, mean, rstd, rows,
                                                                cols, (T*)dx, lddx, (dw || db) ? part : nullptr);
   count_launch();
@@ -527,20 +591,20 @@ static int bwd_pick(const void* dy, long lddy, const void* x, long ldx, const fl
   if (cols <= (long)VEC * TPR * K) \
     return bwd_launch<T, VEC, TPR, K, RB>(dy, lddy, x, ldx, w, mean, rstd, rows, (int)cols, dx, lddx, dw, db, part, st);
   if (vec) {
-    PL_BWD(V, 32, 1, 4)
-    PL_BWD(V, 64, 1, 4)
-    PL_BWD(V, 128, 1, 4)
-    PL_BWD(V, 256, 1, 4)
-    PL_BWD(V, 512, 1, 4)
-    PL_BWD(V, 512, 2, 2)
+    PL_BWD(V, 32, 1, 2)
+    PL_BWD(V, 64, 1, 2)
+    PL_BWD(V, 128, 1, 2)
+    PL_BWD(V, 256, 1, 2)
+    PL_BWD(V, 512, 1, 2)
+    PL_BWD(V, 1024, 1, 1)
     PL_BWD(V, 1024, 2, 1)
     if constexpr (V == 4) PL_BWD(V, 1024, 4, 1)
   } else {
     PL_BWD(1, 32, 4, 4)
-    PL_BWD(1, 64, 8, 4)
-    PL_BWD(1, 128, 8, 4)
-    PL_BWD(1, 256, 8, 4)
-    PL_BWD(1, 512, 8, 4)
+    PL_BWD(1, 64, 8, 2)
+    PL_BWD(1, 128, 8, 2)
+    PL_BWD(1, 256, 8, 2)
+    PL_BWD(1, 512, 8, 1)
     PL_BWD(1, 1024, 8, 1)
     PL_BWD(1, 1024, 16, 1)
   }

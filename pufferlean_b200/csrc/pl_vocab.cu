@@ -358,8 +358,8 @@ struct DzSmem {
     return (size_t)rpb * COLS / 8 + (size_t)rpb * K * 8 + (part ? (size_t)8 * COLS * 4 : 0);
   }
 };
-template <int NS>
-__global__ void __launch_bounds__(256)
+template <int NS, bool PART>
+__global__ void __launch_bounds__(256, PART ? 3 : 4)
     vocab_dz_kernel(void* __restrict__ terms, long ld, long V, int K, const int* __restrict__ count, long off, long n,
                     int rpb, RowOut in, const float2* __restrict__ stat, long ld_stat, int seg_shift,
                     float* __restrict__ part) {
@@ -368,27 +368,28 @@ __global__ void __launch_bounds__(256)
   uint32_t* mask = reinterpret_cast<uint32_t*>(dyn_smem);                   // [rpb][COLS / 32]
   uint32_t* hit_at = mask + rpb * (COLS / 32);                              // [rpb K]: row << 16 | column
   float* hit_v = reinterpret_cast<float*>(hit_at + (long)rpb * K);          // [rpb K]
-  float* fold = hit_v + (long)rpb * K;                                      // [8][COLS] (part)
+  float* fold = hit_v + (long)rpb * K;                                      // [8][COLS] (PART)
   __shared__ int warp_n[8];
   const long have = rows_here(count, off, n);
   const long r0 = (long)blockIdx.y * rpb, c0 = (long)blockIdx.x * COLS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint16_t* base = reinterpret_cast<uint16_t*>(terms);
-  float sum[NS][8];
+  uint16_t* base = reinterpret_cast<uint16_t*>(terms) + r0 * ld + c0 + lane * 8;
+  const int left = (int)min((long)COLS, V - c0) - lane * 8;  // columns from this lane's first on
+  float2 sum[NS][4];
 #pragma unroll
   for (int s = 0; s < NS; s++)
 #pragma unroll
-    for (int j = 0; j < 8; j++) sum[s][j] = 0.f;
+    for (int j = 0; j < 4; j++) sum[s][j] = make_float2(0.f, 0.f);
   int hits = 0;
   const int nr = (int)max(0L, min((long)rpb, have - r0));
   if (nr > 0) {
     for (int q = threadIdx.x; q < rpb * (COLS / 32); q += 256) mask[q] = 0u;
     const int total = nr * K;
+    const int* cols = in.col + r0 * K;
+    const int width = (int)min((long)COLS, V - c0);
     int mine = 0;
-    for (int q = threadIdx.x; q < total; q += 256) {
-      const long d = in.col[r0 * K + q] - c0;
-      mine += d >= 0 && d < COLS && d + c0 < V;
-    }
+#pragma unroll 4
+    for (int q = threadIdx.x; q < total; q += 256) mine += (unsigned)(__ldg(cols + q) - (int)c0) < (unsigned)width;
     // exclusive prefix over the threads
     int pre = mine;
 #pragma unroll
@@ -406,10 +407,10 @@ __global__ void __launch_bounds__(256)
     }
     if (mine) {
       for (int q = threadIdx.x; q < total; q += 256) {
-        const long d = in.col[r0 * K + q] - c0;
-        if (d >= 0 && d < COLS && d + c0 < V) {
+        const unsigned d = (unsigned)(__ldg(cols + q) - (int)c0);
+        if (d < (unsigned)width) {
           const int row = q / K;
-          hit_at[at] = (uint32_t)row << 16 | (uint32_t)d;
+          hit_at[at] = (uint32_t)row << 16 | d;
           hit_v[at] = in.val[r0 * K + q];
           atomicOr(&mask[row * (COLS / 32) + (int)(d >> 5)], 1u << (d & 31));
           at++;
@@ -419,76 +420,80 @@ __global__ void __launch_bounds__(256)
     __syncthreads();
 #pragma unroll 2
     for (int q = warp; q < nr; q += 8) {
-      const long i = r0 + q;
-      const float2 f = in.info[i];  // (lse2, scale)
+      const float2 f = __ldg(in.info + r0 + q);  // (lse2, scale)
+      uint4* at4 = reinterpret_cast<uint4*>(base + q * ld);
+      const float2* sr = stat + (r0 + q) * ld_stat;
       uint4 raw[NS];
       float m[NS];
 #pragma unroll
-      for (int s = 0; s < NS; s++) {
-        const long c = c0 + 256 * s + lane * 8;
-        if (c < V) {  // V's pad up to a multiple of 8 lies inside ld
-          raw[s] = *reinterpret_cast<const uint4*>(base + i * ld + c);
-          m[s] = stat[i * ld_stat + (c >> seg_shift)].x;
+      for (int s = 0; s < NS; s++)
+        if (256 * s < left) {  // V's pad up to a multiple of 8 lies inside ld
+          raw[s] = at4[32 * s];
+          m[s] = __ldg(&sr[(int)(c0 + 256 * s + lane * 8) >> seg_shift].x);
         }
-      }
 #pragma unroll
       for (int s = 0; s < NS; s++) {
-        const long c = c0 + 256 * s + lane * 8;
-        if (c >= V) continue;
+        if (256 * s >= left) continue;
         const uint32_t bits = mask[q * (COLS / 32) + 8 * s + (lane >> 2)] >> (8 * (lane & 3)) & 0xffu;
-        const float k = m[s] == -INFINITY ? 0.f : exp2f(m[s] - f.x - 15.f) * f.y;
+        const float k = m[s] == -INFINITY ? 0.f : ex2(m[s] - f.x - 15.f) * f.y;
+        const float2 k2 = make_float2(k, k);
         const __half2* h = reinterpret_cast<const __half2*>(&raw[s]);
-        float v[8];
+        float2 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float2 t = __half22float2(h[j]);
-          v[2 * j] = t.x * k;
-          v[2 * j + 1] = t.y * k;
-        }
+        for (int j = 0; j < 4; j++) v[j] = __fmul2_rn(__half22float2(h[j]), k2);
         if (f.y == 0.f || bits) {  // a row that does not count; columns whose values are listed
 #pragma unroll
-          for (int j = 0; j < 8; j++)
-            if (f.y == 0.f || (bits >> j & 1u)) v[j] = 0.f;
+          for (int j = 0; j < 4; j++) {
+            if (f.y == 0.f || (bits >> (2 * j) & 1u)) v[j].x = 0.f;
+            if (f.y == 0.f || (bits >> (2 * j + 1) & 1u)) v[j].y = 0.f;
+          }
         }
         uint4 o;
         uint32_t* u = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          const __nv_bfloat162 b = __float22bfloat162_rn(v[j]);
           u[j] = *reinterpret_cast<const uint32_t*>(&b);
+          if (PART) sum[s][j] = __fadd2_rn(sum[s][j], v[j]);
         }
-        *reinterpret_cast<uint4*>(base + i * ld + c) = o;
-#pragma unroll
-        for (int j = 0; j < 8; j++) sum[s][j] += v[j];
+        at4[32 * s] = o;
       }
     }
   }
-  for (long i = r0 + nr + warp; i < min(r0 + rpb, (have + 63) / 64 * 64); i += 8)
+  for (long q = nr + warp; q < min((long)rpb, (have + 63) / 64 * 64 - r0); q += 8)
 #pragma unroll
-    for (int s = 0; s < NS; s++) {
-      const long c = c0 + 256 * s + lane * 8;
-      if (c < V) *reinterpret_cast<uint4*>(base + i * ld + c) = make_uint4(0u, 0u, 0u, 0u);
-    }
-  if (part) {
+    for (int s = 0; s < NS; s++)
+      if (256 * s < left) reinterpret_cast<uint4*>(base + q * ld)[32 * s] = make_uint4(0u, 0u, 0u, 0u);
+  if (PART) {
 #pragma unroll
     for (int s = 0; s < NS; s++)
 #pragma unroll
-      for (int j = 0; j < 8; j += 4)
-        *reinterpret_cast<float4*>(fold + warp * COLS + 256 * s + lane * 8 + j) =
-            make_float4(sum[s][j], sum[s][j + 1], sum[s][j + 2], sum[s][j + 3]);
+      for (int j = 0; j < 4; j += 2)
+        *reinterpret_cast<float4*>(fold + warp * COLS + 256 * s + lane * 8 + 2 * j) =
+            make_float4(sum[s][j].x, sum[s][j].y, sum[s][j + 1].x, sum[s][j + 1].y);
   }
   __syncthreads();
+  uint16_t* tile = reinterpret_cast<uint16_t*>(terms) + r0 * ld + c0;
   for (int h = threadIdx.x; h < hits; h += 256)
-    base[(r0 + (hit_at[h] >> 16)) * ld + c0 + (hit_at[h] & 0xffffu)] =
-        __bfloat16_as_ushort(__float2bfloat16_rn(hit_v[h]));
-  if (!part) return;
-  for (int c = threadIdx.x; c < COLS && c0 + c < V; c += 256) {
+    tile[(hit_at[h] >> 16) * ld + (hit_at[h] & 0xffffu)] = __bfloat16_as_ushort(__float2bfloat16_rn(hit_v[h]));
+  if (!PART) return;
+  // thread t owns the block's columns t, t + 256, ...
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+    const int c = 256 * s + threadIdx.x;
     float t = fold[c];
 #pragma unroll
     for (int q = 1; q < 8; q++) t += fold[q * COLS + c];
-    for (int h = 0; h < hits; h++)
-      if ((hit_at[h] & 0xffffu) == (uint32_t)c) t += hit_v[h];
-    part[(long)blockIdx.y * V + c0 + c] = t;
+    fold[c] = t;
+  }
+  for (int h = 0; h < hits; h++) {
+    const uint32_t c = hit_at[h] & 0xffffu;
+    if ((c & 255u) == threadIdx.x) fold[c] += hit_v[h];
+  }
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+    const int c = 256 * s + threadIdx.x;
+    if (c0 + c < V) part[(long)blockIdx.y * V + c0 + c] = fold[c];
   }
 }
 
@@ -736,13 +741,13 @@ struct VocabCall {
 
 static bool rows16(const void* p, size_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 
-template <int NS>
+template <int NS, bool PART>
 static int dz_launch(const VocabPlan& p, uint8_t* ws, long V, long K, const int* count, long off, long n, RowOut ro,
                      float* part, cudaStream_t st) {
-  const size_t smem = DzSmem<NS>::bytes(p.rpb, K, part != nullptr);
+  const size_t smem = DzSmem<NS>::bytes(p.rpb, K, PART);
   if (smem > 48 * 1024)
-    PL_CUDA(cudaFuncSetAttribute(vocab_dz_kernel<NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  vocab_dz_kernel<NS><<<dim3((unsigned)ceil_div(V, 256 * NS), (unsigned)(round_up(n, 64) / p.rpb)), 256, smem, st>>>(
+    PL_CUDA(cudaFuncSetAttribute(vocab_dz_kernel<NS, PART>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  vocab_dz_kernel<NS, PART><<<dim3((unsigned)ceil_div(V, 256 * NS), (unsigned)(round_up(n, 64) / p.rpb)), 256, smem, st>>>(
       ws + p.terms, p.ldt, V, (int)K, count, off, n, p.rpb, ro, (const float2*)(ws + p.stat), p.ld_stat,
       p.bn == 256 ? 7 : 6, part);
   count_launch();
@@ -868,8 +873,9 @@ static int vocab_run(const VocabCall& c) {
     if (!c.grad) continue;
     const bool last = q == p.pieces - 1;
     float* part = bias ? (float*)(ws + p.part) : nullptr;
-    rc = p.ns == 4 ? dz_launch<4>(p, ws, V, k1, count, off, n, ro, part, st)
-                   : dz_launch<1>(p, ws, V, k1, count, off, n, ro, part, st);
+    const auto dz = p.ns == 4 ? (bias ? dz_launch<4, true> : dz_launch<4, false>)
+                              : (bias ? dz_launch<1, true> : dz_launch<1, false>);
+    rc = dz(p, ws, V, k1, count, off, n, ro, part, st);
     if (rc) return rc;
     if (bias) {
       vocab_dbias_kernel<<<(unsigned)ceil_div(V, 256), 256, 0, st>>>(part, (int)(round_up(n, 64) / p.rpb), V,

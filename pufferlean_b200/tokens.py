@@ -20,6 +20,7 @@ import torch
 from . import PufferError, _check, lib
 
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+_NORM_TYPES = (_F32, _BF16)
 
 
 def _need(ok, what, msg, *args):
@@ -29,94 +30,99 @@ def _need(ok, what, msg, *args):
 
 def _matrix(t, what, name, dtypes, device=None):
     """Checks a 2-D tensor of contiguous rows on the GPU; returns its row stride in elements."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.dim() == 2 and (
+            device is None or t.device == device):
+        rows, cols = t.shape
+        st, sc = t.stride()
+        if sc == 1 and st >= cols:
+            return st
+        if cols <= 1 and rows <= 1:
+            return 1
+        if cols == 1 and st >= 1:  # a stride over one value says nothing
+            return st
+        if rows <= 1 and sc == 1:
+            return cols
+        raise PufferError(f"{what}: {name} must have contiguous rows that do not overlap (shape {(rows, cols)}, strides "
+                          f"{(st, sc)})")
     _need(isinstance(t, torch.Tensor) and t.is_cuda, what, "%s must be a CUDA tensor", name)
     _need(t.dim() == 2, what, "%s must have two dimensions, has %d", name, t.dim())
     _need(t.dtype in dtypes, what, "%s has type %s", name, t.dtype)
-    _need(device is None or t.device == device, what, "%s is on %s, not on %s", name, t.device, device)
-    rows, cols = t.shape
-    st, sc = t.stride()
-    _need(cols <= 1 or sc == 1, what, "%s: the values of a row must be contiguous (stride %d)", name, sc)
-    if rows <= 1:
-        return max(cols, st) if st >= cols else cols
-    _need(st >= cols, what, "%s: row stride %d below %d columns", name, st, cols)
-    return st
+    raise PufferError(f"{what}: {name} is on {t.device}, not on {device}")
 
 
 def _vector(t, what, name, dtype, shape, device):
-    """Checks a contiguous tensor of this type and shape (or None); returns its address."""
-    if t is None:
-        return None
+    """Checks a contiguous tensor of this type and shape; returns its address."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous():
+        return t.data_ptr()
     _need(isinstance(t, torch.Tensor) and t.device == device, what, "%s must be a tensor on %s", name, device)
     _need(t.dtype == dtype, what, "%s has type %s, not %s", name, t.dtype, dtype)
     _need(tuple(t.shape) == tuple(shape), what, "%s has shape %s, not %s", name, tuple(t.shape), tuple(shape))
-    _need(t.is_contiguous(), what, "%s must be contiguous", name)
-    return t.data_ptr()
+    raise PufferError(f"{what}: {name} must be contiguous")
 
 
-class _On:
-    """Makes a tensor's device current for torch and for the library, and names its current stream."""
+def _enter(device):
+    """Makes a tensor's device the library's for this call; returns (torch's device to go back to or None, the stream
+    torch is on there). The checks above and this run on every call: a small call costs little more than they do."""
+    index = device.index
+    was = torch.cuda.current_device()
+    lib().pl_set_device(index)
+    return (None if was == index else was), torch._C._cuda_getCurrentRawStream(index)
 
-    __slots__ = ("guard", "index")
 
-    def __init__(self, device):
-        self.index = device.index
-        self.guard = None if self.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        _check(lib().pl_set_device(self.index), "pl_set_device")
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-            lib().pl_set_device(torch.cuda.current_device())
-        return False
+def _leave(was):
+    if was is not None:
+        lib().pl_set_device(was)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(y, mean, rstd) of the rows of x [rows, cols] (f32 or bf16); weight and bias [cols] f32 or None, mean and rstd
     [rows] f32 (what layer_norm_grad takes)."""
     what = "layer_norm"
-    ldx = _matrix(x, what, "x", (_F32, _BF16))
+    ldx = _matrix(x, what, "x", _NORM_TYPES)
     rows, cols = x.shape
-    wp = _vector(weight, what, "weight", _F32, (cols,), x.device)
-    bp = _vector(bias, what, "bias", _F32, (cols,), x.device)
-    with _On(x.device) as st:
-        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-        stats = torch.empty((2, rows), dtype=_F32, device=x.device)
-        at = stats.data_ptr()
-        _check(lib().pl_layernorm_dev(x.data_ptr(), ldx, wp, bp, rows, cols, eps, x.dtype == _BF16, y.data_ptr(), cols,
-                                      at, at + 4 * rows, st), "pl_layernorm_dev")
-    return y, stats[0], stats[1]
+    dev, dtype = x.device, x.dtype
+    wp = None if weight is None else _vector(weight, what, "weight", _F32, (cols,), dev)
+    bp = None if bias is None else _vector(bias, what, "bias", _F32, (cols,), dev)
+    y = torch.empty((rows, cols), dtype=dtype, device=dev)
+    mean = torch.empty(rows, dtype=_F32, device=dev)
+    rstd = torch.empty(rows, dtype=_F32, device=dev)
+    was, st = _enter(dev)
+    rc = lib().pl_layernorm_dev(x.data_ptr(), ldx, wp, bp, rows, cols, eps, dtype is _BF16, y.data_ptr(), cols,
+                                mean.data_ptr(), rstd.data_ptr(), st)
+    _leave(was)
+    if rc:
+        _check(rc, what)
+    return y, mean, rstd
 
 
 def layer_norm_grad(dy, x, weight, mean, rstd, params=True):
     """(dx, dweight, dbias) of layer_norm: dx in x's type, dweight and dbias [cols] f32 (None with params=False)."""
     what = "layer_norm_grad"
-    ldx = _matrix(x, what, "x", (_F32, _BF16))
+    ldx = _matrix(x, what, "x", _NORM_TYPES)
     rows, cols = x.shape
-    lddy = _matrix(dy, what, "dy", (x.dtype,), x.device)
+    dev, dtype = x.device, x.dtype
+    lddy = _matrix(dy, what, "dy", (dtype,), dev)
     _need(dy.shape == x.shape, what, "dy has shape %s, not %s", tuple(dy.shape), tuple(x.shape))
-    wp = _vector(weight, what, "weight", _F32, (cols,), x.device)
-    mp = _vector(mean, what, "mean", _F32, (rows,), x.device)
-    rp = _vector(rstd, what, "rstd", _F32, (rows,), x.device)
-    _need(mp is not None and rp is not None, what, "mean and rstd are needed")
-    with _On(x.device) as st:
-        L = lib()
-        dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-        dp = ws = None
-        size = 0
-        if params:
-            dp = torch.empty((2, cols), dtype=_F32, device=x.device)
-            size = L.pl_layernorm_grad_ws(rows, cols)
-            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-        _check(L.pl_layernorm_grad_dev(dy.data_ptr(), lddy, x.data_ptr(), ldx, wp, mp, rp, rows, cols, x.dtype == _BF16,
-                                       dx.data_ptr(), cols, dp[0].data_ptr() if params else None,
-                                       dp[1].data_ptr() if params else None, ws.data_ptr() if params else None, size,
-                                       st), "pl_layernorm_grad_dev")
-    return (dx, dp[0], dp[1]) if params else (dx, None, None)
+    wp = None if weight is None else _vector(weight, what, "weight", _F32, (cols,), dev)
+    _need(mean is not None and rstd is not None, what, "mean and rstd are needed")
+    mp = _vector(mean, what, "mean", _F32, (rows,), dev)
+    rp = _vector(rstd, what, "rstd", _F32, (rows,), dev)
+    dx = torch.empty((rows, cols), dtype=dtype, device=dev)
+    dw = db = dwp = dbp = wsp = None
+    size = 0
+    if params:
+        dw = torch.empty(cols, dtype=_F32, device=dev)
+        db = torch.empty(cols, dtype=_F32, device=dev)
+        size = lib().pl_layernorm_grad_ws(rows, cols)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        dwp, dbp, wsp = dw.data_ptr(), db.data_ptr(), ws.data_ptr()
+    was, st = _enter(dev)
+    rc = lib().pl_layernorm_grad_dev(dy.data_ptr(), lddy, x.data_ptr(), ldx, wp, mp, rp, rows, cols, dtype is _BF16,
+                                     dx.data_ptr(), cols, dwp, dbp, wsp, size, st)
+    _leave(was)
+    if rc:
+        _check(rc, what)
+    return dx, dw, db
 
 
 def _head(what, x, w, bias, ids, teacher, temperature, row_scale, grad, dw_f32=False, piece_bytes=0):
@@ -127,7 +133,7 @@ def _head(what, x, w, bias, ids, teacher, temperature, row_scale, grad, dw_f32=F
     v = w.shape[0]
     _need(w.shape[1] == d, what, "w has %d columns, x has %d", w.shape[1], d)
     _need(v > 0 and d > 0, what, "w has shape %s", tuple(w.shape))
-    bp = _vector(bias, what, "bias", _BF16, (v,), dev)
+    bp = None if bias is None else _vector(bias, what, "bias", _BF16, (v,), dev)
     distill = teacher is not None
     if distill:
         _need(isinstance(ids, torch.Tensor) and ids.dim() == 2 and ids.shape[1] > 0, what,
@@ -140,33 +146,36 @@ def _head(what, x, w, bias, ids, teacher, temperature, row_scale, grad, dw_f32=F
         k = 0
         _need(ids is not None, what, "target is needed")
         ip = _vector(ids, what, "target", _I32, (n,), dev)
-    sp = _vector(row_scale, what, "row_scale", _F32, (n,), dev)
-    with _On(dev) as st:
-        L = lib()
-        aligned = ldx % 8 == 0 and ldw % 8 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0
-        size = L.pl_vocab_ws(n, v, d, k, bias is not None, grad, aligned, piece_bytes)
-        out = torch.empty((2, n), dtype=_F32, device=dev)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        lp, wsp = out.data_ptr(), ws.data_ptr()
-        if not grad:
-            if distill:
-                rc = L.pl_vocab_distill_dev(x.data_ptr(), ldx, w.data_ptr(), ldw, bp, ip, tp, k, temperature, n, v, d, lp,
-                                            lp + 4 * n, wsp, size, st)
-            else:
-                rc = L.pl_vocab_ce_dev(x.data_ptr(), ldx, w.data_ptr(), ldw, bp, ip, n, v, d, lp, lp + 4 * n, wsp, size, st)
-            _check(rc, what)
-            return out[0], out[1]
+    sp = None if row_scale is None else _vector(row_scale, what, "row_scale", _F32, (n,), dev)
+    L = lib()
+    aligned = ldx % 8 == 0 and ldw % 8 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0
+    loss = torch.empty(n, dtype=_F32, device=dev)
+    lse = torch.empty(n, dtype=_F32, device=dev)
+    dx = dw = db = None
+    if grad:
         dx = torch.empty((n, d), dtype=_BF16, device=dev)
         dw = torch.empty((v, d), dtype=_F32 if dw_f32 else _BF16, device=dev)
         db = torch.empty(v, dtype=dw.dtype, device=dev) if bias is not None else None
-        tail = (sp, n, v, d, lp, lp + 4 * n, dx.data_ptr(), d, dw.data_ptr(), d, None if db is None else db.data_ptr(),
-                dw_f32, piece_bytes, wsp, size, st)
+    size = L.pl_vocab_ws(n, v, d, k, bias is not None, grad, aligned, piece_bytes)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    head = (x.data_ptr(), ldx, w.data_ptr(), ldw, bp, ip)
+    tail = (n, v, d, loss.data_ptr(), lse.data_ptr())
+    room = (ws.data_ptr(), size)
+    was, st = _enter(dev)
+    if grad:
+        tail = (sp, *tail, dx.data_ptr(), d, dw.data_ptr(), d, None if db is None else db.data_ptr(), dw_f32, piece_bytes)
         if distill:
-            rc = L.pl_vocab_distill_grad_dev(x.data_ptr(), ldx, w.data_ptr(), ldw, bp, ip, tp, k, temperature, *tail)
+            rc = L.pl_vocab_distill_grad_dev(*head, tp, k, temperature, *tail, *room, st)
         else:
-            rc = L.pl_vocab_ce_grad_dev(x.data_ptr(), ldx, w.data_ptr(), ldw, bp, ip, *tail)
+            rc = L.pl_vocab_ce_grad_dev(*head, *tail, *room, st)
+    elif distill:
+        rc = L.pl_vocab_distill_dev(*head, tp, k, temperature, *tail, *room, st)
+    else:
+        rc = L.pl_vocab_ce_dev(*head, *tail, *room, st)
+    _leave(was)
+    if rc:
         _check(rc, what)
-    return out[0], out[1], dx, dw, db
+    return (loss, lse, dx, dw, db) if grad else (loss, lse)
 
 
 def vocab_ce(x, w, target, bias=None):
