@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(128)
 // it. With `part` the column sums of the unrounded values go to part[row tile][V] for dbias. Rows from the count to
 // the next multiple of 64 are zeroed (the weight-gradient product reads whole k-blocks of rows).
 // Bound by HBM: 4 bytes per term.
+constexpr int kDzScan = 16;  // answer entries of a block: 256 kDzScan at most
 template <int NS>
 struct DzSmem {
   static constexpr int COLS = 256 * NS;
@@ -375,11 +376,11 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint16_t* base = reinterpret_cast<uint16_t*>(terms) + r0 * ld + c0 + lane * 8;
   const int left = (int)min((long)COLS, V - c0) - lane * 8;  // columns from this lane's first on
-  float2 sum[NS][4];
+  float sum[NS][8];
 #pragma unroll
   for (int s = 0; s < NS; s++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) sum[s][j] = make_float2(0.f, 0.f);
+    for (int j = 0; j < 8; j++) sum[s][j] = 0.f;
   int hits = 0;
   const int nr = (int)max(0L, min((long)rpb, have - r0));
   if (nr > 0) {
@@ -387,9 +388,22 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
     const int total = nr * K;
     const int* cols = in.col + r0 * K;
     const int width = (int)min((long)COLS, V - c0);
-    int mine = 0;
-#pragma unroll 4
-    for (int q = threadIdx.x; q < total; q += 256) mine += (unsigned)(__ldg(cols + q) - (int)c0) < (unsigned)width;
+    uint32_t found = 0;  // bit 4 i + j: entry 4 (threadIdx.x + 256 i) + j lies in the tile
+    int4 e[kDzScan / 4];
+#pragma unroll
+    for (int i = 0; i < kDzScan / 4; i++) {
+      const int q = 4 * (threadIdx.x + 256 * i);
+      if (q < total) e[i] = __ldg(reinterpret_cast<const int4*>(cols + q));  // the list's rows go on past `total`
+    }
+#pragma unroll
+    for (int i = 0; i < kDzScan / 4; i++) {
+      const int q = 4 * (threadIdx.x + 256 * i);
+      if (q < total && (unsigned)(e[i].x - (int)c0) < (unsigned)width) found |= 1u << (4 * i);
+      if (q + 1 < total && (unsigned)(e[i].y - (int)c0) < (unsigned)width) found |= 2u << (4 * i);
+      if (q + 2 < total && (unsigned)(e[i].z - (int)c0) < (unsigned)width) found |= 4u << (4 * i);
+      if (q + 3 < total && (unsigned)(e[i].w - (int)c0) < (unsigned)width) found |= 8u << (4 * i);
+    }
+    const int mine = __popc(found);
     // exclusive prefix over the threads
     int pre = mine;
 #pragma unroll
@@ -405,17 +419,16 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
       if (q < warp) at += warp_n[q];
       hits += warp_n[q];
     }
-    if (mine) {
-      for (int q = threadIdx.x; q < total; q += 256) {
-        const unsigned d = (unsigned)(__ldg(cols + q) - (int)c0);
-        if (d < (unsigned)width) {
-          const int row = q / K;
-          hit_at[at] = (uint32_t)row << 16 | d;
-          hit_v[at] = in.val[r0 * K + q];
-          atomicOr(&mask[row * (COLS / 32) + (int)(d >> 5)], 1u << (d & 31));
-          at++;
-        }
-      }
+    for (; found; found &= found - 1) {
+      const int i = __ffs(found) - 1;
+      hit_at[at++] = 4 * (threadIdx.x + 256 * (i >> 2)) + (i & 3);
+    }
+    __syncthreads();
+    for (int h = threadIdx.x; h < hits; h += 256) {
+      const uint32_t q = hit_at[h], row = q / (uint32_t)K, d = __ldg(cols + q) - (int)c0;
+      hit_at[h] = row << 16 | d;
+      hit_v[h] = in.val[r0 * K + q];
+      atomicOr(&mask[row * (COLS / 32) + (d >> 5)], 1u << (d & 31));
     }
     __syncthreads();
 #pragma unroll 2
@@ -435,26 +448,28 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
       for (int s = 0; s < NS; s++) {
         if (256 * s >= left) continue;
         const uint32_t bits = mask[q * (COLS / 32) + 8 * s + (lane >> 2)] >> (8 * (lane & 3)) & 0xffu;
-        const float k = m[s] == -INFINITY ? 0.f : ex2(m[s] - f.x - 15.f) * f.y;
+        if (__any_sync(__activemask(), bits)) {  // rare: columns whose values are listed
+          uint32_t* t = reinterpret_cast<uint32_t*>(&raw[s]);
+#pragma unroll
+          for (int j = 0; j < 4; j++) t[j] &= ~((bits >> (2 * j) & 1u) * 0xffffu | (bits >> (2 * j + 1) & 1u) * 0xffff0000u);
+        }
+        // a row that does not count has scale 0 (its x is zero, so its terms are finite)
+        const float k = m[s] == -INFINITY || f.y == 0.f ? 0.f : ex2(m[s] - f.x - 15.f) * f.y;
         const float2 k2 = make_float2(k, k);
         const __half2* h = reinterpret_cast<const __half2*>(&raw[s]);
         float2 v[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = __fmul2_rn(__half22float2(h[j]), k2);
-        if (f.y == 0.f || bits) {  // a row that does not count; columns whose values are listed
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            if (f.y == 0.f || (bits >> (2 * j) & 1u)) v[j].x = 0.f;
-            if (f.y == 0.f || (bits >> (2 * j + 1) & 1u)) v[j].y = 0.f;
-          }
-        }
         uint4 o;
         uint32_t* u = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const __nv_bfloat162 b = __float22bfloat162_rn(v[j]);
           u[j] = *reinterpret_cast<const uint32_t*>(&b);
-          if (PART) sum[s][j] = __fadd2_rn(sum[s][j], v[j]);
+          if (PART) {
+            sum[s][2 * j] += v[j].x;
+            sum[s][2 * j + 1] += v[j].y;
+          }
         }
         at4[32 * s] = o;
       }
@@ -468,9 +483,9 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
 #pragma unroll
     for (int s = 0; s < NS; s++)
 #pragma unroll
-      for (int j = 0; j < 4; j += 2)
-        *reinterpret_cast<float4*>(fold + warp * COLS + 256 * s + lane * 8 + 2 * j) =
-            make_float4(sum[s][j].x, sum[s][j].y, sum[s][j + 1].x, sum[s][j + 1].y);
+      for (int j = 0; j < 8; j += 4)
+        *reinterpret_cast<float4*>(fold + warp * COLS + 256 * s + lane * 8 + j) =
+            make_float4(sum[s][j], sum[s][j + 1], sum[s][j + 2], sum[s][j + 3]);
   }
   __syncthreads();
   uint16_t* tile = reinterpret_cast<uint16_t*>(terms) + r0 * ld + c0;
@@ -486,10 +501,19 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
     for (int q = 1; q < 8; q++) t += fold[q * COLS + c];
     fold[c] = t;
   }
-  for (int h = 0; h < hits; h++) {
+  __syncthreads();
+  for (int h = threadIdx.x; h < hits; h += 256) {  // the first listed value of a column adds all of that column's
     const uint32_t c = hit_at[h] & 0xffffu;
-    if ((c & 255u) == threadIdx.x) fold[c] += hit_v[h];
+    float t = 0.f;
+    bool first = true;
+    for (int g = 0; g < hits; g++) {
+      const bool same = (hit_at[g] & 0xffffu) == c;
+      first = first && !(same && g < h);
+      t += same ? hit_v[g] : 0.f;
+    }
+    if (first) fold[c] += t;
   }
+  __syncthreads();
 #pragma unroll
   for (int s = 0; s < NS; s++) {
     const int c = 256 * s + threadIdx.x;
@@ -676,7 +700,7 @@ static VocabPlan vocab_plan(long N, long V, long D, long K, bool bias, bool grad
   p.ns = ceil_div(V, 1024) * ceil_div(N, 64) >= 2 * sms ? 4 : 1;
   p.rpb = 64;
   const long cols = 256L * p.ns;
-  while (p.rpb > 8 && (p.rpb * k1 > 4096 || ceil_div(V, cols) * ceil_div(N, p.rpb) < 2 * sms ||
+  while (p.rpb > 8 && (p.rpb * k1 > 256 * kDzScan || ceil_div(V, cols) * ceil_div(N, p.rpb) < 2 * sms ||
                        (double)p.rpb * k1 * (V < cols ? 1.0 : (double)cols / V) > 512.0))
     p.rpb /= 2;
   size_t at = 0;
