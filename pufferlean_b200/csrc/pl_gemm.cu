@@ -91,6 +91,18 @@ int gemm_sms() {
   return (dev >= 0 && dev < 64 && num_sms[dev] > 0) ? num_sms[dev] : 148;
 }
 
+// Mode 2's products for CTA pairs: both operands MN-major; the large-vocabulary head's logits and sliced products,
+// where an odd number of 128-row tiles (half a pair idle on the last) costs at most an eighth: 300 rows of logits over
+// 65,536 x 1,024 took 72 us on single CTAs and 80 on pairs, 4,096 rows 445 and 369.
+bool gemm_paired(int bn, int epi, bool a_mn, bool b_mn, int M) {
+  uint32_t smem;
+  const long tiles = ceil_div(M, 128);
+  const bool want = g_pair_mode == 1 ||
+                    (g_pair_mode == 2 && ((a_mn && b_mn) || ((epi == EPI_VOCAB || epi == EPI_SLICE) &&
+                                                             (tiles % 2 == 0 || tiles > 8))));
+  return want && bn == 256 && epi != EPI_PPO && M > 128 && gemm_pair_instance(bn, epi, a_mn, b_mn, &smem) != nullptr;
+}
+
 int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const Operand& B, int M, int N, int K,
                 int batch, const EpiArgs& ep_in, cudaStream_t st) {
   const int bn_in = bn;
@@ -102,8 +114,8 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
              "GEMM B storage %ldx%ld too small for N=%d K=%d", B.rows, B.cols, N, K);
   uint32_t smem = 0;
   GemmKernel k = nullptr;
-  const bool pair = (g_pair_mode == 1 || (g_pair_mode == 2 && a_mn && b_mn)) && bn == 256 && epi != EPI_PPO && epi != EPI_SLICE && M > 128 &&
-                    (k = gemm_pair_instance(bn, epi, a_mn, b_mn, &smem)) != nullptr;
+  const bool pair = gemm_paired(bn, epi, a_mn, b_mn, M);
+  if (pair) k = gemm_pair_instance(bn, epi, a_mn, b_mn, &smem);
   // the data gradient of a short-K product (the head's, K <= 128) is a memory-bound epilogue: 128-wide
   // tiles whose aux comes through TMA into shared memory (needs the staged stores, checked below)
   bool at = false;
@@ -166,7 +178,7 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
   if (pair) {
     // one cluster of two CTAs per pair tile of 256 rows, at most one CTA per SM
     const long ptiles = ceil_div(N, bn) * ceil_div(M, 256) * (long)(splits > 1 ? splits : batch);
-    const long pairs = ptiles < sms / 2 ? ptiles : sms / 2;
+    const long pairs = ptiles < sms / 2 && epi != EPI_SLICE ? ptiles : sms / 2;
     grid = dim3((unsigned)(2 * pairs), 1, 1);
   } else {
     const long tiles = ceil_div(N, bn) * ceil_div(M, 128) * (long)(splits > 1 ? splits : batch);

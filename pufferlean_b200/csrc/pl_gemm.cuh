@@ -31,20 +31,20 @@ enum EpiKind : int {
   EPI_SLICE = 6,  // out(f32) = acc; the tiles of an incomplete last wave are split along K (SliceShape)
 };
 
-// EPI_SLICE: tiles go to the CTAs in whole waves; the `rem` tiles of the last, incomplete one are cut along K into q
+// EPI_SLICE: tiles go to the `grid` CTAs (or CTA pairs) in whole waves; the `rem` tiles of the last, incomplete one are cut along K into q
 // slices each, as many as keep every CTA busy, and the CTAs of one slice walk the same k-blocks at the same time (so
 // they still share what they read of the operands through L2; dealing the k-blocks out in one line, every CTA at
 // another place of the long axis, made the product of 4,096 x 1,024 x 65,537 take 520 instead of 396 us). Slices go
-// to slabs of [128][BN] f32, slice z of the i-th of these tiles to slab z rem + i, and whoever reads the result adds
+// to slabs of [bm][bn] f32, slice z of the i-th of these tiles to slab z rem + i, and whoever reads the result adds
 // them in order (slice_sum8). The extents may be known on the device only, so the shape is worked out there.
 struct SliceShape {
   int num_n, num_m, kb, rem, q;
   long full;  // tiles of the whole waves
 };
-__host__ __device__ inline SliceShape slice_shape(int M, int N, int K, int bn, int grid) {
+__host__ __device__ inline SliceShape slice_shape(int M, int N, int K, int bm, int bn, int grid) {
   SliceShape s;
   s.num_n = (N + bn - 1) / bn;
-  s.num_m = (M + 127) / 128;
+  s.num_m = (M + bm - 1) / bm;
   s.kb = (K + 63) / 64;
   const long tiles = (long)s.num_n * s.num_m;
   s.full = tiles / grid * grid;
@@ -102,7 +102,7 @@ struct EpiArgs {
   const int* target;
   const int* row_ids;
   float* ut;
-  float* slabs;  // EPI_SLICE: [gridDim.x][128][BN]
+  float* slabs;  // EPI_SLICE: [gridDim.x * 128][BN]
   // EPI_F32, optional: out += alpha*acc instead of out = alpha*acc
   int accum;
   // Rows that exist (optional): the extent M (dyn_k = 0) or K (dyn_k = 1) of this call is
@@ -359,15 +359,15 @@ __device__ __forceinline__ TileIdx tile_of(int t, int num_n, int num_m) {
 }
 
 // Order of the head's logit tiles (EPI_VOCAB): the weight matrix is the large operand, so m is the fast
-// index inside groups of 32 row tiles: the CTAs that run at one time share a few column panels of the
-// weights (read once from HBM per group) and the group's 4,096 rows stay in L2.
-constexpr int kVocabGroupM = 32;
-template <int EPI>
+// index inside groups of 4,096 rows: the CTAs that run at one time share a few column panels of the
+// weights (read once from HBM per group) and the group's rows stay in L2.
+constexpr int kVocabGroupRows = 4096;
+template <int EPI, int GROUP>
 __device__ __forceinline__ TileIdx tile_at(int t, int num_n, int num_m) {
   if constexpr (EPI == EPI_VOCAB) {
-    const int g = t / (kVocabGroupM * num_n), first = g * kVocabGroupM;
-    const int gm = min(kVocabGroupM, num_m - first);
-    const int q = t - g * (kVocabGroupM * num_n);
+    const int g = t / (GROUP * num_n), first = g * GROUP;
+    const int gm = min(GROUP, num_m - first);
+    const int q = t - g * (GROUP * num_n);
     TileIdx r;
     r.n = q / gm;
     r.m = first + q - r.n * gm;
@@ -378,18 +378,18 @@ __device__ __forceinline__ TileIdx tile_at(int t, int num_n, int num_m) {
   }
 }
 
-// The tiles (and their ranges of k-blocks) that a CTA works on, in order: every gridDim.x-th tile, whole or one
-// split-K slice of it; with EPI_SLICE the whole waves and then one slice of the rest.
-template <int EPI>
+// The tiles (of BM rows, and their ranges of k-blocks) that a CTA or pair works on, in order: every step-th tile,
+// whole or one split-K slice of it; with EPI_SLICE the whole waves and then one slice of the rest.
+template <int EPI, int BM>
 struct TileWalk {
   int num_n, num_m, kb, per_split, k_splits;
-  long t, total;
+  long t, step, total;
   SliceShape s;
   long slab;  // EPI_SLICE: where the part goes (-1: out)
-  __device__ __forceinline__ TileWalk(int num_n_, int num_m_, int total_, int kb_, int per_split_, int k_splits_,
-                                      const SliceShape& s_)
-      : num_n(num_n_), num_m(num_m_), kb(kb_), per_split(per_split_), k_splits(k_splits_), t(blockIdx.x), total(total_),
-        s(s_), slab(-1) {}
+  __device__ __forceinline__ TileWalk(int first, int step_, int num_n_, int num_m_, int total_, int kb_, int per_split_,
+                                      int k_splits_, const SliceShape& s_)
+      : num_n(num_n_), num_m(num_m_), kb(kb_), per_split(per_split_), k_splits(k_splits_), t(first), step(step_),
+        total(total_), s(s_), slab(-1) {}
   __device__ __forceinline__ bool next(TileIdx& ti, int& b0, int& b1) {
     if constexpr (EPI == EPI_SLICE) {
       b0 = 0;
@@ -407,12 +407,12 @@ struct TileWalk {
           slab = i;
         }
       }
-      t += gridDim.x;
+      t += step;
       return true;
     } else {
       if (t >= total) return false;
-      ti = tile_at<EPI>((int)t, num_n, num_m);
-      t += gridDim.x;
+      ti = tile_at<EPI, kVocabGroupRows / BM>((int)t, num_n, num_m);
+      t += step;
       if (k_splits > 1) {
         b0 = ti.z * per_split;
         b1 = min(kb, b0 + per_split);
@@ -612,14 +612,14 @@ __device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, const VocabPre
         make_float2(top, ((sum[0] + sum[1]) + (sum[2] + sum[3])) * (1.f / 32768.f));
 }
 
-// EPI_SLICE: this warp's 32 rows x BN/2 columns to out, or to the slab of a slice; a lane writes its row in 32-byte
+// EPI_SLICE: this warp's 32 rows x BN/2 columns to out, or to the slabs from row slab_row on (>= 0); a lane writes its row in 32-byte
 // pieces (out's rows are padded to a multiple of 8 columns).
 template <int BN>
 __device__ __forceinline__ void epilogue_slice(const EpiArgs& ep, uint32_t t_row, int m_tile, int n_tile, int rows,
-                                               long slab, bool have_acc, int sub, int half, int lane) {
+                                               long slab_row, bool have_acc, int sub, int half, int lane) {
   const int row = m_tile * 128 + sub * 32 + lane, n0 = n_tile * BN;
-  float* at = slab < 0 ? reinterpret_cast<float*>(ep.out) + (long)row * ep.ldo + n0
-                       : ep.slabs + (slab * 128 + sub * 32 + lane) * BN;
+  float* at = slab_row < 0 ? reinterpret_cast<float*>(ep.out) + (long)row * ep.ldo + n0
+                           : ep.slabs + (slab_row + sub * 32 + lane) * BN;
 #pragma unroll
   for (int c = 0; c < BN / 2; c += 32) {
     const int c0 = half * (BN / 2) + c;
@@ -645,19 +645,19 @@ __device__ __forceinline__ void epilogue_slice(const EpiArgs& ep, uint32_t t_row
   }
 }
 
-// Eight values of row `row` at columns [col, col + 8) of a product that EPI_SLICE left in out and slabs (bn: its
-// column tile).
-__device__ __forceinline__ void slice_sum8(const SliceShape& s, const float* out, long ldo, const float* slabs, int bn,
-                                           long row, int col, float (&v)[8]) {
+// Eight values of row `row` at columns [col, col + 8) of a product that EPI_SLICE left in out and slabs (its tile
+// is bm x bn).
+__device__ __forceinline__ void slice_sum8(const SliceShape& s, const float* out, long ldo, const float* slabs, int bm,
+                                           int bn, long row, int col, float (&v)[8]) {
   const int nt = col / bn;
-  const long t = (row >> 7) * s.num_n + nt;
+  const long mt = row / bm, t = mt * s.num_n + nt;
   const bool whole = t < s.full || s.q == 1;
-  const float* p = whole ? out + row * ldo + col : slabs + ((t - s.full) * 128 + (row & 127)) * bn + (col - nt * bn);
+  const float* p = whole ? out + row * ldo + col : slabs + ((t - s.full) * bm + (row - mt * bm)) * bn + (col - nt * bn);
   const int parts = whole ? 1 : s.q;
 #pragma unroll
   for (int j = 0; j < 8; j++) v[j] = 0.f;
 #pragma unroll 4
-  for (int z = 0; z < parts; z++, p += (long)s.rem * 128 * bn) {
+  for (int z = 0; z < parts; z++, p += (long)s.rem * bm * bn) {
     const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
     v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
   }
@@ -1229,8 +1229,8 @@ __global__ void __launch_bounds__(320, 1)
   const uint32_t tmem_base = *tmem_slot;
 
   SliceShape shape{};
-  if constexpr (EPI == EPI_SLICE) shape = slice_shape(M, N, K, BN, gridDim.x);
-  TileWalk<EPI> walk(num_n, num_m, total_tiles, total_kb, per_split, ep.k_splits, shape);
+  if constexpr (EPI == EPI_SLICE) shape = slice_shape(M, N, K, BM, BN, gridDim.x);
+  TileWalk<EPI, BM> walk(blockIdx.x, gridDim.x, num_n, num_m, total_tiles, total_kb, per_split, ep.k_splits, shape);
   TileIdx ti;
   int b0, b1;
 
@@ -1349,7 +1349,7 @@ __global__ void __launch_bounds__(320, 1)
       tc::tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t)(buf * BN) + ((uint32_t)(sub * 32) << 16);
       if constexpr (EPI == EPI_SLICE)
-        epilogue_slice<BN>(ep, t_row, ti.m, ti.n, M, walk.slab, b1 > b0, sub, half, lane);
+        epilogue_slice<BN>(ep, t_row, ti.m, ti.n, M, walk.slab < 0 ? -1 : walk.slab * BM, b1 > b0, sub, half, lane);
       else if constexpr (EPI == EPI_VOCAB)
         epilogue_vocab<BN>(ep, pre, t_row, ti.m, ti.n, M, sub, half, lane, red + (warp - 2) * (BN / 2));
       else
@@ -1470,28 +1470,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
   tc::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  auto kb_range = [&](int z, int& b0, int& b1) {
-    if (ep.k_splits > 1) {
-      b0 = z * per_split;
-      b1 = min(total_kb, b0 + per_split);
-      if (b1 < b0) b1 = b0;
-    } else {
-      b0 = 0;
-      b1 = total_kb;
-    }
-  };
+  SliceShape shape{};
+  if constexpr (EPI == EPI_SLICE) shape = slice_shape(M, N, K, 2 * BM, BN, npairs);
+  TileWalk<EPI, 2 * BM> walk(pair, npairs, num_n, num_m, total_tiles, total_kb, per_split, ep.k_splits, shape);
+  TileIdx ti;
+  int b0, b1;
 
   if (warp == 0) {
     if (lane == 0) {
       // ---------------- TMA producer of this CTA's halves; the even CTA arms full[s] for both
       long it = 0;
-      for (int t = pair; t < total_tiles && !*abort_flag; t += npairs) {
-        const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
+      while (!*abort_flag && walk.next(ti, b0, b1)) {
         const int batch = ep.k_splits > 1 ? 0 : ti.z;
         const int arow = ti.m * 2 * BM + (int)rank * BM;
         const int brow = ti.n * BN + (int)rank * BNH;
-        int b0, b1;
-        kb_range(ti.z, b0, b1);
         for (int kb = b0; kb < b1; kb++, it++) {
           const int s = (int)(it % STAGES);
           if (it >= STAGES &&
@@ -1528,10 +1520,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
       // ---------------- MMA issuer of the pair (even CTA, one thread)
       long it = 0;
       int j = 0;
-      for (int t = pair; t < total_tiles && !*abort_flag; t += npairs, j++) {
-        const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
-        int b0, b1;
-        kb_range(ti.z, b0, b1);
+      for (; !*abort_flag && walk.next(ti, b0, b1); j++) {
         const int buf = j & 1;
         if (j >= 2 &&
             !tc::mbar_wait(&acc_empty[buf], (uint32_t)(((j >> 1) - 1) & 1), ep.err, PL_ERR_MBAR_TIMEOUT | 3)) {
@@ -1558,13 +1547,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
             tc::umma_bf16_pair(d_tmem, ad, bd, IDESC, (kb > b0 || kk > 0) ? 1u : 0u);
           }
           // stage s is free in both CTAs once these MMAs complete
-          const uint32_t e = tc::smem_u32(&empty[s]);
-          tc::umma_commit_pair(tc::cluster_addr(e, 0));
-          tc::umma_commit_pair(tc::cluster_addr(e, 1));
+          tc::umma_commit_both(tc::smem_u32(&empty[s]));
         }
-        const uint32_t f = tc::smem_u32(&acc_full[buf]);
-        tc::umma_commit_pair(tc::cluster_addr(f, 0));
-        tc::umma_commit_pair(tc::cluster_addr(f, 1));
+        tc::umma_commit_both(tc::smem_u32(&acc_full[buf]));
       }
       if (j > 0) tc::mbar_wait(&acc_full[(j - 1) & 1], (uint32_t)(((j - 1) >> 1) & 1), ep.err, PL_ERR_MBAR_TIMEOUT | 5);
     }
@@ -1574,12 +1559,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
     const int half = (warp - 2) >> 2;
     uint32_t stg_seq = 0;  // chunks this warp has staged: picks the staging tile
     int j = 0;
-    for (int t = pair; t < total_tiles; t += npairs, j++) {
-      const TileIdx ti = tile_at<EPI>(t, num_n, num_m);
-      int b0, b1;
-      kb_range(ti.z, b0, b1);
+    for (; walk.next(ti, b0, b1); j++) {
       const int buf = j & 1;
       const int m_blk = ti.m * 2 + (int)rank;
+      VocabPre pre;
+      if constexpr (EPI == EPI_VOCAB) pre = vocab_prefetch<BN>(ep, m_blk, ti.n, M, sub, half, lane);
       const bool ok = tc::mbar_wait(&acc_full[buf], (uint32_t)((j >> 1) & 1), ep.err, PL_ERR_MBAR_TIMEOUT | 6);
       if (!ok || *abort_flag) {
         *abort_flag = 1;
@@ -1589,7 +1573,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
       const uint32_t t_row = tmem_base + (uint32_t)(buf * BN) + ((uint32_t)(sub * 32) << 16);
       // a 128-row block wholly past M (odd CTA, M not a multiple of 256) has nothing to write: its
       // column partials would fall outside the ceil(M / 128) rows the caller provides
-      if (m_blk * BM < M)
+      if (m_blk * BM >= M) {
+      } else if constexpr (EPI == EPI_VOCAB)
+        epilogue_vocab<BN>(ep, pre, t_row, m_blk, ti.n, M, sub, half, lane, red + (warp - 2) * (BN / 2));
+      else if constexpr (EPI == EPI_SLICE)
+        epilogue_slice<BN>(ep, t_row, m_blk, ti.n, M, walk.slab < 0 ? -1 : (walk.slab * 2 + rank) * BM, b1 > b0, sub, half,
+                           lane);
+      else
         epilogue_tile<BN, EPI>(ep, t_row, m_blk, ti.n, ti.z, ep.k_splits > 1 ? 0 : ti.z, b1 > b0, sub, half, lane, red,
                                rowscr, stg_base + (warp - 2) * GemmSmem<BN, EPI>::STG_WARP, &tmC, &tmC2, stg_seq);
       tc::tc_fence_before();
@@ -1631,7 +1621,10 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
 // operands are MN-major (the weight gradients; the default); a negative mode only queries. Returns the
 // previous mode.
 int gemm_set_pair_mode(int mode);
-// CTAs of an EPI_SLICE launch (the current device's SMs): the `grid` of its slice_shape.
+// SMs of the current device. An EPI_SLICE launch runs on all of them: one CTA each with 128-row tiles, or (gemm_paired)
+// pairs with 256-row tiles; its slice_shape follows from that.
 int gemm_sms();
+// Whether gemm_launch takes CTA pairs for such a product.
+bool gemm_paired(int bn, int epi, bool a_mn, bool b_mn, int M);
 
 }  // namespace pl

@@ -24,22 +24,36 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
                : "memory");
 }
+// One try suspends the thread for up to this long (a hint): waiting warps then poll rarely, which leaves issue slots
+// and power to the tensor cores.
+constexpr uint32_t kMbarSuspendNs = 20000;
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(kMbarSuspendNs)
       : "memory");
   return ok != 0;
 }
-// Bounded wait for the phase of `parity` to complete. Returns false (and records `code` in *err)
-// when the limit runs out; a legitimate wait in these kernels lasts microseconds.
+// Bounded wait for the phase of `parity` to complete. Returns false (and records `code` in *err) after
+// four seconds; a legitimate wait in these kernels lasts microseconds. The clock is read on every 256th
+// try only.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code) {
-  for (uint32_t i = 0; i < (1u << 25); ++i)
+  uint64_t since = 0;
+  for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 0u) {
+      uint64_t now;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+      if (since == 0)
+        since = now;
+      else if (now - since > 4000000000ull)
+        break;
+    }
+  }
   if (err) atomicOr(err, code);
   return false;
 }
@@ -223,11 +237,14 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t adesc, 
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Arrives once on the barrier at shared::cluster address `cluster_bar` (either CTA of the pair) when
-// the pair MMAs this thread issued before it have completed.
-__device__ __forceinline__ void umma_commit_pair(uint32_t cluster_bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_bar)
-               : "memory");
+
+// Arrives once on the barrier at shared::cta address `bar` of both CTAs of the pair when the pair MMAs this
+// thread issued before it have completed.
+__device__ __forceinline__ void umma_commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
 }
 
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {

@@ -553,7 +553,7 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 // carries most of the row, and what its rounding to bf16 took away (val - bf16(val)) W[target] is given back, so that
 // dx is rounded once; among many answers no single rounding stands out. One warp per row.
 __global__ void __launch_bounds__(256)
-    vocab_dx_kernel(const float* __restrict__ out, long ldo, const float* __restrict__ slabs, int bn, int grid,
+    vocab_dx_kernel(const float* __restrict__ out, long ldo, const float* __restrict__ slabs, int bm, int bn, int grid,
                     const int* __restrict__ rows, const int* __restrict__ count, long off, long n, long V, long D,
                     int K, RowOut in, const __nv_bfloat16* __restrict__ w, long ldw, __nv_bfloat16* __restrict__ dx,
                     long lddx) {
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(256)
   const int lane = threadIdx.x & 31;
   const long have = rows_here(count, off, n);
   if (i >= have) return;
-  const SliceShape shape = slice_shape((int)have, (int)D, (int)V, bn, grid);
+  const SliceShape shape = slice_shape((int)have, (int)D, (int)V, bm, bn, grid);
   const long r = rows ? rows[off + i] : off + i;
   const bool vec = ((uintptr_t)dx & 15) == 0 && lddx % 8 == 0 && D % 8 == 0;
   __nv_bfloat16* d = dx + r * lddx;
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(256)
   const bool wvec = ((uintptr_t)w & 15) == 0 && ldw % 8 == 0;
   for (long c = lane * 8; c < D; c += 256) {
     float v[8];
-    slice_sum8(shape, out, ldo, slabs, bn, i, (int)c, v);
+    slice_sum8(shape, out, ldo, slabs, bm, bn, i, (int)c, v);
     if (rest != 0.f) {
       if (wvec && c + 8 <= D) {
         const uint4 raw = __ldg(reinterpret_cast<const uint4*>(wr + c));
@@ -604,14 +604,15 @@ __global__ void __launch_bounds__(256)
 // The weight gradient from f32: a sliced product's parts (slabs) or the sum of the pieces (slabs NULL, src = acc);
 // pieces before the last are kept in acc, the last goes to dw in the caller's type. One warp per row and 256 columns.
 __global__ void __launch_bounds__(256)
-    vocab_dw_kernel(const float* __restrict__ src, long lds, const float* __restrict__ slabs, int bn, int grid,
+    vocab_dw_kernel(const float* __restrict__ src, long lds, const float* __restrict__ slabs, int bm, int bn, int grid,
                     const int* __restrict__ count, long off, long n, float* __restrict__ acc, int add, int last, long V,
                     long D, int f32, void* __restrict__ dw, long lddw) {
   const long r = (long)blockIdx.x * 8 + (threadIdx.x >> 5), c = (long)blockIdx.y * 256 + (threadIdx.x & 31) * 8;
   if (r >= V || c >= D) return;
   float v[8];
   if (slabs) {
-    slice_sum8(slice_shape((int)V, (int)D, (int)rows_here(count, off, n), bn, grid), src, lds, slabs, bn, r, (int)c, v);
+    slice_sum8(slice_shape((int)V, (int)D, (int)rows_here(count, off, n), bm, bn, grid), src, lds, slabs, bm, bn, r, (int)c,
+               v);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = src[r * lds + c + j];
@@ -921,9 +922,10 @@ static int vocab_run(const VocabCall& c) {
       const Operand Z{ws + p.terms, p.R, V, p.ldt, 1, 0};
       rc = gemm_launch(p.bd, EPI_SLICE, false, true, Z, W, (int)n, (int)D, (int)V, 1, g, st);
       if (rc) return rc;
-      vocab_dx_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>((const float*)(ws + p.dxs), p.Dp, slabs, p.bd, sms, rows,
-                                                               count, off, n, V, D, (int)k1, ro, w, ldw,
-                                                               (__nv_bfloat16*)c.dx, (long)c.lddx);
+      const bool pairs = gemm_paired(p.bd, EPI_SLICE, false, true, (int)n);
+      vocab_dx_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>((const float*)(ws + p.dxs), p.Dp, slabs, pairs ? 256 : 128,
+                                                               p.bd, pairs ? sms / 2 : sms, rows, count, off, n, V,
+                                                               D, (int)k1, ro, w, ldw, (__nv_bfloat16*)c.dx, (long)c.lddx);
       count_launch();
       PL_LAUNCH("vocab_dx_kernel");
     }
@@ -947,8 +949,10 @@ static int vocab_run(const VocabCall& c) {
       rc = gemm_launch(p.bd, epi, true, true, Zk, Xk, (int)V, (int)D, (int)n, 1, g, st);
       if (rc) return rc;
       if (!direct && (p.dw_slice || last)) {
+        const bool pairs = gemm_paired(p.bd, EPI_SLICE, true, true, (int)V);
         vocab_dw_kernel<<<dim3((unsigned)ceil_div(V, 8), (unsigned)ceil_div(D, 256)), 256, 0, st>>>(
-            p.dw_slice ? (const float*)(ws + p.dws) : acc, p.Dp, p.dw_slice ? slabs : nullptr, p.bd, sms, count, off, n,
+            p.dw_slice ? (const float*)(ws + p.dws) : acc, p.Dp, p.dw_slice ? slabs : nullptr, pairs ? 256 : 128, p.bd,
+            pairs ? sms / 2 : sms, count, off, n,
             acc, p.dw_slice && q > 0, last, V, D, c.dw_f32, c.dw, (long)c.lddw);
         count_launch();
         PL_LAUNCH("vocab_dw_kernel");
