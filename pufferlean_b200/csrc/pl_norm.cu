@@ -37,7 +37,7 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
 // VEC consecutive values of type T as they lie in memory. Rows are read and written once: streaming accesses, so
 // that the weights stay in L1.
 template <typename T, int VEC>
-struct Pack {
+struct __align__(sizeof(T) * VEC) Pack {
   T v[VEC];
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (sizeof(T) * VEC == 16) {
@@ -74,6 +74,101 @@ __device__ __forceinline__ void load_param(const float* __restrict__ p, long c, 
   }
 }
 
+// Sums and products over the VEC values of a vector, two lanes at a time where VEC is even (sm_100's two-lane f32
+// instructions; both kernels are bound by instruction issue before HBM otherwise).
+template <int VEC>
+struct Vec {
+  float v[VEC];
+  __device__ __forceinline__ float2 at(int j) const { return make_float2(v[j], v[j + 1]); }
+  __device__ __forceinline__ void set(int j, float2 f) {
+    v[j] = f.x;
+    v[j + 1] = f.y;
+  }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Vec<VEC> widen(const Pack<T, VEC>& p) {
+  Vec<VEC> o;
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p.v);
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      o.v[j] = __uint_as_float(w[j / 2] << 16);
+      o.v[j + 1] = __uint_as_float(w[j / 2] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) o.v[j] = to_f(p.v[j]);
+  }
+  return o;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> narrow(const Vec<VEC>& f) {
+  Pack<T, VEC> o;
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(o.v);
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f.v[j], f.v[j + 1]);
+      w[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) o.v[j] = from_f<T>(f.v[j]);
+  }
+  return o;
+}
+// a b + c, a + b, a b on every value
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> vfma(const Vec<VEC>& a, const Vec<VEC>& b, const Vec<VEC>& c) {
+  Vec<VEC> o;
+  if constexpr (VEC % 2 == 0) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) o.set(j, __ffma2_rn(a.at(j), b.at(j), c.at(j)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) o.v[j] = __fmaf_rn(a.v[j], b.v[j], c.v[j]);
+  }
+  return o;
+}
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> vadd(const Vec<VEC>& a, const Vec<VEC>& b) {
+  Vec<VEC> o;
+  if constexpr (VEC % 2 == 0) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) o.set(j, __fadd2_rn(a.at(j), b.at(j)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) o.v[j] = a.v[j] + b.v[j];
+  }
+  return o;
+}
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> vmul(const Vec<VEC>& a, const Vec<VEC>& b) {
+  Vec<VEC> o;
+  if constexpr (VEC % 2 == 0) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) o.set(j, __fmul2_rn(a.at(j), b.at(j)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) o.v[j] = a.v[j] * b.v[j];
+  }
+  return o;
+}
+template <int VEC>
+__device__ __forceinline__ Vec<VEC> vall(float f) {
+  Vec<VEC> o;
+#pragma unroll
+  for (int j = 0; j < VEC; j++) o.v[j] = f;
+  return o;
+}
+template <int VEC>
+__device__ __forceinline__ float vsum(const Vec<VEC>& a) {
+  float s = a.v[0];
+#pragma unroll
+  for (int j = 1; j < VEC; j++) s += a.v[j];
+  return s;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -93,9 +188,9 @@ __device__ __forceinline__ float group_sum(float v, float* scr) {
   return warp_sum(lane < NW ? scr[w0 + lane] : 0.f);
 }
 
-// Threads of a block whose rows take TPR threads each, and the blocks that share an SM (`of256` of 256 threads).
+// Threads of a block whose rows take TPR threads each, and the blocks that share an SM.
 __host__ __device__ constexpr int norm_threads(int tpr) { return tpr > 256 ? tpr : 256; }
-__host__ __device__ constexpr int norm_blocks(int tpr, int of256) { return tpr > 256 ? (tpr > 512 ? 1 : (of256 + 1) / 2) : of256; }
+__host__ __device__ constexpr int norm_blocks(int tpr) { return tpr > 256 ? 1 : 2; }
 
 // Sums N values (a power of two up to 32) over the lanes with one exchange less per level than the values kept:
 // lane l returns the total of value l / (32 / N).
@@ -160,11 +255,12 @@ __device__ __forceinline__ float group_sum_n(const float (&s)[N], float (*scr)[3
   return v;
 }
 
-// A block walks the rows, RB of them per group at a time: their loads are issued one step ahead, their sums folded in
-// one butterfly, and the weights stay in registers (read again per row they cost twice the row's own L1 traffic:
-// 65,536 x 2,048 bf16 took 135 us that way).
+// A block walks the rows, RB of them per group at a time, their sums folded in one butterfly and the weights kept in
+// registers (read again per row they cost twice the row's own L1 traffic: 65,536 x 2,048 bf16 took 135 us that way).
+// The next rows are loaded one step ahead; bulk copies into a ring of shared memory instead were no faster (107
+// against 95 us: what bounds the kernel then is the folds' latency, not the loads').
 template <typename T, int VEC, int TPR, int K, int RB>
-__global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR, 3))
+__global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR))
     norm_fwd_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w, const float* __restrict__ b,
                     long rows, int cols, float eps, T* __restrict__ y, long ldy, float* __restrict__ mean,
                     float* __restrict__ rstd) {
@@ -173,83 +269,71 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR, 3))
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float inv = 1.f / (float)cols;
-  float wv[K][VEC], bv[K][VEC];
+  const long step = (long)gridDim.x * G * RB, base0 = (long)blockIdx.x * G * RB;
+  Vec<VEC> wv[K], bv[K];
+  bool in_row[K];
 #pragma unroll
   for (int k = 0; k < K; k++) {
     const int c = (k * TPR + t) * VEC;
-#pragma unroll
-    for (int j = 0; j < VEC; j++) {
-      wv[k][j] = 1.f;
-      bv[k][j] = 0.f;
-    }
-    if (w && c < cols) load_param<VEC>(w, c, wv[k]);
-    if (b && c < cols) load_param<VEC>(b, c, bv[k]);
+    in_row[k] = c < cols;
+    wv[k] = vall<VEC>(1.f);
+    bv[k] = vall<VEC>(0.f);
+    if (w && in_row[k]) load_param<VEC>(w, c, wv[k].v);
+    if (b && in_row[k]) load_param<VEC>(b, c, bv[k].v);
   }
-  Pack<T, VEC> in[RB][K], nx[RB][K];
-  auto load = [&](long r0, Pack<T, VEC> (&p)[RB][K]) {
+  Pack<T, VEC> nx[RB][K];
+  auto load = [&](long r0) {  // what lies outside the matrix reads as zero
 #pragma unroll
     for (int i = 0; i < RB; i++)
 #pragma unroll
       for (int k = 0; k < K; k++) {
-        const int c = (k * TPR + t) * VEC;
-        if (r0 + i < rows && c < cols) p[i][k].load(x + (r0 + i) * ldx + c);
+        if (r0 + i < rows && in_row[k])
+          nx[i][k].load(x + (r0 + i) * ldx + (k * TPR + t) * VEC);
+        else
+          nx[i][k] = narrow<T, VEC>(vall<VEC>(0.f));
       }
   };
-  const long step = (long)gridDim.x * G * RB;
-  load((long)blockIdx.x * G * RB + g * RB, in);
-  for (long base = (long)blockIdx.x * G * RB; base < rows; base += step) {
+  load(base0 + g * RB);
+  for (long base = base0; base < rows; base += step) {
     const long r0 = base + (long)g * RB;
-    if (base + step < rows) load(r0 + step, nx);
-    float s[RB], m[RB];
+    Vec<VEC> f[RB][K];
+    float s[RB];
 #pragma unroll
     for (int i = 0; i < RB; i++) {
-      s[i] = 0.f;
+      Vec<VEC> a = vall<VEC>(0.f);
 #pragma unroll
-      for (int k = 0; k < K; k++)
-        if (r0 + i < rows && (k * TPR + t) * VEC < cols) {
-#pragma unroll
-          for (int j = 0; j < VEC; j++) s[i] += to_f(in[i][k].v[j]);
-        }
+      for (int k = 0; k < K; k++) {
+        f[i][k] = widen<T, VEC>(nx[i][k]);
+        a = vadd(a, f[i][k]);
+      }
+      s[i] = vsum(a);
     }
-    float v = group_sum_n<TPR, RB>(s, scr[0], lane, warp);
+    if (base + step < rows) load(r0 + step);
+    float v = group_sum_n<TPR, RB>(s, scr[0], lane, warp) * inv;
 #pragma unroll
     for (int i = 0; i < RB; i++) {
-      m[i] = __shfl_sync(0xffffffffu, v, i * LV) * inv;
-      s[i] = 0.f;
+      const float m = __shfl_sync(0xffffffffu, v, i * LV);
+      if (t == 0 && r0 + i < rows) mean[r0 + i] = m;
+      Vec<VEC> a = vall<VEC>(0.f);
 #pragma unroll
-      for (int k = 0; k < K; k++)
-        if (r0 + i < rows && (k * TPR + t) * VEC < cols) {
-#pragma unroll
-          for (int j = 0; j < VEC; j++) {
-            const float d = to_f(in[i][k].v[j]) - m[i];
-            s[i] = __fmaf_rn(d, d, s[i]);
-          }
-        }
+      for (int k = 0; k < K; k++) {
+        f[i][k] = vadd(f[i][k], vall<VEC>(-m));
+        if (in_row[k]) a = vfma(f[i][k], f[i][k], a);
+      }
+      s[i] = vsum(a);
     }
     v = group_sum_n<TPR, RB>(s, scr[1], lane, warp);  // its barrier also ends the reads of scr[0]
+    v = 1.f / sqrtf(v * inv + eps);
 #pragma unroll
     for (int i = 0; i < RB; i++) {
-      const float r = 1.f / sqrtf(__shfl_sync(0xffffffffu, v, i * LV) * inv + eps);
-      if (r0 + i < rows) {
-        if (t == 0) {
-          mean[r0 + i] = m[i];
-          rstd[r0 + i] = r;
-        }
+      const float r = __shfl_sync(0xffffffffu, v, i * LV);
+      if (r0 + i >= rows) break;
+      if (t == 0) rstd[r0 + i] = r;
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-          const int c = (k * TPR + t) * VEC;
-          if (c >= cols) break;
-          Pack<T, VEC> out;
-#pragma unroll
-          for (int j = 0; j < VEC; j++) out.v[j] = from_f<T>((to_f(in[i][k].v[j]) - m[i]) * r * wv[k][j] + bv[k][j]);
-          out.store(y + (r0 + i) * ldy + c);
-        }
-      }
+      for (int k = 0; k < K; k++)
+        if (in_row[k])
+          narrow<T, VEC>(vfma(vmul(f[i][k], vall<VEC>(r)), wv[k], bv[k])).store(y + (r0 + i) * ldy + (k * TPR + t) * VEC);
     }
-#pragma unroll
-    for (int i = 0; i < RB; i++)
-#pragma unroll
-      for (int k = 0; k < K; k++) in[i][k] = nx[i][k];
   }
 }
 
@@ -291,109 +375,87 @@ __global__ void __launch_bounds__(512)
 // blocks' column sums go to `part` ([grid][2][cols]) and are added in block order by norm_param_kernel.
 // Wide rows leave few registers per thread: RB falls, and the weight is read again (from L1) for each row.
 template <typename T, int VEC, int TPR, int K, int RB>
-__global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR, 2))
+__global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR))
     norm_bwd_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ x, long ldx,
                     const float* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
                     long rows, int cols, T* __restrict__ dx, long lddx, float* __restrict__ part) {
   constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR, E = VEC * K;
   constexpr int NV = 2 * RB, LV = 32 / NV;  // values of an iteration, lanes that hold one of them
   constexpr bool KEEP_W = TPR < 1024;
-  __shared__ float scr[2][NV][32];          // [iteration parity][value][warp]
-  extern __shared__ float fold[];           // [G][2][TPR * E] (G > 1)
+  __shared__ float scr[2][NV][32];  // [iteration parity][value][warp]
+  extern __shared__ float fold[];   // [G][2][TPR * E] (G > 1)
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float inv = 1.f / (float)cols;
-  float wv[K][VEC], dw[E], db[E];
+  const long step = (long)gridDim.x * G * RB, base0 = (long)blockIdx.x * G * RB;
+  Vec<VEC> wv[K], dw[K], db[K];
+  bool in_row[K];
   auto load_w = [&](int k) {
-    const int c = (k * TPR + t) * VEC;
-#pragma unroll
-    for (int j = 0; j < VEC; j++) wv[k][j] = 1.f;
-    if (w && c < cols) load_param<VEC>(w, c, wv[k]);
+    wv[k] = vall<VEC>(1.f);
+    if (w && in_row[k]) load_param<VEC>(w, (k * TPR + t) * VEC, wv[k].v);
   };
-  if (KEEP_W) {
 #pragma unroll
-    for (int k = 0; k < K; k++) load_w(k);
+  for (int k = 0; k < K; k++) in_row[k] = (k * TPR + t) * VEC < cols;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    dw[k] = db[k] = vall<VEC>(0.f);
+    if (KEEP_W) load_w(k);
   }
-#pragma unroll
-  for (int e = 0; e < E; e++) dw[e] = db[e] = 0.f;
-
-  Pack<T, VEC> xi[RB][K], di[RB][K], xn[RB][K], dn[RB][K];
-  float m[RB], r[RB], mn[RB], rn[RB];
-  auto load = [&](long r0, Pack<T, VEC> (&px)[RB][K], Pack<T, VEC> (&pd)[RB][K], float (&pm)[RB], float (&pr)[RB]) {
+  Pack<T, VEC> xn[RB][K], dn[RB][K];
+  float mn[RB], rn[RB];
+  auto load = [&](long r0) {  // what lies outside the matrix: dy = 0 keeps it out of every sum
 #pragma unroll
     for (int i = 0; i < RB; i++) {
       const bool ok = r0 + i < rows;
 #pragma unroll
       for (int k = 0; k < K; k++) {
-        const int c = (k * TPR + t) * VEC;
-        if (ok && c < cols) {
-          px[i][k].load(x + (r0 + i) * ldx + c);
-          pd[i][k].load(dy + (r0 + i) * lddy + c);
-        } else {  // nothing there: dy = 0 keeps it out of every sum
-#pragma unroll
-          for (int j = 0; j < VEC; j++) px[i][k].v[j] = pd[i][k].v[j] = from_f<T>(0.f);
+        if (ok && in_row[k]) {
+          xn[i][k].load(x + (r0 + i) * ldx + (k * TPR + t) * VEC);
+          dn[i][k].load(dy + (r0 + i) * lddy + (k * TPR + t) * VEC);
+        } else {
+          xn[i][k] = dn[i][k] = narrow<T, VEC>(vall<VEC>(0.f));
         }
       }
-      pm[i] = ok ? __ldg(mean + r0 + i) : 0.f;
-      pr[i] = ok ? __ldg(rstd + r0 + i) : 0.f;
+      mn[i] = ok ? __ldg(mean + r0 + i) : 0.f;
+      rn[i] = ok ? __ldg(rstd + r0 + i) : 0.f;
     }
   };
+  load(base0 + g * RB);
   int parity = 0;
-  const long step = (long)gridDim.x * G * RB;
-  load((long)blockIdx.x * G * RB + g * RB, xi, di, m, r);
-  for (long base = (long)blockIdx.x * G * RB; base < rows; base += step, parity ^= 1) {
+  for (long base = base0; base < rows; base += step, parity ^= 1) {
     const long r0 = base + (long)g * RB;
-    if (base + step < rows) load(r0 + step, xn, dn, mn, rn);
-    float s[NV];
+    Vec<VEC> xh[RB][K], gg[RB][K];
+    float r[RB], s[NV];
 #pragma unroll
     for (int i = 0; i < RB; i++) {
-      float s1 = 0.f, s2 = 0.f;
+      r[i] = rn[i];
+      Vec<VEC> s1 = vall<VEC>(0.f), s2 = vall<VEC>(0.f);
 #pragma unroll
       for (int k = 0; k < K; k++) {
         if (!KEEP_W) load_w(k);
-#pragma unroll
-        for (int j = 0; j < VEC; j++) {
-          const float d = to_f(di[i][k].v[j]), xh = (to_f(xi[i][k].v[j]) - m[i]) * r[i], gg = d * wv[k][j];
-          s1 += gg;
-          s2 = __fmaf_rn(gg, xh, s2);
-          dw[k * VEC + j] = __fmaf_rn(d, xh, dw[k * VEC + j]);
-          db[k * VEC + j] += d;
-        }
+        const Vec<VEC> d = widen<T, VEC>(dn[i][k]);
+        xh[i][k] = vmul(vadd(widen<T, VEC>(xn[i][k]), vall<VEC>(-mn[i])), vall<VEC>(r[i]));
+        gg[i][k] = vmul(d, wv[k]);
+        s1 = vadd(s1, gg[i][k]);
+        s2 = vfma(gg[i][k], xh[i][k], s2);
+        dw[k] = vfma(d, xh[i][k], dw[k]);
+        db[k] = vadd(db[k], d);
       }
-      s[2 * i] = s1;
-      s[2 * i + 1] = s2;
+      s[2 * i] = vsum(s1);
+      s[2 * i + 1] = vsum(s2);
     }
-    const float v = group_sum_n<TPR, NV>(s, scr[parity], lane, warp);  // the other parity's barrier ended its reads
+    if (base + step < rows) load(r0 + step);
+    const float v = -inv * group_sum_n<TPR, NV>(s, scr[parity], lane, warp);  // the other parity's barrier ended its reads
 #pragma unroll
     for (int i = 0; i < RB; i++) {
-      const float a1 = __shfl_sync(0xffffffffu, v, 2 * i * LV) * inv;        // mean of g
-      const float a2 = __shfl_sync(0xffffffffu, v, (2 * i + 1) * LV) * inv;  // mean of g xh
-      if (r0 + i < rows) {
+      const Vec<VEC> a1 = vall<VEC>(__shfl_sync(0xffffffffu, v, 2 * i * LV));        // - mean of g
+      const Vec<VEC> a2 = vall<VEC>(__shfl_sync(0xffffffffu, v, (2 * i + 1) * LV));  // - mean of g xh
+      if (r0 + i >= rows) break;
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-          const int c = (k * TPR + t) * VEC;
-          if (c >= cols) break;
-          if (!KEEP_W) load_w(k);
-          Pack<T, VEC> out;
-#pragma unroll
-          for (int j = 0; j < VEC; j++) {
-            const float xh = (to_f(xi[i][k].v[j]) - m[i]) * r[i];
-            const float gg = to_f(di[i][k].v[j]) * wv[k][j];
-            out.v[j] = from_f<T>((gg - a1 - xh * a2) * r[i]);
-          }
-          out.store(dx + (r0 + i) * lddx + c);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < RB; i++) {
-#pragma unroll
-      for (int k = 0; k < K; k++) {
-        xi[i][k] = xn[i][k];
-        di[i][k] = dn[i][k];
-      }
-      m[i] = mn[i];
-      r[i] = rn[i];
+      for (int k = 0; k < K; k++)
+        if (in_row[k])
+          narrow<T, VEC>(vmul(vfma(xh[i][k], a2, vadd(gg[i][k], a1)), vall<VEC>(r[i])))
+              .store(dx + (r0 + i) * lddx + (k * TPR + t) * VEC);
     }
   }
   if (!part) return;
@@ -405,8 +467,8 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR, 2))
 #pragma unroll
       for (int j = 0; j < VEC; j++) {
         const int c = (k * TPR + t) * VEC + j;
-        fold[(g * 2) * W + c] = dw[k * VEC + j];
-        fold[(g * 2 + 1) * W + c] = db[k * VEC + j];
+        fold[(g * 2) * W + c] = dw[k].v[j];
+        fold[(g * 2 + 1) * W + c] = db[k].v[j];
       }
     __syncthreads();
     for (int c = threadIdx.x; c < cols; c += THREADS) {
@@ -426,8 +488,8 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR, 2))
       for (int j = 0; j < VEC; j++) {
         const int c = (k * TPR + t) * VEC + j;
         if (c < cols) {
-          pw[c] = dw[k * VEC + j];
-          pw[cols + c] = db[k * VEC + j];
+          pw[c] = dw[k].v[j];
+          pw[cols + c] = db[k].v[j];
         }
       }
   }
@@ -508,7 +570,7 @@ template <typename T, int VEC, int TPR, int K, int RB>
 static int fwd_launch(const void* x, long ldx, const float* w, const float* b, long rows, int cols, float eps, void* y,
                       long ldy, float* mean, float* rstd, cudaStream_t st) {
   constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR;
-  const long need = ceil_div(rows, (long)G * RB), most = (long)kNormSms * norm_blocks(TPR, 3);
+  const long need = ceil_div(rows, (long)G * RB), most = (long)kNormSms * norm_blocks(TPR);
   // few rows: one per group, so that more SMs have some (latency); many: RB at a time
   if constexpr (RB > 1)
     if (need < most / 2) return fwd_launch<T, VEC, TPR, K, 1>(x, ldx, w, b, rows, cols, eps, y, ldy, mean, rstd, st);
@@ -529,14 +591,24 @@ static int fwd_pick(const void* x, long ldx, const float* w, const float* b, lon
   if (cols <= (long)VEC * TPR * K) \
     return fwd_launch<T, VEC, TPR, K, RB>(x, ldx, w, b, rows, (int)cols, eps, y, ldy, mean, rstd, st);
   if (vec) {
-    PL_FWD(V, 32, 1, 4)
-    PL_FWD(V, 64, 1, 4)
-    PL_FWD(V, 128, 1, 4)
-    PL_FWD(V, 256, 1, 4)
-    PL_FWD(V, 512, 1, 2)
-    PL_FWD(V, 1024, 1, 2)
-    PL_FWD(V, 1024, 2, 1)
-    if constexpr (V == 4) PL_FWD(V, 1024, 4, 1)
+    if constexpr (V == 8) {  // bf16: 16 values per thread
+      PL_FWD(V, 32, 1, 4)
+      PL_FWD(V, 32, 2, 2)
+      PL_FWD(V, 64, 2, 2)
+      PL_FWD(V, 128, 2, 2)
+      PL_FWD(V, 256, 2, 2)
+      PL_FWD(V, 512, 2, 2)
+      PL_FWD(V, 1024, 2, 1)
+    } else {
+      PL_FWD(V, 32, 1, 4)
+      PL_FWD(V, 64, 1, 4)
+      PL_FWD(V, 128, 1, 4)
+      PL_FWD(V, 256, 1, 4)
+      PL_FWD(V, 512, 1, 4)
+      PL_FWD(V, 512, 2, 2)
+      PL_FWD(V, 1024, 2, 1)
+      PL_FWD(V, 1024, 4, 1)
+    }
   } else {
     PL_FWD(1, 32, 4, 4)
     PL_FWD(1, 64, 8, 2)
@@ -565,16 +637,15 @@ static int bwd_launch(const void* dy, long lddy, const void* x, long ldx, const 
                       const float* rstd, long rows, int cols, void* dx, long lddx, float* dw, float* db, float* part,
                       cudaStream_t st) {
   constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR;
-  constexpr size_t SMEM = G > 1 ? (size_t)G * 2 * TPR * VEC * K * 4 : 0;
-  static_assert(SMEM <= 48 * 1024, "column sums of the groups");
-  const long need = ceil_div(rows, (long)G * RB), most = (long)kNormSms * norm_blocks(TPR, 2);
-  static_assert(kNormSms * norm_blocks(TPR, 2) <= kNormParts, "column sums of the blocks");
+  constexpr size_t FOLD = G > 1 ? (size_t)G * 2 * TPR * VEC * K * 4 : 0;
+  const long need = ceil_div(rows, (long)G * RB), most = (long)kNormSms * norm_blocks(TPR);
   if constexpr (RB > 1)
     if (need < most / 2)
       return bwd_launch<T, VEC, TPR, K, 1>(dy, lddy, x, ldx, w, mean, rstd, rows, cols, dx, lddx, dw, db, part, st);
   const int grid = (int)(need < most ? need : most);
-  norm_bwd_kernel<T, VEC, TPR, K, RB><<<grid, THREADS, SMEM, st>>>((const T*)dy, lddy, (const T*)x, ldx, w, mean, rstd, rows,
-                                                               cols, (T*)dx, lddx, (dw || db) ? part : nullptr);
+  static_assert(FOLD <= 48 * 1024, "column sums of the groups");
+  norm_bwd_kernel<T, VEC, TPR, K, RB><<<grid, THREADS, FOLD, st>>>((const T*)dy, lddy, (const T*)x, ldx, w, mean, rstd,
+                                                                   rows, cols, (T*)dx, lddx, (dw || db) ? part : nullptr);
   count_launch();
   PL_LAUNCH("norm_bwd_kernel");
   return (dw || db) ? param_launch(part, grid, cols, dw, db, st) : PL_OK;
@@ -591,14 +662,24 @@ static int bwd_pick(const void* dy, long lddy, const void* x, long ldx, const fl
   if (cols <= (long)VEC * TPR * K) \
     return bwd_launch<T, VEC, TPR, K, RB>(dy, lddy, x, ldx, w, mean, rstd, rows, (int)cols, dx, lddx, dw, db, part, st);
   if (vec) {
-    PL_BWD(V, 32, 1, 2)
-    PL_BWD(V, 64, 1, 2)
-    PL_BWD(V, 128, 1, 2)
-    PL_BWD(V, 256, 1, 2)
-    PL_BWD(V, 512, 1, 2)
-    PL_BWD(V, 1024, 1, 1)
-    PL_BWD(V, 1024, 2, 1)
-    if constexpr (V == 4) PL_BWD(V, 1024, 4, 1)
+    if constexpr (V == 8) {
+      PL_BWD(V, 32, 1, 2)
+      PL_BWD(V, 32, 2, 1)
+      PL_BWD(V, 64, 2, 1)
+      PL_BWD(V, 128, 2, 1)
+      PL_BWD(V, 256, 2, 1)
+      PL_BWD(V, 512, 2, 1)
+      PL_BWD(V, 1024, 2, 1)
+    } else {
+      PL_BWD(V, 32, 1, 4)
+      PL_BWD(V, 64, 1, 4)
+      PL_BWD(V, 128, 1, 4)
+      PL_BWD(V, 256, 1, 4)
+      PL_BWD(V, 512, 1, 4)
+      PL_BWD(V, 512, 2, 2)
+      PL_BWD(V, 1024, 2, 1)
+      PL_BWD(V, 1024, 4, 1)
+    }
   } else {
     PL_BWD(1, 32, 4, 4)
     PL_BWD(1, 64, 8, 2)
