@@ -491,33 +491,34 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
   uint16_t* tile = reinterpret_cast<uint16_t*>(terms) + r0 * ld + c0;
   for (int h = threadIdx.x; h < hits; h += 256)
     tile[(hit_at[h] >> 16) * ld + (hit_at[h] & 0xffffu)] = __bfloat16_as_ushort(__float2bfloat16_rn(hit_v[h]));
-  if (!PART) return;
-  // thread t owns the block's columns t, t + 256, ...
+  if constexpr (PART) {
+    // thread t owns the block's columns t, t + 256, ...
 #pragma unroll
-  for (int s = 0; s < NS; s++) {
-    const int c = 256 * s + threadIdx.x;
-    float t = fold[c];
+    for (int s = 0; s < NS; s++) {
+      const int c = 256 * s + threadIdx.x;
+      float t = fold[c];
 #pragma unroll
-    for (int q = 1; q < 8; q++) t += fold[q * COLS + c];
-    fold[c] = t;
-  }
-  __syncthreads();
-  for (int h = threadIdx.x; h < hits; h += 256) {  // the first listed value of a column adds all of that column's
-    const uint32_t c = hit_at[h] & 0xffffu;
-    float t = 0.f;
-    bool first = true;
-    for (int g = 0; g < hits; g++) {
-      const bool same = (hit_at[g] & 0xffffu) == c;
-      first = first && !(same && g < h);
-      t += same ? hit_v[g] : 0.f;
+      for (int q = 1; q < 8; q++) t += fold[q * COLS + c];
+      fold[c] = t;
     }
-    if (first) fold[c] += t;
-  }
-  __syncthreads();
+    __syncthreads();
+    for (int h = threadIdx.x; h < hits; h += 256) {  // the first listed value of a column adds all of that column's
+      const uint32_t c = hit_at[h] & 0xffffu;
+      float t = 0.f;
+      bool first = true;
+      for (int g = 0; g < hits; g++) {
+        const bool same = (hit_at[g] & 0xffffu) == c;
+        first = first && !(same && g < h);
+        t += same ? hit_v[g] : 0.f;
+      }
+      if (first) fold[c] += t;
+    }
+    __syncthreads();
 #pragma unroll
-  for (int s = 0; s < NS; s++) {
-    const int c = 256 * s + threadIdx.x;
-    if (c0 + c < V) part[(long)blockIdx.y * V + c0 + c] = fold[c];
+    for (int s = 0; s < NS; s++) {
+      const int c = 256 * s + threadIdx.x;
+      if (c0 + c < V) part[(long)blockIdx.y * V + c0 + c] = fold[c];
+    }
   }
 }
 
@@ -644,6 +645,11 @@ __global__ void __launch_bounds__(256)
 // Rows up to which one row tile holds them all: leaving rows out of the products then saves nothing, so no plan is
 // made (two launches fewer; the rows without an answer are zeroed instead).
 constexpr long kVocabOneTile = 128;
+// Weights whose rows do not start at 128-byte lines cost the products' TMA boxes an extra line each. For the three
+// products of a gradient a copy with padded rows pays for itself from about this many rows on: V = 50,048, 4,096 rows,
+// D = 520 / 1,000 / 2,056: 930 / 1,100 / 2,233 us with the copy, 1,114 / 1,108 / 2,328 without; 1,000 rows: 270 / 352 /
+// 678 and 275 / 323 / 598. For the loss alone it does not (4,096 rows: 282 / 341 / 761 and 274 / 310 / 676).
+constexpr long kVocabPackRows = 2048;
 // Bytes of terms that one piece may hold. Fewer pieces mean fewer passes over the f32 weight gradient (each piece
 // after the first adds to it: 8 V D bytes).
 constexpr size_t kVocabPieceBytes = (size_t)4 << 30;
@@ -673,15 +679,15 @@ static size_t carve(size_t& at, size_t bytes) {
 }
 
 // K = 0: cross entropy. x_ok, w_ok: the matrix starts at 16 bytes and its row stride is a multiple of 8 (what TMA
-// needs).
-static VocabPlan vocab_plan(long N, long V, long D, long K, bool bias, bool grad, bool x_ok, bool w_ok, size_t piece_bytes,
-                            int sms) {
+// needs); w_lines: the same for 128 bytes and 64.
+static VocabPlan vocab_plan(long N, long V, long D, long K, bool bias, bool grad, bool x_ok, bool w_ok, bool w_lines,
+                            size_t piece_bytes, int sms) {
   VocabPlan p{};
   const long k1 = K ? K : 1;
   p.compact = N > kVocabOneTile;
   p.pack_x = p.compact || grad || !x_ok;
-  p.pack_w = !w_ok;
-  p.Dp = round_up(D, 8);
+  p.pack_w = !w_ok || (!w_lines && grad && N >= kVocabPackRows);
+  p.Dp = round_up(D, 64);
   p.ldt = round_up(V, 64);
   p.bn = V > 148 * 128 ? 256 : 128;
   p.bd = D > 128 ? 256 : 128;
@@ -765,6 +771,7 @@ struct VocabCall {
 };
 
 static bool rows16(const void* p, size_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
+static bool rows128(const void* p, size_t ld) { return ((uintptr_t)p & 127) == 0 && ld % 64 == 0; }
 
 template <int NS, bool PART>
 static int dz_launch(const VocabPlan& p, uint8_t* ws, long V, long K, const int* count, long off, long n, RowOut ro,
@@ -811,7 +818,7 @@ static int vocab_run(const VocabCall& c) {
   }
   const int sms = gemm_sms();
   const VocabPlan p = vocab_plan(N, V, D, K, c.bias != nullptr, c.grad, rows16(c.x, c.ldx), rows16(c.w, c.ldw),
-                                 c.piece_bytes, sms);
+                                 rows128(c.w, c.ldw), c.piece_bytes, sms);
   PL_REQUIRE(c.ws && c.ws_bytes >= p.bytes && ((uintptr_t)c.ws & 255) == 0, PL_ERR_INVALID,
              "%s: %zu bytes of workspace (256-byte aligned), %zu needed", c.what, c.ws ? c.ws_bytes : (size_t)0, p.bytes);
   uint8_t* ws = (uint8_t*)c.ws;
@@ -970,7 +977,7 @@ size_t pl_vocab_ws(size_t N, size_t V, size_t D, size_t K, uint8_t bias, uint8_t
                    size_t piece_bytes) {
   if (N == 0 || V == 0 || D == 0) return 0;
   const bool ok = aligned != 0;
-  return pl::vocab_plan((long)N, (long)V, (long)D, (long)K, bias != 0, grad != 0, ok, ok, piece_bytes,
+  return pl::vocab_plan((long)N, (long)V, (long)D, (long)K, bias != 0, grad != 0, ok, ok, ok, piece_bytes,
                         pl::gemm_sms())
       .bytes;
 }
