@@ -556,8 +556,8 @@ int pl_layernorm_grad_dev(const void* dy, size_t lddy, const void* x, size_t ldx
  * p = softmax(teacher / temperature) over the present entries, loss_n = sum_k p_k (log p_k - u_n,id_k) + lse_n = KL(p | q).
  * A row with no entry is left out like a negative target; entries that name the same id add up.
  *
- * ws: pl_vocab_ws bytes (K = 0 for the cross entropy, else at most 512; aligned = 1 when x starts at
- * 16 bytes with a row stride that is a multiple of 8 and w at 128 with one that is a multiple of 64). The gradient forms keep one piece of rows' softmax terms there (2 bytes each): piece_bytes
+ * ws: pl_vocab_ws bytes (K = 0 for the cross entropy, else at most 512; aligned = 1 when x and dw
+ * start at 16 bytes with row strides that are multiples of 8, and w at 128 with one that is a multiple of 64). The gradient forms keep one piece of rows' softmax terms there (2 bytes each): piece_bytes
  * bounds that piece, 0 = 4 GiB; the results do not depend on it beyond the order of dw's f32 sums.
  * dx [N x D] bf16; dw [V x D] and dbias [V] (given exactly when bias is) bf16, or f32 with dw_f32 = 1 (f32 sums of
  * products of bf16-rounded gradients). row_scale [N] f32 or NULL (ones). */

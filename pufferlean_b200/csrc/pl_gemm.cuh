@@ -31,11 +31,11 @@ enum EpiKind : int {
   EPI_SLICE = 6,  // out(f32) = acc; the tiles of an incomplete last wave are split along K (SliceShape)
 };
 
-// EPI_SLICE: tiles go to the `grid` CTAs (or CTA pairs) in whole waves; the `rem` tiles of the last, incomplete one are cut along K into q
-// slices each, as many as keep every CTA busy, and the CTAs of one slice walk the same k-blocks at the same time (so
-// they still share what they read of the operands through L2; dealing the k-blocks out in one line, every CTA at
-// another place of the long axis, made the product of 4,096 x 1,024 x 65,537 take 520 instead of 396 us). Slices go
-// to slabs of [bm][bn] f32, slice z of the i-th of these tiles to slab z rem + i, and whoever reads the result adds
+// EPI_SLICE: tiles go to the `grid` CTAs (or CTA pairs) in whole waves; the `rem` tiles of the last, incomplete one
+// are cut along K into q slices each, so that few CTAs idle, and the CTAs of one slice walk the same k-blocks at the
+// same time (so they still share what they read of the operands through L2; dealing the k-blocks out in one line, every
+// CTA at another place of the long axis, made the product of 4,096 x 1,024 x 65,537 take 520 instead of 396 us). Slices
+// go to slabs of [bm][bn] f32, slice z of the i-th of these tiles to slab z rem + i, and whoever reads the result adds
 // them in order (slice_sum8). The extents may be known on the device only, so the shape is worked out there.
 struct SliceShape {
   int num_n, num_m, kb, rem, q;
@@ -49,11 +49,24 @@ __host__ __device__ inline SliceShape slice_shape(int M, int N, int K, int bm, i
   const long tiles = (long)s.num_n * s.num_m;
   s.full = tiles / grid * grid;
   s.rem = (int)(tiles - s.full);
-  s.q = s.rem ? grid / s.rem : 1;
-  if (s.q > s.kb / 4) s.q = s.kb / 4;  // a slice costs a slab's write and read: at least four k-blocks each
-  if (s.q < 1) s.q = 1;
+  // one wave of slices where that keeps three CTAs in four busy, else the number (up to 6) that idles least: 85 tiles
+  // on 148 CTAs are cut in 5 (425 slices, three waves, 96 % busy)
+  int q = s.rem ? grid / s.rem : 1;
+  if (s.rem && s.rem * q * 4 < grid * 3) {
+    int best = 0;
+    for (int c = q; c <= 6; c++) {
+      const int items = s.rem * c, busy = items * 1024 / ((items + grid - 1) / grid * grid);
+      if (busy > best) {
+        best = busy;
+        q = c;
+      }
+    }
+  }
+  if (q > s.kb / 4) q = s.kb / 4;  // a slice costs a slab's write and read: at least four k-blocks each
+  s.q = q < 1 ? 1 : q;
   return s;
 }
+constexpr int kSliceSlabs = 5;  // slabs of a launch, in multiples of its grid: rem q < 0.75 grid * 6
 
 struct EpiArgs {
   void* out;
@@ -93,16 +106,16 @@ struct EpiArgs {
   // fold_scale[batch] for the next product. Every warp computes the same s.
   float* fold_scale;
   double fold_eps;
-  // EPI_VOCAB: u = acc * scale2 + vbias[col] * scale2 (vbias optional), the segment statistics [rows][ld_stat]
+  // EPI_VOCAB: u = acc * scale2 + vbias[col] * bias_scale2 (vbias optional), the segment statistics [rows][ld_stat]
   // (max, sum) of every row, and optionally ut[row] = u at column target[row_ids ? row_ids[row] : row]
-  float scale2;
+  float scale2, bias_scale2;
   const __nv_bfloat16* vbias;
   float2* stat;
   long ld_stat;
   const int* target;
   const int* row_ids;
   float* ut;
-  float* slabs;  // EPI_SLICE: [gridDim.x * 128][BN]
+  float* slabs;  // EPI_SLICE: [kSliceSlabs * gridDim.x * 128][BN]
   // EPI_F32, optional: out += alpha*acc instead of out = alpha*acc
   int accum;
   // Rows that exist (optional): the extent M (dyn_k = 0) or K (dyn_k = 1) of this call is
@@ -519,7 +532,7 @@ __device__ __forceinline__ VocabPre vocab_prefetch(const EpiArgs& ep, int m_tile
 }
 
 // EPI_VOCAB: this warp's 32 rows x BN/2 columns of a logit tile, one row per lane, its BN/2 accumulators in
-// registers. In log2 units u = acc * scale2 + bias * scale2, m = max u, s = sum 2^(u - m): the pair goes to
+// registers. In log2 units u = acc * scale2 + bias * bias_scale2, m = max u, s = sum 2^(u - m): the pair goes to
 // stat[row][2 n_tile + half], u of the row's target column to ut[row]. With `out` the terms leave as f16 scaled by
 // 2^15, so the largest is 2^15 exactly and 11 bits of mantissa hold down to 2^-29 of it; bf16 would cost a second
 // rounding of 2^-8 when the gradient is formed from them. A lane's terms are one row's, 32 bytes to a store: whole
@@ -545,7 +558,7 @@ __device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, const VocabPre
       const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&pre.bias);
       float b[4] = {__low2float(h[0]), __high2float(h[0]), __low2float(h[1]), __high2float(h[1])};
 #pragma unroll
-      for (int j = 0; j < 4; j++) b[j] = vocab_bias2(b[j], scale);
+      for (int j = 0; j < 4; j++) b[j] = vocab_bias2(b[j], ep.bias_scale2);
       reinterpret_cast<float4*>(bias_sm)[lane] = make_float4(b[0], b[1], b[2], b[3]);
     }
     __syncwarp();

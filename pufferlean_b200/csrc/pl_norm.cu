@@ -392,7 +392,8 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR))
   bool in_row[K];
   auto load_w = [&](int k) {
     wv[k] = vall<VEC>(1.f);
-    if (w && in_row[k]) load_param<VEC>(w, (k * TPR + t) * VEC, wv[k].v);
+    const int c = (k * TPR + t) * VEC;
+    if (w && c < cols) load_param<VEC>(w, c, wv[k].v);
   };
 #pragma unroll
   for (int k = 0; k < K; k++) in_row[k] = (k * TPR + t) * VEC < cols;

@@ -106,18 +106,29 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-// rows[0 .. *count) = the rows that count, in order; loss = lse = 0 for the others. One block.
+// rows[0 .. *count) = the rows that count, in order; loss = lse = 0 for the others. One block, four rows to a thread.
 __global__ void __launch_bounds__(1024)
     vocab_plan_kernel(Answers a, long N, int* __restrict__ rows, int* __restrict__ count, float* __restrict__ loss,
                       float* __restrict__ lse) {
   __shared__ int warp_n[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int base = 0;
-  for (long r0 = 0; r0 < N; r0 += 1024) {
-    const long r = r0 + threadIdx.x;
-    const bool in = r < N && row_counts(a, r);
-    const unsigned mask = __ballot_sync(0xffffffffu, in);
-    if (lane == 0) warp_n[warp] = __popc(mask);
+  for (long r0 = 0; r0 < N; r0 += 4096) {
+    const long r = r0 + 4 * threadIdx.x;
+    bool in[4];
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      in[j] = r + j < N && row_counts(a, r + j);
+      mine += in[j];
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += t;
+    }
+    if (lane == 31) warp_n[warp] = upto;
     __syncthreads();
     int n = warp_n[lane];
 #pragma unroll
@@ -125,12 +136,16 @@ __global__ void __launch_bounds__(1024)
       const int t = __shfl_up_sync(0xffffffffu, n, o);
       if (lane >= o) n += t;
     }
-    const int before = base + (warp ? __shfl_sync(0xffffffffu, n, warp - 1) : 0);
-    if (in) {
-      rows[before + __popc(mask & ((1u << lane) - 1u))] = (int)r;
-    } else if (r < N) {
-      loss[r] = 0.f;
-      lse[r] = 0.f;
+    const int before = __shfl_sync(0xffffffffu, n, (warp + 31) & 31);
+    int at = base + (warp ? before : 0) + upto - mine;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (in[j]) {
+        rows[at++] = (int)(r + j);
+      } else if (r + j < N) {
+        loss[r + j] = 0.f;
+        lse[r + j] = 0.f;
+      }
     }
     base += __shfl_sync(0xffffffffu, n, 31);
     __syncthreads();
@@ -138,8 +153,28 @@ __global__ void __launch_bounds__(1024)
   if (threadIdx.x == 0) *count = base;
 }
 
+// A warp's part [c0, c1) of a row (c0 a multiple of 1,024): 16 bytes to a lane where both rows start at 16 bytes.
+__device__ __forceinline__ void copy_row(__nv_bfloat16* __restrict__ d, const __nv_bfloat16* __restrict__ s, long c0, long c1,
+                                         bool in, bool vec, int lane) {
+  const __nv_bfloat16 zero = __float2bfloat16_rn(0.f);
+  long c = c0;
+  if (vec) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const long at = c0 + 256 * k + lane * 8;
+      if (at + 8 <= c1)
+        *reinterpret_cast<uint4*>(d + at) = in ? *reinterpret_cast<const uint4*>(s + at) : make_uint4(0, 0, 0, 0);
+    }
+    c = c0 + (c1 - c0) / 8 * 8;
+    if (c + lane < c1) d[c + lane] = in ? s[c + lane] : zero;
+  } else {
+#pragma unroll 16
+    for (c += lane; c < c1; c += 32) d[c] = in ? s[c] : zero;
+  }
+}
+
 // dst[i] = src[row i] for i < n (row i = rows[off + i] of the plan, or i itself without one; the row is zero where
-// it does not count), rows up to the next multiple of 64 zeroed. One warp per row.
+// it does not count), rows up to the next multiple of 64 zeroed. One warp per row and 1,024 columns.
 __global__ void __launch_bounds__(256)
     vocab_pack_kernel(const __nv_bfloat16* __restrict__ src, long ld, long D, Answers a, const int* __restrict__ rows,
                       const int* __restrict__ count, long off, long n, __nv_bfloat16* __restrict__ dst, long ldd) {
@@ -155,16 +190,18 @@ __global__ void __launch_bounds__(256)
     else
       in = row_counts(a, r);
   }
-  __nv_bfloat16* d = dst + i * ldd;
-  const __nv_bfloat16* s = src + r * ld;
-  if (((uintptr_t)src & 15) == 0 && ld % 8 == 0 && D % 8 == 0) {
-#pragma unroll 4
-    for (long c = lane * 8; c < D; c += 256)
-      *reinterpret_cast<uint4*>(d + c) = in ? *reinterpret_cast<const uint4*>(s + c) : make_uint4(0, 0, 0, 0);
-  } else {
-#pragma unroll 4
-    for (long c = lane; c < D; c += 32) d[c] = in ? s[c] : __float2bfloat16_rn(0.f);
-  }
+  const long c0 = (long)blockIdx.y * 1024, c1 = min(D, c0 + 1024);
+  copy_row(dst + i * ldd, src + r * ld, c0, c1, in, ((uintptr_t)src & 15) == 0 && ld % 8 == 0, lane);
+}
+
+// dst = src, rows of D values: a gradient that TMA could not write where the caller wants it.
+__global__ void __launch_bounds__(256)
+    vocab_copy_kernel(const __nv_bfloat16* __restrict__ src, long ld, long n, long D, __nv_bfloat16* __restrict__ dst,
+                      long ldd) {
+  const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= n) return;
+  const long c0 = (long)blockIdx.y * 1024, c1 = min(D, c0 + 1024);
+  copy_row(dst + i * ldd, src + i * ld, c0, c1, true, false, threadIdx.x & 31);
 }
 
 // The row's lse in log2 units from its segments' (max, sum); a fixed order over the threads t of `threads`.
@@ -522,15 +559,25 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
   }
 }
 
-// sum (+)= the row tiles' column sums; on the last piece dbias = sum (f32 or bf16).
-__global__ void __launch_bounds__(256)
+// sum (+)= the row tiles' column sums; on the last piece dbias = sum (f32 or bf16). 32 columns to a block, 32 slices of
+// the tiles, both folded in a fixed order.
+__global__ void __launch_bounds__(1024)
     vocab_dbias_kernel(const float* __restrict__ part, int tiles, long V, float* __restrict__ acc, int first, int last,
                        int f32, void* __restrict__ dbias) {
-  const long v = (long)blockIdx.x * 256 + threadIdx.x;
-  if (v >= V) return;
-  float s = first ? 0.f : acc[v];
-#pragma unroll 8
-  for (int q = 0; q < tiles; q++) s += part[(long)q * V + v];
+  __shared__ float scr[32][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const long c0 = (long)blockIdx.x * 32;
+  float s = 0.f;
+  if (c0 + lane < V) {
+#pragma unroll 4
+    for (int q = slice; q < tiles; q += 32) s += part[(long)q * V + c0 + lane];
+  }
+  scr[slice][lane] = s;
+  __syncthreads();
+  s = warp_sum_f(scr[lane][slice]);  // warp `slice` folds column `slice` of the block
+  const long v = c0 + slice;
+  if (lane || v >= V) return;
+  if (!first) s += acc[v];
   if (!last)
     acc[v] = s;
   else if (f32)
@@ -552,7 +599,8 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 
 // dx row rows[off + i] = row i of the sliced product dz W, in bf16. With one answer per row (K = 1) its column of dz
 // carries most of the row, and what its rounding to bf16 took away (val - bf16(val)) W[target] is given back, so that
-// dx is rounded once; among many answers no single rounding stands out. One warp per row.
+// dx is rounded once; among many answers no single rounding stands out. One warp per row and 256
+// columns.
 __global__ void __launch_bounds__(256)
     vocab_dx_kernel(const float* __restrict__ out, long ldo, const float* __restrict__ slabs, int bm, int bn, int grid,
                     const int* __restrict__ rows, const int* __restrict__ count, long off, long n, long V, long D,
@@ -573,32 +621,32 @@ __global__ void __launch_bounds__(256)
     wr = w + (long)in.col[i] * ldw;
   }
   const bool wvec = ((uintptr_t)w & 15) == 0 && ldw % 8 == 0;
-  for (long c = lane * 8; c < D; c += 256) {
-    float v[8];
-    slice_sum8(shape, out, ldo, slabs, bm, bn, i, (int)c, v);
-    if (rest != 0.f) {
-      if (wvec && c + 8 <= D) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(wr + c));
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+  const long c = (long)blockIdx.y * 256 + lane * 8;
+  if (c >= D) return;
+  float v[8];
+  slice_sum8(shape, out, ldo, slabs, bm, bn, i, (int)c, v);
+  if (rest != 0.f) {
+    if (wvec && c + 8 <= D) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(wr + c));
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float2 f = __bfloat1622float2(h[j]);
-          v[2 * j] = __fmaf_rn(rest, f.x, v[2 * j]);
-          v[2 * j + 1] = __fmaf_rn(rest, f.y, v[2 * j + 1]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          if (c + j < D) v[j] = __fmaf_rn(rest, __bfloat162float(wr[c + j]), v[j]);
+      for (int j = 0; j < 4; j++) {
+        const float2 f = __bfloat1622float2(h[j]);
+        v[2 * j] = __fmaf_rn(rest, f.x, v[2 * j]);
+        v[2 * j + 1] = __fmaf_rn(rest, f.y, v[2 * j + 1]);
       }
-    }
-    if (vec) {
-      *reinterpret_cast<uint4*>(d + c) = pack8(v);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        if (c + j < D) d[c + j] = __float2bfloat16_rn(v[j]);
+        if (c + j < D) v[j] = __fmaf_rn(rest, __bfloat162float(wr[c + j]), v[j]);
     }
+  }
+  if (vec) {
+    *reinterpret_cast<uint4*>(d + c) = pack8(v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (c + j < D) d[c + j] = __float2bfloat16_rn(v[j]);
   }
 }
 
@@ -658,6 +706,7 @@ constexpr size_t kVocabMaxK = 512;  // entries of a row: its lists stay in share
 struct VocabPlan {
   bool compact, pack_x, pack_w;
   bool dw_slice;   // dW by a sliced product
+  bool dw_copy;    // dW in padded rows, then copied to the caller's
   long Dp;         // row stride of the packed matrices and of the f32 products
   long ldt;        // row stride of the terms
   int bn;          // column tile of the logits product
@@ -679,9 +728,9 @@ static size_t carve(size_t& at, size_t bytes) {
 }
 
 // K = 0: cross entropy. x_ok, w_ok: the matrix starts at 16 bytes and its row stride is a multiple of 8 (what TMA
-// needs); w_lines: the same for 128 bytes and 64.
+// needs); w_lines: the same for 128 bytes and 64. dw_copy: the bf16 weight gradient cannot be written by TMA.
 static VocabPlan vocab_plan(long N, long V, long D, long K, bool bias, bool grad, bool x_ok, bool w_ok, bool w_lines,
-                            size_t piece_bytes, int sms) {
+                            bool dw_copy, size_t piece_bytes, int sms) {
   VocabPlan p{};
   const long k1 = K ? K : 1;
   p.compact = N > kVocabOneTile;
@@ -731,8 +780,9 @@ static VocabPlan vocab_plan(long N, long V, long D, long K, bool bias, bool grad
     p.col = carve(at, (size_t)p.R * k1 * 4);
     p.val = carve(at, (size_t)p.R * k1 * 4);
     p.dxs = carve(at, (size_t)p.R * p.Dp * 4);
-    p.slabs = carve(at, (size_t)sms * 128 * p.bd * 4);
-    if (p.dw_slice) p.dws = carve(at, (size_t)V * p.Dp * 4);
+    p.slabs = carve(at, (size_t)kSliceSlabs * sms * 128 * p.bd * 4);
+    p.dw_copy = dw_copy && !p.dw_slice && p.pieces == 1;
+    if (p.dw_slice || p.dw_copy) p.dws = carve(at, (size_t)V * p.Dp * (p.dw_slice ? 4 : 2));
     if (p.pieces > 1) p.dwacc = carve(at, (size_t)V * p.Dp * 4);
     if (bias) {
       p.part = carve(at, (size_t)(p.R / p.rpb) * V * 4);
@@ -818,7 +868,8 @@ static int vocab_run(const VocabCall& c) {
   }
   const int sms = gemm_sms();
   const VocabPlan p = vocab_plan(N, V, D, K, c.bias != nullptr, c.grad, rows16(c.x, c.ldx), rows16(c.w, c.ldw),
-                                 rows128(c.w, c.ldw), c.piece_bytes, sms);
+                                 rows128(c.w, c.ldw), c.grad && !c.dw_f32 && !rows16(c.dw, c.lddw),
+                                 c.piece_bytes, sms);
   PL_REQUIRE(c.ws && c.ws_bytes >= p.bytes && ((uintptr_t)c.ws & 255) == 0, PL_ERR_INVALID,
              "%s: %zu bytes of workspace (256-byte aligned), %zu needed", c.what, c.ws ? c.ws_bytes : (size_t)0, p.bytes);
   uint8_t* ws = (uint8_t*)c.ws;
@@ -846,7 +897,7 @@ static int vocab_run(const VocabCall& c) {
   long ldw = (long)c.ldw;
   if (p.pack_w) {
     __nv_bfloat16* wp = (__nv_bfloat16*)(ws + p.wp);
-    vocab_pack_kernel<<<(unsigned)ceil_div(round_up(V, 64), 8), 256, 0, st>>>(w, ldw, D, Answers{}, nullptr, nullptr, 0, V,
+    vocab_pack_kernel<<<dim3((unsigned)ceil_div(round_up(V, 64), 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(w, ldw, D, Answers{}, nullptr, nullptr, 0, V,
                                                                              wp, p.Dp);
     count_launch();
     PL_LAUNCH("vocab_pack_kernel");
@@ -859,7 +910,7 @@ static int vocab_run(const VocabCall& c) {
     long ldx = (long)c.ldx;
     if (p.pack_x) {
       __nv_bfloat16* xp = (__nv_bfloat16*)(ws + p.xp);
-      vocab_pack_kernel<<<(unsigned)ceil_div(round_up(n, 64), 8), 256, 0, st>>>(x, ldx, D, a, rows, count, off, n, xp,
+      vocab_pack_kernel<<<dim3((unsigned)ceil_div(round_up(n, 64), 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(x, ldx, D, a, rows, count, off, n, xp,
                                                                                p.Dp);
       count_launch();
       PL_LAUNCH("vocab_pack_kernel");
@@ -874,7 +925,12 @@ static int vocab_run(const VocabCall& c) {
       e.ldo = p.ldt;
       e.out_rows = (int)n;
       e.out_cols = (int)V;
-      e.scale2 = scale2;
+      // The tensor core's accumulator truncates: over steps of 16 products a logit loses on average D 2^-30 of itself
+      // (measured over D = 64 .. 8,192, hidden states that lean towards the weight row or not: 0.9 .. 1.0e-9 D), which
+      // at D = 4,096 is 4e-6, many times what rounding to nearest would leave. The scale gives that back; what remains
+      // is 2e-7 .. 7e-7.
+      e.scale2 = (float)((double)kLog2e / c.temperature * (1.0 + (double)D / (1 << 30)));
+      e.bias_scale2 = scale2;
       e.vbias = bias;
       e.stat = (float2*)(ws + p.stat);
       e.ld_stat = p.ld_stat;
@@ -910,7 +966,7 @@ static int vocab_run(const VocabCall& c) {
     rc = dz(p, ws, V, k1, count, off, n, ro, part, st);
     if (rc) return rc;
     if (bias) {
-      vocab_dbias_kernel<<<(unsigned)ceil_div(V, 256), 256, 0, st>>>(part, (int)(round_up(n, 64) / p.rpb), V,
+      vocab_dbias_kernel<<<(unsigned)ceil_div(V, 32), 1024, 0, st>>>(part, (int)(round_up(n, 64) / p.rpb), V,
                                                                     (float*)(ws + p.dbacc), q == 0, last, c.dw_f32,
                                                                     c.dbias);
       count_launch();
@@ -930,7 +986,7 @@ static int vocab_run(const VocabCall& c) {
       rc = gemm_launch(p.bd, EPI_SLICE, false, true, Z, W, (int)n, (int)D, (int)V, 1, g, st);
       if (rc) return rc;
       const bool pairs = gemm_paired(p.bd, EPI_SLICE, false, true, (int)n);
-      vocab_dx_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>((const float*)(ws + p.dxs), p.Dp, slabs, pairs ? 256 : 128,
+      vocab_dx_kernel<<<dim3((unsigned)ceil_div(n, 8), (unsigned)ceil_div(D, 256)), 256, 0, st>>>((const float*)(ws + p.dxs), p.Dp, slabs, pairs ? 256 : 128,
                                                                p.bd, pairs ? sms / 2 : sms, rows, count, off, n, V,
                                                                D, (int)k1, ro, w, ldw, (__nv_bfloat16*)c.dx, (long)c.lddx);
       count_launch();
@@ -945,16 +1001,23 @@ static int vocab_run(const VocabCall& c) {
       g.dyn_off = (int)off;
       g.dyn_k = 1;
       const bool direct = !p.dw_slice && (p.pieces == 1 || c.dw_f32);
+      const bool via = direct && p.dw_copy;  // in bf16 rows that TMA can write, then copied
       float* acc = (float*)(ws + p.dwacc);
       const int epi = p.dw_slice ? EPI_SLICE : (direct && !c.dw_f32 ? EPI_BF16 : EPI_F32);
-      g.out = p.dw_slice ? (void*)(ws + p.dws) : (direct ? c.dw : (void*)acc);
-      g.ldo = direct ? (long)c.lddw : p.Dp;
+      g.out = p.dw_slice || via ? (void*)(ws + p.dws) : (direct ? c.dw : (void*)acc);
+      g.ldo = direct && !via ? (long)c.lddw : p.Dp;
       g.slabs = slabs;
       g.accum = !p.dw_slice && q > 0;
       const Operand Xk{x, n, D, ldx, 1, 0};
       const Operand Zk{ws + p.terms, n, V, p.ldt, 1, 0};
       rc = gemm_launch(p.bd, epi, true, true, Zk, Xk, (int)V, (int)D, (int)n, 1, g, st);
       if (rc) return rc;
+      if (via) {
+        vocab_copy_kernel<<<dim3((unsigned)ceil_div(V, 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(
+            (const __nv_bfloat16*)(ws + p.dws), p.Dp, V, D, (__nv_bfloat16*)c.dw, (long)c.lddw);
+        count_launch();
+        PL_LAUNCH("vocab_copy_kernel");
+      }
       if (!direct && (p.dw_slice || last)) {
         const bool pairs = gemm_paired(p.bd, EPI_SLICE, true, true, (int)V);
         vocab_dw_kernel<<<dim3((unsigned)ceil_div(V, 8), (unsigned)ceil_div(D, 256)), 256, 0, st>>>(
@@ -977,7 +1040,7 @@ size_t pl_vocab_ws(size_t N, size_t V, size_t D, size_t K, uint8_t bias, uint8_t
                    size_t piece_bytes) {
   if (N == 0 || V == 0 || D == 0) return 0;
   const bool ok = aligned != 0;
-  return pl::vocab_plan((long)N, (long)V, (long)D, (long)K, bias != 0, grad != 0, ok, ok, ok, piece_bytes,
+  return pl::vocab_plan((long)N, (long)V, (long)D, (long)K, bias != 0, grad != 0, ok, ok, ok, !ok, piece_bytes,
                         pl::gemm_sms())
       .bytes;
 }

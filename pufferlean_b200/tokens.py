@@ -148,7 +148,7 @@ def _head(what, x, w, bias, ids, teacher, temperature, row_scale, grad, dw_f32=F
         ip = _vector(ids, what, "target", _I32, (n,), dev)
     sp = None if row_scale is None else _vector(row_scale, what, "row_scale", _F32, (n,), dev)
     L = lib()
-    aligned = ldx % 8 == 0 and ldw % 64 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 128 == 0
+    aligned = d % 8 == 0 and ldx % 8 == 0 and ldw % 64 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 128 == 0
     loss = torch.empty(n, dtype=_F32, device=dev)
     lse = torch.empty(n, dtype=_F32, device=dev)
     dx = dw = db = None
