@@ -60,6 +60,11 @@ def _vector(t, what, name, dtype, shape, device):
     raise PufferError(f"{what}: {name} must be contiguous")
 
 
+def _like(t):
+    """A new contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _enter(device):
     """Makes a tensor's device the library's for this call; returns (torch's device to go back to or None, the stream
     torch is on there). The checks above and this run on every call: a small call costs little more than they do."""
@@ -83,9 +88,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     dev, dtype = x.device, x.dtype
     wp = None if weight is None else _vector(weight, what, "weight", _F32, (cols,), dev)
     bp = None if bias is None else _vector(bias, what, "bias", _F32, (cols,), dev)
-    y = torch.empty((rows, cols), dtype=dtype, device=dev)
+    y = _like(x)
     mean = torch.empty(rows, dtype=_F32, device=dev)
-    rstd = torch.empty(rows, dtype=_F32, device=dev)
+    rstd = torch.empty_like(mean)
     was, st = _enter(dev)
     rc = lib().pl_layernorm_dev(x.data_ptr(), ldx, wp, bp, rows, cols, eps, dtype is _BF16, y.data_ptr(), cols,
                                 mean.data_ptr(), rstd.data_ptr(), st)
@@ -107,12 +112,12 @@ def layer_norm_grad(dy, x, weight, mean, rstd, params=True):
     _need(mean is not None and rstd is not None, what, "mean and rstd are needed")
     mp = _vector(mean, what, "mean", _F32, (rows,), dev)
     rp = _vector(rstd, what, "rstd", _F32, (rows,), dev)
-    dx = torch.empty((rows, cols), dtype=dtype, device=dev)
+    dx = _like(x)
     dw = db = dwp = dbp = wsp = None
     size = 0
     if params:
         dw = torch.empty(cols, dtype=_F32, device=dev)
-        db = torch.empty(cols, dtype=_F32, device=dev)
+        db = torch.empty_like(dw)
         size = lib().pl_layernorm_grad_ws(rows, cols)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         dwp, dbp, wsp = dw.data_ptr(), db.data_ptr(), ws.data_ptr()
@@ -150,12 +155,12 @@ def _head(what, x, w, bias, ids, teacher, temperature, row_scale, grad, dw_f32=F
     L = lib()
     aligned = d % 8 == 0 and ldx % 8 == 0 and ldw % 64 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 128 == 0
     loss = torch.empty(n, dtype=_F32, device=dev)
-    lse = torch.empty(n, dtype=_F32, device=dev)
+    lse = torch.empty_like(loss)
     dx = dw = db = None
     if grad:
-        dx = torch.empty((n, d), dtype=_BF16, device=dev)
-        dw = torch.empty((v, d), dtype=_F32 if dw_f32 else _BF16, device=dev)
-        db = torch.empty(v, dtype=dw.dtype, device=dev) if bias is not None else None
+        dx = _like(x)
+        dw = torch.empty((v, d), dtype=_F32, device=dev) if dw_f32 else _like(w)
+        db = torch.empty_like(bias, dtype=dw.dtype) if bias is not None else None
     size = L.pl_vocab_ws(n, v, d, k, bias is not None, grad, aligned, piece_bytes)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     head = (x.data_ptr(), ldx, w.data_ptr(), ldw, bp, ip)
