@@ -1162,6 +1162,10 @@ def main():
     if args.impl == "reference":
         if rank != 0:
             return 0
+        if args.workload == "c1" and not os.path.exists(os.path.join(ROOT, "oracle", "_ref", "libref_cpu.so")):
+            print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref/libref_cpu.so was not built: the "
+                              "reference's C sources are not on this machine"}), flush=True)
+            return 0
         if args.workload == "c1":
             base = reference_c1(wl, max(1, args.steps), min(args.warmup, 1))
         else:

@@ -44,9 +44,9 @@ def build():
 
 def reference_dir():
     """The reference checkout: $PL_REFERENCE_DIR, else a directory named `reference` beside this
-    repository; None when neither exists (the GPU box, which uses the prebuilt oracle/_ref files)."""
+    repository; None when neither holds its C sources (the GPU box, which uses the prebuilt oracle/_ref files)."""
     cand = os.environ.get("PL_REFERENCE_DIR") or os.path.join(os.path.dirname(os.path.dirname(HERE)), "reference")
-    return cand if os.path.isdir(cand) else None
+    return cand if os.path.isfile(os.path.join(cand, "ffi", "pufferffi.c")) else None
 
 
 def orc():
