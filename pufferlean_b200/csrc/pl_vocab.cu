@@ -153,24 +153,53 @@ __global__ void __launch_bounds__(1024)
   if (threadIdx.x == 0) *count = base;
 }
 
-// A warp's part [c0, c1) of a row (c0 a multiple of 1,024): 16 bytes to a lane where both rows start at 16 bytes.
-__device__ __forceinline__ void copy_row(__nv_bfloat16* __restrict__ d, const __nv_bfloat16* __restrict__ s, long c0, long c1,
-                                         bool in, bool vec, int lane) {
-  const __nv_bfloat16 zero = __float2bfloat16_rn(0.f);
-  long c = c0;
-  if (vec) {
+// Eight values at s, which need not be aligned: from the two 16-byte words that hold them. Reads the seven values
+// before s and after s + 8 at most.
+__device__ __forceinline__ uint4 load8_any(const __nv_bfloat16* s) {
+  const uint32_t sh = (uint32_t)((uintptr_t)s & 15);
+  const uint4* p = reinterpret_cast<const uint4*>((uintptr_t)s - sh);
+  const uint4 a = p[0];
+  if (sh == 0) return a;
+  const uint4 b = p[1];
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const uint32_t q = sh >> 2, bits = (sh & 3) * 8;
+  uint32_t u[5];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const long at = c0 + 256 * k + lane * 8;
-      if (at + 8 <= c1)
-        *reinterpret_cast<uint4*>(d + at) = in ? *reinterpret_cast<const uint4*>(s + at) : make_uint4(0, 0, 0, 0);
+  for (int j = 0; j < 5; j++)
+    u[j] = q == 0 ? w[j] : (q == 1 ? w[j + 1] : (q == 2 ? w[j + 2] : w[j + 3 < 8 ? j + 3 : 7]));
+  return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits),
+                    __funnelshift_r(u[2], u[3], bits), __funnelshift_r(u[3], u[4], bits));
+}
+
+// A warp's part of a row: values [c0, c0 + 1,024) of D, of any alignment on either side; zeros if not `in`. The middle
+// goes 16 bytes to a lane, aligned where it is written.
+__device__ __forceinline__ void copy_row(__nv_bfloat16* __restrict__ d, const __nv_bfloat16* __restrict__ s, long c0, long D,
+                                         bool in, int lane) {
+  const __nv_bfloat16 zero = __float2bfloat16_rn(0.f);
+  const long c1 = min(D, c0 + 1024);
+  const long head = min(c1, c0 + (long)((16 - ((uintptr_t)(d + c0) & 15)) & 15) / 2);  // first aligned value
+  const bool same = (((uintptr_t)d ^ (uintptr_t)s) & 15) == 0;
+  if (c0 + lane < head) d[c0 + lane] = in ? s[c0 + lane] : zero;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const long c = head + 256 * k + lane * 8;
+    if (c + 8 <= c1) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (in) {
+        if (same || (c >= 7 && c + 15 <= D)) {
+          v = load8_any(s + c);
+        } else {  // the row's ends, value by value
+          __align__(16) __nv_bfloat16 t[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) t[j] = s[c + j];
+          v = *reinterpret_cast<const uint4*>(t);
+        }
+      }
+      *reinterpret_cast<uint4*>(d + c) = v;
     }
-    c = c0 + (c1 - c0) / 8 * 8;
-    if (c + lane < c1) d[c + lane] = in ? s[c + lane] : zero;
-  } else {
-#pragma unroll 16
-    for (c += lane; c < c1; c += 32) d[c] = in ? s[c] : zero;
   }
+  const long tail = head + (c1 - head) / 8 * 8 + lane;
+  if (tail < c1) d[tail] = in ? s[tail] : zero;
 }
 
 // dst[i] = src[row i] for i < n (row i = rows[off + i] of the plan, or i itself without one; the row is zero where
@@ -190,8 +219,7 @@ __global__ void __launch_bounds__(256)
     else
       in = row_counts(a, r);
   }
-  const long c0 = (long)blockIdx.y * 1024, c1 = min(D, c0 + 1024);
-  copy_row(dst + i * ldd, src + r * ld, c0, c1, in, ((uintptr_t)src & 15) == 0 && ld % 8 == 0, lane);
+  copy_row(dst + i * ldd, src + r * ld, (long)blockIdx.y * 1024, D, in, lane);
 }
 
 // dst = src, rows of D values: a gradient that TMA could not write where the caller wants it.
@@ -200,8 +228,7 @@ __global__ void __launch_bounds__(256)
                       long ldd) {
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (i >= n) return;
-  const long c0 = (long)blockIdx.y * 1024, c1 = min(D, c0 + 1024);
-  copy_row(dst + i * ldd, src + i * ld, c0, c1, true, false, threadIdx.x & 31);
+  copy_row(dst + i * ldd, src + i * ld, (long)blockIdx.y * 1024, D, true, threadIdx.x & 31);
 }
 
 // The row's lse in log2 units from its segments' (max, sum); a fixed order over the threads t of `threads`.
@@ -319,6 +346,13 @@ __global__ void __launch_bounds__(128)
     for (int j = 0; j < 4; j++) {
       id[j] = k0 + j < K ? ids2[r * K + k0 + j] : -1;
       wr[j] = w + (id[j] >= 0 && id[j] < V ? (long)id[j] : 0L) * ldw;  // absent entries read row 0, to no effect
+    }
+    if ((id[0] & id[1] & id[2] & id[3]) < 0) {  // four absent entries
+      if (o.info && lane < 4 && k0 + lane < K) {
+        o.col[i * K + k0 + lane] = -1;
+        o.val[i * K + k0 + lane] = 0.f;
+      }
+      continue;
     }
     float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
