@@ -156,6 +156,9 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
     PL_REQUIRE(batch == 1 && ep.k_splits <= 1 && ep.slabs && (((uintptr_t)ep.out | (uintptr_t)ep.slabs) & 31) == 0 &&
                    ep.ldo % 8 == 0 && ep.ldo >= ep.out_cols,
                PL_ERR_INVALID, "a sliced product needs slabs and 32-byte rows (ldo = %ld)", ep.ldo);
+  if (epi == EPI_DIRECT)
+    PL_REQUIRE(batch == 1 && ep.k_splits <= 1 && ((uintptr_t)ep.out & 31) == 0 && ep.ldo % 16 == 0, PL_ERR_INVALID,
+               "a product written directly needs 32-byte rows (ldo = %ld)", ep.ldo);
   if (epi == EPI_VOCAB && ep.out)
     PL_REQUIRE(((uintptr_t)ep.out & 31) == 0 && ep.ldo % 64 == 0 && ep.ldo >= ep.out_cols, PL_ERR_INVALID,
                "the head's terms need 32-byte rows (ldo = %ld)", ep.ldo);

@@ -28,6 +28,7 @@ enum EpiKind : int {
   EPI_PPO = 4,    // logits+value = acc + bias -> PPO objective gradient dOut(bf16) + column sums
   EPI_VOCAB = 5,  // u = acc * scale2 + bias2 (log2 units) -> per row and BN/2 columns: max, sum of 2^(u - max);
                   // optionally out(f16) = 2^(u - max + 15)  [large-vocabulary heads]
+  EPI_DIRECT = 7,  // out(bf16) = acc, written from registers in 32-byte pieces  [wide outputs of short products]
   EPI_SLICE = 6,  // out(f32) = acc; the tiles of an incomplete last wave are split along K (SliceShape)
 };
 
@@ -625,6 +626,45 @@ __device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, const VocabPre
         make_float2(top, ((sum[0] + sum[1]) + (sum[2] + sum[3])) * (1.f / 32768.f));
 }
 
+// EPI_DIRECT: this warp's 32 rows x BN/2 columns as bf16, a lane's row in 32-byte pieces (rows of out start at 32
+// bytes). Nothing waits for shared memory, so a product of few k-blocks runs at the rate of its writes.
+template <int BN>
+__device__ __forceinline__ void epilogue_direct(const EpiArgs& ep, uint32_t t_row, int m_tile, int n_tile, int rows,
+                                                bool have_acc, int sub, int half, int lane) {
+  constexpr int W = BN / 2, NQ = W / 16;
+  const int row = m_tile * 128 + sub * 32 + lane, n0 = n_tile * BN + half * W;
+  const int left = ep.out_cols - n0;
+  if (m_tile * 128 + sub * 32 >= rows || left <= 0) return;  // warp-uniform
+  uint32_t r[NQ][16];
+#pragma unroll
+  for (int q = 0; q < NQ; q++) tc::tmem_ld16(t_row + half * W + 16 * q, r[q]);
+  tc::tmem_wait_ld();
+#pragma unroll
+  for (int q = 0; q < NQ; q++) tc::tmem_tie16(r[q]);
+  if (row >= rows) return;
+  __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(ep.out) + (long)row * ep.ldo + n0;
+#pragma unroll
+  for (int q = 0; q < NQ; q++) {
+    if (16 * q >= left) break;
+    uint32_t u[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[q][2 * j]), __uint_as_float(r[q][2 * j + 1]));
+      u[j] = have_acc ? *reinterpret_cast<const uint32_t*>(&h) : 0u;
+    }
+    if (16 * q + 16 <= left) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at + 16 * q), "r"(u[0]), "r"(u[1]),
+                   "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                   : "memory");
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (16 * q + j < left)
+          at[16 * q + j] = __ushort_as_bfloat16((unsigned short)(u[j / 2] >> (16 * (j & 1)) & 0xffffu));
+    }
+  }
+}
+
 // EPI_SLICE: this warp's 32 rows x BN/2 columns to out, or to the slabs from row slab_row on (>= 0); a lane writes its row in 32-byte
 // pieces (out's rows are padded to a multiple of 8 columns).
 template <int BN>
@@ -659,9 +699,9 @@ __device__ __forceinline__ void epilogue_slice(const EpiArgs& ep, uint32_t t_row
 }
 
 // Eight values of row `row` at columns [col, col + 8) of a product that EPI_SLICE left in out and slabs (its tile
-// is bm x bn).
+// is bm x bn): the sum of the slices z0, z0 + dz, ... (0 and 1: all of them).
 __device__ __forceinline__ void slice_sum8(const SliceShape& s, const float* out, long ldo, const float* slabs, int bm,
-                                           int bn, long row, int col, float (&v)[8]) {
+                                           int bn, long row, int col, float (&v)[8], int z0, int dz) {
   const int nt = col / bn;
   const long mt = row / bm, t = mt * s.num_n + nt;
   const bool whole = t < s.full || s.q == 1;
@@ -670,8 +710,9 @@ __device__ __forceinline__ void slice_sum8(const SliceShape& s, const float* out
 #pragma unroll
   for (int j = 0; j < 8; j++) v[j] = 0.f;
 #pragma unroll 4
-  for (int z = 0; z < parts; z++, p += (long)s.rem * bm * bn) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  for (int z = z0; z < parts; z += dz) {
+    const float* at = p + (long)z * s.rem * bm * bn;
+    const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 4);
     v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
   }
 }
@@ -1361,7 +1402,9 @@ __global__ void __launch_bounds__(320, 1)
       }
       tc::tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t)(buf * BN) + ((uint32_t)(sub * 32) << 16);
-      if constexpr (EPI == EPI_SLICE)
+      if constexpr (EPI == EPI_DIRECT)
+        epilogue_direct<BN>(ep, t_row, ti.m, ti.n, M, b1 > b0, sub, half, lane);
+      else if constexpr (EPI == EPI_SLICE)
         epilogue_slice<BN>(ep, t_row, ti.m, ti.n, M, walk.slab < 0 ? -1 : walk.slab * BM, b1 > b0, sub, half, lane);
       else if constexpr (EPI == EPI_VOCAB)
         epilogue_vocab<BN>(ep, pre, t_row, ti.m, ti.n, M, sub, half, lane, red + (warp - 2) * (BN / 2));
@@ -1587,7 +1630,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
       // a 128-row block wholly past M (odd CTA, M not a multiple of 256) has nothing to write: its
       // column partials would fall outside the ceil(M / 128) rows the caller provides
       if (m_blk * BM >= M) {
-      } else if constexpr (EPI == EPI_VOCAB)
+      } else if constexpr (EPI == EPI_DIRECT)
+        epilogue_direct<BN>(ep, t_row, m_blk, ti.n, M, b1 > b0, sub, half, lane);
+      else if constexpr (EPI == EPI_VOCAB)
         epilogue_vocab<BN>(ep, pre, t_row, m_blk, ti.n, M, sub, half, lane, red + (warp - 2) * (BN / 2));
       else if constexpr (EPI == EPI_SLICE)
         epilogue_slice<BN>(ep, t_row, m_blk, ti.n, M, walk.slab < 0 ? -1 : (walk.slab * 2 + rank) * BM, b1 > b0, sub, half,
@@ -1631,7 +1676,7 @@ bool gemm_store_map(CUtensorMap* map, const void* ptr, long rows, long cols, lon
 int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const Operand& B, int M, int N, int K,
                 int batch, const EpiArgs& ep, cudaStream_t st);
 // 0 = single-CTA tiles only, 1 = CTA pairs where eligible, 2 = CTA pairs for the products whose two
-// operands are MN-major (the weight gradients; the default); a negative mode only queries. Returns the
+// operands are MN-major (the weight gradients) and the large-vocabulary head's (the default); a negative mode only queries. Returns the
 // previous mode.
 int gemm_set_pair_mode(int mode);
 // SMs of the current device. An EPI_SLICE launch runs on all of them: one CTA each with 128-row tiles, or (gemm_paired)

@@ -40,6 +40,8 @@ GemmKernel gemm_instance(int bn, int epi, bool a_mn, bool b_mn, uint32_t* smem) 
   PL_INST(256, false, false, EPI_VOCAB)
   PL_INST(128, true, true, EPI_BF16)
   PL_INST(256, true, true, EPI_BF16)
+  PL_INST(128, true, true, EPI_DIRECT)
+  PL_INST(256, true, true, EPI_DIRECT)
   PL_INST(128, false, true, EPI_SLICE)
   PL_INST(256, false, true, EPI_SLICE)
   PL_INST(128, true, true, EPI_SLICE)

@@ -27,6 +27,7 @@ GemmKernel gemm_pair_instance(int bn, int epi, bool a_mn, bool b_mn, uint32_t* s
   PL_INST_PAIR(256, false, false, EPI_VOCAB)
   PL_INST_PAIR(256, false, true, EPI_SLICE)
   PL_INST_PAIR(256, true, true, EPI_SLICE)
+  PL_INST_PAIR(256, true, true, EPI_DIRECT)
   return nullptr;
 }
 

@@ -9,10 +9,15 @@
 // Rows without an answer (a negative target, no entry present) are taken out before the products: a plan kernel
 // lists the rows that count, the products' row extent is read from the device. One product gives the logits: its
 // epilogue (pl_gemm.cuh, EPI_VOCAB) folds each row's 128 columns to (max, sum) and, when gradients are wanted,
-// leaves 2^(u - max) in f16 in a buffer of as many rows as the workspace allows. Once the row's statistics are
-// known these terms become dz in place (bf16, the one rounding of the gradient), and two more products give dx
-// and dW. Three products of 2 N V D flops is also the least that the gradients need; recomputing the logits
-// instead of keeping the terms would make it four.
+// leaves 2^(u - max) in f16 for a piece of the rows. Once the rows' statistics are known these terms become dz in
+// place (bf16, the one rounding of the gradient), and two more products give dx and dW. Three products of 2 N V D
+// flops are also the least that the gradients need; recomputing the logits instead of keeping the terms would make it
+// four.
+//
+// What bounds it: the three products run at the rate of the tensor cores under the power cap (16,384 x 131,072 x 2,048:
+// 23.0 ms for 26.4 TFLOP on a board whose cuBLAS does 1,390 TFLOP/s for seconds, 19.0 ms of products at that rate); the
+// pass from terms to gradients at HBM's (2,048 x 131,072: 162 us for 1.07 GB); with few rows the reading of W and the
+// writing of dW; with few rows of a small vocabulary the launches.
 #include <cuda_fp16.h>
 
 #include "pl_common.cuh"
@@ -52,17 +57,18 @@ __global__ void __launch_bounds__(128)
     vocab_teacher_kernel(const int* __restrict__ ids, const float* __restrict__ teacher, long N, int K, float tscale,
                          int* __restrict__ ids2, float* __restrict__ p, float* __restrict__ ent,
                          uint8_t* __restrict__ has) {
-  extern __shared__ uint8_t dyn_smem[];
+  extern __shared__ __align__(16) uint8_t dyn_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long r = (long)blockIdx.x * 4 + warp;
   if (r >= N) return;
-  int* id_s = reinterpret_cast<int*>(dyn_smem) + warp * 2 * K;
-  float* p_s = reinterpret_cast<float*>(id_s + K);
+  const int K4 = (K + 3) / 4 * 4;
+  int* id_s = reinterpret_cast<int*>(dyn_smem) + warp * 2 * K4;
+  float* p_s = reinterpret_cast<float*>(id_s + K4);
   float top = -INFINITY;
   bool any = false;
-  for (int k = lane; k < K; k += 32) {
-    int id = ids[r * K + k];
-    const float t = teacher[r * K + k];
+  for (int k = lane; k < K4; k += 32) {
+    int id = k < K ? ids[r * K + k] : -1;
+    const float t = k < K ? teacher[r * K + k] : -INFINITY;
     if (t == -INFINITY) id = -1;
     id_s[k] = id;
     p_s[k] = t;
@@ -79,7 +85,7 @@ __global__ void __launch_bounds__(128)
   tot = warp_sum_f(tot);
   const float log_tot = log2f(tot);
   float e = 0.f;
-  for (int k = lane; k < K; k += 32) {
+  for (int k = lane; k < K4; k += 32) {
     float q = 0.f;
     if (id_s[k] >= 0) {
       const float l = (p_s[k] - top) * tscale - log_tot;
@@ -92,11 +98,17 @@ __global__ void __launch_bounds__(128)
   __syncwarp();
   for (int k = lane; k < K; k += 32) {
     const int id = id_s[k];
-    float q = p_s[k];
+    float q = 0.f;
     bool first = id >= 0;
-    for (int g = 0; first && g < k; g++) first = id_s[g] != id;
-    if (first)
-      for (int g = k + 1; g < K; g++) q += id_s[g] == id ? p_s[g] : 0.f;
+#pragma unroll 2
+    for (int g = 0; g < K4; g += 4) {  // every entry of this id from k on; one before k makes it that one's
+      const int4 i4 = *reinterpret_cast<const int4*>(id_s + g);
+      const float4 p4 = *reinterpret_cast<const float4*>(p_s + g);
+      if (i4.x == id) q += p4.x, first = first && g >= k;
+      if (i4.y == id) q += p4.y, first = first && g + 1 >= k;
+      if (i4.z == id) q += p4.z, first = first && g + 2 >= k;
+      if (i4.w == id) q += p4.w, first = first && g + 3 >= k;
+    }
     ids2[r * K + k] = first ? id : -1;
     p[r * K + k] = first ? q : 0.f;
   }
@@ -203,10 +215,12 @@ __device__ __forceinline__ void copy_row(__nv_bfloat16* __restrict__ d, const __
 }
 
 // dst[i] = src[row i] for i < n (row i = rows[off + i] of the plan, or i itself without one; the row is zero where
-// it does not count), rows up to the next multiple of 64 zeroed. One warp per row and 1,024 columns.
+// it does not count), rows up to the next multiple of 64 zeroed; with `again` the same once more that many rows below.
+// One warp per row and 1,024 columns.
 __global__ void __launch_bounds__(256)
     vocab_pack_kernel(const __nv_bfloat16* __restrict__ src, long ld, long D, Answers a, const int* __restrict__ rows,
-                      const int* __restrict__ count, long off, long n, __nv_bfloat16* __restrict__ dst, long ldd) {
+                      const int* __restrict__ count, long off, long n, __nv_bfloat16* __restrict__ dst, long ldd,
+                      long again) {
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const long have = rows_here(count, off, n);
@@ -220,6 +234,7 @@ __global__ void __launch_bounds__(256)
       in = row_counts(a, r);
   }
   copy_row(dst + i * ldd, src + r * ld, (long)blockIdx.y * 1024, D, in, lane);
+  if (again) copy_row(dst + (i + again) * ldd, src + r * ld, (long)blockIdx.y * 1024, D, in, lane);
 }
 
 // dst = src, rows of D values: a gradient that TMA could not write where the caller wants it.
@@ -263,8 +278,84 @@ struct RowOut {
   float* val;
 };
 
-// Cross entropy, one warp per row: the target's logit comes from the product itself (ut), so that loss = lse - u
-// carries no difference between two ways of summing.
+// The logits of a row's answer entries, in log2 units: products of length D with gathered rows of W, summed in f32
+// (the f16 terms would not do for the loss). Four entries to a warp, so that each value of x read serves four, and
+// 16 to a block: rows with long lists are spread over blocks. Bound by the gathered rows, 2 D bytes an entry.
+__global__ void __launch_bounds__(128)
+    vocab_dots_kernel(const __nv_bfloat16* __restrict__ x, long ldx, const __nv_bfloat16* __restrict__ w, long ldw,
+                      const __nv_bfloat16* __restrict__ bias, long V, long D, int K, const int* __restrict__ ids2,
+                      float scale2, const int* __restrict__ rows, const int* __restrict__ count, long off,
+                      float* __restrict__ uk) {
+  const long i = blockIdx.x;
+  if (count && off + i >= *count) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long r = rows ? rows[off + i] : off + i;
+  const int k0 = (blockIdx.y * 4 + warp) * 4;
+  if (k0 >= K) return;
+  const __nv_bfloat16* xr = x + i * ldx;
+  const __nv_bfloat16* wr[4];
+  int id[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    id[j] = k0 + j < K ? ids2[r * K + k0 + j] : -1;
+    wr[j] = w + (id[j] >= 0 && id[j] < V ? (long)id[j] : 0L) * ldw;  // absent entries read row 0, to no effect
+  }
+  if ((id[0] & id[1] & id[2] & id[3]) < 0) return;
+  const bool vec = ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && ldx % 8 == 0 && ldw % 8 == 0;
+  const long Dv = vec ? D / 8 * 8 : 0;
+  float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (long c = lane * 8; c < Dv; c += 256) {
+    const uint4 xv = *reinterpret_cast<const uint4*>(xr + c);
+    uint4 wv[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) wv[j] = __ldg(reinterpret_cast<const uint4*>(wr[j] + c));
+    const __nv_bfloat162* xh = reinterpret_cast<const __nv_bfloat162*>(&xv);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const float2 f = __bfloat1622float2(xh[q]);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float2 g = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&wv[j])[q]);
+        d[j] = __fmaf_rn(f.x, g.x, d[j]);
+        d[j] = __fmaf_rn(f.y, g.y, d[j]);
+      }
+    }
+  }
+  for (long c = Dv + lane; c < D; c += 32) {
+    const float f = __bfloat162float(xr[c]);
+#pragma unroll
+    for (int j = 0; j < 4; j++) d[j] = __fmaf_rn(f, __bfloat162float(wr[j][c]), d[j]);
+  }
+  // the four sums in one butterfly: lane l ends with that of entry l / 8
+  const bool hi = lane & 16, hi2 = lane & 8;
+  const float a0 = (hi ? d[2] : d[0]) + __shfl_xor_sync(0xffffffffu, hi ? d[0] : d[2], 16);
+  const float a1 = (hi ? d[3] : d[1]) + __shfl_xor_sync(0xffffffffu, hi ? d[1] : d[3], 16);
+  float t = (hi2 ? a1 : a0) + __shfl_xor_sync(0xffffffffu, hi2 ? a0 : a1, 8);
+#pragma unroll
+  for (int o = 4; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  const int k = k0 + (lane >> 3);
+  if ((lane & 7) == 0 && k < K) {
+    const int c = ids2[r * K + k];
+    uk[i * K + k] = __fmaf_rn(t, scale2, bias && c >= 0 && c < V ? vocab_bias2(__bfloat162float(bias[c]), scale2) : 0.f);
+  }
+}
+
+// One warp per row: its lse from the segments, the loss, and what the gradient needs.
+__device__ __forceinline__ void row_without(long r, long i, int K, int lane, float* loss, float* lse, const RowOut& o) {
+  if (lane == 0) {
+    loss[r] = 0.f;
+    lse[r] = 0.f;
+    if (o.info) o.info[i] = make_float2(0.f, 0.f);
+  }
+  if (o.info)
+    for (int k = lane; k < K; k += 32) {
+      o.col[i * K + k] = -1;
+      o.val[i * K + k] = 0.f;
+    }
+}
+// Cross entropy: the target's logit comes from the product itself (ut), so that loss = lse - u carries no difference
+// between two ways of summing.
 __global__ void __launch_bounds__(256)
     vocab_ce_rows_kernel(const int* __restrict__ target, long V, const float* __restrict__ row_scale,
                          const int* __restrict__ rows, const int* __restrict__ count, long off, long n,
@@ -275,18 +366,9 @@ __global__ void __launch_bounds__(256)
   if (i >= rows_here(count, off, n)) return;
   const long r = rows ? rows[off + i] : off + i;
   const int t = target[r];
+  if (t < 0) return row_without(r, i, 1, lane, loss, lse, o);
   float lse2 = seg_lse(warp_join(seg_fold(stat + i * ld_stat, ld_stat, lane, 32)));
   if (lane) return;
-  if (t < 0) {
-    loss[r] = 0.f;
-    lse[r] = 0.f;
-    if (o.info) {
-      o.info[i] = make_float2(0.f, 0.f);
-      o.col[i] = -1;
-      o.val[i] = 0.f;
-    }
-    return;
-  }
   float u = 0.f;
   if (t >= V)
     lse2 = NAN;  // a target past the vocabulary: seen in the loss
@@ -301,117 +383,44 @@ __global__ void __launch_bounds__(256)
     o.val[i] = (exp2f(u - lse2) - 1.f) * scale;
   }
 }
-
-// Distillation, one block per row: the logits of the entries are products of length D with gathered rows of W, four
-// entries at a time per warp.
-__global__ void __launch_bounds__(128)
-    vocab_distill_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx, const __nv_bfloat16* __restrict__ w,
-                              long ldw, const __nv_bfloat16* __restrict__ bias, long V, long D, int K,
-                              const int* __restrict__ ids2, const float* __restrict__ p, const float* __restrict__ ent,
-                              const uint8_t* __restrict__ has, float scale2, float inv_t,
+// Distillation: ids2, p, ent of the teacher kernel, uk of the dots kernel.
+__global__ void __launch_bounds__(256)
+    vocab_distill_rows_kernel(long V, int K, const int* __restrict__ ids2, const float* __restrict__ p,
+                              const float* __restrict__ ent, const uint8_t* __restrict__ has, float inv_t,
                               const float* __restrict__ row_scale, const int* __restrict__ rows,
-                              const int* __restrict__ count, long off, const float2* __restrict__ stat, long ld_stat,
-                              float* __restrict__ loss, float* __restrict__ lse, RowOut o) {
-  __shared__ float2 seg_s[4];
-  __shared__ float acc_s[4];
-  __shared__ int bad_s[4];
-  const long i = blockIdx.x;
-  if (count && off + i >= *count) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+                              const int* __restrict__ count, long off, long n, const float2* __restrict__ stat,
+                              long ld_stat, const float* __restrict__ uk, float* __restrict__ loss,
+                              float* __restrict__ lse, RowOut o) {
+  const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (i >= rows_here(count, off, n)) return;
   const long r = rows ? rows[off + i] : off + i;
-  if (!rows && !has[r]) {
-    if (threadIdx.x == 0) {
-      loss[r] = 0.f;
-      lse[r] = 0.f;
-      if (o.info) o.info[i] = make_float2(0.f, 0.f);
-    }
-    if (o.info)
-      for (int k = threadIdx.x; k < K; k += 128) o.col[i * K + k] = -1;
-    return;
-  }
-  const float2 mine = warp_join(seg_fold(stat + i * ld_stat, ld_stat, threadIdx.x, 128));
-  if (lane == 0) seg_s[warp] = mine;
-  __syncthreads();
-  const float lse2 = seg_lse(seg_join(seg_join(seg_s[0], seg_s[1]), seg_join(seg_s[2], seg_s[3])));
+  if (!has[r]) return row_without(r, i, K, lane, loss, lse, o);
+  float lse2 = seg_lse(warp_join(seg_fold(stat + i * ld_stat, ld_stat, lane, 32)));
   const float scale = (row_scale ? row_scale[r] : 1.f) * inv_t;
-  const __nv_bfloat16* xr = x + i * ldx;
-  const bool vec = ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && ldx % 8 == 0 && ldw % 8 == 0;
-  const long Dv = vec ? D / 8 * 8 : 0;
   float acc = 0.f;
   bool bad = false;
-  for (int k0 = warp * 4; k0 < K; k0 += 16) {
-    const __nv_bfloat16* wr[4];
-    int id[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      id[j] = k0 + j < K ? ids2[r * K + k0 + j] : -1;
-      wr[j] = w + (id[j] >= 0 && id[j] < V ? (long)id[j] : 0L) * ldw;  // absent entries read row 0, to no effect
+  for (int k = lane; k < K; k += 32) {
+    const int c = ids2[r * K + k];
+    float val = 0.f;
+    if (c >= V) {
+      bad = true;
+    } else if (c >= 0) {
+      const float q = p[r * K + k], u = uk[i * K + k];
+      if (!(q == 0.f)) acc = __fmaf_rn(-q, u, acc);
+      val = (exp2f(u - lse2) - q) * scale;
     }
-    if ((id[0] & id[1] & id[2] & id[3]) < 0) {  // four absent entries
-      if (o.info && lane < 4 && k0 + lane < K) {
-        o.col[i * K + k0 + lane] = -1;
-        o.val[i * K + k0 + lane] = 0.f;
-      }
-      continue;
-    }
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-    for (long c = lane * 8; c < Dv; c += 256) {
-      const uint4 xv = *reinterpret_cast<const uint4*>(xr + c);
-      uint4 wv[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) wv[j] = __ldg(reinterpret_cast<const uint4*>(wr[j] + c));
-      const __nv_bfloat162* xh = reinterpret_cast<const __nv_bfloat162*>(&xv);
-#pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const float2 f = __bfloat1622float2(xh[q]);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float2 g = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&wv[j])[q]);
-          d[j] = __fmaf_rn(f.x, g.x, d[j]);
-          d[j] = __fmaf_rn(f.y, g.y, d[j]);
-        }
-      }
-    }
-    for (long c = Dv + lane; c < D; c += 32) {
-      const float f = __bfloat162float(xr[c]);
-#pragma unroll
-      for (int j = 0; j < 4; j++) d[j] = __fmaf_rn(f, __bfloat162float(wr[j][c]), d[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++) d[j] = warp_sum_f(d[j]);
-    // lane j finishes entry k0 + j
-    const float dot = lane == 0 ? d[0] : (lane == 1 ? d[1] : (lane == 2 ? d[2] : d[3]));
-    if (lane < 4 && k0 + lane < K) {
-      const int c = ids2[r * K + k0 + lane];
-      float val = 0.f;
-      if (c >= V) {
-        bad = true;
-      } else if (c >= 0) {
-        const float q = p[r * K + k0 + lane];
-        const float u = __fmaf_rn(dot, scale2, bias ? vocab_bias2(__bfloat162float(bias[c]), scale2) : 0.f);
-        if (!(q == 0.f)) acc = __fmaf_rn(-q, u, acc);
-        val = (exp2f(u - lse2) - q) * scale;
-      }
-      if (o.info) {
-        o.col[i * K + k0 + lane] = c;
-        o.val[i * K + k0 + lane] = val;
-      }
+    if (o.info) {
+      o.col[i * K + k] = c;
+      o.val[i * K + k] = val;
     }
   }
   acc = warp_sum_f(acc);
-  bad = __any_sync(0xffffffffu, bad);
+  if (__any_sync(0xffffffffu, bad)) lse2 = NAN;  // an id past the vocabulary: seen in the loss
   if (lane == 0) {
-    acc_s[warp] = acc;
-    bad_s[warp] = bad;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const bool any_bad = bad_s[0] | bad_s[1] | bad_s[2] | bad_s[3];  // an id past the vocabulary: seen in the loss
-    const float l2 = any_bad ? NAN : lse2;
-    loss[r] = (ent[r] + ((acc_s[0] + acc_s[1]) + (acc_s[2] + acc_s[3])) + l2) * kLn2;
-    lse[r] = l2 * kLn2;
-    if (o.info) o.info[i] = make_float2(l2, scale);
+    loss[r] = (ent[r] + acc + lse2) * kLn2;
+    lse[r] = lse2 * kLn2;
+    if (o.info) o.info[i] = make_float2(lse2, scale);
   }
 }
 
@@ -420,7 +429,8 @@ __global__ void __launch_bounds__(128)
 // 256. The block first lists the answer entries that fall into its tile (in an order that depends on nothing but the
 // entries) and marks them in a bit mask; the walk leaves marked columns out, and the listed values are written after
 // it. With `part` the column sums of the unrounded values go to part[row tile][V] for dbias. Rows from the count to
-// the next multiple of 64 are zeroed (the weight-gradient product reads whole k-blocks of rows).
+// the next multiple of 64 are zeroed (the weight-gradient product reads whole k-blocks of rows). With `lo` the rounding
+// errors go, in bf16 too, to the rows `lo` below.
 // Bound by HBM: 4 bytes per term.
 constexpr int kDzScan = 16;  // answer entries of a block: 256 kDzScan at most
 template <int NS>
@@ -433,7 +443,7 @@ struct DzSmem {
 template <int NS, bool PART>
 __global__ void __launch_bounds__(256, PART ? 3 : 4)
     vocab_dz_kernel(void* __restrict__ terms, long ld, long V, int K, const int* __restrict__ count, long off, long n,
-                    int rpb, RowOut in, const float2* __restrict__ stat, long ld_stat, int seg_shift,
+                    int rpb, long lo, RowOut in, const float2* __restrict__ stat, long ld_stat, int seg_shift,
                     float* __restrict__ part) {
   constexpr int COLS = 256 * NS;
   extern __shared__ __align__(16) uint8_t dyn_smem[];
@@ -543,13 +553,25 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
           }
         }
         at4[32 * s] = o;
+        if (lo) {  // what the rounding took away, `lo` rows below
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float2 h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[j]));
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[j].x - h.x, v[j].y - h.y);
+            u[j] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          *reinterpret_cast<uint4*>(base + (q + lo) * ld + 256 * s) = o;
+        }
       }
     }
   }
   for (long q = nr + warp; q < min((long)rpb, (have + 63) / 64 * 64 - r0); q += 8)
 #pragma unroll
     for (int s = 0; s < NS; s++)
-      if (256 * s < left) reinterpret_cast<uint4*>(base + q * ld)[32 * s] = make_uint4(0u, 0u, 0u, 0u);
+      if (256 * s < left) {
+        reinterpret_cast<uint4*>(base + q * ld)[32 * s] = make_uint4(0u, 0u, 0u, 0u);
+        if (lo) reinterpret_cast<uint4*>(base + (q + lo) * ld)[32 * s] = make_uint4(0u, 0u, 0u, 0u);
+      }
   if (PART) {
 #pragma unroll
     for (int s = 0; s < NS; s++)
@@ -560,8 +582,12 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
   }
   __syncthreads();
   uint16_t* tile = reinterpret_cast<uint16_t*>(terms) + r0 * ld + c0;
-  for (int h = threadIdx.x; h < hits; h += 256)
-    tile[(hit_at[h] >> 16) * ld + (hit_at[h] & 0xffffu)] = __bfloat16_as_ushort(__float2bfloat16_rn(hit_v[h]));
+  for (int h = threadIdx.x; h < hits; h += 256) {
+    uint16_t* at = tile + (hit_at[h] >> 16) * ld + (hit_at[h] & 0xffffu);
+    const __nv_bfloat16 b = __float2bfloat16_rn(hit_v[h]);
+    *at = __bfloat16_as_ushort(b);
+    if (lo) at[lo * ld] = __bfloat16_as_ushort(__float2bfloat16_rn(hit_v[h] - __bfloat162float(b)));
+  }
   if constexpr (PART) {
     // thread t owns the block's columns t, t + 256, ...
 #pragma unroll
@@ -631,34 +657,74 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return o;
 }
 
+// A lane's eight values of a sliced product at row `row` (plus, with `lo`, that many rows below), columns [c, c + 8). SPLIT: the block's warps share the
+// slices and warp 0 has the sums (added in a fixed order). False where the lane has nothing to write.
+template <bool SPLIT>
+__device__ __forceinline__ bool slices_of(const SliceShape& s, const float* out, long ldo, const float* slabs, int bm,
+                                          int bn, long row, long lo, long c, long D, float (&v)[8]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (!SPLIT) {
+    if (c >= D) return false;
+    slice_sum8(s, out, ldo, slabs, bm, bn, row, (int)c, v, 0, 1);
+    if (lo) {
+      float l[8];
+      slice_sum8(s, out, ldo, slabs, bm, bn, row + lo, (int)c, l, 0, 1);
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] += l[j];
+    }
+    return true;
+  } else {
+    __shared__ float part[8][256];
+    if (c < D) {
+      slice_sum8(s, out, ldo, slabs, bm, bn, row, (int)c, v, warp, 8);
+      if (lo) {
+        float l[8];
+        slice_sum8(s, out, ldo, slabs, bm, bn, row + lo, (int)c, l, warp, 8);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] += l[j];
+      }
+      *reinterpret_cast<float4*>(&part[warp][lane * 8]) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(&part[warp][lane * 8 + 4]) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    __syncthreads();
+    if (warp || c >= D) return false;
+#pragma unroll
+    for (int q = 1; q < 8; q++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] += part[q][lane * 8 + j];
+    return true;
+  }
+}
+
 // dx row rows[off + i] = row i of the sliced product dz W, in bf16. With one answer per row (K = 1) its column of dz
 // carries most of the row, and what its rounding to bf16 took away (val - bf16(val)) W[target] is given back, so that
-// dx is rounded once; among many answers no single rounding stands out. One warp per row and 256
-// columns.
+// dx is rounded once; among many answers no single rounding stands out. With `lo` the product's row lo + i holds what
+// dz's rounding took from row i. One warp per row and 256
+// columns, or (SPLIT, for many slices) one block, its warps taking every eighth slice.
+template <bool SPLIT>
 __global__ void __launch_bounds__(256)
     vocab_dx_kernel(const float* __restrict__ out, long ldo, const float* __restrict__ slabs, int bm, int bn, int grid,
                     const int* __restrict__ rows, const int* __restrict__ count, long off, long n, long V, long D,
-                    int K, RowOut in, const __nv_bfloat16* __restrict__ w, long ldw, __nv_bfloat16* __restrict__ dx,
-                    long lddx) {
-  const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+                    long lo, int K, RowOut in, const __nv_bfloat16* __restrict__ w, long ldw,
+                    __nv_bfloat16* __restrict__ dx, long lddx) {
+  const long i = SPLIT ? blockIdx.x : (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const long have = rows_here(count, off, n);
   if (i >= have) return;
-  const SliceShape shape = slice_shape((int)have, (int)D, (int)V, bm, bn, grid);
+  const SliceShape shape = slice_shape((int)(lo ? 2 * lo : have), (int)D, (int)V, bm, bn, grid);
   const long r = rows ? rows[off + i] : off + i;
   const bool vec = ((uintptr_t)dx & 15) == 0 && lddx % 8 == 0 && D % 8 == 0;
   __nv_bfloat16* d = dx + r * lddx;
   float rest = 0.f;
   const __nv_bfloat16* wr = w;
-  if (K == 1 && in.col[i] >= 0 && in.col[i] < V) {
+  if (K == 1 && !lo && in.col[i] >= 0 && in.col[i] < V) {
     rest = in.val[i] - __bfloat162float(__float2bfloat16_rn(in.val[i]));
     wr = w + (long)in.col[i] * ldw;
   }
   const bool wvec = ((uintptr_t)w & 15) == 0 && ldw % 8 == 0;
   const long c = (long)blockIdx.y * 256 + lane * 8;
-  if (c >= D) return;
   float v[8];
-  slice_sum8(shape, out, ldo, slabs, bm, bn, i, (int)c, v);
+  if (!slices_of<SPLIT>(shape, out, ldo, slabs, bm, bn, i, lo, c, D, v)) return;
   if (rest != 0.f) {
     if (wvec && c + 8 <= D) {
       const uint4 raw = __ldg(reinterpret_cast<const uint4*>(wr + c));
@@ -685,18 +751,22 @@ __global__ void __launch_bounds__(256)
 }
 
 // The weight gradient from f32: a sliced product's parts (slabs) or the sum of the pieces (slabs NULL, src = acc);
-// pieces before the last are kept in acc, the last goes to dw in the caller's type. One warp per row and 256 columns.
+// pieces before the last are kept in acc, the last goes to dw in the caller's type. One warp per row and 256 columns,
+// or one block (SPLIT).
+template <bool SPLIT>
 __global__ void __launch_bounds__(256)
     vocab_dw_kernel(const float* __restrict__ src, long lds, const float* __restrict__ slabs, int bm, int bn, int grid,
                     const int* __restrict__ count, long off, long n, float* __restrict__ acc, int add, int last, long V,
                     long D, int f32, void* __restrict__ dw, long lddw) {
-  const long r = (long)blockIdx.x * 8 + (threadIdx.x >> 5), c = (long)blockIdx.y * 256 + (threadIdx.x & 31) * 8;
-  if (r >= V || c >= D) return;
+  const long r = SPLIT ? blockIdx.x : (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const long c = (long)blockIdx.y * 256 + (threadIdx.x & 31) * 8;
+  if (r >= V) return;
   float v[8];
   if (slabs) {
-    slice_sum8(slice_shape((int)V, (int)D, (int)rows_here(count, off, n), bm, bn, grid), src, lds, slabs, bm, bn, r, (int)c,
-               v);
+    const SliceShape shape = slice_shape((int)V, (int)D, (int)rows_here(count, off, n), bm, bn, grid);
+    if (!slices_of<SPLIT>(shape, src, lds, slabs, bm, bn, r, 0, c, D, v)) return;
   } else {
+    if (c >= D) return;
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = src[r * lds + c + j];
   }
@@ -727,18 +797,29 @@ __global__ void __launch_bounds__(256)
 // Rows up to which one row tile holds them all: leaving rows out of the products then saves nothing, so no plan is
 // made (two launches fewer; the rows without an answer are zeroed instead).
 constexpr long kVocabOneTile = 128;
+// Rows up to which the row tile has room for dz twice over: its bf16 values and, 64 rows below, the bf16 values of what
+// their rounding took away (x is repeated there too). The products then carry 16 bits of dz for the price of 8: the
+// row tile and, up to 32 rows, the k-block are no larger. With many rows single roundings average out; with few they
+// stood out (12 rows: dx and dw off by 2.6e-3, bf16's own rounding of them 1.7e-3).
+constexpr long kVocabLo = 64;
 // Weights whose rows do not start at 128-byte lines cost the products' TMA boxes an extra line each. For the three
 // products of a gradient a copy with padded rows pays for itself from about this many rows on: V = 50,048, 4,096 rows,
 // D = 520 / 1,000 / 2,056: 930 / 1,100 / 2,233 us with the copy, 1,114 / 1,108 / 2,328 without; 1,000 rows: 270 / 352 /
 // 678 and 275 / 323 / 598. For the loss alone it does not (4,096 rows: 282 / 341 / 761 and 274 / 310 / 676).
 constexpr long kVocabPackRows = 2048;
+// Rows up to which the weight gradient (V x D values out, a short inner axis) is bound by its writes and goes out from
+// registers: V = 118,208, D = 3,712, 5 / 256 rows: the whole call 522 / 719 us, 556 / 737 through shared memory and
+// TMA stores; from 1,024 rows on the two do not differ.
+constexpr long kVocabDirectRows = 512;
 // Bytes of terms that one piece may hold. Fewer pieces mean fewer passes over the f32 weight gradient (each piece
 // after the first adds to it: 8 V D bytes).
 constexpr size_t kVocabPieceBytes = (size_t)4 << 30;
+constexpr int kSplitSlices = 8;     // slices of a product that one warp still adds up by itself
 constexpr size_t kVocabMaxK = 512;  // entries of a row: its lists stay in shared memory
 
 struct VocabPlan {
   bool compact, pack_x, pack_w;
+  long lo;         // rows below dz where its rounding errors go (0: nowhere)
   bool dw_slice;   // dW by a sliced product
   bool dw_copy;    // dW in padded rows, then copied to the caller's
   long Dp;         // row stride of the packed matrices and of the f32 products
@@ -752,7 +833,7 @@ struct VocabPlan {
   int ns;          // its columns, in 256s
   size_t bytes;
   // offsets into the workspace
-  size_t ids2, p, ent, has, rows, count, xp, wp, stat, ut, terms, info, col, val, dxs, slabs, dws, dwacc, part, dbacc;
+  size_t ids2, p, ent, has, rows, count, xp, wp, stat, ut, uk, terms, info, col, val, dxs, slabs, dws, dwacc, part, dbacc;
 };
 
 static size_t carve(size_t& at, size_t bytes) {
@@ -769,6 +850,7 @@ static VocabPlan vocab_plan(long N, long V, long D, long K, bool bias, bool grad
   const long k1 = K ? K : 1;
   p.compact = N > kVocabOneTile;
   p.pack_x = p.compact || grad || !x_ok;
+  p.lo = grad && N <= kVocabLo ? kVocabLo : 0;
   p.pack_w = !w_ok || (!w_lines && grad && N >= kVocabPackRows);
   p.Dp = round_up(D, 64);
   p.ldt = round_up(V, 64);
@@ -807,7 +889,10 @@ static VocabPlan vocab_plan(long N, long V, long D, long K, bool bias, bool grad
   if (p.pack_x) p.xp = carve(at, (size_t)p.R * p.Dp * 2);
   if (p.pack_w) p.wp = carve(at, (size_t)round_up(V, 64) * p.Dp * 2);
   p.stat = carve(at, (size_t)p.R * p.ld_stat * 8);
-  if (!K) p.ut = carve(at, (size_t)p.R * 4);
+  if (K)
+    p.uk = carve(at, (size_t)p.R * K * 4);
+  else
+    p.ut = carve(at, (size_t)p.R * 4);
   if (grad) {
     p.terms = carve(at, (size_t)p.R * p.ldt * 2);
     p.info = carve(at, (size_t)p.R * 8);
@@ -864,7 +949,7 @@ static int dz_launch(const VocabPlan& p, uint8_t* ws, long V, long K, const int*
   if (smem > 48 * 1024)
     PL_CUDA(cudaFuncSetAttribute(vocab_dz_kernel<NS, PART>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   vocab_dz_kernel<NS, PART><<<dim3((unsigned)ceil_div(V, 256 * NS), (unsigned)(round_up(n, 64) / p.rpb)), 256, smem, st>>>(
-      ws + p.terms, p.ldt, V, (int)K, count, off, n, p.rpb, ro, (const float2*)(ws + p.stat), p.ld_stat,
+      ws + p.terms, p.ldt, V, (int)K, count, off, n, p.rpb, p.lo, ro, (const float2*)(ws + p.stat), p.ld_stat,
       p.bn == 256 ? 7 : 6, part);
   count_launch();
   PL_LAUNCH("vocab_dz_kernel");
@@ -873,7 +958,7 @@ static int dz_launch(const VocabPlan& p, uint8_t* ws, long V, long K, const int*
 
 static int vocab_run(const VocabCall& c) {
   PL_REQUIRE(c.V > 0 && c.D > 0, PL_ERR_INVALID, "%s: V = %zu, D = %zu", c.what, c.V, c.D);
-  PL_REQUIRE(c.N <= (1u << 30) && c.V <= (1u << 30) && c.D <= (1u << 24), PL_ERR_INVALID,
+  PL_REQUIRE(c.N <= (1u << 30) && c.V <= (1u << 30) && c.D <= (1u << 22), PL_ERR_INVALID,
              "%s: N = %zu, V = %zu, D = %zu is too large", c.what, c.N, c.V, c.D);
   PL_REQUIRE(c.K <= kVocabMaxK, PL_ERR_INVALID, "%s: K = %zu entries, at most %zu", c.what, c.K, kVocabMaxK);
   PL_REQUIRE(c.ldx >= c.D && c.ldw >= c.D, PL_ERR_INVALID, "%s: row strides %zu, %zu below D = %zu", c.what, c.ldx, c.ldw,
@@ -914,7 +999,7 @@ static int vocab_run(const VocabCall& c) {
   const __nv_bfloat16* bias = (const __nv_bfloat16*)c.bias;
   Answers a{K ? nullptr : c.ids, K ? ws + p.has : nullptr};
   if (K) {
-    const size_t smem = (size_t)4 * 2 * K * 4;
+    const size_t smem = (size_t)4 * 2 * round_up(K, 4) * 4;
     vocab_teacher_kernel<<<(unsigned)ceil_div(N, 4), 128, smem, st>>>(c.ids, c.teacher, N, (int)K, scale2,
                                                                      (int*)(ws + p.ids2), (float*)(ws + p.p),
                                                                      (float*)(ws + p.ent), ws + p.has);
@@ -931,21 +1016,23 @@ static int vocab_run(const VocabCall& c) {
   long ldw = (long)c.ldw;
   if (p.pack_w) {
     __nv_bfloat16* wp = (__nv_bfloat16*)(ws + p.wp);
-    vocab_pack_kernel<<<dim3((unsigned)ceil_div(round_up(V, 64), 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(w, ldw, D, Answers{}, nullptr, nullptr, 0, V,
-                                                                             wp, p.Dp);
+    vocab_pack_kernel<<<dim3((unsigned)ceil_div(round_up(V, 64), 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(
+        w, ldw, D, Answers{}, nullptr, nullptr, 0, V, wp, p.Dp, 0);
     count_launch();
     PL_LAUNCH("vocab_pack_kernel");
     w = wp;
     ldw = p.Dp;
   }
+  const long lo = p.lo;  // (then one piece, no plan)
   for (int q = 0; q < p.pieces; q++) {
     const long off = (long)q * p.R, n = N - off < p.R ? N - off : p.R;
+    const long n2 = lo ? 2 * lo : n;  // rows of the products with dz
     const __nv_bfloat16* x = (const __nv_bfloat16*)c.x;  // without a plan there is one piece
     long ldx = (long)c.ldx;
     if (p.pack_x) {
       __nv_bfloat16* xp = (__nv_bfloat16*)(ws + p.xp);
-      vocab_pack_kernel<<<dim3((unsigned)ceil_div(round_up(n, 64), 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(x, ldx, D, a, rows, count, off, n, xp,
-                                                                               p.Dp);
+      vocab_pack_kernel<<<dim3((unsigned)ceil_div(round_up(n, 64), 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(
+          x, ldx, D, a, rows, count, off, n, xp, p.Dp, lo);
       count_launch();
       PL_LAUNCH("vocab_pack_kernel");
       x = xp;
@@ -981,10 +1068,14 @@ static int vocab_run(const VocabCall& c) {
     RowOut ro{};
     if (c.grad) ro = RowOut{(float2*)(ws + p.info), (int*)(ws + p.col), (float*)(ws + p.val)};
     if (K) {
-      vocab_distill_rows_kernel<<<(unsigned)n, 128, 0, st>>>(
-          x, ldx, w, ldw, bias, V, D, (int)K, (const int*)(ws + p.ids2), (const float*)(ws + p.p),
-          (const float*)(ws + p.ent), ws + p.has, scale2, inv_t, c.row_scale, rows, count, off,
-          (const float2*)(ws + p.stat), p.ld_stat, c.loss, c.lse, ro);
+      vocab_dots_kernel<<<dim3((unsigned)n, (unsigned)ceil_div(K, 16)), 128, 0, st>>>(
+          x, ldx, w, ldw, bias, V, D, (int)K, (const int*)(ws + p.ids2), scale2, rows, count, off, (float*)(ws + p.uk));
+      count_launch();
+      PL_LAUNCH("vocab_dots_kernel");
+      vocab_distill_rows_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(
+          V, (int)K, (const int*)(ws + p.ids2), (const float*)(ws + p.p), (const float*)(ws + p.ent), ws + p.has, inv_t,
+          c.row_scale, rows, count, off, n, (const float2*)(ws + p.stat), p.ld_stat, (const float*)(ws + p.uk), c.loss,
+          c.lse, ro);
     } else {
       vocab_ce_rows_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(c.ids, V, c.row_scale, rows, count, off, n,
                                                                     (const float2*)(ws + p.stat), p.ld_stat,
@@ -1012,17 +1103,20 @@ static int vocab_run(const VocabCall& c) {
       g.out = ws + p.dxs;
       g.ldo = p.Dp;
       g.slabs = slabs;
-      g.out_rows = (int)n;
+      g.out_rows = (int)n2;
       g.out_cols = (int)D;
       g.dyn_rows = count;
       g.dyn_off = (int)off;
       const Operand Z{ws + p.terms, p.R, V, p.ldt, 1, 0};
-      rc = gemm_launch(p.bd, EPI_SLICE, false, true, Z, W, (int)n, (int)D, (int)V, 1, g, st);
+      rc = gemm_launch(p.bd, EPI_SLICE, false, true, Z, W, (int)n2, (int)D, (int)V, 1, g, st);
       if (rc) return rc;
-      const bool pairs = gemm_paired(p.bd, EPI_SLICE, false, true, (int)n);
-      vocab_dx_kernel<<<dim3((unsigned)ceil_div(n, 8), (unsigned)ceil_div(D, 256)), 256, 0, st>>>((const float*)(ws + p.dxs), p.Dp, slabs, pairs ? 256 : 128,
-                                                               p.bd, pairs ? sms / 2 : sms, rows, count, off, n, V,
-                                                               D, (int)k1, ro, w, ldw, (__nv_bfloat16*)c.dx, (long)c.lddx);
+      const bool pairs = gemm_paired(p.bd, EPI_SLICE, false, true, (int)n2);
+      const int bm = pairs ? 256 : 128, grid = pairs ? sms / 2 : sms;
+      const bool split = slice_shape((int)n2, (int)D, (int)V, bm, p.bd, grid).q > kSplitSlices;
+      (split ? vocab_dx_kernel<true> : vocab_dx_kernel<false>)<<<
+          dim3((unsigned)(split ? n : ceil_div(n, 8)), (unsigned)ceil_div(D, 256)), 256, 0, st>>>(
+          (const float*)(ws + p.dxs), p.Dp, slabs, bm, p.bd, grid, rows, count, off, n, V, D, lo, (int)k1, ro, w,
+          ldw, (__nv_bfloat16*)c.dx, (long)c.lddx);
       count_launch();
       PL_LAUNCH("vocab_dx_kernel");
     }
@@ -1037,14 +1131,16 @@ static int vocab_run(const VocabCall& c) {
       const bool direct = !p.dw_slice && (p.pieces == 1 || c.dw_f32);
       const bool via = direct && p.dw_copy;  // in bf16 rows that TMA can write, then copied
       float* acc = (float*)(ws + p.dwacc);
-      const int epi = p.dw_slice ? EPI_SLICE : (direct && !c.dw_f32 ? EPI_BF16 : EPI_F32);
+      const bool rows32 = via || (((uintptr_t)c.dw & 31) == 0 && c.lddw % 16 == 0);
+      const int bf16_out = rows32 && n <= kVocabDirectRows ? EPI_DIRECT : EPI_BF16;
+      const int epi = p.dw_slice ? EPI_SLICE : (direct && !c.dw_f32 ? bf16_out : EPI_F32);
       g.out = p.dw_slice || via ? (void*)(ws + p.dws) : (direct ? c.dw : (void*)acc);
       g.ldo = direct && !via ? (long)c.lddw : p.Dp;
       g.slabs = slabs;
       g.accum = !p.dw_slice && q > 0;
-      const Operand Xk{x, n, D, ldx, 1, 0};
-      const Operand Zk{ws + p.terms, n, V, p.ldt, 1, 0};
-      rc = gemm_launch(p.bd, epi, true, true, Zk, Xk, (int)V, (int)D, (int)n, 1, g, st);
+      const Operand Xk{x, n2, D, ldx, 1, 0};
+      const Operand Zk{ws + p.terms, n2, V, p.ldt, 1, 0};
+      rc = gemm_launch(p.bd, epi, true, true, Zk, Xk, (int)V, (int)D, (int)n2, 1, g, st);
       if (rc) return rc;
       if (via) {
         vocab_copy_kernel<<<dim3((unsigned)ceil_div(V, 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(
@@ -1054,9 +1150,11 @@ static int vocab_run(const VocabCall& c) {
       }
       if (!direct && (p.dw_slice || last)) {
         const bool pairs = gemm_paired(p.bd, EPI_SLICE, true, true, (int)V);
-        vocab_dw_kernel<<<dim3((unsigned)ceil_div(V, 8), (unsigned)ceil_div(D, 256)), 256, 0, st>>>(
-            p.dw_slice ? (const float*)(ws + p.dws) : acc, p.Dp, p.dw_slice ? slabs : nullptr, pairs ? 256 : 128, p.bd,
-            pairs ? sms / 2 : sms, count, off, n,
+        const int bm = pairs ? 256 : 128, grid = pairs ? sms / 2 : sms;
+        const bool split = p.dw_slice && slice_shape((int)V, (int)D, (int)n, bm, p.bd, grid).q > kSplitSlices;
+        (split ? vocab_dw_kernel<true> : vocab_dw_kernel<false>)<<<
+            dim3((unsigned)(split ? V : ceil_div(V, 8)), (unsigned)ceil_div(D, 256)), 256, 0, st>>>(
+            p.dw_slice ? (const float*)(ws + p.dws) : acc, p.Dp, p.dw_slice ? slabs : nullptr, bm, p.bd, grid, count, off, n,
             acc, p.dw_slice && q > 0, last, V, D, c.dw_f32, c.dw, (long)c.lddw);
         count_launch();
         PL_LAUNCH("vocab_dw_kernel");

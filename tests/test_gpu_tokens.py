@@ -594,3 +594,26 @@ def test_vocab_lse_is_unbiased(D):
     lse = tokens.vocab_ce(x, w, torch.zeros(8192, dtype=torch.int32, device="cuda"))[1].double()
     z = (x.double() @ w.double().t())[:, 0]
     assert abs(float(((lse - z) * z).sum() / (z * z).sum())) < 2.0 ** -21
+
+
+@pytest.mark.parametrize("N", [1, 5, 33, 64])
+@pytest.mark.parametrize("K", [0, 4])
+def test_vocab_few_rows_round_once(N, K):
+    """Up to 64 rows the gradients carry dz in two parts: what is left is their own rounding to bf16 and the f16 terms'
+    (H of each probability's share)."""
+    x, w, b, ids, teacher, scale = _head_case(_gen(40 + N), N, 900, 128, K, True, 0, 0, left_out=0.0)
+    T = 1.5 if K else 1.0
+    ref = _head_ref(x, w, b, ids, teacher, T, scale)
+    tol_z, _ = _head_tol(ref, x, w, b, ids, T)
+    if K:
+        _, _, dx, dw, _ = tokens.vocab_distill_grad(x, w, ids, teacher, b, T, scale)
+    else:
+        _, _, dx, dw, _ = tokens.vocab_ce_grad(x, w, ids, b, scale)
+    off = 2 * B * B * ref["dz"].abs() + (H + 4 * tol_z[:, None] + 2.0 ** -18) * (ref["s"].abs() * ref["q"]) \
+        + 2.0 ** -18 * ref["dz"].abs() + 2.0 ** -40
+    off = torch.where(ref["has"][:, None], off, 0.0)
+    dxr = ref["dz"] @ w.double()
+    _close(dx, dxr, off @ w.double().abs() + 1e-4 * B * (ref["dz"].abs() @ w.double().abs()) + B * 1.01 * dxr.abs(), "dx")
+    dwr = ref["dz"].t() @ x.double()
+    _close(dw, dwr, off.t() @ x.double().abs() + 1e-4 * B * (ref["dz"].abs().t() @ x.double().abs())
+           + B * 1.01 * dwr.abs(), "dw")
