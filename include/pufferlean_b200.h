@@ -559,8 +559,9 @@ int pl_layernorm_grad_dev(const void* dy, size_t lddy, const void* x, size_t ldx
  * ws: pl_vocab_ws bytes (K = 0 for the cross entropy, else at most 512; aligned = 1 when x and dw
  * start at 16 bytes with row strides that are multiples of 8, and w at 128 with one that is a multiple of 64). The gradient forms keep one piece of rows' softmax terms there (2 bytes each): piece_bytes
  * bounds that piece, 0 = 4 GiB; the results do not depend on it beyond the order of dw's f32 sums.
- * dx [N x D] bf16; dw [V x D] and dbias [V] (given exactly when bias is) bf16, or f32 with dw_f32 = 1 (f32 sums of
- * products of bf16-rounded gradients). row_scale [N] f32 or NULL (ones). */
+ * dx [N x D] bf16; dw [V x D] and dbias [V] (given exactly when bias is) bf16, or f32 with dw_f32 = 1. dw's f32 sums are
+ * of products whose logit gradients were rounded to bf16 (up to 64 rows: to two bf16 parts). row_scale [N] f32 or NULL
+ * (ones). */
 size_t pl_vocab_ws(size_t N, size_t V, size_t D, size_t K, uint8_t bias, uint8_t grad, uint8_t aligned,
                    size_t piece_bytes);
 int pl_vocab_ce_dev(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, const int32_t* target,

@@ -1676,8 +1676,8 @@ bool gemm_store_map(CUtensorMap* map, const void* ptr, long rows, long cols, lon
 int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const Operand& B, int M, int N, int K,
                 int batch, const EpiArgs& ep, cudaStream_t st);
 // 0 = single-CTA tiles only, 1 = CTA pairs where eligible, 2 = CTA pairs for the products whose two
-// operands are MN-major (the weight gradients) and the large-vocabulary head's (the default); a negative mode only queries. Returns the
-// previous mode.
+// operands are MN-major (the weight gradients) and the large-vocabulary head's (the default); a negative
+// mode only queries. Returns the previous mode.
 int gemm_set_pair_mode(int mode);
 // SMs of the current device. An EPI_SLICE launch runs on all of them: one CTA each with 128-row tiles, or (gemm_paired)
 // pairs with 256-row tiles; its slice_shape follows from that.

@@ -15,6 +15,8 @@ Gradients are of sum_n row_scale_n * loss_n (descent).
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import PufferError, _check, lib
@@ -42,8 +44,8 @@ def _matrix(t, what, name, dtypes, device=None):
             return st
         if rows <= 1 and sc == 1:
             return cols
-        raise PufferError(f"{what}: {name} must have contiguous rows that do not overlap (shape {(rows, cols)}, strides "
-                          f"{(st, sc)})")
+        raise PufferError(f"{what}: {name} must have contiguous rows that do not overlap (shape {(rows, cols)}, "
+                          f"strides {(st, sc)})")
     _need(isinstance(t, torch.Tensor) and t.is_cuda, what, "%s must be a CUDA tensor", name)
     _need(t.dim() == 2, what, "%s must have two dimensions, has %d", name, t.dim())
     _need(t.dtype in dtypes, what, "%s has type %s", name, t.dtype)
@@ -58,6 +60,11 @@ def _vector(t, what, name, dtype, shape, device):
     _need(t.dtype == dtype, what, "%s has type %s, not %s", name, t.dtype, dtype)
     _need(tuple(t.shape) == tuple(shape), what, "%s has shape %s, not %s", name, tuple(t.shape), tuple(shape))
     raise PufferError(f"{what}: {name} must be contiguous")
+
+
+@functools.lru_cache(maxsize=1024)
+def _vocab_ws(n, v, d, k, bias, grad, aligned, piece_bytes):
+    return lib().pl_vocab_ws(n, v, d, k, bias, grad, aligned, piece_bytes)
 
 
 def _like(t):
@@ -161,14 +168,15 @@ def _head(what, x, w, bias, ids, teacher, temperature, row_scale, grad, dw_f32=F
         dx = _like(x)
         dw = torch.empty((v, d), dtype=_F32, device=dev) if dw_f32 else _like(w)
         db = torch.empty_like(bias, dtype=dw.dtype) if bias is not None else None
-    size = L.pl_vocab_ws(n, v, d, k, bias is not None, grad, aligned, piece_bytes)
+    size = _vocab_ws(n, v, d, k, bias is not None, grad, aligned, piece_bytes)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     head = (x.data_ptr(), ldx, w.data_ptr(), ldw, bp, ip)
     tail = (n, v, d, loss.data_ptr(), lse.data_ptr())
     room = (ws.data_ptr(), size)
     was, st = _enter(dev)
     if grad:
-        tail = (sp, *tail, dx.data_ptr(), d, dw.data_ptr(), d, None if db is None else db.data_ptr(), dw_f32, piece_bytes)
+        tail = (sp, *tail, dx.data_ptr(), d, dw.data_ptr(), d, None if db is None else db.data_ptr(), dw_f32,
+                piece_bytes)
         if distill:
             rc = L.pl_vocab_distill_grad_dev(*head, tp, k, temperature, *tail, *room, st)
         else:
