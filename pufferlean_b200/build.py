@@ -1,5 +1,5 @@
 """Builds the CUDA library in-tree: pufferlean_b200/_build/libpufferlean_b200.so (and the Lean
-adapter libpufferlean_lean.so). sm_100a only; nvcc links the CUDA runtime statically, so the
+adapter libpufferlean_lean.so, and pl_torch.so, the module behind pufferlean_b200/tokens.py). sm_100a only; nvcc links the CUDA runtime statically, so the
 library does not depend on which libcudart another package in the process loaded.
 
     python -m pufferlean_b200.build [--clean] [-j N]
@@ -9,10 +9,12 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -25,6 +27,7 @@ CXXFLAGS = ["-std=c++17", "-O2", "-fPIC", "-ffp-contract=off", "-I" + os.path.jo
             "-I/usr/local/cuda/include"]
 LIB = os.path.join(BUILD, "libpufferlean_b200.so")
 LEAN_LIB = os.path.join(BUILD, "libpufferlean_lean.so")
+TORCH_EXT = os.path.join(BUILD, "pl_torch.so")
 
 
 def _compile(src: str, verbose: bool) -> str:
@@ -44,10 +47,30 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _torch_ext(verbose: bool) -> None:
+    """The module that takes torch tensors (pufferlean_b200/tokens.py); left out where torch is not installed."""
+    src = os.path.join(CSRC, "pl_torch.cpp")
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return
+    torch = spec.submodule_search_locations[0]
+    if os.path.exists(TORCH_EXT) and os.path.getmtime(TORCH_EXT) >= max(
+            os.path.getmtime(p) for p in (src, LIB, os.path.join(ROOT, "include", "pufferlean_b200.h"))):
+        return
+    cmd = ["g++"] + CXXFLAGS + ["-shared", "-o", TORCH_EXT, src, "-isystem", os.path.join(torch, "include"), "-isystem",
+                                os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+                                "-I" + sysconfig.get_paths()["include"], "-L" + BUILD, "-lpufferlean_b200",
+                                "-L" + os.path.join(torch, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+                                "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+
+
 def build(jobs: int | None = None, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cpp")))
-    srcs = [s for s in srcs if not os.path.basename(s).startswith("pl_lean")]
+    srcs = [s for s in srcs if not os.path.basename(s).startswith(("pl_lean", "pl_torch"))]
     with cf.ThreadPoolExecutor(max_workers=jobs or os.cpu_count() or 4) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
     newest = max(os.path.getmtime(o) for o in objs)
@@ -66,6 +89,7 @@ def build(jobs: int | None = None, verbose: bool = False) -> str:
             if verbose:
                 print(" ".join(cmd), flush=True)
             subprocess.check_call(cmd)
+    _torch_ext(verbose)
     return LIB
 
 
