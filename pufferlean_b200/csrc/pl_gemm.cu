@@ -200,7 +200,10 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
       if (nconf < 256) configured[nconf++] = (void*)k;
     }
   }
-  k<<<grid, 320, smem, st>>>(ma, mb, mc, mc2, M, N, K, ep);
+  if (ep.pdl)
+    PL_CUDA(launch_early(k, grid, dim3(320), smem, st, ma, mb, mc, mc2, M, N, K, ep));
+  else
+    k<<<grid, 320, smem, st>>>(ma, mb, mc, mc2, M, N, K, ep);
   count_launch();
   PL_LAUNCH("tc_gemm_kernel");
   return PL_OK;

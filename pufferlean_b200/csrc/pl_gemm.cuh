@@ -123,6 +123,7 @@ struct EpiArgs {
   // clamp(*dyn_rows - dyn_off, 0, extent given by the host).
   const int* dyn_rows;
   int dyn_off, dyn_k;
+  int pdl;  // the launch may start while the kernel before it in the stream finishes
 };
 
 // s = 1 / (sqrt(sum_i diag_i) + eps) over the m bf16 diagonal entries of a matrix (leading dimension
@@ -1238,19 +1239,7 @@ __global__ void __launch_bounds__(320, 1)
   uint32_t* tmem_slot = (uint32_t*)(aux_empty + 2);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
-  if (ep.dyn_rows) {  // the rows that exist, counted on the device by an earlier kernel of the stream
-    const int have = max(0, *ep.dyn_rows - ep.dyn_off);
-    if (ep.dyn_k)
-      K = min(K, have);
-    else
-      M = min(M, have);
-  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int num_n = (N + BN - 1) / BN, num_m = (M + BM - 1) / BM;
-  const int num_z = ep.k_splits > 1 ? ep.k_splits : (ep.nbatch > 1 ? ep.nbatch : 1);
-  const int total_tiles = num_n * num_m * num_z;
-  const int total_kb = (K + BK - 1) / BK;
-  const int per_split = ep.k_splits > 1 ? (total_kb + ep.k_splits - 1) / ep.k_splits : total_kb;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
@@ -1282,6 +1271,22 @@ __global__ void __launch_bounds__(320, 1)
   tc::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  // What earlier kernels of the stream wrote (or still read) is touched from here on only: a launch that may start early
+  // (EpiArgs::pdl) has done its set-up by now.
+  grid_wait();
+  grid_next();
+  if (ep.dyn_rows) {  // the rows that exist, counted on the device by an earlier kernel of the stream
+    const int have = max(0, *ep.dyn_rows - ep.dyn_off);
+    if (ep.dyn_k)
+      K = min(K, have);
+    else
+      M = min(M, have);
+  }
+  const int num_n = (N + BN - 1) / BN, num_m = (M + BM - 1) / BM;
+  const int num_z = ep.k_splits > 1 ? ep.k_splits : (ep.nbatch > 1 ? ep.nbatch : 1);
+  const int total_tiles = num_n * num_m * num_z;
+  const int total_kb = (K + BK - 1) / BK;
+  const int per_split = ep.k_splits > 1 ? (total_kb + ep.k_splits - 1) / ep.k_splits : total_kb;
   SliceShape shape{};
   if constexpr (EPI == EPI_SLICE) shape = slice_shape(M, N, K, BM, BN, gridDim.x);
   TileWalk<EPI, BM> walk(blockIdx.x, gridDim.x, num_n, num_m, total_tiles, total_kb, per_split, ep.k_splits, shape);
@@ -1485,21 +1490,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
-  if (ep.dyn_rows) {  // the rows that exist, counted on the device by an earlier kernel of the stream
-    const int have = max(0, *ep.dyn_rows - ep.dyn_off);
-    if (ep.dyn_k)
-      K = min(K, have);
-    else
-      M = min(M, have);
-  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_ctarank();
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-  const int num_n = (N + BN - 1) / BN, num_m = (M + 2 * BM - 1) / (2 * BM);
-  const int num_z = ep.k_splits > 1 ? ep.k_splits : (ep.nbatch > 1 ? ep.nbatch : 1);
-  const int total_tiles = num_n * num_m * num_z;
-  const int total_kb = (K + BK - 1) / BK;
-  const int per_split = ep.k_splits > 1 ? (total_kb + ep.k_splits - 1) / ep.k_splits : total_kb;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
@@ -1526,6 +1519,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
   tc::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  grid_wait();
+  grid_next();
+  if (ep.dyn_rows) {  // the rows that exist, counted on the device by an earlier kernel of the stream
+    const int have = max(0, *ep.dyn_rows - ep.dyn_off);
+    if (ep.dyn_k)
+      K = min(K, have);
+    else
+      M = min(M, have);
+  }
+  const int num_n = (N + BN - 1) / BN, num_m = (M + 2 * BM - 1) / (2 * BM);
+  const int num_z = ep.k_splits > 1 ? ep.k_splits : (ep.nbatch > 1 ? ep.nbatch : 1);
+  const int total_tiles = num_n * num_m * num_z;
+  const int total_kb = (K + BK - 1) / BK;
+  const int per_split = ep.k_splits > 1 ? (total_kb + ep.k_splits - 1) / ep.k_splits : total_kb;
   SliceShape shape{};
   if constexpr (EPI == EPI_SLICE) shape = slice_shape(M, N, K, 2 * BM, BN, npairs);
   TileWalk<EPI, 2 * BM> walk(pair, npairs, num_n, num_m, total_tiles, total_kb, per_split, ep.k_splits, shape);

@@ -264,6 +264,8 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR))
     norm_fwd_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w, const float* __restrict__ b,
                     long rows, int cols, float eps, T* __restrict__ y, long ldy, float* __restrict__ mean,
                     float* __restrict__ rstd) {
+  grid_wait();
+  grid_next();
   constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR, LV = 32 / RB;
   __shared__ float scr[2][RB][32];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
@@ -344,6 +346,8 @@ __global__ void __launch_bounds__(512)
     norm_fwd_wide_kernel(const T* __restrict__ x, long ldx, const float* __restrict__ w, const float* __restrict__ b,
                          long rows, long cols, float eps, T* __restrict__ y, long ldy, float* __restrict__ mean,
                          float* __restrict__ rstd) {
+  grid_wait();
+  grid_next();
   __shared__ float scr[2][32];
   const long row = blockIdx.x;
   const T* xr = x + row * ldx;
@@ -379,6 +383,8 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR))
     norm_bwd_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ x, long ldx,
                     const float* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
                     long rows, int cols, T* __restrict__ dx, long lddx, float* __restrict__ part) {
+  grid_wait();
+  grid_next();
   constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR, E = VEC * K;
   constexpr int NV = 2 * RB, LV = 32 / NV;  // values of an iteration, lanes that hold one of them
   constexpr bool KEEP_W = TPR < 1024;
@@ -501,6 +507,8 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR))
 __global__ void __launch_bounds__(1024)
     norm_param_kernel(const float* __restrict__ part, int parts, long cols, float* __restrict__ dw,
                       float* __restrict__ db) {
+  grid_wait();
+  grid_next();
   __shared__ float scr[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const long c = (long)blockIdx.x * 32 + lane;
@@ -524,6 +532,8 @@ __global__ void __launch_bounds__(512)
     norm_bwd_wide_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ x, long ldx,
                          const float* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
                          long rows, long cols, T* __restrict__ dx, long lddx) {
+  grid_wait();
+  grid_next();
   __shared__ float scr[2][32];
   const long row = blockIdx.x;
   const float m = mean[row], r = rstd[row], inv = 1.f / (float)cols;
@@ -546,6 +556,8 @@ __global__ void __launch_bounds__(256)
     norm_bwd_wide_param_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ x, long ldx,
                                const float* __restrict__ mean, const float* __restrict__ rstd, long rows, long cols,
                                float* __restrict__ part) {
+  grid_wait();
+  grid_next();
   const long c = (long)blockIdx.x * 256 + threadIdx.x;
   if (c >= cols) return;
   float a = 0.f, b = 0.f;
@@ -575,10 +587,9 @@ static int fwd_launch(const void* x, long ldx, const float* w, const float* b, l
   // few rows: one per group, so that more SMs have some (latency); many: RB at a time
   if constexpr (RB > 1)
     if (need < most / 2) return fwd_launch<T, VEC, TPR, K, 1>(x, ldx, w, b, rows, cols, eps, y, ldy, mean, rstd, st);
-  norm_fwd_kernel<T, VEC, TPR, K, RB><<<(unsigned)(need < most ? need : most), THREADS, 0, st>>>(
-      (const T*)x, ldx, w, b, rows, cols, eps, (T*)y, ldy, mean, rstd);
+  PL_CUDA(launch_early(norm_fwd_kernel<T, VEC, TPR, K, RB>, (unsigned)(need < most ? need : most), THREADS, 0, st,
+                        (const T*)x, ldx, w, b, rows, cols, eps, (T*)y, ldy, mean, rstd));
   count_launch();
-  PL_LAUNCH("norm_fwd_kernel");
   return PL_OK;
 }
 
@@ -620,16 +631,16 @@ static int fwd_pick(const void* x, long ldx, const float* w, const float* b, lon
     PL_FWD(1, 1024, 16, 1)
   }
 #undef PL_FWD
-  norm_fwd_wide_kernel<T><<<(unsigned)rows, 512, 0, st>>>((const T*)x, ldx, w, b, rows, cols, eps, (T*)y, ldy, mean, rstd);
+  PL_CUDA(launch_early(norm_fwd_wide_kernel<T>, (unsigned)rows, 512, 0, st, (const T*)x, ldx, w, b, rows, cols, eps,
+                       (T*)y, ldy, mean, rstd));
   count_launch();
-  PL_LAUNCH("norm_fwd_wide_kernel");
   return PL_OK;
 }
 
 static int param_launch(const float* part, int parts, long cols, float* dw, float* db, cudaStream_t st) {
-  norm_param_kernel<<<dim3((unsigned)ceil_div(cols, 32), 2), 1024, 0, st>>>(part, parts, cols, dw, db);
+  PL_CUDA(launch_early(norm_param_kernel, dim3((unsigned)ceil_div(cols, 32), 2), 1024, 0, st, part, parts, cols, dw,
+                       db));
   count_launch();
-  PL_LAUNCH("norm_param_kernel");
   return PL_OK;
 }
 
@@ -645,10 +656,9 @@ static int bwd_launch(const void* dy, long lddy, const void* x, long ldx, const 
       return bwd_launch<T, VEC, TPR, K, 1>(dy, lddy, x, ldx, w, mean, rstd, rows, cols, dx, lddx, dw, db, part, st);
   const int grid = (int)(need < most ? need : most);
   static_assert(FOLD <= 48 * 1024, "column sums of the groups");
-  norm_bwd_kernel<T, VEC, TPR, K, RB><<<grid, THREADS, FOLD, st>>>((const T*)dy, lddy, (const T*)x, ldx, w, mean, rstd,
-                                                                   rows, cols, (T*)dx, lddx, (dw || db) ? part : nullptr);
+  PL_CUDA(launch_early(norm_bwd_kernel<T, VEC, TPR, K, RB>, grid, THREADS, FOLD, st, (const T*)dy, lddy, (const T*)x,
+                       ldx, w, mean, rstd, rows, cols, (T*)dx, lddx, (dw || db) ? part : nullptr));
   count_launch();
-  PL_LAUNCH("norm_bwd_kernel");
   return (dw || db) ? param_launch(part, grid, cols, dw, db, st) : PL_OK;
 }
 
@@ -691,16 +701,14 @@ static int bwd_pick(const void* dy, long lddy, const void* x, long ldx, const fl
     PL_BWD(1, 1024, 16, 1)
   }
 #undef PL_BWD
-  norm_bwd_wide_kernel<T><<<(unsigned)rows, 512, 0, st>>>((const T*)dy, lddy, (const T*)x, ldx, w, mean, rstd, rows,
-                                                          cols, (T*)dx, lddx);
+  PL_CUDA(launch_early(norm_bwd_wide_kernel<T>, (unsigned)rows, 512, 0, st, (const T*)dy, lddy, (const T*)x, ldx, w,
+                       mean, rstd, rows, cols, (T*)dx, lddx));
   count_launch();
-  PL_LAUNCH("norm_bwd_wide_kernel");
   if (!dw && !db) return PL_OK;
   const int slices = (int)(rows < 64 ? rows : 64);
-  norm_bwd_wide_param_kernel<T><<<dim3((unsigned)ceil_div(cols, 256), slices), 256, 0, st>>>(
-      (const T*)dy, lddy, (const T*)x, ldx, mean, rstd, rows, cols, part);
+  PL_CUDA(launch_early(norm_bwd_wide_param_kernel<T>, dim3((unsigned)ceil_div(cols, 256), slices), 256, 0, st,
+                        (const T*)dy, lddy, (const T*)x, ldx, mean, rstd, rows, cols, part));
   count_launch();
-  PL_LAUNCH("norm_bwd_wide_param_kernel");
   return param_launch(part, slices, cols, dw, db, st);
 }
 

@@ -57,6 +57,8 @@ __global__ void __launch_bounds__(128)
     vocab_teacher_kernel(const int* __restrict__ ids, const float* __restrict__ teacher, long N, int K, float tscale,
                          int* __restrict__ ids2, float* __restrict__ p, float* __restrict__ ent,
                          uint8_t* __restrict__ has) {
+  grid_wait();
+  grid_next();
   extern __shared__ __align__(16) uint8_t dyn_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long r = (long)blockIdx.x * 4 + warp;
@@ -122,6 +124,8 @@ __global__ void __launch_bounds__(128)
 __global__ void __launch_bounds__(1024)
     vocab_plan_kernel(Answers a, long N, int* __restrict__ rows, int* __restrict__ count, float* __restrict__ loss,
                       float* __restrict__ lse) {
+  grid_wait();
+  grid_next();
   __shared__ int warp_n[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int base = 0;
@@ -221,6 +225,8 @@ __global__ void __launch_bounds__(256)
     vocab_pack_kernel(const __nv_bfloat16* __restrict__ src, long ld, long D, Answers a, const int* __restrict__ rows,
                       const int* __restrict__ count, long off, long n, __nv_bfloat16* __restrict__ dst, long ldd,
                       long again) {
+  grid_wait();
+  grid_next();
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const long have = rows_here(count, off, n);
@@ -241,6 +247,8 @@ __global__ void __launch_bounds__(256)
 __global__ void __launch_bounds__(256)
     vocab_copy_kernel(const __nv_bfloat16* __restrict__ src, long ld, long n, long D, __nv_bfloat16* __restrict__ dst,
                       long ldd) {
+  grid_wait();
+  grid_next();
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (i >= n) return;
   copy_row(dst + i * ldd, src + i * ld, (long)blockIdx.y * 1024, D, true, threadIdx.x & 31);
@@ -286,6 +294,8 @@ __global__ void __launch_bounds__(128)
                       const __nv_bfloat16* __restrict__ bias, long V, long D, int K, const int* __restrict__ ids2,
                       float scale2, const int* __restrict__ rows, const int* __restrict__ count, long off,
                       float* __restrict__ uk) {
+  grid_wait();
+  grid_next();
   const long i = blockIdx.x;
   if (count && off + i >= *count) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -361,6 +371,8 @@ __global__ void __launch_bounds__(256)
                          const int* __restrict__ rows, const int* __restrict__ count, long off, long n,
                          const float2* __restrict__ stat, long ld_stat, const float* __restrict__ ut,
                          float* __restrict__ loss, float* __restrict__ lse, RowOut o) {
+  grid_wait();
+  grid_next();
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (i >= rows_here(count, off, n)) return;
@@ -391,6 +403,8 @@ __global__ void __launch_bounds__(256)
                               const int* __restrict__ count, long off, long n, const float2* __restrict__ stat,
                               long ld_stat, const float* __restrict__ uk, float* __restrict__ loss,
                               float* __restrict__ lse, RowOut o) {
+  grid_wait();
+  grid_next();
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (i >= rows_here(count, off, n)) return;
@@ -445,6 +459,8 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
     vocab_dz_kernel(void* __restrict__ terms, long ld, long V, int K, const int* __restrict__ count, long off, long n,
                     int rpb, long lo, RowOut in, const float2* __restrict__ stat, long ld_stat, int seg_shift,
                     float* __restrict__ part) {
+  grid_wait();
+  grid_next();
   constexpr int COLS = 256 * NS;
   extern __shared__ __align__(16) uint8_t dyn_smem[];
   uint32_t* mask = reinterpret_cast<uint32_t*>(dyn_smem);                   // [rpb][COLS / 32]
@@ -624,6 +640,8 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
 __global__ void __launch_bounds__(1024)
     vocab_dbias_kernel(const float* __restrict__ part, int tiles, long V, float* __restrict__ acc, int first, int last,
                        int f32, void* __restrict__ dbias) {
+  grid_wait();
+  grid_next();
   __shared__ float scr[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const long c0 = (long)blockIdx.x * 32;
@@ -707,6 +725,8 @@ __global__ void __launch_bounds__(256)
                     const int* __restrict__ rows, const int* __restrict__ count, long off, long n, long V, long D,
                     long lo, int K, RowOut in, const __nv_bfloat16* __restrict__ w, long ldw,
                     __nv_bfloat16* __restrict__ dx, long lddx) {
+  grid_wait();
+  grid_next();
   const long i = SPLIT ? blockIdx.x : (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const long have = rows_here(count, off, n);
@@ -758,6 +778,8 @@ __global__ void __launch_bounds__(256)
     vocab_dw_kernel(const float* __restrict__ src, long lds, const float* __restrict__ slabs, int bm, int bn, int grid,
                     const int* __restrict__ count, long off, long n, float* __restrict__ acc, int add, int last, long V,
                     long D, int f32, void* __restrict__ dw, long lddw) {
+  grid_wait();
+  grid_next();
   const long r = SPLIT ? blockIdx.x : (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const long c = (long)blockIdx.y * 256 + (threadIdx.x & 31) * 8;
   if (r >= V) return;
@@ -948,11 +970,10 @@ static int dz_launch(const VocabPlan& p, uint8_t* ws, long V, long K, const int*
   const size_t smem = DzSmem<NS>::bytes(p.rpb, K, PART);
   if (smem > 48 * 1024)
     PL_CUDA(cudaFuncSetAttribute(vocab_dz_kernel<NS, PART>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  vocab_dz_kernel<NS, PART><<<dim3((unsigned)ceil_div(V, 256 * NS), (unsigned)(round_up(n, 64) / p.rpb)), 256, smem, st>>>(
-      ws + p.terms, p.ldt, V, (int)K, count, off, n, p.rpb, p.lo, ro, (const float2*)(ws + p.stat), p.ld_stat,
-      p.bn == 256 ? 7 : 6, part);
+  const dim3 grid((unsigned)ceil_div(V, 256 * NS), (unsigned)(round_up(n, 64) / p.rpb));
+  PL_CUDA(launch_early(vocab_dz_kernel<NS, PART>, grid, 256, smem, st, ws + p.terms, p.ldt, V, (int)K, count, off, n, p.rpb, p.lo, ro,
+                       (const float2*)(ws + p.stat), p.ld_stat, p.bn == 256 ? 7 : 6, part));
   count_launch();
-  PL_LAUNCH("vocab_dz_kernel");
   return PL_OK;
 }
 
@@ -1000,26 +1021,22 @@ static int vocab_run(const VocabCall& c) {
   Answers a{K ? nullptr : c.ids, K ? ws + p.has : nullptr};
   if (K) {
     const size_t smem = (size_t)4 * 2 * round_up(K, 4) * 4;
-    vocab_teacher_kernel<<<(unsigned)ceil_div(N, 4), 128, smem, st>>>(c.ids, c.teacher, N, (int)K, scale2,
-                                                                     (int*)(ws + p.ids2), (float*)(ws + p.p),
-                                                                     (float*)(ws + p.ent), ws + p.has);
+    PL_CUDA(launch_early(vocab_teacher_kernel, (unsigned)ceil_div(N, 4), 128, smem, st, c.ids, c.teacher, N, (int)K,
+                         scale2, (int*)(ws + p.ids2), (float*)(ws + p.p), (float*)(ws + p.ent), ws + p.has));
     count_launch();
-    PL_LAUNCH("vocab_teacher_kernel");
   }
   if (p.compact) {
     if (c.grad) PL_CUDA(cudaMemset2DAsync(c.dx, c.lddx * 2, 0, c.D * 2, c.N, st));  // rows that do not count
-    vocab_plan_kernel<<<1, 1024, 0, st>>>(a, N, rows, count, c.loss, c.lse);
+    PL_CUDA(launch_early(vocab_plan_kernel, 1, 1024, 0, st, a, N, rows, count, c.loss, c.lse));
     count_launch();
-    PL_LAUNCH("vocab_plan_kernel");
   }
   const __nv_bfloat16* w = (const __nv_bfloat16*)c.w;
   long ldw = (long)c.ldw;
   if (p.pack_w) {
     __nv_bfloat16* wp = (__nv_bfloat16*)(ws + p.wp);
-    vocab_pack_kernel<<<dim3((unsigned)ceil_div(round_up(V, 64), 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(
-        w, ldw, D, Answers{}, nullptr, nullptr, 0, V, wp, p.Dp, 0);
+    PL_CUDA(launch_early(vocab_pack_kernel, dim3((unsigned)ceil_div(round_up(V, 64), 8), (unsigned)ceil_div(D, 1024)),
+                         256, 0, st, w, ldw, D, Answers{}, nullptr, nullptr, 0, V, wp, p.Dp, 0));
     count_launch();
-    PL_LAUNCH("vocab_pack_kernel");
     w = wp;
     ldw = p.Dp;
   }
@@ -1031,10 +1048,9 @@ static int vocab_run(const VocabCall& c) {
     long ldx = (long)c.ldx;
     if (p.pack_x) {
       __nv_bfloat16* xp = (__nv_bfloat16*)(ws + p.xp);
-      vocab_pack_kernel<<<dim3((unsigned)ceil_div(round_up(n, 64), 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(
-          x, ldx, D, a, rows, count, off, n, xp, p.Dp, lo);
+      const dim3 grid((unsigned)ceil_div(round_up(n, 64), 8), (unsigned)ceil_div(D, 1024));
+      PL_CUDA(launch_early(vocab_pack_kernel, grid, 256, 0, st, x, ldx, D, a, rows, count, off, n, xp, p.Dp, lo));
       count_launch();
-      PL_LAUNCH("vocab_pack_kernel");
       x = xp;
       ldx = p.Dp;
     }
@@ -1042,6 +1058,7 @@ static int vocab_run(const VocabCall& c) {
     const Operand X{x, p.pack_x ? p.R : n, D, ldx, 1, 0}, W{w, V, D, ldw, 1, 0};
     {
       EpiArgs e{};
+      e.pdl = 1;
       e.out = c.grad ? ws + p.terms : nullptr;
       e.ldo = p.ldt;
       e.out_rows = (int)n;
@@ -1068,21 +1085,20 @@ static int vocab_run(const VocabCall& c) {
     RowOut ro{};
     if (c.grad) ro = RowOut{(float2*)(ws + p.info), (int*)(ws + p.col), (float*)(ws + p.val)};
     if (K) {
-      vocab_dots_kernel<<<dim3((unsigned)n, (unsigned)ceil_div(K, 16)), 128, 0, st>>>(
-          x, ldx, w, ldw, bias, V, D, (int)K, (const int*)(ws + p.ids2), scale2, rows, count, off, (float*)(ws + p.uk));
+      PL_CUDA(launch_early(vocab_dots_kernel, dim3((unsigned)n, (unsigned)ceil_div(K, 16)), 128, 0, st, x, ldx, w,
+                           ldw, bias, V, D, (int)K, (const int*)(ws + p.ids2), scale2, rows, count, off,
+                           (float*)(ws + p.uk)));
       count_launch();
-      PL_LAUNCH("vocab_dots_kernel");
-      vocab_distill_rows_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(
-          V, (int)K, (const int*)(ws + p.ids2), (const float*)(ws + p.p), (const float*)(ws + p.ent), ws + p.has, inv_t,
-          c.row_scale, rows, count, off, n, (const float2*)(ws + p.stat), p.ld_stat, (const float*)(ws + p.uk), c.loss,
-          c.lse, ro);
+      PL_CUDA(launch_early(vocab_distill_rows_kernel, (unsigned)ceil_div(n, 8), 256, 0, st, V, (int)K,
+                           (const int*)(ws + p.ids2), (const float*)(ws + p.p), (const float*)(ws + p.ent),
+                           ws + p.has, inv_t, c.row_scale, rows, count, off, n, (const float2*)(ws + p.stat),
+                           p.ld_stat, (const float*)(ws + p.uk), c.loss, c.lse, ro));
     } else {
-      vocab_ce_rows_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(c.ids, V, c.row_scale, rows, count, off, n,
-                                                                    (const float2*)(ws + p.stat), p.ld_stat,
-                                                                    (const float*)(ws + p.ut), c.loss, c.lse, ro);
+      PL_CUDA(launch_early(vocab_ce_rows_kernel, (unsigned)ceil_div(n, 8), 256, 0, st, c.ids, V, c.row_scale, rows,
+                           count, off, n, (const float2*)(ws + p.stat), p.ld_stat, (const float*)(ws + p.ut), c.loss,
+                           c.lse, ro));
     }
     count_launch();
-    PL_LAUNCH("vocab_rows_kernel");
     if (!c.grad) continue;
     const bool last = q == p.pieces - 1;
     float* part = bias ? (float*)(ws + p.part) : nullptr;
@@ -1091,15 +1107,14 @@ static int vocab_run(const VocabCall& c) {
     rc = dz(p, ws, V, k1, count, off, n, ro, part, st);
     if (rc) return rc;
     if (bias) {
-      vocab_dbias_kernel<<<(unsigned)ceil_div(V, 32), 1024, 0, st>>>(part, (int)(round_up(n, 64) / p.rpb), V,
-                                                                    (float*)(ws + p.dbacc), q == 0, last, c.dw_f32,
-                                                                    c.dbias);
+      const int tiles = (int)(round_up(n, 64) / p.rpb);
+      PL_CUDA(launch_early(vocab_dbias_kernel, (unsigned)ceil_div(V, 32), 1024, 0, st, part, tiles, V, (float*)(ws + p.dbacc), q == 0, last, c.dw_f32, c.dbias));
       count_launch();
-      PL_LAUNCH("vocab_dbias_kernel");
     }
     float* slabs = (float*)(ws + p.slabs);
     {  // dx = dz W
       EpiArgs g{};
+      g.pdl = 1;
       g.out = ws + p.dxs;
       g.ldo = p.Dp;
       g.slabs = slabs;
@@ -1113,15 +1128,15 @@ static int vocab_run(const VocabCall& c) {
       const bool pairs = gemm_paired(p.bd, EPI_SLICE, false, true, (int)n2);
       const int bm = pairs ? 256 : 128, grid = pairs ? sms / 2 : sms;
       const bool split = slice_shape((int)n2, (int)D, (int)V, bm, p.bd, grid).q > kSplitSlices;
-      (split ? vocab_dx_kernel<true> : vocab_dx_kernel<false>)<<<
-          dim3((unsigned)(split ? n : ceil_div(n, 8)), (unsigned)ceil_div(D, 256)), 256, 0, st>>>(
-          (const float*)(ws + p.dxs), p.Dp, slabs, bm, p.bd, grid, rows, count, off, n, V, D, lo, (int)k1, ro, w,
-          ldw, (__nv_bfloat16*)c.dx, (long)c.lddx);
+      PL_CUDA(launch_early((split ? vocab_dx_kernel<true> : vocab_dx_kernel<false>),
+                           dim3((unsigned)(split ? n : ceil_div(n, 8)), (unsigned)ceil_div(D, 256)), 256, 0, st,
+                           (const float*)(ws + p.dxs), p.Dp, slabs, bm, p.bd, grid, rows, count, off, n, V, D, lo,
+                           (int)k1, ro, w, ldw, (__nv_bfloat16*)c.dx, (long)c.lddx));
       count_launch();
-      PL_LAUNCH("vocab_dx_kernel");
     }
     {  // dW (+)= dz^T x: to the caller's matrix, to the f32 sum of the pieces, or sliced
       EpiArgs g{};
+      g.pdl = 1;
       g.alpha = 1.f;
       g.out_rows = (int)V;
       g.out_cols = (int)D;
@@ -1143,21 +1158,21 @@ static int vocab_run(const VocabCall& c) {
       rc = gemm_launch(p.bd, epi, true, true, Zk, Xk, (int)V, (int)D, (int)n2, 1, g, st);
       if (rc) return rc;
       if (via) {
-        vocab_copy_kernel<<<dim3((unsigned)ceil_div(V, 8), (unsigned)ceil_div(D, 1024)), 256, 0, st>>>(
-            (const __nv_bfloat16*)(ws + p.dws), p.Dp, V, D, (__nv_bfloat16*)c.dw, (long)c.lddw);
+        PL_CUDA(launch_early(vocab_copy_kernel, dim3((unsigned)ceil_div(V, 8), (unsigned)ceil_div(D, 1024)), 256, 0,
+                             st, (const __nv_bfloat16*)(ws + p.dws), p.Dp, V, D, (__nv_bfloat16*)c.dw,
+                             (long)c.lddw));
         count_launch();
-        PL_LAUNCH("vocab_copy_kernel");
       }
       if (!direct && (p.dw_slice || last)) {
         const bool pairs = gemm_paired(p.bd, EPI_SLICE, true, true, (int)V);
         const int bm = pairs ? 256 : 128, grid = pairs ? sms / 2 : sms;
         const bool split = p.dw_slice && slice_shape((int)V, (int)D, (int)n, bm, p.bd, grid).q > kSplitSlices;
-        (split ? vocab_dw_kernel<true> : vocab_dw_kernel<false>)<<<
-            dim3((unsigned)(split ? V : ceil_div(V, 8)), (unsigned)ceil_div(D, 256)), 256, 0, st>>>(
-            p.dw_slice ? (const float*)(ws + p.dws) : acc, p.Dp, p.dw_slice ? slabs : nullptr, bm, p.bd, grid, count, off, n,
-            acc, p.dw_slice && q > 0, last, V, D, c.dw_f32, c.dw, (long)c.lddw);
+        PL_CUDA(launch_early((split ? vocab_dw_kernel<true> : vocab_dw_kernel<false>),
+                             dim3((unsigned)(split ? V : ceil_div(V, 8)), (unsigned)ceil_div(D, 256)), 256, 0, st,
+                              p.dw_slice ? (const float*)(ws + p.dws) : acc, p.Dp, p.dw_slice ? slabs : nullptr, bm,
+                             p.bd, grid, count, off, n, acc, p.dw_slice && q > 0, last, V, D, c.dw_f32, c.dw,
+                             (long)c.lddw));
         count_launch();
-        PL_LAUNCH("vocab_dw_kernel");
       }
     }
   }
