@@ -438,13 +438,19 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Rows up to which the row tile has room for dz twice over: its bf16 values and, 64 rows below, the bf16 values of what
+// their rounding took away (x is repeated there too). The products then carry 16 bits of dz for the price of 8: the
+// row tile and, up to 32 rows, the k-block are no larger. With many rows single roundings average out; with few they
+// stood out (12 rows: dx and dw off by 2.6e-3, bf16's own rounding of them 1.7e-3).
+constexpr long kVocabLo = 64;
+
 // The f16 terms of a tile of `rpb` rows x 256 NS columns become dz in place (bf16): t 2^(max - lse - 15) scale, and
 // at the answer's columns the f32 values of the rows kernels. A warp walks the rows, a lane owns 8 columns of every
 // 256. The block first lists the answer entries that fall into its tile (in an order that depends on nothing but the
 // entries) and marks them in a bit mask; the walk leaves marked columns out, and the listed values are written after
 // it. With `part` the column sums of the unrounded values go to part[row tile][V] for dbias. Rows from the count to
-// the next multiple of 64 are zeroed (the weight-gradient product reads whole k-blocks of rows). With `lo` the rounding
-// errors go, in bf16 too, to the rows `lo` below.
+// the next multiple of 64 are zeroed (the weight-gradient product reads whole k-blocks of rows). With LO the rounding
+// errors go, in bf16 too, to the rows kVocabLo below.
 // Bound by HBM: 4 bytes per term.
 constexpr int kDzScan = 16;  // answer entries of a block: 256 kDzScan at most
 template <int NS>
@@ -454,11 +460,12 @@ struct DzSmem {
     return (size_t)rpb * COLS / 8 + (size_t)rpb * K * 8 + (part ? (size_t)8 * COLS * 4 : 0);
   }
 };
-template <int NS, bool PART>
+template <int NS, bool PART, bool LO>
 __global__ void __launch_bounds__(256, PART ? 3 : 4)
     vocab_dz_kernel(void* __restrict__ terms, long ld, long V, int K, const int* __restrict__ count, long off, long n,
-                    int rpb, long lo, RowOut in, const float2* __restrict__ stat, long ld_stat, int seg_shift,
+                    int rpb, RowOut in, const float2* __restrict__ stat, long ld_stat, int seg_shift,
                     float* __restrict__ part) {
+  constexpr long lo = LO ? kVocabLo : 0;
   grid_wait();
   grid_next();
   constexpr int COLS = 256 * NS;
@@ -569,7 +576,7 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
           }
         }
         at4[32 * s] = o;
-        if (lo) {  // what the rounding took away, `lo` rows below
+        if constexpr (LO) {  // what the rounding took away, `lo` rows below
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const float2 h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[j]));
@@ -586,7 +593,7 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
     for (int s = 0; s < NS; s++)
       if (256 * s < left) {
         reinterpret_cast<uint4*>(base + q * ld)[32 * s] = make_uint4(0u, 0u, 0u, 0u);
-        if (lo) reinterpret_cast<uint4*>(base + (q + lo) * ld)[32 * s] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (LO) reinterpret_cast<uint4*>(base + (q + lo) * ld)[32 * s] = make_uint4(0u, 0u, 0u, 0u);
       }
   if (PART) {
 #pragma unroll
@@ -602,7 +609,7 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
     uint16_t* at = tile + (hit_at[h] >> 16) * ld + (hit_at[h] & 0xffffu);
     const __nv_bfloat16 b = __float2bfloat16_rn(hit_v[h]);
     *at = __bfloat16_as_ushort(b);
-    if (lo) at[lo * ld] = __bfloat16_as_ushort(__float2bfloat16_rn(hit_v[h] - __bfloat162float(b)));
+    if constexpr (LO) at[lo * ld] = __bfloat16_as_ushort(__float2bfloat16_rn(hit_v[h] - __bfloat162float(b)));
   }
   if constexpr (PART) {
     // thread t owns the block's columns t, t + 256, ...
@@ -819,11 +826,6 @@ __global__ void __launch_bounds__(256)
 // Rows up to which one row tile holds them all: leaving rows out of the products then saves nothing, so no plan is
 // made (two launches fewer; the rows without an answer are zeroed instead).
 constexpr long kVocabOneTile = 128;
-// Rows up to which the row tile has room for dz twice over: its bf16 values and, 64 rows below, the bf16 values of what
-// their rounding took away (x is repeated there too). The products then carry 16 bits of dz for the price of 8: the
-// row tile and, up to 32 rows, the k-block are no larger. With many rows single roundings average out; with few they
-// stood out (12 rows: dx and dw off by 2.6e-3, bf16's own rounding of them 1.7e-3).
-constexpr long kVocabLo = 64;
 // Weights whose rows do not start at 128-byte lines cost the products' TMA boxes an extra line each. For the three
 // products of a gradient a copy with padded rows pays for itself from about this many rows on: V = 50,048, 4,096 rows,
 // D = 520 / 1,000 / 2,056: 930 / 1,100 / 2,233 us with the copy, 1,114 / 1,108 / 2,328 without; 1,000 rows: 270 / 352 /
@@ -964,14 +966,14 @@ struct VocabCall {
 static bool rows16(const void* p, size_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 static bool rows128(const void* p, size_t ld) { return ((uintptr_t)p & 127) == 0 && ld % 64 == 0; }
 
-template <int NS, bool PART>
+template <int NS, bool PART, bool LO>
 static int dz_launch(const VocabPlan& p, uint8_t* ws, long V, long K, const int* count, long off, long n, RowOut ro,
                      float* part, cudaStream_t st) {
   const size_t smem = DzSmem<NS>::bytes(p.rpb, K, PART);
   if (smem > 48 * 1024)
-    PL_CUDA(cudaFuncSetAttribute(vocab_dz_kernel<NS, PART>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    PL_CUDA(cudaFuncSetAttribute(vocab_dz_kernel<NS, PART, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const dim3 grid((unsigned)ceil_div(V, 256 * NS), (unsigned)(round_up(n, 64) / p.rpb));
-  PL_CUDA(launch_early(vocab_dz_kernel<NS, PART>, grid, 256, smem, st, ws + p.terms, p.ldt, V, (int)K, count, off, n, p.rpb, p.lo, ro,
+  PL_CUDA(launch_early(vocab_dz_kernel<NS, PART, LO>, grid, 256, smem, st, ws + p.terms, p.ldt, V, (int)K, count, off, n, p.rpb, ro,
                        (const float2*)(ws + p.stat), p.ld_stat, p.bn == 256 ? 7 : 6, part));
   count_launch();
   return PL_OK;
@@ -1102,8 +1104,11 @@ static int vocab_run(const VocabCall& c) {
     if (!c.grad) continue;
     const bool last = q == p.pieces - 1;
     float* part = bias ? (float*)(ws + p.part) : nullptr;
-    const auto dz = p.ns == 4 ? (bias ? dz_launch<4, true> : dz_launch<4, false>)
-                              : (bias ? dz_launch<1, true> : dz_launch<1, false>);
+    const auto wide = lo ? (bias ? dz_launch<4, true, true> : dz_launch<4, false, true>)
+                         : (bias ? dz_launch<4, true, false> : dz_launch<4, false, false>);
+    const auto narrow = lo ? (bias ? dz_launch<1, true, true> : dz_launch<1, false, true>)
+                           : (bias ? dz_launch<1, true, false> : dz_launch<1, false, false>);
+    const auto dz = p.ns == 4 ? wide : narrow;
     rc = dz(p, ws, V, k1, count, off, n, ro, part, st);
     if (rc) return rc;
     if (bias) {
