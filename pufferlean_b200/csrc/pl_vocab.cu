@@ -642,26 +642,27 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
   }
 }
 
-// sum (+)= the row tiles' column sums; on the last piece dbias = sum (f32 or bf16). 32 columns to a block, 32 slices of
+// sum (+)= the row tiles' column sums; on the last piece dbias = sum (f32 or bf16). 32 columns to a block, S slices of
 // the tiles, both folded in a fixed order.
-__global__ void __launch_bounds__(1024)
+template <int S>
+__global__ void __launch_bounds__(32 * S)
     vocab_dbias_kernel(const float* __restrict__ part, int tiles, long V, float* __restrict__ acc, int first, int last,
                        int f32, void* __restrict__ dbias) {
   grid_wait();
   grid_next();
-  __shared__ float scr[32][33];
+  __shared__ float scr[S][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const long c0 = (long)blockIdx.x * 32;
+  const long v = (long)blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c0 + lane < V) {
-#pragma unroll 4
-    for (int q = slice; q < tiles; q += 32) s += part[(long)q * V + c0 + lane];
+  if (v < V) {
+#pragma unroll 8
+    for (int q = slice; q < tiles; q += S) s += part[(long)q * V + v];
   }
   scr[slice][lane] = s;
   __syncthreads();
-  s = warp_sum_f(scr[lane][slice]);  // warp `slice` folds column `slice` of the block
-  const long v = c0 + slice;
-  if (lane || v >= V) return;
+  if (slice || v >= V) return;
+#pragma unroll
+  for (int q = 1; q < S; q++) s += scr[q][lane];
   if (!first) s += acc[v];
   if (!last)
     acc[v] = s;
@@ -682,8 +683,9 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return o;
 }
 
-// A lane's eight values of a sliced product at row `row` (plus, with `lo`, that many rows below), columns [c, c + 8). SPLIT: the block's warps share the
-// slices and warp 0 has the sums (added in a fixed order). False where the lane has nothing to write.
+// A lane's eight values of a sliced product at row `row` (plus, with `lo`, that many rows below), columns [c, c + 8).
+// SPLIT: the block's warps share the slices and warp 0 has the sums (added in a fixed order). False where the lane has
+// nothing to write.
 template <bool SPLIT>
 __device__ __forceinline__ bool slices_of(const SliceShape& s, const float* out, long ldo, const float* slabs, int bm,
                                           int bn, long row, long lo, long c, long D, float (&v)[8]) {
@@ -1113,7 +1115,11 @@ static int vocab_run(const VocabCall& c) {
     if (rc) return rc;
     if (bias) {
       const int tiles = (int)(round_up(n, 64) / p.rpb);
-      PL_CUDA(launch_early(vocab_dbias_kernel, (unsigned)ceil_div(V, 32), 1024, 0, st, part, tiles, V, (float*)(ws + p.dbacc), q == 0, last, c.dw_f32, c.dbias));
+      // a few dozen tiles: eight loads to a thread; thousands (many rows of a small vocabulary): more threads
+      const bool few = tiles <= 256;
+      PL_CUDA(launch_early(few ? vocab_dbias_kernel<8> : vocab_dbias_kernel<32>, (unsigned)ceil_div(V, 32),
+                           few ? 256 : 1024, 0, st, part, tiles, V, (float*)(ws + p.dbacc), q == 0, last, c.dw_f32,
+                           c.dbias));
       count_launch();
     }
     float* slabs = (float*)(ws + p.slabs);
