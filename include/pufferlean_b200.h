@@ -533,7 +533,8 @@ int pl_policy_restore(const char* path, size_t* P, size_t* handle);
  * with a stride that is a multiple of 8 go to the tensor cores as they lie, others are copied first. Workspaces are
  * the caller's (256-byte aligned, no contents kept between calls): calls on several streams need one each.
  *
- * Gradients here are of sum_n scale_n loss_n (descent); Muon ascends, so pass negative scales for it. */
+ * Gradients here are of sum_n scale_n loss_n (descent); Muon ascends, so pass negative scales for it.
+ * No output and no workspace may overlap an input or one another. */
 
 /* Layer norm over the columns of x [rows x cols] (f32, or bf16 with bf16 = 1; y likewise): y = (x - mean) rstd w + b,
  * rstd = 1 / sqrt(var + eps). w, b [cols] f32, each may be NULL; mean, rstd [rows] f32 are written for the gradient. */
@@ -556,9 +557,10 @@ int pl_layernorm_grad_dev(const void* dy, size_t lddy, const void* x, size_t ldx
  * p = softmax(teacher / temperature) over the present entries, loss_n = sum_k p_k (log p_k - u_n,id_k) + lse_n = KL(p | q).
  * A row with no entry is left out like a negative target; entries that name the same id add up.
  *
- * ws: pl_vocab_ws bytes (K = 0 for the cross entropy, else at most 512; aligned = 1 when x and dw
- * start at 16 bytes with row strides that are multiples of 8, and w at 128 with one that is a multiple of 64). The gradient forms keep one piece of rows' softmax terms there (2 bytes each): piece_bytes
- * bounds that piece, 0 = 4 GiB; the results do not depend on it beyond the order of dw's f32 sums.
+ * ws: pl_vocab_ws bytes (K = 0 for the cross entropy, else at most 512; aligned = 1 when x and dw start at 16 bytes
+ * with row strides that are multiples of 8, and w at 128 with one that is a multiple of 64). The gradient forms keep
+ * one piece of rows' softmax terms there (2 bytes each): piece_bytes bounds that piece, 0 = 4 GiB; the results do not
+ * depend on it beyond the order of dw's f32 sums.
  * dx [N x D] bf16; dw [V x D] and dbias [V] (given exactly when bias is) bf16, or f32 with dw_f32 = 1. dw's f32 sums are
  * of products whose logit gradients were rounded to bf16 (up to 64 rows: to two bf16 parts). row_scale [N] f32 or NULL
  * (ones). */

@@ -617,3 +617,60 @@ def test_vocab_few_rows_round_once(N, K):
     dwr = ref["dz"].t() @ x.double()
     _close(dw, dwr, off.t() @ x.double().abs() + 1e-4 * B * (ref["dz"].abs().t() @ x.double().abs())
            + B * 1.01 * dwr.abs(), "dw")
+
+
+@pytest.mark.parametrize("N,V,D,K", [(40, 70, 32, 512), (300, 600, 64, 300), (9, 3000, 200, 128)])
+def test_vocab_distill_long_lists(N, V, D, K):
+    """As many entries as a row may have, and lists that name most of the vocabulary, some of it many times."""
+    x, w, b, ids, teacher, scale = _head_case(_gen(K), N, V, D, K, True, 0, 0)
+    _check_head(x, w, b, ids, teacher, 1.0, scale)
+
+
+def test_vocab_wide_rows():
+    x, w, b, ids, _, scale = _head_case(_gen(77), 140, 500, 9001, 0, True, 3, 1)
+    _check_head(x, w, b, ids, None, 1.0, scale)
+
+
+def test_vocab_past_32_bits():
+    """Terms beyond 2^31 elements, in two pieces: rows at both ends against 64 bits, and the weight gradient of a few
+    tokens summed over all rows."""
+    g = _gen(99)
+    N, V, D = 16500, 131100, 64
+    x, w = _randn(g, N, D).to(BF16), (_randn(g, V, D) * 0.2).to(BF16)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda").to(torch.int32)
+    t[-3] = V - 1
+    t[5] = 0
+    loss, lse, dx, dw, _ = tokens.vocab_ce_grad(x, w, t)
+    rows = torch.tensor([0, 5, 8191, 8192, 12345, N - 3, N - 1], device="cuda")
+    ones = torch.ones(len(rows), device="cuda")
+    xs, ts = x[rows], t[rows]
+    ref = _head_ref(xs, w, None, ts, None, 1.0, ones)
+    tol_z, tol_loss = _head_tol(ref, xs, w, None, ts, 1.0)
+    _close(loss[rows], ref["loss"], tol_loss, "loss")
+    _close(lse[rows], ref["lse"], tol_loss, "lse")
+    off = (B + H) * ref["dz"].abs() + (H + 4 * tol_z[:, None] + 2.0 ** -18) * ref["q"] + 2.0 ** -18 * ref["dz"].abs()
+    wa = w.double().abs()
+    dxr = ref["dz"] @ w.double()
+    _close(dx[rows], dxr, off @ wa + (V / 16 + 200) * F2 * (ref["dz"].abs() @ wa) + B * 1.01 * dxr.abs(), "dx")
+    cols = torch.tensor([0, 1, 77777, V - 1], device="cuda")
+    q = torch.exp(x.double() @ w[cols].double().t() - lse.double()[:, None])
+    dz = q - (t[:, None] == cols[None]).double()
+    dwr = dz.t() @ x.double()
+    xa = x.double().abs()
+    off = (B + H) * dz.abs() + (H + 2.0 ** -16) * q
+    _close(dw[cols], dwr, off.t() @ xa + (N / 16 + 200) * F2 * (dz.abs().t() @ xa) + B * 1.01 * dwr.abs(), "dw")
+
+
+def test_layer_norm_past_32_bits():
+    rows, cols = 140000, 16384
+    x = torch.empty(rows, cols, dtype=BF16, device="cuda")
+    x.normal_(generator=_gen(3))
+    y, m, r = tokens.layer_norm(x)
+    at = torch.tensor([0, 1, 131071, 131072, rows - 1], device="cuda")
+    yr, mr, rr = _norm_ref(x[at], None, None, 1e-5)
+    _close(m[at], mr, torch.full_like(mr, 64 * F2 * 6), "mean")
+    _close(y[at], yr, (B + 2.0 ** -16) * yr.abs() + 2.0 ** -16, "y")
+    dx, dw, db = tokens.layer_norm_grad(y, x, None, m, r)
+    dxr, _, _, xh, gg = _norm_grad_ref(y[at], x[at], None, m[at], r[at])
+    _close(dx[at], dxr, B * dxr.abs() + 2.0 ** -16 * (1 + xh.abs()) * (1 + gg.abs()), "dx")
+    assert torch.isfinite(dw).all() and torch.isfinite(db).all()
