@@ -549,6 +549,9 @@ int pl_layernorm_grad_dev(const void* dy, size_t lddy, const void* x, size_t ldx
 
 /* The head's logits are u = (x w^T + bias) / temperature with x [N x D], w [V x D], bias [V] or NULL, all bf16
  * (f32 accumulation); they are never written out. loss, lse [N] f32.
+ * A bias of -inf, or a large negative one, masks its token. A finite bias / temperature counts as at most 6.9e37 in
+ * size (1e38 in units of log 2), so that the type's lowest value stays finite; a row whose tokens are all masked by one
+ * finite value has the uniform distribution, by -inf a loss of NaN.
  *
  * Cross entropy: target [N] int32, loss_n = lse_n - u_n,target (minus the log-probability of the target). A negative
  * target leaves the row out: loss = lse = 0, no gradient, and no work in the products. A target >= V makes the row's

@@ -601,9 +601,12 @@ __device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, const VocabPre
 #pragma unroll
     for (int i = 0; i < 4; i++) mx[i] = fmaxf(mx[i], v[j + i]);
   }
-  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;  // scale > 0
-  const float ref = top == -INFINITY ? 0.f : top;  // a row with nothing but -inf here: every term 0
-  const float shift = 15.f - ref;
+  const float big = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  const float top = big * scale;  // scale > 0
+  // The difference to the maximum first, then the 15: in 15 - max the 15 is rounded away beside a large logit (a finite
+  // mask on every token), in v scale - max the product and the maximum are rounded apart.
+  const float neg = big == -INFINITY ? 0.f : -big;  // a row with nothing but -inf here: every term 0
+  const float2 neg2 = make_float2(neg, neg), scale2 = make_float2(scale, scale), up2 = make_float2(15.f, 15.f);
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   const bool ok = row < rows;
   uint16_t* out = reinterpret_cast<uint16_t*>(ep.out) + (long)row * ep.ldo + n0;
@@ -612,7 +615,8 @@ __device__ __forceinline__ void epilogue_vocab(const EpiArgs& ep, const VocabPre
     uint32_t u[8];
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
-      const float a = ex2(__fmaf_rn(v[c + j], scale, shift)), b = ex2(__fmaf_rn(v[c + j + 1], scale, shift));
+      const float2 e = __ffma2_rn(__fadd2_rn(make_float2(v[c + j], v[c + j + 1]), neg2), scale2, up2);
+      const float a = ex2(e.x), b = ex2(e.y);
       sum[j & 3] += a;
       sum[(j & 3) + 1] += b;
       const __half2 h = __floats2half2_rn(a, b);

@@ -254,7 +254,9 @@ __global__ void __launch_bounds__(256)
   copy_row(dst + i * ldd, src + i * ld, (long)blockIdx.y * 1024, D, true, threadIdx.x & 31);
 }
 
-// The row's lse in log2 units from its segments' (max, sum); a fixed order over the threads t of `threads`.
+// The row's (max, sum) in log2 units from its segments'; a fixed order over the threads t of `threads`. The two are kept
+// apart: beside a large maximum (a finite mask on every token) f32 has no room for the logarithm of the sum, and the
+// loss and the gradient need only differences to the maximum.
 __device__ __forceinline__ float2 seg_fold(const float2* __restrict__ sr, long segs, int t, int threads) {
   float m = -INFINITY, s = 0.f;
   for (long q = t; q < segs; q += threads) {
@@ -276,9 +278,9 @@ __device__ __forceinline__ float2 warp_join(float2 v) {
     v = seg_join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
   return v;
 }
-__device__ __forceinline__ float seg_lse(float2 v) { return (v.x == -INFINITY ? 0.f : v.x) + log2f(v.y); }
+__device__ __forceinline__ float2 seg_row(float2 v) { return make_float2(v.x == -INFINITY ? 0.f : v.x, v.y); }
 
-// What the gradient needs of a row of the piece: info[i] = (lse in log2 units, scale / T; 0 where it does not
+// What the gradient needs of a row of the piece: info[i] = (max in log2 units, scale / T / sum; 0 where it does not
 // count), and per answer entry the column (-1: absent) and the gradient there, in f32.
 struct RowOut {
   float2* info;
@@ -379,23 +381,25 @@ __global__ void __launch_bounds__(256)
   const long r = rows ? rows[off + i] : off + i;
   const int t = target[r];
   if (t < 0) return row_without(r, i, 1, lane, loss, lse, o);
-  float lse2 = seg_lse(warp_join(seg_fold(stat + i * ld_stat, ld_stat, lane, 32)));
+  float2 ms = seg_row(warp_join(seg_fold(stat + i * ld_stat, ld_stat, lane, 32)));
   if (lane) return;
   float u = 0.f;
   if (t >= V)
-    lse2 = NAN;  // a target past the vocabulary: seen in the loss
+    ms.y = NAN;  // a target past the vocabulary: seen in the loss
   else
     u = ut[i];
-  loss[r] = (lse2 - u) * kLn2;
-  lse[r] = lse2 * kLn2;
+  const float log_sum = log2f(ms.y);
+  loss[r] = ((ms.x - u) + log_sum) * kLn2;
+  lse[r] = (ms.x + log_sum) * kLn2;
   if (o.info) {
     const float scale = row_scale ? row_scale[r] : 1.f;
-    o.info[i] = make_float2(lse2, scale);
+    o.info[i] = make_float2(ms.x, scale == 0.f ? 0.f : scale / ms.y);
     o.col[i] = t;
-    o.val[i] = (exp2f(u - lse2) - 1.f) * scale;
+    o.val[i] = (exp2f(u - ms.x) / ms.y - 1.f) * scale;
   }
 }
-// Distillation: ids2, p, ent of the teacher kernel, uk of the dots kernel.
+// Distillation: ids2, p, ent of the teacher kernel, uk of the dots kernel. The p of a row sum to one, so the row's
+// maximum is taken from every u before they are weighted.
 __global__ void __launch_bounds__(256)
     vocab_distill_rows_kernel(long V, int K, const int* __restrict__ ids2, const float* __restrict__ p,
                               const float* __restrict__ ent, const uint8_t* __restrict__ has, float inv_t,
@@ -410,7 +414,7 @@ __global__ void __launch_bounds__(256)
   if (i >= rows_here(count, off, n)) return;
   const long r = rows ? rows[off + i] : off + i;
   if (!has[r]) return row_without(r, i, K, lane, loss, lse, o);
-  float lse2 = seg_lse(warp_join(seg_fold(stat + i * ld_stat, ld_stat, lane, 32)));
+  float2 ms = seg_row(warp_join(seg_fold(stat + i * ld_stat, ld_stat, lane, 32)));
   const float scale = (row_scale ? row_scale[r] : 1.f) * inv_t;
   float acc = 0.f;
   bool bad = false;
@@ -420,9 +424,9 @@ __global__ void __launch_bounds__(256)
     if (c >= V) {
       bad = true;
     } else if (c >= 0) {
-      const float q = p[r * K + k], u = uk[i * K + k];
+      const float q = p[r * K + k], u = uk[i * K + k] - ms.x;
       if (!(q == 0.f)) acc = __fmaf_rn(-q, u, acc);
-      val = (exp2f(u - lse2) - q) * scale;
+      val = (exp2f(u) / ms.y - q) * scale;
     }
     if (o.info) {
       o.col[i * K + k] = c;
@@ -430,11 +434,12 @@ __global__ void __launch_bounds__(256)
     }
   }
   acc = warp_sum_f(acc);
-  if (__any_sync(0xffffffffu, bad)) lse2 = NAN;  // an id past the vocabulary: seen in the loss
+  if (__any_sync(0xffffffffu, bad)) ms.y = NAN;  // an id past the vocabulary: seen in the loss
   if (lane == 0) {
-    loss[r] = (ent[r] + acc + lse2) * kLn2;
-    lse[r] = lse2 * kLn2;
-    if (o.info) o.info[i] = make_float2(lse2, scale);
+    const float log_sum = log2f(ms.y);
+    loss[r] = (ent[r] + acc + log_sum) * kLn2;
+    lse[r] = (ms.x + log_sum) * kLn2;
+    if (o.info) o.info[i] = make_float2(ms.x, scale == 0.f ? 0.f : scale / ms.y);
   }
 }
 
@@ -444,10 +449,11 @@ __global__ void __launch_bounds__(256)
 // stood out (12 rows: dx and dw off by 2.6e-3, bf16's own rounding of them 1.7e-3).
 constexpr long kVocabLo = 64;
 
-// The f16 terms of a tile of `rpb` rows x 256 NS columns become dz in place (bf16): t 2^(max - lse - 15) scale, and
-// at the answer's columns the f32 values of the rows kernels. A warp walks the rows, a lane owns 8 columns of every
-// 256. The block first lists the answer entries that fall into its tile (in an order that depends on nothing but the
-// entries) and marks them in a bit mask; the walk leaves marked columns out, and the listed values are written after
+// The f16 terms of a tile of `rpb` rows x 256 NS columns become dz in place (bf16): t 2^(segment's max - max - 15)
+// scale / sum, and at the answer's columns the f32 values of the rows kernels. A warp walks the rows, a lane owns 8
+// columns of every 256. The block first lists the answer entries that fall into its tile (in an order that depends on
+// nothing but the entries) and marks them in a bit mask; the walk leaves marked columns out, and the listed values are
+// written after
 // it. With `part` the column sums of the unrounded values go to part[row tile][V] for dbias. Rows from the count to
 // the next multiple of 64 are zeroed (the weight-gradient product reads whole k-blocks of rows). With LO the rounding
 // errors go, in bf16 too, to the rows kVocabLo below.
@@ -537,7 +543,7 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
     __syncthreads();
 #pragma unroll 2
     for (int q = warp; q < nr; q += 8) {
-      const float2 f = __ldg(in.info + r0 + q);  // (lse2, scale)
+      const float2 f = __ldg(in.info + r0 + q);  // (max, scale / sum)
       uint4* at4 = reinterpret_cast<uint4*>(base + q * ld);
       const float2* sr = stat + (r0 + q) * ld_stat;
       uint4 raw[NS];

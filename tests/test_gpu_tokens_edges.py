@@ -1,0 +1,73 @@
+"""Edges of the token-policy operators: logits that a mask or a constant makes equal over the whole vocabulary.
+Tolerances as in test_gpu_tokens.py."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from pufferlean_b200 import tokens  # noqa: E402
+from .test_gpu_tokens import B, BF16, F2, F64, H, _answers, _close, _gen, _head_case  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+# ------------------------------------------------------------------------------------------------ equal logits
+def _check_flat(x, w, b, ids, teacher, T, scale, logit):
+    """Every logit of row n is logit[n], exactly, so q = 1 / V however large it is. What is left of _check_head's bounds
+    is without the logits' own error. (logsumexp would lose log V beside a large logit in 64 bits too.)"""
+    N, V = len(x), w.shape[0]
+    if teacher is None:
+        loss, lse, dx, dw, db = tokens.vocab_ce_grad(x, w, ids, b, scale)
+    else:
+        loss, lse, dx, dw, db = tokens.vocab_distill_grad(x, w, ids, teacher, b, T, scale)
+    want, ent, has = _answers(ids, teacher, V, T)
+    log_v = math.log(V)
+    _close(loss, torch.where(has, ent + log_v, 0.0), 2.0 ** -20 * (1 + log_v + ent.abs()), "loss")
+    u = logit / T
+    if float(u.abs().max()) < 6e37:  # above, a bias counts as 1e38 in units of log 2
+        _close(lse, torch.where(has, u + log_v, 0.0), 2.0 ** -21 * (1 + log_v + u.abs()), "lse")
+    s = torch.where(has, scale.double() / T, 0.0)[:, None]
+    dz = s * (1.0 / V - want)
+    off = (B + H) * dz.abs() + (H + 2.0 ** -18) * s.abs() / V + 2.0 ** -18 * dz.abs()
+    xd = torch.where(has[:, None], x.double(), 0.0)
+    wa, xa = w.double().abs(), xd.abs()
+    dxr, dwr = dz @ w.double(), dz.t() @ xd
+    _close(dx, dxr, off @ wa + (V / 16 + 200) * F2 * (dz.abs() @ wa) + B * 1.01 * dxr.abs() + 1e-30, "dx")
+    _close(dw, dwr, off.t() @ xa + (N / 16 + 200) * F2 * (dz.abs().t() @ xa) + B * 1.01 * dwr.abs() + 1e-30, "dw")
+    if b is not None:
+        dbr = dz.sum(0)
+        _close(db, dbr, off.sum(0) + (N + 200) * F2 * dz.abs().sum(0) + B * 1.01 * dbr.abs() + 1e-30, "dbias")
+
+
+@pytest.mark.parametrize("value", [torch.finfo(BF16).min, -1e30, -2.0 ** 29, -1.5 * 2.0 ** 26, -1.25 * 2.0 ** 23, 2.0 ** 25,
+                                   -1e4, 0.0])
+@pytest.mark.parametrize("K,T", [(0, 1.0), (3, 2.0)])
+@pytest.mark.parametrize("N,V", [(20, 1500), (300, 1500), (140, 19100)])
+def test_whole_vocabulary_masked(N, V, K, T, value):
+    """One finite bias on every token (a mask that leaves a row nothing): the softmax is uniform, as in plain f32. The
+    hidden states and the weights share no column, so that the bias is all there is to a logit."""
+    x, w, b, ids, teacher, scale = _head_case(_gen(N + V + K), N, V, 64, K, True, 0, 0)
+    x[:, 32:] = 0
+    w[:, :32] = 0
+    b[:] = value
+    _check_flat(x, w, b, ids, teacher, T, scale, torch.full((N,), float(b[0]), dtype=F64, device="cuda"))
+
+
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 24, 1.5 * 2.0 ** 27, 2.0 ** 60])
+@pytest.mark.parametrize("N,V", [(20, 1500), (300, 19100)])
+def test_equal_large_logits(N, V, size):
+    """The same from the product: every token has one large logit."""
+    g = _gen(N + V)
+    x, w, _, ids, _, scale = _head_case(g, N, V, 64, 0, False, 0, 0)
+    x[:, 32:] = 0
+    w[:, :32] = 0
+    x[:, 0] = torch.where(torch.rand(N, generator=g, device="cuda") < 0.5, -1.0, 1.0).to(BF16)
+    w[:, 0] = size
+    _check_flat(x, w, None, ids, None, 1.0, scale, x[:, 0].double() * size)
