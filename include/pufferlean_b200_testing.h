@@ -83,6 +83,9 @@ int pl_test_lstm_quad(int mode);
 int pl_test_comm_fake(int mode);
 /* Number of communicator aborts the fakes have received. */
 int pl_test_comm_fake_aborts(void);
+/* The table that remembers how much dynamic shared memory a kernel may use on a device, without the device: `set` is
+ * called (and its status returned) when `kernel` is not yet known to be allowed `bytes` on `device`. */
+int pl_test_raise_smem(int device, const void* kernel, size_t bytes, int (*set)(const void* kernel, size_t bytes));
 /* Reads and clears the device-side bounded-wait error word (0 = none). */
 int pl_test_device_error(unsigned* code);
 

@@ -187,19 +187,8 @@ int gemm_launch(int bn, int epi, bool a_mn, bool b_mn, const Operand& A, const O
     const long tiles = ceil_div(N, bn) * ceil_div(M, 128) * (long)(splits > 1 ? splits : batch);
     grid = dim3((unsigned)(tiles < sms && epi != EPI_SLICE ? tiles : sms), 1, 1);
   }
-  static std::mutex mu;
-  {
-    std::lock_guard<std::mutex> g(mu);
-    static void* configured[256];
-    static int nconf = 0;
-    bool found = false;
-    for (int i = 0; i < nconf; i++)
-      if (configured[i] == (void*)k) found = true;
-    if (!found) {
-      PL_CUDA(cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-      if (nconf < 256) configured[nconf++] = (void*)k;
-    }
-  }
+  rc = raise_smem((const void*)k, smem);
+  if (rc) return rc;
   if (ep.pdl)
     PL_CUDA(launch_early(k, grid, dim3(320), smem, st, ma, mb, mc, mc2, M, N, K, ep));
   else

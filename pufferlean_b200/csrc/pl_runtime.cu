@@ -125,4 +125,37 @@ void* scratch(int slot, size_t bytes) {
   }
   return g_scratch[dev][slot];
 }
+
+struct SmemLimit {
+  const void* kernel;
+  size_t bytes;
+};
+static SmemLimit g_smem[64][256];
+static int g_smem_n[64];
+static std::mutex g_smem_mu;
+
+int raise_smem_on(int device, const void* kernel, size_t bytes, int (*set)(const void*, size_t)) {
+  if (device < 0 || device >= 64) return set(kernel, bytes);
+  std::lock_guard<std::mutex> g(g_smem_mu);
+  SmemLimit* t = g_smem[device];
+  int i = 0;
+  while (i < g_smem_n[device] && t[i].kernel != kernel) i++;
+  if (i < g_smem_n[device] && t[i].bytes >= bytes) return PL_OK;
+  const int rc = set(kernel, bytes);
+  if (rc == PL_OK && i < 256) {
+    t[i] = SmemLimit{kernel, bytes};
+    if (i == g_smem_n[device]) g_smem_n[device]++;
+  }
+  return rc;
+}
+
+static int set_smem(const void* kernel, size_t bytes) {
+  PL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return PL_OK;
+}
+int raise_smem(const void* kernel, size_t bytes) {
+  int dev = 0;
+  PL_CUDA(cudaGetDevice(&dev));
+  return raise_smem_on(dev, kernel, bytes, set_smem);
+}
 }  // namespace pl

@@ -2,6 +2,7 @@
 #include "../../include/pufferlean_b200_testing.h"
 #include "pl_gemm.cuh"
 #include "pl_mlp.cuh"
+#include "pl_runtime.h"
 
 extern "C" int pl_test_gemm(const pl_test_gemm_args* g, void* stream) {
   PL_REQUIRE(g != nullptr, PL_ERR_INVALID, "pl_test_gemm: NULL args");
@@ -46,6 +47,10 @@ extern "C" int pl_test_gemm_pair_mode(int mode) { return pl::gemm_set_pair_mode(
 extern "C" int pl_test_ns_small_mode(int mode) { return pl::ns_set_small_mode(mode); }
 extern "C" int pl_test_ns_chain_mode(int mode) { return pl::ns_set_chain_mode(mode); }
 extern "C" int pl_test_ns_chain_capture(int mode) { return pl::ns_set_chain_capture(mode); }
+
+extern "C" int pl_test_raise_smem(int device, const void* kernel, size_t bytes, int (*set)(const void*, size_t)) {
+  return pl::raise_smem_on(device, kernel, bytes, set);
+}
 
 extern "C" int pl_test_device_error(unsigned* code) {
   unsigned* w = pl::device_error_word();

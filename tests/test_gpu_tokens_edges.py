@@ -1,4 +1,5 @@
-"""Edges of the token-policy operators: logits that a mask or a constant makes equal over the whole vocabulary.
+"""Edges of the token-policy operators: logits that a mask or a constant makes equal over the whole vocabulary, and a
+process that uses them on two devices.
 Tolerances as in test_gpu_tokens.py."""
 import math
 
@@ -71,3 +72,14 @@ def test_equal_large_logits(N, V, size):
     x[:, 0] = torch.where(torch.rand(N, generator=g, device="cuda") < 0.5, -1.0, 1.0).to(BF16)
     w[:, 0] = size
     _check_flat(x, w, None, ids, None, 1.0, scale, x[:, 0].double() * size)
+
+
+# ------------------------------------------------------------------------------------------------ devices
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_two_devices():
+    """One process, one device after the other: the same bits on both."""
+    x, w, b, ids, _, scale = _head_case(_gen(3), 300, 3000, 128, 0, True, 0, 0)
+    one = tokens.vocab_ce_grad(x, w, ids, b, scale)
+    two = tokens.vocab_ce_grad(*(t.to("cuda:1") for t in (x, w, ids, b, scale)))
+    for p, q in zip(one, two):
+        assert torch.equal(p, q.to("cuda:0"))
