@@ -86,6 +86,9 @@ int pl_test_comm_fake_aborts(void);
 /* The table that remembers how much dynamic shared memory a kernel may use on a device, without the device: `set` is
  * called (and its status returned) when `kernel` is not yet known to be allowed `bytes` on `device`. */
 int pl_test_raise_smem(int device, const void* kernel, size_t bytes, int (*set)(const void* kernel, size_t bytes));
+/* The dynamic shared memory that the kernel from softmax terms to gradients (1,024 columns, with a bias) may use on the
+ * current device. */
+int pl_test_vocab_dz_smem(int* bytes);
 /* Reads and clears the device-side bounded-wait error word (0 = none). */
 int pl_test_device_error(unsigned* code);
 

@@ -20,6 +20,7 @@
 // writing of dW; with few rows of a small vocabulary the launches.
 #include <cuda_fp16.h>
 
+#include "../../include/pufferlean_b200_testing.h"
 #include "pl_common.cuh"
 #include "pl_gemm.cuh"
 #include "pl_runtime.h"
@@ -465,6 +466,7 @@ struct DzSmem {
   static size_t bytes(int rpb, long K, bool part) {
     return (size_t)rpb * COLS / 8 + (size_t)rpb * K * 8 + (part ? (size_t)8 * COLS * 4 : 0);
   }
+  static size_t most(bool part) { return bytes(64, 256 * kDzScan / 64, part); }  // of every plan
 };
 template <int NS, bool PART, bool LO>
 __global__ void __launch_bounds__(256, PART ? 3 : 4)
@@ -978,8 +980,9 @@ template <int NS, bool PART, bool LO>
 static int dz_launch(const VocabPlan& p, uint8_t* ws, long V, long K, const int* count, long off, long n, RowOut ro,
                      float* part, cudaStream_t st) {
   const size_t smem = DzSmem<NS>::bytes(p.rpb, K, PART);
-  if (smem > 48 * 1024)
-    PL_CUDA(cudaFuncSetAttribute(vocab_dz_kernel<NS, PART, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  // once per device, to what the largest call needs: another thread's call may launch the same kernel at any time
+  const int rc = raise_smem((const void*)vocab_dz_kernel<NS, PART, LO>, DzSmem<NS>::most(PART));
+  if (rc) return rc;
   const dim3 grid((unsigned)ceil_div(V, 256 * NS), (unsigned)(round_up(n, 64) / p.rpb));
   PL_CUDA(launch_early(vocab_dz_kernel<NS, PART, LO>, grid, 256, smem, st, ws + p.terms, p.ldt, V, (int)K, count, off, n, p.rpb, ro,
                        (const float2*)(ws + p.stat), p.ld_stat, p.bn == 256 ? 7 : 6, part));
@@ -1199,6 +1202,13 @@ static int vocab_run(const VocabCall& c) {
 }  // namespace pl
 
 extern "C" {
+
+int pl_test_vocab_dz_smem(int* bytes) {
+  cudaFuncAttributes a;
+  PL_CUDA(cudaFuncGetAttributes(&a, (const void*)pl::vocab_dz_kernel<4, true, false>));
+  *bytes = a.maxDynamicSharedSizeBytes;
+  return PL_OK;
+}
 
 size_t pl_vocab_ws(size_t N, size_t V, size_t D, size_t K, uint8_t bias, uint8_t grad, uint8_t aligned,
                    size_t piece_bytes) {

@@ -1,12 +1,15 @@
-"""Edges of the token-policy operators: logits that a mask or a constant makes equal over the whole vocabulary, and a
-process that uses them on two devices.
+"""Edges of the token-policy operators: logits that a mask or a constant makes equal over the whole vocabulary, a process
+that uses them on two devices, and calls from two threads.
 Tolerances as in test_gpu_tokens.py."""
+import ctypes as C
 import math
+import threading
 
 import pytest
 
 torch = pytest.importorskip("torch")
 
+import pufferlean_b200 as plb  # noqa: E402
 from pufferlean_b200 import tokens  # noqa: E402
 from .test_gpu_tokens import B, BF16, F2, F64, H, _answers, _close, _gen, _head_case  # noqa: E402
 
@@ -83,3 +86,55 @@ def test_two_devices():
     two = tokens.vocab_ce_grad(*(t.to("cuda:1") for t in (x, w, ids, b, scale)))
     for p, q in zip(one, two):
         assert torch.equal(p, q.to("cuda:0"))
+
+
+# ------------------------------------------------------------------------------------------------ threads
+class _DistillCall:
+    """A distillation with gradients through the C entry, with buffers and a stream of its own. With these sizes the
+    kernel from terms to gradients takes 53,248 bytes of shared memory at K = 64 and 51,200 at K = 20."""
+    N, V, D = 4096, 5000, 8
+
+    def __init__(self, K):
+        self.K = K
+        self.x, self.w, self.b, self.ids, self.teacher, _ = _head_case(_gen(K), self.N, self.V, self.D, K, True, 0, 0)
+        self.size = plb.lib().pl_vocab_ws(self.N, self.V, self.D, K, 1, 1, 0, 0)
+        self.ws = torch.empty(self.size, dtype=torch.uint8, device="cuda")
+        self.out = [torch.empty(s, dtype=t, device="cuda") for s, t in
+                    ((self.N, torch.float32), (self.N, torch.float32), ((self.N, self.D), BF16), ((self.V, self.D), BF16),
+                     (self.V, BF16))]
+        self.stream = torch.cuda.Stream()
+
+    def __call__(self):
+        loss, lse, dx, dw, db = (t.data_ptr() for t in self.out)
+        return plb.lib().pl_vocab_distill_grad_dev(
+            self.x.data_ptr(), self.D, self.w.data_ptr(), self.D, self.b.data_ptr(), self.ids.data_ptr(),
+            self.teacher.data_ptr(), self.K, 1.0, None, self.N, self.V, self.D, loss, lse, dx, self.D, dw, self.D, db, 0, 0,
+            self.ws.data_ptr(), self.size, self.stream.cuda_stream)
+
+
+def test_two_threads():
+    """Calls of one kernel with different needs from two threads: every launch is accepted, the bits are one thread's."""
+    calls = [_DistillCall(64), _DistillCall(20)]
+    torch.cuda.synchronize()
+    limit = C.c_int()
+    want = []
+    for c in calls:
+        assert c() == 0, plb.lib().pl_last_error()
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in c.out])
+        # what was allowed for the first call still is after the second, smaller one
+        assert plb.lib().pl_test_vocab_dz_smem(C.byref(limit)) == 0 and limit.value >= 53248
+    failed = []
+
+    def go(c):
+        for _ in range(200):
+            if c():
+                failed.append(plb.lib().pl_last_error())
+
+    threads = [threading.Thread(target=go, args=(c,)) for c in calls]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not failed
+    for c, w in zip(calls, want):
+        assert all(torch.equal(p, q) for p, q in zip(c.out, w))

@@ -1,6 +1,7 @@
 """The table of shared-memory limits behind the library's launches, without a device: a limit belongs to one kernel on one
 device, and it only ever grows."""
 import ctypes as C
+import threading
 
 import pytest
 
@@ -32,6 +33,28 @@ def test_failed_limit_is_not_remembered(raise_smem):
     assert raise_smem(62, 0x1000, 100, SET(lambda k, n: calls.append(n) or -3)) == -3
     assert raise_smem(62, 0x1000, 100, SET(lambda k, n: calls.append(n) or 0)) == 0
     assert calls == [100, 100]
+
+
+def test_limit_never_falls(raise_smem):
+    """Two threads that ask for different sizes of one kernel: no call lowers what an earlier one was promised."""
+    limit, seen = [0], []
+
+    def put(k, n):
+        seen.append((limit[0], n))
+        limit[0] = n
+        return 0
+
+    on = SET(put)
+
+    def go(sizes):
+        for n in sizes * 50:
+            assert raise_smem(59, 0x7000, n, on) == 0
+            assert limit[0] >= n
+
+    threads = [threading.Thread(target=go, args=(s,)) for s in ([53248, 51200], [51200, 73728, 50000])]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert limit[0] == 73728 and all(b > a for a, b in seen)
 
 
 def test_full_table_still_sets(raise_smem):
