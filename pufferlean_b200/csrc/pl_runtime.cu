@@ -33,21 +33,23 @@ int check_cuda(cudaError_t e, const char* what) {
 
 void count_launch(uint64_t n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
-static unsigned* g_err_word[64];
-static std::mutex g_err_mu;
+// The word is a variable of the module, so that its first use allocates and clears nothing: that would end a stream
+// capture that a library call runs in.
+static __device__ unsigned g_err_word;
 
 unsigned* device_error_word() {
+  static std::atomic<unsigned*> at[64];
   int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return nullptr;
-  std::lock_guard<std::mutex> g(g_err_mu);
-  if (!g_err_word[dev]) {
-    unsigned* p = nullptr;
-    if (cudaMalloc(&p, sizeof(unsigned)) != cudaSuccess) return nullptr;
-    cudaMemset(p, 0, sizeof(unsigned));
-    g_err_word[dev] = p;
-  }
-  return g_err_word[dev];
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (unsigned* p = at[dev].load(std::memory_order_relaxed)) return p;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // the address itself may be asked for during a capture
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+  void* p = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&p, g_err_word);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return nullptr;
+  at[dev].store((unsigned*)p, std::memory_order_relaxed);
+  return (unsigned*)p;
 }
 
 int device_error_check() {

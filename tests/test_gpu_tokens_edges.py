@@ -1,8 +1,11 @@
 """Edges of the token-policy operators: logits that a mask or a constant makes equal over the whole vocabulary, a process
-that uses them on two devices, and calls from two threads.
+that uses them on two devices, calls from two threads, and a process whose first call is captured.
 Tolerances as in test_gpu_tokens.py."""
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -138,3 +141,49 @@ def test_two_threads():
     assert not failed
     for c, w in zip(calls, want):
         assert all(torch.equal(p, q) for p, q in zip(c.out, w))
+
+
+# ------------------------------------------------------------------------------------------------ capture
+FIRST_CALL = """
+import sys
+import torch
+from pufferlean_b200 import tokens
+
+g = torch.Generator(device="cuda").manual_seed(1)
+x = torch.randn(300, 64, generator=g, device="cuda").to(torch.bfloat16)
+w = torch.randn(2000, 64, generator=g, device="cuda").to(torch.bfloat16)
+b = torch.randn(2000, generator=g, device="cuda").to(torch.bfloat16)
+ids = torch.randint(0, 2000, (300, 5), generator=g, device="cuda").to(torch.int32)
+teacher = torch.randn(300, 5, generator=g, device="cuda")
+gain = torch.ones(64, device="cuda")
+
+
+def step():
+    y, m, r = tokens.layer_norm(x, gain)
+    if sys.argv[1] == "ce":
+        out = tokens.vocab_ce_grad(y, w, ids[:, 0].contiguous(), b)
+    else:
+        out = tokens.vocab_distill_grad(y, w, ids, teacher, b, 2.0)
+    return out + tokens.layer_norm_grad(out[2], x, gain, m, r)
+
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+for t in got:
+    t.zero_()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(got, step()))
+print("same bits")
+"""
+
+
+@pytest.mark.parametrize("which", ["ce", "distill"])
+def test_first_call_can_be_captured(which):
+    """A process whose first calls of all are made under capture: nothing has to be run before."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", FIRST_CALL, which], capture_output=True, text=True, timeout=300, cwd=root,
+                       env=dict(os.environ, PYTHONPATH=root))
+    assert p.returncode == 0 and "same bits" in p.stdout, p.stderr[-2000:]
