@@ -42,6 +42,11 @@ const char* pl_last_error(void);
 int pl_device_count(void);
 /* Selects the device later calls from this thread use (default 0). */
 int pl_set_device(int device);
+/* Waits for the current device and says whether a wait inside one of its kernels ran out since this was last asked:
+ * PL_OK, or PL_ERR_DEVICE_TIMEOUT (and the record is cleared). Such waits are bounded, so that a fault ends in an error
+ * and not in a hang; a kernel that gives up leaves its outputs unwritten. Calls that return before their work is done
+ * (the *_dev entries) cannot say so themselves. Not during a stream capture. */
+int pl_device_check(void);
 /* Number of this library's kernels launched since load (all threads, all devices). */
 uint64_t pl_kernel_launch_count(void);
 
@@ -547,7 +552,10 @@ int pl_layernorm_grad_dev(const void* dy, size_t lddy, const void* x, size_t ldx
                           const float* rstd, size_t rows, size_t cols, uint8_t bf16, void* dx, size_t lddx, float* dw,
                           float* db, void* ws, size_t ws_bytes, void* stream);
 
-/* The head's logits are u = (x w^T + bias) / temperature with x [N x D], w [V x D], bias [V] or NULL, all bf16
+/* A head call whose products gave up waiting (pl_device_check) cannot return an error. As long as the record stands,
+ * the rows that count get a loss of NaN, and the gradients of these calls are NaN.
+ *
+ * The head's logits are u = (x w^T + bias) / temperature with x [N x D], w [V x D], bias [V] or NULL, all bf16
  * (f32 accumulation); they are never written out. loss, lse [N] f32.
  * A bias of -inf, or a large negative one, masks its token. A finite bias / temperature counts as at most 6.9e37 in
  * size (1e38 in units of log 2), so that the type's lowest value stays finite; a row whose tokens are all masked by one

@@ -91,6 +91,8 @@ int pl_test_raise_smem(int device, const void* kernel, size_t bytes, int (*set)(
 int pl_test_vocab_dz_smem(int* bytes);
 /* Reads and clears the device-side bounded-wait error word (0 = none). */
 int pl_test_device_error(unsigned* code);
+/* Writes that word, as a wait that runs out would. */
+int pl_test_set_device_error(unsigned code);
 
 #ifdef __cplusplus
 }

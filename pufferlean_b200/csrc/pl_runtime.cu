@@ -94,6 +94,13 @@ int pl_set_device(int device) {
   return PL_OK;
 }
 
+int pl_device_check(void) {
+  int rc = pl::require_device();
+  if (rc) return rc;
+  PL_CUDA(cudaDeviceSynchronize());  // streams that do not wait for the default one too
+  return pl::device_error_check();
+}
+
 uint64_t pl_kernel_launch_count(void) { return pl::g_launches.load(); }
 
 }  // extern "C"

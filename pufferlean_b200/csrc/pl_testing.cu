@@ -62,3 +62,10 @@ extern "C" int pl_test_device_error(unsigned* code) {
   if (code) *code = v;
   return PL_OK;
 }
+
+extern "C" int pl_test_set_device_error(unsigned code) {
+  unsigned* w = pl::device_error_word();
+  PL_REQUIRE(w, PL_ERR_CUDA, "pl_test_set_device_error: no error word");
+  PL_CUDA(cudaMemcpy(w, &code, sizeof(unsigned), cudaMemcpyHostToDevice));
+  return PL_OK;
+}

@@ -262,6 +262,28 @@ PyObject* vocab(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// check(device index): waits for the device and raises if a wait inside one of the library's kernels ran out
+PyObject* check_device(PyObject*, PyObject* o) {
+  HANDLE_TH_ERRORS
+  const char* what = "check";
+  try {
+    const long index = PyLong_AsLong(o);
+    if (PyErr_Occurred()) return nullptr;
+    if (index < 0 || index >= pl_device_count()) refuse(what, "no CUDA device %ld", index);
+    const On on(at::Device(at::kCUDA, (c10::DeviceIndex)index));
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = pl_device_check();
+    Py_END_ALLOW_THREADS
+    check(rc, what);
+    Py_RETURN_NONE;
+  } catch (const Refused& r) {
+    PyErr_SetString(puffer_error, r.msg.c_str());
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 // set_error(PufferError): the exception that refusals and failed calls raise
 PyObject* set_error(PyObject*, PyObject* e) {
   Py_XINCREF(e);
@@ -273,6 +295,7 @@ PyMethodDef methods[] = {
     {"layer_norm", (PyCFunction)(void (*)(void))layer_norm, METH_FASTCALL, nullptr},
     {"layer_norm_grad", (PyCFunction)(void (*)(void))layer_norm_grad, METH_FASTCALL, nullptr},
     {"vocab", (PyCFunction)(void (*)(void))vocab, METH_FASTCALL, nullptr},
+    {"check", check_device, METH_O, nullptr},
     {"set_error", set_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

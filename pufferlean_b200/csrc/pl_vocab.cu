@@ -354,6 +354,10 @@ __global__ void __launch_bounds__(128)
   }
 }
 
+// The sum of a row, or NaN while the device's error word holds a wait that ran out: its segments may not have been
+// written, and nothing else tells the caller.
+__device__ __forceinline__ float sum_or_nan(float s, const unsigned* err) { return err && *err ? NAN : s; }
+
 // One warp per row: its lse from the segments, the loss, and what the gradient needs.
 __device__ __forceinline__ void row_without(long r, long i, int K, int lane, float* loss, float* lse, const RowOut& o) {
   if (lane == 0) {
@@ -373,7 +377,8 @@ __global__ void __launch_bounds__(256)
     vocab_ce_rows_kernel(const int* __restrict__ target, long V, const float* __restrict__ row_scale,
                          const int* __restrict__ rows, const int* __restrict__ count, long off, long n,
                          const float2* __restrict__ stat, long ld_stat, const float* __restrict__ ut,
-                         float* __restrict__ loss, float* __restrict__ lse, RowOut o) {
+                         const unsigned* __restrict__ err, float* __restrict__ loss, float* __restrict__ lse,
+                         RowOut o) {
   grid_wait();
   grid_next();
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -384,6 +389,7 @@ __global__ void __launch_bounds__(256)
   if (t < 0) return row_without(r, i, 1, lane, loss, lse, o);
   float2 ms = seg_row(warp_join(seg_fold(stat + i * ld_stat, ld_stat, lane, 32)));
   if (lane) return;
+  ms.y = sum_or_nan(ms.y, err);
   float u = 0.f;
   if (t >= V)
     ms.y = NAN;  // a target past the vocabulary: seen in the loss
@@ -406,8 +412,8 @@ __global__ void __launch_bounds__(256)
                               const float* __restrict__ ent, const uint8_t* __restrict__ has, float inv_t,
                               const float* __restrict__ row_scale, const int* __restrict__ rows,
                               const int* __restrict__ count, long off, long n, const float2* __restrict__ stat,
-                              long ld_stat, const float* __restrict__ uk, float* __restrict__ loss,
-                              float* __restrict__ lse, RowOut o) {
+                              long ld_stat, const float* __restrict__ uk, const unsigned* __restrict__ err,
+                              float* __restrict__ loss, float* __restrict__ lse, RowOut o) {
   grid_wait();
   grid_next();
   const long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -416,6 +422,7 @@ __global__ void __launch_bounds__(256)
   const long r = rows ? rows[off + i] : off + i;
   if (!has[r]) return row_without(r, i, K, lane, loss, lse, o);
   float2 ms = seg_row(warp_join(seg_fold(stat + i * ld_stat, ld_stat, lane, 32)));
+  ms.y = sum_or_nan(ms.y, err);
   const float scale = (row_scale ? row_scale[r] : 1.f) * inv_t;
   float acc = 0.f;
   bool bad = false;
@@ -1031,6 +1038,7 @@ static int vocab_run(const VocabCall& c) {
   const float inv_t = (float)(1.0 / c.temperature);
   const float scale2 = (float)((double)kLog2e / c.temperature);
   const __nv_bfloat16* bias = (const __nv_bfloat16*)c.bias;
+  const unsigned* err = device_error_word();
   Answers a{K ? nullptr : c.ids, K ? ws + p.has : nullptr};
   if (K) {
     const size_t smem = (size_t)4 * 2 * round_up(K, 4) * 4;
@@ -1105,11 +1113,11 @@ static int vocab_run(const VocabCall& c) {
       PL_CUDA(launch_early(vocab_distill_rows_kernel, (unsigned)ceil_div(n, 8), 256, 0, st, V, (int)K,
                            (const int*)(ws + p.ids2), (const float*)(ws + p.p), (const float*)(ws + p.ent),
                            ws + p.has, inv_t, c.row_scale, rows, count, off, n, (const float2*)(ws + p.stat),
-                           p.ld_stat, (const float*)(ws + p.uk), c.loss, c.lse, ro));
+                           p.ld_stat, (const float*)(ws + p.uk), err, c.loss, c.lse, ro));
     } else {
       PL_CUDA(launch_early(vocab_ce_rows_kernel, (unsigned)ceil_div(n, 8), 256, 0, st, c.ids, V, c.row_scale, rows,
-                           count, off, n, (const float2*)(ws + p.stat), p.ld_stat, (const float*)(ws + p.ut), c.loss,
-                           c.lse, ro));
+                           count, off, n, (const float2*)(ws + p.stat), p.ld_stat, (const float*)(ws + p.ut), err,
+                           c.loss, c.lse, ro));
     }
     count_launch();
     if (!c.grad) continue;

@@ -18,7 +18,7 @@ from __future__ import annotations
 import importlib.util
 import os
 
-import torch  # noqa: F401 - the module below is linked against it
+import torch
 
 from . import HERE, PufferError, lib
 
@@ -37,6 +37,21 @@ def _load():
 
 
 _ext = _load()
+
+
+def check(device=None):
+    """Waits for a device (torch's current one) and raises PufferError if a wait inside one of this package's kernels ran
+    out since the last check. Such waits are bounded: a fault ends in unwritten outputs, not in a hang, and the calls
+    below, which return before their work is done, cannot report it. Until this has been called their losses and
+    gradients are NaN then. For a training loop: where it synchronizes anyway. Not during a stream capture."""
+    if device is None:
+        index = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    else:
+        device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if device.type != "cuda":
+            raise PufferError(f"check: {device} is not a CUDA device")
+        index = torch.cuda.current_device() if device.index is None else device.index
+    _ext.check(index)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):

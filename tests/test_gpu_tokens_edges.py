@@ -1,5 +1,6 @@
 """Edges of the token-policy operators: logits that a mask or a constant makes equal over the whole vocabulary, a process
-that uses them on two devices, calls from two threads, and a process whose first call is captured.
+that uses them on two devices, calls from two threads, a process whose first call is captured, and device
+waits that ran out.
 Tolerances as in test_gpu_tokens.py."""
 import ctypes as C
 import math
@@ -187,3 +188,56 @@ def test_first_call_can_be_captured(which):
     p = subprocess.run([sys.executable, "-c", FIRST_CALL, which], capture_output=True, text=True, timeout=300, cwd=root,
                        env=dict(os.environ, PYTHONPATH=root))
     assert p.returncode == 0 and "same bits" in p.stdout, p.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------------------------------ waits that ran out
+@pytest.mark.parametrize("K", [0, 3])
+@pytest.mark.parametrize("N", [40, 300])
+def test_wait_that_ran_out_is_seen(N, K):
+    """A recorded timeout (written from the host) makes the losses and gradients NaN until check() has reported it; then
+    the calls are what they were."""
+    x, w, b, ids, teacher, scale = _head_case(_gen(N + K), N, 700, 64, K, True, 0, 0)
+    has = (ids >= 0) if K == 0 else ((ids >= 0) & (teacher > -math.inf)).any(1)
+
+    def call():
+        if K == 0:
+            return (tokens.vocab_ce(x, w, ids, b)[0],) + tokens.vocab_ce_grad(x, w, ids, b, scale)
+        return (tokens.vocab_distill(x, w, ids, teacher, b)[0],) + tokens.vocab_distill_grad(x, w, ids, teacher, b, 1.0, scale)
+
+    tokens.check()
+    want = call()
+    assert plb.lib().pl_test_set_device_error(0x103) == 0
+    try:
+        bad, loss, _, dx, dw, db = call()
+        for t in (bad, loss):
+            assert torch.isnan(t[has]).all() and not t[~has].any()
+        assert torch.isnan(dx[has].float()).all() and not dx[~has].any()
+        assert torch.isnan(dw.float()).all() and torch.isnan(db.float()).all()
+    finally:
+        with pytest.raises(plb.PufferError, match="ran out"):
+            tokens.check()
+    tokens.check()
+    for device in (0, "cuda", torch.device("cuda", 0)):
+        tokens.check(device)
+    assert all(torch.equal(p, q) for p, q in zip(want, call()))
+
+
+def test_check_waits_for_every_stream():
+    """A record that a stream of its own has yet to write is seen. (The write comes after work of some milliseconds.)"""
+    a = torch.ones(8192, 8192, device="cuda")
+    tokens.check()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(10):
+            a @ a
+        done = torch.cuda.Event()
+        done.record()
+    tokens.check()
+    assert done.query()
+
+
+def test_check_refuses():
+    for device in ("cpu", torch.cuda.device_count(), -1):
+        with pytest.raises((plb.PufferError, RuntimeError)):
+            tokens.check(device)
