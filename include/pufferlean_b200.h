@@ -42,6 +42,8 @@ const char* pl_last_error(void);
 int pl_device_count(void);
 /* Selects the device later calls from this thread use (default 0). */
 int pl_set_device(int device);
+/* The device that is. */
+int pl_get_device(int* device);
 /* Waits for the current device and says whether a wait inside one of its kernels ran out since this was last asked:
  * PL_OK, or PL_ERR_DEVICE_TIMEOUT (and the record is cleared). Such waits are bounded, so that a fault ends in an error
  * and not in a hang; a kernel that gives up leaves its outputs unwritten. Calls that return before their work is done

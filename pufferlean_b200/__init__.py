@@ -116,6 +116,7 @@ def _bind_optional(L):
         "pl_lstm_reuse_inputs": ([C.c_int], C.c_int),
         "pl_lstm_gae_boot_norm": ([_dp] * 4 + [_sz, _sz, _d, _d, _dp], C.c_int),
         "pl_device_check": ([], C.c_int),
+        "pl_get_device": ([C.POINTER(C.c_int)], C.c_int),
         "pl_layernorm_dev": ([_vp, _sz, _vp, _vp, _sz, _sz, _d, C.c_uint8, _vp, _sz, _vp, _vp, _vp], C.c_int),
         "pl_layernorm_grad_ws": ([_sz, _sz], _sz),
         "pl_layernorm_grad_dev": ([_vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _sz, C.c_uint8, _vp, _sz, _vp, _vp, _vp, _sz,

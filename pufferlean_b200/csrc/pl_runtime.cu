@@ -94,6 +94,12 @@ int pl_set_device(int device) {
   return PL_OK;
 }
 
+int pl_get_device(int* device) {
+  PL_REQUIRE(device, PL_ERR_INVALID, "pl_get_device: NULL");
+  PL_CUDA(cudaGetDevice(device));
+  return PL_OK;
+}
+
 int pl_device_check(void) {
   int rc = pl::require_device();
   if (rc) return rc;

@@ -101,12 +101,18 @@ PyObject* tuple_of(const at::Tensor (&ts)[N], size_t n) {
   return r;
 }
 
-// The tensors' device for torch and for the library while a call runs, and torch's stream there.
+int library_device() {
+  int d;
+  check(pl_get_device(&d), "pl_get_device");
+  return d;
+}
+// The tensors' device for torch and for the library while a call runs, and torch's stream there. Both get back the
+// device that each had: a caller may have given the library another one than torch's.
 struct On {
-  c10::cuda::CUDAGuard guard;
   int was, now;
+  c10::cuda::CUDAGuard guard;
   void* stream;
-  explicit On(const at::Device& d) : guard(d), was(guard.original_device().index()), now(d.index()) {
+  explicit On(const at::Device& d) : was(library_device()), now(d.index()), guard(d) {
     check(pl_set_device(now), "pl_set_device");
     stream = c10::cuda::getCurrentCUDAStream(d.index()).stream();
   }

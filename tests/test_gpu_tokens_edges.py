@@ -92,6 +92,22 @@ def test_two_devices():
         assert torch.equal(p, q.to("cuda:0"))
 
 
+@pytest.mark.parametrize("device", range(max(1, min(2, torch.cuda.device_count()))))
+def test_the_librarys_device_stays(device):
+    """The device that the caller gave the library is still the library's after a call on cuda:0 tensors, and torch's is
+    still torch's."""
+    L, now = plb.lib(), C.c_int()
+    x = torch.ones(4, 64, device="cuda:0")
+    before = torch.cuda.current_device()
+    assert L.pl_set_device(device) == 0
+    try:
+        tokens.layer_norm(x)
+        assert L.pl_get_device(C.byref(now)) == 0 and now.value == device
+    finally:
+        assert L.pl_set_device(before) == 0
+    assert torch.cuda.current_device() == before
+
+
 # ------------------------------------------------------------------------------------------------ threads
 class _DistillCall:
     """A distillation with gradients through the C entry, with buffers and a stream of its own. With these sizes the

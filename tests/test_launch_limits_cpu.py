@@ -1,6 +1,6 @@
 """The table of shared-memory limits behind the library's launches, without a device: a limit belongs to one kernel on one
-device, and it only ever grows; and what the check of a device
-says where there is none."""
+device, and it only ever grows; and what the calls about
+a device say where there is none."""
 import ctypes as C
 import threading
 
@@ -65,6 +65,10 @@ def test_full_table_still_sets(raise_smem):
         assert raise_smem(63, k, 64, on) == 0
     assert raise_smem(63, 299, 64, on) == 0 and raise_smem(63, 5, 64, on) == 0
     assert calls == list(range(1, 300)) + [299]
+
+
+def test_get_device_refuses_null():
+    assert plb.lib().pl_get_device(None) == -1
 
 
 def test_device_check_needs_a_device():
