@@ -48,12 +48,15 @@ def _compile(src: str, verbose: bool) -> str:
 
 
 def _torch_ext(verbose: bool) -> None:
-    """The module that takes torch tensors (pufferlean_b200/tokens.py); left out where torch is not installed."""
+    """The module that takes torch tensors (pufferlean_b200/tokens.py); left out where torch is not installed or was
+    built without CUDA."""
     src = os.path.join(CSRC, "pl_torch.cpp")
     spec = importlib.util.find_spec("torch")
     if spec is None or not spec.submodule_search_locations:
         return
     torch = spec.submodule_search_locations[0]
+    if not os.path.exists(os.path.join(torch, "lib", "libc10_cuda.so")):
+        return
     if os.path.exists(TORCH_EXT) and os.path.getmtime(TORCH_EXT) >= max(
             os.path.getmtime(p) for p in (src, LIB, os.path.join(ROOT, "include", "pufferlean_b200.h"))):
         return
