@@ -1,6 +1,6 @@
 """Edges of the token-policy operators: logits that a mask or a constant makes equal over the whole vocabulary, a process
-that uses them on two devices, calls from two threads, a process whose first call is captured, and device
-waits that ran out.
+that uses them on two devices, calls from two threads, a process whose first call is captured, device
+waits that ran out, and matrices of more than 2^31 elements.
 Tolerances as in test_gpu_tokens.py."""
 import ctypes as C
 import math
@@ -15,7 +15,8 @@ torch = pytest.importorskip("torch")
 
 import pufferlean_b200 as plb  # noqa: E402
 from pufferlean_b200 import tokens  # noqa: E402
-from .test_gpu_tokens import B, BF16, F2, F64, H, _answers, _close, _gen, _head_case  # noqa: E402
+from .test_gpu_tokens import (B, BF16, F2, F64, H, _answers, _close, _gen, _head_case, _head_ref, _head_tol,  # noqa: E402
+                              _norm_grad_ref, _randn)
 
 pytestmark = pytest.mark.gpu
 
@@ -257,3 +258,68 @@ def test_check_refuses():
     for device in ("cpu", torch.cuda.device_count(), -1):
         with pytest.raises((plb.PufferError, RuntimeError)):
             tokens.check(device)
+
+
+# ------------------------------------------------------------------------------------------------ past 32 bits
+@pytest.mark.parametrize("piece_bytes,rows", [(6 << 30, (0, 5, 8191, 16375, 16376, 16377, 16400, 16497, 16499)),
+                                              (0, (0, 5, 8191, 8318, 8319, 8320, 8321, 16497, 16499))])
+def test_vocab_terms_past_32_bits(piece_bytes, rows):
+    """16,500 rows of terms, 131,136 apart: 2^31 elements end inside row 16,376 when one piece holds them all; by the
+    default bound there are two pieces, of 8,320 rows and the rest. Rows on both sides of either border, and the
+    gradients of a few tokens, which sum over all rows."""
+    g = _gen(98)
+    N, V, D = 16500, 131100, 64
+    x, w = _randn(g, N, D).to(BF16), (_randn(g, V, D) * 0.2).to(BF16)
+    b = (0.3 * _randn(g, V)).to(BF16)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda").to(torch.int32)
+    cols = torch.tensor([0, 1, 77777, V - 1], device="cuda")
+    rows = torch.tensor(rows, device="cuda")
+    t[rows] = cols.repeat(3)[:len(rows)].to(torch.int32)  # their answers lie in the columns that are looked at
+    scale = torch.ones(N, device="cuda")
+    scale[rows] = 64.0  # one of these rows in the wrong place stands out of a sum over all
+    loss, lse, dx, dw, db = tokens.vocab_ce_grad(x, w, t, b, scale, False, piece_bytes)
+    xs, ts = x[rows], t[rows]
+    ref = _head_ref(xs, w, b, ts, None, 1.0, scale[rows])
+    tol_z, tol_loss = _head_tol(ref, xs, w, b, ts, 1.0)
+    _close(loss[rows], ref["loss"], tol_loss, "loss")
+    _close(lse[rows], ref["lse"], tol_loss, "lse")
+    off = (B + H) * ref["dz"].abs() + (H + 4 * tol_z[:, None] + 2.0 ** -18) * ref["s"].abs() * ref["q"] \
+        + 2.0 ** -18 * ref["dz"].abs()
+    wa = w.double().abs()
+    dxr = ref["dz"] @ w.double()
+    _close(dx[rows], dxr, off @ wa + (V / 16 + 200) * F2 * (ref["dz"].abs() @ wa) + B * 1.01 * dxr.abs(), "dx")
+    sd = scale.double()[:, None]
+    lse64 = torch.empty(N, dtype=F64, device="cuda")
+    for r in range(0, N, 500):
+        lse64[r:r + 500] = torch.logsumexp(x[r:r + 500].double() @ w.double().t() + b.double(), 1)
+    _close(lse, lse64, 2.0 ** -16 * (1 + lse64.abs()), "lse of every row")
+    q = torch.exp(x.double() @ w[cols].double().t() + b[cols].double() - lse64[:, None])
+    dz = sd * (q - (t[:, None] == cols[None]).double())
+    xa = x.double().abs()
+    off = (B + H) * dz.abs() + (H + 2.0 ** -15) * sd * q
+    dwr, dbr = dz.t() @ x.double(), dz.sum(0)
+    _close(dw[cols], dwr, off.t() @ xa + (N / 16 + 200) * F2 * (dz.abs().t() @ xa) + B * 1.01 * dwr.abs(), "dw")
+    _close(db[cols], dbr, off.sum(0) + (N + 200) * F2 * dz.abs().sum(0) + B * 1.01 * dbr.abs(), "dbias")
+
+
+def test_layer_norm_sums_past_32_bits():
+    """The parameters' gradients sum over rows on both sides of element 2^31 (row 131,072); the rows there weigh a
+    thousandfold, so that one left out or taken twice stands out."""
+    rows, cols = 140000, 16384
+    x = torch.empty(rows, cols, dtype=BF16, device="cuda")
+    x.normal_(generator=_gen(3))
+    y, m, r = tokens.layer_norm(x)
+    y[131070:131075] *= 1000
+    y[-1] *= 1000
+    dx, dw, db = tokens.layer_norm_grad(y, x, None, m, r)
+    at = torch.tensor([0, 1, 8191, 8192, cols - 1], device="cuda")
+    xh = (x[:, at].double() - m.double()[:, None]) * r.double()[:, None]
+    dy = y[:, at].double()
+    n = rows / 148 + 64  # a block's rows one after the other, then the blocks' sums
+    off_xh = F2 * (x[:, at].double().abs() + m.double()[:, None].abs()) * r.double()[:, None]
+    _close(dw[at], (dy * xh).sum(0), n * F2 * (dy.abs() * xh.abs()).sum(0) + (dy.abs() * off_xh).sum(0), "dw")
+    _close(db[at], dy.sum(0), n * F2 * dy.abs().sum(0), "db")
+    some = torch.tensor([131071, 131072, 131074, rows - 1], device="cuda")
+    dxr, _, _, xh, gg = _norm_grad_ref(y[some], x[some], None, m[some], r[some])
+    size = gg.abs() + gg.abs().mean(1, keepdim=True) + xh.abs() * (gg * xh).abs().mean(1, keepdim=True)
+    _close(dx[some], dxr, B * dxr.abs() + 2.0 ** -16 * r[some].double()[:, None] * size, "dx")
