@@ -11,7 +11,8 @@ include/pufferlean_b200.h (pl_layernorm_dev, pl_vocab_ce_dev, ...). There is no 
     loss, lse, dy, dw, db = vocab_ce_grad(y2d, head, target, head_bias, row_scale)
     dx, dweight, dbias = layer_norm_grad(dy, x, weight, mean, rstd)
 
-Gradients are of sum_n row_scale_n * loss_n (descent).
+Gradients are of sum_n row_scale_n * loss_n (descent). The results carry no autograd graph, whatever their inputs require:
+gradients come from the *_grad calls, and a loss of these calls adds nothing to a backward().
 """
 from __future__ import annotations
 

@@ -1,6 +1,6 @@
 """Edges of the token-policy operators: logits that a mask or a constant makes equal over the whole vocabulary, a process
 that uses them on two devices, calls from two threads, a process whose first call is captured, device
-waits that ran out, and matrices of more than 2^31 elements.
+waits that ran out, inputs that require gradients, and matrices of more than 2^31 elements.
 Tolerances as in test_gpu_tokens.py."""
 import ctypes as C
 import math
@@ -258,6 +258,25 @@ def test_check_refuses():
     for device in ("cpu", torch.cuda.device_count(), -1):
         with pytest.raises((plb.PufferError, RuntimeError)):
             tokens.check(device)
+
+
+# ------------------------------------------------------------------------------------------------ autograd
+def test_results_carry_no_graph():
+    """Parameters that require a gradient are taken as they are; nothing that comes back does, and the bits are the same."""
+    x, w, b, ids, teacher, scale = _head_case(_gen(17), 70, 300, 64, 3, True, 0, 0)
+    gain = torch.ones(64, device="cuda")
+
+    def calls():
+        y, m, r = tokens.layer_norm(x, gain)
+        return ((y, m, r) + tokens.layer_norm_grad(x, x, gain, m, r) + tokens.vocab_ce(x, w, ids[:, 0].contiguous(), b)
+                + tokens.vocab_ce_grad(x, w, ids[:, 0].contiguous(), b, scale) + tokens.vocab_distill(x, w, ids, teacher, b)
+                + tokens.vocab_distill_grad(x, w, ids, teacher, b, 1.0, scale))
+
+    want = calls()
+    x, w, b, gain = (t.detach().requires_grad_() for t in (x, w, b, gain))
+    got = calls()
+    assert not any(t.requires_grad for t in got)
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
 
 
 # ------------------------------------------------------------------------------------------------ past 32 bits
