@@ -567,13 +567,16 @@ int pl_layernorm_grad_dev(const void* dy, size_t lddy, const void* x, size_t ldx
  * target leaves the row out: loss = lse = 0, no gradient, and no work in the products. A target >= V makes the row's
  * loss (and the gradients) NaN.
  * Distillation: ids, teacher [N x K] (int32, f32 logits); a negative id or a teacher logit of -inf is an absent entry.
- * p = softmax(teacher / temperature) over the present entries, loss_n = sum_k p_k (log p_k - u_n,id_k) + lse_n = KL(p | q).
- * A row with no entry is left out like a negative target; entries that name the same id add up.
+ * p = softmax(teacher / temperature) over the present entries, loss_n = sum_k p_k (log p_k - u_n,id_k) + lse_n, which is
+ * KL(p | q) where the row's ids differ. Entries that name the same id add up in the gradient and in the sum with u; the
+ * log p_k are the single entries' (the loss is then below KL of the added-up p, by a number that no gradient sees). A
+ * row with no entry is left out like a negative target.
  *
  * ws: pl_vocab_ws bytes (K = 0 for the cross entropy, else at most 512; aligned = 1 when x and dw start at 16 bytes
  * with row strides that are multiples of 8, and w at 128 with one that is a multiple of 64). The gradient forms keep
- * one piece of rows' softmax terms there (2 bytes each): piece_bytes bounds that piece, 0 = 4 GiB; the results do not
- * depend on it beyond the order of dw's f32 sums.
+ * one piece of rows' softmax terms there (2 bytes each): piece_bytes bounds that piece, 0 = 4 GiB. loss and
+ * lse do not depend on it; the order of the f32 sums behind dx, dw and dbias does, and each piece after the first reads
+ * and writes dw's f32 sums once more.
  * dx [N x D] bf16; dw [V x D] and dbias [V] (given exactly when bias is) bf16, or f32 with dw_f32 = 1. dw's f32 sums are
  * of products whose logit gradients were rounded to bf16 (up to 64 rows: to two bf16 parts). row_scale [N] f32 or NULL
  * (ones). */

@@ -75,14 +75,17 @@ def vocab_ce(x, w, target, bias=None):
 
 def vocab_ce_grad(x, w, target, bias=None, row_scale=None, dw_f32=False, piece_bytes=0):
     """(loss, lse, dx, dw, dbias) of sum_n row_scale_n loss_n: dx bf16, dw and dbias bf16 or (dw_f32) f32, dbias None
-    without a bias. piece_bytes bounds the softmax terms held at a time (0: 4 GiB)."""
+    without a bias. dw_f32 saves the last rounding only: the logits' gradient goes into the products as bf16 (up to 64
+    rows: as two bf16 parts). piece_bytes bounds the softmax terms held at a time (0: 4 GiB); loss and lse do not depend
+    on it, the order of the gradients' sums does."""
     return _ext.vocab("vocab_ce_grad", x, w, target, None, bias, 1.0, row_scale, True, dw_f32, piece_bytes)
 
 
 def vocab_distill(x, w, ids, teacher, bias=None, temperature=1.0):
     """(loss, lse) [N] f32 of the head's distribution q = softmax((x w^T + bias) / temperature) against the teacher's
     p = softmax(teacher / temperature) over its K top entries (ids, teacher [N, K]; a negative id or a logit of -inf is
-    absent): loss = KL(p | q). A row without entries is left out (loss = lse = 0)."""
+    absent): loss = sum_k p_k (log p_k - log q_id(k)), KL(p | q) where the row's ids differ (entries of one id add up, their
+    log p_k stay the single ones). A row without entries is left out (loss = lse = 0)."""
     if teacher is None:
         raise PufferError("vocab_distill: teacher is needed")
     return _ext.vocab("vocab_distill", x, w, ids, teacher, bias, temperature, None, False, False, 0)
