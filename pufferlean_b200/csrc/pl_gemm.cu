@@ -92,8 +92,11 @@ int gemm_sms() {
 }
 
 // Mode 2's products for CTA pairs: both operands MN-major; the large-vocabulary head's logits and sliced products,
-// where an odd number of 128-row tiles (half a pair idle on the last) costs at most an eighth: 300 rows of logits over
-// 65,536 x 1,024 took 72 us on single CTAs and 80 on pairs, 4,096 rows 445 and 369.
+// where an odd number of 128-row tiles (half a pair idle on the last) costs at most an eighth. Whole calls over 65,536 x
+// 1,024, every product on single CTAs / on pairs, us: the loss alone of 200 rows 55 / 53, 300 rows 65 / 69, 1,100 rows
+// 128 / 138, 4,096 rows 385 / 384 (4,096 rows of 32,768 x 2,048: 376 / 363); with gradients 200 rows 175 / 162, 300 rows
+// 203 / 197, 1,100 rows 445 / 435, 4,096 rows 1,467 / 1,362. So pairs pay in the gradients' products; in the logits an
+// odd tile above eight costs more than they gain.
 bool gemm_paired(int bn, int epi, bool a_mn, bool b_mn, int M) {
   uint32_t smem;
   const long tiles = ceil_div(M, 128);

@@ -375,8 +375,8 @@ __device__ __forceinline__ TileIdx tile_of(int t, int num_n, int num_m) {
 
 // Order of the head's logit tiles (EPI_VOCAB): the weight matrix is the large operand, so m is the fast index inside
 // groups of 4,096 rows: the CTAs that run at one time share a few column panels of the weights (read once from HBM per
-// group) and the group's rows stay in L2. 16,384 x 131,072 x 2,048 with gradients takes 23.7-24.0 ms with this group,
-// 24.2-24.6 with 2,048 rows, 23.7-24.2 with 8,192 and 24.6 with all.
+// group) and the group's rows stay in L2. 16,384 x 131,072 x 2,048 with gradients, on one board, takes 23.7-24.0 ms with
+// this group, 24.2-24.6 with 2,048 rows, 23.7-24.2 with 8,192 and 24.6 with all.
 constexpr int kVocabGroupRows = 4096;
 template <int EPI, int GROUP>
 __device__ __forceinline__ TileIdx tile_at(int t, int num_n, int num_m) {

@@ -8,6 +8,12 @@
 // of that size. So a row is read once and stays in registers: TPR threads own a row, thread t its columns
 // (k TPR + t) VEC + j, k < K, j < VEC, with 16-byte loads where base, row stride and width allow them and single
 // values otherwise. The variance is taken about the mean (a second pass over the registers, not over memory).
+//
+// Measured, us and share of a copy's 6,449 GB/s: 65,536 x 2,048 bf16 forward 93 (90 %), backward 149 (84 %); 65,536 x
+// 1,024 f32 forward 88 (95 %). Less is reached where values go singly (65,536 x 1,003 bf16: 74 and 114, 55 and 54 %) and
+// in rows of more than 8,192 columns: up to 16,384 a block of 1,024 threads has 64 registers each and spills (forward
+// 48 to 112 bytes a thread, backward 344 to 544; 8,192 x 16,384 bf16: 161 and 319, 52 and 39 %; f32: 198 and 602, 84 and
+// 41 %), and beyond that rows are read again from L2, value by value (4,096 x 20,000 bf16: 127 and 283, 40 and 27 %).
 #include "pl_common.cuh"
 #include "pl_runtime.h"
 

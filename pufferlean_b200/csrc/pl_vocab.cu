@@ -1,5 +1,6 @@
 // A large-vocabulary head and what it is trained with: softmax cross entropy against one target per row, and
-// distillation from a teacher's top logits, forward and with gradients, without the logits ever being kept.
+// distillation from a teacher's top logits, forward and with gradients. The losses alone keep no logits; the gradients
+// keep the softmax terms of a piece of the rows, 2 bytes each.
 //
 //   u = (x W^T + bias) / T          rows n < N, vocabulary v < V, hidden width D
 //   lse_n = log sum_v exp u_nv      p_nk: the answer's probabilities (one entry of 1, or softmax(teacher / T))
@@ -15,8 +16,8 @@
 // four.
 //
 // What bounds it: the three products run at the rate of the tensor cores under the power cap (16,384 x 131,072 x 2,048:
-// 23.0 ms for 26.4 TFLOP on a board whose cuBLAS does 1,390 TFLOP/s for seconds, 19.0 ms of products at that rate); the
-// pass from terms to gradients at HBM's (2,048 x 131,072: 162 us for 1.07 GB); with few rows the reading of W and the
+// 22.9 to 26.5 ms by board for 26.4 TFLOP; 18.8 ms at the 1,405 TFLOP/s that cuBLAS holds for seconds); the
+// pass from terms to gradients at HBM's (2,048 x 131,072: 161 us for 1.07 GB); with few rows the reading of W and the
 // writing of dW; with few rows of a small vocabulary the launches.
 #include <cuda_fp16.h>
 
@@ -637,7 +638,11 @@ __global__ void __launch_bounds__(256, PART ? 3 : 4)
       fold[c] = t;
     }
     __syncthreads();
-    for (int h = threadIdx.x; h < hits; h += 256) {  // the first listed value of a column adds all of that column's
+    // The first listed value of a column adds all of that column's. Quadratic in the values listed: nothing beside the
+    // walk when a row's answers are spread over the vocabulary, but not when they crowd into one tile (4,096 x 65,537 x
+    // 1,024 with a bias, the whole call: 64 answers a row spread evenly 1,675 us, by Zipf's law 2,003, all among the
+    // first 1,024 tokens 2,547; 20 answers 1,434, 1,445 and 1,635).
+    for (int h = threadIdx.x; h < hits; h += 256) {
       const uint32_t c = hit_at[h] & 0xffffu;
       float t = 0.f;
       bool first = true;
@@ -844,16 +849,19 @@ __global__ void __launch_bounds__(256)
 // made (two launches fewer; the rows without an answer are zeroed instead).
 constexpr long kVocabOneTile = 128;
 // Weights whose rows do not start at 128-byte lines cost the products' TMA boxes an extra line each. For the three
-// products of a gradient a copy with padded rows pays for itself from about this many rows on: V = 50,048, 4,096 rows,
+// products of a gradient a copy with padded rows pays for itself with enough rows: V = 50,048, 4,096 rows,
 // D = 520 / 1,000 / 2,056: 930 / 1,100 / 2,233 us with the copy, 1,114 / 1,108 / 2,328 without; 1,000 rows: 270 / 352 /
-// 678 and 275 / 323 / 598. For the loss alone it does not (4,096 rows: 282 / 341 / 761 and 274 / 310 / 676).
+// 678 and 275 / 323 / 598. One number for every D is a compromise: on straight lines between these figures the two meet
+// below 1,000 rows at D = 520, near 3,400 at D = 1,000 and near 2,400 at D = 2,056. For the loss alone the copy does not
+// pay (4,096 rows: 282 / 341 / 761 and 274 / 310 / 676).
 constexpr long kVocabPackRows = 2048;
 // Rows up to which the weight gradient (V x D values out, a short inner axis) is bound by its writes and goes out from
 // registers: V = 118,208, D = 3,712, 5 / 256 rows: the whole call 522 / 719 us, 556 / 737 through shared memory and
 // TMA stores; from 1,024 rows on the two do not differ.
 constexpr long kVocabDirectRows = 512;
 // Bytes of terms that one piece may hold. Fewer pieces mean fewer passes over the f32 weight gradient (each piece
-// after the first adds to it: 8 V D bytes).
+// after the first adds to it: 8 V D bytes). 4,096 x 65,537 x 1,024 in one piece / in two: 1.54-1.71 / 2.20-2.26 ms with
+// a bf16 weight gradient, 1.62-1.76 / 1.93-2.07 ms with an f32 one.
 constexpr size_t kVocabPieceBytes = (size_t)4 << 30;
 constexpr int kSplitSlices = 8;     // slices of a product that one warp still adds up by itself
 constexpr size_t kVocabMaxK = 512;  // entries of a row: its lists stay in shared memory
