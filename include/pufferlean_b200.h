@@ -554,6 +554,72 @@ int pl_layernorm_grad_dev(const void* dy, size_t lddy, const void* x, size_t ldx
                           const float* rstd, size_t rows, size_t cols, uint8_t bf16, void* dx, size_t lddx, float* dw,
                           float* db, void* ws, size_t ws_bytes, void* stream);
 
+/* The norms around a block of a residual network, with its gate and residual scale (RMS norms: rms(z) = z rstd,
+ * rstd = 1 / sqrt(mean z^2 + eps)). Rows are f32, or bf16 with bf16 = 1, all of one call's alike:
+ *   r = x + scale sigmoid(gate) w_branch rms(branch),  y = w rms(r)
+ * gate may be NULL (no gate: factor 1), w_branch and w [cols] f32 too (ones); post = 0 leaves the first norm out (branch as
+ * it is, times w_branch). The second norm is of r as it is stored. rstd_branch (with post), rstd [rows] f32 are written
+ * for the gradient. */
+int pl_block_norm_dev(const void* x, size_t ldx, const void* branch, size_t ldb, const void* gate, size_t ldg,
+                      const float* w_branch, const float* w, double scale, double eps, uint8_t post, size_t rows,
+                      size_t cols, uint8_t bf16, void* r, size_t ldr, void* y, size_t ldy, float* rstd_branch,
+                      float* rstd, void* stream);
+/* Its gradient, from dr (of the residual stream behind the block; NULL: zero) and dy: dx, dbranch, dgate (with a gate) in
+ * the rows' type; dw_branch, dw [cols] f32, each may be NULL (summed in a fixed order). rstd_branch NULL: post = 0.
+ * ws: pl_block_norm_grad_ws(rows, cols) bytes when dw_branch or dw is wanted. */
+size_t pl_block_norm_grad_ws(size_t rows, size_t cols);
+int pl_block_norm_grad_dev(const void* dr, size_t lddr, const void* dy, size_t lddy, const void* branch, size_t ldb,
+                           const void* gate, size_t ldg, const void* r, size_t ldr, const float* rstd_branch,
+                           const float* rstd, const float* w_branch, const float* w, double scale, size_t rows,
+                           size_t cols, uint8_t bf16, void* dx, size_t lddx, void* dbranch, size_t lddb, void* dgate,
+                           size_t lddg, float* dw_branch, float* dw, void* ws, size_t ws_bytes, void* stream);
+
+/* One token per row of logits [rows x V] (f32, or bf16 with bf16 = 1; V up to 262,144), drawn with the given number
+ * u [rows] in [0, 1). With e_i = exp((z_i - max z) / temperature), and in the order of falling z, equal ones by index: the
+ * first top_k stay (0, or V and more: all); of these those before which less than top_p of their mass comes (1 and more:
+ * all); of these those with e_i >= min_p. The first always stays. token = the first that stays, by index, at which the sum
+ * of the e that stay passes u times their total; logp = its log-probability among those that stay. Sums are f64.
+ * Temperature 0 takes the first in that order (logp 0). temperature, top_k, top_p, min_p [rows], or NULL: the number
+ * beside it for all rows. A logit of -inf is never drawn. A row that holds a NaN or +inf, or -inf alone, or whose u or
+ * options are NaN, whose temperature is negative or infinite, gets token -1 and logp NaN. */
+int pl_sample_dev(const void* logits, size_t ld, size_t rows, size_t V, uint8_t bf16, const float* u,
+                  const float* temperature, double temperature_all, const int32_t* top_k, size_t top_k_all,
+                  const float* top_p, double top_p_all, const float* min_p, double min_p_all, int32_t* token, float* logp,
+                  void* stream);
+
+/* The gated delta rule: every head of values keeps a state S [dk x dv] (f32), and with a = exp(g)
+ *   u_t = beta_t (v_t - a_t S_{t-1}^T k_t),  S_t = a_t S_{t-1} + k_t u_t^T,  o_t = scale S_t^T q_t
+ * q, k [tokens][heads_k][dk], v, o [tokens][heads_v][dv] bf16, g, beta [tokens][heads_v] f32; head h of the values goes with
+ * head h / (heads_v / heads_k) of queries and keys. dk up to 128, dv up to 1,024. Strides of tokens and heads are in
+ * elements (the last dimension is contiguous); o and gradients are packed. g = -inf (or below -104) forgets the
+ * (finite) state: an episode's first token. Keys of length one and beta in (0, 2) keep the rule stable.
+ *
+ * Sequences lie one behind the other: sequence s has tokens offsets[s] to offsets[s + 1] - 1 (int32 on the device,
+ * not falling; NULL: `sequences` of equal length). Tokens in front of the first and behind the last belong to none: their outputs
+ * are zero. state (NULL: zero) and final_state are [sequences][heads_v][dk][dv] f32. ws: pl_delta_ws bytes; saved, for
+ * the gradient: pl_delta_saved bytes, or NULL; both 256-byte aligned. */
+typedef struct {
+  size_t tokens, sequences, heads_k, heads_v, dk, dv;
+  size_t q_token, q_head, k_token, k_head, v_token, v_head;
+  double scale;
+} pl_delta_shape;
+size_t pl_delta_ws(const pl_delta_shape* s, uint8_t grad);
+size_t pl_delta_saved(const pl_delta_shape* s);
+int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g, const float* beta,
+                 const int32_t* offsets, const float* state, void* o, float* final_state, void* saved, size_t saved_bytes,
+                 void* ws, size_t ws_bytes, void* stream);
+/* Its gradient, from dout [tokens][heads_v][dv] bf16 (strides in elements) and dfinal (of final_state; NULL: zero): dq, dk,
+ * dv bf16, dg, dbeta f32 (zero dg at a token that forgets), dstate (of state; may be NULL). Sums go in a fixed order; what
+ * heads of values add to the shared queries and keys is added in their order. */
+int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token, size_t do_head, const float* dfinal,
+                      const void* q, const void* k, const void* v, const float* g, const float* beta,
+                      const int32_t* offsets, const void* saved, size_t saved_bytes, void* dq, void* dk, void* dv, float* dg,
+                      float* dbeta, float* dstate, void* ws, size_t ws_bytes, void* stream);
+/* One token of every row: the rule with tokens = rows, state and state_out [rows][heads_v][dk][dv] (state_out may be
+ * state), o [rows][heads_v][dv]. */
+int pl_delta_step_dev(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g,
+                      const float* beta, const float* state, float* state_out, void* o, void* stream);
+
 /* A head call whose products gave up waiting (pl_device_check) cannot return an error. As long as the record stands,
  * the rows that count get a loss of NaN, and the gradients of these calls are NaN.
  *

@@ -33,6 +33,12 @@ class MgNet(C.Structure):
     _fields_ = [("D", _sz), ("H", _sz), ("L", _sz), ("A", _sz), ("K", _sz), ("enc_act", C.c_int)]
 
 
+class DeltaShape(C.Structure):
+    """pl_delta_shape: sizes and strides (in elements) of a call of the gated delta rule."""
+    _fields_ = [(x, _sz) for x in ("tokens", "sequences", "heads_k", "heads_v", "dk", "dv", "q_token", "q_head", "k_token",
+                                   "k_head", "v_token", "v_head")] + [("scale", _d)]
+
+
 class MgHyper(C.Structure):
     """pl_mg_hyper: the MinGRU update's hyperparameters."""
     _fields_ = [(x, _d) for x in ("gamma", "lam", "rhoClip", "cClip", "prioAlpha", "annealBeta", "wd", "mu", "eps",
@@ -121,6 +127,17 @@ def _bind_optional(L):
         "pl_layernorm_grad_ws": ([_sz, _sz], _sz),
         "pl_layernorm_grad_dev": ([_vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _sz, C.c_uint8, _vp, _sz, _vp, _vp, _vp, _sz,
                                    _vp], C.c_int),
+        "pl_sample_dev": ([_vp, _sz, _sz, _sz, C.c_uint8, _vp, _vp, _d, _vp, _sz, _vp, _d, _vp, _d, _vp, _vp, _vp], C.c_int),
+        "pl_block_norm_dev": ([_vp, _sz] * 3 + [_vp, _vp, _d, _d, C.c_uint8, _sz, _sz, C.c_uint8, _vp, _sz, _vp, _sz, _vp,
+                                                _vp, _vp], C.c_int),
+        "pl_block_norm_grad_ws": ([_sz, _sz], _sz),
+        "pl_block_norm_grad_dev": ([_vp, _sz] * 5 + [_vp] * 4 + [_d, _sz, _sz, C.c_uint8] + [_vp, _sz] * 3
+                                   + [_vp, _vp, _vp, _sz, _vp], C.c_int),
+        "pl_delta_ws": ([C.POINTER(DeltaShape), C.c_uint8], _sz),
+        "pl_delta_saved": ([C.POINTER(DeltaShape)], _sz),
+        "pl_delta_dev": ([C.POINTER(DeltaShape)] + [_vp] * 10 + [_sz, _vp, _sz, _vp], C.c_int),
+        "pl_delta_grad_dev": ([C.POINTER(DeltaShape), _vp, _sz, _sz] + [_vp] * 8 + [_sz] + [_vp] * 7 + [_sz, _vp], C.c_int),
+        "pl_delta_step_dev": ([C.POINTER(DeltaShape)] + [_vp] * 9, C.c_int),
         "pl_vocab_ws": ([_sz] * 4 + [C.c_uint8] * 3 + [_sz], _sz),
         "pl_vocab_ce_dev": ([_vp, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _vp], C.c_int),
         "pl_vocab_ce_grad_dev": ([_vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _vp, _sz, _vp,

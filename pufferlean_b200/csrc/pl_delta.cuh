@@ -1,0 +1,235 @@
+// What the kernels of the gated delta rule share: the cut of packed sequences into chunks of 64 tokens, copies of tiles
+// into shared memory, and products of bf16 tiles whose f32 operands are carried as two bf16 parts.
+#pragma once
+#include "pl_common.cuh"
+
+namespace pl {
+
+constexpr int kC = 64;    // tokens of a chunk
+constexpr int kLd = 72;   // row stride of a 64-column bf16 tile in shared memory: rows 16 bytes apart in the banks
+
+struct DeltaArgs {
+  long n;                      // tokens
+  int seqs, hk, hv, dk, dv, dvp;  // dvp: dv rounded up to 64
+  const int* offsets;          // [seqs + 1], or NULL: sequences of n / seqs tokens
+  long ldq, hsq, ldk, hsk, ldv, hsv;  // strides of tokens and heads
+  const __nv_bfloat16 *q, *k, *v;
+  const float *g, *beta;  // [n][hv]
+  float scale;
+  bool vec;  // q, k, v rows start at 16-byte boundaries
+};
+
+// Sequence s's tokens, whatever the offsets hold: inside [0, n].
+__device__ __forceinline__ void seq_bounds(const DeltaArgs& a, int s, long& from, long& to) {
+  if (a.offsets) {
+    from = a.offsets[s];
+    to = a.offsets[s + 1];
+  } else {
+    from = a.n / a.seqs * s;
+    to = from + a.n / a.seqs;
+  }
+  from = from < 0 ? 0 : from > a.n ? a.n : from;
+  to = to < from ? from : to > a.n ? a.n : to;
+}
+// Chunk c of sequence s has slot from / 64 + s + c: no two share one (a sequence of L tokens has at most L / 64 + 1
+// chunks, and the next one's first slot is at least that much further), and all are below n / 64 + seqs.
+__device__ __forceinline__ long seq_slot(const DeltaArgs& a, int s) {
+  long from, to;
+  seq_bounds(a, s, from, to);
+  return from / kC + s;
+}
+__host__ __device__ __forceinline__ long slot_count(long n, long seqs) { return n / kC + seqs; }
+
+// The chunk of a slot: its first token and how many it has (0: none).
+__device__ __forceinline__ int slot_chunk(const DeltaArgs& a, long slot, long& start) {
+  int lo = 0, hi = a.seqs - 1;  // the last sequence whose first slot is not behind this one
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (seq_slot(a, mid) <= slot) lo = mid;
+    else hi = mid - 1;
+  }
+  long from, to;
+  seq_bounds(a, lo, from, to);
+  start = from + (slot - from / kC - lo) * kC;
+  if (start < from || start >= to) return 0;
+  return (int)(to - start < kC ? to - start : kC);
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(void* dst, const void* src, int bytes) {  // the rest of the 16 bytes is zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// rows x COLS values into a tile of row stride LD, from rows of `stride`; what is outside rows x cols becomes zero. With
+// vec the copies are asynchronous (cp_commit, cp_wait); without, plain stores.
+template <int COLS, int LD, int THREADS>
+__device__ __forceinline__ void copy_tile(__nv_bfloat16* dst, const __nv_bfloat16* src, long stride, int rows, int cols,
+                                          bool vec) {
+  if (vec) {
+    for (int i = threadIdx.x; i < kC * (COLS / 8); i += THREADS) {
+      const int r = i / (COLS / 8), c = i % (COLS / 8) * 8;
+      int bytes = r < rows ? (cols - c) * 2 : 0;
+      bytes = bytes < 0 ? 0 : bytes > 16 ? 16 : bytes;
+      cp16(dst + r * LD + c, bytes ? src + (long)r * stride + c : src, bytes);
+    }
+  } else {
+    for (int i = threadIdx.x; i < kC * COLS; i += THREADS) {
+      const int r = i / COLS, c = i % COLS;
+      dst[r * LD + c] = r < rows && c < cols ? src[(long)r * stride + c] : __float2bfloat16_rn(0.f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- products
+// m16n8k16 products of one warp on bf16 tiles in shared memory. An operand lies either along k (rows of m or n) or
+// across it (rows of k); ldmatrix transposes the latter.
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The 16 x 16 fragment of A at (m, k): along k, or across.
+template <bool ACROSS, int LD>
+__device__ __forceinline__ void frag_a(uint32_t (&r)[4], const __nv_bfloat16* t, int m, int k) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (!ACROSS)
+    ldsm4(r, smem_u32(t + (m + (lane & 15)) * LD + k + (lane >> 4) * 8));
+  else
+    ldsm4t(r, smem_u32(t + (k + (lane & 7) + ((lane >> 4) & 1) * 8) * LD + m + ((lane >> 3) & 1) * 8));
+}
+// Two n-tiles of B at (k, n): b[0], b[1] for columns n.., b[2], b[3] for n + 8..
+template <bool ACROSS, int LD>
+__device__ __forceinline__ void frag_b(uint32_t (&r)[4], const __nv_bfloat16* t, int k, int n) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (!ACROSS)
+    ldsm4(r, smem_u32(t + (n + (lane & 7) + ((lane >> 4) & 1) * 8) * LD + k + ((lane >> 3) & 1) * 8));
+  else
+    ldsm4t(r, smem_u32(t + (k + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + n + ((lane >> 4) & 1) * 8));
+}
+
+// acc (16 x 8 NT at (m, n)) += A B over k in [k0, k1). A f32 operand is two bf16 parts, the second one the rounding of what the
+// first leaves (2^-17 of the value is lost, the product of the two second parts with it); lo = nullptr: bf16 as it is.
+template <bool A_ACROSS, int LDA, bool B_ACROSS, int LDB, int NT>
+__device__ __forceinline__ void product(float (&acc)[NT][4], const __nv_bfloat16* a, const __nv_bfloat16* alo,
+                                        const __nv_bfloat16* b, const __nv_bfloat16* blo, int m, int n, int k0, int k1) {
+#pragma unroll 2
+  for (int k = k0; k < k1; k += 16) {
+    uint32_t x[4], xl[4];
+    frag_a<A_ACROSS, LDA>(x, a, m, k);
+    if (alo) frag_a<A_ACROSS, LDA>(xl, alo, m, k);
+#pragma unroll
+    for (int t = 0; t < NT; t += 2) {
+      uint32_t y[4];
+      frag_b<B_ACROSS, LDB>(y, b, k, n + t * 8);
+      mma(acc[t], x, y[0], y[1]);
+      mma(acc[t + 1], x, y[2], y[3]);
+      if (alo) {
+        mma(acc[t], xl, y[0], y[1]);
+        mma(acc[t + 1], xl, y[2], y[3]);
+      }
+      if (blo) {
+        frag_b<B_ACROSS, LDB>(y, blo, k, n + t * 8);
+        mma(acc[t], x, y[0], y[1]);
+        mma(acc[t + 1], x, y[2], y[3]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(x - __low2float(h), y - __high2float(h));
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// A fragment's pair of values at (row, col) of a tile, as two parts.
+template <int LD>
+__device__ __forceinline__ void put2(__nv_bfloat16* hi, __nv_bfloat16* lo, int row, int col, float x, float y) {
+  uint32_t h, l;
+  split2(x, y, h, l);
+  *reinterpret_cast<uint32_t*>(hi + row * LD + col) = h;
+  *reinterpret_cast<uint32_t*>(lo + row * LD + col) = l;
+}
+
+template <int NT>
+__device__ __forceinline__ void zero(float (&acc)[NT][4]) {
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[t][e] = 0.f;
+}
+
+// The decays of a chunk's tokens, by the block's first warp: cum (f64 sum of g since the last reset or the chunk's start), era
+// (resets so far), since = the factor on the state before the chunk (zero behind a reset), until = the factor from a
+// token to the chunk's end (zero in front of a reset). A g of -inf resets, and so does one below -104, whose
+// factor f32 cannot hold.
+struct Decay {
+  double cum[kC];
+  int era[kC];
+  float since[kC], until[kC], beta[kC];
+};
+__device__ __forceinline__ void chunk_decay(const DeltaArgs& a, Decay& d, long start, int len, int h) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    double cum[2];
+    int era[2];
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      const int t = half * 32 + lane;
+      const float g = t < len ? a.g[(start + t) * a.hv + h] : 0.f;
+      d.beta[t] = t < len ? a.beta[(start + t) * a.hv + h] : 0.f;
+      const bool reset = g < -104.f;
+      double s = reset ? 0.0 : (double)g;
+      int e = reset;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {  // (sum, resets) of the tokens up to this one; a reset forgets the sum before it
+        const double up = __shfl_up_sync(0xffffffffu, s, o);
+        const int ue = __shfl_up_sync(0xffffffffu, e, o);
+        if (lane >= o) {
+          if (e == 0) s += up;
+          e += ue;
+        }
+      }
+      if (half) {
+        const double last = __shfl_sync(0xffffffffu, cum[0], 31);
+        if (e == 0) s += last;
+        e += __shfl_sync(0xffffffffu, era[0], 31);
+      }
+      cum[half] = s;
+      era[half] = e;
+    }
+    const double end = __shfl_sync(0xffffffffu, cum[1], 31);
+    const int last = __shfl_sync(0xffffffffu, era[1], 31);
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      const int t = half * 32 + lane;
+      d.cum[t] = cum[half];
+      d.era[t] = era[half];
+      d.since[t] = era[half] == 0 ? expf((float)cum[half]) : 0.f;
+      d.until[t] = era[half] == last ? expf((float)(end - cum[half])) : 0.f;
+    }
+  }
+}
+// The factor from token j to token i >= j.
+__device__ __forceinline__ float decay(const Decay& d, int i, int j) {
+  return d.era[i] == d.era[j] ? expf((float)(d.cum[i] - d.cum[j])) : 0.f;
+}
+
+}  // namespace pl

@@ -1,5 +1,6 @@
 """Operators of a token policy on CUDA tensors: layer norm, the large-vocabulary head's cross entropy, and
-distillation of a teacher's top logits into the head, each forward and with its gradients.
+distillation of a teacher's top logits into the head, each forward and with its gradients; drawing tokens from logits; the
+norms around a block with its gate and residual scale; and a matrix memory per head, the gated delta rule.
 
 A policy whose actions are tokens ends in a layer norm and a head of V outputs, V in the tens of thousands (the
 update paths of this package stop at 128). These calls take torch tensors as they lie (rows may be strided, the last
@@ -96,3 +97,64 @@ def vocab_distill_grad(x, w, ids, teacher, bias=None, temperature=1.0, row_scale
     if teacher is None:
         raise PufferError("vocab_distill_grad: teacher is needed")
     return _ext.vocab("vocab_distill_grad", x, w, ids, teacher, bias, temperature, row_scale, True, dw_f32, piece_bytes)
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(token int32, logp f32) [N]: one token per row of logits [N, V] (f32 or bf16, V up to 262,144), drawn with the given
+    numbers u [N] f32 in [0, 1), so that a draw can be repeated. The options are numbers, or tensors [N] with one for each
+    row (f32; top_k int32). By falling logit, equal ones by index: the first top_k stay (0: all); of these those before
+    which less than top_p of their mass comes; of these those with at least min_p of the largest probability; the first
+    always. logp is the token's log-probability among those that stay, at this temperature (what an importance ratio
+    divides by). temperature 0 takes the first. A logit of -inf is never drawn; a row with a NaN or +inf, with nothing but
+    -inf, or with an option that is NaN, gets token -1 and logp NaN."""
+    return _ext.sample(logits, u, temperature, top_k, top_p, min_p)
+
+
+def block_norm(x, branch, gate=None, branch_weight=None, weight=None, scale=1.0, eps=1e-5, post=True):
+    """(r, y, rstd_branch, rstd): a block's output on its way back into the residual stream x, and the next block's input.
+    r = x + scale * sigmoid(gate) * branch_weight * rms(branch), y = weight * rms(r) with rms(z) = z / sqrt(mean z^2 + eps).
+    x, branch, gate [rows, cols] f32 or bf16 (gate None: no gate), the weights [cols] f32 or None. post=False leaves the
+    first norm out (rstd_branch None). The statistics [rows] f32 are what block_norm_grad takes."""
+    return _ext.block_norm(x, branch, gate, branch_weight, weight, scale, eps, post)
+
+
+def block_norm_grad(dr, dy, branch, gate, r, rstd_branch, rstd, branch_weight=None, weight=None, scale=1.0, params=True):
+    """(dx, dbranch, dgate, dbranch_weight, dweight) of block_norm from the gradients dr of r (None: zero) and dy of y. dgate
+    is None without a gate, the weights' gradients [cols] f32 with params=False."""
+    return _ext.block_norm_grad(dr, dy, branch, gate, r, rstd_branch, rstd, branch_weight, weight, scale, params)
+
+
+def _scale(q, scale):
+    return q.shape[-1] ** -0.5 if scale is None else scale
+
+
+def delta_rule(q, k, v, g, beta, offsets=None, state=None, scale=None, save=False):
+    """(o, final_state, saved): the gated delta rule over packed sequences. Every head of values keeps a matrix S, and with
+    a = exp(g): u_t = beta_t (v_t - a_t S^T k_t), S <- a_t S + k_t u_t^T, o_t = scale S^T q_t (scale None: dk ** -0.5).
+
+    q, k [N, Hk, dk], v [N, Hv, dv] bf16 (views of one wider projection will do), g, beta [N, Hv] f32, state and final_state
+    [S, Hv, dk, dv] f32; dk up to 128, dv up to 1,024, Hv a multiple of Hk. offsets [S + 1] int32: sequence s has rows
+    offsets[s] to offsets[s + 1]; None: as many sequences of one length as `state` has (one without a state). Rows outside all
+    sequences get zeros. g = -inf forgets the state: an episode's first token. With keys of length one and beta below 2 the
+    rule is stable. `saved` (None without save) is what delta_rule_grad takes."""
+    if offsets is not None:
+        sequences = offsets.shape[0] - 1
+    else:
+        sequences = 1 if state is None else state.shape[0]
+    o, final, saved = _ext.delta_rule(q, k, v, g, beta, offsets, sequences, state, _scale(q, scale), save)
+    return o, final, ((saved, sequences) if save else None)
+
+
+def delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved, scale=None):
+    """(dq, dk, dv, dg, dbeta, dstate) of delta_rule from the gradients do [N, Hv, dv] bf16 of o and dstate of the final
+    state (None: zero); the last of the results is that of the first state. The other arguments are the forward call's, `saved`
+    what it returned. dq, dk, dv bf16, dg, dbeta, dstate f32."""
+    if saved is None:
+        raise PufferError("delta_rule_grad: saved is needed (delta_rule with save=True)")
+    return _ext.delta_rule_grad(q, k, v, g, beta, offsets, saved[1], do, dstate, _scale(q, scale), saved[0])
+
+
+def delta_rule_step(q, k, v, g, beta, state, scale=None, out=None):
+    """(o, state): delta_rule for one token of every row, state [N, Hv, dk, dv] f32. The new states go into `out`, which may
+    be `state` itself, or a new tensor."""
+    return _ext.delta_rule_step(q, k, v, g, beta, state, _scale(q, scale), out)
