@@ -8,18 +8,22 @@
 // Every sum is f64, and so is every exponential behind one: a row of V near-equal tokens has V borders, and f32 sums
 // (1e-7 off) would move one of them across u in 2 rows of 100 at V = 131,072.
 //
-// Many rows: a CTA per row, which walks it again for each step below (from L2: the rows in flight fit there). Few rows: a cluster of
-// CTAs per row, each with a contiguous slice in shared memory.
+// Many rows: a CTA per row, which walks it from L2 for each step below (the rows in flight fit there). Few rows: a cluster
+// of CTAs per row, each with a contiguous slice in shared memory.
 //
-// The border of top-k or top-p is found in three steps. (1) One or two walks with f32 weights put counts or masses into 64
-// bins of d = max - z, each thread's its own (no atomics), the second walk's around the border that the first one shows:
-// this proposes an interval [zb, za] of logits. (2) A walk in f64 takes the masses above, in and below the interval and
-// lists what lies in it. (3) If these say that the border is inside, which they do but for a few rows in a million, the list is
-// sorted and the border is exact. Otherwise, or if the list overflows (more equal logits than it holds), the border's
-// key is searched bit by bit. So the f32 sums cost time where they are off, never a token.
+// Without filters that is one walk with f64 sums by warp, segment and lane; the segment of u's place is walked once more.
+// The border of top-k or top-p is found in three steps. (1) A sample of the row and a walk with f32 weights put counts or
+// masses into 64 bins of d = ref - z, each thread's its own (no atomics): this proposes an interval [zb, za] of logits
+// around the border. (2) A walk in f64 takes the masses above, in and below the interval and lists what lies in it. (3) If
+// these say that the border is inside, which they do but for a few rows in a million, the list is sorted and the border
+// is exact. If the proposal fails, more walks propose; if the list overflows (more equal logits than it holds), the
+// border's key is searched bit by bit. So sample and f32 sums cost time where they are off, never a token. top_k up to 1,024 takes
+// one walk: the sample gives a bound that surely more than k pass, and what passes it is listed and sorted.
 //
-// Bound by the f64 pipe: one walk of 11 f64 operations per logit is 5.5 clocks per 32 logits on an SM, 100 us at 1,024 x
-// 131,072 (HBM: 41 us in bf16).
+// Exponents refer to the sample's largest logit instead of the row's: f64 has the room (2^900), and the walk that needs it
+// finds the largest on its way.
+//
+// Bound by the f64 pipe: one walk of 12 f64 operations per logit is 6 clocks per 32 logits on an SM.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -67,29 +71,67 @@ __device__ __forceinline__ float exp2_fast(float y) {
   return e;
 }
 
-// exp((z - max) / T) in f64: 2^y, y = n / 16 + r with 2^(n / 16) from a table and 2^r, |r| <= 1/32, from five terms of its series
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+  return m;
+}
+
+// exp((z - ref) / T) in f64: 2^y, y = n / 16 + r with 2^(n / 16) from a table and 2^r, |r| <= 1/32, from five terms of its series
 // (the sixth is 1.4e-13 of the value at most).
 struct Exp {
-  double max, c;  // c = log2(e) / T
+  double ref, c;  // c = log2(e) / T
   const double* tab;
-  __device__ __forceinline__ double operator()(float z) const {
-    // the f32's bits as a double (a conversion has a quarter of the rate); below 2^-126 it is off by as little
-    const uint32_t b = __float_as_uint(z);
-    const double d = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + (896u << 20))), (int)(b << 29));
-    const double y = (d - max) * c;
+  // N values step by step side by side: one after the other, each waits out the latency of a dozen f64 operations.
+  template <int N>
+  __device__ __forceinline__ void many(const float* z, double* e) const {
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the rounded integer
-    const double s = fma(y, 16.0, magic);
-    const int n = __double2loint(s);
-    const double r = fma(s - magic, -0.0625, y);
     const double l = 0.6931471805599453094;
-    double q = l * l * l * l * l / 120.0;
-    q = fma(q, r, l * l * l * l / 24.0);
-    q = fma(q, r, l * l * l / 6.0);
-    q = fma(q, r, l * l / 2.0);
-    q = fma(q, r, l);
-    q = fma(q, r, 1.0) * tab[n & 15];
-    const double e = __hiloint2double(__double2hiint(q) + (n >> 4) * (1 << 20), __double2loint(q));
-    return (uint32_t)__double2hiint(y) < 0xc08f4000u ? e : 0.0;  // y > -1000: by the order of negative doubles' bits
+    double y[N], s[N], q[N];
+    int n[N];
+    bool in[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) {  // the f32's bits as a double (a conversion has a quarter of the rate); below 2^-126 it is off by as little
+      const uint32_t b = __float_as_uint(z[j]);
+      y[j] = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + (896u << 20))), (int)(b << 29)) - ref;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) y[j] *= c;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      in[j] = (uint32_t)__double2hiint(y[j]) < 0xc08f4000u;  // y > -1000: by the order of negative doubles' bits
+      s[j] = fma(y[j], 16.0, magic);
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      n[j] = __double2loint(s[j]);
+      s[j] -= magic;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) y[j] = fma(s[j], -0.0625, y[j]);
+    const double k5 = l * l * l * l * l / 120.0, k4 = l * l * l * l / 24.0, k3 = l * l * l / 6.0, k2 = l * l / 2.0;
+#pragma unroll
+    for (int j = 0; j < N; j++) q[j] = fma(k5, y[j], k4);
+#pragma unroll
+    for (int j = 0; j < N; j++) q[j] = fma(q[j], y[j], k3);
+#pragma unroll
+    for (int j = 0; j < N; j++) q[j] = fma(q[j], y[j], k2);
+#pragma unroll
+    for (int j = 0; j < N; j++) q[j] = fma(q[j], y[j], l);
+#pragma unroll
+    for (int j = 0; j < N; j++) q[j] = fma(q[j], y[j], 1.0);
+#pragma unroll
+    for (int j = 0; j < N; j++) q[j] *= tab[n[j] & 15];
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const double x = __hiloint2double(__double2hiint(q[j]) + (n[j] >> 4) * (1 << 20), __double2loint(q[j]));
+      e[j] = in[j] ? x : 0.0;
+    }
+  }
+  __device__ __forceinline__ double operator()(float z) const {
+    double e;
+    many<1>(&z, &e);
+    return e;
   }
 };
 
@@ -173,28 +215,37 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     if constexpr (VEC == 4) return __uint_as_float(u4[j]);
     else return __uint_as_float(j & 1 ? u4[j / 2] & 0xffff0000u : u4[j / 2] << 16);
   };
-  // f(value, index in the row) for the values of warp w's iterations [i0, i1), and done(iteration) behind each; U vectors are
-  // loaded at a time.
+  // f(VEC values, the first one's index in the row) for the vectors of warp w's iterations [i0, i1), and done(iteration)
+  // behind each; U vectors are loaded at a time. What f computes of all values before it branches on one of them overlaps.
   auto walk_part = [&](auto unroll, int w, int i0, int i1, auto f, auto done) {
     constexpr int U = decltype(unroll)::value;
     for (int it = i0; it < i1; it += U) {
       uint4 x[U];
+      const int v0 = w * per_warp + it * 32;  // the warp's first vector
+      if (SOLO && it + U <= i1 && v0 * VEC >= shift && (v0 + 32 * U) * VEC - shift <= len) {
+        const uint4* at = reinterpret_cast<const uint4*>(src - shift) + v0 + lane;
 #pragma unroll
-      for (int q = 0; q < U; q++) {
-        const int v = w * per_warp + (it + q) * 32 + lane;
-        if (it + q < i1 && v < vecs) {
-          if constexpr (SOLO) x[q] = fetch(v);
-          else x[q] = *reinterpret_cast<const uint4*>(cache + v * VEC);
-        } else {
-          const uint32_t none = VEC == 4 ? 0xff800000u : 0xff80ff80u;
-          x[q] = make_uint4(none, none, none, none);
+        for (int q = 0; q < U; q++) x[q] = __ldg(at + 32 * q);
+      } else {
+#pragma unroll
+        for (int q = 0; q < U; q++) {
+          const int v = v0 + q * 32 + lane;
+          if (it + q < i1 && v < vecs) {
+            if constexpr (SOLO) x[q] = fetch(v);
+            else x[q] = *reinterpret_cast<const uint4*>(cache + v * VEC);
+          } else {
+            const uint32_t none = VEC == 4 ? 0xff800000u : 0xff80ff80u;
+            x[q] = make_uint4(none, none, none, none);
+          }
         }
       }
 #pragma unroll
       for (int q = 0; q < U; q++) {
-        const uint32_t i = (uint32_t)(first + (w * per_warp + (it + q) * 32 + lane) * VEC - shift);
+        const uint32_t i = (uint32_t)(first + (v0 + q * 32 + lane) * VEC - shift);
+        float z[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; j++) f(value(x[q], j), i + j);
+        for (int j = 0; j < VEC; j++) z[j] = value(x[q], j);
+        f(z, i);
         if (it + q < i1) done(it + q);
       }
     }
@@ -203,51 +254,99 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
   using Four = std::integral_constant<int, 4>;
+  using ByCount = std::false_type;
+  using ByMass = std::true_type;
 
-  // ---- the largest logit
-  float top = -INFINITY, nan = 0.f;
+  // ---- a sample of the slice (all of it, if it is short), and its largest logit as what exponents refer to: any logit
+  // not far below the largest will do, and the walks below find the largest on their way
   if constexpr (!SOLO) {
     for (int it = 0; it < its; it++) {
       const int v = warp * per_warp + it * 32 + lane;
       if (v < vecs) *reinterpret_cast<uint4*>(cache + v * VEC) = fetch(v);
-    }  // a thread reads what it stored itself
-  }
-  walk_part(Four(), warp, 0, its,
-            [&](float z, uint32_t) {
-              top = fmaxf(top, z);
-              if (z != z) nan = 1.f;
-            },
-            nothing);
-  if (tid < 16) sh.tab[tid] = exp2((double)tid / 16.0);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    nan = fmaxf(nan, __shfl_xor_sync(0xffffffffu, nan, o));
-  }
-  if (lane == 0) {
-    sh.fwarp[warp][0] = top;
-    sh.fwarp[warp][1] = nan;
-  }
-  if (tid == 0) sh.count = 0;
-  sync();
-  top = -INFINITY, nan = 0.f;
-  for (int q = 0; q < ranks; q++) {
-    const float* other = of_rank(&sh.fwarp[0][0], q);
-    for (int w = 0; w < kWarps; w++) {
-      top = fmaxf(top, other[4 * w]);
-      nan = fmaxf(nan, other[4 * w + 1]);
     }
+    __syncthreads();
   }
-  if (!fine || nan != 0.f || fabsf(top) == INFINITY) {  // the same for every CTA of the cluster
+  constexpr int kSample = 4;  // vectors per thread
+  const int sampled = vecs < kSample * kThreads ? vecs : kSample * kThreads;
+  auto walk_sample = [&](auto f) {
+    uint4 x[kSample];
+#pragma unroll
+    for (int q = 0; q < kSample; q++) {
+      const int n = q * kThreads + tid;
+      const uint32_t none = VEC == 4 ? 0xff800000u : 0xff80ff80u;
+      x[q] = make_uint4(none, none, none, none);
+      if (n < sampled) {
+        const int v = vecs <= kSample * kThreads ? n : (int)((long)n * vecs / (kSample * kThreads));
+        if constexpr (SOLO) x[q] = fetch(v);
+        else x[q] = *reinterpret_cast<const uint4*>(cache + v * VEC);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kSample; q++) {
+      float z[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j++) z[j] = value(x[q], j);
+      f(z, 0u);
+    }
+  };
+  auto largest = [&](const float (&z)[VEC], float m) {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) m = max_nan(m, z[j]);
+    return m;
+  };
+  if (tid < 16) sh.tab[tid] = exp2((double)tid / 16.0);
+  if (tid == 0) sh.count = 0;
+  // The largest of the cluster's numbers, NaN if one of them is.
+  auto max_of_all = [&](float m) __attribute__((always_inline)) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) sh.fwarp[warp][0] = m;
+    sync();
+    for (int q = 0; q < ranks; q++) {
+      const float* other = of_rank(&sh.fwarp[0][0], q);
+      for (int w = 0; w < kWarps; w++) m = max_nan(m, other[4 * w]);
+    }
+    sync();
+    return m;
+  };
+  float ref = -INFINITY;
+  walk_sample([&](const float(&z)[VEC], uint32_t) { ref = largest(z, ref); });
+  ref = max_of_all(ref);
+  float top = ref;  // the largest logit, once a walk over all of them is done
+  auto walk_max = [&]() __attribute__((always_inline)) {
+    float m = -INFINITY;
+    walk_part(Four(), warp, 0, its, [&](const float(&z)[VEC], uint32_t) { m = largest(z, m); }, nothing);
+    ref = top = max_of_all(m);
+  };
+  const bool plain = k == 0 && top_p >= 1.0 && min_p <= 0.0;
+  const bool few = k > 0 && k <= kList / 2, nucleus = k == 0 && top_p < 1.0;
+  bool known = false;  // whether `top` is of all
+  if (ref == -INFINITY || !(plain || few || nucleus)) {
+    walk_max();
+    known = true;
+  }
+  auto bad = [&](float z) { return !(fabsf(z) < INFINITY); };
+  auto refuse = [&] {
     if (rank == 0 && tid == 0) {
       a.token[row] = -1;
       a.logp[row] = __int_as_float(0x7fffffff);
     }
     sync();
+  };
+  if (!fine || bad(top)) {  // the same for every CTA of the cluster
+    refuse();
     return;
   }
-  const Exp exp_of = {(double)top, 1.4426950408889634074 / temp, sh.tab};
+  Exp exp_of = {(double)ref, 1.4426950408889634074 / temp, sh.tab};
   const float cf = (float)fmin(exp_of.c, 1e37);
+  float zfloor = ref - 750.f * (float)temp;  // below it every e is zero: such logits are left out of counts, too
+  auto refer_to = [&](float z) {
+    ref = z;
+    exp_of.ref = (double)z;
+    zfloor = z - 750.f * (float)temp;
+  };
+  // After a walk that found `top`: whether the exponents were too far above their reference. (f64: 2^900; f32: 2^60)
+  auto too_far = [&](float most) { return ((double)top - (double)ref) * exp_of.c > (double)most; };
 
   // ---- sums over the cluster, in rank order: N numbers per thread; every thread gets them
   int turn = 0;
@@ -276,13 +375,14 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
   // ---- what stays: z > tz, and z = tz up to index tidx
   float tz = -INFINITY;
   uint32_t tidx = 0xffffffffu;
+  bool bounded = false;  // whether any is known
   auto stays = [&](float z, uint32_t i) { return z > tz || (z == tz && i <= tidx); };
 
   auto push = [&](float z, uint32_t i) {  // to rank 0's list: (~key, index), which sorts by falling z, then index
     const int n = atomicAdd(of_rank(&sh.count, 0), 1);
     if (n < kList) of_rank(list, 0)[n] = (unsigned long long)(~key_of(z)) << 32 | i;
   };
-  auto sort_list = [&](int n) {  // by the threads of rank 0; up to the next power of two with ~0
+  auto sort_list = [&](int n) __attribute__((always_inline)) {  // by the threads of rank 0; up to the next power of two with ~0
     int size = 64;
     while (size < n) size *= 2;
     for (int i = n + tid; i < size; i += kThreads) list[i] = ~0ull;
@@ -324,99 +424,124 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     return base + (lane ? up : 0.0);
   };
 
-  // Below it every e is zero: such logits are left out of counts, too.
-  const float zfloor = top - 750.f * (float)temp;
-
-  // ---- step 1: bins of d = (max - z) by f32 weights among what stays so far; [lo, hi] of d around the border. By mass: equal
-  // steps of 3/8 T; by count: quarters of octaves up to 750 T (beyond it e is zero); then 62 steps of the interval.
-  // Ends when about `room` members are left, or the weight of the interval and all above it (all) is.
-  auto propose = [&](bool by_mass, double want, bool share, bool all, float& za, float& zb) {
-    const float end = 750.f * (float)temp;
-    float lo = 0.f, inv = (float)kBins / fmaxf(24.f * (float)temp, 1e-36f);
-    const int octaves = (int)(__float_as_uint(fmaxf(end, 1e-30f)) >> 21) - (kBins - 1);
-    float d0 = 0.f, d1 = INFINITY;
-    for (int level = 0; level < 3; level++) {
-      const bool by_octave = level == 0 && !by_mass;
-      for (int b = 0; b < kBins; b++) hist[b * kThreads + tid] = 0.f;
-      walk_part(Two(), warp, 0, its,
-                [&](float z, uint32_t i) {
-                  if (!(z >= zfloor) || !stays(z, i)) return;
-                  const float d = top - z;
-                  int b;
-                  if (by_octave) b = min(max((int)(__float_as_uint(d) >> 21) - octaves, 0), kBins - 1);
-                  else b = __float_as_int(fminf(fmaxf((d - lo) * inv, 0.f), (float)(kBins - 1)) + 12582912.f) & (kBins - 1);
-                  hist[b * kThreads + tid] += by_mass ? exp2_fast(-d * cf) : 1.f;
-                },
-                nothing);
-      __syncthreads();
-      for (int b = warp; b < kBins; b += kWarps) {
-        double s = 0.0;
-        for (int q = 0; q < kThreads / 32; q++) s += (double)hist[b * kThreads + q * 32 + lane];
-        s = warp_add(s);
-        if (lane == 0) sh.x[turn][b] = s;
-      }
-      sync();
-      double bin[2];  // this lane's two bins, over the cluster; every warp alike
+  // ---- step 1: bins of d = ref - z by f32 weights among what stays so far; an interval [d0, d1] around the border. By
+  // mass: equal steps of 3/8 T, from 6 T above the reference on; by count: quarters of octaves up to 750 T (beyond it e is zero).
+  struct Span {
+    float d0, d1;        // the border's interval
+    double until, most;  // how much there is down to d1; the most tokens that the interval (all: everything down to d1) holds
+    bool inside;         // it touches neither the first nor the last bin
+  };
+  auto bins = [&](auto walk, auto weighing, bool by_octave, bool all, double want, double fuzz, bool share, float lo,
+                  float inv) __attribute__((always_inline)) {
+    constexpr bool by_mass = decltype(weighing)::value;
+    const int octaves = (int)(__float_as_uint(fmaxf(750.f * (float)temp, 1e-30f)) >> 21) - (kBins - 1);
+    for (int b = 0; b < kBins; b++) hist[b * kThreads + tid] = 0.f;
+    const float shift_b = -lo * inv;
+    walk([&](const float(&z)[VEC], uint32_t i) {
+      int b[VEC];
+      float w[VEC];
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        bin[h] = 0.0;
-        for (int q = 0; q < ranks; q++) bin[h] += *of_rank(&sh.x[turn][2 * lane + h], q);
+      for (int j = 0; j < VEC; j++) {
+        const float d = ref - z[j];
+        if (by_octave) b[j] = min(max((int)(__float_as_uint(fmaxf(d, 0.f)) >> 21) - octaves, 0), kBins - 1);
+        else  // rounded to the nearest bin by the sum with 1.5 * 2^23; -inf is in the last one and weighs nothing
+          b[j] = __float_as_int(fminf(fmaxf(__fmaf_rn(d, inv, shift_b), 0.f), (float)(kBins - 1)) + 12582912.f) & (kBins - 1);
+        if constexpr (by_mass) w[j] = exp2_fast(-d * cf);
+        else w[j] = z[j] >= zfloor ? 1.f : 0.f;
+        if (bounded) w[j] = stays(z[j], i + j) ? w[j] : 0.f;
       }
-      turn ^= 1;
-      double inc = bin[0] + bin[1];
 #pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const double up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      const double total = __shfl_sync(0xffffffffu, inc, 31);
-      const double target = share ? want * total : want, fuzz = by_mass ? 3e-5 * total : 0.0;
-      // the first bin at whose end the border can have come, and the first by whose end it must have
-      const double end0 = inc - bin[1], end1 = inc;
-      const unsigned can0 = __ballot_sync(0xffffffffu, end0 >= target - fuzz), can1 = __ballot_sync(0xffffffffu, end1 >= target - fuzz);
-      const unsigned must0 = __ballot_sync(0xffffffffu, end0 >= target + fuzz), must1 = __ballot_sync(0xffffffffu, end1 >= target + fuzz);
-      auto first_of = [](unsigned m0, unsigned m1) {
-        const int i0 = m0 ? 2 * (__ffs(m0) - 1) : kBins - 1, i1 = m1 ? 2 * (__ffs(m1) - 1) + 1 : kBins - 1;
-        return min(i0, i1);
-      };
-      const int b0 = first_of(can0, can1), b1 = first_of(must0, must1);
-      double members = 0.0, until = 0.0;
+      for (int j = 0; j < VEC; j++) hist[b[j] * kThreads + tid] += w[j];
+    });
+    __syncthreads();
+    for (int b = warp; b < kBins; b += kWarps) {
+      float s = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; h++)
-        if (2 * lane + h <= b1) {
-          until += bin[h];
-          if (2 * lane + h >= b0) members += bin[h];
-        }
-      members = warp_add(members);
-      until = warp_add(until);
-      __syncthreads();  // the bins may be cleared again
-      // bins 0 and 63 hold what is outside as well: there the interval's ends stay as they were
-      if (by_octave) {
-        if (b0 > 0) d0 = __uint_as_float((uint32_t)(b0 + octaves) << 21);
-        if (b1 < kBins - 1) d1 = __uint_as_float((uint32_t)(b1 + 1 + octaves) << 21);
-      } else {
-        const float step = 1.f / inv;
-        if (b0 > 0) d0 = fmaxf(d0, lo + ((float)b0 - 0.51f) * step);
-        if (b1 < kBins - 1) d1 = fminf(d1, lo + ((float)b1 + 0.51f) * step);
-      }
-      za = d0 > 0.f ? top - d0 * 0.999999f : INFINITY;
-      zb = fmaxf(top - d1 * 1.000001f, zfloor);
-      // by mass, the bin's tokens are counted by the weight of its far end
-      const double many = all ? until : by_mass ? members * exp2((double)fminf(d1 * cf, 1000.f)) : members;
-      if (many <= 0.6 * kList || d1 == INFINITY || !(d1 > d0)) break;
-      inv = fminf((float)(kBins - 2) / (d1 - d0), 1e30f);
-      lo = d0 - 1.f / inv;
+      for (int q = 0; q < kThreads / 32; q++) s += hist[b * kThreads + q * 32 + lane];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) sh.x[turn][b] = (double)s;
     }
+    sync();
+    double bin[2];  // this lane's two bins, over the cluster; every warp alike
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      bin[h] = 0.0;
+      for (int q = 0; q < ranks; q++) bin[h] += *of_rank(&sh.x[turn][2 * lane + h], q);
+    }
+    turn ^= 1;
+    double inc = bin[0] + bin[1];
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const double up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    const double total = __shfl_sync(0xffffffffu, inc, 31);
+    const double target = share ? want * total : want, off = share ? fuzz * total : fuzz;
+    // the first bin by whose end the border can have come, and the first by whose end it must have
+    const double end0 = inc - bin[1], end1 = inc;
+    auto first_from = [&](double x) {
+      const unsigned m0 = __ballot_sync(0xffffffffu, end0 >= x), m1 = __ballot_sync(0xffffffffu, end1 >= x);
+      return min(m0 ? 2 * (__ffs(m0) - 1) : kBins - 1, m1 ? 2 * (__ffs(m1) - 1) + 1 : kBins - 1);
+    };
+    const int b0 = first_from(target - off), b1 = first_from(target + off);
+    double members = 0.0, until = 0.0;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+      if (2 * lane + h <= b1) {
+        until += bin[h];
+        if (2 * lane + h >= b0) members += bin[h];
+      }
+    members = warp_add(members);
+    until = warp_add(until);
+    __syncthreads();  // the bins may be cleared again
+    Span r;
+    r.until = until;
+    r.inside = b0 > 0 && b1 < kBins - 1;
+    if (by_octave) {
+      r.d0 = b0 > 0 ? __uint_as_float((uint32_t)(b0 + octaves) << 21) : -INFINITY;
+      r.d1 = b1 < kBins - 1 ? __uint_as_float((uint32_t)(b1 + 1 + octaves) << 21) : INFINITY;
+    } else {
+      const float step = 1.f / inv;
+      r.d0 = b0 > 0 ? lo + ((float)b0 - 0.51f) * step : -INFINITY;
+      r.d1 = b1 < kBins - 1 ? lo + ((float)b1 + 0.51f) * step : INFINITY;
+    }
+    // by mass, tokens are counted by the weight of the interval's far end
+    r.most = all ? until : by_mass ? members * exp2((double)fmaxf(fminf(r.d1 * cf, 1000.f), -1000.f)) : members;
+    return r;
+  };
+  const float mass_lo = -6.f * (float)temp, mass_inv = fminf((float)kBins / fmaxf(24.f * (float)temp, 1e-36f), 1e30f);
+  auto walk_all = [&](auto f) { walk_part(Two(), warp, 0, its, f, nothing); };
+  auto ends = [&](const Span& r, float& za, float& zb) {  // of logits, a little outside the interval's of d
+    za = r.d0 > -INFINITY ? ref - (r.d0 - fabsf(r.d0) * 1e-6f) : INFINITY;
+    zb = fmaxf(ref - (r.d1 + fabsf(r.d1) * 1e-6f), zfloor);
+  };
+  // By walks over all logits: the second and third one's 62 steps cut up the interval that the one before it showed.
+  auto propose = [&](auto weighing, double want, bool share, bool all, float& za, float& zb) __attribute__((always_inline)) {
+    constexpr bool by_mass = decltype(weighing)::value;
+    const double fuzz = by_mass ? 3e-5 : 0.0;
+    Span r = bins(walk_all, weighing, !by_mass, all, want, fuzz, share, mass_lo, mass_inv);
+    for (int level = 1; level < 3; level++) {
+      const float d0 = fmaxf(r.d0, by_mass ? mass_lo : 0.f);
+      if (r.most <= 0.6 * kList || r.d1 == INFINITY || !(r.d1 > d0)) break;
+      const float inv = fminf((float)(kBins - 2) / (r.d1 - d0), 1e30f), was0 = r.d0, was1 = r.d1;
+      r = bins(walk_all, weighing, false, all, want, fuzz, share, d0 - 1.f / inv, inv);
+      r.d0 = fmaxf(r.d0, was0);  // the outer bins hold what is outside as well: there the ends stay
+      r.d1 = fminf(r.d1, was1);
+    }
+    ends(r, za, zb);
   };
 
   // The border's key by bits, among the logits in [zb, za] whose order is not known; `above`: what the others above them weigh.
-  auto search = [&](bool by_mass, double above, double want, float za, float zb) {
+  auto search = [&](bool by_mass, double above, double want, float za, float zb) __attribute__((always_inline)) {
     auto in = [&](float z, uint32_t i) { return z <= za && z >= zb && stays(z, i); };
     auto weight_from = [&](uint32_t from) {
       double s[1] = {0.0};
       walk_part(One(), warp, 0, its,
-                [&](float z, uint32_t i) {
-                  if (in(z, i) && key_of(z) >= from) s[0] += by_mass ? exp_of(z) : 1.0;
+                [&](const float(&z)[VEC], uint32_t i) {
+#pragma unroll
+                  for (int j = 0; j < VEC; j++)
+                    if (in(z[j], i + j) && key_of(z[j]) >= from) s[0] += by_mass ? exp_of(z[j]) : 1.0;
                 },
                 nothing);
       sums(s);
@@ -424,8 +549,10 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     };
     float low = INFINITY, high = -INFINITY;
     walk_part(One(), warp, 0, its,
-              [&](float z, uint32_t i) {
-                if (in(z, i)) low = fminf(low, z), high = fmaxf(high, z);
+              [&](const float(&z)[VEC], uint32_t i) {
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                  if (in(z[j], i + j)) low = fminf(low, z[j]), high = fmaxf(high, z[j]);
               },
               nothing);
 #pragma unroll
@@ -457,8 +584,10 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     const float z0 = of_key(key);
     double equals[1] = {0.0};
     walk_part(One(), warp, 0, its,
-              [&](float z, uint32_t i) {
-                if (z == z0 && stays(z, i)) equals[0] += 1.0;
+              [&](const float(&z)[VEC], uint32_t i) {
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                  if (z[j] == z0 && stays(z[j], i + j)) equals[0] += 1.0;
               },
               nothing);
     const double own = warp_add(equals[0]);
@@ -473,29 +602,25 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     __syncthreads();
     for (int w = 0; w < warp; w++) before += sh.warp[w][0];
     if (before < need && need <= before + own) {  // the warp that holds the need-th equal
-      int n = 0;
-      uint32_t mine[VEC];
       walk_part(One(), warp, 0, its,
-                [&](float z, uint32_t i) {
-                  const bool is = z == z0 && stays(z, i);
+                [&](const float(&z)[VEC], uint32_t i) {
+                  int n = 0;
 #pragma unroll
-                  for (int j = 0; j < VEC; j++)
-                    if (is && n == j) mine[j] = i;
-                  n += is;
-                },
-                [&](int) {
+                  for (int j = 0; j < VEC; j++) n += z[j] == z0 && stays(z[j], i + j);
                   int inc = n;
                   for (int o = 1; o < 32; o *= 2) {
                     const int up = __shfl_up_sync(0xffffffffu, inc, o);
                     if (lane >= o) inc += up;
                   }
-                  const int left = (int)(need - before) - (inc - n);  // this lane's left-th is the one
+                  int left = (int)(need - before) - (inc - n);  // this lane's left-th is the one
+                  if (left >= 1 && left <= n) {
 #pragma unroll
-                  for (int j = 0; j < VEC; j++)
-                    if (left == j + 1 && left <= n) sh.found = (int)mine[j];
+                    for (int j = 0; j < VEC; j++)
+                      if (z[j] == z0 && stays(z[j], i + j) && --left == 0) sh.found = (int)i + j;
+                  }
                   before += (double)__shfl_sync(0xffffffffu, inc, 31);
-                  n = 0;
-                });
+                },
+                nothing);
     }
     sync();
     int found = -1;
@@ -503,9 +628,10 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     sync();
     tz = z0;
     tidx = (uint32_t)found;
+    bounded = true;
   };
   // The border in rank 0's list of n: the last entry before which less than `want` comes, `above` included.
-  auto border = [&](bool by_mass, double above, double want, int n) {
+  auto border = [&](bool by_mass, double above, double want, int n) __attribute__((always_inline)) {
     int m = 0;
     if (rank == 0) {
       sort_list(n);
@@ -532,26 +658,70 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     sync();
     tz = *of_rank(&sh.tz, 0);
     tidx = *of_rank(&sh.tidx, 0);
+    bounded = true;
     m = *of_rank(&sh.found, 0);
     sync();
     return m;
   };
 
-  if (k > 0) {
-    float za, zb;
-    const bool few = k <= kList / 2;
-    propose(false, (double)k, false, few, za, zb);
-    double above[1] = {0.0};
+  // The listing of what is in [zb, za], by count; `above` it
+  auto list_walk = [&](float za, float zb, bool all, double& above, float& most) {
+    double n[1] = {0.0};
+    float m = -INFINITY;
     walk_part(Four(), warp, 0, its,
-              [&](float z, uint32_t i) {
-                if (z > za && !few) above[0] += 1.0;
-                else if (z >= zb) push(z, i);
+              [&](const float(&z)[VEC], uint32_t i) {
+                const float high = largest(z, -INFINITY);
+                m = max_nan(m, high);
+                if (high < zb) return;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                  if (!(z[j] >= zb)) continue;
+                  if (z[j] > za && !all) n[0] += 1.0;
+                  else push(z[j], i + j);
+                }
               },
               nothing);
-    sums(above);
-    const int n = *of_rank(&sh.count, 0);
+    most = max_of_all(m);
+    sums(n);
+    above = n[0];
+    const int listed = *of_rank(&sh.count, 0);
     sync();
     if (tid == 0) sh.count = 0;
+    return listed;
+  };
+  if (k > 0) {
+    float za = INFINITY, zb = zfloor;
+    double above = 0.0;
+    int n = kList + 1;
+    if (few) {
+      // the sample's share of k, and four of its standard deviations and a few more: a list of all that is above that
+      const double share = fmin(1.0, (double)(kSample * kThreads) * VEC * ranks / a.V);
+      const double of_k = share * k, want = share < 1.0 ? of_k + 4.0 * sqrt(of_k) + 8.0 : (double)k;
+      const Span r = bins(walk_sample, ByCount(), true, true, want, 0.0, false, 0.f, 0.f);
+      float most = top;
+      if (r.until <= 0.8 * share * kList || r.until < want) {  // (less than wanted: the sample has no more that count)
+        if (r.until >= want) ends(r, za, zb);
+        n = list_walk(INFINITY, zb, true, above, most);
+        known = true;
+        top = most;
+      }
+    }
+    if (!known) walk_max(), known = true;
+    if (bad(top)) {
+      refuse();
+      return;
+    }
+    if (ref != top) {
+      // what is left out below zfloor has no mass beside the largest either
+      const float was = zfloor;
+      refer_to(top);
+      if (zb == was) zb = zfloor;
+    }
+    if (!(few && n <= kList && (n >= k || zb == zfloor))) {
+      propose(ByCount(), (double)k, false, few, za, zb);
+      float unused;
+      n = list_walk(za, zb, few, above, unused);
+    }
     if (few && n <= kList && (n >= k || zb == zfloor)) {  // the list holds all of the first k: the rest is rank 0's
       if (rank == 0) {
         sort_list(n);
@@ -606,39 +776,58 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
           }
           const unsigned long long e1 = list[best != 0xffffffffu ? (int)best : back];
           a.token[row] = (int)(e1 >> 32);
-          a.logp[row] = (float)(((double)of_key((uint32_t)e1) - (double)top) / temp - log(total));
+          a.logp[row] = (float)(((double)of_key((uint32_t)e1) - (double)ref) / temp - log(total));
         }
       }
       sync();
       return;
     }
-    if (!few && n <= kList && above[0] < (double)k && above[0] + n >= (double)k)
-      border(false, above[0], (double)k, n);
-    else if (few || zb > zfloor || above[0] + n >= (double)k)  // (otherwise no more than k have any mass)
+    if (!few && n <= kList && above < (double)k && above + n >= (double)k)
+      border(false, above, (double)k, n);
+    else if (few || zb > zfloor || above + n >= (double)k)  // (otherwise no more than k have any mass)
       search(false, 0.0, (double)k, INFINITY, zfloor);
   }
 
   // ---- step 2: the f64 walk. Above [zb, za] what stays goes into sums by warp, segment of its iterations, and lane; the rest of it,
   // and the members, into sums of their own.
   const int seg_its = (its + kSegs - 1) / kSegs;
-  double w3[3];  // mass above, in, below
-  auto f64_walk = [&](float za, float zb, double floor, bool listing) {
+  double w3[3];  // mass above, in, and of all
+  constexpr int kPlain = 0, kKept = 1, kListing = 2;
+  auto f64_walk = [&](auto mode, float za, float zb, double floor) {
+    constexpr int MODE = decltype(mode)::value;
     double s = 0.0;
+    float m = -INFINITY;
     w3[0] = w3[1] = w3[2] = 0.0;
     for (int g = 0; g < kSegs; g++) sub[(warp * kSegs + g) * 32 + lane] = 0.0;
     walk_part(Two(), warp, 0, its,
-              [&](float z, uint32_t i) {
-                double e = exp_of(z);
-                e = stays(z, i) && e >= floor ? e : 0.0;
-                if (!listing) {
-                  s += e;
-                  return;
-                }
-                s += z > za ? e : 0.0;
-                w3[2] += z < zb ? e : 0.0;
-                if (z <= za && z >= zb && e > 0.0) {
-                  w3[1] += e;
-                  push(z, i);
+              [&](const float(&z)[VEC], uint32_t i) {
+                double e[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; j += 4) exp_of.template many<4>(z + j, e + j);
+                if constexpr (MODE == kPlain) {
+                  m = largest(z, m);
+#pragma unroll
+                  for (int j = 0; j < VEC; j++) s += e[j];
+                } else if constexpr (MODE == kKept) {
+#pragma unroll
+                  for (int j = 0; j < VEC; j++) s += stays(z[j], i + j) && e[j] >= floor ? e[j] : 0.0;
+                } else {
+                  unsigned in = 0;
+#pragma unroll
+                  for (int j = 0; j < VEC; j++) {
+                    if (bounded) e[j] = stays(z[j], i + j) ? e[j] : 0.0;
+                    w3[2] += e[j];
+                    s += z[j] > za ? e[j] : 0.0;
+                    if (z[j] <= za && z[j] >= zb) in |= 1u << j;
+                  }
+                  if (in) {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++)
+                      if ((in >> j & 1) && e[j] > 0.0) {
+                        w3[1] += e[j];
+                        push(z[j], i + j);
+                      }
+                  }
                 }
               },
               [&](int it) {
@@ -648,18 +837,66 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
                   s = 0.0;
                 }
               });
+    return m;
   };
+  using Plain = std::integral_constant<int, kPlain>;
+  using Kept = std::integral_constant<int, kKept>;
+  using Listing = std::integral_constant<int, kListing>;
   bool summed = false;
   int members = 0;  // of rank 0's list that stay, in `sub` not counted
+  if (plain) {
+    for (;;) {
+      const float m = max_of_all(f64_walk(Plain(), 0.f, 0.f, 0.0));
+      top = m;
+      if (bad(top)) {
+        refuse();
+        return;
+      }
+      if (!too_far(900.f)) break;
+      refer_to(top);
+    }
+    summed = true;
+  }
   if (top_p < 1.0) {
     float za, zb;
-    propose(true, top_p, true, false, za, zb);
-    f64_walk(za, zb, 0.0, true);
+    bool proposed = false;
+    if (!known) {
+      // the sample's interval, with 6 % of the mass on either side for its error, cut up by one walk over all
+      const Span r = bins(walk_sample, ByMass(), false, false, top_p, 0.06, true, mass_lo, mass_inv);
+      const float d0 = fmaxf(r.d0, mass_lo), d1 = fminf(r.d1, mass_lo + (float)kBins / mass_inv);
+      const float inv = fminf((float)(kBins - 2) / (d1 - d0), 1e30f);
+      float m = -INFINITY;
+      const Span all = bins(
+          [&](auto f) {
+            walk_part(Two(), warp, 0, its,
+                      [&](const float(&z)[VEC], uint32_t i) {
+                        m = largest(z, m);
+                        f(z, i);
+                      },
+                      nothing);
+          },
+          ByMass(), false, false, top_p, 3e-5, true, d0 - 1.f / inv, inv);
+      top = max_of_all(m);
+      known = true;
+      if (bad(top)) {
+        refuse();
+        return;
+      }
+      if (all.inside && all.most <= 0.6 * kList && !too_far(60.f)) {
+        ends(all, za, zb);
+        proposed = true;
+      }
+    }
+    if (!proposed) {
+      refer_to(top);
+      propose(ByMass(), top_p, true, false, za, zb);
+    }
+    f64_walk(Listing(), za, zb, 0.0);
     sums(w3);
     const int n = *of_rank(&sh.count, 0);
     sync();
     if (tid == 0) sh.count = 0;
-    const double want = top_p * (w3[0] + w3[1] + w3[2]);
+    const double want = top_p * w3[2];
     const bool inside = w3[0] < want && w3[0] + w3[1] >= want;
     if (inside && n <= kList) {
       members = border(true, w3[0], want, n);
@@ -672,9 +909,10 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
   }
 
   // ---- the draw: the segment that holds u's place is walked once more
+  const double floor = min_p > 0.0 ? min_p * exp_of(top) : 0.0;
   if (!summed) {
     __syncthreads();
-    f64_walk(-INFINITY, -INFINITY, min_p, false);
+    f64_walk(Kept(), 0.f, 0.f, floor);
     members = 0;
   }
   __syncthreads();
@@ -731,16 +969,16 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     const int seg = __reduce_max_sync(0xffffffffu, held);
     at = __shfl_sync(0xffffffffu, start, seg / 4);
     const int w = seg / kSegs, i0 = seg % kSegs * seg_its, i1 = min(its, i0 + seg_its);
-    int pick = -1, back = -1, n = 0;
-    double e[VEC], mine = 0.0;
+    int pick = -1, back = -1;
     walk_part(One(), w, i0, i1,
-              [&](float z, uint32_t i) {
-                const double x = exp_of(z);
-                e[n] = stays(z, i) && x >= min_p ? x : 0.0;
-                mine += e[n];
-                n++;
-              },
-              [&](int it) {
+              [&](const float(&z)[VEC], uint32_t i) {
+                double e[VEC], mine = 0.0;
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                  e[j] = exp_of(z[j]);
+                  e[j] = stays(z[j], i + j) && e[j] >= floor ? e[j] : 0.0;
+                  mine += e[j];
+                }
                 double inc = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o *= 2) {
@@ -753,14 +991,13 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
                 for (int j = 0; j < VEC; j++) {
                   here += e[j];
                   if (e[j] > 0.0) {
-                    back = (int)first + (w * per_warp + it * 32 + lane) * VEC - shift + j;
+                    back = (int)i + j;
                     if (pick < 0 && here > target) pick = back;
                   }
                 }
                 at += __shfl_sync(0xffffffffu, inc, 31);
-                mine = 0.0;
-                n = 0;
-              });
+              },
+              nothing);
     const unsigned lowest = __reduce_min_sync(0xffffffffu, (unsigned)pick);
     back = __reduce_max_sync(0xffffffffu, back);
     const int token = lowest != 0xffffffffu ? (int)lowest : back;
@@ -769,7 +1006,7 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
       if constexpr (VEC == 4) z = src[token - first];
       else z = __bfloat162float(src[token - first]);
       a.token[row] = token;
-      a.logp[row] = (float)(((double)z - (double)top) / temp - log(total));
+      a.logp[row] = (float)(((double)z - (double)ref) / temp - log(total));
     }
   }
   sync();
