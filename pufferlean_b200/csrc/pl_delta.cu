@@ -130,8 +130,12 @@ __global__ void __launch_bounds__(256) delta_step_kernel(const StepArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------- X and P of all chunks
-// Per slot and value head: X as two bf16 parts, P as two bf16 parts, each 64 x 64.
-constexpr long kMats = 4L * kC * kC;
+// Per slot and value head: X and P, triangular, as two bf16 parts each (in the order X, its second part, P, its second part), and
+// since, until, beta of the chunk's tokens.
+struct __align__(16) Mats {
+  __nv_bfloat16 x[2][kTri], p[2][kTri];
+  float since[kC], until[kC], beta[kC];
+};
 
 constexpr int kPrepThreads = 128;
 template <int DK>
@@ -143,7 +147,7 @@ struct PrepShared {
   Decay d;
 };
 template <int DK>
-__global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArgs a, __nv_bfloat16* __restrict__ mats) {
+__global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArgs a, Mats* __restrict__ mats) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
@@ -166,10 +170,15 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArg
   product<false, LD, false, LD>(qk, sh.q, nullptr, sh.k, nullptr, warp * 16, 0, 0, DK);
   for (int e = 0; e < group; e++) {
     const int h = kh * group + e;
-    __nv_bfloat16* out = mats + (slot * a.hv + h) * kMats;
+    Mats& out = mats[slot * a.hv + h];
     __syncthreads();
     chunk_decay(a, sh.d, start, len, h);
     __syncthreads();
+    if (tid < kC) {
+      out.since[tid] = sh.d.since[tid];
+      out.until[tid] = sh.d.until[tid];
+      out.beta[tid] = sh.d.beta[tid];
+    }
 #pragma unroll
     for (int t = 0; t < 8; t++)
 #pragma unroll
@@ -182,10 +191,12 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArg
           p[c] = j + c <= i ? qk[t][half * 2 + c] * f : 0.f;
           sh.at[j + c][i] = j + c < i ? kk[t][half * 2 + c] * f * sh.d.beta[j + c] : 0.f;
         }
-        uint32_t hi, lo;
-        split2(p[0], p[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(out + 2 * kC * kC + i * kC + j) = hi;
-        *reinterpret_cast<uint32_t*>(out + 3 * kC * kC + i * kC + j) = lo;
+        if (j >> 4 <= warp) {
+          uint32_t hi, lo;
+          split2(p[0], p[1], hi, lo);
+          *reinterpret_cast<uint32_t*>(out.p[0] + tri_at(i, j)) = hi;
+          *reinterpret_cast<uint32_t*>(out.p[1] + tri_at(i, j)) = lo;
+        }
       }
     __syncthreads();
     // the inverse's two diagonal blocks, a column per thread: x_i -= A_ij x_j as soon as x_j is known
@@ -232,30 +243,41 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArg
     for (int i = tid; i < kC * kC / 2; i += kPrepThreads) {
       const int r = i / (kC / 2), c = i % (kC / 2) * 2;
       uint32_t hi, lo;
+      if (c >> 4 > r >> 4) continue;
       split2(sh.x[r][c], sh.x[r][c + 1], hi, lo);
-      *reinterpret_cast<uint32_t*>(out + r * kC + c) = hi;
-      *reinterpret_cast<uint32_t*>(out + kC * kC + r * kC + c) = lo;
+      *reinterpret_cast<uint32_t*>(out.x[0] + tri_at(r, c)) = hi;
+      *reinterpret_cast<uint32_t*>(out.x[1] + tri_at(r, c)) = lo;
     }
   }
 }
 
 // ---------------------------------------------------------------------------------------------- the chain forward
-constexpr int kScanThreads = 256;
+// What a chain leaves for the gradient, per slot, value head and 64 columns of v, as two bf16 parts one behind the other: a
+// state [2][dk][64], rows [2][64][64].
+__device__ __forceinline__ long state_at(const DeltaArgs& a, long slot, int h, int slice) {
+  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * a.dk * 64;
+}
+__device__ __forceinline__ long rows_at(const DeltaArgs& a, long slot, int h, int slice) {
+  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * kC * 64;
+}
+
+constexpr int kScanThreads = 512;
 struct ScanArgs {
   DeltaArgs d;
-  const __nv_bfloat16* mats;
+  const Mats* mats;
   const float* state;  // [seqs][hv][dk][dv], or NULL: zero
   __nv_bfloat16* o;    // [n][hv][dv]
   float* final_state;
-  float *kept, *y;  // for the gradient: S per slot [hv][dk][dvp], Y per slot [hv][64][dvp]; or NULL
+  __nv_bfloat16 *kept, *y;  // for the gradient: S and Y of every slot; or NULL
 };
 template <int DK>
 struct ScanShared {
-  __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], v[kC * kLd];
-  __nv_bfloat16 mats[4][kC * kLd];  // X, its second part, P, its second part
-  __nv_bfloat16 s[2][DK * kLd];     // the state's columns
+  struct In {  // a chunk's inputs, loaded while the chunk before it is worked on
+    __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], v[kC * kLd];
+    Mats m;
+  } in[2];
+  __nv_bfloat16 s[2][DK * kLd];  // the state's columns
   __nv_bfloat16 r[2][kC * kLd], u[2][kC * kLd], w[2][kC * kLd];
-  Decay d;
 };
 
 // Rows that no sequence holds, in front of the first and behind the last: zero. Called by the blocks of those two.
@@ -270,22 +292,36 @@ __device__ __forceinline__ void zero_rows(const DeltaArgs& a, int seq, T* out, l
   }
 }
 
-// A block per sequence, value head and 64 of its columns. Warps hold the state in registers, 16 rows x 64 columns
-// each (dk <= 64: x 32); its two bf16 parts in shared memory are the operand of the next chunk's products.
+// A block per sequence, value head and 64 of its columns, 16 warps. They hold the state in registers, 16 rows x 32 columns
+// each (dk <= 64: x 16); its two bf16 parts in shared memory are the operand of the next chunk's products. (With one part of
+// S, U and P in what goes into o alone, a fifth of the products, o would be 2.5e-3 off instead of 1.7e-3.)
 template <int DK>
 __global__ void __launch_bounds__(kScanThreads) delta_scan_kernel(const ScanArgs p) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
   ScanShared<DK>& sh = *reinterpret_cast<ScanShared<DK>*>(mem);
-  constexpr int LD = DK + 8, NS = DK == 128 ? 8 : 4;  // n-tiles of a warp's part of the state
+  constexpr int LD = DK + 8, NS = DK / 32;  // n-tiles of a warp's part of the state
   const DeltaArgs& a = p.d;
-  const int c0 = blockIdx.x * 64, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
+  const int slice = blockIdx.x, c0 = slice * 64, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-  const int sm = DK == 128 ? warp * 16 : (warp & 3) * 16, sn = DK == 128 ? 0 : (warp >> 2) * 32;
+  const int sm = warp % (DK / 16) * 16, sn = warp / (DK / 16) * NS * 8;
   long from, to;
   seq_bounds(a, seq, from, to);
+  const long slot0 = from / kC + seq;
+  auto load = [&](long c) {
+    const long start = from + c * kC;
+    const int len = (int)(to - start < kC ? to - start : kC);
+    auto& in = sh.in[c & 1];
+    copy_tile<DK, LD, kScanThreads>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
+    copy_flat<kScanThreads>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats));
+    copy_tile<64, kLd, kScanThreads>(in.v, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vec);
+    copy_tile<DK, LD, kScanThreads>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
+    cp_commit();
+  };
+  const long chunks = (to - from + kC - 1) / kC;
+  if (chunks) load(0);
   zero_rows(a, seq, p.o + (long)h * a.dv + c0, (long)a.hv * a.dv, cols);
   float s[NS][4];
   const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + c0;
@@ -296,46 +332,39 @@ __global__ void __launch_bounds__(kScanThreads) delta_scan_kernel(const ScanArgs
       const int i = sm + (lane >> 2) + (e >> 1) * 8, j = sn + t * 8 + (lane & 3) * 2 + (e & 1);
       s[t][e] = p.state && i < a.dk && j < cols ? p.state[sbase + (long)i * a.dv + j] : 0.f;
     }
-  long slot = from / kC + seq;
-  for (long start = from; start < to; start += kC, slot++) {
+  for (long c = 0; c < chunks; c++) {
+    const long start = from + c * kC, slot = slot0 + c;
     const int len = (int)(to - start < kC ? to - start : kC);
-    const __nv_bfloat16* mats = p.mats + (slot * a.hv + h) * kMats;
-    copy_tile<DK, LD, kScanThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
-    copy_tile<DK, LD, kScanThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
-    copy_tile<64, kLd, kScanThreads>(sh.v, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vec);
-#pragma unroll
-    for (int m = 0; m < 4; m++) copy_tile<64, kLd, kScanThreads>(sh.mats[m], mats + m * kC * kC, kC, kC, kC, true);
-    cp_commit();
-    chunk_decay(a, sh.d, start, len, h);
+    const auto& in = sh.in[c & 1];
 #pragma unroll
     for (int t = 0; t < NS; t++)
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int i = sm + (lane >> 2) + half * 8, j = sn + t * 8 + (lane & 3) * 2;
-        put2<kLd>(sh.s[0], sh.s[1], i, j, s[t][half * 2], s[t][half * 2 + 1]);
-        if (p.kept && i < a.dk)
-          *reinterpret_cast<float2*>(p.kept + ((slot * a.hv + h) * a.dk + i) * a.dvp + c0 + j) =
-              make_float2(s[t][half * 2], s[t][half * 2 + 1]);
-      }
+      for (int half = 0; half < 2; half++)
+        put2<kLd>(sh.s[0], sh.s[1], sm + (lane >> 2) + half * 8, sn + t * 8 + (lane & 3) * 2, s[t][half * 2],
+                  s[t][half * 2 + 1]);
     cp_wait<0>();
     __syncthreads();
-    // warps 0 to 3: V - E K S; warps 4 to 7: E Q S
-    const int m0 = (warp & 3) * 16, i0 = m0 + (lane >> 2);
-    float acc[8][4];
+    if (c + 1 < chunks) load(c + 1);
+    if (p.kept)
+#pragma unroll
+      for (int part = 0; part < 2; part++)
+        tile_out<kScanThreads>(p.kept + state_at(a, slot, h, slice) + part * a.dk * 64, sh.s[part], a.dk);
+    // warps 0 to 7: V - E K S; warps 8 to 15: E Q S; 16 rows x 32 columns each
+    const int m0 = (warp & 3) * 16, n0 = (warp >> 2 & 1) * 32, i0 = m0 + (lane >> 2);
+    float acc[4][4];
     zero(acc);
-    product<false, LD, true, kLd>(acc, warp < 4 ? sh.k : sh.q, nullptr, sh.s[0], sh.s[1], m0, 0, 0, DK);
+    product<false, LD, true, kLd>(acc, warp < 8 ? in.k : in.q, nullptr, sh.s[0], sh.s[1], m0, n0, 0, DK);
 #pragma unroll
     for (int half = 0; half < 2; half++) {
       const int i = i0 + half * 8;
-      const float f = sh.d.since[i];
+      const float f = in.m.since[i];
 #pragma unroll
-      for (int t = 0; t < 8; t++) {
-        const int j = t * 8 + (lane & 3) * 2;
+      for (int t = 0; t < 4; t++) {
+        const int j = n0 + t * 8 + (lane & 3) * 2;
         float x = f == 0.f ? 0.f : f * acc[t][half * 2], y = f == 0.f ? 0.f : f * acc[t][half * 2 + 1];
-        if (warp < 4) {
-          x = __bfloat162float(sh.v[i * kLd + j]) - x;
-          y = __bfloat162float(sh.v[i * kLd + j + 1]) - y;
-          put2<kLd>(sh.r[0], sh.r[1], i, j, x, y);
+        if (warp < 8) {
+          const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(in.v + i * kLd + j);
+          put2<kLd>(sh.r[0], sh.r[1], i, j, __low2float(v) - x, __high2float(v) - y);
         } else {
           acc[t][half * 2] = x;
           acc[t][half * 2 + 1] = y;
@@ -343,48 +372,58 @@ __global__ void __launch_bounds__(kScanThreads) delta_scan_kernel(const ScanArgs
       }
     }
     __syncthreads();
-    {  // Y = X R, X lower triangular
-      const int n0 = (warp >> 2) * 32;
-      float y[4][4];
+    {  // Y = X R, 16 rows x 16 columns of every warp
+      const int y0 = (warp >> 2) * 16;
+      float y[2][4];
       zero(y);
-      product<false, kLd, true, kLd>(y, sh.mats[0], sh.mats[1], sh.r[0], sh.r[1], m0, n0, 0, m0 + 16);
+      tri_product<false, true, kLd>(y, in.m.x[0], in.m.x[1], sh.r[0], sh.r[1], warp & 3, y0);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = i0 + half * 8;
-        const float b = sh.d.beta[i], f = sh.d.until[i];
+        const float b = in.m.beta[i], f = in.m.until[i];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-          const int j = n0 + t * 8 + (lane & 3) * 2;
-          const float y0 = y[t][half * 2], y1 = y[t][half * 2 + 1];
-          if (p.y) *reinterpret_cast<float2*>(p.y + ((slot * a.hv + h) * kC + i) * a.dvp + c0 + j) = make_float2(y0, y1);
-          put2<kLd>(sh.u[0], sh.u[1], i, j, b * y0, b * y1);
-          put2<kLd>(sh.w[0], sh.w[1], i, j, f * b * y0, f * b * y1);
+        for (int t = 0; t < 2; t++) {
+          const int j = y0 + t * 8 + (lane & 3) * 2;
+          const float y1 = y[t][half * 2], y2 = y[t][half * 2 + 1];
+          if (p.y) {
+            uint32_t hi, lo;
+            split2(y1, y2, hi, lo);
+            __nv_bfloat16* to_y = p.y + rows_at(a, slot, h, slice) + i * 64 + j;
+            *reinterpret_cast<uint32_t*>(to_y) = hi;
+            *reinterpret_cast<uint32_t*>(to_y + kC * 64) = lo;
+          }
+          put2<kLd>(sh.u[0], sh.u[1], i, j, b * y1, b * y2);
+          put2<kLd>(sh.w[0], sh.w[1], i, j, f * b * y1, f * b * y2);
         }
       }
     }
     __syncthreads();
-    if (warp >= 4) {
-      product<false, kLd, true, kLd>(acc, sh.mats[2], sh.mats[3], sh.u[0], sh.u[1], m0, 0, 0, m0 + 16);
+    const float keep = in.m.since[kC - 1];
+#pragma unroll
+    for (int t = 0; t < NS; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
+    product<true, LD, true, kLd>(s, in.k, nullptr, sh.w[0], sh.w[1], sm, sn, 0, kC);
+    if (warp >= 8) {
+      tri_product<false, true, kLd>(acc, in.m.p[0], in.m.p[1], sh.u[0], sh.u[1], warp & 3, n0);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = i0 + half * 8;
         if (i >= len) continue;
         __nv_bfloat16* o = p.o + (start + i) * a.hv * a.dv + (long)h * a.dv + c0;
 #pragma unroll
-        for (int t = 0; t < 8; t++) {
-          const int j = t * 8 + (lane & 3) * 2;
-          if (j < cols) o[j] = __float2bfloat16_rn(a.scale * acc[t][half * 2]);
-          if (j + 1 < cols) o[j + 1] = __float2bfloat16_rn(a.scale * acc[t][half * 2 + 1]);
+        for (int t = 0; t < 4; t++) {
+          const int j = n0 + t * 8 + (lane & 3) * 2;
+          const float x = a.scale * acc[t][half * 2], y = a.scale * acc[t][half * 2 + 1];
+          if (a.dv % 2 == 0 && j + 1 < cols) {
+            *reinterpret_cast<__nv_bfloat162*>(o + j) = __floats2bfloat162_rn(x, y);
+          } else {
+            if (j < cols) o[j] = __float2bfloat16_rn(x);
+            if (j + 1 < cols) o[j + 1] = __float2bfloat16_rn(y);
+          }
         }
       }
     }
-    const float keep = sh.d.since[kC - 1];
-#pragma unroll
-    for (int t = 0; t < NS; t++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-    product<true, LD, true, kLd>(s, sh.k, nullptr, sh.w[0], sh.w[1], sm, sn, 0, kC);
-    __syncthreads();
   }
 #pragma unroll
   for (int t = 0; t < NS; t++)
@@ -398,37 +437,51 @@ __global__ void __launch_bounds__(kScanThreads) delta_scan_kernel(const ScanArgs
 // ---------------------------------------------------------------------------------------------- the chain back
 struct BackArgs {
   DeltaArgs d;
-  const __nv_bfloat16* mats;
+  const Mats* mats;
   const __nv_bfloat16* dout;  // [n][hv][dv], strides below
   long ldo, hso;
   bool vec_o;
-  const float* dfinal;     // [seqs][hv][dk][dv], or NULL: zero
-  __nv_bfloat16* dv;       // [n][hv][dv]
-  float* dstate;           // or NULL
-  float *ds, *dr;          // dS' per slot [hv][dk][dvp], dR per slot [hv][64][dvp]
+  const float* dfinal;        // [seqs][hv][dk][dv], or NULL: zero
+  __nv_bfloat16* dv;          // [n][hv][dv]
+  float* dstate;              // or NULL
+  __nv_bfloat16 *ds, *dr;     // dS' and dR of every slot
 };
 template <int DK>
 struct BackShared {
-  __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], o[kC * kLd];
-  __nv_bfloat16 mats[4][kC * kLd];
+  struct In {
+    __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], o[kC * kLd];
+    Mats m;
+  } in[2];
   __nv_bfloat16 s[2][DK * kLd];
   __nv_bfloat16 u[2][kC * kLd], r[2][kC * kLd], w[2][kC * kLd];
-  Decay d;
 };
+// As the chain forward, from the last chunk to the first.
 template <int DK>
 __global__ void __launch_bounds__(kScanThreads) delta_back_kernel(const BackArgs p) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
   BackShared<DK>& sh = *reinterpret_cast<BackShared<DK>*>(mem);
-  constexpr int LD = DK + 8, NS = DK == 128 ? 8 : 4;
+  constexpr int LD = DK + 8, NS = DK / 32;
   const DeltaArgs& a = p.d;
-  const int c0 = blockIdx.x * 64, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
+  const int slice = blockIdx.x, c0 = slice * 64, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-  const int sm = DK == 128 ? warp * 16 : (warp & 3) * 16, sn = DK == 128 ? 0 : (warp >> 2) * 32;
+  const int sm = warp % (DK / 16) * 16, sn = warp / (DK / 16) * NS * 8;
   long from, to;
   seq_bounds(a, seq, from, to);
+  const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
+  auto load = [&](long c) {
+    const long start = from + c * kC;
+    const int len = (int)(to - start < kC ? to - start : kC);
+    auto& in = sh.in[c & 1];
+    copy_tile<DK, LD, kScanThreads>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
+    copy_flat<kScanThreads>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats));
+    copy_tile<64, kLd, kScanThreads>(in.o, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
+    copy_tile<DK, LD, kScanThreads>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
+    cp_commit();
+  };
+  if (chunks) load(chunks - 1);
   zero_rows(a, seq, p.dv + (long)h * a.dv + c0, (long)a.hv * a.dv, cols);
   float s[NS][4];
   const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + c0;
@@ -439,42 +492,35 @@ __global__ void __launch_bounds__(kScanThreads) delta_back_kernel(const BackArgs
       const int i = sm + (lane >> 2) + (e >> 1) * 8, j = sn + t * 8 + (lane & 3) * 2 + (e & 1);
       s[t][e] = p.dfinal && i < a.dk && j < cols ? p.dfinal[sbase + (long)i * a.dv + j] : 0.f;
     }
-  for (long c = (to - from + kC - 1) / kC - 1; c >= 0; c--) {
-    const long start = from + c * kC, slot = from / kC + seq + c;
+  const int mt = warp & 3, m0 = mt * 16, n0 = (warp >> 2) * 16, i0 = m0 + (lane >> 2);  // 16 x 16 of a 64 x 64 tile
+  for (long c = chunks - 1; c >= 0; c--) {
+    const long start = from + c * kC, slot = slot0 + c;
     const int len = (int)(to - start < kC ? to - start : kC);
-    const __nv_bfloat16* mats = p.mats + (slot * a.hv + h) * kMats;
-    copy_tile<DK, LD, kScanThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
-    copy_tile<DK, LD, kScanThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
-    copy_tile<64, kLd, kScanThreads>(sh.o, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
-#pragma unroll
-    for (int m = 0; m < 4; m++) copy_tile<64, kLd, kScanThreads>(sh.mats[m], mats + m * kC * kC, kC, kC, kC, true);
-    cp_commit();
-    chunk_decay(a, sh.d, start, len, h);
+    const auto& in = sh.in[c & 1];
 #pragma unroll
     for (int t = 0; t < NS; t++)
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int i = sm + (lane >> 2) + half * 8, j = sn + t * 8 + (lane & 3) * 2;
-        put2<kLd>(sh.s[0], sh.s[1], i, j, s[t][half * 2], s[t][half * 2 + 1]);
-        if (i < a.dk)
-          *reinterpret_cast<float2*>(p.ds + ((slot * a.hv + h) * a.dk + i) * a.dvp + c0 + j) =
-              make_float2(s[t][half * 2], s[t][half * 2 + 1]);
-      }
+      for (int half = 0; half < 2; half++)
+        put2<kLd>(sh.s[0], sh.s[1], sm + (lane >> 2) + half * 8, sn + t * 8 + (lane & 3) * 2, s[t][half * 2],
+                  s[t][half * 2 + 1]);
     cp_wait<0>();
     __syncthreads();
-    const int m0 = (warp & 3) * 16, n0 = (warp >> 2) * 32, i0 = m0 + (lane >> 2);
-    {  // diag(beta) dU = beta (F K dS' + scale P^T dO), P^T upper triangular
-      float x[4][4], y[4][4];
+    if (c > 0) load(c - 1);
+#pragma unroll
+    for (int part = 0; part < 2; part++)
+      tile_out<kScanThreads>(p.ds + state_at(a, slot, h, slice) + part * a.dk * 64, sh.s[part], a.dk);
+    {  // diag(beta) dU = beta (F K dS' + scale P^T dO)
+      float x[2][4], y[2][4];
       zero(x);
       zero(y);
-      product<false, LD, true, kLd>(x, sh.k, nullptr, sh.s[0], sh.s[1], m0, n0, 0, DK);
-      product<true, kLd, true, kLd>(y, sh.mats[2], sh.mats[3], sh.o, nullptr, m0, n0, m0, kC);
+      product<false, LD, true, kLd>(x, in.k, nullptr, sh.s[0], sh.s[1], m0, n0, 0, DK);
+      tri_product<true, true, kLd>(y, in.m.p[0], in.m.p[1], in.o, nullptr, mt, n0);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = i0 + half * 8;
-        const float b = sh.d.beta[i], f = sh.d.until[i];
+        const float b = in.m.beta[i], f = in.m.until[i];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
+        for (int t = 0; t < 2; t++) {
           float z[2];
 #pragma unroll
           for (int e = 0; e < 2; e++)
@@ -486,42 +532,49 @@ __global__ void __launch_bounds__(kScanThreads) delta_back_kernel(const BackArgs
     // scale E dO, the operand of Q's part
     for (int i = tid; i < kC * 32; i += kScanThreads) {
       const int r = i >> 5, cc = (i & 31) * 2;
-      const float f = a.scale * sh.d.since[r];
-      const float x = __bfloat162float(sh.o[r * kLd + cc]), y = __bfloat162float(sh.o[r * kLd + cc + 1]);
-      put2<kLd>(sh.w[0], sh.w[1], r, cc, f == 0.f ? 0.f : f * x, f == 0.f ? 0.f : f * y);
+      const float f = a.scale * in.m.since[r];
+      const __nv_bfloat162 o = *reinterpret_cast<const __nv_bfloat162*>(in.o + r * kLd + cc);
+      put2<kLd>(sh.w[0], sh.w[1], r, cc, f == 0.f ? 0.f : f * __low2float(o), f == 0.f ? 0.f : f * __high2float(o));
     }
     __syncthreads();
     {  // dR = X^T (beta dU)
-      float x[4][4];
+      float x[2][4];
       zero(x);
-      product<true, kLd, true, kLd>(x, sh.mats[0], sh.mats[1], sh.u[0], sh.u[1], m0, n0, m0, kC);
+      tri_product<true, true, kLd>(x, in.m.x[0], in.m.x[1], sh.u[0], sh.u[1], mt, n0);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = i0 + half * 8;
-        const float f = -sh.d.since[i];
+        const float f = -in.m.since[i];
         __nv_bfloat16* dv = p.dv + (start + i) * a.hv * a.dv + (long)h * a.dv + c0;
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
+        for (int t = 0; t < 2; t++) {
           const int j = n0 + t * 8 + (lane & 3) * 2;
           const float y0 = x[t][half * 2], y1 = x[t][half * 2 + 1];
-          *reinterpret_cast<float2*>(p.dr + ((slot * a.hv + h) * kC + i) * a.dvp + c0 + j) = make_float2(y0, y1);
+          uint32_t hi, lo;
+          split2(y0, y1, hi, lo);
+          __nv_bfloat16* to_r = p.dr + rows_at(a, slot, h, slice) + i * 64 + j;
+          *reinterpret_cast<uint32_t*>(to_r) = hi;
+          *reinterpret_cast<uint32_t*>(to_r + kC * 64) = lo;
           if (i < len) {
-            if (j < cols) dv[j] = __float2bfloat16_rn(y0);
-            if (j + 1 < cols) dv[j + 1] = __float2bfloat16_rn(y1);
+            if (a.dv % 2 == 0 && j + 1 < cols) {
+              *reinterpret_cast<uint32_t*>(dv + j) = hi;
+            } else {
+              if (j < cols) dv[j] = __float2bfloat16_rn(y0);
+              if (j + 1 < cols) dv[j + 1] = __float2bfloat16_rn(y1);
+            }
           }
           put2<kLd>(sh.r[0], sh.r[1], i, j, f == 0.f ? 0.f : f * y0, f == 0.f ? 0.f : f * y1);
         }
       }
     }
-    __syncthreads();
-    const float keep = sh.d.since[kC - 1];
+    const float keep = in.m.since[kC - 1];
 #pragma unroll
     for (int t = 0; t < NS; t++)
 #pragma unroll
       for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-    product<true, LD, true, kLd>(s, sh.q, nullptr, sh.w[0], sh.w[1], sm, sn, 0, kC);
-    product<true, LD, true, kLd>(s, sh.k, nullptr, sh.r[0], sh.r[1], sm, sn, 0, kC);
+    product<true, LD, true, kLd>(s, in.q, nullptr, sh.w[0], sh.w[1], sm, sn, 0, kC);
     __syncthreads();
+    product<true, LD, true, kLd>(s, in.k, nullptr, sh.r[0], sh.r[1], sm, sn, 0, kC);
   }
   if (!p.dstate) return;
 #pragma unroll
@@ -539,139 +592,167 @@ struct GradArgs {
   const __nv_bfloat16* dout;
   long ldo, hso;
   bool vec_o;
-  const float *kept, *y, *ds, *dr;
+  const __nv_bfloat16 *kept, *y, *ds, *dr;
   __nv_bfloat16 *dq, *dk;  // [n][hk][dk]
   float *dg, *dbeta;       // [n][hv]
 };
 template <int DK>
 struct GradShared {
-  __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], o[kC * kLd];
-  __nv_bfloat16 s[2][DK * kLd], ds[2][DK * kLd];
-  __nv_bfloat16 y[2][kC * kLd], r[2][kC * kLd];
-  __nv_bfloat16 p[2][kC * kLd], m[2][kC * kLd];  // scale dO U^T * D, -M
-  float row[2][kC], col[4][kC], krow[2][kC], sum[8];
+  __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)];
+  __nv_bfloat16 o[2][kC * kLd], r[2][2][kC * kLd];  // by turns: the next step's are on their way
+  __nv_bfloat16 s[2][DK * kLd], ds[2][DK * kLd], y[2][kC * kLd];
+  __nv_bfloat16 p[2][kC * kLd], m[2][kC * kLd];     // scale dO U^T * D, -M
+  float row[4][kC], col[4][kC], krow[4][kC], sum[16];
   Decay d;
 };
-// rows x 64 of f32 values as two bf16 parts
-template <int THREADS>
-__device__ __forceinline__ void split_tile(__nv_bfloat16* hi, __nv_bfloat16* lo, const float* src, long stride, int rows,
-                                           int all) {
-  for (int i = threadIdx.x; i < all * 16; i += THREADS) {
-    const int r = i >> 4, c = (i & 15) * 4;
-    const float4 f = r < rows ? *reinterpret_cast<const float4*>(src + (long)r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-    put2<kLd>(hi, lo, r, c, f.x, f.y);
-    put2<kLd>(hi, lo, r, c + 2, f.z, f.w);
-  }
-}
-// A block per chunk and key head: its value heads one after the other, so that what they add to dq and dk stays in
-// registers and is added in their order.
+// A block per chunk and key head, 16 warps: its value heads one after the other, so that what they add to dq and dk stays in
+// registers and is added in their order; of each, 64 columns of v after the other (a step). A step's loads are under
+// way during the one before it.
 template <int DK>
 __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs p) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
   GradShared<DK>& sh = *reinterpret_cast<GradShared<DK>*>(mem);
-  constexpr int LD = DK + 8, NK = DK / 16;  // n-tiles of a warp's half of dk
+  constexpr int LD = DK + 8, NK = DK / 32;  // n-tiles of a warp's quarter of dk
   const DeltaArgs& a = p.d;
   const long slot = blockIdx.x;
   const int kh = blockIdx.y, group = a.hv / a.hk, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   long start;
   const int len = slot_chunk(a, slot, start);
   if (len == 0) return;
+  const int slices = a.dvp / 64, steps = group * slices;
+  auto load_a = [&](int t) {  // S, dO, dR
+    const int h = kh * group + t / slices, slice = t % slices, c0 = slice * 64;
+    const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
+    copy_tile<64, kLd, kScanThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
+#pragma unroll
+    for (int part = 0; part < 2; part++) {
+      tile_in<kScanThreads>(sh.s[part], p.kept + state_at(a, slot, h, slice) + part * a.dk * 64, a.dk);
+      tile_in<kScanThreads>(sh.r[t & 1][part], p.dr + rows_at(a, slot, h, slice) + part * kC * 64, kC);
+    }
+    cp_commit();
+  };
+  auto load_b = [&](int t) {  // dS', Y
+    const int h = kh * group + t / slices, slice = t % slices;
+#pragma unroll
+    for (int part = 0; part < 2; part++) {
+      tile_in<kScanThreads>(sh.ds[part], p.ds + state_at(a, slot, h, slice) + part * a.dk * 64, a.dk);
+      tile_in<kScanThreads>(sh.y[part], p.y + rows_at(a, slot, h, slice) + part * kC * 64, kC);
+    }
+    cp_commit();
+  };
   copy_tile<DK, LD, kScanThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
   copy_tile<DK, LD, kScanThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
-  cp_commit();
+  load_a(0);
+  load_b(0);
+  // the states' rows behind dk stay zero
+  for (int i = a.dk * kLd + tid; i < DK * kLd; i += kScanThreads)
+    sh.s[0][i] = sh.s[1][i] = sh.ds[0][i] = sh.ds[1][i] = __float2bfloat16_rn(0.f);
   const int wr = warp & 3, wc = warp >> 2, m0 = wr * 16, i0 = m0 + (lane >> 2);
-  const int n0 = wc * 32, d0 = wc * (DK / 2);  // this warp's columns of a 64 x 64 tile, of a 64 x dk tile
-  float dq[NK][4], dk[NK][4];
+  const int n0 = wc * 16, d0 = wc * (DK / 4);  // this warp's columns of a 64 x 64 tile, of a 64 x dk tile
+  float dq[NK][4], dk[NK][4], oy[2][4], ry[2][4], qrow[2], krow[2], inner = 0.f;
   zero(dq);
   zero(dk);
-  for (int e = 0; e < group; e++) {
-    const int h = kh * group + e;
-    const long at = slot * a.hv + h;
-    chunk_decay(a, sh.d, start, len, h);
-    float oy[4][4], ry[4][4], es[NK][4], ty[NK][4];
-    zero(oy);
-    zero(ry);
-    zero(ty);
-    float inner = 0.f;  // <S, dS'>
-    float qrow[2] = {0.f, 0.f};
-    float rs[NK][4];
-    zero(es);
-    zero(rs);
-    for (int c0 = 0; c0 < a.dv; c0 += 64) {
-      const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-      __syncthreads();
-      copy_tile<64, kLd, kScanThreads>(sh.o, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
-      cp_commit();
-      const float *s = p.kept + at * a.dk * a.dvp + c0, *ds = p.ds + at * a.dk * a.dvp + c0;
-      for (int i = tid; i < DK * 16; i += kScanThreads) {
-        const int r = i >> 4, c = (i & 15) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        if (r < a.dk) {
-          x = *reinterpret_cast<const float4*>(s + (long)r * a.dvp + c);
-          y = *reinterpret_cast<const float4*>(ds + (long)r * a.dvp + c);
-        }
-        inner += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
-        put2<kLd>(sh.s[0], sh.s[1], r, c, x.x, x.y);
-        put2<kLd>(sh.s[0], sh.s[1], r, c + 2, x.z, x.w);
-        put2<kLd>(sh.ds[0], sh.ds[1], r, c, y.x, y.y);
-        put2<kLd>(sh.ds[0], sh.ds[1], r, c + 2, y.z, y.w);
-      }
-      split_tile<kScanThreads>(sh.y[0], sh.y[1], p.y + at * kC * a.dvp + c0, a.dvp, kC, kC);
-      split_tile<kScanThreads>(sh.r[0], sh.r[1], p.dr + at * kC * a.dvp + c0, a.dvp, kC, kC);
-      cp_wait<0>();
-      __syncthreads();
-      product<false, kLd, false, kLd>(oy, sh.o, nullptr, sh.y[0], sh.y[1], m0, n0, 0, 64);
-      product<false, kLd, false, kLd>(ry, sh.r[0], sh.r[1], sh.y[0], sh.y[1], m0, n0, 0, 64);
-      product<false, kLd, false, kLd>(es, sh.o, nullptr, sh.s[0], sh.s[1], m0, d0, 0, 64);
-      product<false, kLd, false, kLd>(rs, sh.r[0], sh.r[1], sh.s[0], sh.s[1], m0, d0, 0, 64);
-      product<false, kLd, false, kLd>(ty, sh.y[0], sh.y[1], sh.ds[0], sh.ds[1], m0, d0, 0, 64);
+  for (int t = 0; t < steps; t++) {
+    const int h = kh * group + t / slices;
+    const __nv_bfloat16* o = sh.o[t & 1];
+    const __nv_bfloat16 *r = sh.r[t & 1][0], *rl = sh.r[t & 1][1];
+    if (t % slices == 0) {
+      chunk_decay(a, sh.d, start, len, h);
+      zero(oy);
+      zero(ry);
+      inner = qrow[0] = qrow[1] = krow[0] = krow[1] = 0.f;
     }
-    // E dO S^T, -E dR S^T and F U dS'^T into dq and dk; e_i and K . (dS' Y) by row
-    float krow[2] = {0.f, 0.f};
+    cp_wait<1>();
+    __syncthreads();
+    float x[NK][4];
+    zero(x);
+    product<false, kLd, false, kLd>(x, o, nullptr, sh.s[0], sh.s[1], m0, d0, 0, 64);
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
+    for (int half = 0; half < 2; half++) {  // scale E dO S^T, and what it adds to e_i
       const int i = i0 + half * 8;
-      const float f = sh.d.since[i], t = sh.d.until[i], b = sh.d.beta[i];
+      const float f = sh.d.since[i] * a.scale;
 #pragma unroll
-      for (int n = 0; n < NK; n++)
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-          const int j = d0 + n * 8 + (lane & 3) * 2 + c, x = half * 2 + c;
-          const float eq = f == 0.f ? 0.f : a.scale * f * es[n][x], ek = f == 0.f ? 0.f : f * rs[n][x];
-          const float tk = t == 0.f ? 0.f : t * ty[n][x];
-          const float kv = __bfloat162float(sh.k[i * LD + j]);
-          qrow[half] = __fmaf_rn(__bfloat162float(sh.q[i * LD + j]), eq, qrow[half]);
-          qrow[half] = __fmaf_rn(kv, -ek, qrow[half]);
-          krow[half] = __fmaf_rn(kv, tk, krow[half]);
-          dq[n][x] += eq;
-          dk[n][x] += b * tk - ek;
-        }
+      for (int n = 0; n < NK; n++) {
+        const __nv_bfloat162 q = *reinterpret_cast<const __nv_bfloat162*>(sh.q + i * LD + d0 + n * 8 + (lane & 3) * 2);
+        const float v0 = f == 0.f ? 0.f : f * x[n][half * 2], v1 = f == 0.f ? 0.f : f * x[n][half * 2 + 1];
+        qrow[half] = __fmaf_rn(__low2float(q), v0, __fmaf_rn(__high2float(q), v1, qrow[half]));
+        dq[n][half * 2] += v0;
+        dq[n][half * 2 + 1] += v1;
+      }
     }
+    zero(x);
+    product<false, kLd, false, kLd>(x, r, rl, sh.s[0], sh.s[1], m0, d0, 0, 64);
+#pragma unroll
+    for (int half = 0; half < 2; half++) {  // -E dR S^T
+      const int i = i0 + half * 8;
+      const float f = -sh.d.since[i];
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        const __nv_bfloat162 k = *reinterpret_cast<const __nv_bfloat162*>(sh.k + i * LD + d0 + n * 8 + (lane & 3) * 2);
+        const float v0 = f == 0.f ? 0.f : f * x[n][half * 2], v1 = f == 0.f ? 0.f : f * x[n][half * 2 + 1];
+        qrow[half] = __fmaf_rn(__low2float(k), v0, __fmaf_rn(__high2float(k), v1, qrow[half]));
+        dk[n][half * 2] += v0;
+        dk[n][half * 2 + 1] += v1;
+      }
+    }
+    cp_wait<0>();
+    __syncthreads();
+    for (int i = tid; i < DK * 32; i += kScanThreads) {  // <S, dS'>
+      const int at = (i >> 5) * kLd + (i & 31) * 2;
+      auto two = [&](const __nv_bfloat16* hi, const __nv_bfloat16* lo) {
+        const __nv_bfloat162 h2 = *reinterpret_cast<const __nv_bfloat162*>(hi + at), l2 = *reinterpret_cast<const __nv_bfloat162*>(lo + at);
+        return make_float2(__low2float(h2) + __low2float(l2), __high2float(h2) + __high2float(l2));
+      };
+      const float2 u = two(sh.s[0], sh.s[1]), v = two(sh.ds[0], sh.ds[1]);
+      inner = __fmaf_rn(u.x, v.x, __fmaf_rn(u.y, v.y, inner));
+    }
+    __syncthreads();
+    if (t + 1 < steps) load_a(t + 1);
+    zero(x);
+    product<false, kLd, false, kLd>(x, sh.y[0], sh.y[1], sh.ds[0], sh.ds[1], m0, d0, 0, 64);
+#pragma unroll
+    for (int half = 0; half < 2; half++) {  // F U dS'^T, and K_i . (dS' Y_i)
+      const int i = i0 + half * 8;
+      const float f = sh.d.until[i], b = sh.d.beta[i];
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        const __nv_bfloat162 k = *reinterpret_cast<const __nv_bfloat162*>(sh.k + i * LD + d0 + n * 8 + (lane & 3) * 2);
+        const float v0 = f == 0.f ? 0.f : f * x[n][half * 2], v1 = f == 0.f ? 0.f : f * x[n][half * 2 + 1];
+        krow[half] = __fmaf_rn(__low2float(k), v0, __fmaf_rn(__high2float(k), v1, krow[half]));
+        dk[n][half * 2] = __fmaf_rn(b, v0, dk[n][half * 2]);
+        dk[n][half * 2 + 1] = __fmaf_rn(b, v1, dk[n][half * 2 + 1]);
+      }
+    }
+    product<false, kLd, false, kLd>(oy, o, nullptr, sh.y[0], sh.y[1], m0, n0, 0, 64);
+    product<false, kLd, false, kLd>(ry, r, rl, sh.y[0], sh.y[1], m0, n0, 0, 64);
+    __syncthreads();
+    if (t + 1 < steps) load_b(t + 1);
+    if ((t + 1) % slices) continue;
     // K K^T and Q K^T where this warp has dR Y^T and dO Y^T
-    float kk[4][4], qk[4][4], col[4][2];
+    float kk[2][4], qk[2][4];
     zero(kk);
     zero(qk);
     product<false, LD, false, LD>(kk, sh.k, nullptr, sh.k, nullptr, m0, n0, 0, DK);
     product<false, LD, false, LD>(qk, sh.q, nullptr, sh.k, nullptr, m0, n0, 0, DK);
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      col[t][0] = col[t][1] = 0.f;
+    for (int n = 0; n < 2; n++) {
+      float col[2] = {0.f, 0.f};
 #pragma unroll
       for (int half = 0; half < 2; half++) {
-        const int i = i0 + half * 8, j = n0 + t * 8 + (lane & 3) * 2;
+        const int i = i0 + half * 8, j = n0 + n * 8 + (lane & 3) * 2;
         float po[2], mm[2];
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          const int x = half * 2 + c;
+          const int e = half * 2 + c;
           const bool low = j + c <= i, strict = j + c < i;
           const float f = low ? decay(sh.d, i, j + c) : 0.f, b = sh.d.beta[j + c];
-          const float o = low ? a.scale * f * oy[t][x] : 0.f, r = strict ? f * ry[t][x] : 0.f;
-          po[c] = b * o;
-          mm[c] = -b * r;
-          qrow[half] += (low ? qk[t][x] * po[c] : 0.f) + (strict ? kk[t][x] * mm[c] : 0.f);
-          col[t][c] += (low ? qk[t][x] * o : 0.f) - (strict ? kk[t][x] * r : 0.f);
+          const float ov = low ? a.scale * f * oy[n][e] : 0.f, rv = strict ? f * ry[n][e] : 0.f;
+          po[c] = b * ov;
+          mm[c] = -b * rv;
+          qrow[half] += (low ? qk[n][e] * po[c] : 0.f) + (strict ? kk[n][e] * mm[c] : 0.f);
+          col[c] += (low ? qk[n][e] * ov : 0.f) - (strict ? kk[n][e] * rv : 0.f);
         }
         put2<kLd>(sh.p[0], sh.p[1], i, j, po[0], po[1]);
         put2<kLd>(sh.m[0], sh.m[1], i, j, mm[0], mm[1]);
@@ -679,18 +760,18 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
 #pragma unroll
       for (int c = 0; c < 2; c++)
 #pragma unroll
-        for (int o = 4; o < 32; o *= 2) col[t][c] += __shfl_xor_sync(0xffffffffu, col[t][c], o);
+        for (int w = 4; w < 32; w *= 2) col[c] += __shfl_xor_sync(0xffffffffu, col[c], w);
       if (lane < 4) {
-        sh.col[wr][n0 + t * 8 + lane * 2] = col[t][0];
-        sh.col[wr][n0 + t * 8 + lane * 2 + 1] = col[t][1];
+        sh.col[wr][n0 + n * 8 + lane * 2] = col[0];
+        sh.col[wr][n0 + n * 8 + lane * 2 + 1] = col[1];
       }
     }
 #pragma unroll
     for (int half = 0; half < 2; half++) {
 #pragma unroll
-      for (int o = 1; o < 4; o *= 2) {
-        qrow[half] += __shfl_xor_sync(0xffffffffu, qrow[half], o);
-        krow[half] += __shfl_xor_sync(0xffffffffu, krow[half], o);
+      for (int w = 1; w < 4; w *= 2) {
+        qrow[half] += __shfl_xor_sync(0xffffffffu, qrow[half], w);
+        krow[half] += __shfl_xor_sync(0xffffffffu, krow[half], w);
       }
       if ((lane & 3) == 0) {
         sh.row[wc][i0 + half * 8] = qrow[half];
@@ -698,7 +779,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
       }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, o);
+    for (int w = 16; w; w >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, w);
     if (lane == 0) sh.sum[warp] = inner;
     __syncthreads();
     product<false, kLd, true, LD>(dq, sh.p[0], sh.p[1], sh.k, nullptr, m0, d0, 0, m0 + 16);
@@ -710,40 +791,38 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
       float end = 0.f, sum[2];
       int era[2];
 #pragma unroll
-      for (int w = 0; w < 8; w++) end += sh.sum[w];
+      for (int w = 0; w < 16; w++) end += sh.sum[w];
       end = keep == 0.f ? 0.f : keep * end;
       float tail = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = half * 32 + lane;
-        const float kd = sh.krow[0][i] + sh.krow[1][i];
-        float c = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) c += sh.col[w][i];
+        const float kd = (sh.krow[0][i] + sh.krow[1][i]) + (sh.krow[2][i] + sh.krow[3][i]);
+        const float c = (sh.col[0][i] + sh.col[1][i]) + (sh.col[2][i] + sh.col[3][i]);
         if (i < len) p.dbeta[(start + i) * a.hv + h] = kd + c;
         tail += sh.d.beta[i] * kd;  // F_i u_i . (K_i dS')
-        sum[half] = sh.row[0][i] + sh.row[1][i] - sh.d.beta[i] * (kd + c);
+        sum[half] = (sh.row[0][i] + sh.row[1][i]) + (sh.row[2][i] + sh.row[3][i]) - sh.d.beta[i] * (kd + c);
         era[half] = sh.d.era[i];
       }
 #pragma unroll
-      for (int o = 16; o; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
+      for (int w = 16; w; w >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, w);
       const int last = __shfl_sync(0xffffffffu, era[1], 31);
       float behind = end + tail;  // of the tokens behind this half, as far as they are of era `last`
       int behind_era = last;
 #pragma unroll
       for (int half = 1; half >= 0; half--) {
-        float x = sum[half];
+        float v = sum[half];
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-          const float up = __shfl_down_sync(0xffffffffu, x, o);
-          const int ue = __shfl_down_sync(0xffffffffu, era[half], o);
-          if (lane + o < 32 && ue == era[half]) x += up;
+        for (int w = 1; w < 32; w *= 2) {
+          const float up = __shfl_down_sync(0xffffffffu, v, w);
+          const int ue = __shfl_down_sync(0xffffffffu, era[half], w);
+          if (lane + w < 32 && ue == era[half]) v += up;
         }
-        if (era[half] == behind_era) x += behind;
+        if (era[half] == behind_era) v += behind;
         const int i = half * 32 + lane;
         const bool reset = i < len && a.g[(start + i) * a.hv + h] < -104.f;
-        if (i < len) p.dg[(start + i) * a.hv + h] = reset ? 0.f : x;
-        behind = __shfl_sync(0xffffffffu, x, 0);
+        if (i < len) p.dg[(start + i) * a.hv + h] = reset ? 0.f : v;
+        behind = __shfl_sync(0xffffffffu, v, 0);
         behind_era = __shfl_sync(0xffffffffu, era[half], 0);
       }
     }
@@ -755,15 +834,20 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
     if (i >= len) continue;
     const long to = ((start + i) * a.hk + kh) * a.dk;
 #pragma unroll
-    for (int n = 0; n < NK; n++)
+    for (int n = 0; n < NK; n++) {
+      const int j = d0 + n * 8 + (lane & 3) * 2;
+      if (a.dk % 2 == 0 && j + 1 < a.dk) {
+        *reinterpret_cast<__nv_bfloat162*>(p.dq + to + j) = __floats2bfloat162_rn(dq[n][half * 2], dq[n][half * 2 + 1]);
+        *reinterpret_cast<__nv_bfloat162*>(p.dk + to + j) = __floats2bfloat162_rn(dk[n][half * 2], dk[n][half * 2 + 1]);
+      } else {
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
-        const int j = d0 + n * 8 + (lane & 3) * 2 + c;
-        if (j < a.dk) {
-          p.dq[to + j] = __float2bfloat16_rn(dq[n][half * 2 + c]);
-          p.dk[to + j] = __float2bfloat16_rn(dk[n][half * 2 + c]);
-        }
+        for (int c = 0; c < 2; c++)
+          if (j + c < a.dk) {
+            p.dq[to + j + c] = __float2bfloat16_rn(dq[n][half * 2 + c]);
+            p.dk[to + j + c] = __float2bfloat16_rn(dk[n][half * 2 + c]);
+          }
       }
+    }
   }
 }
 // Rows that no sequence holds: their gradients are zero.
@@ -829,7 +913,7 @@ static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 static size_t heads_slots(const pl_delta_shape* s) {
   return (size_t)slot_count((long)s->tokens, (long)s->sequences) * s->heads_v;
 }
-static size_t mats_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * kMats * 2); }
+static size_t mats_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * sizeof(Mats)); }
 static size_t states_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * s->dk * round_up((long)s->dv, 64) * 4); }
 static size_t rows_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * kC * round_up((long)s->dv, 64) * 4); }
 
@@ -841,7 +925,7 @@ static int launch_wide(void (*kernel)(A), dim3 grid, int threads, size_t smem, c
   count_launch();
   return PL_OK;
 }
-static int prep(const DeltaArgs& a, __nv_bfloat16* mats, cudaStream_t st) {
+static int prep(const DeltaArgs& a, Mats* mats, cudaStream_t st) {
   const dim3 grid((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
   const bool wide = a.dk > 64;
   const size_t smem = wide ? sizeof(PrepShared<128>) : sizeof(PrepShared<64>);
@@ -896,13 +980,13 @@ int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const vo
   cudaStream_t st = (cudaStream_t)stream;
   const DeltaArgs a = delta_args(s, q, k, v, g, beta, offsets);
   if (s->tokens) {
-    rc = prep(a, (__nv_bfloat16*)ws, st);
+    rc = prep(a, (Mats*)ws, st);
     if (rc) return rc;
   }
-  ScanArgs p = {a, (const __nv_bfloat16*)ws, state, (__nv_bfloat16*)o, final_state, nullptr, nullptr};
+  ScanArgs p = {a, (const Mats*)ws, state, (__nv_bfloat16*)o, final_state, nullptr, nullptr};
   if (saved) {
-    p.kept = (float*)saved;
-    p.y = (float*)((char*)saved + states_bytes(s));
+    p.kept = (__nv_bfloat16*)saved;
+    p.y = (__nv_bfloat16*)((char*)saved + states_bytes(s));
   }
   const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
   return a.dk > 64 ? launch_wide(delta_scan_kernel<128>, grid, kScanThreads, sizeof(ScanShared<128>), st, p)
@@ -932,20 +1016,20 @@ int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token
   cudaStream_t st = (cudaStream_t)stream;
   const DeltaArgs a = delta_args(s, q, k, v, g, beta, offsets);
   char* w = (char*)ws;
-  float *ds = (float*)(w + mats_bytes(s)), *dr = (float*)(w + mats_bytes(s) + states_bytes(s));
+  __nv_bfloat16 *ds = (__nv_bfloat16*)(w + mats_bytes(s)), *dr = (__nv_bfloat16*)(w + mats_bytes(s) + states_bytes(s));
   const bool vec_o = rows16(dout, do_token, do_head);
   if (s->tokens) {
-    rc = prep(a, (__nv_bfloat16*)ws, st);
+    rc = prep(a, (Mats*)ws, st);
     if (rc) return rc;
   }
-  const BackArgs b = {a, (const __nv_bfloat16*)ws, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, dfinal,
+  const BackArgs b = {a, (const Mats*)ws, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, dfinal,
                       (__nv_bfloat16*)dv, dstate, ds, dr};
   const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
   rc = a.dk > 64 ? launch_wide(delta_back_kernel<128>, grid, kScanThreads, sizeof(BackShared<128>), st, b)
                  : launch_wide(delta_back_kernel<64>, grid, kScanThreads, sizeof(BackShared<64>), st, b);
   if (rc || s->tokens == 0) return rc;
-  const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, (const float*)saved,
-                      (const float*)((const char*)saved + states_bytes(s)), ds, dr, (__nv_bfloat16*)dq, (__nv_bfloat16*)dk,
+  const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, (const __nv_bfloat16*)saved,
+                      (const __nv_bfloat16*)((const char*)saved + states_bytes(s)), ds, dr, (__nv_bfloat16*)dq, (__nv_bfloat16*)dk,
                       dg, dbeta};
   const dim3 chunks((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
   rc = a.dk > 64 ? launch_wide(delta_grad_kernel<128>, chunks, kScanThreads, sizeof(GradShared<128>), st, p)

@@ -85,6 +85,22 @@ __device__ __forceinline__ void copy_tile(__nv_bfloat16* dst, const __nv_bfloat1
   }
 }
 
+// n bytes (a multiple of 16) as they lie.
+template <int THREADS>
+__device__ __forceinline__ void copy_flat(void* dst, const void* src, int n) {
+  for (int i = threadIdx.x * 16; i < n; i += THREADS * 16) cp16((char*)dst + i, (const char*)src + i, 16);
+}
+// `rows` rows of 64 values (128 bytes, one behind the other in memory) into, or out of, a tile of stride kLd.
+template <int THREADS>
+__device__ __forceinline__ void tile_in(__nv_bfloat16* tile, const __nv_bfloat16* src, int rows) {
+  for (int i = threadIdx.x; i < rows * 8; i += THREADS) cp16(tile + (i >> 3) * kLd + (i & 7) * 8, src + i * 8, 16);
+}
+template <int THREADS>
+__device__ __forceinline__ void tile_out(__nv_bfloat16* dst, const __nv_bfloat16* tile, int rows) {
+  for (int i = threadIdx.x; i < rows * 8; i += THREADS)
+    *reinterpret_cast<uint4*>(dst + i * 8) = *reinterpret_cast<const uint4*>(tile + (i >> 3) * kLd + (i & 7) * 8);
+}
+
 // ---------------------------------------------------------------------------------------------- products
 // m16n8k16 products of one warp on bf16 tiles in shared memory. An operand lies either along k (rows of m or n) or
 // across it (rows of k); ldmatrix transposes the latter.
@@ -146,6 +162,51 @@ __device__ __forceinline__ void product(float (&acc)[NT][4], const __nv_bfloat16
       }
       if (blo) {
         frag_b<B_ACROSS, LDB>(y, blo, k, n + t * 8);
+        mma(acc[t], x, y[0], y[1]);
+        mma(acc[t + 1], x, y[2], y[3]);
+      }
+    }
+  }
+}
+
+// A lower triangular 64 x 64 matrix as the ten 16 x 16 blocks on and below its diagonal, block (r, c) the r (r + 1) / 2 + c-th;
+// in a block, row i's two 16-byte pieces change places where i & 4, so that ldmatrix's eight rows are in eight places.
+constexpr int kTri = 10 * 256;
+__host__ __device__ __forceinline__ int tri_at(int i, int j) {
+  const int r = i >> 4, c = j >> 4, y = i & 15, x = j & 15;
+  return (r * (r + 1) / 2 + c) * 256 + y * 16 + (((x >> 3) ^ ((y >> 2) & 1)) << 3) + (x & 7);
+}
+// The fragment of block (r, c), or of its transpose.
+template <bool ACROSS>
+__device__ __forceinline__ void frag_tri(uint32_t (&x)[4], const __nv_bfloat16* t, int r, int c) {
+  const int lane = threadIdx.x & 31;
+  const __nv_bfloat16* b = t + (r * (r + 1) / 2 + c) * 256;
+  const int y = ACROSS ? (lane & 7) + ((lane >> 4) & 1) * 8 : lane & 15, p = ACROSS ? (lane >> 3) & 1 : lane >> 4;
+  const uint32_t at = smem_u32(b + y * 16 + ((p ^ ((y >> 2) & 1)) << 3));
+  if constexpr (ACROSS) ldsm4t(x, at);
+  else ldsm4(x, at);
+}
+// acc (16 x 8 NT at row block mt, column n) += T B or (ACROSS) T^T B, T triangular in parts hi, lo (lo = nullptr: hi alone).
+template <bool ACROSS, bool B_ACROSS, int LDB, int NT>
+__device__ __forceinline__ void tri_product(float (&acc)[NT][4], const __nv_bfloat16* hi, const __nv_bfloat16* lo,
+                                            const __nv_bfloat16* b, const __nv_bfloat16* blo, int mt, int n) {
+  const int k0 = ACROSS ? mt : 0, k1 = ACROSS ? 4 : mt + 1;
+  for (int k = k0; k < k1; k++) {
+    uint32_t x[4], xl[4];
+    frag_tri<ACROSS>(x, hi, ACROSS ? k : mt, ACROSS ? mt : k);
+    if (lo) frag_tri<ACROSS>(xl, lo, ACROSS ? k : mt, ACROSS ? mt : k);
+#pragma unroll
+    for (int t = 0; t < NT; t += 2) {
+      uint32_t y[4];
+      frag_b<B_ACROSS, LDB>(y, b, k * 16, n + t * 8);
+      mma(acc[t], x, y[0], y[1]);
+      mma(acc[t + 1], x, y[2], y[3]);
+      if (lo) {
+        mma(acc[t], xl, y[0], y[1]);
+        mma(acc[t + 1], xl, y[2], y[3]);
+      }
+      if (blo) {
+        frag_b<B_ACROSS, LDB>(y, blo, k * 16, n + t * 8);
         mma(acc[t], x, y[0], y[1]);
         mma(acc[t + 1], x, y[2], y[3]);
       }
