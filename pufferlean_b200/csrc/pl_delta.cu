@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArg
   float kk[8][4], qk[8][4];  // rows 16 warp.. of K K^T and Q K^T
   zero(kk);
   zero(qk);
-  product<false, LD, false, LD>(kk, sh.k, nullptr, sh.k, nullptr, warp * 16, 0, 0, DK);
-  product<false, LD, false, LD>(qk, sh.q, nullptr, sh.k, nullptr, warp * 16, 0, 0, DK);
+  product<false, LD, 0, false, LD, 0, DK / 16>(kk, sh.k, sh.k, warp * 16, 0);
+  product<false, LD, 0, false, LD, 0, DK / 16>(qk, sh.q, sh.k, warp * 16, 0);
   for (int e = 0; e < group; e++) {
     const int h = kh * group + e;
     Mats& out = mats[slot * a.hv + h];
@@ -262,6 +262,7 @@ __device__ __forceinline__ long rows_at(const DeltaArgs& a, long slot, int h, in
 }
 
 constexpr int kScanThreads = 512;
+constexpr int kRows = kC * kLd;  // a 64 x 64 tile: the distance of its second part
 struct ScanArgs {
   DeltaArgs d;
   const Mats* mats;
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_scan_kernel(const ScanArgs
     const int m0 = (warp & 3) * 16, n0 = (warp >> 2 & 1) * 32, i0 = m0 + (lane >> 2);
     float acc[4][4];
     zero(acc);
-    product<false, LD, true, kLd>(acc, warp < 8 ? in.k : in.q, nullptr, sh.s[0], sh.s[1], m0, n0, 0, DK);
+    product<false, LD, 0, true, kLd, DK * kLd, DK / 16>(acc, warp < 8 ? in.k : in.q, sh.s[0], m0, n0);
 #pragma unroll
     for (int half = 0; half < 2; half++) {
       const int i = i0 + half * 8;
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_scan_kernel(const ScanArgs
       const int y0 = (warp >> 2) * 16;
       float y[2][4];
       zero(y);
-      tri_product<false, true, kLd>(y, in.m.x[0], in.m.x[1], sh.r[0], sh.r[1], warp & 3, y0);
+      tri_product<false, true, kLd, kRows>(y, in.m.x[0], sh.r[0], warp & 3, y0);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = i0 + half * 8;
@@ -403,9 +404,9 @@ __global__ void __launch_bounds__(kScanThreads) delta_scan_kernel(const ScanArgs
     for (int t = 0; t < NS; t++)
 #pragma unroll
       for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-    product<true, LD, true, kLd>(s, in.k, nullptr, sh.w[0], sh.w[1], sm, sn, 0, kC);
+    product<true, LD, 0, true, kLd, kRows, 4>(s, in.k, sh.w[0], sm, sn);
     if (warp >= 8) {
-      tri_product<false, true, kLd>(acc, in.m.p[0], in.m.p[1], sh.u[0], sh.u[1], warp & 3, n0);
+      tri_product<false, true, kLd, kRows>(acc, in.m.p[0], sh.u[0], warp & 3, n0);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = i0 + half * 8;
@@ -513,8 +514,8 @@ __global__ void __launch_bounds__(kScanThreads) delta_back_kernel(const BackArgs
       float x[2][4], y[2][4];
       zero(x);
       zero(y);
-      product<false, LD, true, kLd>(x, in.k, nullptr, sh.s[0], sh.s[1], m0, n0, 0, DK);
-      tri_product<true, true, kLd>(y, in.m.p[0], in.m.p[1], in.o, nullptr, mt, n0);
+      product<false, LD, 0, true, kLd, DK * kLd, DK / 16>(x, in.k, sh.s[0], m0, n0);
+      tri_product<true, true, kLd, 0>(y, in.m.p[0], in.o, mt, n0);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = i0 + half * 8;
@@ -540,7 +541,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_back_kernel(const BackArgs
     {  // dR = X^T (beta dU)
       float x[2][4];
       zero(x);
-      tri_product<true, true, kLd>(x, in.m.x[0], in.m.x[1], sh.u[0], sh.u[1], mt, n0);
+      tri_product<true, true, kLd, kRows>(x, in.m.x[0], sh.u[0], mt, n0);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = i0 + half * 8;
@@ -572,9 +573,9 @@ __global__ void __launch_bounds__(kScanThreads) delta_back_kernel(const BackArgs
     for (int t = 0; t < NS; t++)
 #pragma unroll
       for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-    product<true, LD, true, kLd>(s, in.q, nullptr, sh.w[0], sh.w[1], sm, sn, 0, kC);
+    product<true, LD, 0, true, kLd, kRows, 4>(s, in.q, sh.w[0], sm, sn);
     __syncthreads();
-    product<true, LD, true, kLd>(s, in.k, nullptr, sh.r[0], sh.r[1], sm, sn, 0, kC);
+    product<true, LD, 0, true, kLd, kRows, 4>(s, in.k, sh.r[0], sm, sn);
   }
   if (!p.dstate) return;
 #pragma unroll
@@ -657,7 +658,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
   for (int t = 0; t < steps; t++) {
     const int h = kh * group + t / slices;
     const __nv_bfloat16* o = sh.o[t & 1];
-    const __nv_bfloat16 *r = sh.r[t & 1][0], *rl = sh.r[t & 1][1];
+    const __nv_bfloat16* r = sh.r[t & 1][0];
     if (t % slices == 0) {
       chunk_decay(a, sh.d, start, len, h);
       zero(oy);
@@ -668,7 +669,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
     __syncthreads();
     float x[NK][4];
     zero(x);
-    product<false, kLd, false, kLd>(x, o, nullptr, sh.s[0], sh.s[1], m0, d0, 0, 64);
+    product<false, kLd, 0, false, kLd, DK * kLd, 4>(x, o, sh.s[0], m0, d0);
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // scale E dO S^T, and what it adds to e_i
       const int i = i0 + half * 8;
@@ -683,7 +684,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
       }
     }
     zero(x);
-    product<false, kLd, false, kLd>(x, r, rl, sh.s[0], sh.s[1], m0, d0, 0, 64);
+    product<false, kLd, kRows, false, kLd, DK * kLd, 4>(x, r, sh.s[0], m0, d0);
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // -E dR S^T
       const int i = i0 + half * 8;
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
     __syncthreads();
     if (t + 1 < steps) load_a(t + 1);
     zero(x);
-    product<false, kLd, false, kLd>(x, sh.y[0], sh.y[1], sh.ds[0], sh.ds[1], m0, d0, 0, 64);
+    product<false, kLd, kRows, false, kLd, DK * kLd, 4>(x, sh.y[0], sh.ds[0], m0, d0);
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // F U dS'^T, and K_i . (dS' Y_i)
       const int i = i0 + half * 8;
@@ -725,8 +726,8 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
         dk[n][half * 2 + 1] = __fmaf_rn(b, v1, dk[n][half * 2 + 1]);
       }
     }
-    product<false, kLd, false, kLd>(oy, o, nullptr, sh.y[0], sh.y[1], m0, n0, 0, 64);
-    product<false, kLd, false, kLd>(ry, r, rl, sh.y[0], sh.y[1], m0, n0, 0, 64);
+    product<false, kLd, 0, false, kLd, kRows, 4>(oy, o, sh.y[0], m0, n0);
+    product<false, kLd, kRows, false, kLd, kRows, 4>(ry, r, sh.y[0], m0, n0);
     __syncthreads();
     if (t + 1 < steps) load_b(t + 1);
     if ((t + 1) % slices) continue;
@@ -734,8 +735,8 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
     float kk[2][4], qk[2][4];
     zero(kk);
     zero(qk);
-    product<false, LD, false, LD>(kk, sh.k, nullptr, sh.k, nullptr, m0, n0, 0, DK);
-    product<false, LD, false, LD>(qk, sh.q, nullptr, sh.k, nullptr, m0, n0, 0, DK);
+    product<false, LD, 0, false, LD, 0, DK / 16>(kk, sh.k, sh.k, m0, n0);
+    product<false, LD, 0, false, LD, 0, DK / 16>(qk, sh.q, sh.k, m0, n0);
 #pragma unroll
     for (int n = 0; n < 2; n++) {
       float col[2] = {0.f, 0.f};
@@ -782,10 +783,10 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
     for (int w = 16; w; w >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, w);
     if (lane == 0) sh.sum[warp] = inner;
     __syncthreads();
-    product<false, kLd, true, LD>(dq, sh.p[0], sh.p[1], sh.k, nullptr, m0, d0, 0, m0 + 16);
-    product<true, kLd, true, LD>(dk, sh.p[0], sh.p[1], sh.q, nullptr, m0, d0, m0, kC);
-    product<false, kLd, true, LD>(dk, sh.m[0], sh.m[1], sh.k, nullptr, m0, d0, 0, m0 + 16);
-    product<true, kLd, true, LD>(dk, sh.m[0], sh.m[1], sh.k, nullptr, m0, d0, m0, kC);
+    product_part<false, kLd, kRows, true, LD, 0>(dq, sh.p[0], sh.k, m0, d0, 0, wr + 1);
+    product_part<true, kLd, kRows, true, LD, 0>(dk, sh.p[0], sh.q, m0, d0, wr, 4);
+    product_part<false, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, 0, wr + 1);
+    product_part<true, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, wr, 4);
     if (warp == 0) {  // dbeta, and dg by sums of W's rows less its columns from the chunk's end, cut at resets
       const float keep = sh.d.since[kC - 1];
       float end = 0.f, sum[2];

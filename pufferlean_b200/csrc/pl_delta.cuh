@@ -121,52 +121,64 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The 16 x 16 fragment of A at (m, k): along k, or across.
+// Where this lane's rows of the 16 x 16 fragment at (0, 0) of an operand start, in elements: of A, along k or across, and of two
+// n-tiles of B (registers 0, 1 for the columns from n on, 2, 3 for n + 8).
 template <bool ACROSS, int LD>
-__device__ __forceinline__ void frag_a(uint32_t (&r)[4], const __nv_bfloat16* t, int m, int k) {
+__device__ __forceinline__ int lane_a() {
   const int lane = threadIdx.x & 31;
-  if constexpr (!ACROSS)
-    ldsm4(r, smem_u32(t + (m + (lane & 15)) * LD + k + (lane >> 4) * 8));
-  else
-    ldsm4t(r, smem_u32(t + (k + (lane & 7) + ((lane >> 4) & 1) * 8) * LD + m + ((lane >> 3) & 1) * 8));
+  if constexpr (!ACROSS) return (lane & 15) * LD + (lane >> 4) * 8;
+  else return ((lane & 7) + ((lane >> 4) & 1) * 8) * LD + ((lane >> 3) & 1) * 8;
 }
-// Two n-tiles of B at (k, n): b[0], b[1] for columns n.., b[2], b[3] for n + 8..
 template <bool ACROSS, int LD>
-__device__ __forceinline__ void frag_b(uint32_t (&r)[4], const __nv_bfloat16* t, int k, int n) {
+__device__ __forceinline__ int lane_b() {
   const int lane = threadIdx.x & 31;
-  if constexpr (!ACROSS)
-    ldsm4(r, smem_u32(t + (n + (lane & 7) + ((lane >> 4) & 1) * 8) * LD + k + ((lane >> 3) & 1) * 8));
-  else
-    ldsm4t(r, smem_u32(t + (k + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + n + ((lane >> 4) & 1) * 8));
+  if constexpr (!ACROSS) return ((lane & 7) + ((lane >> 4) & 1) * 8) * LD + ((lane >> 3) & 1) * 8;
+  else return ((lane & 7) + ((lane >> 3) & 1) * 8) * LD + ((lane >> 4) & 1) * 8;
+}
+template <bool ACROSS>
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
+  if constexpr (ACROSS) ldsm4t(r, at);
+  else ldsm4(r, at);
 }
 
-// acc (16 x 8 NT at (m, n)) += A B over k in [k0, k1). A f32 operand is two bf16 parts, the second one the rounding of what the
-// first leaves (2^-17 of the value is lost, the product of the two second parts with it); lo = nullptr: bf16 as it is.
-template <bool A_ACROSS, int LDA, bool B_ACROSS, int LDB, int NT>
-__device__ __forceinline__ void product(float (&acc)[NT][4], const __nv_bfloat16* a, const __nv_bfloat16* alo,
-                                        const __nv_bfloat16* b, const __nv_bfloat16* blo, int m, int n, int k0, int k1) {
-#pragma unroll 2
-  for (int k = k0; k < k1; k += 16) {
+// acc (16 x 8 NT at (m, n)) += A B over KS steps of 16 along k, from tile rows and columns (m, k = 0), (k = 0, n) on. A f32
+// operand is two bf16 parts, the second one the rounding of what the first leaves, ALO or BLO elements behind it (2^-17 of the
+// value is lost, the product of the two second parts with it); 0: bf16 as it is. Addresses are one register and constants.
+template <bool A_ACROSS, int LDA, int ALO, bool B_ACROSS, int LDB, int BLO, int KS, int NT>
+__device__ __forceinline__ void product(float (&acc)[NT][4], const __nv_bfloat16* a, const __nv_bfloat16* b, int m, int n) {
+  const uint32_t pa = smem_u32(a + (A_ACROSS ? m : m * LDA) + lane_a<A_ACROSS, LDA>());
+  const uint32_t pb = smem_u32(b + (B_ACROSS ? n : n * LDB) + lane_b<B_ACROSS, LDB>());
+#pragma unroll
+  for (int k = 0; k < KS; k++) {
     uint32_t x[4], xl[4];
-    frag_a<A_ACROSS, LDA>(x, a, m, k);
-    if (alo) frag_a<A_ACROSS, LDA>(xl, alo, m, k);
+    ldsm<A_ACROSS>(x, pa + k * 32 * (A_ACROSS ? LDA : 1));
+    if constexpr (ALO != 0) ldsm<A_ACROSS>(xl, pa + ALO * 2 + k * 32 * (A_ACROSS ? LDA : 1));
 #pragma unroll
     for (int t = 0; t < NT; t += 2) {
       uint32_t y[4];
-      frag_b<B_ACROSS, LDB>(y, b, k, n + t * 8);
+      const uint32_t at = pb + k * 32 * (B_ACROSS ? LDB : 1) + t * 16 * (B_ACROSS ? 1 : LDB);
+      ldsm<B_ACROSS>(y, at);
       mma(acc[t], x, y[0], y[1]);
       mma(acc[t + 1], x, y[2], y[3]);
-      if (alo) {
+      if constexpr (ALO != 0) {
         mma(acc[t], xl, y[0], y[1]);
         mma(acc[t + 1], xl, y[2], y[3]);
       }
-      if (blo) {
-        frag_b<B_ACROSS, LDB>(y, blo, k, n + t * 8);
+      if constexpr (BLO != 0) {
+        ldsm<B_ACROSS>(y, at + BLO * 2);
         mma(acc[t], x, y[0], y[1]);
         mma(acc[t + 1], x, y[2], y[3]);
       }
     }
   }
+}
+// The same over the row blocks [k0, k1) of k.
+template <bool A_ACROSS, int LDA, int ALO, bool B_ACROSS, int LDB, int BLO, int NT>
+__device__ __forceinline__ void product_part(float (&acc)[NT][4], const __nv_bfloat16* a, const __nv_bfloat16* b, int m,
+                                             int n, int k0, int k1) {
+  for (int k = k0; k < k1; k++)
+    product<A_ACROSS, LDA, ALO, B_ACROSS, LDB, BLO, 1>(acc, a + k * 16 * (A_ACROSS ? LDA : 1),
+                                                       b + k * 16 * (B_ACROSS ? LDB : 1), m, n);
 }
 
 // A lower triangular 64 x 64 matrix as the ten 16 x 16 blocks on and below its diagonal, block (r, c) the r (r + 1) / 2 + c-th;
@@ -176,39 +188,37 @@ __host__ __device__ __forceinline__ int tri_at(int i, int j) {
   const int r = i >> 4, c = j >> 4, y = i & 15, x = j & 15;
   return (r * (r + 1) / 2 + c) * 256 + y * 16 + (((x >> 3) ^ ((y >> 2) & 1)) << 3) + (x & 7);
 }
-// The fragment of block (r, c), or of its transpose.
-template <bool ACROSS>
-__device__ __forceinline__ void frag_tri(uint32_t (&x)[4], const __nv_bfloat16* t, int r, int c) {
+// acc (16 x 8 NT at row block mt, column n) += T B or (ACROSS) T^T B; T in one or two parts, B across.
+template <bool ACROSS, bool TWO, int LDB, int BLO, int NT>
+__device__ __forceinline__ void tri_product(float (&acc)[NT][4], const __nv_bfloat16* tri, const __nv_bfloat16* b, int mt,
+                                            int n) {
   const int lane = threadIdx.x & 31;
-  const __nv_bfloat16* b = t + (r * (r + 1) / 2 + c) * 256;
   const int y = ACROSS ? (lane & 7) + ((lane >> 4) & 1) * 8 : lane & 15, p = ACROSS ? (lane >> 3) & 1 : lane >> 4;
-  const uint32_t at = smem_u32(b + y * 16 + ((p ^ ((y >> 2) & 1)) << 3));
-  if constexpr (ACROSS) ldsm4t(x, at);
-  else ldsm4(x, at);
-}
-// acc (16 x 8 NT at row block mt, column n) += T B or (ACROSS) T^T B, T triangular in parts hi, lo (lo = nullptr: hi alone).
-template <bool ACROSS, bool B_ACROSS, int LDB, int NT>
-__device__ __forceinline__ void tri_product(float (&acc)[NT][4], const __nv_bfloat16* hi, const __nv_bfloat16* lo,
-                                            const __nv_bfloat16* b, const __nv_bfloat16* blo, int mt, int n) {
-  const int k0 = ACROSS ? mt : 0, k1 = ACROSS ? 4 : mt + 1;
-  for (int k = k0; k < k1; k++) {
+  const uint32_t pt = smem_u32(tri + y * 16 + ((p ^ ((y >> 2) & 1)) << 3));
+  const uint32_t pb = smem_u32(b + n + lane_b<true, LDB>());
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    if (ACROSS ? k < mt : k > mt) continue;
+    const int r = ACROSS ? k : mt, c = ACROSS ? mt : k;
+    const uint32_t at = pt + (r * (r + 1) / 2 + c) * 512;
     uint32_t x[4], xl[4];
-    frag_tri<ACROSS>(x, hi, ACROSS ? k : mt, ACROSS ? mt : k);
-    if (lo) frag_tri<ACROSS>(xl, lo, ACROSS ? k : mt, ACROSS ? mt : k);
+    ldsm<ACROSS>(x, at);
+    if constexpr (TWO) ldsm<ACROSS>(xl, at + kTri * 2);
 #pragma unroll
     for (int t = 0; t < NT; t += 2) {
-      uint32_t y[4];
-      frag_b<B_ACROSS, LDB>(y, b, k * 16, n + t * 8);
-      mma(acc[t], x, y[0], y[1]);
-      mma(acc[t + 1], x, y[2], y[3]);
-      if (lo) {
-        mma(acc[t], xl, y[0], y[1]);
-        mma(acc[t + 1], xl, y[2], y[3]);
+      uint32_t v[4];
+      const uint32_t bt = pb + k * 32 * LDB + t * 16;
+      ldsm<true>(v, bt);
+      mma(acc[t], x, v[0], v[1]);
+      mma(acc[t + 1], x, v[2], v[3]);
+      if constexpr (TWO) {
+        mma(acc[t], xl, v[0], v[1]);
+        mma(acc[t + 1], xl, v[2], v[3]);
       }
-      if (blo) {
-        frag_b<B_ACROSS, LDB>(y, blo, k * 16, n + t * 8);
-        mma(acc[t], x, y[0], y[1]);
-        mma(acc[t + 1], x, y[2], y[3]);
+      if constexpr (BLO != 0) {
+        ldsm<true>(v, bt + BLO * 2);
+        mma(acc[t], x, v[0], v[1]);
+        mma(acc[t + 1], x, v[2], v[3]);
       }
     }
   }
