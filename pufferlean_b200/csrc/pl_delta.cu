@@ -253,16 +253,14 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArg
 
 // ---------------------------------------------------------------------------------------------- the chain forward
 // What a chain leaves for the gradient, per slot, value head and 64 columns of v, as two bf16 parts one behind the other: a
-// state [2][dk][64], rows [2][64][64].
+// state, transposed, [2][64][dkp], and rows, transposed, [2][64][64 tokens].
 __device__ __forceinline__ long state_at(const DeltaArgs& a, long slot, int h, int slice) {
-  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * a.dk * 64;
+  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * 64 * a.dkp;
 }
 __device__ __forceinline__ long rows_at(const DeltaArgs& a, long slot, int h, int slice) {
   return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * kC * 64;
 }
 
-constexpr int kScanThreads = 512;
-constexpr int kRows = kC * kLd;  // a 64 x 64 tile: the distance of its second part
 struct ScanArgs {
   DeltaArgs d;
   const Mats* mats;
@@ -271,14 +269,11 @@ struct ScanArgs {
   float* final_state;
   __nv_bfloat16 *kept, *y;  // for the gradient: S and Y of every slot; or NULL
 };
-template <int DK>
-struct ScanShared {
-  struct In {  // a chunk's inputs, loaded while the chunk before it is worked on
-    __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], v[kC * kLd];
-    Mats m;
-  } in[2];
-  __nv_bfloat16 s[2][DK * kLd];  // the state's columns
-  __nv_bfloat16 r[2][kC * kLd], u[2][kC * kLd], w[2][kC * kLd];
+// A chunk's inputs, loaded while the chunk before it is worked on; x: v (forward), dO (back), of WARPS x 16 columns.
+template <int DK, int WARPS>
+struct ChainIn {
+  __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], x[kC * (WARPS * 16 + 8)];
+  Mats m;
 };
 
 // Rows that no sequence holds, in front of the first and behind the last: zero. Called by the blocks of those two.
@@ -293,146 +288,191 @@ __device__ __forceinline__ void zero_rows(const DeltaArgs& a, int seq, T* out, l
   }
 }
 
-// A block per sequence, value head and 64 of its columns, 16 warps. They hold the state in registers, 16 rows x 32 columns
-// each (dk <= 64: x 16); its two bf16 parts in shared memory are the operand of the next chunk's products. (With one part of
-// S, U and P in what goes into o alone, a fifth of the products, o would be 2.5e-3 off instead of 1.7e-3.)
-template <int DK>
-__global__ void __launch_bounds__(kScanThreads) delta_scan_kernel(const ScanArgs p) {
+// The state's columns of a warp, transposed, between memory [dk][dv] and registers [16 of dv][dk].
+template <int NT>
+__device__ __forceinline__ void state_in(float (&s)[NT][4], const float* src, int dk, int dv, int cols) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int j = (lane >> 2) + (e >> 1) * 8, i = t * 8 + (lane & 3) * 2 + (e & 1);
+      s[t][e] = src && i < dk && j < cols ? src[(long)i * dv + j] : 0.f;
+    }
+}
+template <int NT>
+__device__ __forceinline__ void state_out(const float (&s)[NT][4], float* dst, int dk, int dv, int cols) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int j = (lane >> 2) + (e >> 1) * 8, i = t * 8 + (lane & 3) * 2 + (e & 1);
+      if (i < dk && j < cols) dst[(long)i * dv + j] = s[t][e];
+    }
+}
+// An accumulator [16 of dv][8 NT] as two parts into [2][64][row] from `dst` (this warp's first row) on.
+template <int NT>
+__device__ __forceinline__ void parts_out(const float (&s)[NT][4], __nv_bfloat16* dst, int row, long second) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      uint32_t hi, lo;
+      split2(s[t][half * 2], s[t][half * 2 + 1], hi, lo);
+      __nv_bfloat16* at = dst + ((lane >> 2) + half * 8) * row + t * 8 + (lane & 3) * 2;
+      *reinterpret_cast<uint32_t*>(at) = hi;
+      *reinterpret_cast<uint32_t*>(at + second) = lo;
+    }
+}
+// 64 rows of 16 values that this warp put at `tile`, to rows of `stride` in memory, `cols` of them.
+template <int LD>
+__device__ __forceinline__ void rows_out(const __nv_bfloat16* tile, __nv_bfloat16* dst, long stride, int len, int cols,
+                                         bool vec) {
+  const int lane = threadIdx.x & 31;
+  if (vec && cols >= 16) {
+    for (int i = lane; i < len * 2; i += 32)
+      *reinterpret_cast<uint4*>(dst + (i >> 1) * stride + (i & 1) * 8) =
+          *reinterpret_cast<const uint4*>(tile + (i >> 1) * LD + (i & 1) * 8);
+  } else {
+    for (int i = lane; i < len * 16; i += 32)
+      if ((i & 15) < cols) dst[(i >> 4) * stride + (i & 15)] = tile[(i >> 4) * LD + (i & 15)];
+  }
+}
+
+// A block per sequence, value head and WARPS x 16 columns of v, a warp for each 16. Transposed, the state S^T [16][dk] stays in
+// a warp's registers for the whole sequence, and everything that the chunk makes of it: an accumulator's layout is that of
+// a first operand, so K S, R, Y, U and F U go from one product into the next as they are, split into two bf16 parts, and the warps
+// never wait for one another but for the inputs. (With R, Y, U and the state's parts in shared memory, shared by 16 warps in
+// four steps with barriers, a chunk of 64 columns took 5.6 us, half of it waiting for shared memory.)
+template <int DK, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 2 : 1) delta_scan_kernel(const ScanArgs p) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
-  ScanShared<DK>& sh = *reinterpret_cast<ScanShared<DK>*>(mem);
-  constexpr int LD = DK + 8, NS = DK / 32;  // n-tiles of a warp's part of the state
+  using In = ChainIn<DK, WARPS>;
+  In* ins = reinterpret_cast<In*>(mem);
+  constexpr int LD = DK + 8, LDX = WARPS * 16 + 8, NK = DK / 8, THREADS = WARPS * 32;
   const DeltaArgs& a = p.d;
-  const int slice = blockIdx.x, c0 = slice * 64, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-  const int sm = warp % (DK / 16) * 16, sn = warp / (DK / 16) * NS * 8;
+  const int c0 = blockIdx.x * WARPS * 16, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int cols = a.dv - c0 < WARPS * 16 ? a.dv - c0 : WARPS * 16;
+  const int w0 = c0 + warp * 16, mine = a.dv - w0 < 16 ? a.dv - w0 : 16;  // this warp's columns (none: <= 0)
   long from, to;
   seq_bounds(a, seq, from, to);
-  const long slot0 = from / kC + seq;
+  const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
   auto load = [&](long c) {
     const long start = from + c * kC;
     const int len = (int)(to - start < kC ? to - start : kC);
-    auto& in = sh.in[c & 1];
-    copy_tile<DK, LD, kScanThreads>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
-    copy_flat<kScanThreads>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats));
-    copy_tile<64, kLd, kScanThreads>(in.v, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vec);
-    copy_tile<DK, LD, kScanThreads>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
+    In& in = ins[c & 1];
+    copy_tile<DK, LD, THREADS>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
+    copy_tile<DK, LD, THREADS>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
+    copy_tile<WARPS * 16, LDX, THREADS>(in.x, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vec);
+    copy_flat<THREADS>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats));
     cp_commit();
   };
-  const long chunks = (to - from + kC - 1) / kC;
   if (chunks) load(0);
   zero_rows(a, seq, p.o + (long)h * a.dv + c0, (long)a.hv * a.dv, cols);
-  float s[NS][4];
-  const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + c0;
-#pragma unroll
-  for (int t = 0; t < NS; t++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int i = sm + (lane >> 2) + (e >> 1) * 8, j = sn + t * 8 + (lane & 3) * 2 + (e & 1);
-      s[t][e] = p.state && i < a.dk && j < cols ? p.state[sbase + (long)i * a.dv + j] : 0.f;
-    }
+  float s[NK][4];
+  const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
+  state_in(s, p.state ? p.state + sbase : nullptr, a.dk, a.dv, mine);
+  const bool vec_o = a.dv % 8 == 0 && (uintptr_t)p.o % 16 == 0;
+  const int slice = w0 / 64, row = w0 % 64;
   for (long c = 0; c < chunks; c++) {
     const long start = from + c * kC, slot = slot0 + c;
     const int len = (int)(to - start < kC ? to - start : kC);
-    const auto& in = sh.in[c & 1];
-#pragma unroll
-    for (int t = 0; t < NS; t++)
-#pragma unroll
-      for (int half = 0; half < 2; half++)
-        put2<kLd>(sh.s[0], sh.s[1], sm + (lane >> 2) + half * 8, sn + t * 8 + (lane & 3) * 2, s[t][half * 2],
-                  s[t][half * 2 + 1]);
+    In& in = ins[c & 1];
     cp_wait<0>();
     __syncthreads();
     if (c + 1 < chunks) load(c + 1);
-    if (p.kept)
+    if (w0 >= a.dvp) continue;  // (up to there the gradient's kernel reads, zeros beyond dv)
+    if (p.kept) parts_out(s, p.kept + state_at(a, slot, h, slice) + row * DK, DK, 64l * DK);
+    float r[8][4], o[8][4];  // (K S)^T, (Q S)^T: [16 of dv][64 tokens]
+    zero(r);
+    zero(o);
+    {
+      const uint32_t pk = smem_u32(in.k + lane_b<false, LD>()), pq = smem_u32(in.q + lane_b<false, LD>());
 #pragma unroll
-      for (int part = 0; part < 2; part++)
-        tile_out<kScanThreads>(p.kept + state_at(a, slot, h, slice) + part * a.dk * 64, sh.s[part], a.dk);
-    // warps 0 to 7: V - E K S; warps 8 to 15: E Q S; 16 rows x 32 columns each
-    const int m0 = (warp & 3) * 16, n0 = (warp >> 2 & 1) * 32, i0 = m0 + (lane >> 2);
-    float acc[4][4];
-    zero(acc);
-    product<false, LD, 0, true, kLd, DK * kLd, DK / 16>(acc, warp < 8 ? in.k : in.q, sh.s[0], m0, n0);
+      for (int k = 0; k < DK / 16; k++) {
+        const Parts x = parts_of(s[2 * k], s[2 * k + 1]);
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
-      const int i = i0 + half * 8;
-      const float f = in.m.since[i];
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        const int j = n0 + t * 8 + (lane & 3) * 2;
-        float x = f == 0.f ? 0.f : f * acc[t][half * 2], y = f == 0.f ? 0.f : f * acc[t][half * 2 + 1];
-        if (warp < 8) {
-          const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(in.v + i * kLd + j);
-          put2<kLd>(sh.r[0], sh.r[1], i, j, __low2float(v) - x, __high2float(v) - y);
-        } else {
-          acc[t][half * 2] = x;
-          acc[t][half * 2 + 1] = y;
+        for (int n = 0; n < 4; n++) {
+          uint32_t y[4];
+          ldsm<false>(y, pk + n * 32 * LD + k * 32);
+          mma2(r[2 * n], r[2 * n + 1], x, y);
+          ldsm<false>(y, pq + n * 32 * LD + k * 32);
+          mma2(o[2 * n], o[2 * n + 1], x, y);
         }
       }
     }
-    __syncthreads();
-    {  // Y = X R, 16 rows x 16 columns of every warp
-      const int y0 = (warp >> 2) * 16;
-      float y[2][4];
-      zero(y);
-      tri_product<false, true, kLd, kRows>(y, in.m.x[0], sh.r[0], warp & 3, y0);
+    const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, LDX>());
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int i = i0 + half * 8;
-        const float b = in.m.beta[i], f = in.m.until[i];
+    for (int n = 0; n < 4; n++) {  // R = V - E K S, E Q S
+      uint32_t v[4];
+      ldsm<true>(v, px + n * 32 * LDX);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-          const int j = y0 + t * 8 + (lane & 3) * 2;
-          const float y1 = y[t][half * 2], y2 = y[t][half * 2 + 1];
-          if (p.y) {
-            uint32_t hi, lo;
-            split2(y1, y2, hi, lo);
-            __nv_bfloat16* to_y = p.y + rows_at(a, slot, h, slice) + i * 64 + j;
-            *reinterpret_cast<uint32_t*>(to_y) = hi;
-            *reinterpret_cast<uint32_t*>(to_y + kC * 64) = lo;
-          }
-          put2<kLd>(sh.u[0], sh.u[1], i, j, b * y1, b * y2);
-          put2<kLd>(sh.w[0], sh.w[1], i, j, f * b * y1, f * b * y2);
+      for (int t = 0; t < 2; t++) {
+        const float2 f = *reinterpret_cast<const float2*>(in.m.since + n * 16 + t * 8 + (lane & 3) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float fe = e & 1 ? f.y : f.x;
+          const uint32_t vv = v[t * 2 + (e >> 1)];
+          float(&rr)[4] = r[2 * n + t], (&oo)[4] = o[2 * n + t];
+          rr[e] = __uint_as_float(e & 1 ? vv & 0xffff0000u : vv << 16) - (fe == 0.f ? 0.f : fe * rr[e]);
+          oo[e] = fe == 0.f ? 0.f : fe * oo[e];
         }
       }
     }
-    __syncthreads();
+    float y[8][4];  // Y^T = R^T X^T
+    zero(y);
+    const uint32_t tx = tri_lane<false>(in.m.x[0]), tp = tri_lane<false>(in.m.p[0]);
+#pragma unroll
+    for (int k = 0; k < 4; k++) tri_step<false>(y, parts_of(r[2 * k], r[2 * k + 1]), tx, k);
+    if (p.y) parts_out(y, p.y + rows_at(a, slot, h, slice) + row * 64, 64, 64l * 64);
+#pragma unroll
+    for (int t = 0; t < 8; t++) {  // U
+      const float2 b = *reinterpret_cast<const float2*>(in.m.beta + t * 8 + (lane & 3) * 2);
+      y[t][0] *= b.x, y[t][2] *= b.x;
+      y[t][1] *= b.y, y[t][3] *= b.y;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) tri_step<false>(o, parts_of(y[2 * k], y[2 * k + 1]), tp, k);
+    __syncwarp();  // the warp's columns of v have been read: o takes their place on its way out
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[2 * n][e] *= a.scale, o[2 * n + 1][e] *= a.scale;
+      store_across(smem_u32(in.x + (n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * LDX + warp * 16 + ((lane >> 3) & 1) * 8),
+                   o[2 * n], o[2 * n + 1]);
+    }
+    __syncwarp();
+    rows_out<LDX>(in.x + warp * 16, p.o + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_o);
     const float keep = in.m.since[kC - 1];
 #pragma unroll
-    for (int t = 0; t < NS; t++)
+    for (int t = 0; t < NK; t++)
 #pragma unroll
       for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-    product<true, LD, 0, true, kLd, kRows, 4>(s, in.k, sh.w[0], sm, sn);
-    if (warp >= 8) {
-      tri_product<false, true, kLd, kRows>(acc, in.m.p[0], sh.u[0], warp & 3, n0);
+    const uint32_t pk = smem_u32(in.k + lane_b<true, LD>());
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int i = i0 + half * 8;
-        if (i >= len) continue;
-        __nv_bfloat16* o = p.o + (start + i) * a.hv * a.dv + (long)h * a.dv + c0;
+    for (int k = 0; k < 4; k++) {  // S^T += (F U)^T K
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-          const int j = n0 + t * 8 + (lane & 3) * 2;
-          const float x = a.scale * acc[t][half * 2], y = a.scale * acc[t][half * 2 + 1];
-          if (a.dv % 2 == 0 && j + 1 < cols) {
-            *reinterpret_cast<__nv_bfloat162*>(o + j) = __floats2bfloat162_rn(x, y);
-          } else {
-            if (j < cols) o[j] = __float2bfloat16_rn(x);
-            if (j + 1 < cols) o[j + 1] = __float2bfloat16_rn(y);
-          }
-        }
+      for (int t = 0; t < 2; t++) {
+        const float2 f = *reinterpret_cast<const float2*>(in.m.until + k * 16 + t * 8 + (lane & 3) * 2);
+        float(&u)[4] = y[2 * k + t];
+        u[0] *= f.x, u[2] *= f.x;
+        u[1] *= f.y, u[3] *= f.y;
+      }
+      const Parts x = parts_of(y[2 * k], y[2 * k + 1]);
+#pragma unroll
+      for (int n = 0; n < DK / 16; n++) {
+        uint32_t b[4];
+        ldsm<true>(b, pk + k * 32 * LD + n * 32);
+        mma2(s[2 * n], s[2 * n + 1], x, b);
       }
     }
   }
-#pragma unroll
-  for (int t = 0; t < NS; t++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int i = sm + (lane >> 2) + (e >> 1) * 8, j = sn + t * 8 + (lane & 3) * 2 + (e & 1);
-      if (i < a.dk && j < cols) p.final_state[sbase + (long)i * a.dv + j] = s[t][e];
-    }
+  state_out(s, p.final_state + sbase, a.dk, a.dv, mine);
 }
 
 // ---------------------------------------------------------------------------------------------- the chain back
@@ -447,147 +487,141 @@ struct BackArgs {
   float* dstate;              // or NULL
   __nv_bfloat16 *ds, *dr;     // dS' and dR of every slot
 };
-template <int DK>
-struct BackShared {
-  struct In {
-    __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], o[kC * kLd];
-    Mats m;
-  } in[2];
-  __nv_bfloat16 s[2][DK * kLd];
-  __nv_bfloat16 u[2][kC * kLd], r[2][kC * kLd], w[2][kC * kLd];
-};
 // As the chain forward, from the last chunk to the first.
-template <int DK>
-__global__ void __launch_bounds__(kScanThreads) delta_back_kernel(const BackArgs p) {
+template <int DK, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 2 : 1) delta_back_kernel(const BackArgs p) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
-  BackShared<DK>& sh = *reinterpret_cast<BackShared<DK>*>(mem);
-  constexpr int LD = DK + 8, NS = DK / 32;
+  using In = ChainIn<DK, WARPS>;
+  In* ins = reinterpret_cast<In*>(mem);
+  constexpr int LD = DK + 8, LDX = WARPS * 16 + 8, NK = DK / 8, THREADS = WARPS * 32;
   const DeltaArgs& a = p.d;
-  const int slice = blockIdx.x, c0 = slice * 64, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-  const int sm = warp % (DK / 16) * 16, sn = warp / (DK / 16) * NS * 8;
+  const int c0 = blockIdx.x * WARPS * 16, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int cols = a.dv - c0 < WARPS * 16 ? a.dv - c0 : WARPS * 16;
+  const int w0 = c0 + warp * 16, mine = a.dv - w0 < 16 ? a.dv - w0 : 16;
   long from, to;
   seq_bounds(a, seq, from, to);
   const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
   auto load = [&](long c) {
     const long start = from + c * kC;
     const int len = (int)(to - start < kC ? to - start : kC);
-    auto& in = sh.in[c & 1];
-    copy_tile<DK, LD, kScanThreads>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
-    copy_flat<kScanThreads>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats));
-    copy_tile<64, kLd, kScanThreads>(in.o, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
-    copy_tile<DK, LD, kScanThreads>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
+    In& in = ins[c & 1];
+    copy_tile<DK, LD, THREADS>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
+    copy_tile<DK, LD, THREADS>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
+    copy_tile<WARPS * 16, LDX, THREADS>(in.x, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
+    copy_flat<THREADS>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats));
     cp_commit();
   };
   if (chunks) load(chunks - 1);
   zero_rows(a, seq, p.dv + (long)h * a.dv + c0, (long)a.hv * a.dv, cols);
-  float s[NS][4];
-  const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + c0;
-#pragma unroll
-  for (int t = 0; t < NS; t++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int i = sm + (lane >> 2) + (e >> 1) * 8, j = sn + t * 8 + (lane & 3) * 2 + (e & 1);
-      s[t][e] = p.dfinal && i < a.dk && j < cols ? p.dfinal[sbase + (long)i * a.dv + j] : 0.f;
-    }
-  const int mt = warp & 3, m0 = mt * 16, n0 = (warp >> 2) * 16, i0 = m0 + (lane >> 2);  // 16 x 16 of a 64 x 64 tile
+  float s[NK][4];  // dS'^T
+  const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
+  state_in(s, p.dfinal ? p.dfinal + sbase : nullptr, a.dk, a.dv, mine);
+  const bool vec_dv = a.dv % 8 == 0 && (uintptr_t)p.dv % 16 == 0;
+  const int slice = w0 / 64, row = w0 % 64;
   for (long c = chunks - 1; c >= 0; c--) {
     const long start = from + c * kC, slot = slot0 + c;
     const int len = (int)(to - start < kC ? to - start : kC);
-    const auto& in = sh.in[c & 1];
-#pragma unroll
-    for (int t = 0; t < NS; t++)
-#pragma unroll
-      for (int half = 0; half < 2; half++)
-        put2<kLd>(sh.s[0], sh.s[1], sm + (lane >> 2) + half * 8, sn + t * 8 + (lane & 3) * 2, s[t][half * 2],
-                  s[t][half * 2 + 1]);
+    In& in = ins[c & 1];
     cp_wait<0>();
     __syncthreads();
     if (c > 0) load(c - 1);
+    if (w0 >= a.dvp) continue;  // (up to there the gradient's kernel reads, zeros beyond dv)
+    parts_out(s, p.ds + state_at(a, slot, h, slice) + row * DK, DK, 64l * DK);
+    float u[8][4], x[8][4];  // (P^T dO)^T, (K dS')^T: [16 of dv][64 tokens]
+    zero(u);
+    zero(x);
+    const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, LDX>());
+    const uint32_t tx = tri_lane<true>(in.m.x[0]), tp = tri_lane<true>(in.m.p[0]);
 #pragma unroll
-    for (int part = 0; part < 2; part++)
-      tile_out<kScanThreads>(p.ds + state_at(a, slot, h, slice) + part * a.dk * 64, sh.s[part], a.dk);
-    {  // diag(beta) dU = beta (F K dS' + scale P^T dO)
-      float x[2][4], y[2][4];
-      zero(x);
-      zero(y);
-      product<false, LD, 0, true, kLd, DK * kLd, DK / 16>(x, in.k, sh.s[0], m0, n0);
-      tri_product<true, true, kLd, 0>(y, in.m.p[0], in.o, mt, n0);
+    for (int k = 0; k < 4; k++) {
+      uint32_t o[4];
+      ldsm<true>(o, px + k * 32 * LDX);
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int i = i0 + half * 8;
-        const float b = in.m.beta[i], f = in.m.until[i];
+      for (int n = 0; n <= k; n++)
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-          float z[2];
+        for (int part = 0; part < 2; part++) {
+          uint32_t y[4];
+          ldsm<true>(y, tp + (k * (k + 1) / 2 + n) * 512 + part * kTri * 2);
+          mma(u[2 * n], o, y[0], y[1]);
+          mma(u[2 * n + 1], o, y[2], y[3]);
+        }
+    }
+    {
+      const uint32_t pk = smem_u32(in.k + lane_b<false, LD>());
 #pragma unroll
-          for (int e = 0; e < 2; e++)
-            z[e] = b * ((f == 0.f ? 0.f : f * x[t][half * 2 + e]) + a.scale * y[t][half * 2 + e]);
-          put2<kLd>(sh.u[0], sh.u[1], i, n0 + t * 8 + (lane & 3) * 2, z[0], z[1]);
+      for (int k = 0; k < DK / 16; k++) {
+        const Parts z = parts_of(s[2 * k], s[2 * k + 1]);
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          uint32_t y[4];
+          ldsm<false>(y, pk + n * 32 * LD + k * 32);
+          mma2(x[2 * n], x[2 * n + 1], z, y);
         }
       }
     }
-    // scale E dO, the operand of Q's part
-    for (int i = tid; i < kC * 32; i += kScanThreads) {
-      const int r = i >> 5, cc = (i & 31) * 2;
-      const float f = a.scale * in.m.since[r];
-      const __nv_bfloat162 o = *reinterpret_cast<const __nv_bfloat162*>(in.o + r * kLd + cc);
-      put2<kLd>(sh.w[0], sh.w[1], r, cc, f == 0.f ? 0.f : f * __low2float(o), f == 0.f ? 0.f : f * __high2float(o));
-    }
-    __syncthreads();
-    {  // dR = X^T (beta dU)
-      float x[2][4];
-      zero(x);
-      tri_product<true, true, kLd, kRows>(x, in.m.x[0], sh.u[0], mt, n0);
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int i = i0 + half * 8;
-        const float f = -in.m.since[i];
-        __nv_bfloat16* dv = p.dv + (start + i) * a.hv * a.dv + (long)h * a.dv + c0;
+    for (int t = 0; t < 8; t++) {  // beta dU = beta (F K dS' + scale P^T dO)
+      const float2 b = *reinterpret_cast<const float2*>(in.m.beta + t * 8 + (lane & 3) * 2);
+      const float2 f = *reinterpret_cast<const float2*>(in.m.until + t * 8 + (lane & 3) * 2);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-          const int j = n0 + t * 8 + (lane & 3) * 2;
-          const float y0 = x[t][half * 2], y1 = x[t][half * 2 + 1];
-          uint32_t hi, lo;
-          split2(y0, y1, hi, lo);
-          __nv_bfloat16* to_r = p.dr + rows_at(a, slot, h, slice) + i * 64 + j;
-          *reinterpret_cast<uint32_t*>(to_r) = hi;
-          *reinterpret_cast<uint32_t*>(to_r + kC * 64) = lo;
-          if (i < len) {
-            if (a.dv % 2 == 0 && j + 1 < cols) {
-              *reinterpret_cast<uint32_t*>(dv + j) = hi;
-            } else {
-              if (j < cols) dv[j] = __float2bfloat16_rn(y0);
-              if (j + 1 < cols) dv[j + 1] = __float2bfloat16_rn(y1);
-            }
-          }
-          put2<kLd>(sh.r[0], sh.r[1], i, j, f == 0.f ? 0.f : f * y0, f == 0.f ? 0.f : f * y1);
-        }
+      for (int e = 0; e < 4; e++) {
+        const float fe = e & 1 ? f.y : f.x, be = e & 1 ? b.y : b.x;
+        u[t][e] = be * ((fe == 0.f ? 0.f : fe * x[t][e]) + a.scale * u[t][e]);
       }
     }
+    zero(x);  // dR^T = (beta dU)^T X
+#pragma unroll
+    for (int k = 0; k < 4; k++) tri_step<true>(x, parts_of(u[2 * k], u[2 * k + 1]), tx, k);
+    parts_out(x, p.dr + rows_at(a, slot, h, slice) + row * 64, 64, 64l * 64);
     const float keep = in.m.since[kC - 1];
 #pragma unroll
-    for (int t = 0; t < NS; t++)
+    for (int t = 0; t < NK; t++)
 #pragma unroll
       for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-    product<true, LD, 0, true, kLd, kRows, 4>(s, in.q, sh.w[0], sm, sn);
-    __syncthreads();
-    product<true, LD, 0, true, kLd, kRows, 4>(s, in.k, sh.r[0], sm, sn);
-  }
-  if (!p.dstate) return;
+    const uint32_t pk = smem_u32(in.k + lane_b<true, LD>()), pq = smem_u32(in.q + lane_b<true, LD>());
 #pragma unroll
-  for (int t = 0; t < NS; t++)
+    for (int k = 0; k < 4; k++) {  // dS^T += scale (E dO)^T Q - (E dR)^T K
+      uint32_t o[4];
+      ldsm<true>(o, px + k * 32 * LDX);
+      float eo[2][4], er[2][4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int i = sm + (lane >> 2) + (e >> 1) * 8, j = sn + t * 8 + (lane & 3) * 2 + (e & 1);
-      if (i < a.dk && j < cols) p.dstate[sbase + (long)i * a.dv + j] = s[t][e];
+      for (int t = 0; t < 2; t++) {
+        const float2 f = *reinterpret_cast<const float2*>(in.m.since + k * 16 + t * 8 + (lane & 3) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float fe = e & 1 ? f.y : f.x;
+          const uint32_t oo = o[t * 2 + (e >> 1)];
+          eo[t][e] = fe == 0.f ? 0.f : a.scale * fe * __uint_as_float(e & 1 ? oo & 0xffff0000u : oo << 16);
+          er[t][e] = fe == 0.f ? 0.f : -fe * x[2 * k + t][e];
+        }
+      }
+      const Parts po = parts_of(eo[0], eo[1]), pr = parts_of(er[0], er[1]);
+#pragma unroll
+      for (int n = 0; n < DK / 16; n++) {
+        uint32_t b[4];
+        ldsm<true>(b, pq + k * 32 * LD + n * 32);
+        mma2(s[2 * n], s[2 * n + 1], po, b);
+        ldsm<true>(b, pk + k * 32 * LD + n * 32);
+        mma2(s[2 * n], s[2 * n + 1], pr, b);
+      }
     }
+    __syncwarp();  // the warp's columns of dO have been read: dv takes their place on its way out
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+      store_across(smem_u32(in.x + (n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * LDX + warp * 16 + ((lane >> 3) & 1) * 8),
+                   x[2 * n], x[2 * n + 1]);
+    __syncwarp();
+    rows_out<LDX>(in.x + warp * 16, p.dv + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_dv);
+  }
+  if (p.dstate) state_out(s, p.dstate + sbase, a.dk, a.dv, mine);
 }
 
 // ---------------------------------------------------------------------------------------------- the other gradients
+constexpr int kGradThreads = 512;
+constexpr int kRows = kC * kLd;  // a 64 x 64 tile: the distance of its second part
 struct GradArgs {
   DeltaArgs d;
   const __nv_bfloat16* dout;
@@ -601,7 +635,7 @@ template <int DK>
 struct GradShared {
   __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)];
   __nv_bfloat16 o[2][kC * kLd], r[2][2][kC * kLd];  // by turns: the next step's are on their way
-  __nv_bfloat16 s[2][DK * kLd], ds[2][DK * kLd], y[2][kC * kLd];
+  __nv_bfloat16 s[2][kC * (DK + 8)], ds[2][kC * (DK + 8)], y[2][kC * kLd];  // transposed, as r
   __nv_bfloat16 p[2][kC * kLd], m[2][kC * kLd];     // scale dO U^T * D, -M
   float row[4][kC], col[4][kC], krow[4][kC], sum[16];
   Decay d;
@@ -610,12 +644,13 @@ struct GradShared {
 // registers and is added in their order; of each, 64 columns of v after the other (a step). A step's loads are under
 // way during the one before it.
 template <int DK>
-__global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs p) {
+__global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs p) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
   GradShared<DK>& sh = *reinterpret_cast<GradShared<DK>*>(mem);
   constexpr int LD = DK + 8, NK = DK / 32;  // n-tiles of a warp's quarter of dk
+  constexpr int kState = kC * LD;           // the distance of a state's second part
   const DeltaArgs& a = p.d;
   const long slot = blockIdx.x;
   const int kh = blockIdx.y, group = a.hv / a.hk, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -626,11 +661,11 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
   auto load_a = [&](int t) {  // S, dO, dR
     const int h = kh * group + t / slices, slice = t % slices, c0 = slice * 64;
     const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-    copy_tile<64, kLd, kScanThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
+    copy_tile<64, kLd, kGradThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
 #pragma unroll
     for (int part = 0; part < 2; part++) {
-      tile_in<kScanThreads>(sh.s[part], p.kept + state_at(a, slot, h, slice) + part * a.dk * 64, a.dk);
-      tile_in<kScanThreads>(sh.r[t & 1][part], p.dr + rows_at(a, slot, h, slice) + part * kC * 64, kC);
+      tile_in<DK, LD, kGradThreads>(sh.s[part], p.kept + state_at(a, slot, h, slice) + part * 64 * DK);
+      tile_in<64, kLd, kGradThreads>(sh.r[t & 1][part], p.dr + rows_at(a, slot, h, slice) + part * kC * 64);
     }
     cp_commit();
   };
@@ -638,18 +673,15 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
     const int h = kh * group + t / slices, slice = t % slices;
 #pragma unroll
     for (int part = 0; part < 2; part++) {
-      tile_in<kScanThreads>(sh.ds[part], p.ds + state_at(a, slot, h, slice) + part * a.dk * 64, a.dk);
-      tile_in<kScanThreads>(sh.y[part], p.y + rows_at(a, slot, h, slice) + part * kC * 64, kC);
+      tile_in<DK, LD, kGradThreads>(sh.ds[part], p.ds + state_at(a, slot, h, slice) + part * 64 * DK);
+      tile_in<64, kLd, kGradThreads>(sh.y[part], p.y + rows_at(a, slot, h, slice) + part * kC * 64);
     }
     cp_commit();
   };
-  copy_tile<DK, LD, kScanThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
-  copy_tile<DK, LD, kScanThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
+  copy_tile<DK, LD, kGradThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
+  copy_tile<DK, LD, kGradThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
   load_a(0);
   load_b(0);
-  // the states' rows behind dk stay zero
-  for (int i = a.dk * kLd + tid; i < DK * kLd; i += kScanThreads)
-    sh.s[0][i] = sh.s[1][i] = sh.ds[0][i] = sh.ds[1][i] = __float2bfloat16_rn(0.f);
   const int wr = warp & 3, wc = warp >> 2, m0 = wr * 16, i0 = m0 + (lane >> 2);
   const int n0 = wc * 16, d0 = wc * (DK / 4);  // this warp's columns of a 64 x 64 tile, of a 64 x dk tile
   float dq[NK][4], dk[NK][4], oy[2][4], ry[2][4], qrow[2], krow[2], inner = 0.f;
@@ -669,7 +701,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
     __syncthreads();
     float x[NK][4];
     zero(x);
-    product<false, kLd, 0, false, kLd, DK * kLd, 4>(x, o, sh.s[0], m0, d0);
+    product<false, kLd, 0, true, LD, kState, 4>(x, o, sh.s[0], m0, d0);
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // scale E dO S^T, and what it adds to e_i
       const int i = i0 + half * 8;
@@ -684,7 +716,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
       }
     }
     zero(x);
-    product<false, kLd, kRows, false, kLd, DK * kLd, 4>(x, r, sh.s[0], m0, d0);
+    product<true, kLd, kRows, true, LD, kState, 4>(x, r, sh.s[0], m0, d0);
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // -E dR S^T
       const int i = i0 + half * 8;
@@ -700,8 +732,8 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
     }
     cp_wait<0>();
     __syncthreads();
-    for (int i = tid; i < DK * 32; i += kScanThreads) {  // <S, dS'>
-      const int at = (i >> 5) * kLd + (i & 31) * 2;
+    for (int i = tid; i < kC * DK / 2; i += kGradThreads) {  // <S, dS'>
+      const int at = i / (DK / 2) * LD + i % (DK / 2) * 2;
       auto two = [&](const __nv_bfloat16* hi, const __nv_bfloat16* lo) {
         const __nv_bfloat162 h2 = *reinterpret_cast<const __nv_bfloat162*>(hi + at), l2 = *reinterpret_cast<const __nv_bfloat162*>(lo + at);
         return make_float2(__low2float(h2) + __low2float(l2), __high2float(h2) + __high2float(l2));
@@ -712,7 +744,7 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
     __syncthreads();
     if (t + 1 < steps) load_a(t + 1);
     zero(x);
-    product<false, kLd, kRows, false, kLd, DK * kLd, 4>(x, sh.y[0], sh.ds[0], m0, d0);
+    product<true, kLd, kRows, true, LD, kState, 4>(x, sh.y[0], sh.ds[0], m0, d0);
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // F U dS'^T, and K_i . (dS' Y_i)
       const int i = i0 + half * 8;
@@ -726,8 +758,8 @@ __global__ void __launch_bounds__(kScanThreads) delta_grad_kernel(const GradArgs
         dk[n][half * 2 + 1] = __fmaf_rn(b, v1, dk[n][half * 2 + 1]);
       }
     }
-    product<false, kLd, 0, false, kLd, kRows, 4>(oy, o, sh.y[0], m0, n0);
-    product<false, kLd, kRows, false, kLd, kRows, 4>(ry, r, sh.y[0], m0, n0);
+    product<false, kLd, 0, true, kLd, kRows, 4>(oy, o, sh.y[0], m0, n0);
+    product<true, kLd, kRows, true, kLd, kRows, 4>(ry, r, sh.y[0], m0, n0);
     __syncthreads();
     if (t + 1 < steps) load_b(t + 1);
     if ((t + 1) % slices) continue;
@@ -893,6 +925,7 @@ static DeltaArgs delta_args(const pl_delta_shape* s, const void* q, const void* 
   a.hv = (int)s->heads_v;
   a.dk = (int)s->dk;
   a.dv = (int)s->dv;
+  a.dkp = s->dk > 64 ? 128 : 64;
   a.dvp = (int)round_up((long)s->dv, 64);
   a.offsets = offsets;
   a.ldq = (long)s->q_token;
@@ -915,7 +948,9 @@ static size_t heads_slots(const pl_delta_shape* s) {
   return (size_t)slot_count((long)s->tokens, (long)s->sequences) * s->heads_v;
 }
 static size_t mats_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * sizeof(Mats)); }
-static size_t states_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * s->dk * round_up((long)s->dv, 64) * 4); }
+static size_t states_bytes(const pl_delta_shape* s) {
+  return up256(heads_slots(s) * (s->dk > 64 ? 128 : 64) * round_up((long)s->dv, 64) * 4);
+}
 static size_t rows_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * kC * round_up((long)s->dv, 64) * 4); }
 
 template <typename A>
@@ -925,6 +960,12 @@ static int launch_wide(void (*kernel)(A), dim3 grid, int threads, size_t smem, c
   PL_CUDA(launch_early(kernel, grid, dim3(threads), smem, st, args));
   count_launch();
   return PL_OK;
+}
+// A chain takes 128 columns of v per block if there are that many and enough chains to fill the SMs that way (K and Q are
+// read once for 128 columns then), 64 otherwise.
+static bool wide_chains(const DeltaArgs& a) { return a.dv > 64 && (long)a.seqs * a.hv * (a.dvp / 64) > 148; }
+static dim3 chain_grid(const DeltaArgs& a, bool wide) {
+  return dim3((unsigned)ceil_div(a.dv, wide ? 128 : 64), (unsigned)a.hv, (unsigned)a.seqs);
 }
 static int prep(const DeltaArgs& a, Mats* mats, cudaStream_t st) {
   const dim3 grid((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
@@ -989,9 +1030,13 @@ int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const vo
     p.kept = (__nv_bfloat16*)saved;
     p.y = (__nv_bfloat16*)((char*)saved + states_bytes(s));
   }
-  const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
-  return a.dk > 64 ? launch_wide(delta_scan_kernel<128>, grid, kScanThreads, sizeof(ScanShared<128>), st, p)
-                   : launch_wide(delta_scan_kernel<64>, grid, kScanThreads, sizeof(ScanShared<64>), st, p);
+  const bool wide = wide_chains(a);
+  const dim3 grid = chain_grid(a, wide);
+  if (a.dk > 64)
+    return wide ? launch_wide(delta_scan_kernel<128, 8>, grid, 256, 2 * sizeof(ChainIn<128, 8>), st, p)
+                : launch_wide(delta_scan_kernel<128, 4>, grid, 128, 2 * sizeof(ChainIn<128, 4>), st, p);
+  return wide ? launch_wide(delta_scan_kernel<64, 8>, grid, 256, 2 * sizeof(ChainIn<64, 8>), st, p)
+              : launch_wide(delta_scan_kernel<64, 4>, grid, 128, 2 * sizeof(ChainIn<64, 4>), st, p);
 }
 
 int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token, size_t do_head, const float* dfinal,
@@ -1025,16 +1070,21 @@ int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token
   }
   const BackArgs b = {a, (const Mats*)ws, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, dfinal,
                       (__nv_bfloat16*)dv, dstate, ds, dr};
-  const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
-  rc = a.dk > 64 ? launch_wide(delta_back_kernel<128>, grid, kScanThreads, sizeof(BackShared<128>), st, b)
-                 : launch_wide(delta_back_kernel<64>, grid, kScanThreads, sizeof(BackShared<64>), st, b);
+  const bool wide = wide_chains(a);
+  const dim3 grid = chain_grid(a, wide);
+  if (a.dk > 64)
+    rc = wide ? launch_wide(delta_back_kernel<128, 8>, grid, 256, 2 * sizeof(ChainIn<128, 8>), st, b)
+              : launch_wide(delta_back_kernel<128, 4>, grid, 128, 2 * sizeof(ChainIn<128, 4>), st, b);
+  else
+    rc = wide ? launch_wide(delta_back_kernel<64, 8>, grid, 256, 2 * sizeof(ChainIn<64, 8>), st, b)
+              : launch_wide(delta_back_kernel<64, 4>, grid, 128, 2 * sizeof(ChainIn<64, 4>), st, b);
   if (rc || s->tokens == 0) return rc;
   const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, (const __nv_bfloat16*)saved,
                       (const __nv_bfloat16*)((const char*)saved + states_bytes(s)), ds, dr, (__nv_bfloat16*)dq, (__nv_bfloat16*)dk,
                       dg, dbeta};
   const dim3 chunks((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
-  rc = a.dk > 64 ? launch_wide(delta_grad_kernel<128>, chunks, kScanThreads, sizeof(GradShared<128>), st, p)
-                 : launch_wide(delta_grad_kernel<64>, chunks, kScanThreads, sizeof(GradShared<64>), st, p);
+  rc = a.dk > 64 ? launch_wide(delta_grad_kernel<128>, chunks, kGradThreads, sizeof(GradShared<128>), st, p)
+                 : launch_wide(delta_grad_kernel<64>, chunks, kGradThreads, sizeof(GradShared<64>), st, p);
   if (rc || !offsets) return rc;
   PL_CUDA(launch_early(delta_rest_kernel, dim3(64), dim3(256), 0, st, p));
   count_launch();

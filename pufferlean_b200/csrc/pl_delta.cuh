@@ -10,7 +10,7 @@ constexpr int kLd = 72;   // row stride of a 64-column bf16 tile in shared memor
 
 struct DeltaArgs {
   long n;                      // tokens
-  int seqs, hk, hv, dk, dv, dvp;  // dvp: dv rounded up to 64
+  int seqs, hk, hv, dk, dv, dkp, dvp;  // dkp: 64 or 128; dvp: dv rounded up to 64
   const int* offsets;          // [seqs + 1], or NULL: sequences of n / seqs tokens
   long ldq, hsq, ldk, hsk, ldv, hsv;  // strides of tokens and heads
   const __nv_bfloat16 *q, *k, *v;
@@ -90,15 +90,11 @@ template <int THREADS>
 __device__ __forceinline__ void copy_flat(void* dst, const void* src, int n) {
   for (int i = threadIdx.x * 16; i < n; i += THREADS * 16) cp16((char*)dst + i, (const char*)src + i, 16);
 }
-// `rows` rows of 64 values (128 bytes, one behind the other in memory) into, or out of, a tile of stride kLd.
-template <int THREADS>
-__device__ __forceinline__ void tile_in(__nv_bfloat16* tile, const __nv_bfloat16* src, int rows) {
-  for (int i = threadIdx.x; i < rows * 8; i += THREADS) cp16(tile + (i >> 3) * kLd + (i & 7) * 8, src + i * 8, 16);
-}
-template <int THREADS>
-__device__ __forceinline__ void tile_out(__nv_bfloat16* dst, const __nv_bfloat16* tile, int rows) {
-  for (int i = threadIdx.x; i < rows * 8; i += THREADS)
-    *reinterpret_cast<uint4*>(dst + i * 8) = *reinterpret_cast<const uint4*>(tile + (i >> 3) * kLd + (i & 7) * 8);
+// 64 rows of COLS values, one behind the other in memory, into a tile of row stride LD.
+template <int COLS, int LD, int THREADS>
+__device__ __forceinline__ void tile_in(__nv_bfloat16* tile, const __nv_bfloat16* src) {
+  for (int i = threadIdx.x; i < kC * COLS / 8; i += THREADS)
+    cp16(tile + i / (COLS / 8) * LD + i % (COLS / 8) * 8, src + i * 8, 16);
 }
 
 // ---------------------------------------------------------------------------------------------- products
@@ -188,42 +184,6 @@ __host__ __device__ __forceinline__ int tri_at(int i, int j) {
   const int r = i >> 4, c = j >> 4, y = i & 15, x = j & 15;
   return (r * (r + 1) / 2 + c) * 256 + y * 16 + (((x >> 3) ^ ((y >> 2) & 1)) << 3) + (x & 7);
 }
-// acc (16 x 8 NT at row block mt, column n) += T B or (ACROSS) T^T B; T in one or two parts, B across.
-template <bool ACROSS, bool TWO, int LDB, int BLO, int NT>
-__device__ __forceinline__ void tri_product(float (&acc)[NT][4], const __nv_bfloat16* tri, const __nv_bfloat16* b, int mt,
-                                            int n) {
-  const int lane = threadIdx.x & 31;
-  const int y = ACROSS ? (lane & 7) + ((lane >> 4) & 1) * 8 : lane & 15, p = ACROSS ? (lane >> 3) & 1 : lane >> 4;
-  const uint32_t pt = smem_u32(tri + y * 16 + ((p ^ ((y >> 2) & 1)) << 3));
-  const uint32_t pb = smem_u32(b + n + lane_b<true, LDB>());
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    if (ACROSS ? k < mt : k > mt) continue;
-    const int r = ACROSS ? k : mt, c = ACROSS ? mt : k;
-    const uint32_t at = pt + (r * (r + 1) / 2 + c) * 512;
-    uint32_t x[4], xl[4];
-    ldsm<ACROSS>(x, at);
-    if constexpr (TWO) ldsm<ACROSS>(xl, at + kTri * 2);
-#pragma unroll
-    for (int t = 0; t < NT; t += 2) {
-      uint32_t v[4];
-      const uint32_t bt = pb + k * 32 * LDB + t * 16;
-      ldsm<true>(v, bt);
-      mma(acc[t], x, v[0], v[1]);
-      mma(acc[t + 1], x, v[2], v[3]);
-      if constexpr (TWO) {
-        mma(acc[t], xl, v[0], v[1]);
-        mma(acc[t + 1], xl, v[2], v[3]);
-      }
-      if constexpr (BLO != 0) {
-        ldsm<true>(v, bt + BLO * 2);
-        mma(acc[t], x, v[0], v[1]);
-        mma(acc[t + 1], x, v[2], v[3]);
-      }
-    }
-  }
-}
-
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
   const __nv_bfloat162 l = __floats2bfloat162_rn(x - __low2float(h), y - __high2float(h));
@@ -237,6 +197,60 @@ __device__ __forceinline__ void put2(__nv_bfloat16* hi, __nv_bfloat16* lo, int r
   split2(x, y, h, l);
   *reinterpret_cast<uint32_t*>(hi + row * LD + col) = h;
   *reinterpret_cast<uint32_t*>(lo + row * LD + col) = l;
+}
+
+// ---- products whose first operand is in registers: an accumulator's two neighbouring n-tiles, 16 rows x 16 columns, are
+// the fragment of A for 16 steps of k, as two bf16 parts.
+struct Parts {
+  uint32_t hi[4], lo[4];
+};
+__device__ __forceinline__ Parts parts_of(const float (&x)[4], const float (&y)[4]) {
+  Parts p;
+  split2(x[0], x[1], p.hi[0], p.lo[0]);
+  split2(x[2], x[3], p.hi[1], p.lo[1]);
+  split2(y[0], y[1], p.hi[2], p.lo[2]);
+  split2(y[2], y[3], p.hi[3], p.lo[3]);
+  return p;
+}
+// c[0], c[1] (two n-tiles) += A B, B bf16 as it is / in two parts (y, yl).
+__device__ __forceinline__ void mma2(float (&c0)[4], float (&c1)[4], const Parts& a, const uint32_t (&y)[4]) {
+  mma(c0, a.hi, y[0], y[1]);
+  mma(c1, a.hi, y[2], y[3]);
+  mma(c0, a.lo, y[0], y[1]);
+  mma(c1, a.lo, y[2], y[3]);
+}
+// acc [dv][64 tokens] += A T^T (ACROSS = false: column block n over blocks k <= n) or A T (ACROSS: over k >= n) for the k-th 16
+// columns of A; T triangular, two parts.
+template <bool ACROSS>
+__device__ __forceinline__ void tri_step(float (&acc)[8][4], const Parts& a, uint32_t tri, int k) {
+#pragma unroll
+  for (int n = 0; n < 4; n++) {
+    if (ACROSS ? n > k : n < k) continue;
+    const int r = ACROSS ? k : n, c = ACROSS ? n : k;
+    const uint32_t at = tri + (r * (r + 1) / 2 + c) * 512;
+    uint32_t y[4];
+    ldsm<ACROSS>(y, at);
+    mma2(acc[2 * n], acc[2 * n + 1], a, y);
+    ldsm<ACROSS>(y, at + kTri * 2);
+    mma(acc[2 * n], a.hi, y[0], y[1]);
+    mma(acc[2 * n + 1], a.hi, y[2], y[3]);
+  }
+}
+// This lane's place in a triangular matrix's first block as B: [n][k] as it lies, or (ACROSS) [k][n].
+template <bool ACROSS>
+__device__ __forceinline__ uint32_t tri_lane(const __nv_bfloat16* t) {
+  const int lane = threadIdx.x & 31;
+  const int y = (lane & 7) + ((ACROSS ? lane >> 3 : lane >> 4) & 1) * 8, p = (ACROSS ? lane >> 4 : lane >> 3) & 1;
+  return smem_u32(t + y * 16 + ((p ^ ((y >> 2) & 1)) << 3));
+}
+// Four 8 x 8 blocks of an accumulator [dv][token] into rows of tokens: n-tiles t and t + 1, 16 values of every token.
+__device__ __forceinline__ void store_across(uint32_t at, const float (&x)[4], const float (&y)[4]) {
+  const __nv_bfloat162 v[4] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3]),
+                               __floats2bfloat162_rn(y[0], y[1]), __floats2bfloat162_rn(y[2], y[3])};
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
 }
 
 template <int NT>
