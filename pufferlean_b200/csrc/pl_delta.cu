@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArg
   long start;
   const int len = slot_chunk(a, slot, start);
   if (len == 0) return;
-  copy_tile<DK, LD, kPrepThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
-  copy_tile<DK, LD, kPrepThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
+  copy_tile<DK, LD, kPrepThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec, threadIdx.x);
+  copy_tile<DK, LD, kPrepThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec, threadIdx.x);
   cp_commit();
   cp_wait<0>();
   __syncthreads();
@@ -269,22 +269,29 @@ struct ScanArgs {
   float* final_state;
   __nv_bfloat16 *kept, *y;  // for the gradient: S and Y of every slot; or NULL
 };
-// A chunk's inputs, loaded while the chunk before it is worked on; x: v (forward), dO (back), of WARPS x 16 columns.
-template <int DK, int WARPS>
+// A chunk's inputs, loaded while the chunk before it is worked on; x: 64 columns of v (forward), of dO (back).
+template <int DK>
 struct ChainIn {
-  __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], x[kC * (WARPS * 16 + 8)];
+  __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], x[kC * kLd];
   Mats m;
+};
+constexpr int kChainThreads = 256;  // four warps for the chain, 16 columns of v each, and four that work for them
+template <int DK>
+struct ScanShared {
+  ChainIn<DK> in[2];
+  uint4 s[4][DK / 8 * 32];  // a warp's state, in two parts
+  uint4 y[4][8 * 32];       // its Y
 };
 
 // Rows that no sequence holds, in front of the first and behind the last: zero. Called by the blocks of those two.
-template <typename T>
-__device__ __forceinline__ void zero_rows(const DeltaArgs& a, int seq, T* out, long ld, int cols) {
+template <int THREADS, typename T>
+__device__ __forceinline__ void zero_rows(const DeltaArgs& a, int seq, T* out, long ld, int cols, int tid) {
   long from, to;
   seq_bounds(a, seq, from, to);
   for (int side = 0; side < 2; side++) {
     if (side ? seq != a.seqs - 1 : seq != 0) continue;
     const long r0 = side ? to : 0, r1 = side ? a.n : from;
-    for (long i = r0 * cols + threadIdx.x; i < r1 * cols; i += blockDim.x) out[i / cols * ld + i % cols] = T(0.f);
+    for (long i = r0 * cols + tid; i < r1 * cols; i += THREADS) out[i / cols * ld + i % cols] = T(0.f);
   }
 }
 
@@ -326,153 +333,193 @@ __device__ __forceinline__ void parts_out(const float (&s)[NT][4], __nv_bfloat16
       *reinterpret_cast<uint32_t*>(at + second) = lo;
     }
 }
+// The same from parts that have been made: `half` of DK / 16 fragments of a first operand.
+__device__ __forceinline__ void part_out(const uint32_t (&r)[4], __nv_bfloat16* dst, int row, int k) {
+  const int lane = threadIdx.x & 31;
+  __nv_bfloat16* at = dst + (lane >> 2) * row + k * 16 + (lane & 3) * 2;
+  *reinterpret_cast<uint32_t*>(at) = r[0];
+  *reinterpret_cast<uint32_t*>(at + 8 * row) = r[1];
+  *reinterpret_cast<uint32_t*>(at + 8) = r[2];
+  *reinterpret_cast<uint32_t*>(at + 8 * row + 8) = r[3];
+}
 // 64 rows of 16 values that this warp put at `tile`, to rows of `stride` in memory, `cols` of them.
-template <int LD>
 __device__ __forceinline__ void rows_out(const __nv_bfloat16* tile, __nv_bfloat16* dst, long stride, int len, int cols,
                                          bool vec) {
   const int lane = threadIdx.x & 31;
   if (vec && cols >= 16) {
     for (int i = lane; i < len * 2; i += 32)
       *reinterpret_cast<uint4*>(dst + (i >> 1) * stride + (i & 1) * 8) =
-          *reinterpret_cast<const uint4*>(tile + (i >> 1) * LD + (i & 1) * 8);
+          *reinterpret_cast<const uint4*>(tile + (i >> 1) * kLd + (i & 1) * 8);
   } else {
     for (int i = lane; i < len * 16; i += 32)
-      if ((i & 15) < cols) dst[(i >> 4) * stride + (i & 15)] = tile[(i >> 4) * LD + (i & 15)];
+      if ((i & 15) < cols) dst[(i >> 4) * stride + (i & 15)] = tile[(i >> 4) * kLd + (i & 15)];
   }
 }
+// Where this lane's row of n-tiles 2 n, 2 n + 1 of an accumulator [16 of dv][tokens] goes in a tile of tokens.
+__device__ __forceinline__ uint32_t across_at(const __nv_bfloat16* tile, int n) {
+  const int lane = threadIdx.x & 31;
+  return smem_u32(tile + (n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * kLd + ((lane >> 3) & 1) * 8);
+}
 
-// A block per sequence, value head and WARPS x 16 columns of v, a warp for each 16. Transposed, the state S^T [16][dk] stays in
-// a warp's registers for the whole sequence, and everything that the chunk makes of it: an accumulator's layout is that of
-// a first operand, so K S, R, Y, U and F U go from one product into the next as they are, split into two bf16 parts, and the warps
-// never wait for one another but for the inputs. (With R, Y, U and the state's parts in shared memory, shared by 16 warps in
-// four steps with barriers, a chunk of 64 columns took 5.6 us, half of it waiting for shared memory.)
-template <int DK, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 2 : 1) delta_scan_kernel(const ScanArgs p) {
+// A block per sequence, value head and 64 columns of v. A warp of the chain keeps 16 columns of the state, transposed [16][dk], in
+// registers for the whole sequence, and everything that a chunk makes of it: an accumulator's layout is that of a first
+// operand, so K S, R, Y and F U go from one product into the next as they are, split into two bf16 parts. What the next
+// chunk's state does not wait for is another warp's, which gets the state's parts and Y through shared memory: loading the next
+// chunk, Q S and P U, o, and what the gradient needs. (All in one warp, a chunk took 5.5 us; with R, Y, U and the state's
+// parts in shared memory, shared by 16 warps in four steps with barriers, 5.6.) The products are 316 and 188 of 16 x 8 x 16
+// per chunk: 8 cycles each on a quarter of an SM.
+template <int DK>
+__global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const ScanArgs p) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
-  using In = ChainIn<DK, WARPS>;
-  In* ins = reinterpret_cast<In*>(mem);
-  constexpr int LD = DK + 8, LDX = WARPS * 16 + 8, NK = DK / 8, THREADS = WARPS * 32;
+  ScanShared<DK>& sh = *reinterpret_cast<ScanShared<DK>*>(mem);
+  constexpr int LD = DK + 8, NK = DK / 8;
   const DeltaArgs& a = p.d;
-  const int c0 = blockIdx.x * WARPS * 16, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int cols = a.dv - c0 < WARPS * 16 ? a.dv - c0 : WARPS * 16;
+  const int slice = blockIdx.x, c0 = slice * 64, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3;
+  const bool chain = threadIdx.x < 128;
   const int w0 = c0 + warp * 16, mine = a.dv - w0 < 16 ? a.dv - w0 : 16;  // this warp's columns (none: <= 0)
   long from, to;
   seq_bounds(a, seq, from, to);
   const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
-  auto load = [&](long c) {
-    const long start = from + c * kC;
-    const int len = (int)(to - start < kC ? to - start : kC);
-    In& in = ins[c & 1];
-    copy_tile<DK, LD, THREADS>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
-    copy_tile<DK, LD, THREADS>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
-    copy_tile<WARPS * 16, LDX, THREADS>(in.x, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vec);
-    copy_flat<THREADS>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats));
-    cp_commit();
-  };
-  if (chunks) load(0);
-  zero_rows(a, seq, p.o + (long)h * a.dv + c0, (long)a.hv * a.dv, cols);
-  float s[NK][4];
-  const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
-  state_in(s, p.state ? p.state + sbase : nullptr, a.dk, a.dv, mine);
-  const bool vec_o = a.dv % 8 == 0 && (uintptr_t)p.o % 16 == 0;
-  const int slice = w0 / 64, row = w0 % 64;
-  for (long c = 0; c < chunks; c++) {
-    const long start = from + c * kC, slot = slot0 + c;
-    const int len = (int)(to - start < kC ? to - start : kC);
-    In& in = ins[c & 1];
-    cp_wait<0>();
-    __syncthreads();
-    if (c + 1 < chunks) load(c + 1);
-    if (w0 >= a.dvp) continue;  // (up to there the gradient's kernel reads, zeros beyond dv)
-    if (p.kept) parts_out(s, p.kept + state_at(a, slot, h, slice) + row * DK, DK, 64l * DK);
-    float r[8][4], o[8][4];  // (K S)^T, (Q S)^T: [16 of dv][64 tokens]
-    zero(r);
-    zero(o);
-    {
-      const uint32_t pk = smem_u32(in.k + lane_b<false, LD>()), pq = smem_u32(in.q + lane_b<false, LD>());
+  const int s_ready = 1 + warp, y_ready = 5 + warp;
+  if (chain) {
+    float s[NK][4];
+    const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
+    state_in(s, p.state ? p.state + sbase : nullptr, a.dk, a.dv, mine);
+    for (long c = 0; c < chunks; c++) {
+      ChainIn<DK>& in = sh.in[c & 1];
+      block_wait();
+      float r[8][4];  // (K S)^T: [16 of dv][64 tokens]
+      zero(r);
+      const uint32_t pk = smem_u32(in.k + lane_b<false, LD>());
 #pragma unroll
       for (int k = 0; k < DK / 16; k++) {
         const Parts x = parts_of(s[2 * k], s[2 * k + 1]);
+        give(sh.s[warp], 2 * k, x.hi);
+        give(sh.s[warp], 2 * k + 1, x.lo);
+        step<false, 4>(r, x, pk + k * 32, 32 * LD);
+      }
+      pair_arrive(s_ready);
+      const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>());
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-          uint32_t y[4];
-          ldsm<false>(y, pk + n * 32 * LD + k * 32);
-          mma2(r[2 * n], r[2 * n + 1], x, y);
-          ldsm<false>(y, pq + n * 32 * LD + k * 32);
-          mma2(o[2 * n], o[2 * n + 1], x, y);
+      for (int n = 0; n < 4; n++) {  // R = V - E K S
+        uint32_t v[4];
+        ldsm<true>(v, px + n * 32 * kLd);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const float2 f = *reinterpret_cast<const float2*>(in.m.since + n * 16 + t * 8 + (lane & 3) * 2);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float fe = e & 1 ? f.y : f.x;
+            const uint32_t vv = v[t * 2 + (e >> 1)];
+            float(&rr)[4] = r[2 * n + t];
+            rr[e] = __uint_as_float(e & 1 ? vv & 0xffff0000u : vv << 16) - (fe == 0.f ? 0.f : fe * rr[e]);
+          }
         }
       }
-    }
-    const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, LDX>());
+      float y[8][4];  // Y^T = R^T X^T
+      zero(y);
+      const uint32_t tx = tri_lane<false>(in.m.x[0]);
 #pragma unroll
-    for (int n = 0; n < 4; n++) {  // R = V - E K S, E Q S
-      uint32_t v[4];
-      ldsm<true>(v, px + n * 32 * LDX);
+      for (int k = 0; k < 4; k++) tri_step<false>(y, parts_of(r[2 * k], r[2 * k + 1]), tx, k);
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const float2 f = *reinterpret_cast<const float2*>(in.m.since + n * 16 + t * 8 + (lane & 3) * 2);
+      for (int t = 0; t < 8; t++) give(sh.y[warp], t, y[t]);
+      pair_arrive(y_ready);
+      const float keep = in.m.since[kC - 1];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float fe = e & 1 ? f.y : f.x;
-          const uint32_t vv = v[t * 2 + (e >> 1)];
-          float(&rr)[4] = r[2 * n + t], (&oo)[4] = o[2 * n + t];
-          rr[e] = __uint_as_float(e & 1 ? vv & 0xffff0000u : vv << 16) - (fe == 0.f ? 0.f : fe * rr[e]);
-          oo[e] = fe == 0.f ? 0.f : fe * oo[e];
+      for (int t = 0; t < NK; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
+      const uint32_t pt = smem_u32(in.k + lane_b<true, LD>());
+#pragma unroll
+      for (int k = 0; k < 4; k++) {  // S^T += (F U)^T K
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const float2 f = *reinterpret_cast<const float2*>(in.m.until + k * 16 + t * 8 + (lane & 3) * 2);
+          const float2 b = *reinterpret_cast<const float2*>(in.m.beta + k * 16 + t * 8 + (lane & 3) * 2);
+          float(&u)[4] = y[2 * k + t];
+          u[0] *= f.x * b.x, u[2] *= f.x * b.x;
+          u[1] *= f.y * b.y, u[3] *= f.y * b.y;
         }
+        step<true, DK / 16>(s, parts_of(y[2 * k], y[2 * k + 1]), pt + k * 32 * LD, 32);
       }
     }
-    float y[8][4];  // Y^T = R^T X^T
-    zero(y);
-    const uint32_t tx = tri_lane<false>(in.m.x[0]), tp = tri_lane<false>(in.m.p[0]);
+    state_out(s, p.final_state + sbase, a.dk, a.dv, mine);
+    return;
+  }
+  // the chain's helpers
+  const int tid = threadIdx.x - 128, cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
+  auto load = [&](long c) {
+    const long start = from + c * kC;
+    const int len = (int)(to - start < kC ? to - start : kC);
+    ChainIn<DK>& in = sh.in[c & 1];
+    copy_tile<DK, LD, 128>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec, tid);
+    copy_tile<64, kLd, 128>(in.x, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vec, tid);
+    copy_flat<128>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats), tid);
+    copy_tile<DK, LD, 128>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec, tid);
+    cp_commit();
+  };
+  if (chunks) load(0);
+  zero_rows<128>(a, seq, p.o + (long)h * a.dv + c0, (long)a.hv * a.dv, cols, tid);
+  const bool vec_o = a.dv % 8 == 0 && (uintptr_t)p.o % 16 == 0;
+  for (long c = 0; c < chunks; c++) {
+    const long start = from + c * kC, slot = slot0 + c;
+    const int len = (int)(to - start < kC ? to - start : kC);
+    ChainIn<DK>& in = sh.in[c & 1];
+    cp_wait<0>();
+    block_wait();
+    if (c + 1 < chunks) load(c + 1);
+    float o[8][4];  // (Q S)^T
+    zero(o);
+    const uint32_t pq = smem_u32(in.q + lane_b<false, LD>());
+    pair_wait(s_ready);
 #pragma unroll
-    for (int k = 0; k < 4; k++) tri_step<false>(y, parts_of(r[2 * k], r[2 * k + 1]), tx, k);
-    if (p.y) parts_out(y, p.y + rows_at(a, slot, h, slice) + row * 64, 64, 64l * 64);
+    for (int k = 0; k < DK / 16; k++) {
+      Parts x;
+      take(sh.s[warp], 2 * k, x.hi);
+      take(sh.s[warp], 2 * k + 1, x.lo);
+      if (p.kept) {
+        __nv_bfloat16* to_s = p.kept + state_at(a, slot, h, slice) + warp * 16 * DK;
+        part_out(x.hi, to_s, DK, k);
+        part_out(x.lo, to_s + 64 * DK, DK, k);
+      }
+      step<false, 4>(o, x, pq + k * 32, 32 * LD);
+    }
+#pragma unroll
+    for (int t = 0; t < 8; t++) {
+      const float2 f = *reinterpret_cast<const float2*>(in.m.since + t * 8 + (lane & 3) * 2);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float fe = e & 1 ? f.y : f.x;
+        o[t][e] = fe == 0.f ? 0.f : fe * o[t][e];
+      }
+    }
+    float y[8][4];
+    pair_wait(y_ready);
+#pragma unroll
+    for (int t = 0; t < 8; t++) take(sh.y[warp], t, y[t]);
+    if (p.y) parts_out(y, p.y + rows_at(a, slot, h, slice) + warp * 16 * 64, 64, 64l * 64);
 #pragma unroll
     for (int t = 0; t < 8; t++) {  // U
       const float2 b = *reinterpret_cast<const float2*>(in.m.beta + t * 8 + (lane & 3) * 2);
       y[t][0] *= b.x, y[t][2] *= b.x;
       y[t][1] *= b.y, y[t][3] *= b.y;
     }
+    const uint32_t tp = tri_lane<false>(in.m.p[0]);
 #pragma unroll
     for (int k = 0; k < 4; k++) tri_step<false>(o, parts_of(y[2 * k], y[2 * k + 1]), tp, k);
-    __syncwarp();  // the warp's columns of v have been read: o takes their place on its way out
+    // the chain has read these columns of v before it gave Y: o takes their place on its way out
 #pragma unroll
     for (int n = 0; n < 4; n++) {
 #pragma unroll
       for (int e = 0; e < 4; e++) o[2 * n][e] *= a.scale, o[2 * n + 1][e] *= a.scale;
-      store_across(smem_u32(in.x + (n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * LDX + warp * 16 + ((lane >> 3) & 1) * 8),
-                   o[2 * n], o[2 * n + 1]);
+      store_across(across_at(in.x + warp * 16, n), o[2 * n], o[2 * n + 1]);
     }
     __syncwarp();
-    rows_out<LDX>(in.x + warp * 16, p.o + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_o);
-    const float keep = in.m.since[kC - 1];
-#pragma unroll
-    for (int t = 0; t < NK; t++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-    const uint32_t pk = smem_u32(in.k + lane_b<true, LD>());
-#pragma unroll
-    for (int k = 0; k < 4; k++) {  // S^T += (F U)^T K
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const float2 f = *reinterpret_cast<const float2*>(in.m.until + k * 16 + t * 8 + (lane & 3) * 2);
-        float(&u)[4] = y[2 * k + t];
-        u[0] *= f.x, u[2] *= f.x;
-        u[1] *= f.y, u[3] *= f.y;
-      }
-      const Parts x = parts_of(y[2 * k], y[2 * k + 1]);
-#pragma unroll
-      for (int n = 0; n < DK / 16; n++) {
-        uint32_t b[4];
-        ldsm<true>(b, pk + k * 32 * LD + n * 32);
-        mma2(s[2 * n], s[2 * n + 1], x, b);
-      }
-    }
+    rows_out(in.x + warp * 16, p.o + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_o);
   }
-  state_out(s, p.final_state + sbase, a.dk, a.dv, mine);
 }
 
 // ---------------------------------------------------------------------------------------------- the chain back
@@ -487,136 +534,184 @@ struct BackArgs {
   float* dstate;              // or NULL
   __nv_bfloat16 *ds, *dr;     // dS' and dR of every slot
 };
-// As the chain forward, from the last chunk to the first.
-template <int DK, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 2 : 1) delta_back_kernel(const BackArgs p) {
+template <int DK>
+struct BackShared {
+  ChainIn<DK> in[2];
+  uint4 s[4][DK / 8 * 32];  // a warp's dS', in two parts
+  uint4 x[4][8 * 32];       // scale P^T dO from the helper, then dR to it
+  uint4 q[4][DK / 8 * 32];  // scale (E dO)^T Q from the helper
+};
+// As the chain forward, from the last chunk to the first. The helpers' products, of dO with P and Q, need nothing of the chain.
+template <int DK>
+__global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const BackArgs p) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
-  using In = ChainIn<DK, WARPS>;
-  In* ins = reinterpret_cast<In*>(mem);
-  constexpr int LD = DK + 8, LDX = WARPS * 16 + 8, NK = DK / 8, THREADS = WARPS * 32;
+  BackShared<DK>& sh = *reinterpret_cast<BackShared<DK>*>(mem);
+  constexpr int LD = DK + 8, NK = DK / 8;
   const DeltaArgs& a = p.d;
-  const int c0 = blockIdx.x * WARPS * 16, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int cols = a.dv - c0 < WARPS * 16 ? a.dv - c0 : WARPS * 16;
+  const int slice = blockIdx.x, c0 = slice * 64, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3;
+  const bool chain = threadIdx.x < 128;
   const int w0 = c0 + warp * 16, mine = a.dv - w0 < 16 ? a.dv - w0 : 16;
   long from, to;
   seq_bounds(a, seq, from, to);
   const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
-  auto load = [&](long c) {
-    const long start = from + c * kC;
-    const int len = (int)(to - start < kC ? to - start : kC);
-    In& in = ins[c & 1];
-    copy_tile<DK, LD, THREADS>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
-    copy_tile<DK, LD, THREADS>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
-    copy_tile<WARPS * 16, LDX, THREADS>(in.x, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
-    copy_flat<THREADS>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats));
-    cp_commit();
-  };
-  if (chunks) load(chunks - 1);
-  zero_rows(a, seq, p.dv + (long)h * a.dv + c0, (long)a.hv * a.dv, cols);
-  float s[NK][4];  // dS'^T
-  const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
-  state_in(s, p.dfinal ? p.dfinal + sbase : nullptr, a.dk, a.dv, mine);
-  const bool vec_dv = a.dv % 8 == 0 && (uintptr_t)p.dv % 16 == 0;
-  const int slice = w0 / 64, row = w0 % 64;
-  for (long c = chunks - 1; c >= 0; c--) {
-    const long start = from + c * kC, slot = slot0 + c;
-    const int len = (int)(to - start < kC ? to - start : kC);
-    In& in = ins[c & 1];
-    cp_wait<0>();
-    __syncthreads();
-    if (c > 0) load(c - 1);
-    if (w0 >= a.dvp) continue;  // (up to there the gradient's kernel reads, zeros beyond dv)
-    parts_out(s, p.ds + state_at(a, slot, h, slice) + row * DK, DK, 64l * DK);
-    float u[8][4], x[8][4];  // (P^T dO)^T, (K dS')^T: [16 of dv][64 tokens]
-    zero(u);
-    zero(x);
-    const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, LDX>());
-    const uint32_t tx = tri_lane<true>(in.m.x[0]), tp = tri_lane<true>(in.m.p[0]);
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      uint32_t o[4];
-      ldsm<true>(o, px + k * 32 * LDX);
-#pragma unroll
-      for (int n = 0; n <= k; n++)
-#pragma unroll
-        for (int part = 0; part < 2; part++) {
-          uint32_t y[4];
-          ldsm<true>(y, tp + (k * (k + 1) / 2 + n) * 512 + part * kTri * 2);
-          mma(u[2 * n], o, y[0], y[1]);
-          mma(u[2 * n + 1], o, y[2], y[3]);
-        }
-    }
-    {
+  const int u_ready = 1 + warp, q_ready = 5 + warp, r_ready = 9 + warp;
+  if (chain) {
+    float s[NK][4];  // dS'^T
+    const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
+    state_in(s, p.dfinal ? p.dfinal + sbase : nullptr, a.dk, a.dv, mine);
+    for (long c = chunks - 1; c >= 0; c--) {
+      ChainIn<DK>& in = sh.in[c & 1];
+      block_wait();
+      float x[8][4];  // (K dS')^T: [16 of dv][64 tokens]
+      zero(x);
       const uint32_t pk = smem_u32(in.k + lane_b<false, LD>());
 #pragma unroll
       for (int k = 0; k < DK / 16; k++) {
         const Parts z = parts_of(s[2 * k], s[2 * k + 1]);
-#pragma unroll
-        for (int n = 0; n < 4; n++) {
-          uint32_t y[4];
-          ldsm<false>(y, pk + n * 32 * LD + k * 32);
-          mma2(x[2 * n], x[2 * n + 1], z, y);
-        }
+        give(sh.s[warp], 2 * k, z.hi);
+        give(sh.s[warp], 2 * k + 1, z.lo);
+        step<false, 4>(x, z, pk + k * 32, 32 * LD);
       }
-    }
+      pair_wait(u_ready);
 #pragma unroll
-    for (int t = 0; t < 8; t++) {  // beta dU = beta (F K dS' + scale P^T dO)
-      const float2 b = *reinterpret_cast<const float2*>(in.m.beta + t * 8 + (lane & 3) * 2);
-      const float2 f = *reinterpret_cast<const float2*>(in.m.until + t * 8 + (lane & 3) * 2);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float fe = e & 1 ? f.y : f.x, be = e & 1 ? b.y : b.x;
-        u[t][e] = be * ((fe == 0.f ? 0.f : fe * x[t][e]) + a.scale * u[t][e]);
-      }
-    }
-    zero(x);  // dR^T = (beta dU)^T X
-#pragma unroll
-    for (int k = 0; k < 4; k++) tri_step<true>(x, parts_of(u[2 * k], u[2 * k + 1]), tx, k);
-    parts_out(x, p.dr + rows_at(a, slot, h, slice) + row * 64, 64, 64l * 64);
-    const float keep = in.m.since[kC - 1];
-#pragma unroll
-    for (int t = 0; t < NK; t++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-    const uint32_t pk = smem_u32(in.k + lane_b<true, LD>()), pq = smem_u32(in.q + lane_b<true, LD>());
-#pragma unroll
-    for (int k = 0; k < 4; k++) {  // dS^T += scale (E dO)^T Q - (E dR)^T K
-      uint32_t o[4];
-      ldsm<true>(o, px + k * 32 * LDX);
-      float eo[2][4], er[2][4];
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const float2 f = *reinterpret_cast<const float2*>(in.m.since + k * 16 + t * 8 + (lane & 3) * 2);
+      for (int t = 0; t < 8; t++) {  // beta dU = beta (F K dS' + scale P^T dO)
+        const float2 b = *reinterpret_cast<const float2*>(in.m.beta + t * 8 + (lane & 3) * 2);
+        const float2 f = *reinterpret_cast<const float2*>(in.m.until + t * 8 + (lane & 3) * 2);
+        float u[4];
+        take(sh.x[warp], t, u);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float fe = e & 1 ? f.y : f.x;
-          const uint32_t oo = o[t * 2 + (e >> 1)];
-          eo[t][e] = fe == 0.f ? 0.f : a.scale * fe * __uint_as_float(e & 1 ? oo & 0xffff0000u : oo << 16);
-          er[t][e] = fe == 0.f ? 0.f : -fe * x[2 * k + t][e];
+          const float fe = e & 1 ? f.y : f.x, be = e & 1 ? b.y : b.x;
+          x[t][e] = be * ((fe == 0.f ? 0.f : fe * x[t][e]) + u[e]);
         }
       }
-      const Parts po = parts_of(eo[0], eo[1]), pr = parts_of(er[0], er[1]);
+      float r[8][4];  // dR^T = (beta dU)^T X
+      zero(r);
+      const uint32_t tx = tri_lane<true>(in.m.x[0]);
 #pragma unroll
-      for (int n = 0; n < DK / 16; n++) {
-        uint32_t b[4];
-        ldsm<true>(b, pq + k * 32 * LD + n * 32);
-        mma2(s[2 * n], s[2 * n + 1], po, b);
-        ldsm<true>(b, pk + k * 32 * LD + n * 32);
-        mma2(s[2 * n], s[2 * n + 1], pr, b);
+      for (int k = 0; k < 4; k++) tri_step<true>(r, parts_of(x[2 * k], x[2 * k + 1]), tx, k);
+#pragma unroll
+      for (int t = 0; t < 8; t++) give(sh.x[warp], t, r[t]);
+      pair_arrive(r_ready);
+      const float keep = in.m.since[kC - 1];
+#pragma unroll
+      for (int t = 0; t < NK; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
+      const uint32_t pt = smem_u32(in.k + lane_b<true, LD>());
+#pragma unroll
+      for (int k = 0; k < 4; k++) {  // dS^T -= (E dR)^T K
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const float2 f = *reinterpret_cast<const float2*>(in.m.since + k * 16 + t * 8 + (lane & 3) * 2);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float fe = e & 1 ? f.y : f.x;
+            r[2 * k + t][e] = fe == 0.f ? 0.f : -fe * r[2 * k + t][e];
+          }
+        }
+        step<true, DK / 16>(s, parts_of(r[2 * k], r[2 * k + 1]), pt + k * 32 * LD, 32);
+      }
+      pair_wait(q_ready);
+#pragma unroll
+      for (int t = 0; t < NK; t++) {
+        float q[4];
+        take(sh.q[warp], t, q);
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[t][e] += q[e];
       }
     }
-    __syncwarp();  // the warp's columns of dO have been read: dv takes their place on its way out
-#pragma unroll
-    for (int n = 0; n < 4; n++)
-      store_across(smem_u32(in.x + (n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * LDX + warp * 16 + ((lane >> 3) & 1) * 8),
-                   x[2 * n], x[2 * n + 1]);
-    __syncwarp();
-    rows_out<LDX>(in.x + warp * 16, p.dv + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_dv);
+    if (p.dstate) state_out(s, p.dstate + sbase, a.dk, a.dv, mine);
+    return;
   }
-  if (p.dstate) state_out(s, p.dstate + sbase, a.dk, a.dv, mine);
+  const int tid = threadIdx.x - 128, cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
+  auto load = [&](long c) {
+    const long start = from + c * kC;
+    const int len = (int)(to - start < kC ? to - start : kC);
+    ChainIn<DK>& in = sh.in[c & 1];
+    copy_tile<DK, LD, 128>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec, tid);
+    copy_flat<128>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats), tid);
+    copy_tile<64, kLd, 128>(in.x, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o, tid);
+    copy_tile<DK, LD, 128>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec, tid);
+    cp_commit();
+  };
+  if (chunks) load(chunks - 1);
+  zero_rows<128>(a, seq, p.dv + (long)h * a.dv + c0, (long)a.hv * a.dv, cols, tid);
+  const bool vec_dv = a.dv % 8 == 0 && (uintptr_t)p.dv % 16 == 0;
+  for (long c = chunks - 1; c >= 0; c--) {
+    const long start = from + c * kC, slot = slot0 + c;
+    const int len = (int)(to - start < kC ? to - start : kC);
+    ChainIn<DK>& in = sh.in[c & 1];
+    cp_wait<0>();
+    block_wait();
+    const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>());
+    uint32_t o[4][4];  // dO^T: [16 of dv][64 tokens]
+#pragma unroll
+    for (int k = 0; k < 4; k++) ldsm<true>(o[k], px + k * 32 * kLd);
+    float u[8][4];  // (P^T dO)^T
+    zero(u);
+    const uint32_t tp = tri_lane<true>(in.m.p[0]);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      Parts x;
+#pragma unroll
+      for (int e = 0; e < 4; e++) x.hi[e] = o[k][e];
+      tri_step<true, false>(u, x, tp, k);
+    }
+#pragma unroll
+    for (int t = 0; t < 8; t++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) u[t][e] *= a.scale;
+      give(sh.x[warp], t, u[t]);
+    }
+    pair_arrive(u_ready);
+    if (c > 0) load(c - 1);
+    {
+      float q[NK][4];
+      zero(q);
+      const uint32_t pq = smem_u32(in.q + lane_b<true, LD>());
+#pragma unroll
+      for (int k = 0; k < 4; k++) {  // scale (E dO)^T Q
+        float eo[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const float2 f = *reinterpret_cast<const float2*>(in.m.since + k * 16 + t * 8 + (lane & 3) * 2);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float fe = e & 1 ? f.y : f.x;
+            const uint32_t oo = o[k][t * 2 + (e >> 1)];
+            eo[t][e] = fe == 0.f ? 0.f : a.scale * fe * __uint_as_float(e & 1 ? oo & 0xffff0000u : oo << 16);
+          }
+        }
+        step<true, DK / 16>(q, parts_of(eo[0], eo[1]), pq + k * 32 * LD, 32);
+      }
+#pragma unroll
+      for (int t = 0; t < NK; t++) give(sh.q[warp], t, q[t]);
+      pair_arrive(q_ready);
+    }
+    float r[8][4];
+    pair_wait(r_ready);
+#pragma unroll
+    for (int k = 0; k < DK / 16; k++) {
+      __nv_bfloat16* to_s = p.ds + state_at(a, slot, h, slice) + warp * 16 * DK;
+      uint32_t x[4];
+      take(sh.s[warp], 2 * k, x);
+      part_out(x, to_s, DK, k);
+      take(sh.s[warp], 2 * k + 1, x);
+      part_out(x, to_s + 64 * DK, DK, k);
+    }
+#pragma unroll
+    for (int t = 0; t < 8; t++) take(sh.x[warp], t, r[t]);
+    parts_out(r, p.dr + rows_at(a, slot, h, slice) + warp * 16 * 64, 64, 64l * 64);
+    // dv takes the place of these columns of dO, which this warp alone has read, on its way out
+#pragma unroll
+    for (int n = 0; n < 4; n++) store_across(across_at(in.x + warp * 16, n), r[2 * n], r[2 * n + 1]);
+    __syncwarp();
+    rows_out(in.x + warp * 16, p.dv + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_dv);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- the other gradients
@@ -661,7 +756,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
   auto load_a = [&](int t) {  // S, dO, dR
     const int h = kh * group + t / slices, slice = t % slices, c0 = slice * 64;
     const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-    copy_tile<64, kLd, kGradThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o);
+    copy_tile<64, kLd, kGradThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o, tid);
 #pragma unroll
     for (int part = 0; part < 2; part++) {
       tile_in<DK, LD, kGradThreads>(sh.s[part], p.kept + state_at(a, slot, h, slice) + part * 64 * DK);
@@ -678,8 +773,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     }
     cp_commit();
   };
-  copy_tile<DK, LD, kGradThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec);
-  copy_tile<DK, LD, kGradThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec);
+  copy_tile<DK, LD, kGradThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec, tid);
+  copy_tile<DK, LD, kGradThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec, tid);
   load_a(0);
   load_b(0);
   const int wr = warp & 3, wc = warp >> 2, m0 = wr * 16, i0 = m0 + (lane >> 2);
@@ -961,12 +1056,6 @@ static int launch_wide(void (*kernel)(A), dim3 grid, int threads, size_t smem, c
   count_launch();
   return PL_OK;
 }
-// A chain takes 128 columns of v per block if there are that many and enough chains to fill the SMs that way (K and Q are
-// read once for 128 columns then), 64 otherwise.
-static bool wide_chains(const DeltaArgs& a) { return a.dv > 64 && (long)a.seqs * a.hv * (a.dvp / 64) > 148; }
-static dim3 chain_grid(const DeltaArgs& a, bool wide) {
-  return dim3((unsigned)ceil_div(a.dv, wide ? 128 : 64), (unsigned)a.hv, (unsigned)a.seqs);
-}
 static int prep(const DeltaArgs& a, Mats* mats, cudaStream_t st) {
   const dim3 grid((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
   const bool wide = a.dk > 64;
@@ -1030,13 +1119,9 @@ int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const vo
     p.kept = (__nv_bfloat16*)saved;
     p.y = (__nv_bfloat16*)((char*)saved + states_bytes(s));
   }
-  const bool wide = wide_chains(a);
-  const dim3 grid = chain_grid(a, wide);
-  if (a.dk > 64)
-    return wide ? launch_wide(delta_scan_kernel<128, 8>, grid, 256, 2 * sizeof(ChainIn<128, 8>), st, p)
-                : launch_wide(delta_scan_kernel<128, 4>, grid, 128, 2 * sizeof(ChainIn<128, 4>), st, p);
-  return wide ? launch_wide(delta_scan_kernel<64, 8>, grid, 256, 2 * sizeof(ChainIn<64, 8>), st, p)
-              : launch_wide(delta_scan_kernel<64, 4>, grid, 128, 2 * sizeof(ChainIn<64, 4>), st, p);
+  const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
+  return a.dk > 64 ? launch_wide(delta_scan_kernel<128>, grid, kChainThreads, sizeof(ScanShared<128>), st, p)
+                   : launch_wide(delta_scan_kernel<64>, grid, kChainThreads, sizeof(ScanShared<64>), st, p);
 }
 
 int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token, size_t do_head, const float* dfinal,
@@ -1070,14 +1155,9 @@ int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token
   }
   const BackArgs b = {a, (const Mats*)ws, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, dfinal,
                       (__nv_bfloat16*)dv, dstate, ds, dr};
-  const bool wide = wide_chains(a);
-  const dim3 grid = chain_grid(a, wide);
-  if (a.dk > 64)
-    rc = wide ? launch_wide(delta_back_kernel<128, 8>, grid, 256, 2 * sizeof(ChainIn<128, 8>), st, b)
-              : launch_wide(delta_back_kernel<128, 4>, grid, 128, 2 * sizeof(ChainIn<128, 4>), st, b);
-  else
-    rc = wide ? launch_wide(delta_back_kernel<64, 8>, grid, 256, 2 * sizeof(ChainIn<64, 8>), st, b)
-              : launch_wide(delta_back_kernel<64, 4>, grid, 128, 2 * sizeof(ChainIn<64, 4>), st, b);
+  const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
+  rc = a.dk > 64 ? launch_wide(delta_back_kernel<128>, grid, kChainThreads, sizeof(BackShared<128>), st, b)
+                 : launch_wide(delta_back_kernel<64>, grid, kChainThreads, sizeof(BackShared<64>), st, b);
   if (rc || s->tokens == 0) return rc;
   const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, (const __nv_bfloat16*)saved,
                       (const __nv_bfloat16*)((const char*)saved + states_bytes(s)), ds, dr, (__nv_bfloat16*)dq, (__nv_bfloat16*)dk,

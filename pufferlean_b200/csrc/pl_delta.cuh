@@ -69,16 +69,16 @@ __device__ __forceinline__ void cp_wait() {
 // vec the copies are asynchronous (cp_commit, cp_wait); without, plain stores.
 template <int COLS, int LD, int THREADS>
 __device__ __forceinline__ void copy_tile(__nv_bfloat16* dst, const __nv_bfloat16* src, long stride, int rows, int cols,
-                                          bool vec) {
+                                          bool vec, int tid) {
   if (vec) {
-    for (int i = threadIdx.x; i < kC * (COLS / 8); i += THREADS) {
+    for (int i = tid; i < kC * (COLS / 8); i += THREADS) {
       const int r = i / (COLS / 8), c = i % (COLS / 8) * 8;
       int bytes = r < rows ? (cols - c) * 2 : 0;
       bytes = bytes < 0 ? 0 : bytes > 16 ? 16 : bytes;
       cp16(dst + r * LD + c, bytes ? src + (long)r * stride + c : src, bytes);
     }
   } else {
-    for (int i = threadIdx.x; i < kC * COLS; i += THREADS) {
+    for (int i = tid; i < kC * COLS; i += THREADS) {
       const int r = i / COLS, c = i % COLS;
       dst[r * LD + c] = r < rows && c < cols ? src[(long)r * stride + c] : __float2bfloat16_rn(0.f);
     }
@@ -87,8 +87,8 @@ __device__ __forceinline__ void copy_tile(__nv_bfloat16* dst, const __nv_bfloat1
 
 // n bytes (a multiple of 16) as they lie.
 template <int THREADS>
-__device__ __forceinline__ void copy_flat(void* dst, const void* src, int n) {
-  for (int i = threadIdx.x * 16; i < n; i += THREADS * 16) cp16((char*)dst + i, (const char*)src + i, 16);
+__device__ __forceinline__ void copy_flat(void* dst, const void* src, int n, int tid) {
+  for (int i = tid * 16; i < n; i += THREADS * 16) cp16((char*)dst + i, (const char*)src + i, 16);
 }
 // 64 rows of COLS values, one behind the other in memory, into a tile of row stride LD.
 template <int COLS, int LD, int THREADS>
@@ -212,30 +212,70 @@ __device__ __forceinline__ Parts parts_of(const float (&x)[4], const float (&y)[
   split2(y[2], y[3], p.hi[3], p.lo[3]);
   return p;
 }
-// c[0], c[1] (two n-tiles) += A B, B bf16 as it is / in two parts (y, yl).
-__device__ __forceinline__ void mma2(float (&c0)[4], float (&c1)[4], const Parts& a, const uint32_t (&y)[4]) {
-  mma(c0, a.hi, y[0], y[1]);
-  mma(c1, a.hi, y[2], y[3]);
-  mma(c0, a.lo, y[0], y[1]);
-  mma(c1, a.lo, y[2], y[3]);
+// acc [16][16 N] += A B for one 16 of k: B bf16, at `at` and every `step` bytes. All first parts go before the second ones:
+// a product waits 25 cycles for the one before it on the same accumulator, and N of them take 8 N.
+template <bool ACROSS, int N>
+__device__ __forceinline__ void step(float (&acc)[2 * N][4], const Parts& a, uint32_t at, int step) {
+  uint32_t y[N][4];
+#pragma unroll
+  for (int n = 0; n < N; n++) ldsm<ACROSS>(y[n], at + n * step);
+#pragma unroll
+  for (int n = 0; n < N; n++) {
+    mma(acc[2 * n], a.hi, y[n][0], y[n][1]);
+    mma(acc[2 * n + 1], a.hi, y[n][2], y[n][3]);
+  }
+#pragma unroll
+  for (int n = 0; n < N; n++) {
+    mma(acc[2 * n], a.lo, y[n][0], y[n][1]);
+    mma(acc[2 * n + 1], a.lo, y[n][2], y[n][3]);
+  }
 }
 // acc [dv][64 tokens] += A T^T (ACROSS = false: column block n over blocks k <= n) or A T (ACROSS: over k >= n) for the k-th 16
-// columns of A; T triangular, two parts.
-template <bool ACROSS>
+// columns of A; T triangular, two parts; A two parts or (TWO = false) its first alone.
+template <bool ACROSS, bool TWO = true>
 __device__ __forceinline__ void tri_step(float (&acc)[8][4], const Parts& a, uint32_t tri, int k) {
+  uint32_t y[4][4], z[4][4];
 #pragma unroll
   for (int n = 0; n < 4; n++) {
     if (ACROSS ? n > k : n < k) continue;
     const int r = ACROSS ? k : n, c = ACROSS ? n : k;
     const uint32_t at = tri + (r * (r + 1) / 2 + c) * 512;
-    uint32_t y[4];
-    ldsm<ACROSS>(y, at);
-    mma2(acc[2 * n], acc[2 * n + 1], a, y);
-    ldsm<ACROSS>(y, at + kTri * 2);
-    mma(acc[2 * n], a.hi, y[0], y[1]);
-    mma(acc[2 * n + 1], a.hi, y[2], y[3]);
+    ldsm<ACROSS>(y[n], at);
+    ldsm<ACROSS>(z[n], at + kTri * 2);
   }
+#pragma unroll
+  for (int part = 0; part < 3; part++)
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      if ((ACROSS ? n > k : n < k) || (part == 1 && !TWO)) continue;
+      const uint32_t(&x)[4] = part == 1 ? a.lo : a.hi;
+      const uint32_t(&b)[4] = part == 2 ? z[n] : y[n];
+      mma(acc[2 * n], x, b[0], b[1]);
+      mma(acc[2 * n + 1], x, b[2], b[3]);
+    }
 }
+// Registers of one warp for another one's same lanes: pieces of 16 bytes per lane at `at`.
+__device__ __forceinline__ void give(uint4* at, int piece, const uint32_t (&r)[4]) {
+  at[piece * 32 + (threadIdx.x & 31)] = make_uint4(r[0], r[1], r[2], r[3]);
+}
+__device__ __forceinline__ void give(uint4* at, int piece, const float (&r)[4]) {
+  at[piece * 32 + (threadIdx.x & 31)] =
+      make_uint4(__float_as_uint(r[0]), __float_as_uint(r[1]), __float_as_uint(r[2]), __float_as_uint(r[3]));
+}
+__device__ __forceinline__ void take(const uint4* at, int piece, uint32_t (&r)[4]) {
+  const uint4 v = at[piece * 32 + (threadIdx.x & 31)];
+  r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
+}
+__device__ __forceinline__ void take(const uint4* at, int piece, float (&r)[4]) {
+  const uint4 v = at[piece * 32 + (threadIdx.x & 31)];
+  r[0] = __uint_as_float(v.x), r[1] = __uint_as_float(v.y), r[2] = __uint_as_float(v.z), r[3] = __uint_as_float(v.w);
+}
+// Barrier `id` of two warps: what the one wrote before it arrives, the other sees after it waits.
+__device__ __forceinline__ void pair_arrive(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
+// All 256 threads of a chain's block, from two places in the code.
+__device__ __forceinline__ void block_wait() { asm volatile("bar.sync 15, 256;" ::: "memory"); }
+__device__ __forceinline__ void pair_wait(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
 // This lane's place in a triangular matrix's first block as B: [n][k] as it lies, or (ACROSS) [k][n].
 template <bool ACROSS>
 __device__ __forceinline__ uint32_t tri_lane(const __nv_bfloat16* t) {
