@@ -140,14 +140,59 @@ struct __align__(16) Mats {
 constexpr int kPrepThreads = 128;
 template <int DK>
 struct PrepShared {
-  __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)];
-  float at[kC][kC + 4];  // N diag(beta), transposed: [j][i]
-  float x[kC][kC + 4];   // its inverse with I
-  float y[32][36];
+  union {
+    struct {
+      __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)];
+    };
+    struct {  // when K K^T and Q K^T are in registers
+      float at[kC][kC + 4];  // N diag(beta), transposed: [j][i]; above its diagonal, nothing is read
+      float x[kC][kC + 4];   // its inverse with I
+      float y[32][36];
+    };
+  };
   Decay d;
 };
+// out = -B (A C) for square blocks of S rows: A = at (transposed) at (r, c), C = x at (c, c), B = x at (r, r), out = x at (r, c); `n`
+// threads per block, thread t of it, `y` for A C.
+template <int S, int N, typename Shared>
+__device__ __forceinline__ void inverse_block(Shared& sh, float (*y)[36], int r, int c, int t) {
+  constexpr int E = S * S / N, P = S / E;  // values per thread, threads per row
+  const int i = t / P, j0 = t % P * E;
+  float s[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) s[e] = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < S; k++) {
+    const float f = sh.at[c + k][r + i];
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(&sh.x[c + k][c + j0 + e]);
+      s[e] = __fmaf_rn(f, v.x, s[e]), s[e + 1] = __fmaf_rn(f, v.y, s[e + 1]);
+      s[e + 2] = __fmaf_rn(f, v.z, s[e + 2]), s[e + 3] = __fmaf_rn(f, v.w, s[e + 3]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(&y[i][j0 + e]) = make_float4(s[e], s[e + 1], s[e + 2], s[e + 3]);
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; e++) s[e] = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < S; k++) {
+    const float f = -sh.x[r + i][r + k];
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(&y[k][j0 + e]);
+      s[e] = __fmaf_rn(f, v.x, s[e]), s[e + 1] = __fmaf_rn(f, v.y, s[e + 1]);
+      s[e + 2] = __fmaf_rn(f, v.z, s[e + 2]), s[e + 3] = __fmaf_rn(f, v.w, s[e + 3]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; e += 4)
+    *reinterpret_cast<float4*>(&sh.x[r + i][c + j0 + e]) = make_float4(s[e], s[e + 1], s[e + 2], s[e + 3]);
+  __syncthreads();
+}
 template <int DK>
-__global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArgs a, Mats* __restrict__ mats) {
+__global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const DeltaArgs a, Mats* __restrict__ mats) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
@@ -158,95 +203,89 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaArg
   long start;
   const int len = slot_chunk(a, slot, start);
   if (len == 0) return;
-  copy_tile<DK, LD, kPrepThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec, threadIdx.x);
-  copy_tile<DK, LD, kPrepThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec, threadIdx.x);
+  copy_tile<DK, LD, kPrepThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vk, tid);
+  copy_tile<DK, LD, kPrepThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
   cp_commit();
+  chunk_decay(a, sh.d, start, len, kh * group);
   cp_wait<0>();
   __syncthreads();
-  float kk[8][4], qk[8][4];  // rows 16 warp.. of K K^T and Q K^T
+  float kk[8][4], qk[8][4];  // rows 16 warp.. of K K^T and Q K^T, up to the diagonal's block
   zero(kk);
   zero(qk);
-  product<false, LD, 0, false, LD, 0, DK / 16>(kk, sh.k, sh.k, warp * 16, 0);
-  product<false, LD, 0, false, LD, 0, DK / 16>(qk, sh.q, sh.k, warp * 16, 0);
+#pragma unroll
+  for (int t = 0; t < 8; t += 2)
+    if (t / 2 <= warp) {
+      float(&kt)[2][4] = *reinterpret_cast<float(*)[2][4]>(kk + t);
+      float(&qt)[2][4] = *reinterpret_cast<float(*)[2][4]>(qk + t);
+      product<false, LD, 0, false, LD, 0, DK / 16>(kt, sh.k, sh.k, warp * 16, t * 8);
+      product<false, LD, 0, false, LD, 0, DK / 16>(qt, sh.q, sh.k, warp * 16, t * 8);
+    }
   for (int e = 0; e < group; e++) {
     const int h = kh * group + e;
     Mats& out = mats[slot * a.hv + h];
     __syncthreads();
-    chunk_decay(a, sh.d, start, len, h);
-    __syncthreads();
+    if (e) {
+      chunk_decay(a, sh.d, start, len, h);
+      __syncthreads();
+    }
     if (tid < kC) {
       out.since[tid] = sh.d.since[tid];
       out.until[tid] = sh.d.until[tid];
       out.beta[tid] = sh.d.beta[tid];
     }
 #pragma unroll
-    for (int t = 0; t < 8; t++)
+    for (int half = 0; half < 2; half++) {
+      const int i = warp * 16 + half * 8 + (lane >> 2), ei = sh.d.era[i];
+      const float2 ci = sh.d.cum[i];
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int i = warp * 16 + half * 8 + (lane >> 2), j = t * 8 + (lane & 3) * 2;
+      for (int t = 0; t < 8; t++) {
+        if (t / 2 > warp) continue;
+        const int j = t * 8 + (lane & 3) * 2;
         float p[2];
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          const float f = j + c <= i ? decay(sh.d, i, j + c) : 0.f;
+          const float f = j + c <= i ? decay(ci, ei, sh.d, j + c) : 0.f;
           p[c] = j + c <= i ? qk[t][half * 2 + c] * f : 0.f;
           sh.at[j + c][i] = j + c < i ? kk[t][half * 2 + c] * f * sh.d.beta[j + c] : 0.f;
         }
-        if (j >> 4 <= warp) {
-          uint32_t hi, lo;
-          split2(p[0], p[1], hi, lo);
-          *reinterpret_cast<uint32_t*>(out.p[0] + tri_at(i, j)) = hi;
-          *reinterpret_cast<uint32_t*>(out.p[1] + tri_at(i, j)) = lo;
-        }
+        uint32_t hi, lo;
+        split2(p[0], p[1], hi, lo);
+        *reinterpret_cast<uint32_t*>(out.p[0] + tri_at(i, j)) = hi;
+        *reinterpret_cast<uint32_t*>(out.p[1] + tri_at(i, j)) = lo;
       }
+    }
     __syncthreads();
-    // the inverse's two diagonal blocks, a column per thread: x_i -= A_ij x_j as soon as x_j is known
+    // the inverse's four diagonal blocks of 16, a column per thread: x_i -= A_ij x_j as soon as x_j is known
     if (tid < 64) {
-      const int b = tid & 32, c = tid & 31;
-      float x[32];
+      const int b = tid & 48, c = tid & 15;
+      float x[16];
 #pragma unroll
-      for (int i = 0; i < 32; i++) x[i] = i == c ? 1.f : 0.f;
+      for (int i = 0; i < 16; i++) x[i] = i == c ? 1.f : 0.f;
 #pragma unroll
-      for (int j = 0; j < 31; j++)
+      for (int j = 0; j < 15; j++)
 #pragma unroll
-        for (int i = j + 1; i < 32; i++) x[i] = __fmaf_rn(-sh.at[b + j][b + i], x[j], x[i]);
+        for (int i = j + 1; i < 16; i++) x[i] = __fmaf_rn(-sh.at[b + j][b + i], x[j], x[i]);
 #pragma unroll
-      for (int i = 0; i < 32; i++) {
-        sh.x[b + i][b + c] = x[i];
-        if (b) sh.x[i][b + c] = 0.f;
-      }
+      for (int i = 0; i < 16; i++) sh.x[b + i][b + c] = x[i];
     }
     __syncthreads();
-    {  // the block below: -X22 (A21 X11), eight values per thread
-      const int i = tid >> 2, c = (tid & 3) * 8;
-      float s[8];
+    inverse_block<16, 64>(sh, sh.y + (tid >> 6) * 16, (tid >> 6) * 32 + 16, (tid >> 6) * 32, tid & 63);
+    if (tid < 64) {  // above the diagonal blocks of 16 the blocks of 32 are zero
+      const int b = tid & 32, r = tid & 31;
+      if (r < 16)
 #pragma unroll
-      for (int q = 0; q < 8; q++) s[q] = 0.f;
-      for (int j = 0; j < 32; j++) {
-        const float f = sh.at[j][32 + i];
-#pragma unroll
-        for (int q = 0; q < 8; q++) s[q] = __fmaf_rn(f, sh.x[j][c + q], s[q]);
-      }
-#pragma unroll
-      for (int q = 0; q < 8; q++) sh.y[i][c + q] = s[q];
-      __syncthreads();
-#pragma unroll
-      for (int q = 0; q < 8; q++) s[q] = 0.f;
-      for (int j = 0; j < 32; j++) {
-        const float f = -sh.x[32 + i][32 + j];
-#pragma unroll
-        for (int q = 0; q < 8; q++) s[q] = __fmaf_rn(f, sh.y[j][c + q], s[q]);
-      }
-#pragma unroll
-      for (int q = 0; q < 8; q++) sh.x[32 + i][c + q] = s[q];
+        for (int c = 16; c < 32; c += 4) *reinterpret_cast<float4*>(&sh.x[b + r][b + c]) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncthreads();
-    for (int i = tid; i < kC * kC / 2; i += kPrepThreads) {
-      const int r = i / (kC / 2), c = i % (kC / 2) * 2;
+    inverse_block<32, 128>(sh, sh.y, 32, 0, tid);
+#pragma unroll 5
+    for (int i = tid; i < kTri / 2; i += kPrepThreads) {  // pair i of the ten blocks, in the order of rows and columns
+      const int b = i >> 7, r = b < 1 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, c = b - r * (r + 1) / 2;
+      const int y = r * 16 + (i >> 3 & 15), x = c * 16 + (i & 7) * 2;
       uint32_t hi, lo;
-      if (c >> 4 > r >> 4) continue;
-      split2(sh.x[r][c], sh.x[r][c + 1], hi, lo);
-      *reinterpret_cast<uint32_t*>(out.x[0] + tri_at(r, c)) = hi;
-      *reinterpret_cast<uint32_t*>(out.x[1] + tri_at(r, c)) = lo;
+      split2(sh.x[y][x], sh.x[y][x + 1], hi, lo);
+      *reinterpret_cast<uint32_t*>(out.x[0] + tri_at(y, x)) = hi;
+      *reinterpret_cast<uint32_t*>(out.x[1] + tri_at(y, x)) = lo;
     }
   }
 }
@@ -455,10 +494,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     const long start = from + c * kC;
     const int len = (int)(to - start < kC ? to - start : kC);
     ChainIn<DK>& in = sh.in[c & 1];
-    copy_tile<DK, LD, 128>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec, tid);
-    copy_tile<64, kLd, 128>(in.x, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vec, tid);
+    copy_tile<DK, LD, 128>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vk, tid);
+    copy_tile<64, kLd, 128>(in.x, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vv, tid);
     copy_flat<128>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats), tid);
-    copy_tile<DK, LD, 128>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec, tid);
+    copy_tile<DK, LD, 128>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
     cp_commit();
   };
   if (chunks) load(0);
@@ -528,7 +567,7 @@ struct BackArgs {
   const Mats* mats;
   const __nv_bfloat16* dout;  // [n][hv][dv], strides below
   long ldo, hso;
-  bool vec_o;
+  int align_o;
   const float* dfinal;        // [seqs][hv][dk][dv], or NULL: zero
   __nv_bfloat16* dv;          // [n][hv][dv]
   float* dstate;              // or NULL
@@ -632,10 +671,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     const long start = from + c * kC;
     const int len = (int)(to - start < kC ? to - start : kC);
     ChainIn<DK>& in = sh.in[c & 1];
-    copy_tile<DK, LD, 128>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec, tid);
+    copy_tile<DK, LD, 128>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vk, tid);
     copy_flat<128>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats), tid);
-    copy_tile<64, kLd, 128>(in.x, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o, tid);
-    copy_tile<DK, LD, 128>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec, tid);
+    copy_tile<64, kLd, 128>(in.x, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.align_o, tid);
+    copy_tile<DK, LD, 128>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
     cp_commit();
   };
   if (chunks) load(chunks - 1);
@@ -721,7 +760,7 @@ struct GradArgs {
   DeltaArgs d;
   const __nv_bfloat16* dout;
   long ldo, hso;
-  bool vec_o;
+  int align_o;
   const __nv_bfloat16 *kept, *y, *ds, *dr;
   __nv_bfloat16 *dq, *dk;  // [n][hk][dk]
   float *dg, *dbeta;       // [n][hv]
@@ -756,7 +795,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
   auto load_a = [&](int t) {  // S, dO, dR
     const int h = kh * group + t / slices, slice = t % slices, c0 = slice * 64;
     const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-    copy_tile<64, kLd, kGradThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.vec_o, tid);
+    copy_tile<64, kLd, kGradThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.align_o, tid);
 #pragma unroll
     for (int part = 0; part < 2; part++) {
       tile_in<DK, LD, kGradThreads>(sh.s[part], p.kept + state_at(a, slot, h, slice) + part * 64 * DK);
@@ -773,8 +812,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     }
     cp_commit();
   };
-  copy_tile<DK, LD, kGradThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vec, tid);
-  copy_tile<DK, LD, kGradThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vec, tid);
+  copy_tile<DK, LD, kGradThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vk, tid);
+  copy_tile<DK, LD, kGradThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
   load_a(0);
   load_b(0);
   const int wr = warp & 3, wc = warp >> 2, m0 = wr * 16, i0 = m0 + (lane >> 2);
@@ -869,13 +908,14 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
       float col[2] = {0.f, 0.f};
 #pragma unroll
       for (int half = 0; half < 2; half++) {
-        const int i = i0 + half * 8, j = n0 + n * 8 + (lane & 3) * 2;
+        const int i = i0 + half * 8, j = n0 + n * 8 + (lane & 3) * 2, ei = sh.d.era[i];
+        const float2 ci = sh.d.cum[i];
         float po[2], mm[2];
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           const int e = half * 2 + c;
           const bool low = j + c <= i, strict = j + c < i;
-          const float f = low ? decay(sh.d, i, j + c) : 0.f, b = sh.d.beta[j + c];
+          const float f = low ? decay(ci, ei, sh.d, j + c) : 0.f, b = sh.d.beta[j + c];
           const float ov = low ? a.scale * f * oy[n][e] : 0.f, rv = strict ? f * ry[n][e] : 0.f;
           po[c] = b * ov;
           mm[c] = -b * rv;
@@ -1008,8 +1048,9 @@ static int check_shape(const char* me, const pl_delta_shape* s, bool step) {
   PL_REQUIRE(s->scale == s->scale, PL_ERR_INVALID, "%s: scale = %g", me, s->scale);
   return PL_OK;
 }
-static bool rows16(const void* p, size_t ld, size_t hs) {
-  return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && hs % 8 == 0;
+static int row_align(const void* p, size_t ld, size_t hs) {
+  const uintptr_t all = (uintptr_t)p | ld * 2 | hs * 2;
+  return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 static DeltaArgs delta_args(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g,
                             const float* beta, const int32_t* offsets) {
@@ -1035,7 +1076,9 @@ static DeltaArgs delta_args(const pl_delta_shape* s, const void* q, const void* 
   a.g = g;
   a.beta = beta;
   a.scale = (float)s->scale;
-  a.vec = rows16(q, s->q_token, s->q_head) && rows16(k, s->k_token, s->k_head) && rows16(v, s->v_token, s->v_head);
+  a.vq = row_align(q, s->q_token, s->q_head);
+  a.vk = row_align(k, s->k_token, s->k_head);
+  a.vv = row_align(v, s->v_token, s->v_head);
   return a;
 }
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -1148,18 +1191,18 @@ int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token
   const DeltaArgs a = delta_args(s, q, k, v, g, beta, offsets);
   char* w = (char*)ws;
   __nv_bfloat16 *ds = (__nv_bfloat16*)(w + mats_bytes(s)), *dr = (__nv_bfloat16*)(w + mats_bytes(s) + states_bytes(s));
-  const bool vec_o = rows16(dout, do_token, do_head);
+  const int align_o = row_align(dout, do_token, do_head);
   if (s->tokens) {
     rc = prep(a, (Mats*)ws, st);
     if (rc) return rc;
   }
-  const BackArgs b = {a, (const Mats*)ws, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, dfinal,
+  const BackArgs b = {a, (const Mats*)ws, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, dfinal,
                       (__nv_bfloat16*)dv, dstate, ds, dr};
   const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
   rc = a.dk > 64 ? launch_wide(delta_back_kernel<128>, grid, kChainThreads, sizeof(BackShared<128>), st, b)
                  : launch_wide(delta_back_kernel<64>, grid, kChainThreads, sizeof(BackShared<64>), st, b);
   if (rc || s->tokens == 0) return rc;
-  const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, vec_o, (const __nv_bfloat16*)saved,
+  const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, (const __nv_bfloat16*)saved,
                       (const __nv_bfloat16*)((const char*)saved + states_bytes(s)), ds, dr, (__nv_bfloat16*)dq, (__nv_bfloat16*)dk,
                       dg, dbeta};
   const dim3 chunks((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);

@@ -1,6 +1,8 @@
 // What the kernels of the gated delta rule share: the cut of packed sequences into chunks of 64 tokens, copies of tiles
 // into shared memory, and products of bf16 tiles whose f32 operands are carried as two bf16 parts.
 #pragma once
+#include <type_traits>
+
 #include "pl_common.cuh"
 
 namespace pl {
@@ -16,7 +18,7 @@ struct DeltaArgs {
   const __nv_bfloat16 *q, *k, *v;
   const float *g, *beta;  // [n][hv]
   float scale;
-  bool vec;  // q, k, v rows start at 16-byte boundaries
+  int vq, vk, vv;  // bytes (16, 8, 4, 2) at whose multiples all rows of q, k, v start
 };
 
 // Sequence s's tokens, whatever the offsets hold: inside [0, n].
@@ -40,13 +42,17 @@ __device__ __forceinline__ long seq_slot(const DeltaArgs& a, int s) {
 }
 __host__ __device__ __forceinline__ long slot_count(long n, long seqs) { return n / kC + seqs; }
 
-// The chunk of a slot: its first token and how many it has (0: none).
+// The chunk of a slot: its first token and how many it has (0: none). By whole warps, 32 sequences at a time: one after the
+// other, the reads of a binary search took longer than what the kernels do with the answer.
 __device__ __forceinline__ int slot_chunk(const DeltaArgs& a, long slot, long& start) {
-  int lo = 0, hi = a.seqs - 1;  // the last sequence whose first slot is not behind this one
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (seq_slot(a, mid) <= slot) lo = mid;
-    else hi = mid - 1;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = a.seqs;  // the last sequence whose first slot is not behind this one: in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32, s = lo + lane * step;
+    const unsigned m = __ballot_sync(0xffffffffu, lane * step < n && seq_slot(a, s) <= slot);
+    const int last = m ? 31 - __clz(m) : 0;
+    lo += last * step;
+    n = n - last * step < step ? n - last * step : step;
   }
   long from, to;
   seq_bounds(a, lo, from, to);
@@ -65,26 +71,43 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// rows x COLS values into a tile of row stride LD, from rows of `stride`; what is outside rows x cols becomes zero. With
-// vec the copies are asynchronous (cp_commit, cp_wait); without, plain stores.
+template <int BYTES>
+__device__ __forceinline__ void cp_few(void* dst, const void* src, int bytes) {  // BYTES 4 or 8
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES), "r"(bytes)
+               : "memory");
+}
+// 64 rows x COLS values into a tile of row stride LD, from rows of `stride`; what is outside rows x cols becomes zero. `align`:
+// the bytes at whose multiples the rows start; at 2, values are copied one by one, otherwise asynchronously (cp_commit,
+// cp_wait).
 template <int COLS, int LD, int THREADS>
 __device__ __forceinline__ void copy_tile(__nv_bfloat16* dst, const __nv_bfloat16* src, long stride, int rows, int cols,
-                                          bool vec, int tid) {
-  if (vec) {
-    for (int i = tid; i < kC * (COLS / 8); i += THREADS) {
-      const int r = i / (COLS / 8), c = i % (COLS / 8) * 8;
+                                          int align, int tid) {
+  auto pieces = [&](auto piece) {
+    constexpr int BYTES = decltype(piece)::value, N = BYTES / 2;
+#pragma unroll 4
+    for (int i = tid; i < kC * (COLS / N); i += THREADS) {
+      const int r = i / (COLS / N), c = i % (COLS / N) * N;
       int bytes = r < rows ? (cols - c) * 2 : 0;
-      bytes = bytes < 0 ? 0 : bytes > 16 ? 16 : bytes;
-      cp16(dst + r * LD + c, bytes ? src + (long)r * stride + c : src, bytes);
+      bytes = bytes < 0 ? 0 : bytes > BYTES ? BYTES : bytes;
+      const __nv_bfloat16* from = bytes ? src + (long)r * stride + c : src;
+      if constexpr (BYTES == 16) cp16(dst + r * LD + c, from, bytes);
+      else cp_few<BYTES>(dst + r * LD + c, from, bytes);
     }
+  };
+  if (align >= 16) {
+    pieces(std::integral_constant<int, 16>());
+  } else if (align == 8) {
+    pieces(std::integral_constant<int, 8>());
+  } else if (align == 4) {
+    pieces(std::integral_constant<int, 4>());
   } else {
+#pragma unroll 8
     for (int i = tid; i < kC * COLS; i += THREADS) {
       const int r = i / COLS, c = i % COLS;
       dst[r * LD + c] = r < rows && c < cols ? src[(long)r * stride + c] : __float2bfloat16_rn(0.f);
     }
   }
 }
-
 // n bytes (a multiple of 16) as they lie.
 template <int THREADS>
 __device__ __forceinline__ void copy_flat(void* dst, const void* src, int n, int tid) {
@@ -301,15 +324,20 @@ __device__ __forceinline__ void zero(float (&acc)[NT][4]) {
     for (int e = 0; e < 4; e++) acc[t][e] = 0.f;
 }
 
-// The decays of a chunk's tokens, by the block's first warp: cum (f64 sum of g since the last reset or the chunk's start), era
-// (resets so far), since = the factor on the state before the chunk (zero behind a reset), until = the factor from a
-// token to the chunk's end (zero in front of a reset). A g of -inf resets, and so does one below -104, whose
-// factor f32 cannot hold.
+// The decays of a chunk's tokens, by the block's first warp: cum (sum of g / ln 2 since the last reset or the chunk's start, in
+// f64 and kept as two f32, so that differences of large sums are right), era (resets so far), since = the factor on
+// the state before the chunk (zero behind a reset), until = the factor from a token to the chunk's end (zero in front of a
+// reset). A g of -inf resets, and so does one below -104, whose factor f32 cannot hold.
 struct Decay {
-  double cum[kC];
+  float2 cum[kC];
   int era[kC];
   float since[kC], until[kC], beta[kC];
 };
+__device__ __forceinline__ float exp2_of(float x) {  // 2^-22 off; zero below 2^-126
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+  return e;
+}
 __device__ __forceinline__ void chunk_decay(const DeltaArgs& a, Decay& d, long start, int len, int h) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
@@ -321,40 +349,40 @@ __device__ __forceinline__ void chunk_decay(const DeltaArgs& a, Decay& d, long s
       const float g = t < len ? a.g[(start + t) * a.hv + h] : 0.f;
       d.beta[t] = t < len ? a.beta[(start + t) * a.hv + h] : 0.f;
       const bool reset = g < -104.f;
-      double s = reset ? 0.0 : (double)g;
-      int e = reset;
+      cum[half] = reset ? 0.0 : (double)g * 1.4426950408889634074;
+      era[half] = reset;
+    }
 #pragma unroll
-      for (int o = 1; o < 32; o *= 2) {  // (sum, resets) of the tokens up to this one; a reset forgets the sum before it
-        const double up = __shfl_up_sync(0xffffffffu, s, o);
-        const int ue = __shfl_up_sync(0xffffffffu, e, o);
+    for (int o = 1; o < 32; o *= 2)  // (sum, resets) of the tokens up to this one; a reset forgets the sum before it
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const double up = __shfl_up_sync(0xffffffffu, cum[half], o);
+        const int ue = __shfl_up_sync(0xffffffffu, era[half], o);
         if (lane >= o) {
-          if (e == 0) s += up;
-          e += ue;
+          if (era[half] == 0) cum[half] += up;
+          era[half] += ue;
         }
       }
-      if (half) {
-        const double last = __shfl_sync(0xffffffffu, cum[0], 31);
-        if (e == 0) s += last;
-        e += __shfl_sync(0xffffffffu, era[0], 31);
-      }
-      cum[half] = s;
-      era[half] = e;
-    }
+    const double first = __shfl_sync(0xffffffffu, cum[0], 31);
+    if (era[1] == 0) cum[1] += first;
+    era[1] += __shfl_sync(0xffffffffu, era[0], 31);
     const double end = __shfl_sync(0xffffffffu, cum[1], 31);
     const int last = __shfl_sync(0xffffffffu, era[1], 31);
 #pragma unroll
     for (int half = 0; half < 2; half++) {
       const int t = half * 32 + lane;
-      d.cum[t] = cum[half];
+      const float hi = (float)cum[half];
+      d.cum[t] = make_float2(hi, (float)(cum[half] - (double)hi));
       d.era[t] = era[half];
-      d.since[t] = era[half] == 0 ? expf((float)cum[half]) : 0.f;
-      d.until[t] = era[half] == last ? expf((float)(end - cum[half])) : 0.f;
+      d.since[t] = era[half] == 0 ? exp2_of(hi) : 0.f;
+      d.until[t] = era[half] == last ? exp2_of((float)(end - cum[half])) : 0.f;
     }
   }
 }
 // The factor from token j to token i >= j.
-__device__ __forceinline__ float decay(const Decay& d, int i, int j) {
-  return d.era[i] == d.era[j] ? expf((float)(d.cum[i] - d.cum[j])) : 0.f;
+__device__ __forceinline__ float decay(float2 ci, int ei, const Decay& d, int j) {
+  const float2 cj = d.cum[j];
+  return ei == d.era[j] ? exp2_of((ci.x - cj.x) + (ci.y - cj.y)) : 0.f;
 }
 
 }  // namespace pl
