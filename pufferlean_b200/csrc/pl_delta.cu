@@ -314,7 +314,9 @@ struct ChainIn {
   __nv_bfloat16 k[kC * (DK + 8)], q[kC * (DK + 8)], x[kC * kLd];
   Mats m;
 };
-constexpr int kChainThreads = 256;  // four warps for the chain, 16 columns of v each, and four that work for them
+// Four warps for the chain, 16 columns of v each, four for products beside it, four for memory.
+constexpr int kChainThreads = 384;
+constexpr int kAll = 15, kMovers = 14;  // barriers of all threads, of the four warps for memory
 template <int DK>
 struct ScanShared {
   ChainIn<DK> in[2];
@@ -403,8 +405,8 @@ __device__ __forceinline__ uint32_t across_at(const __nv_bfloat16* tile, int n) 
 // A block per sequence, value head and 64 columns of v. A warp of the chain keeps 16 columns of the state, transposed [16][dk], in
 // registers for the whole sequence, and everything that a chunk makes of it: an accumulator's layout is that of a first
 // operand, so K S, R, Y and F U go from one product into the next as they are, split into two bf16 parts. What the next
-// chunk's state does not wait for is another warp's, which gets the state's parts and Y through shared memory: loading the next
-// chunk, Q S and P U, o, and what the gradient needs. (All in one warp, a chunk took 5.5 us; with R, Y, U and the state's
+// chunk's state does not wait for is another warp's, which gets the state's parts and Y through shared memory: Q S and P U; a
+// third one's is what goes from and to memory. (All in one warp, a chunk took 5.5 us; with R, Y, U and the state's
 // parts in shared memory, shared by 16 warps in four steps with barriers, 5.6.) The products are 316 and 188 of 16 x 8 x 16
 // per chunk: 8 cycles each on a quarter of an SM.
 template <int DK>
@@ -429,7 +431,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     state_in(s, p.state ? p.state + sbase : nullptr, a.dk, a.dv, mine);
     for (long c = 0; c < chunks; c++) {
       ChainIn<DK>& in = sh.in[c & 1];
-      block_wait();
+      meet<kChainThreads>(kAll);
       float r[8][4];  // (K S)^T: [16 of dv][64 tokens]
       zero(r);
       const uint32_t pk = smem_u32(in.k + lane_b<false, LD>());
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
         give(sh.s[warp], 2 * k + 1, x.lo);
         step<false, 4>(r, x, pk + k * 32, 32 * LD);
       }
-      pair_arrive(s_ready);
+      meet_arrive<96>(s_ready);
       const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>());
 #pragma unroll
       for (int n = 0; n < 4; n++) {  // R = V - E K S
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
       for (int k = 0; k < 4; k++) tri_step<false>(y, parts_of(r[2 * k], r[2 * k + 1]), tx, k);
 #pragma unroll
       for (int t = 0; t < 8; t++) give(sh.y[warp], t, y[t]);
-      pair_arrive(y_ready);
+      meet_arrive<96>(y_ready);
       const float keep = in.m.since[kC - 1];
 #pragma unroll
       for (int t = 0; t < NK; t++)
@@ -485,11 +487,61 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
         step<true, DK / 16>(s, parts_of(y[2 * k], y[2 * k + 1]), pt + k * 32 * LD, 32);
       }
     }
+    if (chunks) meet<kChainThreads>(kAll);
     state_out(s, p.final_state + sbase, a.dk, a.dv, mine);
     return;
   }
-  // the chain's helpers
-  const int tid = threadIdx.x - 128, cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
+  if (threadIdx.x < 256) {  // Q S, P U
+    for (long c = 0; c < chunks; c++) {
+      ChainIn<DK>& in = sh.in[c & 1];
+      meet<kChainThreads>(kAll);
+      float o[8][4];  // (Q S)^T
+      zero(o);
+      const uint32_t pq = smem_u32(in.q + lane_b<false, LD>());
+      meet<96>(s_ready);
+#pragma unroll
+      for (int k = 0; k < DK / 16; k++) {
+        Parts x;
+        take(sh.s[warp], 2 * k, x.hi);
+        take(sh.s[warp], 2 * k + 1, x.lo);
+        step<false, 4>(o, x, pq + k * 32, 32 * LD);
+      }
+#pragma unroll
+      for (int t = 0; t < 8; t++) {
+        const float2 f = *reinterpret_cast<const float2*>(in.m.since + t * 8 + (lane & 3) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float fe = e & 1 ? f.y : f.x;
+          o[t][e] = fe == 0.f ? 0.f : fe * o[t][e];
+        }
+      }
+      const uint32_t tp = tri_lane<false>(in.m.p[0]);
+      meet<96>(y_ready);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        float u[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const float2 b = *reinterpret_cast<const float2*>(in.m.beta + k * 16 + t * 8 + (lane & 3) * 2);
+          take(sh.y[warp], 2 * k + t, u[t]);
+          u[t][0] *= b.x, u[t][2] *= b.x;
+          u[t][1] *= b.y, u[t][3] *= b.y;
+        }
+        tri_step<false>(o, parts_of(u[0], u[1]), tp, k);
+      }
+      // the chain has read these columns of v before it gave Y: o takes their place on its way out
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[2 * n][e] *= a.scale, o[2 * n + 1][e] *= a.scale;
+        store_across(across_at(in.x + warp * 16, n), o[2 * n], o[2 * n + 1]);
+      }
+    }
+    if (chunks) meet<kChainThreads>(kAll);
+    return;
+  }
+  // memory
+  const int tid = threadIdx.x - 256, cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
   auto load = [&](long c) {
     const long start = from + c * kC;
     const int len = (int)(to - start < kC ? to - start : kC);
@@ -500,64 +552,41 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     copy_tile<DK, LD, 128>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
     cp_commit();
   };
+  const bool vec_o = a.dv % 8 == 0 && (uintptr_t)p.o % 16 == 0;
+  auto write_o = [&](long c) {
+    const long start = from + c * kC;
+    rows_out(sh.in[c & 1].x + warp * 16, p.o + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv,
+             (int)(to - start < kC ? to - start : kC), mine, vec_o);
+  };
   if (chunks) load(0);
   zero_rows<128>(a, seq, p.o + (long)h * a.dv + c0, (long)a.hv * a.dv, cols, tid);
-  const bool vec_o = a.dv % 8 == 0 && (uintptr_t)p.o % 16 == 0;
   for (long c = 0; c < chunks; c++) {
-    const long start = from + c * kC, slot = slot0 + c;
-    const int len = (int)(to - start < kC ? to - start : kC);
-    ChainIn<DK>& in = sh.in[c & 1];
     cp_wait<0>();
-    block_wait();
+    meet<kChainThreads>(kAll);
+    if (c > 0) write_o(c - 1);
+    meet<128>(kMovers);  // the place of chunk c - 1's inputs, and of its o, is free
     if (c + 1 < chunks) load(c + 1);
-    float o[8][4];  // (Q S)^T
-    zero(o);
-    const uint32_t pq = smem_u32(in.q + lane_b<false, LD>());
-    pair_wait(s_ready);
+    meet<96>(s_ready);
+    if (p.kept) {
+      __nv_bfloat16* to_s = p.kept + state_at(a, slot0 + c, h, slice) + warp * 16 * DK;
 #pragma unroll
-    for (int k = 0; k < DK / 16; k++) {
-      Parts x;
-      take(sh.s[warp], 2 * k, x.hi);
-      take(sh.s[warp], 2 * k + 1, x.lo);
-      if (p.kept) {
-        __nv_bfloat16* to_s = p.kept + state_at(a, slot, h, slice) + warp * 16 * DK;
-        part_out(x.hi, to_s, DK, k);
-        part_out(x.lo, to_s + 64 * DK, DK, k);
-      }
-      step<false, 4>(o, x, pq + k * 32, 32 * LD);
-    }
-#pragma unroll
-    for (int t = 0; t < 8; t++) {
-      const float2 f = *reinterpret_cast<const float2*>(in.m.since + t * 8 + (lane & 3) * 2);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float fe = e & 1 ? f.y : f.x;
-        o[t][e] = fe == 0.f ? 0.f : fe * o[t][e];
+      for (int k = 0; k < DK / 8; k++) {
+        uint32_t x[4];
+        take(sh.s[warp], k, x);
+        part_out(x, to_s + (k & 1) * 64 * DK, DK, k / 2);
       }
     }
-    float y[8][4];
-    pair_wait(y_ready);
+    meet<96>(y_ready);
+    if (p.y) {
+      float y[8][4];
 #pragma unroll
-    for (int t = 0; t < 8; t++) take(sh.y[warp], t, y[t]);
-    if (p.y) parts_out(y, p.y + rows_at(a, slot, h, slice) + warp * 16 * 64, 64, 64l * 64);
-#pragma unroll
-    for (int t = 0; t < 8; t++) {  // U
-      const float2 b = *reinterpret_cast<const float2*>(in.m.beta + t * 8 + (lane & 3) * 2);
-      y[t][0] *= b.x, y[t][2] *= b.x;
-      y[t][1] *= b.y, y[t][3] *= b.y;
+      for (int t = 0; t < 8; t++) take(sh.y[warp], t, y[t]);
+      parts_out(y, p.y + rows_at(a, slot0 + c, h, slice) + warp * 16 * 64, 64, 64l * 64);
     }
-    const uint32_t tp = tri_lane<false>(in.m.p[0]);
-#pragma unroll
-    for (int k = 0; k < 4; k++) tri_step<false>(o, parts_of(y[2 * k], y[2 * k + 1]), tp, k);
-    // the chain has read these columns of v before it gave Y: o takes their place on its way out
-#pragma unroll
-    for (int n = 0; n < 4; n++) {
-#pragma unroll
-      for (int e = 0; e < 4; e++) o[2 * n][e] *= a.scale, o[2 * n + 1][e] *= a.scale;
-      store_across(across_at(in.x + warp * 16, n), o[2 * n], o[2 * n + 1]);
-    }
-    __syncwarp();
-    rows_out(in.x + warp * 16, p.o + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_o);
+  }
+  if (chunks) {
+    meet<kChainThreads>(kAll);
+    write_o(chunks - 1);
   }
 }
 
@@ -603,7 +632,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     state_in(s, p.dfinal ? p.dfinal + sbase : nullptr, a.dk, a.dv, mine);
     for (long c = chunks - 1; c >= 0; c--) {
       ChainIn<DK>& in = sh.in[c & 1];
-      block_wait();
+      meet<kChainThreads>(kAll);
       float x[8][4];  // (K dS')^T: [16 of dv][64 tokens]
       zero(x);
       const uint32_t pk = smem_u32(in.k + lane_b<false, LD>());
@@ -614,7 +643,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
         give(sh.s[warp], 2 * k + 1, z.lo);
         step<false, 4>(x, z, pk + k * 32, 32 * LD);
       }
-      pair_wait(u_ready);
+      meet<64>(u_ready);
 #pragma unroll
       for (int t = 0; t < 8; t++) {  // beta dU = beta (F K dS' + scale P^T dO)
         const float2 b = *reinterpret_cast<const float2*>(in.m.beta + t * 8 + (lane & 3) * 2);
@@ -634,7 +663,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
       for (int k = 0; k < 4; k++) tri_step<true>(r, parts_of(x[2 * k], x[2 * k + 1]), tx, k);
 #pragma unroll
       for (int t = 0; t < 8; t++) give(sh.x[warp], t, r[t]);
-      pair_arrive(r_ready);
+      meet_arrive<64>(r_ready);
       const float keep = in.m.since[kC - 1];
 #pragma unroll
       for (int t = 0; t < NK; t++)
@@ -654,7 +683,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
         }
         step<true, DK / 16>(s, parts_of(r[2 * k], r[2 * k + 1]), pt + k * 32 * LD, 32);
       }
-      pair_wait(q_ready);
+      meet<64>(q_ready);
 #pragma unroll
       for (int t = 0; t < NK; t++) {
         float q[4];
@@ -666,7 +695,59 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     if (p.dstate) state_out(s, p.dstate + sbase, a.dk, a.dv, mine);
     return;
   }
-  const int tid = threadIdx.x - 128, cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
+  if (threadIdx.x < 256) {  // scale P^T dO and scale (E dO)^T Q
+    for (long c = chunks - 1; c >= 0; c--) {
+      ChainIn<DK>& in = sh.in[c & 1];
+      meet<kChainThreads>(kAll);
+      const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>());
+      uint32_t o[4][4];  // dO^T: [16 of dv][64 tokens]
+#pragma unroll
+      for (int k = 0; k < 4; k++) ldsm<true>(o[k], px + k * 32 * kLd);
+      {
+        float u[8][4];
+        zero(u);
+        const uint32_t tp = tri_lane<true>(in.m.p[0]);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          Parts x;
+#pragma unroll
+          for (int e = 0; e < 4; e++) x.hi[e] = x.lo[e] = o[k][e];
+          tri_step<true, false>(u, x, tp, k);
+        }
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) u[t][e] *= a.scale;
+          give(sh.x[warp], t, u[t]);
+        }
+      }
+      meet_arrive<64>(u_ready);
+      float q[NK][4];
+      zero(q);
+      const uint32_t pq = smem_u32(in.q + lane_b<true, LD>());
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        float eo[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const float2 f = *reinterpret_cast<const float2*>(in.m.since + k * 16 + t * 8 + (lane & 3) * 2);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float fe = e & 1 ? f.y : f.x;
+            const uint32_t oo = o[k][t * 2 + (e >> 1)];
+            eo[t][e] = fe == 0.f ? 0.f : a.scale * fe * __uint_as_float(e & 1 ? oo & 0xffff0000u : oo << 16);
+          }
+        }
+        step<true, DK / 16>(q, parts_of(eo[0], eo[1]), pq + k * 32 * LD, 32);
+      }
+#pragma unroll
+      for (int t = 0; t < NK; t++) give(sh.q[warp], t, q[t]);
+      meet_arrive<64>(q_ready);
+    }
+    return;
+  }
+  // memory
+  const int tid = threadIdx.x - 256, cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
   auto load = [&](long c) {
     const long start = from + c * kC;
     const int len = (int)(to - start < kC ? to - start : kC);
@@ -685,67 +766,21 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     const int len = (int)(to - start < kC ? to - start : kC);
     ChainIn<DK>& in = sh.in[c & 1];
     cp_wait<0>();
-    block_wait();
-    const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>());
-    uint32_t o[4][4];  // dO^T: [16 of dv][64 tokens]
-#pragma unroll
-    for (int k = 0; k < 4; k++) ldsm<true>(o[k], px + k * 32 * kLd);
-    float u[8][4];  // (P^T dO)^T
-    zero(u);
-    const uint32_t tp = tri_lane<true>(in.m.p[0]);
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      Parts x;
-#pragma unroll
-      for (int e = 0; e < 4; e++) x.hi[e] = o[k][e];
-      tri_step<true, false>(u, x, tp, k);
-    }
-#pragma unroll
-    for (int t = 0; t < 8; t++) {
-#pragma unroll
-      for (int e = 0; e < 4; e++) u[t][e] *= a.scale;
-      give(sh.x[warp], t, u[t]);
-    }
-    pair_arrive(u_ready);
+    meet<kChainThreads>(kAll);
     if (c > 0) load(c - 1);
-    {
-      float q[NK][4];
-      zero(q);
-      const uint32_t pq = smem_u32(in.q + lane_b<true, LD>());
-#pragma unroll
-      for (int k = 0; k < 4; k++) {  // scale (E dO)^T Q
-        float eo[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-          const float2 f = *reinterpret_cast<const float2*>(in.m.since + k * 16 + t * 8 + (lane & 3) * 2);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float fe = e & 1 ? f.y : f.x;
-            const uint32_t oo = o[k][t * 2 + (e >> 1)];
-            eo[t][e] = fe == 0.f ? 0.f : a.scale * fe * __uint_as_float(e & 1 ? oo & 0xffff0000u : oo << 16);
-          }
-        }
-        step<true, DK / 16>(q, parts_of(eo[0], eo[1]), pq + k * 32 * LD, 32);
-      }
-#pragma unroll
-      for (int t = 0; t < NK; t++) give(sh.q[warp], t, q[t]);
-      pair_arrive(q_ready);
-    }
     float r[8][4];
-    pair_wait(r_ready);
+    meet<64>(r_ready);
+    __nv_bfloat16* to_s = p.ds + state_at(a, slot, h, slice) + warp * 16 * DK;
 #pragma unroll
-    for (int k = 0; k < DK / 16; k++) {
-      __nv_bfloat16* to_s = p.ds + state_at(a, slot, h, slice) + warp * 16 * DK;
+    for (int k = 0; k < DK / 8; k++) {
       uint32_t x[4];
-      take(sh.s[warp], 2 * k, x);
-      part_out(x, to_s, DK, k);
-      take(sh.s[warp], 2 * k + 1, x);
-      part_out(x, to_s + 64 * DK, DK, k);
+      take(sh.s[warp], k, x);
+      part_out(x, to_s + (k & 1) * 64 * DK, DK, k / 2);
     }
 #pragma unroll
     for (int t = 0; t < 8; t++) take(sh.x[warp], t, r[t]);
     parts_out(r, p.dr + rows_at(a, slot, h, slice) + warp * 16 * 64, 64, 64l * 64);
-    // dv takes the place of these columns of dO, which this warp alone has read, on its way out
+    // the helper has read these columns of dO before the chain could give dR: dv takes their place on its way out
 #pragma unroll
     for (int n = 0; n < 4; n++) store_across(across_at(in.x + warp * 16, n), r[2 * n], r[2 * n + 1]);
     __syncwarp();

@@ -257,25 +257,23 @@ __device__ __forceinline__ void step(float (&acc)[2 * N][4], const Parts& a, uin
 // columns of A; T triangular, two parts; A two parts or (TWO = false) its first alone.
 template <bool ACROSS, bool TWO = true>
 __device__ __forceinline__ void tri_step(float (&acc)[8][4], const Parts& a, uint32_t tri, int k) {
-  uint32_t y[4][4], z[4][4];
+  uint32_t y[4][4];
 #pragma unroll
-  for (int n = 0; n < 4; n++) {
-    if (ACROSS ? n > k : n < k) continue;
-    const int r = ACROSS ? k : n, c = ACROSS ? n : k;
-    const uint32_t at = tri + (r * (r + 1) / 2 + c) * 512;
-    ldsm<ACROSS>(y[n], at);
-    ldsm<ACROSS>(z[n], at + kTri * 2);
-  }
+  for (int part = 0; part < 3; part++) {
 #pragma unroll
-  for (int part = 0; part < 3; part++)
+    for (int n = 0; n < 4; n++) {
+      if (part == 1 || (ACROSS ? n > k : n < k)) continue;
+      const int r = ACROSS ? k : n, c = ACROSS ? n : k;
+      ldsm<ACROSS>(y[n], tri + (r * (r + 1) / 2 + c) * 512 + (part == 2 ? kTri * 2 : 0));
+    }
 #pragma unroll
     for (int n = 0; n < 4; n++) {
       if ((ACROSS ? n > k : n < k) || (part == 1 && !TWO)) continue;
       const uint32_t(&x)[4] = part == 1 ? a.lo : a.hi;
-      const uint32_t(&b)[4] = part == 2 ? z[n] : y[n];
-      mma(acc[2 * n], x, b[0], b[1]);
-      mma(acc[2 * n + 1], x, b[2], b[3]);
+      mma(acc[2 * n], x, y[n][0], y[n][1]);
+      mma(acc[2 * n + 1], x, y[n][2], y[n][3]);
     }
+  }
 }
 // Registers of one warp for another one's same lanes: pieces of 16 bytes per lane at `at`.
 __device__ __forceinline__ void give(uint4* at, int piece, const uint32_t (&r)[4]) {
@@ -293,11 +291,16 @@ __device__ __forceinline__ void take(const uint4* at, int piece, float (&r)[4]) 
   const uint4 v = at[piece * 32 + (threadIdx.x & 31)];
   r[0] = __uint_as_float(v.x), r[1] = __uint_as_float(v.y), r[2] = __uint_as_float(v.z), r[3] = __uint_as_float(v.w);
 }
-// Barrier `id` of two warps: what the one wrote before it arrives, the other sees after it waits.
-__device__ __forceinline__ void pair_arrive(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
-// All 256 threads of a chain's block, from two places in the code.
-__device__ __forceinline__ void block_wait() { asm volatile("bar.sync 15, 256;" ::: "memory"); }
-__device__ __forceinline__ void pair_wait(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+// Barrier `id` of THREADS threads: what those that arrive wrote before, those that wait see behind it. Every one of a round's threads
+// comes once, by one or the other.
+template <int THREADS>
+__device__ __forceinline__ void meet_arrive(int id) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+}
+template <int THREADS>
+__device__ __forceinline__ void meet(int id) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+}
 
 // This lane's place in a triangular matrix's first block as B: [n][k] as it lies, or (ACROSS) [k][n].
 template <bool ACROSS>
