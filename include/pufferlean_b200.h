@@ -596,8 +596,9 @@ int pl_sample_dev(const void* logits, size_t ld, size_t rows, size_t V, uint8_t 
  *
  * Sequences lie one behind the other: sequence s has tokens offsets[s] to offsets[s + 1] - 1 (int32 on the device,
  * not falling; NULL: `sequences` of equal length). Tokens in front of the first and behind the last belong to none: their outputs
- * are zero. state (NULL: zero) and final_state are [sequences][heads_v][dk][dv] f32. ws: pl_delta_ws bytes; saved, for
- * the gradient: pl_delta_saved bytes, or NULL; both 256-byte aligned. */
+ * are zero. state (NULL: zero) and final_state are [sequences][heads_v][dk][dv] f32. Either saved, for the gradient
+ * (pl_delta_saved bytes), or ws (pl_delta_ws bytes) is needed, 256-byte aligned. A wait for copies that ran out
+ * (pl_device_check) leaves results that are not valid. */
 typedef struct {
   size_t tokens, sequences, heads_k, heads_v, dk, dv;
   size_t q_token, q_head, k_token, k_head, v_token, v_head;

@@ -130,12 +130,20 @@ __global__ void __launch_bounds__(256) delta_step_kernel(const StepArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------- X and P of all chunks
-// Per slot and value head: X and P, triangular, as two bf16 parts each (in the order X, its second part, P, its second part), and
-// since, until, beta of the chunk's tokens.
+// Per slot and value head: X and P, triangular, as two bf16 parts each, and the decays; per slot and key head K and Q in rows as they stand in
+// shared memory, [2][64][dkp + 8], so that the other kernels get them by one bulk copy; per slot its chunk's first token and
+// length (0: none).
 struct __align__(16) Mats {
   __nv_bfloat16 x[2][kTri], p[2][kTri];
-  float since[kC], until[kC], beta[kC];
+  Decay d;
 };
+
+template <int DK>
+constexpr uint32_t kTileBytes = 2 * kC * (DK + 8) * 2;
+template <int DK>
+__device__ __forceinline__ long tile_at(const DeltaArgs& a, long slot, int kh) {
+  return (slot * a.hk + kh) * 2 * kC * (DK + 8);
+}
 
 constexpr int kPrepThreads = 128;
 template <int DK>
@@ -192,7 +200,7 @@ __device__ __forceinline__ void inverse_block(Shared& sh, float (*y)[36], int r,
   __syncthreads();
 }
 template <int DK>
-__global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const DeltaArgs a, Mats* __restrict__ mats) {
+__global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const DeltaArgs a, Mats* __restrict__ mats, __nv_bfloat16* __restrict__ tiles, int2* __restrict__ table) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
@@ -202,13 +210,19 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
   const int kh = blockIdx.y, group = a.hv / a.hk, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   long start;
   const int len = slot_chunk(a, slot, start);
+  if (kh == 0 && tid == 0) table[slot] = make_int2((int)start, len);
   if (len == 0) return;
   copy_tile<DK, LD, kPrepThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vk, tid);
   copy_tile<DK, LD, kPrepThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
   cp_commit();
   chunk_decay(a, sh.d, start, len, kh * group);
   cp_wait<0>();
+  tc::fence_proxy_async_smem();
   __syncthreads();
+  if (tid == 0) {
+    bulk_out(tiles + tile_at<DK>(a, slot, kh), sh.k, kTileBytes<DK>);
+    tc::bulk_commit();
+  }
   float kk[8][4], qk[8][4];  // rows 16 warp.. of K K^T and Q K^T, up to the diagonal's block
   zero(kk);
   zero(qk);
@@ -220,6 +234,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
       product<false, LD, 0, false, LD, 0, DK / 16>(kt, sh.k, sh.k, warp * 16, t * 8);
       product<false, LD, 0, false, LD, 0, DK / 16>(qt, sh.q, sh.k, warp * 16, t * 8);
     }
+  if (tid == 0) tc::bulk_wait_read<0>();  // the places of K and Q are used again
   for (int e = 0; e < group; e++) {
     const int h = kh * group + e;
     Mats& out = mats[slot * a.hv + h];
@@ -228,11 +243,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
       chunk_decay(a, sh.d, start, len, h);
       __syncthreads();
     }
-    if (tid < kC) {
-      out.since[tid] = sh.d.since[tid];
-      out.until[tid] = sh.d.until[tid];
-      out.beta[tid] = sh.d.beta[tid];
-    }
+    if (tid < (int)(sizeof(Decay) / 16)) reinterpret_cast<uint4*>(&out.d)[tid] = reinterpret_cast<const uint4*>(&sh.d)[tid];
 #pragma unroll
     for (int half = 0; half < 2; half++) {
       const int i = warp * 16 + half * 8 + (lane >> 2), ei = sh.d.era[i];
@@ -288,21 +299,24 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
       *reinterpret_cast<uint32_t*>(out.x[1] + tri_at(y, x)) = lo;
     }
   }
+  if (tid == 0) tc::bulk_wait<0>();
 }
 
 // ---------------------------------------------------------------------------------------------- the chain forward
-// What a chain leaves for the gradient, per slot, value head and 64 columns of v, as two bf16 parts one behind the other: a
-// state, transposed, [2][64][dkp], and rows, transposed, [2][64][64 tokens].
+// What a chain leaves for the gradient, per slot, value head and 64 columns of v, as two bf16 parts one behind the other, in
+// rows as they stand in shared memory (one bulk copy): a state, transposed, [2][64][dkp + 8], and rows, transposed,
+// [2][64][72], 64 tokens in each.
 __device__ __forceinline__ long state_at(const DeltaArgs& a, long slot, int h, int slice) {
-  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * 64 * a.dkp;
+  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * 64 * (a.dkp + 8);
 }
 __device__ __forceinline__ long rows_at(const DeltaArgs& a, long slot, int h, int slice) {
-  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * kC * 64;
+  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * kC * kLd;
 }
 
 struct ScanArgs {
   DeltaArgs d;
   const Mats* mats;
+  const __nv_bfloat16* tiles;
   const float* state;  // [seqs][hv][dk][dv], or NULL: zero
   __nv_bfloat16* o;    // [n][hv][dv]
   float* final_state;
@@ -322,6 +336,7 @@ struct ScanShared {
   ChainIn<DK> in[2];
   uint4 s[4][DK / 8 * 32];  // a warp's state, in two parts
   uint4 y[4][8 * 32];       // its Y
+  uint64_t full[2];         // the inputs have come
 };
 
 // Rows that no sequence holds, in front of the first and behind the last: zero. Called by the blocks of those two.
@@ -425,6 +440,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
   seq_bounds(a, seq, from, to);
   const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
   const int s_ready = 1 + warp, y_ready = 5 + warp;
+  if (threadIdx.x == 0) {
+    tc::mbar_init(&sh.full[0], 1);
+    tc::mbar_init(&sh.full[1], 1);
+    tc::fence_mbar_init();
+  }
+  __syncthreads();
   if (chain) {
     float s[NK][4];
     const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
@@ -432,6 +453,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     for (long c = 0; c < chunks; c++) {
       ChainIn<DK>& in = sh.in[c & 1];
       meet<kChainThreads>(kAll);
+      tc::mbar_wait(&sh.full[c & 1], c >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
       float r[8][4];  // (K S)^T: [16 of dv][64 tokens]
       zero(r);
       const uint32_t pk = smem_u32(in.k + lane_b<false, LD>());
@@ -450,7 +472,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
         ldsm<true>(v, px + n * 32 * kLd);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const float2 f = *reinterpret_cast<const float2*>(in.m.since + n * 16 + t * 8 + (lane & 3) * 2);
+          const float2 f = *reinterpret_cast<const float2*>(in.m.d.since + n * 16 + t * 8 + (lane & 3) * 2);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float fe = e & 1 ? f.y : f.x;
@@ -468,7 +490,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
 #pragma unroll
       for (int t = 0; t < 8; t++) give(sh.y[warp], t, y[t]);
       meet_arrive<96>(y_ready);
-      const float keep = in.m.since[kC - 1];
+      const float keep = in.m.d.since[kC - 1];
 #pragma unroll
       for (int t = 0; t < NK; t++)
 #pragma unroll
@@ -478,8 +500,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
       for (int k = 0; k < 4; k++) {  // S^T += (F U)^T K
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const float2 f = *reinterpret_cast<const float2*>(in.m.until + k * 16 + t * 8 + (lane & 3) * 2);
-          const float2 b = *reinterpret_cast<const float2*>(in.m.beta + k * 16 + t * 8 + (lane & 3) * 2);
+          const float2 f = *reinterpret_cast<const float2*>(in.m.d.until + k * 16 + t * 8 + (lane & 3) * 2);
+          const float2 b = *reinterpret_cast<const float2*>(in.m.d.beta + k * 16 + t * 8 + (lane & 3) * 2);
           float(&u)[4] = y[2 * k + t];
           u[0] *= f.x * b.x, u[2] *= f.x * b.x;
           u[1] *= f.y * b.y, u[3] *= f.y * b.y;
@@ -495,6 +517,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     for (long c = 0; c < chunks; c++) {
       ChainIn<DK>& in = sh.in[c & 1];
       meet<kChainThreads>(kAll);
+      tc::mbar_wait(&sh.full[c & 1], c >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
       float o[8][4];  // (Q S)^T
       zero(o);
       const uint32_t pq = smem_u32(in.q + lane_b<false, LD>());
@@ -508,7 +531,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
       }
 #pragma unroll
       for (int t = 0; t < 8; t++) {
-        const float2 f = *reinterpret_cast<const float2*>(in.m.since + t * 8 + (lane & 3) * 2);
+        const float2 f = *reinterpret_cast<const float2*>(in.m.d.since + t * 8 + (lane & 3) * 2);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const float fe = e & 1 ? f.y : f.x;
@@ -522,7 +545,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
         float u[2][4];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const float2 b = *reinterpret_cast<const float2*>(in.m.beta + k * 16 + t * 8 + (lane & 3) * 2);
+          const float2 b = *reinterpret_cast<const float2*>(in.m.d.beta + k * 16 + t * 8 + (lane & 3) * 2);
           take(sh.y[warp], 2 * k + t, u[t]);
           u[t][0] *= b.x, u[t][2] *= b.x;
           u[t][1] *= b.y, u[t][3] *= b.y;
@@ -546,10 +569,14 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     const long start = from + c * kC;
     const int len = (int)(to - start < kC ? to - start : kC);
     ChainIn<DK>& in = sh.in[c & 1];
-    copy_tile<DK, LD, 128>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vk, tid);
+    uint64_t* bar = &sh.full[c & 1];
+    tc::fence_proxy_async_smem();  // what was there has been read the ordinary way
+    if (tid == 0) {
+      tc::mbar_expect_tx(bar, sizeof(Mats) + kTileBytes<DK>);
+      bulk_in(in.k, p.tiles + tile_at<DK>(a, slot0 + c, kh), kTileBytes<DK>, bar);
+      bulk_in(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats), bar);
+    }
     copy_tile<64, kLd, 128>(in.x, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vv, tid);
-    copy_flat<128>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats), tid);
-    copy_tile<DK, LD, 128>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
     cp_commit();
   };
   const bool vec_o = a.dv % 8 == 0 && (uintptr_t)p.o % 16 == 0;
@@ -568,12 +595,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     if (c + 1 < chunks) load(c + 1);
     meet<96>(s_ready);
     if (p.kept) {
-      __nv_bfloat16* to_s = p.kept + state_at(a, slot0 + c, h, slice) + warp * 16 * DK;
+      __nv_bfloat16* to_s = p.kept + state_at(a, slot0 + c, h, slice) + warp * 16 * LD;
 #pragma unroll
       for (int k = 0; k < DK / 8; k++) {
         uint32_t x[4];
         take(sh.s[warp], k, x);
-        part_out(x, to_s + (k & 1) * 64 * DK, DK, k / 2);
+        part_out(x, to_s + (k & 1) * 64 * LD, LD, k / 2);
       }
     }
     meet<96>(y_ready);
@@ -581,7 +608,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
       float y[8][4];
 #pragma unroll
       for (int t = 0; t < 8; t++) take(sh.y[warp], t, y[t]);
-      parts_out(y, p.y + rows_at(a, slot0 + c, h, slice) + warp * 16 * 64, 64, 64l * 64);
+      parts_out(y, p.y + rows_at(a, slot0 + c, h, slice) + warp * 16 * kLd, kLd, (long)kC * kLd);
     }
   }
   if (chunks) {
@@ -594,6 +621,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
 struct BackArgs {
   DeltaArgs d;
   const Mats* mats;
+  const __nv_bfloat16* tiles;
   const __nv_bfloat16* dout;  // [n][hv][dv], strides below
   long ldo, hso;
   int align_o;
@@ -608,6 +636,7 @@ struct BackShared {
   uint4 s[4][DK / 8 * 32];  // a warp's dS', in two parts
   uint4 x[4][8 * 32];       // scale P^T dO from the helper, then dR to it
   uint4 q[4][DK / 8 * 32];  // scale (E dO)^T Q from the helper
+  uint64_t full[2];
 };
 // As the chain forward, from the last chunk to the first. The helpers' products, of dO with P and Q, need nothing of the chain.
 template <int DK>
@@ -626,13 +655,20 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
   seq_bounds(a, seq, from, to);
   const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
   const int u_ready = 1 + warp, q_ready = 5 + warp, r_ready = 9 + warp;
+  if (threadIdx.x == 0) {
+    tc::mbar_init(&sh.full[0], 1);
+    tc::mbar_init(&sh.full[1], 1);
+    tc::fence_mbar_init();
+  }
+  __syncthreads();
   if (chain) {
     float s[NK][4];  // dS'^T
     const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
     state_in(s, p.dfinal ? p.dfinal + sbase : nullptr, a.dk, a.dv, mine);
-    for (long c = chunks - 1; c >= 0; c--) {
-      ChainIn<DK>& in = sh.in[c & 1];
+    for (long c = chunks - 1, it = 0; c >= 0; c--, it++) {
+      ChainIn<DK>& in = sh.in[it & 1];
       meet<kChainThreads>(kAll);
+      tc::mbar_wait(&sh.full[it & 1], it >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
       float x[8][4];  // (K dS')^T: [16 of dv][64 tokens]
       zero(x);
       const uint32_t pk = smem_u32(in.k + lane_b<false, LD>());
@@ -646,8 +682,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
       meet<64>(u_ready);
 #pragma unroll
       for (int t = 0; t < 8; t++) {  // beta dU = beta (F K dS' + scale P^T dO)
-        const float2 b = *reinterpret_cast<const float2*>(in.m.beta + t * 8 + (lane & 3) * 2);
-        const float2 f = *reinterpret_cast<const float2*>(in.m.until + t * 8 + (lane & 3) * 2);
+        const float2 b = *reinterpret_cast<const float2*>(in.m.d.beta + t * 8 + (lane & 3) * 2);
+        const float2 f = *reinterpret_cast<const float2*>(in.m.d.until + t * 8 + (lane & 3) * 2);
         float u[4];
         take(sh.x[warp], t, u);
 #pragma unroll
@@ -664,7 +700,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
 #pragma unroll
       for (int t = 0; t < 8; t++) give(sh.x[warp], t, r[t]);
       meet_arrive<64>(r_ready);
-      const float keep = in.m.since[kC - 1];
+      const float keep = in.m.d.since[kC - 1];
 #pragma unroll
       for (int t = 0; t < NK; t++)
 #pragma unroll
@@ -674,7 +710,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
       for (int k = 0; k < 4; k++) {  // dS^T -= (E dR)^T K
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const float2 f = *reinterpret_cast<const float2*>(in.m.since + k * 16 + t * 8 + (lane & 3) * 2);
+          const float2 f = *reinterpret_cast<const float2*>(in.m.d.since + k * 16 + t * 8 + (lane & 3) * 2);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float fe = e & 1 ? f.y : f.x;
@@ -696,9 +732,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     return;
   }
   if (threadIdx.x < 256) {  // scale P^T dO and scale (E dO)^T Q
-    for (long c = chunks - 1; c >= 0; c--) {
-      ChainIn<DK>& in = sh.in[c & 1];
+    for (long it = 0; it < chunks; it++) {
+      ChainIn<DK>& in = sh.in[it & 1];
       meet<kChainThreads>(kAll);
+      tc::mbar_wait(&sh.full[it & 1], it >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
       const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>());
       uint32_t o[4][4];  // dO^T: [16 of dv][64 tokens]
 #pragma unroll
@@ -730,7 +767,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
         float eo[2][4];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-          const float2 f = *reinterpret_cast<const float2*>(in.m.since + k * 16 + t * 8 + (lane & 3) * 2);
+          const float2 f = *reinterpret_cast<const float2*>(in.m.d.since + k * 16 + t * 8 + (lane & 3) * 2);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float fe = e & 1 ? f.y : f.x;
@@ -749,13 +786,17 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
   // memory
   const int tid = threadIdx.x - 256, cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
   auto load = [&](long c) {
-    const long start = from + c * kC;
+    const long start = from + c * kC, it = chunks - 1 - c;
     const int len = (int)(to - start < kC ? to - start : kC);
-    ChainIn<DK>& in = sh.in[c & 1];
-    copy_tile<DK, LD, 128>(in.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vk, tid);
-    copy_flat<128>(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats), tid);
+    ChainIn<DK>& in = sh.in[it & 1];
+    uint64_t* bar = &sh.full[it & 1];
+    tc::fence_proxy_async_smem();
+    if (tid == 0) {
+      tc::mbar_expect_tx(bar, sizeof(Mats) + kTileBytes<DK>);
+      bulk_in(in.k, p.tiles + tile_at<DK>(a, slot0 + c, kh), kTileBytes<DK>, bar);
+      bulk_in(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats), bar);
+    }
     copy_tile<64, kLd, 128>(in.x, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.align_o, tid);
-    copy_tile<DK, LD, 128>(in.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
     cp_commit();
   };
   if (chunks) load(chunks - 1);
@@ -764,22 +805,22 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
   for (long c = chunks - 1; c >= 0; c--) {
     const long start = from + c * kC, slot = slot0 + c;
     const int len = (int)(to - start < kC ? to - start : kC);
-    ChainIn<DK>& in = sh.in[c & 1];
+    ChainIn<DK>& in = sh.in[(chunks - 1 - c) & 1];
     cp_wait<0>();
     meet<kChainThreads>(kAll);
     if (c > 0) load(c - 1);
     float r[8][4];
     meet<64>(r_ready);
-    __nv_bfloat16* to_s = p.ds + state_at(a, slot, h, slice) + warp * 16 * DK;
+    __nv_bfloat16* to_s = p.ds + state_at(a, slot, h, slice) + warp * 16 * LD;
 #pragma unroll
     for (int k = 0; k < DK / 8; k++) {
       uint32_t x[4];
       take(sh.s[warp], k, x);
-      part_out(x, to_s + (k & 1) * 64 * DK, DK, k / 2);
+      part_out(x, to_s + (k & 1) * 64 * LD, LD, k / 2);
     }
 #pragma unroll
     for (int t = 0; t < 8; t++) take(sh.x[warp], t, r[t]);
-    parts_out(r, p.dr + rows_at(a, slot, h, slice) + warp * 16 * 64, 64, 64l * 64);
+    parts_out(r, p.dr + rows_at(a, slot, h, slice) + warp * 16 * kLd, kLd, (long)kC * kLd);
     // the helper has read these columns of dO before the chain could give dR: dv takes their place on its way out
 #pragma unroll
     for (int n = 0; n < 4; n++) store_across(across_at(in.x + warp * 16, n), r[2 * n], r[2 * n + 1]);
@@ -797,6 +838,9 @@ struct GradArgs {
   long ldo, hso;
   int align_o;
   const __nv_bfloat16 *kept, *y, *ds, *dr;
+  const Mats* mats;
+  const __nv_bfloat16* tiles;
+  const int2* table;
   __nv_bfloat16 *dq, *dk;  // [n][hk][dk]
   float *dg, *dbeta;       // [n][hv]
 };
@@ -807,7 +851,8 @@ struct GradShared {
   __nv_bfloat16 s[2][kC * (DK + 8)], ds[2][kC * (DK + 8)], y[2][kC * kLd];  // transposed, as r
   __nv_bfloat16 p[2][kC * kLd], m[2][kC * kLd];     // scale dO U^T * D, -M
   float row[4][kC], col[4][kC], krow[4][kC], sum[16];
-  Decay d;
+  Decay decay[2];  // by turns, a head's
+  uint64_t full[2];  // S, dO, dR (and K, Q, the decays); dS', Y
 };
 // A block per chunk and key head, 16 warps: its value heads one after the other, so that what they add to dq and dk stays in
 // registers and is added in their order; of each, 64 columns of v after the other (a step). A step's loads are under
@@ -823,32 +868,41 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
   const DeltaArgs& a = p.d;
   const long slot = blockIdx.x;
   const int kh = blockIdx.y, group = a.hv / a.hk, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  long start;
-  const int len = slot_chunk(a, slot, start);
-  if (len == 0) return;
+  if (tid == 0) {
+    tc::mbar_init(&sh.full[0], 1);
+    tc::mbar_init(&sh.full[1], 1);
+    tc::fence_mbar_init();
+  }
+  const int2 chunk = p.table[slot];
+  const long start = chunk.x;
+  if (start < 0 || start >= a.n || chunk.y <= 0) return;  // (inside the tensors, whatever `saved` holds)
+  const int most = (int)(a.n - start < kC ? a.n - start : kC), len = chunk.y < most ? chunk.y : most;
   const int slices = a.dvp / 64, steps = group * slices;
-  auto load_a = [&](int t) {  // S, dO, dR
+  constexpr uint32_t kStateBytes = 2 * kC * LD * 2, kRowsBytes = 2 * kC * kLd * 2;
+  auto load_a = [&](int t) {  // S, dO, dR, a head's decays
     const int h = kh * group + t / slices, slice = t % slices, c0 = slice * 64;
     const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-    copy_tile<64, kLd, kGradThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.align_o, tid);
-#pragma unroll
-    for (int part = 0; part < 2; part++) {
-      tile_in<DK, LD, kGradThreads>(sh.s[part], p.kept + state_at(a, slot, h, slice) + part * 64 * DK);
-      tile_in<64, kLd, kGradThreads>(sh.r[t & 1][part], p.dr + rows_at(a, slot, h, slice) + part * kC * 64);
+    tc::fence_proxy_async_smem();  // what was there has been read the ordinary way
+    if (tid == 64) {
+      tc::mbar_expect_tx(&sh.full[0], kStateBytes + kRowsBytes + (slice == 0 ? sizeof(Decay) : 0) + (t == 0 ? kTileBytes<DK> : 0));
+      if (t == 0) bulk_in(sh.k, p.tiles + tile_at<DK>(a, slot, kh), kTileBytes<DK>, &sh.full[0]);
+      bulk_in(sh.s, p.kept + state_at(a, slot, h, slice), kStateBytes, &sh.full[0]);
+      bulk_in(sh.r[t & 1], p.dr + rows_at(a, slot, h, slice), kRowsBytes, &sh.full[0]);
+      if (slice == 0) bulk_in(&sh.decay[t / slices & 1], &p.mats[slot * a.hv + h].d, sizeof(Decay), &sh.full[0]);
     }
+    copy_tile<64, kLd, kGradThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.align_o, tid);
     cp_commit();
   };
   auto load_b = [&](int t) {  // dS', Y
     const int h = kh * group + t / slices, slice = t % slices;
-#pragma unroll
-    for (int part = 0; part < 2; part++) {
-      tile_in<DK, LD, kGradThreads>(sh.ds[part], p.ds + state_at(a, slot, h, slice) + part * 64 * DK);
-      tile_in<64, kLd, kGradThreads>(sh.y[part], p.y + rows_at(a, slot, h, slice) + part * kC * 64);
+    tc::fence_proxy_async_smem();
+    if (tid == 0) {
+      tc::mbar_expect_tx(&sh.full[1], kStateBytes + kRowsBytes);
+      bulk_in(sh.ds, p.ds + state_at(a, slot, h, slice), kStateBytes, &sh.full[1]);
+      bulk_in(sh.y, p.y + rows_at(a, slot, h, slice), kRowsBytes, &sh.full[1]);
     }
-    cp_commit();
   };
-  copy_tile<DK, LD, kGradThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vk, tid);
-  copy_tile<DK, LD, kGradThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
+  __syncthreads();
   load_a(0);
   load_b(0);
   const int wr = warp & 3, wc = warp >> 2, m0 = wr * 16, i0 = m0 + (lane >> 2);
@@ -860,13 +914,14 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     const int h = kh * group + t / slices;
     const __nv_bfloat16* o = sh.o[t & 1];
     const __nv_bfloat16* r = sh.r[t & 1][0];
+    const Decay& d = sh.decay[t / slices & 1];
     if (t % slices == 0) {
-      chunk_decay(a, sh.d, start, len, h);
       zero(oy);
       zero(ry);
       inner = qrow[0] = qrow[1] = krow[0] = krow[1] = 0.f;
     }
-    cp_wait<1>();
+    cp_wait<0>();
+    tc::mbar_wait(&sh.full[0], t & 1, a.err, PL_ERR_MBAR_TIMEOUT);
     __syncthreads();
     float x[NK][4];
     zero(x);
@@ -874,7 +929,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // scale E dO S^T, and what it adds to e_i
       const int i = i0 + half * 8;
-      const float f = sh.d.since[i] * a.scale;
+      const float f = d.since[i] * a.scale;
 #pragma unroll
       for (int n = 0; n < NK; n++) {
         const __nv_bfloat162 q = *reinterpret_cast<const __nv_bfloat162*>(sh.q + i * LD + d0 + n * 8 + (lane & 3) * 2);
@@ -889,7 +944,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // -E dR S^T
       const int i = i0 + half * 8;
-      const float f = -sh.d.since[i];
+      const float f = -d.since[i];
 #pragma unroll
       for (int n = 0; n < NK; n++) {
         const __nv_bfloat162 k = *reinterpret_cast<const __nv_bfloat162*>(sh.k + i * LD + d0 + n * 8 + (lane & 3) * 2);
@@ -899,8 +954,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
         dk[n][half * 2 + 1] += v1;
       }
     }
-    cp_wait<0>();
-    __syncthreads();
+    tc::mbar_wait(&sh.full[1], t & 1, a.err, PL_ERR_MBAR_TIMEOUT);
     for (int i = tid; i < kC * DK / 2; i += kGradThreads) {  // <S, dS'>
       const int at = i / (DK / 2) * LD + i % (DK / 2) * 2;
       auto two = [&](const __nv_bfloat16* hi, const __nv_bfloat16* lo) {
@@ -917,7 +971,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // F U dS'^T, and K_i . (dS' Y_i)
       const int i = i0 + half * 8;
-      const float f = sh.d.until[i], b = sh.d.beta[i];
+      const float f = d.until[i], b = d.beta[i];
 #pragma unroll
       for (int n = 0; n < NK; n++) {
         const __nv_bfloat162 k = *reinterpret_cast<const __nv_bfloat162*>(sh.k + i * LD + d0 + n * 8 + (lane & 3) * 2);
@@ -943,14 +997,14 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
       float col[2] = {0.f, 0.f};
 #pragma unroll
       for (int half = 0; half < 2; half++) {
-        const int i = i0 + half * 8, j = n0 + n * 8 + (lane & 3) * 2, ei = sh.d.era[i];
-        const float2 ci = sh.d.cum[i];
+        const int i = i0 + half * 8, j = n0 + n * 8 + (lane & 3) * 2, ei = d.era[i];
+        const float2 ci = d.cum[i];
         float po[2], mm[2];
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           const int e = half * 2 + c;
           const bool low = j + c <= i, strict = j + c < i;
-          const float f = low ? decay(ci, ei, sh.d, j + c) : 0.f, b = sh.d.beta[j + c];
+          const float f = low ? decay(ci, ei, d, j + c) : 0.f, b = d.beta[j + c];
           const float ov = low ? a.scale * f * oy[n][e] : 0.f, rv = strict ? f * ry[n][e] : 0.f;
           po[c] = b * ov;
           mm[c] = -b * rv;
@@ -990,7 +1044,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     product_part<false, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, 0, wr + 1);
     product_part<true, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, wr, 4);
     if (warp == 0) {  // dbeta, and dg by sums of W's rows less its columns from the chunk's end, cut at resets
-      const float keep = sh.d.since[kC - 1];
+      const float keep = d.since[kC - 1];
       float end = 0.f, sum[2];
       int era[2];
 #pragma unroll
@@ -1003,9 +1057,9 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
         const float kd = (sh.krow[0][i] + sh.krow[1][i]) + (sh.krow[2][i] + sh.krow[3][i]);
         const float c = (sh.col[0][i] + sh.col[1][i]) + (sh.col[2][i] + sh.col[3][i]);
         if (i < len) p.dbeta[(start + i) * a.hv + h] = kd + c;
-        tail += sh.d.beta[i] * kd;  // F_i u_i . (K_i dS')
-        sum[half] = (sh.row[0][i] + sh.row[1][i]) + (sh.row[2][i] + sh.row[3][i]) - sh.d.beta[i] * (kd + c);
-        era[half] = sh.d.era[i];
+        tail += d.beta[i] * kd;  // F_i u_i . (K_i dS')
+        sum[half] = (sh.row[0][i] + sh.row[1][i]) + (sh.row[2][i] + sh.row[3][i]) - d.beta[i] * (kd + c);
+        era[half] = d.era[i];
       }
 #pragma unroll
       for (int w = 16; w; w >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, w);
@@ -1031,25 +1085,29 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     }
     __syncthreads();
   }
+  // dq and dk leave by way of the places of K and Q, so that rows go out whole
 #pragma unroll
-  for (int half = 0; half < 2; half++) {
-    const int i = i0 + half * 8;
-    if (i >= len) continue;
-    const long to = ((start + i) * a.hk + kh) * a.dk;
+  for (int half = 0; half < 2; half++)
 #pragma unroll
     for (int n = 0; n < NK; n++) {
-      const int j = d0 + n * 8 + (lane & 3) * 2;
-      if (a.dk % 2 == 0 && j + 1 < a.dk) {
-        *reinterpret_cast<__nv_bfloat162*>(p.dq + to + j) = __floats2bfloat162_rn(dq[n][half * 2], dq[n][half * 2 + 1]);
-        *reinterpret_cast<__nv_bfloat162*>(p.dk + to + j) = __floats2bfloat162_rn(dk[n][half * 2], dk[n][half * 2 + 1]);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-          if (j + c < a.dk) {
-            p.dq[to + j + c] = __float2bfloat16_rn(dq[n][half * 2 + c]);
-            p.dk[to + j + c] = __float2bfloat16_rn(dk[n][half * 2 + c]);
-          }
-      }
+      const int at = (i0 + half * 8) * LD + d0 + n * 8 + (lane & 3) * 2;
+      *reinterpret_cast<__nv_bfloat162*>(sh.q + at) = __floats2bfloat162_rn(dq[n][half * 2], dq[n][half * 2 + 1]);
+      *reinterpret_cast<__nv_bfloat162*>(sh.k + at) = __floats2bfloat162_rn(dk[n][half * 2], dk[n][half * 2 + 1]);
+    }
+  __syncthreads();
+  const long row = (long)a.hk * a.dk, to = start * row + (long)kh * a.dk;
+  if (a.dk % 8 == 0 && (((uintptr_t)p.dq | (uintptr_t)p.dk) & 15) == 0) {
+    const int pieces = a.dk / 8;
+    for (int i = tid; i < len * pieces; i += kGradThreads) {
+      const int r = i / pieces, c = i % pieces * 8;
+      *reinterpret_cast<uint4*>(p.dq + to + r * row + c) = *reinterpret_cast<const uint4*>(sh.q + r * LD + c);
+      *reinterpret_cast<uint4*>(p.dk + to + r * row + c) = *reinterpret_cast<const uint4*>(sh.k + r * LD + c);
+    }
+  } else {
+    for (int i = tid; i < len * a.dk; i += kGradThreads) {
+      const int r = i / a.dk, c = i % a.dk;
+      p.dq[to + r * row + c] = sh.q[r * LD + c];
+      p.dk[to + r * row + c] = sh.k[r * LD + c];
     }
   }
 }
@@ -1111,6 +1169,7 @@ static DeltaArgs delta_args(const pl_delta_shape* s, const void* q, const void* 
   a.g = g;
   a.beta = beta;
   a.scale = (float)s->scale;
+  a.err = device_error_word();
   a.vq = row_align(q, s->q_token, s->q_head);
   a.vk = row_align(k, s->k_token, s->k_head);
   a.vv = row_align(v, s->v_token, s->v_head);
@@ -1120,11 +1179,22 @@ static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 static size_t heads_slots(const pl_delta_shape* s) {
   return (size_t)slot_count((long)s->tokens, (long)s->sequences) * s->heads_v;
 }
-static size_t mats_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * sizeof(Mats)); }
-static size_t states_bytes(const pl_delta_shape* s) {
-  return up256(heads_slots(s) * (s->dk > 64 ? 128 : 64) * round_up((long)s->dv, 64) * 4);
+static size_t slots_of(const pl_delta_shape* s) { return (size_t)slot_count((long)s->tokens, (long)s->sequences); }
+static size_t tiles_bytes(const pl_delta_shape* s) {
+  return up256(slots_of(s) * s->heads_k * (s->dk > 64 ? kTileBytes<128> : kTileBytes<64>));
 }
-static size_t rows_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * kC * round_up((long)s->dv, 64) * 4); }
+// Mats, one behind the other; behind them the tiles of K and Q, and the table of chunks.
+static size_t mats_bytes(const pl_delta_shape* s) {
+  return up256(heads_slots(s) * sizeof(Mats)) + tiles_bytes(s) + up256(slots_of(s) * sizeof(int2));
+}
+static __nv_bfloat16* tiles_of(const pl_delta_shape* s, Mats* mats) {
+  return (__nv_bfloat16*)((char*)mats + up256(heads_slots(s) * sizeof(Mats)));
+}
+static int2* table_of(const pl_delta_shape* s, Mats* mats) { return (int2*)((char*)tiles_of(s, mats) + tiles_bytes(s)); }
+static size_t states_bytes(const pl_delta_shape* s) {
+  return up256(heads_slots(s) * (s->dk > 64 ? 136 : 72) * round_up((long)s->dv, 64) * 4);
+}
+static size_t rows_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * kLd * round_up((long)s->dv, 64) * 4); }
 
 template <typename A>
 static int launch_wide(void (*kernel)(A), dim3 grid, int threads, size_t smem, cudaStream_t st, const A& args) {
@@ -1134,14 +1204,14 @@ static int launch_wide(void (*kernel)(A), dim3 grid, int threads, size_t smem, c
   count_launch();
   return PL_OK;
 }
-static int prep(const DeltaArgs& a, Mats* mats, cudaStream_t st) {
+static int prep(const DeltaArgs& a, Mats* mats, __nv_bfloat16* tiles, int2* table, cudaStream_t st) {
   const dim3 grid((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
   const bool wide = a.dk > 64;
   const size_t smem = wide ? sizeof(PrepShared<128>) : sizeof(PrepShared<64>);
   auto kernel = wide ? delta_prep_kernel<128> : delta_prep_kernel<64>;
   int rc = raise_smem((const void*)kernel, smem);
   if (rc) return rc;
-  PL_CUDA(launch_early(kernel, grid, dim3(kPrepThreads), smem, st, a, mats));
+  PL_CUDA(launch_early(kernel, grid, dim3(kPrepThreads), smem, st, a, mats, tiles, table));
   count_launch();
   return PL_OK;
 }
@@ -1160,11 +1230,11 @@ extern "C" {
 
 size_t pl_delta_saved(const pl_delta_shape* s) {
   if (!s || s->sequences == 0) return 0;
-  return pl::states_bytes(s) + pl::rows_bytes(s);
+  return pl::states_bytes(s) + pl::rows_bytes(s) + pl::mats_bytes(s);
 }
 size_t pl_delta_ws(const pl_delta_shape* s, uint8_t grad) {
   if (!s || s->sequences == 0) return 0;
-  return pl::mats_bytes(s) + (grad ? pl::states_bytes(s) + pl::rows_bytes(s) : 0);
+  return grad ? pl::states_bytes(s) + pl::rows_bytes(s) : pl::mats_bytes(s);
 }
 
 int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g, const float* beta,
@@ -1180,7 +1250,7 @@ int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const vo
   if (s->sequences == 0) return PL_OK;
   PL_REQUIRE(final_state && (s->tokens == 0 || (q && k && v && g && beta && o)), PL_ERR_INVALID,
              "%s: NULL inputs or results", me);
-  PL_REQUIRE(ws && (uintptr_t)ws % 256 == 0 && ws_bytes >= pl_delta_ws(s, 0), PL_ERR_INVALID,
+  PL_REQUIRE(saved || (ws && (uintptr_t)ws % 256 == 0 && ws_bytes >= pl_delta_ws(s, 0)), PL_ERR_INVALID,
              "%s: %zu bytes of workspace at 256 bytes needed", me, pl_delta_ws(s, 0));
   PL_REQUIRE(!saved || ((uintptr_t)saved % 256 == 0 && saved_bytes >= pl_delta_saved(s)), PL_ERR_INVALID,
              "%s: %zu bytes at 256 bytes needed for the gradient's states", me, pl_delta_saved(s));
@@ -1188,11 +1258,12 @@ int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const vo
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const DeltaArgs a = delta_args(s, q, k, v, g, beta, offsets);
+  Mats* mats = (Mats*)(saved ? (char*)saved + states_bytes(s) + rows_bytes(s) : ws);
   if (s->tokens) {
-    rc = prep(a, (Mats*)ws, st);
+    rc = prep(a, mats, tiles_of(s, mats), table_of(s, mats), st);
     if (rc) return rc;
   }
-  ScanArgs p = {a, (const Mats*)ws, state, (__nv_bfloat16*)o, final_state, nullptr, nullptr};
+  ScanArgs p = {a, mats, tiles_of(s, mats), state, (__nv_bfloat16*)o, final_state, nullptr, nullptr};
   if (saved) {
     p.kept = (__nv_bfloat16*)saved;
     p.y = (__nv_bfloat16*)((char*)saved + states_bytes(s));
@@ -1224,21 +1295,18 @@ int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const DeltaArgs a = delta_args(s, q, k, v, g, beta, offsets);
-  char* w = (char*)ws;
-  __nv_bfloat16 *ds = (__nv_bfloat16*)(w + mats_bytes(s)), *dr = (__nv_bfloat16*)(w + mats_bytes(s) + states_bytes(s));
+  __nv_bfloat16 *ds = (__nv_bfloat16*)ws, *dr = (__nv_bfloat16*)((char*)ws + states_bytes(s));
   const int align_o = row_align(dout, do_token, do_head);
-  if (s->tokens) {
-    rc = prep(a, (Mats*)ws, st);
-    if (rc) return rc;
-  }
-  const BackArgs b = {a, (const Mats*)ws, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, dfinal,
+  Mats* mats = (Mats*)((char*)saved + states_bytes(s) + rows_bytes(s));
+  const BackArgs b = {a, mats, tiles_of(s, mats), (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, dfinal,
                       (__nv_bfloat16*)dv, dstate, ds, dr};
   const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
   rc = a.dk > 64 ? launch_wide(delta_back_kernel<128>, grid, kChainThreads, sizeof(BackShared<128>), st, b)
                  : launch_wide(delta_back_kernel<64>, grid, kChainThreads, sizeof(BackShared<64>), st, b);
   if (rc || s->tokens == 0) return rc;
   const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, (const __nv_bfloat16*)saved,
-                      (const __nv_bfloat16*)((const char*)saved + states_bytes(s)), ds, dr, (__nv_bfloat16*)dq, (__nv_bfloat16*)dk,
+                      (const __nv_bfloat16*)((const char*)saved + states_bytes(s)), ds, dr, mats, tiles_of(s, mats), table_of(s, mats),
+                      (__nv_bfloat16*)dq, (__nv_bfloat16*)dk,
                       dg, dbeta};
   const dim3 chunks((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
   rc = a.dk > 64 ? launch_wide(delta_grad_kernel<128>, chunks, kGradThreads, sizeof(GradShared<128>), st, p)

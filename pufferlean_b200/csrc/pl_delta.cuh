@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "pl_common.cuh"
+#include "pl_tc.cuh"
 
 namespace pl {
 
@@ -18,6 +19,7 @@ struct DeltaArgs {
   const __nv_bfloat16 *q, *k, *v;
   const float *g, *beta;  // [n][hv]
   float scale;
+  unsigned* err;  // where a wait for copies that ran out is recorded
   int vq, vk, vv;  // bytes (16, 8, 4, 2) at whose multiples all rows of q, k, v start
 };
 
@@ -61,7 +63,7 @@ __device__ __forceinline__ int slot_chunk(const DeltaArgs& a, long slot, long& s
   return (int)(to - start < kC ? to - start : kC);
 }
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+using tc::smem_u32;
 __device__ __forceinline__ void cp16(void* dst, const void* src, int bytes) {  // the rest of the 16 bytes is zero
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
 }
@@ -108,16 +110,18 @@ __device__ __forceinline__ void copy_tile(__nv_bfloat16* dst, const __nv_bfloat1
     }
   }
 }
-// n bytes (a multiple of 16) as they lie.
-template <int THREADS>
-__device__ __forceinline__ void copy_flat(void* dst, const void* src, int n, int tid) {
-  for (int i = tid * 16; i < n; i += THREADS * 16) cp16((char*)dst + i, (const char*)src + i, 16);
+// Bulk copies: 16-byte aligned addresses, a multiple of 16 bytes; into shared memory `bar` counts the bytes that are there, out
+// of it the thread waits by bulk_read. One instruction of one thread, and no traffic through the load and store units,
+// which asynchronous copies of 16 bytes kept busy for a third of a chunk's time. (Row by row, 192 of them per chunk, they
+// were slower than those.)
+__device__ __forceinline__ void bulk_in(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
-// 64 rows of COLS values, one behind the other in memory, into a tile of row stride LD.
-template <int COLS, int LD, int THREADS>
-__device__ __forceinline__ void tile_in(__nv_bfloat16* tile, const __nv_bfloat16* src) {
-  for (int i = threadIdx.x; i < kC * COLS / 8; i += THREADS)
-    cp16(tile + i / (COLS / 8) * LD + i % (COLS / 8) * 8, src + i * 8, 16);
+__device__ __forceinline__ void bulk_out(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
 }
 
 // ---------------------------------------------------------------------------------------------- products
@@ -331,7 +335,7 @@ __device__ __forceinline__ void zero(float (&acc)[NT][4]) {
 // f64 and kept as two f32, so that differences of large sums are right), era (resets so far), since = the factor on
 // the state before the chunk (zero behind a reset), until = the factor from a token to the chunk's end (zero in front of a
 // reset). A g of -inf resets, and so does one below -104, whose factor f32 cannot hold.
-struct Decay {
+struct __align__(16) Decay {
   float2 cum[kC];
   int era[kC];
   float since[kC], until[kC], beta[kC];

@@ -486,7 +486,7 @@ PyObject* delta_rule(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t N = d.s.tokens, hv = d.s.heads_v, dk = d.s.dk, dv = d.s.dv;
     const On on(d.dev);
     at::Tensor out[3] = {fresh({N, hv, dv}, at::kBFloat16, d.dev), fresh({seqs, hv, dk, dv}, at::kFloat, d.dev), at::Tensor()};
-    const size_t size = pl_delta_ws(&d.s, 0), kept = pl_delta_saved(&d.s);
+    const size_t size = save ? 0 : pl_delta_ws(&d.s, 0), kept = pl_delta_saved(&d.s);
     const at::Tensor ws = bytes(size, d.dev);
     if (save) out[2] = bytes(kept, d.dev);
     check(pl_delta_dev(&d.s, d.q->data_ptr(), d.k->data_ptr(), d.v->data_ptr(), d.g, d.beta, (const int32_t*)offsets, state,
