@@ -18,12 +18,12 @@
 
 namespace pl {
 
-// sigmoid(g) and 1 - sigmoid(g), each to full relative precision
+// sigmoid(g), and with it 1 - sigmoid(g), each to full relative precision: e^-g is infinite where sigmoid(g) is zero.
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 __device__ __forceinline__ void sigmoid2(float g, float& a, float& na) {
-  const float t = __expf(-fabsf(g)), inv = __fdividef(1.f, 1.f + t), u = t * inv;
-  a = g >= 0.f ? inv : u;
-  na = g >= 0.f ? u : inv;
-  if (g != g) a = na = g;
+  const float t = __expf(-g);
+  a = __fdividef(1.f, 1.f + t);
+  na = g >= 0.f ? t * a : 1.f - a;
 }
 
 template <typename T>
@@ -88,11 +88,7 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR)) block_fwd
       if constexpr (GATE) {
         const Vec<VEC> f = widen<T, VEC>(ng[k]);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-          float a, na;
-          sigmoid2(f.v[j], a, na);
-          b[k].v[j] *= a;
-        }
+        for (int j = 0; j < VEC; j++) b[k].v[j] *= sigmoid(f.v[j]);
       }
     }
     load(row + step);
@@ -144,8 +140,8 @@ __global__ void __launch_bounds__(512) block_fwd_wide_kernel(const BlockArgs<T> 
   }
   s = 0.f;
   for (long c = threadIdx.x; c < p.cols; c += 512) {
-    float f = to_f(b[c]) * (p.w1 ? p.w1[c] * p.scale : p.scale), a = 1.f, na;
-    if (g) sigmoid2(to_f(g[c]), a, na);
+    float f = to_f(b[c]) * (p.w1 ? p.w1[c] * p.scale : p.scale);
+    const float a = g ? sigmoid(to_f(g[c])) : 1.f;
     const T v = from_f<T>(__fmaf_rn(f * a, rb, to_f(x[c])));
     r[c] = v;
     f = to_f(v);
@@ -357,8 +353,7 @@ __global__ void __launch_bounds__(256)
   float s1 = 0.f, s2 = 0.f;
   for (long row = blockIdx.y; row < p.rows; row += gridDim.y) {
     const float rr = p.rstd[row], rh = to_f(p.r[row * p.ldr + c]) * rr, dy = to_f(p.dy[row * p.lddy + c]);
-    float a = 1.f, na;
-    if (p.gate) sigmoid2(to_f(p.gate[row * p.ldg + c]), a, na);
+    const float a = p.gate ? sigmoid(to_f(p.gate[row * p.ldg + c])) : 1.f;
     const float d = (p.dr ? to_f(p.dr[row * p.lddr + c]) : 0.f) + (dy * w2 - rh * mean[row]) * rr;
     s1 = __fmaf_rn(d * p.scale * a, to_f(p.branch[row * p.ldb + c]) * (p.rstd_b ? p.rstd_b[row] : 1.f), s1);
     s2 = __fmaf_rn(dy, rh, s2);
@@ -394,37 +389,50 @@ static int bwd_launch(const BlockGradArgs<T>& p, float* dw1, float* dw2, cudaStr
   count_launch();
   return p.part ? param_launch(p.part, grid, p.cols, dw1, dw2, st) : PL_OK;
 }
-// The smallest group of threads whose registers hold a row: 8 values per thread as long as a block of 512 threads does,
-// then 16.
-#define PL_PICK(CALL)                      \
-  if (vec) {                               \
-    if constexpr (sizeof(T) == 2) {        \
-      if (cols <= 256) CALL(8, 32, 1);     \
-      if (cols <= 512) CALL(8, 64, 1);     \
-      if (cols <= 1024) CALL(8, 128, 1);   \
-      if (cols <= 2048) CALL(8, 256, 1);   \
-      if (cols <= 4096) CALL(8, 512, 1);   \
-      if (cols <= 8192) CALL(8, 512, 2);   \
-      if (cols <= 16384) CALL(8, 1024, 2); \
-    } else {                               \
-      if (cols <= 128) CALL(4, 32, 1);     \
-      if (cols <= 256) CALL(4, 32, 2);     \
-      if (cols <= 512) CALL(4, 64, 2);     \
-      if (cols <= 1024) CALL(4, 128, 2);   \
-      if (cols <= 2048) CALL(4, 256, 2);   \
-      if (cols <= 4096) CALL(4, 512, 2);   \
-      if (cols <= 8192) CALL(4, 512, 4);   \
-      if (cols <= 16384) CALL(4, 1024, 4); \
-    }                                      \
+// The smallest group of threads whose registers hold a row. Forward with 16 bf16 values per thread (65,536 x 2,048: 234 us, with
+// 8 282), backward with 8, since it has six rows' worth of values in flight (16: 482 -> 882 us, spills); more beyond a block of
+// 512 threads.
+#define PL_PICK_FWD(CALL)                  \
+  if constexpr (sizeof(T) == 2) {          \
+    if (cols <= 256) CALL(8, 32, 1);       \
+    if (cols <= 512) CALL(8, 32, 2);       \
+    if (cols <= 1024) CALL(8, 64, 2);      \
+    if (cols <= 2048) CALL(8, 128, 2);     \
+    if (cols <= 4096) CALL(8, 256, 2);     \
+    if (cols <= 8192) CALL(8, 512, 2);     \
+    if (cols <= 16384) CALL(8, 1024, 2);   \
   } else {                                 \
-    if (cols <= 128) CALL(1, 32, 4);       \
-    if (cols <= 512) CALL(1, 64, 8);       \
-    if (cols <= 1024) CALL(1, 128, 8);     \
-    if (cols <= 2048) CALL(1, 256, 8);     \
-    if (cols <= 4096) CALL(1, 512, 8);     \
-    if (cols <= 8192) CALL(1, 512, 16);    \
-    if (cols <= 16384) CALL(1, 1024, 16);  \
+    PL_PICK_F32(CALL)                      \
   }
+#define PL_PICK_BWD(CALL)                  \
+  if constexpr (sizeof(T) == 2) {          \
+    if (cols <= 256) CALL(8, 32, 1);       \
+    if (cols <= 512) CALL(8, 64, 1);       \
+    if (cols <= 1024) CALL(8, 128, 1);     \
+    if (cols <= 2048) CALL(8, 256, 1);     \
+    if (cols <= 4096) CALL(8, 512, 1);     \
+    if (cols <= 8192) CALL(8, 512, 2);     \
+    if (cols <= 16384) CALL(8, 1024, 2);   \
+  } else {                                 \
+    PL_PICK_F32(CALL)                      \
+  }
+#define PL_PICK_F32(CALL)                  \
+  if (cols <= 128) CALL(4, 32, 1);         \
+  if (cols <= 256) CALL(4, 32, 2);         \
+  if (cols <= 512) CALL(4, 64, 2);         \
+  if (cols <= 1024) CALL(4, 128, 2);       \
+  if (cols <= 2048) CALL(4, 256, 2);       \
+  if (cols <= 4096) CALL(4, 512, 2);       \
+  if (cols <= 8192) CALL(4, 512, 4);       \
+  if (cols <= 16384) CALL(4, 1024, 4);
+#define PL_PICK_SINGLE(CALL)               \
+  if (cols <= 128) CALL(1, 32, 4);         \
+  if (cols <= 512) CALL(1, 64, 8);         \
+  if (cols <= 1024) CALL(1, 128, 8);       \
+  if (cols <= 2048) CALL(1, 256, 8);       \
+  if (cols <= 4096) CALL(1, 512, 8);       \
+  if (cols <= 8192) CALL(1, 512, 16);      \
+  if (cols <= 16384) CALL(1, 1024, 16);
 
 static bool aligned16(const void* p) { return !p || ((uintptr_t)p & 15) == 0; }
 
@@ -436,7 +444,11 @@ static int fwd_pick(const BlockArgs<T>& p, cudaStream_t st) {
                    vec_ok(p.y, p.ldy, sizeof(T)) && aligned16(p.w1) && aligned16(p.w2) &&
                    (cols * sizeof(T)) % 16 == 0;
 #define PL_FWD(VEC, TPR, K) return fwd_launch<T, VEC, TPR, K>(p, st)
-  PL_PICK(PL_FWD)
+  if (vec) {
+    PL_PICK_FWD(PL_FWD)
+  } else {
+    PL_PICK_SINGLE(PL_FWD)
+  }
 #undef PL_FWD
   PL_CUDA(launch_early(block_fwd_wide_kernel<T>, (unsigned)p.rows, 512, 0, st, p));
   count_launch();
@@ -452,7 +464,11 @@ static int bwd_pick(BlockGradArgs<T>& p, float* dw1, float* dw2, float* ws, cuda
                    (!p.gate || (vec_ok(p.gate, p.ldg, sizeof(T)) && vec_ok(p.dg, p.lddg, sizeof(T)))) &&
                    aligned16(p.w1) && aligned16(p.w2) && (cols * sizeof(T)) % 16 == 0;
 #define PL_BWD(VEC, TPR, K) return bwd_launch<T, VEC, TPR, K>(p, dw1, dw2, st)
-  PL_PICK(PL_BWD)
+  if (vec) {
+    PL_PICK_BWD(PL_BWD)
+  } else {
+    PL_PICK_SINGLE(PL_BWD)
+  }
 #undef PL_BWD
   const int slices = (int)(p.rows < kWideSlices ? p.rows : kWideSlices);
   float* mean = p.part ? p.part + (long)slices * 2 * cols : nullptr;
@@ -464,7 +480,10 @@ static int bwd_pick(BlockGradArgs<T>& p, float* dw1, float* dw2, float* ws, cuda
   count_launch();
   return param_launch(p.part, slices, cols, dw1, dw2, st);
 }
-#undef PL_PICK
+#undef PL_PICK_FWD
+#undef PL_PICK_BWD
+#undef PL_PICK_F32
+#undef PL_PICK_SINGLE
 
 template <typename T>
 static int block_fwd(const void* x, size_t ldx, const void* branch, size_t ldb, const void* gate, size_t ldg,
