@@ -226,14 +226,26 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
   float kk[8][4], qk[8][4];  // rows 16 warp.. of K K^T and Q K^T, up to the diagonal's block
   zero(kk);
   zero(qk);
+  {
+    const uint32_t pk = smem_u32(sh.k + warp * 16 * LD + lane_a<false, LD>()), pq = pk + kC * LD * 2;
+    const uint32_t pb = smem_u32(sh.k + lane_b<false, LD>());
 #pragma unroll
-  for (int t = 0; t < 8; t += 2)
-    if (t / 2 <= warp) {
-      float(&kt)[2][4] = *reinterpret_cast<float(*)[2][4]>(kk + t);
-      float(&qt)[2][4] = *reinterpret_cast<float(*)[2][4]>(qk + t);
-      product<false, LD, 0, false, LD, 0, DK / 16>(kt, sh.k, sh.k, warp * 16, t * 8);
-      product<false, LD, 0, false, LD, 0, DK / 16>(qt, sh.q, sh.k, warp * 16, t * 8);
+    for (int k = 0; k < DK / 16; k++) {
+      uint32_t x[4], y[4];
+      ldsm<false>(x, pk + k * 32);
+      ldsm<false>(y, pq + k * 32);
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        if (n > warp) continue;
+        uint32_t b[4];
+        ldsm<false>(b, pb + n * 32 * LD + k * 32);
+        mma(kk[2 * n], x, b[0], b[1]);
+        mma(kk[2 * n + 1], x, b[2], b[3]);
+        mma(qk[2 * n], y, b[0], b[1]);
+        mma(qk[2 * n + 1], y, b[2], b[3]);
+      }
     }
+  }
   if (tid == 0) tc::bulk_wait_read<0>();  // the places of K and Q are used again
   for (int e = 0; e < group; e++) {
     const int h = kh * group + e;
@@ -288,7 +300,42 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
         for (int c = 16; c < 32; c += 4) *reinterpret_cast<float4*>(&sh.x[b + r][b + c]) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncthreads();
-    inverse_block<32, 128>(sh, sh.y, 32, 0, tid);
+    // the block below: -X22 (A21 X11), 4 x 4 values per thread, both first operands read along their rows: A21 lies transposed,
+    // and X22 is put so where `at` is not used
+    for (int i = tid; i < 32 * 32; i += kPrepThreads) sh.at[32 + (i & 31)][i >> 5] = sh.x[32 + (i >> 5)][32 + (i & 31)];
+    __syncthreads();
+    auto block_product = [&](const float (*m)[kC + 4], int m0, const float* c, int ldc, float sign, float (&s)[4][4]) {
+      const int i0 = m0 + (tid >> 3) * 4, j0 = (tid & 7) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[i][j] = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < 32; k++) {
+        const float4 u = *reinterpret_cast<const float4*>(&m[k][i0]), v = *reinterpret_cast<const float4*>(c + k * ldc + j0);
+        const float ui[4] = {sign * u.x, sign * u.y, sign * u.z, sign * u.w}, vj[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[i][j] = __fmaf_rn(ui[i], vj[j], s[i][j]);
+      }
+    };
+    if (tid < 64) {
+      float s[4][4];
+      block_product(sh.at, 32, sh.x[0], kC + 4, 1.f, s);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        *reinterpret_cast<float4*>(&sh.y[(tid >> 3) * 4 + i][(tid & 7) * 4]) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+    }
+    __syncthreads();
+    if (tid < 64) {
+      float s[4][4];
+      block_product(sh.at + 32, 0, sh.y[0], 36, -1.f, s);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        *reinterpret_cast<float4*>(&sh.x[32 + (tid >> 3) * 4 + i][(tid & 7) * 4]) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+    }
+    __syncthreads();
 #pragma unroll 5
     for (int i = tid; i < kTri / 2; i += kPrepThreads) {  // pair i of the ten blocks, in the order of rows and columns
       const int b = i >> 7, r = b < 1 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, c = b - r * (r + 1) / 2;
