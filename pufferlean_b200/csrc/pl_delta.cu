@@ -46,6 +46,17 @@ struct StepArgs {
 template <int VEC>
 struct __align__(4 * VEC) Floats {
   float v[VEC];
+  using Word = typename std::conditional<VEC == 4, float4, typename std::conditional<VEC == 2, float2, float>::type>::type;
+  // read and written once: past the caches (256 rows x 16 heads of 128 x 128: 105 -> 96 us)
+  __device__ __forceinline__ void load(const float* p) {
+    const Word w = __ldcs(reinterpret_cast<const Word*>(p));
+    memcpy(v, &w, sizeof(w));
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    Word w;
+    memcpy(&w, v, sizeof(w));
+    __stcs(reinterpret_cast<Word*>(p), w);
+  }
 };
 template <int VEC, int R>
 __global__ void __launch_bounds__(256) delta_step_kernel(const StepArgs p) {
@@ -65,7 +76,7 @@ __global__ void __launch_bounds__(256) delta_step_kernel(const StepArgs p) {
   for (int r = 0; r < R; r++) {
     const int i = warp + 8 * r;
     if (i < a.dk && in) {
-      x[r] = *reinterpret_cast<const Floats<VEC>*>(s + (long)i * a.dv + col);
+      x[r].load(s + (long)i * a.dv + col);
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; j++) x[r].v[j] = 0.f;
@@ -125,7 +136,7 @@ __global__ void __launch_bounds__(256) delta_step_kernel(const StepArgs p) {
     const float kk = qk[1][i];
 #pragma unroll
     for (int j = 0; j < VEC; j++) x[r].v[j] = __fmaf_rn(kk, u[j], x[r].v[j]);
-    *reinterpret_cast<Floats<VEC>*>(to + (long)i * a.dv + col) = x[r];
+    x[r].store(to + (long)i * a.dv + col);
   }
 }
 
@@ -212,10 +223,11 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
   const int len = slot_chunk(a, slot, start);
   if (kh == 0 && tid == 0) table[slot] = make_int2((int)start, len);
   if (len == 0) return;
+  const Gates gates = load_gates(a, start, len, kh * group);
   copy_tile<DK, LD, kPrepThreads>(sh.k, a.k + start * a.ldk + kh * a.hsk, a.ldk, len, a.dk, a.vk, tid);
   copy_tile<DK, LD, kPrepThreads>(sh.q, a.q + start * a.ldq + kh * a.hsq, a.ldq, len, a.dk, a.vq, tid);
   cp_commit();
-  chunk_decay(a, sh.d, start, len, kh * group);
+  chunk_decay(sh.d, gates);
   cp_wait<0>();
   tc::fence_proxy_async_smem();
   __syncthreads();
@@ -252,7 +264,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
     Mats& out = mats[slot * a.hv + h];
     __syncthreads();
     if (e) {
-      chunk_decay(a, sh.d, start, len, h);
+      chunk_decay(sh.d, load_gates(a, start, len, h));
       __syncthreads();
     }
     if (tid < (int)(sizeof(Decay) / 16)) reinterpret_cast<uint4*>(&out.d)[tid] = reinterpret_cast<const uint4*>(&sh.d)[tid];
@@ -287,7 +299,13 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
 #pragma unroll
       for (int j = 0; j < 15; j++)
 #pragma unroll
-        for (int i = j + 1; i < 16; i++) x[i] = __fmaf_rn(-sh.at[b + j][b + i], x[j], x[i]);
+        for (int i = (j + 1) & 12; i < 16; i += 4) {  // (up to the diagonal a row of `at` is zero)
+          const float4 f = *reinterpret_cast<const float4*>(&sh.at[b + j][b + i]);
+          x[i] = __fmaf_rn(-f.x, x[j], x[i]);
+          x[i + 1] = __fmaf_rn(-f.y, x[j], x[i + 1]);
+          x[i + 2] = __fmaf_rn(-f.z, x[j], x[i + 2]);
+          x[i + 3] = __fmaf_rn(-f.w, x[j], x[i + 3]);
+        }
 #pragma unroll
       for (int i = 0; i < 16; i++) sh.x[b + i][b + c] = x[i];
     }

@@ -345,7 +345,21 @@ __device__ __forceinline__ float exp2_of(float x) {  // 2^-22 off; zero below 2^
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
   return e;
 }
-__device__ __forceinline__ void chunk_decay(const DeltaArgs& a, Decay& d, long start, int len, int h) {
+struct Gates {
+  float g[2], beta[2];  // of tokens lane and lane + 32, in the block's first warp
+};
+__device__ __forceinline__ Gates load_gates(const DeltaArgs& a, long start, int len, int h) {
+  Gates r;
+#pragma unroll
+  for (int half = 0; half < 2; half++) {
+    const int t = half * 32 + threadIdx.x;
+    const bool in = threadIdx.x < 32 && t < len;
+    r.g[half] = in ? a.g[(start + t) * a.hv + h] : 0.f;
+    r.beta[half] = in ? a.beta[(start + t) * a.hv + h] : 0.f;
+  }
+  return r;
+}
+__device__ __forceinline__ void chunk_decay(Decay& d, const Gates& r) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     double cum[2];
@@ -353,8 +367,8 @@ __device__ __forceinline__ void chunk_decay(const DeltaArgs& a, Decay& d, long s
 #pragma unroll
     for (int half = 0; half < 2; half++) {
       const int t = half * 32 + lane;
-      const float g = t < len ? a.g[(start + t) * a.hv + h] : 0.f;
-      d.beta[t] = t < len ? a.beta[(start + t) * a.hv + h] : 0.f;
+      const float g = r.g[half];
+      d.beta[t] = r.beta[half];
       const bool reset = g < -104.f;
       cum[half] = reset ? 0.0 : (double)g * 1.4426950408889634074;
       era[half] = reset;

@@ -1036,10 +1036,11 @@ static int sample_variant(const SampleArgs& a, long rows, int ranks, cudaStream_
 }
 template <typename T>
 static int sample_launch(SampleArgs& a, long rows, cudaStream_t st) {
-  // Rows that leave more than half of the places for CTAs (two per SM) empty are split, as long as a part keeps 2,048 values; a part
-  // has to fit into shared memory.
+  // Rows that leave more than half of the places for CTAs (two per SM) empty are split in up to four, as long as a part keeps 2,048
+  // values (32 rows of 32,768 with top_k 50: 24 us whole, 27 in two, 23 in four, 33 in eight, whose barriers cost more;
+  // by mass alone 68, 62, 56 and 66); a part has to fit into shared memory.
   int ranks = 1;
-  while (ranks < 8 && a.V > 2048 * ranks && rows * ranks * 2 <= 2 * 148) ranks *= 2;
+  while (ranks < 4 && a.V > 2048 * ranks && rows * ranks * 2 <= 2 * 148) ranks *= 2;
   while (ranks > 1 && ranks < 8 && (long)a.V * sizeof(T) > 98304L * ranks) ranks *= 2;
   a.slice = (int)round_up(ceil_div(a.V, ranks), 8);
   return ranks == 1 ? sample_variant<T, true>(a, rows, 1, st) : sample_variant<T, false>(a, rows, ranks, st);
