@@ -200,6 +200,28 @@ def test_streams_capture_and_bits():
     assert all(torch.equal(a, b) for a, b in zip(g, want))
 
 
+def test_more_than_2_31_values():
+    """The last rows of a matrix whose offsets pass 32 bits are those of a small one; sums over all rows see each row once."""
+    rows, cols, last = 1_050_000, 2048, 5
+    small = _inputs(last, cols, BF16, True, 0, 0, 2)
+    big = [torch.zeros(rows, cols, device="cuda", dtype=BF16) if t.dim() == 2 else t for t in small]
+    for b, t in zip(big, small):
+        if b.dim() == 2:
+            b[rows - last:] = t
+    x, branch, gate, w1, w2, dr, dy = big
+    r, y, rb, rr = tokens.block_norm(x, branch, gate, w1, w2)
+    sr, sy, srb, srr = tokens.block_norm(small[0], small[1], small[2], w1, w2)
+    for a, b in ((r, sr), (y, sy), (rb, srb), (rr, srr)):
+        assert torch.equal(a[rows - last:], b)
+    del x, y
+    g = tokens.block_norm_grad(dr, dy, branch, gate, r, rb, rr, w1, w2)
+    sg = tokens.block_norm_grad(small[5], small[6], small[1], small[2], sr, srb, srr, w1, w2)
+    for a, b in zip(g[:3], sg[:3]):
+        assert torch.equal(a[rows - last:], b)
+    for a, b in zip(g[3:], sg[3:]):  # every other row adds exact zeros; the five rows' order differs
+        assert ((a - b).abs() <= 8 * F2 * 5 * (1 + b.abs())).all()
+
+
 def test_no_rows_and_refusals():
     x = torch.zeros(4, 16, device="cuda")
     w = torch.ones(16, device="cuda")

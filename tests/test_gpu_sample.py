@@ -217,6 +217,21 @@ def test_same_bits_streams_and_capture():
     assert torch.equal(out[0], torch.roll(want[1][0], 1)) and torch.equal(out[1], torch.roll(want[1][1], 1))
 
 
+def test_more_than_2_31_logits():
+    n, v = 16500, 131072
+    x = torch.empty(n, v, device="cuda", dtype=BF16)
+    tail, u = _logits(3, v, BF16, 12)
+    x[:-3] = 0
+    x[:, 5] = 30.0
+    x[-3:] = tail
+    us = torch.full((n,), 0.5, device="cuda")
+    us[-3:] = u
+    token, logp = tokens.sample(x, us, 1.0, 0, 0.9)
+    want = tokens.sample(tail, u, 1.0, 0, 0.9)
+    assert torch.equal(token[-3:], want[0]) and torch.equal(logp[-3:], want[1])
+    assert (token[:-3] == 5).all()
+
+
 def test_refusals():
     x, u = _logits(4, 64, F32, 1)
     k = torch.ones(4, dtype=torch.int64, device="cuda")
