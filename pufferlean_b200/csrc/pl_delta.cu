@@ -1020,14 +1020,20 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
       }
     }
     tc::mbar_wait(&sh.full[1], t & 1, a.err, PL_ERR_MBAR_TIMEOUT);
-    for (int i = tid; i < kC * DK / 2; i += kGradThreads) {  // <S, dS'>
-      const int at = i / (DK / 2) * LD + i % (DK / 2) * 2;
-      auto two = [&](const __nv_bfloat16* hi, const __nv_bfloat16* lo) {
-        const __nv_bfloat162 h2 = *reinterpret_cast<const __nv_bfloat162*>(hi + at), l2 = *reinterpret_cast<const __nv_bfloat162*>(lo + at);
-        return make_float2(__low2float(h2) + __low2float(l2), __high2float(h2) + __high2float(l2));
+#pragma unroll
+    for (int i = tid; i < kC * DK / 8; i += kGradThreads) {  // <S, dS'>, eight values at a time
+      const int at = i / (DK / 8) * LD + i % (DK / 8) * 8;
+      const uint4 sh4 = *reinterpret_cast<const uint4*>(sh.s[0] + at), sl4 = *reinterpret_cast<const uint4*>(sh.s[1] + at);
+      const uint4 dh4 = *reinterpret_cast<const uint4*>(sh.ds[0] + at), dl4 = *reinterpret_cast<const uint4*>(sh.ds[1] + at);
+      auto add = [&](uint32_t a, uint32_t b, uint32_t c, uint32_t e) {
+        inner = __fmaf_rn(__uint_as_float(a << 16) + __uint_as_float(b << 16), __uint_as_float(c << 16) + __uint_as_float(e << 16), inner);
+        a &= 0xffff0000u, b &= 0xffff0000u, c &= 0xffff0000u, e &= 0xffff0000u;
+        inner = __fmaf_rn(__uint_as_float(a) + __uint_as_float(b), __uint_as_float(c) + __uint_as_float(e), inner);
       };
-      const float2 u = two(sh.s[0], sh.s[1]), v = two(sh.ds[0], sh.ds[1]);
-      inner = __fmaf_rn(u.x, v.x, __fmaf_rn(u.y, v.y, inner));
+      add(sh4.x, sl4.x, dh4.x, dl4.x);
+      add(sh4.y, sl4.y, dh4.y, dl4.y);
+      add(sh4.z, sl4.z, dh4.z, dl4.z);
+      add(sh4.w, sl4.w, dh4.w, dl4.w);
     }
     __syncthreads();
     if (t + 1 < steps) load_a(t + 1);
@@ -1108,7 +1114,9 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     product_part<true, kLd, kRows, true, LD, 0>(dk, sh.p[0], sh.q, m0, d0, wr, 4);
     product_part<false, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, 0, wr + 1);
     product_part<true, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, wr, 4);
-    if (warp == 0) {  // dbeta, and dg by sums of W's rows less its columns from the chunk's end, cut at resets
+    // dbeta, and dg by sums of W's rows less its columns from the chunk's end, cut at resets: by the first warp, for the last head
+    // while the others write dq and dk
+    auto gates = [&] {
       const float keep = d.since[kC - 1];
       float end = 0.f, sum[2];
       int era[2];
@@ -1142,37 +1150,46 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
         }
         if (era[half] == behind_era) v += behind;
         const int i = half * 32 + lane;
-        const bool reset = i < len && a.g[(start + i) * a.hv + h] < -104.f;
+        const int before = __shfl_up_sync(0xffffffffu, era[half], 1), across = __shfl_sync(0xffffffffu, era[0], 31);
+        const bool reset = era[half] != (lane ? before : half ? across : 0);
         if (i < len) p.dg[(start + i) * a.hv + h] = reset ? 0.f : v;
         behind = __shfl_sync(0xffffffffu, v, 0);
         behind_era = __shfl_sync(0xffffffffu, era[half], 0);
       }
+    };
+    if (t + 1 < steps) {
+      if (warp == 0) gates();
+      __syncthreads();
+      continue;
     }
+    __syncthreads();  // dq and dk leave by way of the places of K and Q, so that rows go out whole
+#pragma unroll
+    for (int half = 0; half < 2; half++)
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        const int at = (i0 + half * 8) * LD + d0 + n * 8 + (lane & 3) * 2;
+        *reinterpret_cast<__nv_bfloat162*>(sh.q + at) = __floats2bfloat162_rn(dq[n][half * 2], dq[n][half * 2 + 1]);
+        *reinterpret_cast<__nv_bfloat162*>(sh.k + at) = __floats2bfloat162_rn(dk[n][half * 2], dk[n][half * 2 + 1]);
+      }
     __syncthreads();
-  }
-  // dq and dk leave by way of the places of K and Q, so that rows go out whole
-#pragma unroll
-  for (int half = 0; half < 2; half++)
-#pragma unroll
-    for (int n = 0; n < NK; n++) {
-      const int at = (i0 + half * 8) * LD + d0 + n * 8 + (lane & 3) * 2;
-      *reinterpret_cast<__nv_bfloat162*>(sh.q + at) = __floats2bfloat162_rn(dq[n][half * 2], dq[n][half * 2 + 1]);
-      *reinterpret_cast<__nv_bfloat162*>(sh.k + at) = __floats2bfloat162_rn(dk[n][half * 2], dk[n][half * 2 + 1]);
+    if (warp == 0) {
+      gates();
+      return;
     }
-  __syncthreads();
-  const long row = (long)a.hk * a.dk, to = start * row + (long)kh * a.dk;
-  if (a.dk % 8 == 0 && (((uintptr_t)p.dq | (uintptr_t)p.dk) & 15) == 0) {
-    const int pieces = a.dk / 8;
-    for (int i = tid; i < len * pieces; i += kGradThreads) {
-      const int r = i / pieces, c = i % pieces * 8;
-      *reinterpret_cast<uint4*>(p.dq + to + r * row + c) = *reinterpret_cast<const uint4*>(sh.q + r * LD + c);
-      *reinterpret_cast<uint4*>(p.dk + to + r * row + c) = *reinterpret_cast<const uint4*>(sh.k + r * LD + c);
-    }
-  } else {
-    for (int i = tid; i < len * a.dk; i += kGradThreads) {
-      const int r = i / a.dk, c = i % a.dk;
-      p.dq[to + r * row + c] = sh.q[r * LD + c];
-      p.dk[to + r * row + c] = sh.k[r * LD + c];
+    const long row = (long)a.hk * a.dk, to = start * row + (long)kh * a.dk;
+    if (a.dk % 8 == 0 && (((uintptr_t)p.dq | (uintptr_t)p.dk) & 15) == 0) {
+      const int pieces = a.dk / 8;
+      for (int i = tid - 32; i < len * pieces; i += kGradThreads - 32) {
+        const int r = i / pieces, c = i % pieces * 8;
+        *reinterpret_cast<uint4*>(p.dq + to + r * row + c) = *reinterpret_cast<const uint4*>(sh.q + r * LD + c);
+        *reinterpret_cast<uint4*>(p.dk + to + r * row + c) = *reinterpret_cast<const uint4*>(sh.k + r * LD + c);
+      }
+    } else {
+      for (int i = tid - 32; i < len * a.dk; i += kGradThreads - 32) {
+        const int r = i / a.dk, c = i % a.dk;
+        p.dq[to + r * row + c] = sh.q[r * LD + c];
+        p.dk[to + r * row + c] = sh.k[r * LD + c];
+      }
     }
   }
 }
