@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     bool inside;         // it touches neither the first nor the last bin
   };
   auto bins = [&](auto walk, auto weighing, bool by_octave, bool all, double want, double fuzz, bool share, float lo,
-                  float inv) __attribute__((always_inline)) {
+                  float inv, bool fine_fuzz = false) __attribute__((always_inline)) {
     constexpr bool by_mass = decltype(weighing)::value;
     const int octaves = (int)(__float_as_uint(fmaxf(750.f * (float)temp, 1e-30f)) >> 21) - (kBins - 1);
     for (int b = 0; b < kBins; b++) hist[b * kThreads + tid] = 0.f;
@@ -477,14 +477,29 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
       if (lane >= o) inc += up;
     }
     const double total = __shfl_sync(0xffffffffu, inc, 31);
-    const double target = share ? want * total : want, off = share ? fuzz * total : fuzz;
-    // the first bin by whose end the border can have come, and the first by whose end it must have
-    const double end0 = inc - bin[1], end1 = inc;
+    const double target = share ? want * total : want;
+    // the first bin by whose end the border can have come, and the first by whose end it must have. The weights are off by a
+    // share of what they are, so what lies behind the border is compared where that is less than what lies in front of it.
+    const bool behind = fine_fuzz && total - target < target;
+    double sum0 = inc - bin[1], sum1 = inc, goal = target, off = (fine_fuzz ? target : total) * fuzz;
+    if (behind) {
+      double suf = bin[0] + bin[1];
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const double down = __shfl_down_sync(0xffffffffu, suf, o);
+        if (lane + o < 32) suf += down;
+      }
+      const double rest = (1.0 - want) * total;
+      sum1 = -(suf - bin[0] - bin[1]);  // behind this lane's second bin
+      sum0 = sum1 - bin[1];
+      goal = -rest;
+      off = rest * fuzz;
+    }
     auto first_from = [&](double x) {
-      const unsigned m0 = __ballot_sync(0xffffffffu, end0 >= x), m1 = __ballot_sync(0xffffffffu, end1 >= x);
+      const unsigned m0 = __ballot_sync(0xffffffffu, sum0 >= x), m1 = __ballot_sync(0xffffffffu, sum1 >= x);
       return min(m0 ? 2 * (__ffs(m0) - 1) : kBins - 1, m1 ? 2 * (__ffs(m1) - 1) + 1 : kBins - 1);
     };
-    const int b0 = first_from(target - off), b1 = first_from(target + off);
+    const int b0 = first_from(goal - off), b1 = first_from(goal + off);
     double members = 0.0, until = 0.0;
 #pragma unroll
     for (int h = 0; h < 2; h++)
@@ -520,12 +535,13 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
   auto propose = [&](auto weighing, double want, bool share, bool all, float& za, float& zb) __attribute__((always_inline)) {
     constexpr bool by_mass = decltype(weighing)::value;
     const double fuzz = by_mass ? 3e-5 : 0.0;
-    Span r = bins(walk_all, weighing, !by_mass, all, want, fuzz, share, mass_lo, mass_inv);
+    // (from the largest logit to 42 T below it, where e is 1e-18 of the largest)
+    Span r = bins(walk_all, weighing, !by_mass, all, want, fuzz, share, 0.f, mass_inv * (24.f / 42.f), by_mass);
     for (int level = 1; level < 3; level++) {
-      const float d0 = fmaxf(r.d0, by_mass ? mass_lo : 0.f);
+      const float d0 = fmaxf(r.d0, 0.f);
       if (r.most <= 0.6 * kList || r.d1 == INFINITY || !(r.d1 > d0)) break;
       const float inv = fminf((float)(kBins - 2) / (r.d1 - d0), 1e30f), was0 = r.d0, was1 = r.d1;
-      r = bins(walk_all, weighing, false, all, want, fuzz, share, d0 - 1.f / inv, inv);
+      r = bins(walk_all, weighing, false, all, want, fuzz, share, d0 - 1.f / inv, inv, by_mass);
       r.d0 = fmaxf(r.d0, was0);  // the outer bins hold what is outside as well: there the ends stay
       r.d1 = fminf(r.d1, was1);
     }
@@ -875,7 +891,7 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
                       },
                       nothing);
           },
-          ByMass(), false, false, top_p, 3e-5, true, d0 - 1.f / inv, inv);
+          ByMass(), false, false, top_p, 3e-5, true, d0 - 1.f / inv, inv, true);
       top = max_of_all(m);
       known = true;
       if (bad(top)) {

@@ -84,7 +84,7 @@ def test_sizes_and_layouts(n, v, dtype, pad, offset):
 def test_widest(v, dtype):
     for sigma in (0.01, 1.0, 4.0):
         x, u = _logits(2, v, dtype, v, sigma=sigma)
-        for o in (dict(), dict(k=50, p=0.95), dict(p=0.9), dict(p=0.9999), dict(k=30000, p=0.5), dict(min_p=0.3)):
+        for o in (dict(), dict(k=50, p=0.95), dict(p=0.9), dict(p=0.9999), dict(p=0.9999999), dict(p=1e-4), dict(k=30000, p=0.5), dict(min_p=0.3)):
             _check(x, u, **o)
 
 
