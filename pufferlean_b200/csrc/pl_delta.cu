@@ -141,9 +141,11 @@ __global__ void __launch_bounds__(256) delta_step_kernel(const StepArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------- X and P of all chunks
-// Per slot and value head: X and P, triangular, as two bf16 parts each, and the decays; per slot and key head K and Q in rows as they stand in
-// shared memory, [2][64][dkp + 8], so that the other kernels get them by one bulk copy; per slot its chunk's first token and
-// length (0: none).
+// Per slot and value head: X and P, triangular, as two bf16 parts each, and the decays; per slot and key head K and Q in
+// rows as they stand in shared memory, [2][64][dkp + 8], so that the other kernels get them by one bulk copy; per slot its
+// chunk's first token and length (0: none).
+// Measured: 8,192 chunks of a head, dk = 128, in 210 us, where their 730 MB would take 110: a block's dozen steps (search,
+// copies, decays, two products, the inverse in blocks of 16 and 32) wait for one another, four blocks to an SM.
 struct __align__(16) Mats {
   __nv_bfloat16 x[2][kTri], p[2][kTri];
   Decay d;
@@ -171,8 +173,8 @@ struct PrepShared {
   };
   Decay d;
 };
-// out = -B (A C) for square blocks of S rows: A = at (transposed) at (r, c), C = x at (c, c), B = x at (r, r), out = x at (r, c); `n`
-// threads per block, thread t of it, `y` for A C.
+// out = -B (A C) for square blocks of S rows: A = at (transposed) at (r, c), C = x at (c, c), B = x at (r, r), out = x at
+// (r, c); N threads per block of the matrix, thread t of them; `y` for A C.
 template <int S, int N, typename Shared>
 __device__ __forceinline__ void inverse_block(Shared& sh, float (*y)[36], int r, int c, int t) {
   constexpr int E = S * S / N, P = S / E;  // values per thread, threads per row
@@ -211,7 +213,8 @@ __device__ __forceinline__ void inverse_block(Shared& sh, float (*y)[36], int r,
   __syncthreads();
 }
 template <int DK>
-__global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const DeltaArgs a, Mats* __restrict__ mats, __nv_bfloat16* __restrict__ tiles, int2* __restrict__ table) {
+__global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(
+    const DeltaArgs a, Mats* __restrict__ mats, __nv_bfloat16* __restrict__ tiles, int2* __restrict__ table) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
@@ -351,7 +354,8 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const Delta
       block_product(sh.at + 32, 0, sh.y[0], 36, -1.f, s);
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        *reinterpret_cast<float4*>(&sh.x[32 + (tid >> 3) * 4 + i][(tid & 7) * 4]) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+        *reinterpret_cast<float4*>(&sh.x[32 + (tid >> 3) * 4 + i][(tid & 7) * 4]) =
+            make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
     }
     __syncthreads();
 #pragma unroll 5
@@ -482,13 +486,14 @@ __device__ __forceinline__ uint32_t across_at(const __nv_bfloat16* tile, int n) 
   return smem_u32(tile + (n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * kLd + ((lane >> 3) & 1) * 8);
 }
 
-// A block per sequence, value head and 64 columns of v. A warp of the chain keeps 16 columns of the state, transposed [16][dk], in
-// registers for the whole sequence, and everything that a chunk makes of it: an accumulator's layout is that of a first
-// operand, so K S, R, Y and F U go from one product into the next as they are, split into two bf16 parts. What the next
-// chunk's state does not wait for is another warp's, which gets the state's parts and Y through shared memory: Q S and P U; a
-// third one's is what goes from and to memory. (All in one warp, a chunk took 5.5 us; with R, Y, U and the state's
-// parts in shared memory, shared by 16 warps in four steps with barriers, 5.6.) The products are 316 and 188 of 16 x 8 x 16
-// per chunk: 8 cycles each on a quarter of an SM.
+// A block per sequence, value head and 64 columns of v. A warp of the chain keeps 16 columns of the state, transposed
+// [16][dk], in registers for the whole sequence, and everything that a chunk makes of it: an accumulator's layout is that
+// of a first operand, so K S, R, Y and F U go from one product into the next as they are, split into two bf16 parts. What the
+// next chunk's state does not wait for is another warp's, which gets the state's parts and Y through shared memory: Q S
+// and P U; a third one's is what goes from and to memory.
+// A chunk takes 3.9 us, 6,600 clocks. Its products are 316 and 188 of 16 x 8 x 16 for each scheduler, 8 clocks each: 4,032.
+// (All in one warp it took 5.5 us; with R, Y, U and the state's parts in shared memory, shared by 16 warps in four steps with
+// barriers, 5.6.) 4 x 8,192 tokens of 16 heads of 128 x 128: 500 us, 128 of 148 SMs with a chain of 128 chunks each.
 template <int DK>
 __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const ScanArgs p) {
   grid_wait();
@@ -704,6 +709,7 @@ struct BackShared {
   uint64_t full[2];
 };
 // As the chain forward, from the last chunk to the first. The helpers' products, of dO with P and Q, need nothing of the chain.
+// 64 x 512 tokens of 8 heads of 128 x 128: 339 us (forward, with what the gradient needs written out: 328).
 template <int DK>
 __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const BackArgs p) {
   grid_wait();
@@ -921,7 +927,7 @@ struct GradShared {
 };
 // A block per chunk and key head, 16 warps: its value heads one after the other, so that what they add to dq and dk stays in
 // registers and is added in their order; of each, 64 columns of v after the other (a step). A step's loads are under
-// way during the one before it.
+// way during the one before it. 4,096 chunks of a head in 534 us: 35,000 clocks each, of which the products take 16,000.
 template <int DK>
 __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs p) {
   grid_wait();
@@ -949,7 +955,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
     tc::fence_proxy_async_smem();  // what was there has been read the ordinary way
     if (tid == 64) {
-      tc::mbar_expect_tx(&sh.full[0], kStateBytes + kRowsBytes + (slice == 0 ? sizeof(Decay) : 0) + (t == 0 ? kTileBytes<DK> : 0));
+      tc::mbar_expect_tx(&sh.full[0], kStateBytes + kRowsBytes + (slice == 0 ? sizeof(Decay) : 0) +
+                                          (t == 0 ? kTileBytes<DK> : 0));
       if (t == 0) bulk_in(sh.k, p.tiles + tile_at<DK>(a, slot, kh), kTileBytes<DK>, &sh.full[0]);
       bulk_in(sh.s, p.kept + state_at(a, slot, h, slice), kStateBytes, &sh.full[0]);
       bulk_in(sh.r[t & 1], p.dr + rows_at(a, slot, h, slice), kRowsBytes, &sh.full[0]);
@@ -1026,7 +1033,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
       const uint4 sh4 = *reinterpret_cast<const uint4*>(sh.s[0] + at), sl4 = *reinterpret_cast<const uint4*>(sh.s[1] + at);
       const uint4 dh4 = *reinterpret_cast<const uint4*>(sh.ds[0] + at), dl4 = *reinterpret_cast<const uint4*>(sh.ds[1] + at);
       auto add = [&](uint32_t a, uint32_t b, uint32_t c, uint32_t e) {
-        inner = __fmaf_rn(__uint_as_float(a << 16) + __uint_as_float(b << 16), __uint_as_float(c << 16) + __uint_as_float(e << 16), inner);
+        inner = __fmaf_rn(__uint_as_float(a << 16) + __uint_as_float(b << 16),
+                          __uint_as_float(c << 16) + __uint_as_float(e << 16), inner);
         a &= 0xffff0000u, b &= 0xffff0000u, c &= 0xffff0000u, e &= 0xffff0000u;
         inner = __fmaf_rn(__uint_as_float(a) + __uint_as_float(b), __uint_as_float(c) + __uint_as_float(e), inner);
       };
@@ -1114,8 +1122,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     product_part<true, kLd, kRows, true, LD, 0>(dk, sh.p[0], sh.q, m0, d0, wr, 4);
     product_part<false, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, 0, wr + 1);
     product_part<true, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, wr, 4);
-    // dbeta, and dg by sums of W's rows less its columns from the chunk's end, cut at resets: by the first warp, for the last head
-    // while the others write dq and dk
+    // dbeta, and dg by sums of W's rows less its columns from the chunk's end, cut at resets: by the first warp, for the last
+    // head while the others write dq and dk
     auto gates = [&] {
       const float keep = d.since[kC - 1];
       float end = 0.f, sum[2];
@@ -1387,7 +1395,8 @@ int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token
                  : launch_wide(delta_back_kernel<64>, grid, kChainThreads, sizeof(BackShared<64>), st, b);
   if (rc || s->tokens == 0) return rc;
   const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, (const __nv_bfloat16*)saved,
-                      (const __nv_bfloat16*)((const char*)saved + states_bytes(s)), ds, dr, mats, tiles_of(s, mats), table_of(s, mats),
+                      (const __nv_bfloat16*)((const char*)saved + states_bytes(s)), ds, dr, mats,
+                      tiles_of(s, mats), table_of(s, mats),
                       (__nv_bfloat16*)dq, (__nv_bfloat16*)dk,
                       dg, dbeta};
   const dim3 chunks((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);

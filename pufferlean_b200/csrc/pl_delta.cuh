@@ -295,8 +295,8 @@ __device__ __forceinline__ void take(const uint4* at, int piece, float (&r)[4]) 
   const uint4 v = at[piece * 32 + (threadIdx.x & 31)];
   r[0] = __uint_as_float(v.x), r[1] = __uint_as_float(v.y), r[2] = __uint_as_float(v.z), r[3] = __uint_as_float(v.w);
 }
-// Barrier `id` of THREADS threads: what those that arrive wrote before, those that wait see behind it. Every one of a round's threads
-// comes once, by one or the other.
+// Barrier `id` of THREADS threads: what those that arrive wrote before, those that wait see behind it. Each of them comes once
+// before any comes again, by one or the other.
 template <int THREADS>
 __device__ __forceinline__ void meet_arrive(int id) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory");

@@ -17,13 +17,15 @@
 // around the border. (2) A walk in f64 takes the masses above, in and below the interval and lists what lies in it. (3) If
 // these say that the border is inside, which they do but for a few rows in a million, the list is sorted and the border
 // is exact. If the proposal fails, more walks propose; if the list overflows (more equal logits than it holds), the
-// border's key is searched bit by bit. So sample and f32 sums cost time where they are off, never a token. top_k up to 1,024 takes
-// one walk: the sample gives a bound that surely more than k pass, and what passes it is listed and sorted.
+// border's key is searched bit by bit. So sample and f32 sums cost time where they are off, never a token. top_k up to 1,024
+// takes one walk: the sample gives a bound that surely more than k pass, and what passes it is listed and sorted.
 //
 // Exponents refer to the sample's largest logit instead of the row's: f64 has the room (2^900), and the walk that needs it
 // finds the largest on its way.
 //
-// Bound by the f64 pipe: one walk of 12 f64 operations per logit is 6 clocks per 32 logits on an SM.
+// Bound by instructions: the f64 walk is 45 per 32 logits (12 of them f64, 6 clocks of an SM's f64 pipe), the f32 walk 20, at
+// half an instruction per clock and scheduler. 1,024 x 131,072 bf16: 249 us without filters, 630 to 670 with top_p 0.9,
+// 174 with top_k 50 (HBM: 41); 2,047 x 50,021 f32 249 (63).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -91,7 +93,7 @@ struct Exp {
     int n[N];
     bool in[N];
 #pragma unroll
-    for (int j = 0; j < N; j++) {  // the f32's bits as a double (a conversion has a quarter of the rate); below 2^-126 it is off by as little
+    for (int j = 0; j < N; j++) {  // the f32's bits as a double (a conversion has a quarter of the rate); 2^-126 off near zero
       const uint32_t b = __float_as_uint(z[j]);
       y[j] = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + (896u << 20))), (int)(b << 29)) - ref;
     }
@@ -653,7 +655,10 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
       sort_list(n);
       double e[8], total;
 #pragma unroll
-      for (int j = 0; j < 8; j++) e[j] = 8 * tid + j < n ? (by_mass ? exp_of(of_key(~(uint32_t)(list[8 * tid + j] >> 32))) : 1.0) : 0.0;
+      for (int j = 0; j < 8; j++) {
+        const int i = 8 * tid + j;
+        e[j] = i < n ? (by_mass ? exp_of(of_key(~(uint32_t)(list[i] >> 32))) : 1.0) : 0.0;
+      }
       double at = above + list_scan(e, total);
       int mine = 0;
 #pragma unroll
@@ -804,8 +809,8 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
       search(false, 0.0, (double)k, INFINITY, zfloor);
   }
 
-  // ---- step 2: the f64 walk. Above [zb, za] what stays goes into sums by warp, segment of its iterations, and lane; the rest of it,
-  // and the members, into sums of their own.
+  // ---- step 2: the f64 walk. Above [zb, za] what stays goes into sums by warp, segment of its iterations, and lane; the
+  // members, and all of it, into sums of their own.
   const int seg_its = (its + kSegs - 1) / kSegs;
   double w3[3];  // mass above, in, and of all
   constexpr int kPlain = 0, kKept = 1, kListing = 2;
@@ -1052,8 +1057,8 @@ static int sample_variant(const SampleArgs& a, long rows, int ranks, cudaStream_
 }
 template <typename T>
 static int sample_launch(SampleArgs& a, long rows, cudaStream_t st) {
-  // Rows that leave more than half of the places for CTAs (two per SM) empty are split in up to four, as long as a part keeps 2,048
-  // values (32 rows of 32,768 with top_k 50: 24 us whole, 27 in two, 23 in four, 33 in eight, whose barriers cost more;
+  // Rows that leave more than half of the places for CTAs (two per SM) empty are split in up to four, as long as a part
+  // keeps 2,048 values (32 rows of 32,768 with top_k 50: 24 us whole, 27 in two, 23 in four, 33 in eight, whose barriers cost more;
   // by mass alone 68, 62, 56 and 66); a part has to fit into shared memory.
   int ranks = 1;
   while (ranks < 4 && a.V > 2048 * ranks && rows * ranks * 2 <= 2 * 148) ranks *= 2;
