@@ -156,6 +156,19 @@ def test_gradients_are_differences(post):
             assert abs((ends[0] - ends[1]) / (2 * h) - float(grad.reshape(-1)[at])) < 5e-3, (i, at)
 
 
+def test_weights_at_any_float():
+    """Weights that begin at 4 bytes take the single-value path: the same results to the rounding of its sums' order."""
+    x, branch, gate, w1, w2, dr, dy = _inputs(9, 256, F32, True, 0, 0, 4)
+    off = lambda w: torch.cat([w[:1], w])[1:]
+    assert off(w1).data_ptr() % 16
+    a = tokens.block_norm(x, branch, gate, w1, w2)
+    b = tokens.block_norm(x, branch, gate, off(w1), off(w2))
+    ga = tokens.block_norm_grad(dr, dy, branch, gate, a[0], a[2], a[3], w1, w2)
+    gb = tokens.block_norm_grad(dr, dy, branch, gate, a[0], a[2], a[3], off(w1), off(w2))
+    for p, q in zip(a + ga, b + gb):
+        assert ((p - q).abs() <= 64 * F2 * (1 + p.abs() + 16)).all()
+
+
 def test_extremes():
     """Gates at both ends, rows of zeros, infinities in one row that leave the others alone."""
     x = torch.randn(4, 64, device="cuda")

@@ -155,7 +155,8 @@ def test_resets(reset):
     assert (grads[3][g < -104] == 0).all()
 
 
-@pytest.mark.parametrize("layout", [dict(pad=8), dict(pad=3), dict(wide=8), dict(wide=5, pad=1)])
+@pytest.mark.parametrize("layout", [dict(pad=8), dict(pad=4), dict(pad=2), dict(pad=3), dict(wide=8), dict(wide=4),
+                                    dict(wide=2), dict(wide=5, pad=1)])
 def test_strides(layout):
     _check([100, 31], 2, 4, 64, 72, seed=11, **layout)
     _check([100, 31], 2, 2, 100, 40, seed=12, **layout)
@@ -260,6 +261,23 @@ def test_step(n, hk, hv, dk, dv):
     bad[0] = math.nan  # a reset forgets whatever was there
     o2, new2 = tokens.delta_rule_step(q, k, v, g, beta, bad, 0.3, out=bad)
     assert new2.data_ptr() == bad.data_ptr() and torch.equal(o2, o) and torch.equal(new2, new)
+
+
+def test_states_at_any_float():
+    """States that begin at 4 or 8 bytes give the same bits as aligned ones."""
+    q, k, v, g, beta, offsets, state, _, _ = _inputs([3], 1, 2, 32, 128, 4)
+    state = torch.randn(3, 2, 32, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    want = tokens.delta_rule_step(q, k, v, g, beta, state)
+    one = tokens.delta_rule(q, k, v, g, beta, offsets, state[:1].contiguous())
+    for shift in (1, 2, 3):
+        buf = torch.zeros(state.numel() + 4, device="cuda")
+        moved = buf[shift:shift + state.numel()].view_as(state)
+        moved.copy_(state)
+        o, new = tokens.delta_rule_step(q, k, v, g, beta, moved, out=moved)
+        assert torch.equal(new, want[1]) and (o.float() - want[0].float()).abs().max() <= B * want[0].float().abs().max()
+        moved.copy_(state)
+        again = tokens.delta_rule(q, k, v, g, beta, offsets, moved[:1])
+        assert torch.equal(again[0], one[0]) and torch.equal(again[1], one[1])
 
 
 def test_steps_are_the_sequence():
