@@ -15,10 +15,12 @@
 // the first one's result.
 //
 // Measured, 65,536 x 2,048 bf16 with gate: 211 to 234 us forward (97 to 88 % of a copy's 6,545 GB/s), 424 back (77 %); without a
-// gate 177 and 284; f32 with gate 396 and 646 (the copy's rate). Back, rows of 4,096, 8,192 and 16,384 bf16 columns reach 67,
-// 50 and 22 %: their registers spill.
+// gate 177 and 284; f32 with gate 396 and 646 (the copy's rate). Back, rows of 4,096, 8,192 and 16,384 bf16 columns, a cluster
+// of blocks each, reach 73, 68 and 59 %.
+#include <atomic>
 #include "pl_rows.cuh"
 #include "pl_runtime.h"
+#include "pl_tc.cuh"
 
 namespace pl {
 
@@ -169,34 +171,69 @@ struct BlockGradArgs {
   long rows, cols;
   T *dx, *db, *dg;
   long lddx, lddb, lddg;
-  float *part;  // [blocks][2][cols] column sums of the blocks' rows (dw1, dw2), or NULL
+  float *part;  // [clusters][2][cols] column sums of the clusters' rows (dw1, dw2), or NULL
+  long width;   // columns of a block: all, or of a cluster's block (rank width .. (rank + 1) width)
+  unsigned* err;
 };
 
-template <typename T, int VEC, int TPR, int K, bool GATE>
+// Sum over a row that C blocks of TPR threads share (a fixed order, the same in all of them). `scr` holds 32 floats, or one
+// per warp of the cluster, of the block's own for this call. The warps' sums go to the other blocks' shared memory with
+// their barrier's count of bytes, in its phase `phase`: a barrier of the cluster would wait for the rows' stores as well
+// (32,768 x 4,096 bf16 with gate back: 591 us instead of 449).
+template <int TPR, int C>
+__device__ __forceinline__ float row_sum(float v, float* scr, uint64_t* bar, uint32_t phase, int rank, unsigned* err) {
+  if constexpr (C == 1) {
+    return group_sum<TPR>(v, scr);
+  } else {
+    constexpr int NW = TPR / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) tc::mbar_expect_tx(bar, C * NW * 4);
+    v = warp_sum(v);
+    if (lane < C)
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(
+                       tc::cluster_addr(tc::smem_u32(scr + rank * NW + warp), lane)),
+                   "r"(__float_as_uint(v)), "r"(tc::cluster_addr(tc::smem_u32(bar), lane))
+                   : "memory");
+    v = tc::mbar_wait(bar, phase, err, PL_ERR_MBAR_TIMEOUT) ? 0.f : __int_as_float(0x7fffffff);  // NaN: no gradient
+#pragma unroll
+    for (int q = 0; q < (C * NW + 31) / 32; q++)
+      if (q * 32 + lane < C * NW) v += scr[q * 32 + lane];
+    return warp_sum(v);
+  }
+}
+
+// C: blocks per row, a cluster. A row's slot of `scr` is written again two rows later, by which time the writer has every
+// warp's sum of the next row, sent behind its reads of this one.
+template <typename T, int VEC, int TPR, int K, int C, bool GATE>
 __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR)) block_bwd_kernel(const BlockGradArgs<T> p) {
   grid_wait();
   grid_next();
   constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR;
-  constexpr bool KEEP_W = TPR < 1024;  // 64 registers do not hold the weights too: read from L1 for each row then
-  __shared__ float scr[2][2][32];      // [row parity][fold]
-  extern __shared__ float fold[];      // [G][2][TPR * VEC * K] (G > 1)
-  const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
+  static_assert(C == 1 || G == 1, "the rows of a cluster");
+  __shared__ float scr[2][2][C * TPR / 32 > 32 ? C * TPR / 32 : 32];  // [row parity][fold]
+  extern __shared__ float fold[];                                     // [G][2][TPR * VEC * K] (G > 1)
+  const int t = threadIdx.x % TPR, g = threadIdx.x / TPR, rank = C > 1 ? blockIdx.x % C : 0;
   const float inv = 1.f / (float)p.cols;
-  const long step = (long)gridDim.x * G;
+  const long first = (long)(blockIdx.x / C) * G, step = (long)(gridDim.x / C) * G, c0 = rank * p.width;
   const bool has_dr = p.dr != nullptr;
+  __shared__ uint64_t bar[2][2];
+  if constexpr (C > 1) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < 4; i++) tc::mbar_init(&bar[i >> 1][i & 1], 1);
+      tc::fence_mbar_init();
+    }
+    tc::cluster_sync();  // the others' barriers are there
+  }
   Vec<VEC> w1[K], w2[K], s1[K], s2[K];
   bool in_row[K];
-  auto load_w = [&](int k) {
-    const long c = (long)(k * TPR + t) * VEC;
-    w1[k] = w2[k] = vall<VEC>(1.f);
-    if (p.w1 && c < p.cols) load_param<VEC>(p.w1, c, w1[k].v);
-    if (p.w2 && c < p.cols) load_param<VEC>(p.w2, c, w2[k].v);
-  };
 #pragma unroll
   for (int k = 0; k < K; k++) {
-    in_row[k] = (long)(k * TPR + t) * VEC < p.cols;
+    const long c = c0 + (k * TPR + t) * VEC;
+    in_row[k] = c < p.cols && (C == 1 || c < c0 + p.width);
     s1[k] = s2[k] = vall<VEC>(0.f);
-    if (KEEP_W) load_w(k);
+    w1[k] = w2[k] = vall<VEC>(1.f);
+    if (p.w1 && in_row[k]) load_param<VEC>(p.w1, c, w1[k].v);
+    if (p.w2 && in_row[k]) load_param<VEC>(p.w2, c, w2[k].v);
   }
   Pack<T, VEC> nd[K], ny[K], nb[K], nr[K], ng[GATE ? K : 1];
   float nrb, nrr;
@@ -204,7 +241,7 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR)) block_bwd
     const bool ok = row < p.rows;
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      const long c = (long)(k * TPR + t) * VEC;
+      const long c = c0 + (k * TPR + t) * VEC;
       nd[k] = ny[k] = nb[k] = nr[k] = narrow<T, VEC>(vall<VEC>(0.f));
       if constexpr (GATE) ng[k] = nd[k];
       if (ok && in_row[k]) {
@@ -218,16 +255,16 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR)) block_bwd
     nrr = ok ? __ldg(p.rstd + row) : 0.f;
     nrb = ok ? (p.rstd_b ? __ldg(p.rstd_b + row) : 1.f) : 0.f;
   };
-  load((long)blockIdx.x * G + g);
+  load(first + g);
   int parity = 0;
-  for (long base = (long)blockIdx.x * G; base < p.rows; base += step, parity ^= 1) {
+  uint32_t phase = 0;  // of the barriers of this parity, a phase per use
+  for (long base = first; base < p.rows; base += step, phase ^= parity, parity ^= 1) {
     const long row = base + g;
     const float rr = nrr, rb = nrb;
     Vec<VEC> d[K], rh[K], gy[K], bh[K], c1[GATE ? K : 1], c2[GATE ? K : 1];
     Vec<VEC> s = vall<VEC>(0.f);
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      if (!KEEP_W) load_w(k);
       rh[k] = vmul(widen<T, VEC>(nr[k]), vall<VEC>(rr));
       gy[k] = widen<T, VEC>(ny[k]);
       s2[k] = vfma(gy[k], rh[k], s2[k]);
@@ -245,11 +282,11 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR)) block_bwd
       }
     }
     if constexpr (!GATE) load(row + step);
-    const float m1 = -inv * group_sum<TPR>(vsum(s), scr[parity][0]);
+    const float m1 = -inv * row_sum<TPR, C>(vsum(s), scr[parity][0], &bar[parity][0], phase, rank, p.err);
     s = vall<VEC>(0.f);
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      const long c = (long)(k * TPR + t) * VEC;
+      const long c = c0 + (k * TPR + t) * VEC;
       d[k] = vfma(vfma(rh[k], vall<VEC>(m1), gy[k]), vall<VEC>(rr), d[k]);
       if (row < p.rows && in_row[k]) narrow<T, VEC>(d[k]).store(p.dx + row * p.lddx + c);
       if constexpr (GATE) {
@@ -264,16 +301,17 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR)) block_bwd
     }
     if constexpr (GATE) load(row + step);  // (before the first fold the registers do not do for both: 470 us instead of 420)
     float m2 = 0.f;
-    if (p.rstd_b) m2 = -inv * group_sum<TPR>(vsum(s), scr[parity][1]);
+    if (p.rstd_b) m2 = -inv * row_sum<TPR, C>(vsum(s), scr[parity][1], &bar[parity][1], phase, rank, p.err);
     if (row < p.rows)
 #pragma unroll
       for (int k = 0; k < K; k++)
         if (in_row[k])
           narrow<T, VEC>(vmul(vfma(bh[k], vall<VEC>(m2), d[k]), vall<VEC>(rb)))
-              .store(p.db + row * p.lddb + (long)(k * TPR + t) * VEC);
+              .store(p.db + row * p.lddb + c0 + (k * TPR + t) * VEC);
   }
+  if constexpr (C > 1) tc::cluster_sync();  // none leaves while another may still send to it
   if (!p.part) return;
-  float* pw = p.part + (long)blockIdx.x * 2 * p.cols;
+  float* pw = p.part + (long)(blockIdx.x / C) * 2 * p.cols;
   if constexpr (G > 1) {
     constexpr int W = TPR * VEC * K;
 #pragma unroll
@@ -300,8 +338,8 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR)) block_bwd
     for (int k = 0; k < K; k++)
 #pragma unroll
       for (int j = 0; j < VEC; j++) {
-        const long c = (long)(k * TPR + t) * VEC + j;
-        if (c < p.cols) {
+        const long c = c0 + (k * TPR + t) * VEC + j;
+        if (in_row[k]) {
           pw[c] = s1[k].v[j];
           pw[p.cols + c] = s2[k].v[j];
         }
@@ -384,21 +422,60 @@ static int fwd_launch(const BlockArgs<T>& p, cudaStream_t st) {
   count_launch();
   return PL_OK;
 }
-template <typename T, int VEC, int TPR, int K>
-static int bwd_launch(const BlockGradArgs<T>& p, float* dw1, float* dw2, cudaStream_t st) {
+// Clusters of the kernel that the device holds at once, or 0 where it does not say. More in the grid than these would run when
+// the first are done, a whole share of the rows later: 37 clusters of four blocks, an SM each, leave four to a second turn
+// (8,192 x 16,384 bf16 with gate: 897 us, with the 33 that fit 558).
+static int resident_clusters(const void* kernel, std::atomic<int>* known, cudaLaunchConfig_t cfg, int c) {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if ((n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  cfg.gridDim = (unsigned)c;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 0;
+  }
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+template <typename T, int VEC, int TPR, int K, int C, bool GATE>
+static int bwd_launch(BlockGradArgs<T>& p, float* dw1, float* dw2, cudaStream_t st) {
   constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR;
   constexpr size_t FOLD = G > 1 ? (size_t)G * 2 * TPR * VEC * K * 4 : 0;
   static_assert(FOLD <= 48 * 1024, "column sums of the groups");
-  const long need = ceil_div(p.rows, G), most = (long)kNormSms * norm_blocks(TPR);
+  auto kernel = block_bwd_kernel<T, VEC, TPR, K, C, GATE>;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = THREADS;
+  cfg.dynamicSmemBytes = FOLD;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = C > 1 ? 2 : 1;
+  const long need = ceil_div(p.rows, G);
+  long most = (long)kNormSms * norm_blocks(TPR) / C;
+  if constexpr (C > 1) {
+    static std::atomic<int> known[64];
+    const int fit = resident_clusters((const void*)kernel, known, cfg, C);
+    if (fit > 0 && fit < most) most = fit;
+    p.err = device_error_word();
+  }
   const int grid = (int)(need < most ? need : most);
-  PL_CUDA(p.gate ? launch_early(block_bwd_kernel<T, VEC, TPR, K, true>, grid, THREADS, FOLD, st, p)
-                 : launch_early(block_bwd_kernel<T, VEC, TPR, K, false>, grid, THREADS, FOLD, st, p));
+  p.width = C > 1 ? round_up(ceil_div(p.cols, C), VEC) : p.cols;
+  cfg.gridDim = (unsigned)(grid * C);
+  PL_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
   count_launch();
   return p.part ? param_launch(p.part, grid, p.cols, dw1, dw2, st) : PL_OK;
 }
 // The smallest group of threads whose registers hold a row. Forward with 16 bf16 values per thread (65,536 x 2,048: 234 us, with
-// 8 282), backward with 8, since it has six rows' worth of values in flight (16: 482 -> 882 us, spills); more beyond a block of
-// 512 threads.
+// 8 282), backward with 8, since it has six rows' worth of values in flight (16: 482 -> 882 us, spills); more forward beyond
+// a block of 512 threads. Backward a row of more than 2,048 columns goes to a cluster, whose blocks keep these 8 (bf16 with
+// gate, 268 MB per matrix: 4,096 columns in a block of 512 threads 487 us, in two of 256 452; 8,192 with 16 values per thread
+// 649, two blocks 485; 16,384 1,490, four blocks 557). Without a gate the next row's load is on its way during the
+// first fold already, and one block is better at 4,096 columns (290 us, two blocks 316; f32 244, 304).
 #define PL_PICK_FWD(CALL)                  \
   if constexpr (sizeof(T) == 2) {          \
     if (cols <= 256) CALL(8, 32, 1);       \
@@ -413,16 +490,30 @@ static int bwd_launch(const BlockGradArgs<T>& p, float* dw1, float* dw2, cudaStr
   }
 #define PL_PICK_BWD(CALL)                  \
   if constexpr (sizeof(T) == 2) {          \
-    if (cols <= 256) CALL(8, 32, 1);       \
-    if (cols <= 512) CALL(8, 64, 1);       \
-    if (cols <= 1024) CALL(8, 128, 1);     \
-    if (cols <= 2048) CALL(8, 256, 1);     \
-    if (cols <= 4096) CALL(8, 512, 1);     \
-    if (cols <= 8192) CALL(8, 512, 2);     \
-    if (cols <= 16384) CALL(8, 1024, 2);   \
+    if (cols <= 256) CALL(8, 32, 1, 1);    \
+    if (cols <= 512) CALL(8, 64, 1, 1);    \
+    if (cols <= 1024) CALL(8, 128, 1, 1);  \
+    if (cols <= 2048) CALL(8, 256, 1, 1);  \
+    PL_PICK_CLUSTER(CALL, 8, 1)            \
   } else {                                 \
-    PL_PICK_F32(CALL)                      \
+    if (cols <= 128) CALL(4, 32, 1, 1);    \
+    if (cols <= 256) CALL(4, 32, 2, 1);    \
+    if (cols <= 512) CALL(4, 64, 2, 1);    \
+    if (cols <= 1024) CALL(4, 128, 2, 1);  \
+    if (cols <= 2048) CALL(4, 256, 2, 1);  \
+    PL_PICK_CLUSTER(CALL, 4, 2)            \
   }
+#define PL_PICK_BWD_SINGLE(CALL)           \
+  if (cols <= 128) CALL(1, 32, 4, 1);      \
+  if (cols <= 512) CALL(1, 64, 8, 1);      \
+  if (cols <= 1024) CALL(1, 128, 8, 1);    \
+  if (cols <= 2048) CALL(1, 256, 8, 1);    \
+  PL_PICK_CLUSTER(CALL, 1, 8)
+#define PL_PICK_CLUSTER(CALL, VEC, K)                                                     \
+  if (cols <= 4096 && !p.gate) return bwd_launch<T, VEC, 512, K, 1, false>(p, dw1, dw2, st); \
+  if (cols <= 4096) return bwd_launch<T, VEC, 256, K, 2, true>(p, dw1, dw2, st);             \
+  if (cols <= 8192) CALL(VEC, 512, K, 2);                                                 \
+  if (cols <= 16384) CALL(VEC, 512, K, 4);
 #define PL_PICK_F32(CALL)                  \
   if (cols <= 128) CALL(4, 32, 1);         \
   if (cols <= 256) CALL(4, 32, 2);         \
@@ -470,11 +561,13 @@ static int bwd_pick(BlockGradArgs<T>& p, float* dw1, float* dw2, float* ws, cuda
                    vec_ok(p.db, p.lddb, sizeof(T)) &&
                    (!p.gate || (vec_ok(p.gate, p.ldg, sizeof(T)) && vec_ok(p.dg, p.lddg, sizeof(T)))) &&
                    aligned16(p.w1) && aligned16(p.w2) && (cols * sizeof(T)) % 16 == 0;
-#define PL_BWD(VEC, TPR, K) return bwd_launch<T, VEC, TPR, K>(p, dw1, dw2, st)
+#define PL_BWD(VEC, TPR, K, C)                                                  \
+  return p.gate ? bwd_launch<T, VEC, TPR, K, C, true>(p, dw1, dw2, st)         \
+                : bwd_launch<T, VEC, TPR, K, C, false>(p, dw1, dw2, st)
   if (vec) {
     PL_PICK_BWD(PL_BWD)
   } else {
-    PL_PICK_SINGLE(PL_BWD)
+    PL_PICK_BWD_SINGLE(PL_BWD)
   }
 #undef PL_BWD
   const int slices = (int)(p.rows < kWideSlices ? p.rows : kWideSlices);
@@ -489,6 +582,8 @@ static int bwd_pick(BlockGradArgs<T>& p, float* dw1, float* dw2, float* ws, cuda
 }
 #undef PL_PICK_FWD
 #undef PL_PICK_BWD
+#undef PL_PICK_BWD_SINGLE
+#undef PL_PICK_CLUSTER
 #undef PL_PICK_F32
 #undef PL_PICK_SINGLE
 

@@ -132,6 +132,38 @@ def test_block(shape, dtype, layout):
         assert only[3] is None and only[4] is None and torch.equal(only[0], got[0]) and torch.equal(only[1], got[1])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(1100, 2056), (700, 2049), (700, 4096), (500, 4104), (500, 5003), (300, 8200), (200, 16384)])
+def test_many_wide_rows(shape, dtype):
+    """Rows that several blocks share, enough of them that each group of blocks has many one after the other."""
+    test_block(shape, dtype, "plain")
+
+
+@pytest.mark.parametrize("cols", [4096, 8192, 16384])
+def test_wide_rows_in_graphs_and_on_two_streams(cols):
+    x, branch, ga, w1, w2, dr, dy = _inputs(400, cols, BF16, True, 0, 0, cols)
+    r, y, rb, rr = tokens.block_norm(x, branch, ga, w1, w2, 1.0, 1e-5, True)
+    call = lambda: tokens.block_norm_grad(dr, dy, branch, ga, r, rb, rr, w1, w2, 1.0)
+    want = call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = call()
+    for _ in range(3):
+        for t in kept:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(kept, want))
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(call())
+    torch.cuda.synchronize()
+    for other in got:
+        assert all(torch.equal(a, b) for a, b in zip(other, want))
+    tokens.check()
+
+
 @pytest.mark.parametrize("post", [True, False])
 def test_gradients_are_differences(post):
     """Central differences of sum(r cr + y cy) in f32 rows: the step h = 1e-2 is off by h^2 of a third derivative of order one
