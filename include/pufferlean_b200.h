@@ -579,9 +579,9 @@ int pl_block_norm_grad_dev(const void* dr, size_t lddr, const void* dy, size_t l
  * first top_k stay (0, or V and more: all); of these those before which less than top_p of their mass comes (1 and more:
  * all); of these those with e_i >= min_p. The first always stays. token = the first that stays, by index, at which the sum
  * of the e that stay passes u times their total; logp = its log-probability among those that stay. Sums are f64.
- * Temperature 0 takes the first in that order (logp 0), one above 1e30 counts as 1e30, a min_p above 1 as 1, a u outside as the
- * nearer end. temperature, top_k, top_p, min_p [rows], or NULL: the number
- * beside it for all rows. A logit of -inf is never drawn. A row that holds a NaN or +inf, or -inf alone, or whose u or
+ * Temperature 0 takes the first in that order (logp 0), one between 0 and 1e-38 counts as 1e-38, one above 1e30 as 1e30, a min_p
+ * above 1 as 1, a u outside as the nearer end. temperature, top_k, top_p, min_p [rows], or NULL: the number beside it for all
+ * rows. A logit of -inf is never drawn. A row that holds a NaN or +inf, or -inf alone, or whose u or
  * options are NaN, whose temperature is negative or infinite, gets token -1 and logp NaN. */
 int pl_sample_dev(const void* logits, size_t ld, size_t rows, size_t V, uint8_t bf16, const float* u,
                   const float* temperature, double temperature_all, const int32_t* top_k, size_t top_k_all,

@@ -39,6 +39,7 @@ namespace pl {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 64, kList = 2048, kSegs = 16;
 constexpr int kMostVocab = 1 << 18;
+constexpr double kLeastTemp = 1e-38, kMostTemp = 1e30;  // a temperature beyond counts as these
 
 struct SampleArgs {
   const void* logits;
@@ -79,10 +80,17 @@ __device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either i
   return m;
 }
 
+// An f32 times 2^-896 as a double, by moving its bits (a conversion has a quarter of the rate): with the exponent's field as it
+// is, zeros and numbers below the smallest normal one are exact as well. -inf is -2^128.
+__device__ __forceinline__ double moved(float z) {
+  const uint32_t b = __float_as_uint(z);
+  return __hiloint2double((int)((b & 0x80000000u) | ((b & 0x7fffffffu) >> 3)), (int)(b << 29));
+}
+
 // exp((z - ref) / T) in f64: 2^y, y = n / 16 + r with 2^(n / 16) from a table and 2^r, |r| <= 1/32, from five terms of its series
-// (the sixth is 1.4e-13 of the value at most).
+// (the sixth is 1.4e-13 of the value at most). Both are moved alike, so that y is exactly zero for equal logits, whatever T.
 struct Exp {
-  double ref, c;  // c = log2(e) / T
+  double ref, c;  // ref 2^-896, log2(e) / T 2^896 (T >= kLeastTemp: below 2^1023)
   const double* tab;
   // N values step by step side by side: one after the other, each waits out the latency of a dozen f64 operations.
   template <int N>
@@ -93,10 +101,7 @@ struct Exp {
     int n[N];
     bool in[N];
 #pragma unroll
-    for (int j = 0; j < N; j++) {  // the f32's bits as a double (a conversion has a quarter of the rate); 2^-126 off near zero
-      const uint32_t b = __float_as_uint(z[j]);
-      y[j] = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + (896u << 20))), (int)(b << 29)) - ref;
-    }
+    for (int j = 0; j < N; j++) y[j] = moved(z[j]) - ref;
 #pragma unroll
     for (int j = 0; j < N; j++) y[j] *= c;
 #pragma unroll
@@ -184,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
   const double mp_given = a.min_p ? (double)a.min_p[row] : a.min_p0;
   const double u_given = (double)a.u[row];
   int k = a.k ? a.k[row] : a.k0;
-  double temp = fmin(t_given, 1e30), top_p = p_given, min_p = fmin(mp_given, 1.0);
+  double temp = fmin(t_given, kMostTemp), top_p = p_given, min_p = fmin(mp_given, 1.0);
   const double u = fmin(fmax(u_given, 0.0), 1.0);
   const bool fine = t_given >= 0.0 && t_given < INFINITY && p_given == p_given && mp_given == mp_given && u_given == u_given;
   if (temp == 0.0 || top_p <= 0.0) k = 1;  // the first in order alone
@@ -193,6 +198,7 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     top_p = 1.0;
     min_p = 0.0;
   }
+  temp = fmax(temp, kLeastTemp);
   if (k <= 0 || k >= a.V) k = 0;
 
   // ---- the slice: vectors of 16 bytes at 16-byte boundaries, a warp's together; around it -inf
@@ -339,16 +345,17 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     refuse();
     return;
   }
-  Exp exp_of = {(double)ref, 1.4426950408889634074 / temp, sh.tab};
-  const float cf = (float)fmin(exp_of.c, 1e37);
+  const double per_logit = 1.4426950408889634074 / temp;
+  Exp exp_of = {moved(ref), per_logit * 0x1p896, sh.tab};
+  const float cf = (float)fmin(per_logit, 1e37);
   float zfloor = ref - 750.f * (float)temp;  // below it every e is zero: such logits are left out of counts, too
   auto refer_to = [&](float z) {
     ref = z;
-    exp_of.ref = (double)z;
+    exp_of.ref = moved(z);
     zfloor = z - 750.f * (float)temp;
   };
   // After a walk that found `top`: whether the exponents were too far above their reference. (f64: 2^900; f32: 2^60)
-  auto too_far = [&](float most) { return ((double)top - (double)ref) * exp_of.c > (double)most; };
+  auto too_far = [&](float most) { return ((double)top - (double)ref) * per_logit > (double)most; };
 
   // ---- sums over the cluster, in rank order: N numbers per thread; every thread gets them
   int turn = 0;
@@ -795,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
             best = min(best, (unsigned)sh.iwarp[w]);
             back = max(back, __float_as_int(sh.fwarp[w][0]));
           }
-          const unsigned long long e1 = list[best != 0xffffffffu ? (int)best : back];
+          const unsigned long long e1 = list[best != 0xffffffffu ? (int)best : max(back, 0)];
           a.token[row] = (int)(e1 >> 32);
           a.logp[row] = (float)(((double)of_key((uint32_t)e1) - (double)ref) / temp - log(total));
         }
@@ -977,6 +984,10 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
     const double x = *of_rank(&sh.x[turn][0], q);
     if (x > 0.0 && from <= target) holder = q, before = from;
     from += x;
+  }
+  if (holder < 0) {  // no mass anywhere, though the largest logit's e is at least 1: an answer all the same
+    refuse();
+    return;
   }
   if (rank == holder && warp == 0) {
     const double up = __shfl_up_sync(0xffffffffu, inc, 1);

@@ -105,8 +105,9 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     row (f32; top_k int32). By falling logit, equal ones by index: the first top_k stay (0: all); of these those before
     which less than top_p of their mass comes; of these those with at least min_p of the largest probability; the first
     always. logp is the token's log-probability among those that stay, at this temperature (what an importance ratio
-    divides by). temperature 0 takes the first, one above 1e30 counts as 1e30, a min_p above 1 as 1. A logit of -inf is never drawn; a row with a NaN or +inf, with nothing but
-    -inf, or with an option that is NaN, gets token -1 and logp NaN."""
+    divides by). temperature 0 takes the first, one between 0 and 1e-38 counts as 1e-38, one above 1e30 as 1e30, a min_p above 1
+    as 1. A logit of -inf is never drawn; a row with a NaN or +inf, with nothing but -inf, or with an option that is NaN, gets
+    token -1 and logp NaN."""
     return _ext.sample(logits, u, temperature, top_k, top_p, min_p)
 
 

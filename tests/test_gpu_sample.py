@@ -177,6 +177,49 @@ def test_temperatures(temp):
         _check(x, u, temp=temp, **o)
 
 
+FILTERS = [dict(), dict(k=3), dict(k=1100), dict(p=0.85), dict(k=40, p=0.85, min_p=0.3), dict(min_p=0.45)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v", [(3, 37), (2, 5003), (301, 1300)])  # few rows: a cluster each, many: a block
+@pytest.mark.parametrize("top", [0.0, -0.0, 1e-40, -1e-40, 3.0])
+def test_tiniest_temperatures(top, n, v, dtype):
+    """The largest logit is zero, or next to it: equal logits (both zeros are one) share the mass at any temperature. (Below 1e-38
+    they count as that: it makes no difference to logits that are further apart than 1e-35.)"""
+    x, u = _logits(n, v, dtype, v)
+    x.sub_(x.max() + 1.0).add_(top)
+    for i, at in enumerate((0, 11, 12, 29, 36)):
+        x[:, at] = -top if top == 0.0 and i % 2 else top
+    for temp in (1e-22, 1e-30, 1e-36, 1e-38, 1e-40, 1.4e-45, 1e-61, 1e-100, 1e-310):
+        for o in FILTERS:
+            token = _check(x, u, temp=temp, **o)
+            assert (token >= 0).all()
+        if temp >= 1e-45:
+            _check(x, u, temp=torch.full((n,), temp, device="cuda"), p=torch.full((n,), 0.85, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v", [(2, 5003), (160, 1300)])
+@pytest.mark.parametrize("temp", [2e-22, 1e-22, 1e-30, 1e-36, 2.0 ** -126])
+def test_logits_as_small_as_the_temperature(temp, n, v, dtype):
+    """Logits of a few temperatures around zero, down to numbers below the smallest normal one."""
+    x, u = _logits(n, v, F32, v)
+    x = (x.double() * temp).to(dtype)
+    x[:, 5], x[:, 6] = 0.0, -0.0
+    for o in FILTERS:
+        _check(x, u, temp=temp, **o)
+
+
+def test_temperatures_below_the_least():
+    x, u = _logits(4, 700, F32, 3)
+    x = x * 1e-37 * 0.1  # differences of a few 1e-38
+    want = tokens.sample(x, u, 1e-38)
+    for temp in (9e-39, 1e-40, 1e-300, torch.full((4,), 1e-42, device="cuda")):
+        got = tokens.sample(x, u, temp)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    _check(x, u, temp=1e-38)
+
+
 @pytest.mark.parametrize("k,p,min_p", [(0, 1.0, 0.0), (6, 1.0, 0.0), (0, 0.8, 0.0), (0, 1.0, 0.1)])
 def test_shares(k, p, min_p):
     """Evenly spaced numbers give every token its share, to one draw."""
