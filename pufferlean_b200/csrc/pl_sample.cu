@@ -1089,7 +1089,7 @@ extern "C" int pl_sample_dev(const void* logits, size_t ld, size_t rows, size_t 
   PL_REQUIRE(V > 0 && V <= (size_t)kMostVocab, PL_ERR_INVALID, "%s: %zu tokens, 1 to %d wanted", me, V, kMostVocab);
   PL_REQUIRE(ld >= V, PL_ERR_INVALID, "%s: a row stride of %zu, below %zu tokens", me, ld, V);
   PL_REQUIRE(rows <= (1u << 27), PL_ERR_INVALID, "%s: %zu rows are too many", me, rows);
-  PL_REQUIRE(temperature || (temperature_all >= 0.0 && temperature_all <= 1e30), PL_ERR_INVALID, "%s: temperature = %g", me,
+  PL_REQUIRE(temperature || (temperature_all >= 0.0 && temperature_all < INFINITY), PL_ERR_INVALID, "%s: temperature = %g", me,
              temperature_all);
   PL_REQUIRE(top_p || top_p_all == top_p_all, PL_ERR_INVALID, "%s: top_p = %g", me, top_p_all);
   PL_REQUIRE(min_p || min_p_all == min_p_all, PL_ERR_INVALID, "%s: min_p = %g", me, min_p_all);

@@ -220,6 +220,14 @@ def test_temperatures_below_the_least():
     _check(x, u, temp=1e-38)
 
 
+def test_temperatures_above_the_most():
+    x, u = _logits(4, 700, F32, 3)
+    want = tokens.sample(x, u, 1e30, 0, 0.7)
+    for temp in (1e31, 1e300, torch.full((4,), 1e38, device="cuda")):
+        got = tokens.sample(x, u, temp, 0, 0.7)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("k,p,min_p", [(0, 1.0, 0.0), (6, 1.0, 0.0), (0, 0.8, 0.0), (0, 1.0, 0.1)])
 def test_shares(k, p, min_p):
     """Evenly spaced numbers give every token its share, to one draw."""

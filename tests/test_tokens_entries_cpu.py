@@ -42,6 +42,7 @@ def test_sample_arguments(L):
         assert call(**bad) == INVALID, bad
         assert L.pl_last_error()
     assert call(rows=0) == 0
+    assert call(rows=0, temp=1e31) == 0 and call(rows=0, temp=1e-310) == 0  # count as the largest and the least
     if plb.device_count() == 0:
         assert call() == NO_DEVICE
 
