@@ -24,12 +24,20 @@
 
 namespace pl {
 
-// sigmoid(g), and with it 1 - sigmoid(g), each to full relative precision: e^-g is infinite where sigmoid(g) is zero.
-__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+// sigmoid(g), and with it 1 - sigmoid(g), for rows of type T. The fast exponential is 2^-21 + |g| 2^-23 of its value off, which the
+// rounding of bf16 rows, 2^-8, hides; f32 rows get the exact one, and 6 units of 2^-23 at any g. The division is 2 units off at
+// most, and zero where sigmoid(g) is below 2^-126.
+template <typename T>
 __device__ __forceinline__ void sigmoid2(float g, float& a, float& na) {
-  const float t = __expf(-g);
+  const float t = sizeof(T) == 2 ? __expf(-g) : expf(-g);  // infinite where sigmoid(g) is zero
   a = __fdividef(1.f, 1.f + t);
   na = g >= 0.f ? t * a : 1.f - a;
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid(float g) {
+  float a, na;
+  sigmoid2<T>(g, a, na);
+  return a;
 }
 
 template <typename T>
@@ -94,7 +102,7 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR)) block_fwd
       if constexpr (GATE) {
         const Vec<VEC> f = widen<T, VEC>(ng[k]);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) b[k].v[j] *= sigmoid(f.v[j]);
+        for (int j = 0; j < VEC; j++) b[k].v[j] *= sigmoid<T>(f.v[j]);
       }
     }
     load(row + step);
@@ -147,7 +155,7 @@ __global__ void __launch_bounds__(512) block_fwd_wide_kernel(const BlockArgs<T> 
   s = 0.f;
   for (long c = threadIdx.x; c < p.cols; c += 512) {
     float f = to_f(b[c]) * (p.w1 ? p.w1[c] * p.scale : p.scale);
-    const float a = g ? sigmoid(to_f(g[c])) : 1.f;
+    const float a = g ? sigmoid<T>(to_f(g[c])) : 1.f;
     const T v = from_f<T>(__fmaf_rn(f * a, rb, to_f(x[c])));
     r[c] = v;
     f = to_f(v);
@@ -276,7 +284,7 @@ __global__ void __launch_bounds__(norm_threads(TPR), norm_blocks(TPR)) block_bwd
         const Vec<VEC> f = widen<T, VEC>(ng[k]);
         Vec<VEC> na;
 #pragma unroll
-        for (int j = 0; j < VEC; j++) sigmoid2(f.v[j], c1[k].v[j], na.v[j]);
+        for (int j = 0; j < VEC; j++) sigmoid2<T>(f.v[j], c1[k].v[j], na.v[j]);
         c1[k] = vmul(c1[k], vall<VEC>(p.scale));
         c2[k] = vmul(vmul(vmul(c1[k], na), bh[k]), w1[k]);
       }
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(512) block_bwd_wide_kernel(const BlockGradArgs
     bh = to_f(b[c]) * rb;
     a = 1.f;
     na = 0.f;
-    if (g) sigmoid2(to_f(g[c]), a, na);
+    if (g) sigmoid2<T>(to_f(g[c]), a, na);
     const float gy = to_f(dy[c]) * (p.w2 ? p.w2[c] : 1.f);
     return (dr ? to_f(dr[c]) : 0.f) + (gy - to_f(r[c]) * rr * m1) * rr;
   };
@@ -398,7 +406,7 @@ __global__ void __launch_bounds__(256)
   float s1 = 0.f, s2 = 0.f;
   for (long row = blockIdx.y; row < p.rows; row += gridDim.y) {
     const float rr = p.rstd[row], rh = to_f(p.r[row * p.ldr + c]) * rr, dy = to_f(p.dy[row * p.lddy + c]);
-    const float a = p.gate ? sigmoid(to_f(p.gate[row * p.ldg + c])) : 1.f;
+    const float a = p.gate ? sigmoid<T>(to_f(p.gate[row * p.ldg + c])) : 1.f;
     const float d = (p.dr ? to_f(p.dr[row * p.lddr + c]) : 0.f) + (dy * w2 - rh * mean[row]) * rr;
     s1 = __fmaf_rn(d * p.scale * a, to_f(p.branch[row * p.ldb + c]) * (p.rstd_b ? p.rstd_b[row] : 1.f), s1);
     s2 = __fmaf_rn(dy, rh, s2);

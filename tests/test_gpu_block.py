@@ -139,6 +139,22 @@ def test_many_wide_rows(shape, dtype):
     test_block(shape, dtype, "plain")
 
 
+@pytest.mark.parametrize("cols", [8, 1003, 4096, 20000])
+def test_f32_gates_at_any_size(cols):
+    """In f32 the gate's error does not grow with its size: an exponential and a division of at most two units each (2^-23), a sum
+    and a product of half a unit: 6 at most. sigmoid times 1 - sigmoid is t / (1 + t)^2: the exponential once, sum and division
+    twice, and up to four products and a difference: 10."""
+    g = torch.linspace(-80.0, 80.0, 3 * cols, device="cuda").view(3, cols)
+    one, zero = torch.ones_like(g), torch.zeros_like(g)
+    r, _, _, rstd = tokens.block_norm(zero, one, g, post=False)
+    a, na = torch.sigmoid(g.double()), torch.sigmoid(-g.double())
+    _close(r, a, 6 * F2 * a, "r")
+    dx, db, dg, _, _ = tokens.block_norm_grad(one, zero, one, g, r, None, rstd)
+    _close(dx, one.double(), 0 * a, "dx")
+    _close(db, a, 6 * F2 * a, "dbranch")
+    _close(dg, a * na, 10 * F2 * a * na, "dgate")
+
+
 @pytest.mark.parametrize("cols", [4096, 8192, 16384])
 def test_wide_rows_in_graphs_and_on_two_streams(cols):
     x, branch, ga, w1, w2, dr, dy = _inputs(400, cols, BF16, True, 0, 0, cols)
