@@ -420,13 +420,15 @@ __global__ void __launch_bounds__(256)
 constexpr long kBlockMost = 16384;  // the widest row that stays in registers
 constexpr int kWideSlices = 64;     // of the rows, for the column sums of wider ones
 
-template <typename T, int VEC, int TPR, int K>
+template <typename T, int VEC, int TPR, int K, bool GATED = true>
 static int fwd_launch(const BlockArgs<T>& p, cudaStream_t st) {
   constexpr int THREADS = norm_threads(TPR), G = THREADS / TPR;
   const long need = ceil_div(p.rows, G), most = (long)kNormSms * norm_blocks(TPR);
   const unsigned grid = (unsigned)(need < most ? need : most);
-  PL_CUDA(p.gate ? launch_early(block_fwd_kernel<T, VEC, TPR, K, true>, grid, THREADS, 0, st, p)
-                 : launch_early(block_fwd_kernel<T, VEC, TPR, K, false>, grid, THREADS, 0, st, p));
+  auto kernel = block_fwd_kernel<T, VEC, TPR, K, false>;
+  if constexpr (GATED)
+    if (p.gate) kernel = block_fwd_kernel<T, VEC, TPR, K, true>;
+  PL_CUDA(launch_early(kernel, grid, THREADS, 0, st, p));
   count_launch();
   return PL_OK;
 }
@@ -484,6 +486,10 @@ static int bwd_launch(BlockGradArgs<T>& p, float* dw1, float* dw2, cudaStream_t 
 // gate, 268 MB per matrix: 4,096 columns in a block of 512 threads 487 us, in two of 256 452; 8,192 with 16 values per thread
 // 649, two blocks 485; 16,384 1,490, four blocks 557). Without a gate the next row's load is on its way during the
 // first fold already, and one block is better at 4,096 columns (290 us, two blocks 316; f32 244, 304).
+// Forward, beyond 8,192 columns, a block of 1,024 threads has 64 registers for each: bf16 rows (spills of 208 bytes) and f32 rows
+// without a gate still gain by it (8,192 x 16,384: 342 us, the walk below 468; f32 501, 574). f32 rows with a gate and
+// rows without 16-byte loads do not, and are walked (604 bytes: 835 us, walked 683; 8,192 x 16,383 with gate bf16 641, 505, f32
+// 1,888, 708).
 #define PL_PICK_FWD(CALL)                  \
   if constexpr (sizeof(T) == 2) {          \
     if (cols <= 256) CALL(8, 32, 1);       \
@@ -530,15 +536,14 @@ static int bwd_launch(BlockGradArgs<T>& p, float* dw1, float* dw2, cudaStream_t 
   if (cols <= 2048) CALL(4, 256, 2);       \
   if (cols <= 4096) CALL(4, 512, 2);       \
   if (cols <= 8192) CALL(4, 512, 4);       \
-  if (cols <= 16384) CALL(4, 1024, 4);
+  if (cols <= 16384 && !p.gate) return fwd_launch<T, 4, 1024, 4, false>(p, st);
 #define PL_PICK_SINGLE(CALL)               \
   if (cols <= 128) CALL(1, 32, 4);         \
   if (cols <= 512) CALL(1, 64, 8);         \
   if (cols <= 1024) CALL(1, 128, 8);       \
   if (cols <= 2048) CALL(1, 256, 8);       \
   if (cols <= 4096) CALL(1, 512, 8);       \
-  if (cols <= 8192) CALL(1, 512, 16);      \
-  if (cols <= 16384) CALL(1, 1024, 16);
+  if (cols <= 8192) CALL(1, 512, 16);
 
 static bool aligned16(const void* p) { return !p || ((uintptr_t)p & 15) == 0; }
 
