@@ -324,13 +324,14 @@ __global__ void __launch_bounds__(kThreads, SOLO ? 3 : 2) sample_kernel(const Sa
   auto walk_max = [&]() __attribute__((always_inline)) {
     float m = -INFINITY;
     walk_part(Four(), warp, 0, its, [&](const float(&z)[VEC], uint32_t) { m = largest(z, m); }, nothing);
-    ref = top = max_of_all(m);
+    top = max_of_all(m);
   };
   const bool plain = k == 0 && top_p >= 1.0 && min_p <= 0.0;
   const bool few = k > 0 && k <= kList / 2, nucleus = k == 0 && top_p < 1.0;
   bool known = false;  // whether `top` is of all
   if (ref == -INFINITY || !(plain || few || nucleus)) {
     walk_max();
+    ref = top;
     known = true;
   }
   auto bad = [&](float z) { return !(fabsf(z) < INFINITY); };

@@ -142,6 +142,21 @@ def test_masks():
             assert (token == -1).all() if masked == -math.inf else (token >= 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v", [(3, 9001), (2, 50021), (150, 9001), (150, 20011)])
+def test_few_tokens_left(n, v, dtype):
+    """All but a few tokens share one value, a mask's or another, and the rest are wherever a sample of the row may miss them."""
+    g = torch.Generator(device="cuda").manual_seed(v + n)
+    u = torch.rand(n, generator=g, device="cuda")
+    for masked in (torch.finfo(dtype).min, -1e9, -700.0, -5.0):
+        for left in (1, 3):
+            x = torch.full((n, v), masked, device="cuda", dtype=dtype)
+            at = torch.randint(0, v, (n, left), generator=g, device="cuda")
+            x.scatter_(1, at, torch.randn(n, left, generator=g, device="cuda").to(dtype))
+            for o in (dict(), dict(k=2), dict(k=50), dict(k=3000), dict(p=0.9), dict(k=50, p=0.5, min_p=0.1), dict(min_p=0.1)):
+                _check(x, u, **o)
+
+
 def test_bad_rows():
     x, u = _logits(9, 300, F32, 1)
     x[0, 7] = math.nan
