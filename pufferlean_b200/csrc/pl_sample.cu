@@ -8,8 +8,8 @@
 // Every sum is f64, and so is every exponential behind one: a row of V near-equal tokens has V borders, and f32 sums
 // (1e-7 off) would move one of them across u in 2 rows of 100 at V = 131,072.
 //
-// Many rows: a CTA per row, which walks it from L2 for each step below (the rows in flight fit there). Few rows: a cluster
-// of CTAs per row, each with a contiguous slice in shared memory.
+// Many rows, and short ones: a CTA per row, which walks it from L2 for each step below (the rows in flight fit there). Few long
+// rows: a cluster of CTAs per row, each with a contiguous slice in shared memory.
 //
 // Without filters that is one walk with f64 sums by warp, segment and lane; the segment of u's place is walked once more.
 // The border of top-k or top-p is found in three steps. (1) A sample of the row and a walk with f32 weights put counts or
@@ -1069,12 +1069,19 @@ static int sample_variant(const SampleArgs& a, long rows, int ranks, cudaStream_
 }
 template <typename T>
 static int sample_launch(SampleArgs& a, long rows, cudaStream_t st) {
-  // Rows that leave more than half of the places for CTAs (two per SM) empty are split in up to four, as long as a part
-  // keeps 2,048 values (32 rows of 32,768 with top_k 50: 24 us whole, 27 in two, 23 in four, 33 in eight, whose barriers cost more;
-  // by mass alone 68, 62, 56 and 66); a part has to fit into shared memory.
-  int ranks = 1;
-  while (ranks < 4 && a.V > 2048 * ranks && rows * ranks * 2 <= 2 * 148) ranks *= 2;
-  while (ranks > 1 && ranks < 8 && (long)a.V * sizeof(T) > 98304L * ranks) ranks *= 2;
+  // Few rows are split over clusters of four, in parts of 4,096 values and more, as long as the clusters fit on the device at once
+  // (66 of four at two CTAs per SM; more run when the first are done). us whole / in four:
+  //              bf16 rows of 8,192   16,384     32,768     65,536     131,072     f32 of 32,768   65,536
+  //   top_k 50,  32 rows  18 / 22     22 / 23    25 / 24    31 / 28    45 / 33     32 / 25         39 / 30
+  //              64       17 / 25     22 / 25    25 / 26    32 / 31    58 / 60     27 / 28         41 / 55
+  //              100      18 / 44     22 / 46    25 / 48    37 / 55    48 / 106    32 / 51         39 / 101
+  //   top_p,     32       35 / 38     64 / 46    69 / 49    115 / 60   202 / 85    74 / 62         124 / 65
+  //              64       39 / 45     51 / 53    69 / 60    113 / 77   202 / 153   75 / 64         124 / 110
+  //              100      39 / 76     55 / 79    81 / 93    114 / 120  202 / 225   78 / 91         124 / 164
+  // Clusters of two gained up to a tenth between 75 and 148 rows of 32,768 and lost as much and more elsewhere. A part has to fit
+  // into shared memory: rows of more than 384 KB go in eight (131,072 f32, top_p, 32 rows 234 / 150, 64 226 / 267).
+  const int parts = (long)a.V * sizeof(T) > 4 * 98304L ? 8 : 4;
+  const int ranks = a.V >= 16384 && rows * parts <= 264 ? parts : 1;
   a.slice = (int)round_up(ceil_div(a.V, ranks), 8);
   return ranks == 1 ? sample_variant<T, true>(a, rows, 1, st) : sample_variant<T, false>(a, rows, ranks, st);
 }

@@ -95,6 +95,20 @@ def test_many_rows():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v", [(4, 16383), (4, 16384), (66, 16400), (67, 16400), (33, 131072), (34, 98311), (3, 200003)])
+def test_both_sides_of_a_split(n, v, dtype):
+    """Rows are split over several blocks from a length and up to a number of rows on: the same tokens on either side."""
+    x, u = _logits(n, v, dtype, n + v, pad=3)
+    for o in (dict(), dict(temp=0.8, k=50, p=0.95), dict(p=0.9)):
+        a = tokens.sample(x, u, *(o.get(key, d) for key, d in (("temp", 1.0), ("k", 0), ("p", 1.0))))
+        _check(x[:4], u[:4], **o)
+        many = 70 if n < 70 else n
+        b = tokens.sample(x.repeat(-(-many // n), 1)[:many], u.repeat(-(-many // n))[:many],
+                          *(o.get(key, d) for key, d in (("temp", 1.0), ("k", 0), ("p", 1.0))))
+        assert torch.equal(a[0], b[0][:n]) and (a[1] - b[1][:n]).abs().max() <= 2.0 ** -22 * a[1].abs().max()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("v", [64, 5000, 131072])
 def test_equal_logits(dtype, v):
     """Borders inside groups of equal logits, down to rows of one value: the lowest indices stay."""
@@ -196,7 +210,7 @@ FILTERS = [dict(), dict(k=3), dict(k=1100), dict(p=0.85), dict(k=40, p=0.85, min
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n,v", [(3, 37), (2, 5003), (301, 1300)])  # few rows: a cluster each, many: a block
+@pytest.mark.parametrize("n,v", [(3, 37), (2, 20011), (301, 1300)])  # a long row: a cluster, otherwise a block
 @pytest.mark.parametrize("top", [0.0, -0.0, 1e-40, -1e-40, 3.0])
 def test_tiniest_temperatures(top, n, v, dtype):
     """The largest logit is zero, or next to it: equal logits (both zeros are one) share the mass at any temperature. (Below 1e-38
@@ -214,7 +228,7 @@ def test_tiniest_temperatures(top, n, v, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n,v", [(2, 5003), (160, 1300)])
+@pytest.mark.parametrize("n,v", [(2, 20011), (160, 1300)])
 @pytest.mark.parametrize("temp", [2e-22, 1e-22, 1e-30, 1e-36, 2.0 ** -126])
 def test_logits_as_small_as_the_temperature(temp, n, v, dtype):
     """Logits of a few temperatures around zero, down to numbers below the smallest normal one."""
