@@ -580,8 +580,8 @@ int pl_block_norm_grad_dev(const void* dr, size_t lddr, const void* dy, size_t l
  * all); of these those with e_i >= min_p. The first always stays. token = the first that stays, by index, at which the sum
  * of the e that stay passes u times their total; logp = its log-probability among those that stay. Sums are f64.
  * Temperature 0 takes the first in that order (logp 0), one between 0 and 1e-38 counts as 1e-38, one above 1e30 as 1e30, a min_p
- * above 1 as 1, a u outside as the nearer end. temperature, top_k, top_p, min_p [rows], or NULL: the number beside it for all
- * rows. A logit of -inf is never drawn. A row that holds a NaN or +inf, or -inf alone, or whose u or
+ * above 1 as 1, a u outside as the nearer end. temperature, top_k (below 0: all), top_p, min_p [rows], or NULL: the number
+ * beside it for all rows. A logit of -inf is never drawn. A row that holds a NaN or +inf, or -inf alone, or whose u or
  * options are NaN, whose temperature is negative or infinite, gets token -1 and logp NaN. */
 int pl_sample_dev(const void* logits, size_t ld, size_t rows, size_t V, uint8_t bf16, const float* u,
                   const float* temperature, double temperature_all, const int32_t* top_k, size_t top_k_all,
@@ -594,11 +594,17 @@ int pl_sample_dev(const void* logits, size_t ld, size_t rows, size_t V, uint8_t 
  * head h / (heads_v / heads_k) of queries and keys. dk up to 128, dv up to 1,024. Strides of tokens and heads are in
  * elements (the last dimension is contiguous); o and gradients are packed. g = -inf (or below -104) forgets the
  * (finite) state: an episode's first token. Keys of length one and beta in (0, 2) keep the rule stable.
+ * All else has to be finite: 64 tokens are worked on at once, and a NaN or an infinity, one that an unstable rule has come to
+ * included, reaches any token of its sequence in its 64 and behind them, whether a token between forgets or not; never
+ * another sequence or a head that does not read it. What a sequence's first token forgets may be anything.
+ * Products carry f32 operands, states among them, as two bf16 parts: f32 results are off by up to 4e-5 of their norm (5e-6 as a
+ * rule), bf16 ones by their own rounding. pl_delta_step_dev computes in f32.
  *
  * Sequences lie one behind the other: sequence s has tokens offsets[s] to offsets[s + 1] - 1 (int32 on the device,
  * not falling; NULL: `sequences` of equal length). Tokens in front of the first and behind the last belong to none: their outputs
  * are zero. state (NULL: zero) and final_state are [sequences][heads_v][dk][dv] f32. Either saved, for the gradient
- * (pl_delta_saved bytes), or ws (pl_delta_ws bytes) is needed, 256-byte aligned. A wait for copies that ran out
+ * (pl_delta_saved bytes: for 64 tokens of a head of 128 x 128 with a key head of its own 163 KB, three times what q, k and v
+ * hold), or ws (pl_delta_ws bytes) is needed, 256-byte aligned. A wait for copies that ran out
  * (pl_device_check) leaves results that are not valid. */
 typedef struct {
   size_t tokens, sequences, heads_k, heads_v, dk, dv;
@@ -610,7 +616,8 @@ size_t pl_delta_saved(const pl_delta_shape* s);
 int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g, const float* beta,
                  const int32_t* offsets, const float* state, void* o, float* final_state, void* saved, size_t saved_bytes,
                  void* ws, size_t ws_bytes, void* stream);
-/* Its gradient, from dout [tokens][heads_v][dv] bf16 (strides in elements) and dfinal (of final_state; NULL: zero): dq, dk,
+/* Its gradient, from what the forward call saved: q, k, v, g and beta are checked as there, but their values are those that
+ * `saved` holds. dout [tokens][heads_v][dv] bf16 (strides in elements) and dfinal (of final_state; NULL: zero): dq, dk,
  * dv bf16, dg, dbeta f32 (zero dg at a token that forgets), dstate (of state; may be NULL). Sums go in a fixed order; what
  * heads of values add to the shared queries and keys is added in their order. */
 int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token, size_t do_head, const float* dfinal,
@@ -618,7 +625,7 @@ int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token
                       const int32_t* offsets, const void* saved, size_t saved_bytes, void* dq, void* dk, void* dv, float* dg,
                       float* dbeta, float* dstate, void* ws, size_t ws_bytes, void* stream);
 /* One token of every row: the rule with tokens = rows, state and state_out [rows][heads_v][dk][dv] (state_out may be
- * state), o [rows][heads_v][dv]. */
+ * state), o [rows][heads_v][dv]. A row that forgets may have any state, NaN too. */
 int pl_delta_step_dev(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g,
                       const float* beta, const float* state, float* state_out, void* o, void* stream);
 

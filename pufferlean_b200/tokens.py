@@ -102,12 +102,13 @@ def vocab_distill_grad(x, w, ids, teacher, bias=None, temperature=1.0, row_scale
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """(token int32, logp f32) [N]: one token per row of logits [N, V] (f32 or bf16, V up to 262,144), drawn with the given
     numbers u [N] f32 in [0, 1), so that a draw can be repeated. The options are numbers, or tensors [N] with one for each
-    row (f32; top_k int32). By falling logit, equal ones by index: the first top_k stay (0: all); of these those before
+    row (f32; top_k int32). As a number a negative top_k or temperature is refused; in a tensor the one means all, the other
+    spoils its row. By falling logit, equal ones by index: the first top_k stay (0: all); of these those before
     which less than top_p of their mass comes; of these those with at least min_p of the largest probability; the first
     always. logp is the token's log-probability among those that stay, at this temperature (what an importance ratio
     divides by). temperature 0 takes the first, one between 0 and 1e-38 counts as 1e-38, one above 1e30 as 1e30, a min_p above 1
-    as 1. A logit of -inf is never drawn; a row with a NaN or +inf, with nothing but -inf, or with an option that is NaN, gets
-    token -1 and logp NaN."""
+    as 1. A logit of -inf is never drawn; a row with a NaN or +inf, with nothing but -inf, with an option that is NaN or
+    with a negative or infinite temperature gets token -1 and logp NaN."""
     return _ext.sample(logits, u, temperature, top_k, top_p, min_p)
 
 
@@ -136,8 +137,14 @@ def delta_rule(q, k, v, g, beta, offsets=None, state=None, scale=None, save=Fals
     q, k [N, Hk, dk], v [N, Hv, dv] bf16 (views of one wider projection will do), g, beta [N, Hv] f32, state and final_state
     [S, Hv, dk, dv] f32; dk up to 128, dv up to 1,024, Hv a multiple of Hk. offsets [S + 1] int32: sequence s has rows
     offsets[s] to offsets[s + 1]; None: as many sequences of one length as `state` has (one without a state). Rows outside all
-    sequences get zeros. g = -inf forgets the state: an episode's first token. With keys of length one and beta below 2 the
-    rule is stable. `saved` (None without save) is what delta_rule_grad takes."""
+    sequences get zeros. g = -inf forgets the (finite) state: an episode's first token. With keys of length one and beta below 2
+    the rule is stable. `saved` (None without save) is what delta_rule_grad takes: for 64 tokens of a head of 128 x 128 with a
+    key head of its own 163 KB, three times what q, k and v hold.
+
+    All inputs but g have to be finite: 64 tokens are worked on at once, so a NaN or an infinity (one that an unstable rule has
+    come to, too) reaches any token of its sequence in its 64 and behind them, past a g of -inf as well; other sequences and
+    heads stay clean, and a sequence's first token with g = -inf forgets any state. f32 results are off by up to 4e-5 of their
+    norm (5e-6 as a rule): products carry f32 operands, states among them, as two bf16 parts."""
     if offsets is not None:
         sequences = offsets.shape[0] - 1
     else:
@@ -149,13 +156,14 @@ def delta_rule(q, k, v, g, beta, offsets=None, state=None, scale=None, save=Fals
 def delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved, scale=None):
     """(dq, dk, dv, dg, dbeta, dstate) of delta_rule from the gradients do [N, Hv, dv] bf16 of o and dstate of the final
     state (None: zero); the last of the results is that of the first state. The other arguments are the forward call's, `saved`
-    what it returned. dq, dk, dv bf16, dg, dbeta, dstate f32."""
+    what it returned, with the values of q, k, v, g and beta that count (changed ones in between change nothing). dq, dk, dv
+    bf16, dg, dbeta, dstate f32."""
     if saved is None:
         raise PufferError("delta_rule_grad: saved is needed (delta_rule with save=True)")
     return _ext.delta_rule_grad(q, k, v, g, beta, offsets, saved[1], do, dstate, _scale(q, scale), saved[0])
 
 
 def delta_rule_step(q, k, v, g, beta, state, scale=None, out=None):
-    """(o, state): delta_rule for one token of every row, state [N, Hv, dk, dv] f32. The new states go into `out`, which may
-    be `state` itself, or a new tensor."""
+    """(o, state): delta_rule for one token of every row, in f32, state [N, Hv, dk, dv]. The new states go into `out`, which may
+    be `state` itself, or a new tensor. A g of -inf forgets any state, one that is not finite too."""
     return _ext.delta_rule_step(q, k, v, g, beta, state, _scale(q, scale), out)

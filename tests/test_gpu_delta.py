@@ -207,6 +207,74 @@ def test_long_sequence_and_offsets():
     assert not o[:n - 100:997].any()
 
 
+@pytest.mark.parametrize("lengths", [[64], [300], [2500], [130, 64, 1, 700]])
+@pytest.mark.parametrize("dk,dv,reset", [(128, 64, 0.0), (64, 72, 0.01), (40, 130, 0.0)])
+def test_both_parts_of_every_operand(lengths, dk, dv, reset):
+    """f32 results by norm. An operand's two bf16 parts are at most 2^-18 of its value off, and so is the product of the second
+    parts, which is left out: 3 * 2^-18 in all for a product of two such operands, of signs that have nothing to do with each
+    other. A result passes through five to twelve products, whose errors add up by squares to sqrt(12) * 3 * 2^-18 at most, and
+    the rule contracts: 4e-5. A second part that is lost is 2^-9, fifty times as much, of its operand."""
+    q, k, v, g, beta, offsets, state, do, dstate = _inputs(lengths, 1, 2, dk, dv, dk + len(lengths), reset=reset)
+    o, final, saved = tokens.delta_rule(q, k, v, g, beta, offsets, state, save=True)
+    grads = tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved)
+    _, rfinal, rgrads, _ = _ref(q, k, v, g, beta, offsets, state, dk ** -0.5, do, dstate)
+    tol = math.sqrt(12) * 3 * 2.0 ** -18
+    floor = 2.0 ** -23 * float((q.double().norm(dim=2) * rgrads[0].norm(dim=2)).norm()
+                               + (k.double().norm(dim=2) * rgrads[1].norm(dim=2)).norm()) * 8
+    _near(final, rfinal, tol, "final")
+    _near(grads[3], rgrads[3], tol, "dg", floor)
+    _near(grads[4], rgrads[4], tol, "dbeta")
+    _near(grads[5], rgrads[5], tol, "dstate")
+
+
+def _same(got, want):
+    return all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (100, 72)])
+def test_what_is_not_finite_stays_where_it_belongs(dk, dv):
+    """A NaN reaches what its sequence has in its chunk and behind it, and nothing else: not the sequences beside it, not the
+    other heads, not rows of no sequence, which are not read either; and a first token that forgets forgets any state."""
+    q, k, v, g, beta, offsets, state, do, dstate = _inputs([100, 150, 70], 2, 4, dk, dv, 17, front=3, behind=9)
+    g[offsets[:-1].long()] = -math.inf
+
+    def both(*a, st=state):
+        q, k, v, g, beta, do = a
+        o, final, saved = tokens.delta_rule(q, k, v, g, beta, offsets, st, save=True)
+        return (o, final) + tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved)
+
+    clean = [t.clone() for t in (q, k, v, g, beta, do)]
+    want = both(*clean)
+    assert _same(both(*clean, st=torch.full_like(state, math.nan)), want)
+    assert _same(both(*clean, st=torch.full_like(state, math.inf)), want)
+    for t in clean:  # rows of no sequence
+        t[:3] = math.nan
+        t[-9:] = -math.inf
+    assert _same(both(*clean), want)
+    for i, t in enumerate(clean):  # the middle sequence, its last chunk; q and k of the second key head, value heads 2 and 3
+        dirty = [x.clone() for x in clean]
+        dirty[i][103 + 140, 1 if i < 2 else 2] = math.nan
+        got = both(*dirty)
+        rows = torch.ones(len(q), dtype=torch.bool, device="cuda")
+        rows[103:253] = False
+        for x, y in zip(got, want):
+            if x.shape[0] == 3:
+                assert torch.equal(x[::2], y[::2]) and torch.equal(x[1, :2], y[1, :2]), i
+            else:
+                heads = 1 if x.shape[1] == 2 else 2
+                assert torch.equal(x[rows], y[rows]) and torch.equal(x[:, :heads], y[:, :heads]), i
+        assert torch.equal(got[0][103:103 + 128], want[0][103:103 + 128]), i  # the chunks before it
+
+
+def test_gradients_take_what_was_saved():
+    q, k, v, g, beta, offsets, state, do, dstate = _inputs([130, 7], 2, 4, 32, 32, 6)
+    _, _, saved = tokens.delta_rule(q, k, v, g, beta, offsets, state, save=True)
+    want = tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved)
+    for t in (q, k, v, g, beta):
+        t.fill_(math.nan)
+    assert _same(tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved), want)
+
+
 def test_optional_gradients():
     q, k, v, g, beta, offsets, state, do, dstate = _inputs([130, 7], 2, 4, 32, 32, 6)
     _, _, saved = tokens.delta_rule(q, k, v, g, beta, offsets, state, save=True)
