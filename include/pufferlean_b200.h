@@ -597,8 +597,8 @@ int pl_sample_dev(const void* logits, size_t ld, size_t rows, size_t V, uint8_t 
  * All else has to be finite: 64 tokens are worked on at once, and a NaN or an infinity, one that an unstable rule has come to
  * included, reaches any token of its sequence in its 64 and behind them, whether a token between forgets or not; never
  * another sequence or a head that does not read it. What a sequence's first token forgets may be anything.
- * Products carry f32 operands, states among them, as two bf16 parts: f32 results are off by up to 4e-5 of their norm (5e-6 as a
- * rule), bf16 ones by their own rounding. pl_delta_step_dev computes in f32.
+ * Products carry f32 operands, states among them, as two bf16 parts: f32 results are 5e-6 of their norm off as a rule, up to 1e-4
+ * where terms cancel, bf16 ones by their own rounding. pl_delta_step_dev computes in f32.
  *
  * Sequences lie one behind the other: sequence s has tokens offsets[s] to offsets[s + 1] - 1 (int32 on the device,
  * not falling; NULL: `sequences` of equal length). Tokens in front of the first and behind the last belong to none: their outputs
