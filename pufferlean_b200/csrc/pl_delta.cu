@@ -141,13 +141,13 @@ __global__ void __launch_bounds__(256) delta_step_kernel(const StepArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------- X and P of all chunks
-// Per slot and value head: X and P, triangular, as two bf16 parts each, and the decays; per slot and key head K and Q in
+// Per slot and value head: X and P, triangular, as three bf16 parts each, and the decays; per slot and key head K and Q in
 // rows as they stand in shared memory, [2][64][dkp + 8], so that the other kernels get them by one bulk copy; per slot its
 // chunk's first token and length (0: none).
 // Measured: 8,192 chunks of a head, dk = 128, in 210 us, where their 730 MB would take 110: a block's dozen steps (search,
 // copies, decays, two products, the inverse in blocks of 16 and 32) wait for one another, four blocks to an SM.
 struct __align__(16) Mats {
-  __nv_bfloat16 x[2][kTri], p[2][kTri];
+  __nv_bfloat16 x[3][kTri], p[3][kTri];
   Decay d;
 };
 
@@ -158,6 +158,8 @@ __device__ __forceinline__ long tile_at(const DeltaArgs& a, long slot, int kh) {
   return (slot * a.hk + kh) * 2 * kC * (DK + 8);
 }
 
+// beta where it divides: not zero. What it adds to X is 1e-12 of what is there.
+__device__ __forceinline__ float beta_of(float b) { return fabsf(b) < 1e-12f ? copysignf(1e-12f, b) : b; }
 constexpr int kPrepThreads = 128;
 template <int DK>
 struct PrepShared {
@@ -284,12 +286,12 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(
         for (int c = 0; c < 2; c++) {
           const float f = j + c <= i ? decay(ci, ei, sh.d, j + c) : 0.f;
           p[c] = j + c <= i ? qk[t][half * 2 + c] * f : 0.f;
-          sh.at[j + c][i] = j + c < i ? kk[t][half * 2 + c] * f * sh.d.beta[j + c] : 0.f;
+          sh.at[j + c][i] = j + c < i ? kk[t][half * 2 + c] * f * beta_of(sh.d.beta[j + c]) : 0.f;
         }
-        uint32_t hi, lo;
-        split2(p[0], p[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(out.p[0] + tri_at(i, j)) = hi;
-        *reinterpret_cast<uint32_t*>(out.p[1] + tri_at(i, j)) = lo;
+        Parts<3> s;
+        split<3>(p[0], p[1], s, 0);
+#pragma unroll
+        for (int c = 0; c < 3; c++) *reinterpret_cast<uint32_t*>(out.p[c] + tri_at(i, j)) = s.p[c][0];
       }
     }
     __syncthreads();
@@ -362,24 +364,30 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(
     for (int i = tid; i < kTri / 2; i += kPrepThreads) {  // pair i of the ten blocks, in the order of rows and columns
       const int b = i >> 7, r = b < 1 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, c = b - r * (r + 1) / 2;
       const int y = r * 16 + (i >> 3 & 15), x = c * 16 + (i & 7) * 2;
-      uint32_t hi, lo;
-      split2(sh.x[y][x], sh.x[y][x + 1], hi, lo);
-      *reinterpret_cast<uint32_t*>(out.x[0] + tri_at(y, x)) = hi;
-      *reinterpret_cast<uint32_t*>(out.x[1] + tri_at(y, x)) = lo;
+      Parts<3> s;
+      split<3>(sh.x[y][x], sh.x[y][x + 1], s, 0);
+#pragma unroll
+      for (int e = 0; e < 3; e++) *reinterpret_cast<uint32_t*>(out.x[e] + tri_at(y, x)) = s.p[e][0];
     }
   }
   if (tid == 0) tc::bulk_wait<0>();
 }
 
 // ---------------------------------------------------------------------------------------------- the chain forward
-// What a chain leaves for the gradient, per slot, value head and 64 columns of v, as two bf16 parts one behind the other, in
-// rows as they stand in shared memory (one bulk copy): a state, transposed, [2][64][dkp + 8], and rows, transposed,
+// What a chain leaves for the products of the last kernel, per slot, value head and 64 columns of v, as two bf16 parts one behind
+// the other, in rows as they stand in shared memory (one bulk copy): a state, transposed, [2][64][dkp + 8], and rows, transposed,
 // [2][64][72], 64 tokens in each.
 __device__ __forceinline__ long state_at(const DeltaArgs& a, long slot, int h, int slice) {
   return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * 64 * (a.dkp + 8);
 }
 __device__ __forceinline__ long rows_at(const DeltaArgs& a, long slot, int h, int slice) {
   return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * kC * kLd;
+}
+
+// What the forward chain leaves for the sums of the chain back, f32: 64 columns of v of 64 tokens as a warp's lanes hold them, four
+// warps, 16 columns each, one behind the other.
+__device__ __forceinline__ uint4* lanes_at(const DeltaArgs& a, void* base, long slot, int h, int slice, int warp) {
+  return (uint4*)base + (((slot * a.hv + h) * (a.dvp / 64) + slice) * 4 + warp) * (8 * 32);
 }
 
 struct ScanArgs {
@@ -389,7 +397,8 @@ struct ScanArgs {
   const float* state;  // [seqs][hv][dk][dv], or NULL: zero
   __nv_bfloat16* o;    // [n][hv][dv]
   float* final_state;
-  __nv_bfloat16 *kept, *y;  // for the gradient: S and Y of every slot; or NULL
+  __nv_bfloat16* kept;  // for the gradient: S of every slot; or NULL
+  float *y, *out;       // and Y and the f32 outputs
 };
 // A chunk's inputs, loaded while the chunk before it is worked on; x: 64 columns of v (forward), of dO (back).
 template <int DK>
@@ -403,7 +412,7 @@ constexpr int kAll = 15, kMovers = 14;  // barriers of all threads, of the four 
 template <int DK>
 struct ScanShared {
   ChainIn<DK> in[2];
-  uint4 s[4][DK / 8 * 32];  // a warp's state, in two parts
+  uint4 s[4][DK / 8 * 32];  // a warp's state, as its lanes hold it
   uint4 y[4][8 * 32];       // its Y
   uint64_t full[2];         // the inputs have come
 };
@@ -458,14 +467,26 @@ __device__ __forceinline__ void parts_out(const float (&s)[NT][4], __nv_bfloat16
       *reinterpret_cast<uint32_t*>(at + second) = lo;
     }
 }
-// The same from parts that have been made: `half` of DK / 16 fragments of a first operand.
-__device__ __forceinline__ void part_out(const uint32_t (&r)[4], __nv_bfloat16* dst, int row, int k) {
+// A warp's state [16 of dv][DK] as its lanes hold it, as two parts into [2][64][DK + 8] from `dst` (its first row) on.
+template <int DK>
+__device__ __forceinline__ void state_parts(const uint4* s, __nv_bfloat16* dst) {
   const int lane = threadIdx.x & 31;
-  __nv_bfloat16* at = dst + (lane >> 2) * row + k * 16 + (lane & 3) * 2;
-  *reinterpret_cast<uint32_t*>(at) = r[0];
-  *reinterpret_cast<uint32_t*>(at + 8 * row) = r[1];
-  *reinterpret_cast<uint32_t*>(at + 8) = r[2];
-  *reinterpret_cast<uint32_t*>(at + 8 * row + 8) = r[3];
+  constexpr int LD = DK + 8;
+#pragma unroll
+  for (int k = 0; k < DK / 16; k++) {
+    float s0[4], s1[4];
+    take(s, 2 * k, s0);
+    take(s, 2 * k + 1, s1);
+    const Parts<2> x = parts_of<2>(s0, s1);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      __nv_bfloat16* at = dst + i * 64 * LD + (lane >> 2) * LD + k * 16 + (lane & 3) * 2;
+      *reinterpret_cast<uint32_t*>(at) = x.p[i][0];
+      *reinterpret_cast<uint32_t*>(at + 8 * LD) = x.p[i][1];
+      *reinterpret_cast<uint32_t*>(at + 8) = x.p[i][2];
+      *reinterpret_cast<uint32_t*>(at + 8 * LD + 8) = x.p[i][3];
+    }
+  }
 }
 // 64 rows of 16 values that this warp put at `tile`, to rows of `stride` in memory, `cols` of them.
 __device__ __forceinline__ void rows_out(const __nv_bfloat16* tile, __nv_bfloat16* dst, long stride, int len, int cols,
@@ -494,13 +515,13 @@ __device__ __forceinline__ uint32_t across_at(const __nv_bfloat16* tile, int n) 
 // A chunk takes 3.9 us, 6,600 clocks. Its products are 316 and 188 of 16 x 8 x 16 for each scheduler, 8 clocks each: 4,032.
 // (All in one warp it took 5.5 us; with R, Y, U and the state's parts in shared memory, shared by 16 warps in four steps with
 // barriers, 5.6.) 4 x 8,192 tokens of 16 heads of 128 x 128: 500 us, 128 of 148 SMs with a chain of 128 chunks each.
-template <int DK>
+template <int DK, bool SAVE>
 __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const ScanArgs p) {
   grid_wait();
   grid_next();
   extern __shared__ __align__(16) unsigned char mem[];
   ScanShared<DK>& sh = *reinterpret_cast<ScanShared<DK>*>(mem);
-  constexpr int LD = DK + 8, NK = DK / 8;
+  constexpr int LD = DK + 8, NK = DK / 8, P = SAVE ? 3 : 2;  // parts of the outputs' operands
   const DeltaArgs& a = p.d;
   const int slice = blockIdx.x, c0 = slice * 64, h = blockIdx.y, seq = blockIdx.z, kh = h / (a.hv / a.hk);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5 & 3;
@@ -509,7 +530,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
   long from, to;
   seq_bounds(a, seq, from, to);
   const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
-  const int s_ready = 1 + warp, y_ready = 5 + warp;
+  const int s_read = 1 + warp, y_ready = 5 + warp;
   if (threadIdx.x == 0) {
     tc::mbar_init(&sh.full[0], 1);
     tc::mbar_init(&sh.full[1], 1);
@@ -520,21 +541,24 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     float s[NK][4];
     const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
     state_in(s, p.state ? p.state + sbase : nullptr, a.dk, a.dv, mine);
+#pragma unroll
+    for (int t = 0; t < NK; t++) give(sh.s[warp], t, s[t]);
     for (long c = 0; c < chunks; c++) {
       ChainIn<DK>& in = sh.in[c & 1];
       meet<kChainThreads>(kAll);
       tc::mbar_wait(&sh.full[c & 1], c >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
-      float r[8][4];  // (K S)^T: [16 of dv][64 tokens]
+      float r[8][4], low[8][4];  // (K S)^T: [16 of dv][64 tokens]
       zero(r);
+      zero(low);
       const uint32_t pk = smem_u32(in.k + lane_b<false, LD>());
 #pragma unroll
       for (int k = 0; k < DK / 16; k++) {
-        const Parts x = parts_of(s[2 * k], s[2 * k + 1]);
-        give(sh.s[warp], 2 * k, x.hi);
-        give(sh.s[warp], 2 * k + 1, x.lo);
-        step<false, 4>(r, x, pk + k * 32, 32 * LD);
+        float s0[4], s1[4];
+        take(sh.s[warp], 2 * k, s0);
+        take(sh.s[warp], 2 * k + 1, s1);
+        step<false, 4>(r, low, parts_of<3>(s0, s1), pk + k * 32, 32 * LD);
       }
-      meet_arrive<96>(s_ready);
+      join(r, low);
       const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>());
 #pragma unroll
       for (int n = 0; n < 4; n++) {  // R = V - E K S
@@ -554,18 +578,14 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
       }
       float y[8][4];  // Y^T = R^T X^T
       zero(y);
-      const uint32_t tx = tri_lane<false>(in.m.x[0]);
+      Parts<3> z[4];
 #pragma unroll
-      for (int k = 0; k < 4; k++) tri_step<false>(y, parts_of(r[2 * k], r[2 * k + 1]), tx, k);
+      for (int k = 0; k < 4; k++) z[k] = parts_of<3>(r[2 * k], r[2 * k + 1]);
+      tri_product<false, 3, 3>(y, z, tri_lane<false>(in.m.x[0]));
 #pragma unroll
       for (int t = 0; t < 8; t++) give(sh.y[warp], t, y[t]);
       meet_arrive<96>(y_ready);
       const float keep = in.m.d.since[kC - 1];
-#pragma unroll
-      for (int t = 0; t < NK; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-      const uint32_t pt = smem_u32(in.k + lane_b<true, LD>());
 #pragma unroll
       for (int k = 0; k < 4; k++) {  // S^T += (F U)^T K
 #pragma unroll
@@ -576,10 +596,20 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
           u[0] *= f.x * b.x, u[2] *= f.x * b.x;
           u[1] *= f.y * b.y, u[3] *= f.y * b.y;
         }
-        step<true, DK / 16>(s, parts_of(y[2 * k], y[2 * k + 1]), pt + k * 32 * LD, 32);
+        z[k] = parts_of<3>(y[2 * k], y[2 * k + 1]);
       }
+      meet<96>(s_read);
+      token_steps<LD, NK>(z, smem_u32(in.k + lane_b<true, LD>()), [&](int t, const float(&add)[4]) {
+        float v[4];
+        take(sh.s[warp], t, v);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = __fmaf_rn(keep, keep == 0.f ? 0.f : v[e], add[e]);
+        give(sh.s[warp], t, v);
+      });
     }
     if (chunks) meet<kChainThreads>(kAll);
+#pragma unroll
+    for (int t = 0; t < NK; t++) take(sh.s[warp], t, s[t]);
     state_out(s, p.final_state + sbase, a.dk, a.dv, mine);
     return;
   }
@@ -588,17 +618,19 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
       ChainIn<DK>& in = sh.in[c & 1];
       meet<kChainThreads>(kAll);
       tc::mbar_wait(&sh.full[c & 1], c >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
-      float o[8][4];  // (Q S)^T
+      float o[8][4], low[8][4];  // (Q S)^T
       zero(o);
+      zero(low);
       const uint32_t pq = smem_u32(in.q + lane_b<false, LD>());
-      meet<96>(s_ready);
 #pragma unroll
       for (int k = 0; k < DK / 16; k++) {
-        Parts x;
-        take(sh.s[warp], 2 * k, x.hi);
-        take(sh.s[warp], 2 * k + 1, x.lo);
-        step<false, 4>(o, x, pq + k * 32, 32 * LD);
+        float s0[4], s1[4];
+        take(sh.s[warp], 2 * k, s0);
+        take(sh.s[warp], 2 * k + 1, s1);
+        step<false, 4>(o, low, parts_of<P>(s0, s1), pq + k * 32, 32 * LD);
       }
+      meet_arrive<96>(s_read);
+      join(o, low);
 #pragma unroll
       for (int t = 0; t < 8; t++) {
         const float2 f = *reinterpret_cast<const float2*>(in.m.d.since + t * 8 + (lane & 3) * 2);
@@ -608,8 +640,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
           o[t][e] = fe == 0.f ? 0.f : fe * o[t][e];
         }
       }
-      const uint32_t tp = tri_lane<false>(in.m.p[0]);
+      zero(low);
       meet<96>(y_ready);
+      Parts<P> z[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         float u[2][4];
@@ -620,14 +653,21 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
           u[t][0] *= b.x, u[t][2] *= b.x;
           u[t][1] *= b.y, u[t][3] *= b.y;
         }
-        tri_step<false>(o, parts_of(u[0], u[1]), tp, k);
+        z[k] = parts_of<P>(u[0], u[1]);
       }
+      tri_product<false, P, P>(low, z, tri_lane<false>(in.m.p[0]));
+      join(o, low);
       // the chain has read these columns of v before it gave Y: o takes their place on its way out
 #pragma unroll
       for (int n = 0; n < 4; n++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) o[2 * n][e] *= a.scale, o[2 * n + 1][e] *= a.scale;
         store_across(across_at(in.x + warp * 16, n), o[2 * n], o[2 * n + 1]);
+      }
+      if constexpr (SAVE) {
+        uint4* to = lanes_at(a, p.out, slot0 + c, h, slice, warp);
+#pragma unroll
+        for (int t = 0; t < 8; t++) give(to, t, o[t]);
       }
     }
     if (chunks) meet<kChainThreads>(kAll);
@@ -663,22 +703,17 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     if (c > 0) write_o(c - 1);
     meet<128>(kMovers);  // the place of chunk c - 1's inputs, and of its o, is free
     if (c + 1 < chunks) load(c + 1);
-    meet<96>(s_ready);
-    if (p.kept) {
-      __nv_bfloat16* to_s = p.kept + state_at(a, slot0 + c, h, slice) + warp * 16 * LD;
-#pragma unroll
-      for (int k = 0; k < DK / 8; k++) {
-        uint32_t x[4];
-        take(sh.s[warp], k, x);
-        part_out(x, to_s + (k & 1) * 64 * LD, LD, k / 2);
-      }
-    }
+    if constexpr (SAVE) state_parts<DK>(sh.s[warp], p.kept + state_at(a, slot0 + c, h, slice) + warp * 16 * LD);
+    meet_arrive<96>(s_read);
     meet<96>(y_ready);
-    if (p.y) {
-      float y[8][4];
+    if constexpr (SAVE) {
+      uint4* to = lanes_at(a, p.y, slot0 + c, h, slice, warp);
 #pragma unroll
-      for (int t = 0; t < 8; t++) take(sh.y[warp], t, y[t]);
-      parts_out(y, p.y + rows_at(a, slot0 + c, h, slice) + warp * 16 * kLd, kLd, (long)kC * kLd);
+      for (int t = 0; t < 8; t++) {
+        uint32_t y[4];
+        take(sh.y[warp], t, y);
+        give(to, t, y);
+      }
     }
   }
   if (chunks) {
@@ -695,21 +730,46 @@ struct BackArgs {
   const __nv_bfloat16* dout;  // [n][hv][dv], strides below
   long ldo, hso;
   int align_o;
-  const float* dfinal;        // [seqs][hv][dk][dv], or NULL: zero
-  __nv_bfloat16* dv;          // [n][hv][dv]
-  float* dstate;              // or NULL
-  __nv_bfloat16 *ds, *dr;     // dS' and dR of every slot
+  const float* dfinal;         // [seqs][hv][dk][dv], or NULL: zero
+  float *yf, *out;             // of the forward pass: Y and the f32 outputs
+  __nv_bfloat16* dv;           // [n][hv][dv]
+  float* dstate;               // or NULL
+  __nv_bfloat16 *ds, *dr, *y;  // dS', dR and Y of every slot
+  float* sums;                 // sums_at
 };
+// Per slot, value head and 16 columns of v, sums over them: of every token Y . Z beta' and o . dO - v . dR, of the chunk F K dS' . U.
+constexpr int kSums = 2 * kC + 2;
+__device__ __forceinline__ long sums_at(const DeltaArgs& a, long slot, int h, int group) {
+  return ((slot * a.hv + h) * (a.dvp / 16) + group) * kSums;
+}
+// A warp's sums over the 16 rows of an accumulator [16][64]; lane l gets those of columns 2 l and 2 l + 1.
+__device__ __forceinline__ float2 column_sums(const float (&v)[8][2]) {
+  const int lane = threadIdx.x & 31;
+  float a[4][2], b[2][2], c[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+      a[t][e] = (lane & 16 ? v[t + 4][e] : v[t][e]) + __shfl_xor_sync(0xffffffffu, lane & 16 ? v[t][e] : v[t + 4][e], 16);
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+      b[t][e] = (lane & 8 ? a[t + 2][e] : a[t][e]) + __shfl_xor_sync(0xffffffffu, lane & 8 ? a[t][e] : a[t + 2][e], 8);
+    c[e] = (lane & 4 ? b[1][e] : b[0][e]) + __shfl_xor_sync(0xffffffffu, lane & 4 ? b[0][e] : b[1][e], 4);
+  }
+  return make_float2(c[0], c[1]);
+}
 template <int DK>
 struct BackShared {
   ChainIn<DK> in[2];
-  uint4 s[4][DK / 8 * 32];  // a warp's dS', in two parts
-  uint4 x[4][8 * 32];       // scale P^T dO from the helper, then dR to it
-  uint4 q[4][DK / 8 * 32];  // scale (E dO)^T Q from the helper
+  __nv_bfloat16 v[kC * kLd];
+  uint4 s[4][DK / 8 * 32];  // a warp's dS', as its lanes hold it
+  uint4 x[4][8 * 32];       // scale P^T dO from the helper, then beta' Z to memory
+  uint4 f[4][8 * 32];       // F K dS'
   uint64_t full[2];
 };
 // As the chain forward, from the last chunk to the first. The helpers' products, of dO with P and Q, need nothing of the chain.
-// 64 x 512 tokens of 8 heads of 128 x 128: 339 us (forward, with what the gradient needs written out: 328).
+// Memory's warps also make the gates' gradients of what passes through them, in f32: dbeta is Z . Y, token by token (X^T beta dU is
+// beta Z; where beta is zero, a tiny one stands in), and dg is sums of o . dO - v . dR.
 template <int DK>
 __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const BackArgs p) {
   grid_wait();
@@ -725,7 +785,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
   long from, to;
   seq_bounds(a, seq, from, to);
   const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
+  constexpr int EP = 3;  // parts of E dR
   const int u_ready = 1 + warp, q_ready = 5 + warp, r_ready = 9 + warp;
+  constexpr int kRead = 13;  // the chain and memory have read dS'
   if (threadIdx.x == 0) {
     tc::mbar_init(&sh.full[0], 1);
     tc::mbar_init(&sh.full[1], 1);
@@ -736,47 +798,53 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     float s[NK][4];  // dS'^T
     const long sbase = ((long)seq * a.hv + h) * a.dk * a.dv + w0;
     state_in(s, p.dfinal ? p.dfinal + sbase : nullptr, a.dk, a.dv, mine);
+#pragma unroll
+    for (int t = 0; t < NK; t++) give(sh.s[warp], t, s[t]);
     for (long c = chunks - 1, it = 0; c >= 0; c--, it++) {
       ChainIn<DK>& in = sh.in[it & 1];
       meet<kChainThreads>(kAll);
       tc::mbar_wait(&sh.full[it & 1], it >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
-      float x[8][4];  // (K dS')^T: [16 of dv][64 tokens]
+      float x[8][4], low[8][4];  // (K dS')^T: [16 of dv][64 tokens]
       zero(x);
+      zero(low);
       const uint32_t pk = smem_u32(in.k + lane_b<false, LD>());
 #pragma unroll
       for (int k = 0; k < DK / 16; k++) {
-        const Parts z = parts_of(s[2 * k], s[2 * k + 1]);
-        give(sh.s[warp], 2 * k, z.hi);
-        give(sh.s[warp], 2 * k + 1, z.lo);
-        step<false, 4>(x, z, pk + k * 32, 32 * LD);
+        float s0[4], s1[4];
+        take(sh.s[warp], 2 * k, s0);
+        take(sh.s[warp], 2 * k + 1, s1);
+        step<false, 4>(x, low, parts_of<3>(s0, s1), pk + k * 32, 32 * LD);
       }
+      meet_arrive<kChainThreads>(kRead);
+      join(x, low);
       meet<64>(u_ready);
 #pragma unroll
-      for (int t = 0; t < 8; t++) {  // beta dU = beta (F K dS' + scale P^T dO)
+      for (int t = 0; t < 8; t++) {  // beta' dU = beta' (F K dS' + scale P^T dO)
         const float2 b = *reinterpret_cast<const float2*>(in.m.d.beta + t * 8 + (lane & 3) * 2);
         const float2 f = *reinterpret_cast<const float2*>(in.m.d.until + t * 8 + (lane & 3) * 2);
         float u[4];
         take(sh.x[warp], t, u);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float fe = e & 1 ? f.y : f.x, be = e & 1 ? b.y : b.x;
-          x[t][e] = be * ((fe == 0.f ? 0.f : fe * x[t][e]) + u[e]);
+          const float fe = e & 1 ? f.y : f.x;
+          x[t][e] = fe == 0.f ? 0.f : fe * x[t][e];
         }
-      }
-      float r[8][4];  // dR^T = (beta dU)^T X
-      zero(r);
-      const uint32_t tx = tri_lane<true>(in.m.x[0]);
+        give(sh.f[warp], t, x[t]);
 #pragma unroll
-      for (int k = 0; k < 4; k++) tri_step<true>(r, parts_of(x[2 * k], x[2 * k + 1]), tx, k);
+        for (int e = 0; e < 4; e++) x[t][e] = beta_of(e & 1 ? b.y : b.x) * (x[t][e] + u[e]);
+      }
+      float r[8][4];  // (beta' Z)^T = (beta' dU)^T X
+      zero(r);
+      {
+        Parts<3> z[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) z[k] = parts_of<3>(x[2 * k], x[2 * k + 1]);
+        tri_product<true, 3, 3>(r, z, tri_lane<true>(in.m.x[0]));
+      }
 #pragma unroll
       for (int t = 0; t < 8; t++) give(sh.x[warp], t, r[t]);
       meet_arrive<64>(r_ready);
-      const float keep = in.m.d.since[kC - 1];
-#pragma unroll
-      for (int t = 0; t < NK; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[t][e] = keep == 0.f ? 0.f : keep * s[t][e];
-      const uint32_t pt = smem_u32(in.k + lane_b<true, LD>());
+      Parts<EP> z[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {  // dS^T -= (E dR)^T K
 #pragma unroll
@@ -788,17 +856,19 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
             r[2 * k + t][e] = fe == 0.f ? 0.f : -fe * r[2 * k + t][e];
           }
         }
-        step<true, DK / 16>(s, parts_of(r[2 * k], r[2 * k + 1]), pt + k * 32 * LD, 32);
+        z[k] = parts_of<EP>(r[2 * k], r[2 * k + 1]);
       }
       meet<64>(q_ready);
+      token_steps<LD, NK>(z, smem_u32(in.k + lane_b<true, LD>()), [&](int t, const float(&add)[4]) {
+        float v[4];
+        take(sh.s[warp], t, v);
 #pragma unroll
-      for (int t = 0; t < NK; t++) {
-        float q[4];
-        take(sh.q[warp], t, q);
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[t][e] += q[e];
-      }
+        for (int e = 0; e < 4; e++) v[e] += add[e];
+        give(sh.s[warp], t, v);
+      });
     }
+#pragma unroll
+    for (int t = 0; t < NK; t++) take(sh.s[warp], t, s[t]);
     if (p.dstate) state_out(s, p.dstate + sbase, a.dk, a.dv, mine);
     return;
   }
@@ -814,14 +884,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
       {
         float u[8][4];
         zero(u);
-        const uint32_t tp = tri_lane<true>(in.m.p[0]);
+        Parts<1> x[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          Parts x;
+        for (int k = 0; k < 4; k++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) x.hi[e] = x.lo[e] = o[k][e];
-          tri_step<true, false>(u, x, tp, k);
-        }
+          for (int e = 0; e < 4; e++) x[k].p[0][e] = o[k][e];
+        tri_product<true, 1, 3>(u, x, tri_lane<true>(in.m.p[0]));
 #pragma unroll
         for (int t = 0; t < 8; t++) {
 #pragma unroll
@@ -830,9 +898,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
         }
       }
       meet_arrive<64>(u_ready);
-      float q[NK][4];
-      zero(q);
-      const uint32_t pq = smem_u32(in.q + lane_b<true, LD>());
+      Parts<3> z[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         float eo[2][4];
@@ -846,10 +912,17 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
             eo[t][e] = fe == 0.f ? 0.f : a.scale * fe * __uint_as_float(e & 1 ? oo & 0xffff0000u : oo << 16);
           }
         }
-        step<true, DK / 16>(q, parts_of(eo[0], eo[1]), pq + k * 32 * LD, 32);
+        z[k] = parts_of<3>(eo[0], eo[1]);
       }
+      const float keep = in.m.d.since[kC - 1];
+      meet<kChainThreads>(kRead);
+      token_steps<LD, NK>(z, smem_u32(in.q + lane_b<true, LD>()), [&](int t, const float(&add)[4]) {
+        float v[4];
+        take(sh.s[warp], t, v);
 #pragma unroll
-      for (int t = 0; t < NK; t++) give(sh.q[warp], t, q[t]);
+        for (int e = 0; e < 4; e++) v[e] = __fmaf_rn(keep, keep == 0.f ? 0.f : v[e], add[e]);
+        give(sh.s[warp], t, v);
+      });
       meet_arrive<64>(q_ready);
     }
     return;
@@ -868,9 +941,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
       bulk_in(&in.m, p.mats + (slot0 + c) * a.hv + h, sizeof(Mats), bar);
     }
     copy_tile<64, kLd, 128>(in.x, p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.align_o, tid);
-    cp_commit();
   };
   if (chunks) load(chunks - 1);
+  cp_commit();
   zero_rows<128>(a, seq, p.dv + (long)h * a.dv + c0, (long)a.hv * a.dv, cols, tid);
   const bool vec_dv = a.dv % 8 == 0 && (uintptr_t)p.dv % 16 == 0;
   for (long c = chunks - 1; c >= 0; c--) {
@@ -879,22 +952,63 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     ChainIn<DK>& in = sh.in[(chunks - 1 - c) & 1];
     cp_wait<0>();
     meet<kChainThreads>(kAll);
+    copy_tile<64, kLd, 128>(sh.v, a.v + start * a.ldv + h * a.hsv + c0, a.ldv, len, cols, a.vv, tid);
+    cp_commit();
     if (c > 0) load(c - 1);
-    float r[8][4];
-    meet<64>(r_ready);
-    __nv_bfloat16* to_s = p.ds + state_at(a, slot, h, slice) + warp * 16 * LD;
+    cp_commit();
+    const uint4 *yf = lanes_at(a, p.yf, slot, h, slice, warp), *of = lanes_at(a, p.out, slot, h, slice, warp);
+    float y[8][4], o[8][4];
 #pragma unroll
-    for (int k = 0; k < DK / 8; k++) {
-      uint32_t x[4];
-      take(sh.s[warp], k, x);
-      part_out(x, to_s + (k & 1) * 64 * LD, LD, k / 2);
+    for (int t = 0; t < 8; t++) {
+      take(yf, t, y[t]);
+      take(of, t, o[t]);
     }
+    state_parts<DK>(sh.s[warp], p.ds + state_at(a, slot, h, slice) + warp * 16 * LD);
+    meet_arrive<kChainThreads>(kRead);
+    parts_out(y, p.y + rows_at(a, slot, h, slice) + warp * 16 * kLd, kLd, (long)kC * kLd);
+    cp_wait<1>();
+    meet<128>(kMovers);  // v is there
+    tc::mbar_wait(&sh.full[(chunks - 1 - c) & 1], (chunks - 1 - c) >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
+    meet<64>(r_ready);
+    const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>()), pv = smem_u32(sh.v + warp * 16 + lane_a<true, kLd>());
+    float zy[8][2], ov[8][2], fu = 0.f;
 #pragma unroll
-    for (int t = 0; t < 8; t++) take(sh.x[warp], t, r[t]);
-    parts_out(r, p.dr + rows_at(a, slot, h, slice) + warp * 16 * kLd, kLd, (long)kC * kLd);
-    // the helper has read these columns of dO before the chain could give dR: dv takes their place on its way out
+    for (int n = 0; n < 4; n++) {
+      uint32_t d4[4], v4[4];
+      ldsm<true>(d4, px + n * 32 * kLd);
+      ldsm<true>(v4, pv + n * 32 * kLd);
+      float r[2][4];
 #pragma unroll
-    for (int n = 0; n < 4; n++) store_across(across_at(in.x + warp * 16, n), r[2 * n], r[2 * n + 1]);
+      for (int t = 0; t < 2; t++) {
+        const int tt = 2 * n + t;
+        const float2 b = *reinterpret_cast<const float2*>(in.m.d.beta + tt * 8 + (lane & 3) * 2);
+        float f[4];
+        take(sh.x[warp], tt, r[t]);
+        take(sh.f[warp], tt, f);
+#pragma unroll
+        for (int e = 0; e < 2; e++) zy[tt][e] = ov[tt][e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t dd = d4[t * 2 + (e >> 1)], vv = v4[t * 2 + (e >> 1)];
+          const float be = e & 1 ? b.y : b.x;
+          zy[tt][e & 1] = __fmaf_rn(r[t][e], y[tt][e], zy[tt][e & 1]);
+          if (be == 0.f) r[t][e] = 0.f;
+          ov[tt][e & 1] = __fmaf_rn(o[tt][e], __uint_as_float(e & 1 ? dd & 0xffff0000u : dd << 16), ov[tt][e & 1]);
+          ov[tt][e & 1] = __fmaf_rn(-r[t][e], __uint_as_float(e & 1 ? vv & 0xffff0000u : vv << 16), ov[tt][e & 1]);
+          fu = __fmaf_rn(be * y[tt][e], f[e], fu);
+        }
+      }
+      // this warp and the helper have read these columns of dO: dv takes their place on its way out
+      store_across(across_at(in.x + warp * 16, n), r[0], r[1]);
+      const float rr[2][4] = {{r[0][0], r[0][1], r[0][2], r[0][3]}, {r[1][0], r[1][1], r[1][2], r[1][3]}};
+      parts_out(rr, p.dr + rows_at(a, slot, h, slice) + warp * 16 * kLd + n * 16, kLd, (long)kC * kLd);
+    }
+    float* sums = p.sums + sums_at(a, slot, h, slice * 4 + warp);
+    reinterpret_cast<float2*>(sums)[lane] = column_sums(zy);
+    reinterpret_cast<float2*>(sums + kC)[lane] = column_sums(ov);
+#pragma unroll
+    for (int w = 16; w; w >>= 1) fu += __shfl_xor_sync(0xffffffffu, fu, w);
+    if (lane == 0) sums[2 * kC] = fu;
     __syncwarp();
     rows_out(in.x + warp * 16, p.dv + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_dv);
   }
@@ -909,6 +1023,7 @@ struct GradArgs {
   long ldo, hso;
   int align_o;
   const __nv_bfloat16 *kept, *y, *ds, *dr;
+  const float* sums;
   const Mats* mats;
   const __nv_bfloat16* tiles;
   const int2* table;
@@ -921,7 +1036,7 @@ struct GradShared {
   __nv_bfloat16 o[2][kC * kLd], r[2][2][kC * kLd];  // by turns: the next step's are on their way
   __nv_bfloat16 s[2][kC * (DK + 8)], ds[2][kC * (DK + 8)], y[2][kC * kLd];  // transposed, as r
   __nv_bfloat16 p[2][kC * kLd], m[2][kC * kLd];     // scale dO U^T * D, -M
-  float row[4][kC], col[4][kC], krow[4][kC], sum[16];
+  float sum[16], gate[2 * kC + 1];
   Decay decay[2];  // by turns, a head's
   uint64_t full[2];  // S, dO, dR (and K, Q, the decays); dS', Y
 };
@@ -979,7 +1094,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
   load_b(0);
   const int wr = warp & 3, wc = warp >> 2, m0 = wr * 16, i0 = m0 + (lane >> 2);
   const int n0 = wc * 16, d0 = wc * (DK / 4);  // this warp's columns of a 64 x 64 tile, of a 64 x dk tile
-  float dq[NK][4], dk[NK][4], oy[2][4], ry[2][4], qrow[2], krow[2], inner = 0.f;
+  float dq[NK][4], dk[NK][4], oy[2][4], ry[2][4], inner = 0.f;
   zero(dq);
   zero(dk);
   for (int t = 0; t < steps; t++) {
@@ -990,7 +1105,20 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     if (t % slices == 0) {
       zero(oy);
       zero(ry);
-      inner = qrow[0] = qrow[1] = krow[0] = krow[1] = 0.f;
+      inner = 0.f;
+      // the chain's sums of this head, by token; warp 4: of the chunk
+      const float* sums = p.sums + sums_at(a, slot, h, 0);
+      float v = 0.f;
+      if (tid < 2 * kC) {
+#pragma unroll 8
+        for (int g = 0; g < a.dvp / 16; g++) v += sums[g * kSums + tid];
+        sh.gate[tid] = v;
+      } else if (warp == 4) {
+        for (int g = lane; g < a.dvp / 16; g += 32) v += sums[g * kSums + 2 * kC];
+#pragma unroll
+        for (int w = 16; w; w >>= 1) v += __shfl_xor_sync(0xffffffffu, v, w);
+        if (lane == 0) sh.gate[2 * kC] = v;
+      }
     }
     cp_wait<0>();
     tc::mbar_wait(&sh.full[0], t & 1, a.err, PL_ERR_MBAR_TIMEOUT);
@@ -999,31 +1127,23 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     zero(x);
     product<false, kLd, 0, true, LD, kState, 4>(x, o, sh.s[0], m0, d0);
 #pragma unroll
-    for (int half = 0; half < 2; half++) {  // scale E dO S^T, and what it adds to e_i
-      const int i = i0 + half * 8;
-      const float f = d.since[i] * a.scale;
+    for (int half = 0; half < 2; half++) {  // scale E dO S^T
+      const float f = d.since[i0 + half * 8] * a.scale;
 #pragma unroll
       for (int n = 0; n < NK; n++) {
-        const __nv_bfloat162 q = *reinterpret_cast<const __nv_bfloat162*>(sh.q + i * LD + d0 + n * 8 + (lane & 3) * 2);
-        const float v0 = f == 0.f ? 0.f : f * x[n][half * 2], v1 = f == 0.f ? 0.f : f * x[n][half * 2 + 1];
-        qrow[half] = __fmaf_rn(__low2float(q), v0, __fmaf_rn(__high2float(q), v1, qrow[half]));
-        dq[n][half * 2] += v0;
-        dq[n][half * 2 + 1] += v1;
+        dq[n][half * 2] += f == 0.f ? 0.f : f * x[n][half * 2];
+        dq[n][half * 2 + 1] += f == 0.f ? 0.f : f * x[n][half * 2 + 1];
       }
     }
     zero(x);
     product<true, kLd, kRows, true, LD, kState, 4>(x, r, sh.s[0], m0, d0);
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // -E dR S^T
-      const int i = i0 + half * 8;
-      const float f = -d.since[i];
+      const float f = -d.since[i0 + half * 8];
 #pragma unroll
       for (int n = 0; n < NK; n++) {
-        const __nv_bfloat162 k = *reinterpret_cast<const __nv_bfloat162*>(sh.k + i * LD + d0 + n * 8 + (lane & 3) * 2);
-        const float v0 = f == 0.f ? 0.f : f * x[n][half * 2], v1 = f == 0.f ? 0.f : f * x[n][half * 2 + 1];
-        qrow[half] = __fmaf_rn(__low2float(k), v0, __fmaf_rn(__high2float(k), v1, qrow[half]));
-        dk[n][half * 2] += v0;
-        dk[n][half * 2 + 1] += v1;
+        dk[n][half * 2] += f == 0.f ? 0.f : f * x[n][half * 2];
+        dk[n][half * 2 + 1] += f == 0.f ? 0.f : f * x[n][half * 2 + 1];
       }
     }
     tc::mbar_wait(&sh.full[1], t & 1, a.err, PL_ERR_MBAR_TIMEOUT);
@@ -1048,16 +1168,12 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     zero(x);
     product<true, kLd, kRows, true, LD, kState, 4>(x, sh.y[0], sh.ds[0], m0, d0);
 #pragma unroll
-    for (int half = 0; half < 2; half++) {  // F U dS'^T, and K_i . (dS' Y_i)
-      const int i = i0 + half * 8;
-      const float f = d.until[i], b = d.beta[i];
+    for (int half = 0; half < 2; half++) {  // F U dS'^T
+      const float f = d.until[i0 + half * 8] * d.beta[i0 + half * 8];
 #pragma unroll
       for (int n = 0; n < NK; n++) {
-        const __nv_bfloat162 k = *reinterpret_cast<const __nv_bfloat162*>(sh.k + i * LD + d0 + n * 8 + (lane & 3) * 2);
-        const float v0 = f == 0.f ? 0.f : f * x[n][half * 2], v1 = f == 0.f ? 0.f : f * x[n][half * 2 + 1];
-        krow[half] = __fmaf_rn(__low2float(k), v0, __fmaf_rn(__high2float(k), v1, krow[half]));
-        dk[n][half * 2] = __fmaf_rn(b, v0, dk[n][half * 2]);
-        dk[n][half * 2 + 1] = __fmaf_rn(b, v1, dk[n][half * 2 + 1]);
+        dk[n][half * 2] += f == 0.f ? 0.f : f * x[n][half * 2];
+        dk[n][half * 2 + 1] += f == 0.f ? 0.f : f * x[n][half * 2 + 1];
       }
     }
     product<false, kLd, 0, true, kLd, kRows, 4>(oy, o, sh.y[0], m0, n0);
@@ -1065,15 +1181,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     __syncthreads();
     if (t + 1 < steps) load_b(t + 1);
     if ((t + 1) % slices) continue;
-    // K K^T and Q K^T where this warp has dR Y^T and dO Y^T
-    float kk[2][4], qk[2][4];
-    zero(kk);
-    zero(qk);
-    product<false, LD, 0, false, LD, 0, DK / 16>(kk, sh.k, sh.k, m0, n0);
-    product<false, LD, 0, false, LD, 0, DK / 16>(qk, sh.q, sh.k, m0, n0);
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
-      float col[2] = {0.f, 0.f};
+    for (int n = 0; n < 2; n++)
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = i0 + half * 8, j = n0 + n * 8 + (lane & 3) * 2, ei = d.era[i];
@@ -1082,38 +1191,13 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           const int e = half * 2 + c;
-          const bool low = j + c <= i, strict = j + c < i;
-          const float f = low ? decay(ci, ei, d, j + c) : 0.f, b = d.beta[j + c];
-          const float ov = low ? a.scale * f * oy[n][e] : 0.f, rv = strict ? f * ry[n][e] : 0.f;
-          po[c] = b * ov;
-          mm[c] = -b * rv;
-          qrow[half] += (low ? qk[n][e] * po[c] : 0.f) + (strict ? kk[n][e] * mm[c] : 0.f);
-          col[c] += (low ? qk[n][e] * ov : 0.f) - (strict ? kk[n][e] * rv : 0.f);
+          const float f = j + c <= i ? d.beta[j + c] * decay(ci, ei, d, j + c) : 0.f;
+          po[c] = j + c <= i ? a.scale * f * oy[n][e] : 0.f;
+          mm[c] = j + c < i ? -f * ry[n][e] : 0.f;
         }
         put2<kLd>(sh.p[0], sh.p[1], i, j, po[0], po[1]);
         put2<kLd>(sh.m[0], sh.m[1], i, j, mm[0], mm[1]);
       }
-#pragma unroll
-      for (int c = 0; c < 2; c++)
-#pragma unroll
-        for (int w = 4; w < 32; w *= 2) col[c] += __shfl_xor_sync(0xffffffffu, col[c], w);
-      if (lane < 4) {
-        sh.col[wr][n0 + n * 8 + lane * 2] = col[0];
-        sh.col[wr][n0 + n * 8 + lane * 2 + 1] = col[1];
-      }
-    }
-#pragma unroll
-    for (int half = 0; half < 2; half++) {
-#pragma unroll
-      for (int w = 1; w < 4; w *= 2) {
-        qrow[half] += __shfl_xor_sync(0xffffffffu, qrow[half], w);
-        krow[half] += __shfl_xor_sync(0xffffffffu, krow[half], w);
-      }
-      if ((lane & 3) == 0) {
-        sh.row[wc][i0 + half * 8] = qrow[half];
-        sh.krow[wc][i0 + half * 8] = krow[half];
-      }
-    }
 #pragma unroll
     for (int w = 16; w; w >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, w);
     if (lane == 0) sh.sum[warp] = inner;
@@ -1122,30 +1206,24 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     product_part<true, kLd, kRows, true, LD, 0>(dk, sh.p[0], sh.q, m0, d0, wr, 4);
     product_part<false, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, 0, wr + 1);
     product_part<true, kLd, kRows, true, LD, 0>(dk, sh.m[0], sh.k, m0, d0, wr, 4);
-    // dbeta, and dg by sums of W's rows less its columns from the chunk's end, cut at resets: by the first warp, for the last
-    // head while the others write dq and dk
+    // dbeta, and dg by sums from the chunk's end, cut at resets: by the first warp, for the last head while the others write dq
+    // and dk
     auto gates = [&] {
       const float keep = d.since[kC - 1];
       float end = 0.f, sum[2];
       int era[2];
 #pragma unroll
       for (int w = 0; w < 16; w++) end += sh.sum[w];
-      end = keep == 0.f ? 0.f : keep * end;
-      float tail = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = half * 32 + lane;
-        const float kd = (sh.krow[0][i] + sh.krow[1][i]) + (sh.krow[2][i] + sh.krow[3][i]);
-        const float c = (sh.col[0][i] + sh.col[1][i]) + (sh.col[2][i] + sh.col[3][i]);
-        if (i < len) p.dbeta[(start + i) * a.hv + h] = kd + c;
-        tail += d.beta[i] * kd;  // F_i u_i . (K_i dS')
-        sum[half] = (sh.row[0][i] + sh.row[1][i]) + (sh.row[2][i] + sh.row[3][i]) - d.beta[i] * (kd + c);
+        if (i < len) p.dbeta[(start + i) * a.hv + h] = sh.gate[i] / beta_of(d.beta[i]);
+        sum[half] = sh.gate[kC + i];
         era[half] = d.era[i];
       }
-#pragma unroll
-      for (int w = 16; w; w >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, w);
       const int last = __shfl_sync(0xffffffffu, era[1], 31);
-      float behind = end + tail;  // of the tokens behind this half, as far as they are of era `last`
+      // of the tokens behind this half, as far as they are of era `last`: <S', dS'>, what is behind the chunk
+      float behind = (keep == 0.f ? 0.f : keep * end) + sh.gate[2 * kC];
       int behind_era = last;
 #pragma unroll
       for (int half = 1; half >= 0; half--) {
@@ -1285,6 +1363,8 @@ static size_t states_bytes(const pl_delta_shape* s) {
   return up256(heads_slots(s) * (s->dk > 64 ? 136 : 72) * round_up((long)s->dv, 64) * 4);
 }
 static size_t rows_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * kLd * round_up((long)s->dv, 64) * 4); }
+static size_t lanes_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * kC * round_up((long)s->dv, 64) * 4); }
+static size_t sums_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * round_up((long)s->dv, 64) / 16 * kSums * 4); }
 
 template <typename A>
 static int launch_wide(void (*kernel)(A), dim3 grid, int threads, size_t smem, cudaStream_t st, const A& args) {
@@ -1294,6 +1374,8 @@ static int launch_wide(void (*kernel)(A), dim3 grid, int threads, size_t smem, c
   count_launch();
   return PL_OK;
 }
+static_assert(sizeof(ScanShared<128>) <= 232448 && sizeof(BackShared<128>) <= 232448 && sizeof(GradShared<128>) <= 232448,
+              "shared memory of a block");
 static int prep(const DeltaArgs& a, Mats* mats, __nv_bfloat16* tiles, int2* table, cudaStream_t st) {
   const dim3 grid((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
   const bool wide = a.dk > 64;
@@ -1320,11 +1402,11 @@ extern "C" {
 
 size_t pl_delta_saved(const pl_delta_shape* s) {
   if (!s || s->sequences == 0) return 0;
-  return pl::states_bytes(s) + pl::rows_bytes(s) + pl::mats_bytes(s);
+  return pl::states_bytes(s) + 2 * pl::lanes_bytes(s) + pl::mats_bytes(s);
 }
 size_t pl_delta_ws(const pl_delta_shape* s, uint8_t grad) {
   if (!s || s->sequences == 0) return 0;
-  return grad ? pl::states_bytes(s) + pl::rows_bytes(s) : pl::mats_bytes(s);
+  return grad ? pl::states_bytes(s) + 2 * pl::rows_bytes(s) + pl::sums_bytes(s) : pl::mats_bytes(s);
 }
 
 int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g, const float* beta,
@@ -1348,19 +1430,21 @@ int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const vo
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const DeltaArgs a = delta_args(s, q, k, v, g, beta, offsets);
-  Mats* mats = (Mats*)(saved ? (char*)saved + states_bytes(s) + rows_bytes(s) : ws);
+  Mats* mats = (Mats*)(saved ? (char*)saved + states_bytes(s) + 2 * lanes_bytes(s) : ws);
   if (s->tokens) {
     rc = prep(a, mats, tiles_of(s, mats), table_of(s, mats), st);
     if (rc) return rc;
   }
-  ScanArgs p = {a, mats, tiles_of(s, mats), state, (__nv_bfloat16*)o, final_state, nullptr, nullptr};
+  ScanArgs p = {a, mats, tiles_of(s, mats), state, (__nv_bfloat16*)o, final_state, nullptr, nullptr, nullptr};
   if (saved) {
     p.kept = (__nv_bfloat16*)saved;
-    p.y = (__nv_bfloat16*)((char*)saved + states_bytes(s));
+    p.y = (float*)((char*)saved + states_bytes(s));
+    p.out = (float*)((char*)saved + states_bytes(s) + lanes_bytes(s));
   }
   const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
-  return a.dk > 64 ? launch_wide(delta_scan_kernel<128>, grid, kChainThreads, sizeof(ScanShared<128>), st, p)
-                   : launch_wide(delta_scan_kernel<64>, grid, kChainThreads, sizeof(ScanShared<64>), st, p);
+  auto kernel = saved ? (a.dk > 64 ? delta_scan_kernel<128, true> : delta_scan_kernel<64, true>)
+                      : (a.dk > 64 ? delta_scan_kernel<128, false> : delta_scan_kernel<64, false>);
+  return launch_wide(kernel, grid, kChainThreads, a.dk > 64 ? sizeof(ScanShared<128>) : sizeof(ScanShared<64>), st, p);
 }
 
 int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token, size_t do_head, const float* dfinal,
@@ -1387,18 +1471,18 @@ int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token
   const DeltaArgs a = delta_args(s, q, k, v, g, beta, offsets);
   __nv_bfloat16 *ds = (__nv_bfloat16*)ws, *dr = (__nv_bfloat16*)((char*)ws + states_bytes(s));
   const int align_o = row_align(dout, do_token, do_head);
-  Mats* mats = (Mats*)((char*)saved + states_bytes(s) + rows_bytes(s));
+  __nv_bfloat16* y = (__nv_bfloat16*)((char*)dr + rows_bytes(s));
+  float* sums = (float*)((char*)y + rows_bytes(s));
+  float *yf = (float*)((char*)saved + states_bytes(s)), *out = (float*)((char*)yf + lanes_bytes(s));
+  Mats* mats = (Mats*)((char*)out + lanes_bytes(s));
   const BackArgs b = {a, mats, tiles_of(s, mats), (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, dfinal,
-                      (__nv_bfloat16*)dv, dstate, ds, dr};
+                      yf, out, (__nv_bfloat16*)dv, dstate, ds, dr, y, sums};
   const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
   rc = a.dk > 64 ? launch_wide(delta_back_kernel<128>, grid, kChainThreads, sizeof(BackShared<128>), st, b)
                  : launch_wide(delta_back_kernel<64>, grid, kChainThreads, sizeof(BackShared<64>), st, b);
   if (rc || s->tokens == 0) return rc;
-  const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, (const __nv_bfloat16*)saved,
-                      (const __nv_bfloat16*)((const char*)saved + states_bytes(s)), ds, dr, mats,
-                      tiles_of(s, mats), table_of(s, mats),
-                      (__nv_bfloat16*)dq, (__nv_bfloat16*)dk,
-                      dg, dbeta};
+  const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, (const __nv_bfloat16*)saved, y, ds, dr,
+                      sums, mats, tiles_of(s, mats), table_of(s, mats), (__nv_bfloat16*)dq, (__nv_bfloat16*)dk, dg, dbeta};
   const dim3 chunks((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
   rc = a.dk > 64 ? launch_wide(delta_grad_kernel<128>, chunks, kGradThreads, sizeof(GradShared<128>), st, p)
                  : launch_wide(delta_grad_kernel<64>, chunks, kGradThreads, sizeof(GradShared<64>), st, p);

@@ -227,57 +227,100 @@ __device__ __forceinline__ void put2(__nv_bfloat16* hi, __nv_bfloat16* lo, int r
 }
 
 // ---- products whose first operand is in registers: an accumulator's two neighbouring n-tiles, 16 rows x 16 columns, are
-// the fragment of A for 16 steps of k, as two bf16 parts.
+// the fragment of A for 16 steps of k, as N bf16 parts: three hold all 24 bits of an f32.
+template <int N>
 struct Parts {
-  uint32_t hi[4], lo[4];
+  uint32_t p[N][4];
 };
-__device__ __forceinline__ Parts parts_of(const float (&x)[4], const float (&y)[4]) {
-  Parts p;
-  split2(x[0], x[1], p.hi[0], p.lo[0]);
-  split2(x[2], x[3], p.hi[1], p.lo[1]);
-  split2(y[0], y[1], p.hi[2], p.lo[2]);
-  split2(y[2], y[3], p.hi[3], p.lo[3]);
-  return p;
+template <int N>
+__device__ __forceinline__ void split(float x, float y, Parts<N>& to, int at) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    to.p[i][at] = *reinterpret_cast<const uint32_t*>(&h);
+    x -= __low2float(h);
+    y -= __high2float(h);
+  }
 }
-// acc [16][16 N] += A B for one 16 of k: B bf16, at `at` and every `step` bytes. All first parts go before the second ones:
-// a product waits 25 cycles for the one before it on the same accumulator, and N of them take 8 N.
-template <bool ACROSS, int N>
-__device__ __forceinline__ void step(float (&acc)[2 * N][4], const Parts& a, uint32_t at, int step) {
+template <int N>
+__device__ __forceinline__ Parts<N> parts_of(const float (&x)[4], const float (&y)[4]) {
+  Parts<N> r;
+  split<N>(x[0], x[1], r, 0);
+  split<N>(x[2], x[3], r, 1);
+  split<N>(y[0], y[1], r, 2);
+  split<N>(y[2], y[3], r, 3);
+  return r;
+}
+// acc [16][16 N] += A B for one 16 of k: B bf16, at `at` and every `step` bytes. The first parts add to `acc` and the others to `low`,
+// which joins it by `join`: the tensor cores cut a sum off behind its 24th bit, towards zero, and a small product added to a large
+// sum costs it as much as a large one. All first parts go before the second ones: a product waits 25 cycles for the one before
+// it on the same accumulator, and N of them take 8 N.
+template <bool ACROSS, int N, int PARTS>
+__device__ __forceinline__ void step(float (&acc)[2 * N][4], float (&low)[2 * N][4], const Parts<PARTS>& a, uint32_t at,
+                                     int step) {
   uint32_t y[N][4];
 #pragma unroll
   for (int n = 0; n < N; n++) ldsm<ACROSS>(y[n], at + n * step);
 #pragma unroll
-  for (int n = 0; n < N; n++) {
-    mma(acc[2 * n], a.hi, y[n][0], y[n][1]);
-    mma(acc[2 * n + 1], a.hi, y[n][2], y[n][3]);
-  }
+  for (int i = 0; i < PARTS; i++)
 #pragma unroll
-  for (int n = 0; n < N; n++) {
-    mma(acc[2 * n], a.lo, y[n][0], y[n][1]);
-    mma(acc[2 * n + 1], a.lo, y[n][2], y[n][3]);
+    for (int n = 0; n < N; n++) {
+      mma(i ? low[2 * n] : acc[2 * n], a.p[i], y[n][0], y[n][1]);
+      mma(i ? low[2 * n + 1] : acc[2 * n + 1], a.p[i], y[n][2], y[n][3]);
+    }
+}
+template <int NT>
+__device__ __forceinline__ void join(float (&acc)[NT][4], const float (&low)[NT][4]) {
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[t][e] += low[t][e];
+}
+// to(t, sum) for the n-tiles t of A B over the four 16 of a chunk's tokens, [16][8 NT], B across; half of them at a time, so that
+// the sums of parts have registers.
+template <int LD, int NT, int PARTS, typename F>
+__device__ __forceinline__ void token_steps(const Parts<PARTS> (&a)[4], uint32_t at, F to) {
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    float acc[NT / 2][4], low[NT / 2][4];
+#pragma unroll
+    for (int t = 0; t < NT / 2; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[t][e] = low[t][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) step<true, NT / 4>(acc, low, a[k], at + k * 32 * LD + q * NT * 8, 32);
+    join(acc, low);
+#pragma unroll
+    for (int t = 0; t < NT / 2; t++) to(q * (NT / 2) + t, acc[t]);
   }
 }
-// acc [dv][64 tokens] += A T^T (ACROSS = false: column block n over blocks k <= n) or A T (ACROSS: over k >= n) for the k-th 16
-// columns of A; T triangular, two parts; A two parts or (TWO = false) its first alone.
-template <bool ACROSS, bool TWO = true>
-__device__ __forceinline__ void tri_step(float (&acc)[8][4], const Parts& a, uint32_t tri, int k) {
-  uint32_t y[4][4];
+// acc [dv][64 tokens] += A T^T (ACROSS = false: column block n over blocks k <= n) or A T (ACROSS: over k >= n) for A's four 16
+// columns; T triangular, three parts. Of parts i and j, those with i + j < PAIRS, the smallest products first.
+template <bool ACROSS, int PARTS, int PAIRS>
+__device__ __forceinline__ void tri_product(float (&acc)[8][4], const Parts<PARTS> (&a)[4], uint32_t tri) {
 #pragma unroll
-  for (int part = 0; part < 3; part++) {
+  for (int ij = PAIRS - 1; ij >= 0; ij--)
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
-      if (part == 1 || (ACROSS ? n > k : n < k)) continue;
-      const int r = ACROSS ? k : n, c = ACROSS ? n : k;
-      ldsm<ACROSS>(y[n], tri + (r * (r + 1) / 2 + c) * 512 + (part == 2 ? kTri * 2 : 0));
+    for (int j = 0; j <= ij; j++) {
+      const int i = ij - j;
+      if (i >= PARTS) continue;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        uint32_t y[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          if (ACROSS ? n > k : n < k) continue;
+          const int r = ACROSS ? k : n, c = ACROSS ? n : k;
+          ldsm<ACROSS>(y[n], tri + (r * (r + 1) / 2 + c) * 512 + j * kTri * 2);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          if (ACROSS ? n > k : n < k) continue;
+          mma(acc[2 * n], a[k].p[i], y[n][0], y[n][1]);
+          mma(acc[2 * n + 1], a[k].p[i], y[n][2], y[n][3]);
+        }
+      }
     }
-#pragma unroll
-    for (int n = 0; n < 4; n++) {
-      if ((ACROSS ? n > k : n < k) || (part == 1 && !TWO)) continue;
-      const uint32_t(&x)[4] = part == 1 ? a.lo : a.hi;
-      mma(acc[2 * n], x, y[n][0], y[n][1]);
-      mma(acc[2 * n + 1], x, y[n][2], y[n][3]);
-    }
-  }
 }
 // Registers of one warp for another one's same lanes: pieces of 16 bytes per lane at `at`.
 __device__ __forceinline__ void give(uint4* at, int piece, const uint32_t (&r)[4]) {
