@@ -374,19 +374,12 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(
 }
 
 // ---------------------------------------------------------------------------------------------- the chain forward
-// What a chain leaves for the products of the last kernel, per slot, value head and 64 columns of v, as two bf16 parts one behind
-// the other, in rows as they stand in shared memory (one bulk copy): a state, transposed, [2][64][dkp + 8], and rows, transposed,
-// [2][64][72], 64 tokens in each.
-__device__ __forceinline__ long state_at(const DeltaArgs& a, long slot, int h, int slice) {
-  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * 64 * (a.dkp + 8);
+// What the chains leave for other kernels, f32, per slot, value head and 64 columns of v, as a warp's lanes hold it, four warps of 16
+// columns one behind the other: states, and rows of 64 tokens.
+__device__ __forceinline__ uint4* states_at(const DeltaArgs& a, const void* base, long slot, int h, int slice, int warp) {
+  return (uint4*)base + (((slot * a.hv + h) * (a.dvp / 64) + slice) * 4 + warp) * (a.dkp / 8 * 32);
 }
-__device__ __forceinline__ long rows_at(const DeltaArgs& a, long slot, int h, int slice) {
-  return ((slot * a.hv + h) * (a.dvp / 64) + slice) * 2 * kC * kLd;
-}
-
-// What the forward chain leaves for the sums of the chain back, f32: 64 columns of v of 64 tokens as a warp's lanes hold them, four
-// warps, 16 columns each, one behind the other.
-__device__ __forceinline__ uint4* lanes_at(const DeltaArgs& a, void* base, long slot, int h, int slice, int warp) {
+__device__ __forceinline__ uint4* lanes_at(const DeltaArgs& a, const void* base, long slot, int h, int slice, int warp) {
   return (uint4*)base + (((slot * a.hv + h) * (a.dvp / 64) + slice) * 4 + warp) * (8 * 32);
 }
 
@@ -397,8 +390,7 @@ struct ScanArgs {
   const float* state;  // [seqs][hv][dk][dv], or NULL: zero
   __nv_bfloat16* o;    // [n][hv][dv]
   float* final_state;
-  __nv_bfloat16* kept;  // for the gradient: S of every slot; or NULL
-  float *y, *out;       // and Y and the f32 outputs
+  float *kept, *y, *out;  // for the gradient: S, Y and the f32 outputs of every slot
 };
 // A chunk's inputs, loaded while the chunk before it is worked on; x: 64 columns of v (forward), of dO (back).
 template <int DK>
@@ -452,41 +444,14 @@ __device__ __forceinline__ void state_out(const float (&s)[NT][4], float* dst, i
       if (i < dk && j < cols) dst[(long)i * dv + j] = s[t][e];
     }
 }
-// An accumulator [16 of dv][8 NT] as two parts into [2][64][row] from `dst` (this warp's first row) on.
-template <int NT>
-__device__ __forceinline__ void parts_out(const float (&s)[NT][4], __nv_bfloat16* dst, int row, long second) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int t = 0; t < NT; t++)
-#pragma unroll
-    for (int half = 0; half < 2; half++) {
-      uint32_t hi, lo;
-      split2(s[t][half * 2], s[t][half * 2 + 1], hi, lo);
-      __nv_bfloat16* at = dst + ((lane >> 2) + half * 8) * row + t * 8 + (lane & 3) * 2;
-      *reinterpret_cast<uint32_t*>(at) = hi;
-      *reinterpret_cast<uint32_t*>(at + second) = lo;
-    }
-}
-// A warp's state [16 of dv][DK] as its lanes hold it, as two parts into [2][64][DK + 8] from `dst` (its first row) on.
-template <int DK>
-__device__ __forceinline__ void state_parts(const uint4* s, __nv_bfloat16* dst) {
-  const int lane = threadIdx.x & 31;
-  constexpr int LD = DK + 8;
-#pragma unroll
-  for (int k = 0; k < DK / 16; k++) {
-    float s0[4], s1[4];
-    take(s, 2 * k, s0);
-    take(s, 2 * k + 1, s1);
-    const Parts<2> x = parts_of<2>(s0, s1);
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      __nv_bfloat16* at = dst + i * 64 * LD + (lane >> 2) * LD + k * 16 + (lane & 3) * 2;
-      *reinterpret_cast<uint32_t*>(at) = x.p[i][0];
-      *reinterpret_cast<uint32_t*>(at + 8 * LD) = x.p[i][1];
-      *reinterpret_cast<uint32_t*>(at + 8) = x.p[i][2];
-      *reinterpret_cast<uint32_t*>(at + 8 * LD + 8) = x.p[i][3];
-    }
+// A warp's tiles from shared memory to memory, by its first lane; they may be written again when it returns.
+__device__ __forceinline__ void lanes_out(void* dst, const void* src, uint32_t bytes) {
+  if ((threadIdx.x & 31) == 0) {
+    bulk_out(dst, src, bytes);
+    tc::bulk_commit();
+    tc::bulk_wait_read<0>();
   }
+  __syncwarp();
 }
 // 64 rows of 16 values that this warp put at `tile`, to rows of `stride` in memory, `cols` of them.
 __device__ __forceinline__ void rows_out(const __nv_bfloat16* tile, __nv_bfloat16* dst, long stride, int len, int cols,
@@ -545,6 +510,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     for (int t = 0; t < NK; t++) give(sh.s[warp], t, s[t]);
     for (long c = 0; c < chunks; c++) {
       ChainIn<DK>& in = sh.in[c & 1];
+      if constexpr (SAVE) tc::fence_proxy_async_smem();  // bulk copies take S and Y
       meet<kChainThreads>(kAll);
       tc::mbar_wait(&sh.full[c & 1], c >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
       float r[8][4], low[8][4];  // (K S)^T: [16 of dv][64 tokens]
@@ -584,6 +550,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
       tri_product<false, 3, 3>(y, z, tri_lane<false>(in.m.x[0]));
 #pragma unroll
       for (int t = 0; t < 8; t++) give(sh.y[warp], t, y[t]);
+      if constexpr (SAVE) tc::fence_proxy_async_smem();
       meet_arrive<96>(y_ready);
       const float keep = in.m.d.since[kC - 1];
 #pragma unroll
@@ -703,23 +670,16 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
     if (c > 0) write_o(c - 1);
     meet<128>(kMovers);  // the place of chunk c - 1's inputs, and of its o, is free
     if (c + 1 < chunks) load(c + 1);
-    if constexpr (SAVE) state_parts<DK>(sh.s[warp], p.kept + state_at(a, slot0 + c, h, slice) + warp * 16 * LD);
+    if constexpr (SAVE) lanes_out(states_at(a, p.kept, slot0 + c, h, slice, warp), sh.s[warp], sizeof(sh.s[0]));
     meet_arrive<96>(s_read);
     meet<96>(y_ready);
-    if constexpr (SAVE) {
-      uint4* to = lanes_at(a, p.y, slot0 + c, h, slice, warp);
-#pragma unroll
-      for (int t = 0; t < 8; t++) {
-        uint32_t y[4];
-        take(sh.y[warp], t, y);
-        give(to, t, y);
-      }
-    }
+    if constexpr (SAVE) lanes_out(lanes_at(a, p.y, slot0 + c, h, slice, warp), sh.y[warp], sizeof(sh.y[0]));
   }
   if (chunks) {
     meet<kChainThreads>(kAll);
     write_o(chunks - 1);
   }
+  if constexpr (SAVE) tc::bulk_wait<0>();
 }
 
 // ---------------------------------------------------------------------------------------------- the chain back
@@ -730,14 +690,14 @@ struct BackArgs {
   const __nv_bfloat16* dout;  // [n][hv][dv], strides below
   long ldo, hso;
   int align_o;
-  const float* dfinal;         // [seqs][hv][dk][dv], or NULL: zero
-  float *yf, *out;             // of the forward pass: Y and the f32 outputs
-  __nv_bfloat16* dv;           // [n][hv][dv]
-  float* dstate;               // or NULL
-  __nv_bfloat16 *ds, *dr, *y;  // dS', dR and Y of every slot
-  float* sums;                 // sums_at
+  const float* dfinal;          // [seqs][hv][dk][dv], or NULL: zero
+  const float *kept, *y, *out;  // of the forward pass: S, Y and the f32 outputs
+  __nv_bfloat16* dv;            // [n][hv][dv]
+  float* dstate;                // or NULL
+  float *ds, *dr;               // dS' and dR of every slot
+  float* sums;                  // sums_at
 };
-// Per slot, value head and 16 columns of v, sums over them: of every token Y . Z beta' and o . dO - v . dR, of the chunk F K dS' . U.
+// Per slot, value head and 16 columns of v, sums over them: of every token Y . Z beta' and o . dO - v . dR, of the chunk <S', dS'>.
 constexpr int kSums = 2 * kC + 2;
 __device__ __forceinline__ long sums_at(const DeltaArgs& a, long slot, int h, int group) {
   return ((slot * a.hv + h) * (a.dvp / 16) + group) * kSums;
@@ -802,6 +762,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     for (int t = 0; t < NK; t++) give(sh.s[warp], t, s[t]);
     for (long c = chunks - 1, it = 0; c >= 0; c--, it++) {
       ChainIn<DK>& in = sh.in[it & 1];
+      tc::fence_proxy_async_smem();  // bulk copies take dS' and dR
       meet<kChainThreads>(kAll);
       tc::mbar_wait(&sh.full[it & 1], it >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
       float x[8][4], low[8][4];  // (K dS')^T: [16 of dv][64 tokens]
@@ -843,6 +804,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
       }
 #pragma unroll
       for (int t = 0; t < 8; t++) give(sh.x[warp], t, r[t]);
+      tc::fence_proxy_async_smem();
       meet_arrive<64>(r_ready);
       Parts<EP> z[4];
 #pragma unroll
@@ -956,22 +918,34 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     cp_commit();
     if (c > 0) load(c - 1);
     cp_commit();
-    const uint4 *yf = lanes_at(a, p.yf, slot, h, slice, warp), *of = lanes_at(a, p.out, slot, h, slice, warp);
+    const uint4 *sf = states_at(a, p.kept, slot, h, slice, warp), *yf = lanes_at(a, p.y, slot, h, slice, warp);
+    const uint4* of = lanes_at(a, p.out, slot, h, slice, warp);
+    lanes_out(states_at(a, p.ds, slot, h, slice, warp), sh.s[warp], sizeof(sh.s[0]));
+    float fu = 0.f;  // <S, dS'> over 16 columns
+#pragma unroll
+    for (int t = 0; t < NK; t++) {
+      float u[4], v[4];
+      take(sf, t, u);
+      take(sh.s[warp], t, v);
+#pragma unroll
+      for (int e = 0; e < 4; e++) fu = __fmaf_rn(u[e], v[e], fu);
+    }
+    meet_arrive<kChainThreads>(kRead);
     float y[8][4], o[8][4];
 #pragma unroll
     for (int t = 0; t < 8; t++) {
       take(yf, t, y[t]);
       take(of, t, o[t]);
     }
-    state_parts<DK>(sh.s[warp], p.ds + state_at(a, slot, h, slice) + warp * 16 * LD);
-    meet_arrive<kChainThreads>(kRead);
-    parts_out(y, p.y + rows_at(a, slot, h, slice) + warp * 16 * kLd, kLd, (long)kC * kLd);
     cp_wait<1>();
     meet<128>(kMovers);  // v is there
     tc::mbar_wait(&sh.full[(chunks - 1 - c) & 1], (chunks - 1 - c) >> 1 & 1, a.err, PL_ERR_MBAR_TIMEOUT);
     meet<64>(r_ready);
     const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>()), pv = smem_u32(sh.v + warp * 16 + lane_a<true, kLd>());
-    float zy[8][2], ov[8][2], fu = 0.f;
+    float zy[8][2], ov[8][2];
+    const float keep = in.m.d.since[kC - 1];
+    fu = keep == 0.f ? 0.f : keep * fu;  // and F K dS' . U: <S', dS'>
+    lanes_out(lanes_at(a, p.dr, slot, h, slice, warp), sh.x[warp], sizeof(sh.x[0]));
 #pragma unroll
     for (int n = 0; n < 4; n++) {
       uint32_t d4[4], v4[4];
@@ -1000,8 +974,6 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
       }
       // this warp and the helper have read these columns of dO: dv takes their place on its way out
       store_across(across_at(in.x + warp * 16, n), r[0], r[1]);
-      const float rr[2][4] = {{r[0][0], r[0][1], r[0][2], r[0][3]}, {r[1][0], r[1][1], r[1][2], r[1][3]}};
-      parts_out(rr, p.dr + rows_at(a, slot, h, slice) + warp * 16 * kLd + n * 16, kLd, (long)kC * kLd);
     }
     float* sums = p.sums + sums_at(a, slot, h, slice * 4 + warp);
     reinterpret_cast<float2*>(sums)[lane] = column_sums(zy);
@@ -1012,6 +984,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     __syncwarp();
     rows_out(in.x + warp * 16, p.dv + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_dv);
   }
+  tc::bulk_wait<0>();
 }
 
 // ---------------------------------------------------------------------------------------------- the other gradients
@@ -1022,8 +995,7 @@ struct GradArgs {
   const __nv_bfloat16* dout;
   long ldo, hso;
   int align_o;
-  const __nv_bfloat16 *kept, *y, *ds, *dr;
-  const float* sums;
+  const float *kept, *y, *ds, *dr, *sums;
   const Mats* mats;
   const __nv_bfloat16* tiles;
   const int2* table;
@@ -1036,9 +1008,30 @@ struct GradShared {
   __nv_bfloat16 o[2][kC * kLd], r[2][2][kC * kLd];  // by turns: the next step's are on their way
   __nv_bfloat16 s[2][kC * (DK + 8)], ds[2][kC * (DK + 8)], y[2][kC * kLd];  // transposed, as r
   __nv_bfloat16 p[2][kC * kLd], m[2][kC * kLd];     // scale dO U^T * D, -M
-  float sum[16], gate[2 * kC + 1];
+  float gate[2 * kC + 1];
   Decay decay[2];  // by turns, a head's
   uint64_t full[2];  // S, dO, dR (and K, Q, the decays); dS', Y
+};
+// A tile [64 of dv][8 NT] in f32, as four warps' lanes hold it, that a block turns into two bf16 parts of it, [2][64][LD], at the same
+// place: read by all, a barrier, written.
+template <int NT>
+struct F32Tile {
+  static constexpr int N = NT * 128 / kGradThreads;
+  uint4 v[N];
+  __device__ __forceinline__ void take(const __nv_bfloat16* from, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = reinterpret_cast<const uint4*>(from)[i * kGradThreads + tid];
+  }
+  template <int LD>
+  __device__ __forceinline__ void give(__nv_bfloat16* to, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int at = i * kGradThreads + tid, lane = at & 31, t = at / 32 % NT, w = at / 32 / NT;
+      __nv_bfloat16* p = to + (w * 16 + (lane >> 2)) * LD + t * 8 + (lane & 3) * 2;
+      put2<LD>(p, p + kC * LD, 0, 0, __uint_as_float(v[i].x), __uint_as_float(v[i].y));
+      put2<LD>(p, p + kC * LD, 8, 0, __uint_as_float(v[i].z), __uint_as_float(v[i].w));
+    }
+  }
 };
 // A block per chunk and key head, 16 warps: its value heads one after the other, so that what they add to dq and dk stays in
 // registers and is added in their order; of each, 64 columns of v after the other (a step). A step's loads are under
@@ -1064,17 +1057,16 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
   if (start < 0 || start >= a.n || chunk.y <= 0) return;  // (inside the tensors, whatever `saved` holds)
   const int most = (int)(a.n - start < kC ? a.n - start : kC), len = chunk.y < most ? chunk.y : most;
   const int slices = a.dvp / 64, steps = group * slices;
-  constexpr uint32_t kStateBytes = 2 * kC * LD * 2, kRowsBytes = 2 * kC * kLd * 2;
+  constexpr uint32_t kStateBytes = kC * DK * 4, kRowsBytes = kC * kC * 4;
   auto load_a = [&](int t) {  // S, dO, dR, a head's decays
     const int h = kh * group + t / slices, slice = t % slices, c0 = slice * 64;
     const int cols = a.dv - c0 < 64 ? a.dv - c0 : 64;
-    tc::fence_proxy_async_smem();  // what was there has been read the ordinary way
     if (tid == 64) {
       tc::mbar_expect_tx(&sh.full[0], kStateBytes + kRowsBytes + (slice == 0 ? sizeof(Decay) : 0) +
                                           (t == 0 ? kTileBytes<DK> : 0));
       if (t == 0) bulk_in(sh.k, p.tiles + tile_at<DK>(a, slot, kh), kTileBytes<DK>, &sh.full[0]);
-      bulk_in(sh.s, p.kept + state_at(a, slot, h, slice), kStateBytes, &sh.full[0]);
-      bulk_in(sh.r[t & 1], p.dr + rows_at(a, slot, h, slice), kRowsBytes, &sh.full[0]);
+      bulk_in(sh.s, states_at(a, p.kept, slot, h, slice, 0), kStateBytes, &sh.full[0]);
+      bulk_in(sh.r[t & 1], lanes_at(a, p.dr, slot, h, slice, 0), kRowsBytes, &sh.full[0]);
       if (slice == 0) bulk_in(&sh.decay[t / slices & 1], &p.mats[slot * a.hv + h].d, sizeof(Decay), &sh.full[0]);
     }
     copy_tile<64, kLd, kGradThreads>(sh.o[t & 1], p.dout + start * p.ldo + h * p.hso + c0, p.ldo, len, cols, p.align_o, tid);
@@ -1082,11 +1074,10 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
   };
   auto load_b = [&](int t) {  // dS', Y
     const int h = kh * group + t / slices, slice = t % slices;
-    tc::fence_proxy_async_smem();
     if (tid == 0) {
       tc::mbar_expect_tx(&sh.full[1], kStateBytes + kRowsBytes);
-      bulk_in(sh.ds, p.ds + state_at(a, slot, h, slice), kStateBytes, &sh.full[1]);
-      bulk_in(sh.y, p.y + rows_at(a, slot, h, slice), kRowsBytes, &sh.full[1]);
+      bulk_in(sh.ds, states_at(a, p.ds, slot, h, slice, 0), kStateBytes, &sh.full[1]);
+      bulk_in(sh.y, lanes_at(a, p.y, slot, h, slice, 0), kRowsBytes, &sh.full[1]);
     }
   };
   __syncthreads();
@@ -1094,7 +1085,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
   load_b(0);
   const int wr = warp & 3, wc = warp >> 2, m0 = wr * 16, i0 = m0 + (lane >> 2);
   const int n0 = wc * 16, d0 = wc * (DK / 4);  // this warp's columns of a 64 x 64 tile, of a 64 x dk tile
-  float dq[NK][4], dk[NK][4], oy[2][4], ry[2][4], inner = 0.f;
+  float dq[NK][4], dk[NK][4], oy[2][4], ry[2][4];
   zero(dq);
   zero(dk);
   for (int t = 0; t < steps; t++) {
@@ -1105,7 +1096,6 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     if (t % slices == 0) {
       zero(oy);
       zero(ry);
-      inner = 0.f;
       // the chain's sums of this head, by token; warp 4: of the chunk
       const float* sums = p.sums + sums_at(a, slot, h, 0);
       float v = 0.f;
@@ -1122,6 +1112,15 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     }
     cp_wait<0>();
     tc::mbar_wait(&sh.full[0], t & 1, a.err, PL_ERR_MBAR_TIMEOUT);
+    {
+      F32Tile<DK / 8> ts;
+      F32Tile<8> tr;
+      ts.take(sh.s[0], tid);
+      tr.take(sh.r[t & 1][0], tid);
+      __syncthreads();
+      ts.template give<LD>(sh.s[0], tid);
+      tr.template give<kLd>(sh.r[t & 1][0], tid);
+    }
     __syncthreads();
     float x[NK][4];
     zero(x);
@@ -1147,24 +1146,16 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
       }
     }
     tc::mbar_wait(&sh.full[1], t & 1, a.err, PL_ERR_MBAR_TIMEOUT);
-#pragma unroll
-    for (int i = tid; i < kC * DK / 8; i += kGradThreads) {  // <S, dS'>, eight values at a time
-      const int at = i / (DK / 8) * LD + i % (DK / 8) * 8;
-      const uint4 sh4 = *reinterpret_cast<const uint4*>(sh.s[0] + at), sl4 = *reinterpret_cast<const uint4*>(sh.s[1] + at);
-      const uint4 dh4 = *reinterpret_cast<const uint4*>(sh.ds[0] + at), dl4 = *reinterpret_cast<const uint4*>(sh.ds[1] + at);
-      auto add = [&](uint32_t a, uint32_t b, uint32_t c, uint32_t e) {
-        inner = __fmaf_rn(__uint_as_float(a << 16) + __uint_as_float(b << 16),
-                          __uint_as_float(c << 16) + __uint_as_float(e << 16), inner);
-        a &= 0xffff0000u, b &= 0xffff0000u, c &= 0xffff0000u, e &= 0xffff0000u;
-        inner = __fmaf_rn(__uint_as_float(a) + __uint_as_float(b), __uint_as_float(c) + __uint_as_float(e), inner);
-      };
-      add(sh4.x, sl4.x, dh4.x, dl4.x);
-      add(sh4.y, sl4.y, dh4.y, dl4.y);
-      add(sh4.z, sl4.z, dh4.z, dl4.z);
-      add(sh4.w, sl4.w, dh4.w, dl4.w);
-    }
+    F32Tile<DK / 8> ts;
+    F32Tile<8> ty;
+    ts.take(sh.ds[0], tid);
+    ty.take(sh.y[0], tid);
+    tc::fence_proxy_async_smem();  // the places of S, dO and dR get new ones
     __syncthreads();
+    ts.template give<LD>(sh.ds[0], tid);
+    ty.template give<kLd>(sh.y[0], tid);
     if (t + 1 < steps) load_a(t + 1);
+    __syncthreads();
     zero(x);
     product<true, kLd, kRows, true, LD, kState, 4>(x, sh.y[0], sh.ds[0], m0, d0);
 #pragma unroll
@@ -1178,6 +1169,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     }
     product<false, kLd, 0, true, kLd, kRows, 4>(oy, o, sh.y[0], m0, n0);
     product<true, kLd, kRows, true, kLd, kRows, 4>(ry, r, sh.y[0], m0, n0);
+    tc::fence_proxy_async_smem();
     __syncthreads();
     if (t + 1 < steps) load_b(t + 1);
     if ((t + 1) % slices) continue;
@@ -1198,9 +1190,6 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
         put2<kLd>(sh.p[0], sh.p[1], i, j, po[0], po[1]);
         put2<kLd>(sh.m[0], sh.m[1], i, j, mm[0], mm[1]);
       }
-#pragma unroll
-    for (int w = 16; w; w >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, w);
-    if (lane == 0) sh.sum[warp] = inner;
     __syncthreads();
     product_part<false, kLd, kRows, true, LD, 0>(dq, sh.p[0], sh.k, m0, d0, 0, wr + 1);
     product_part<true, kLd, kRows, true, LD, 0>(dk, sh.p[0], sh.q, m0, d0, wr, 4);
@@ -1209,11 +1198,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
     // dbeta, and dg by sums from the chunk's end, cut at resets: by the first warp, for the last head while the others write dq
     // and dk
     auto gates = [&] {
-      const float keep = d.since[kC - 1];
-      float end = 0.f, sum[2];
+      float sum[2];
       int era[2];
-#pragma unroll
-      for (int w = 0; w < 16; w++) end += sh.sum[w];
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int i = half * 32 + lane;
@@ -1222,8 +1208,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
         era[half] = d.era[i];
       }
       const int last = __shfl_sync(0xffffffffu, era[1], 31);
-      // of the tokens behind this half, as far as they are of era `last`: <S', dS'>, what is behind the chunk
-      float behind = (keep == 0.f ? 0.f : keep * end) + sh.gate[2 * kC];
+      float behind = sh.gate[2 * kC];  // of the tokens behind this half, as far as they are of era `last`; behind the chunk, <S', dS'>
       int behind_era = last;
 #pragma unroll
       for (int half = 1; half >= 0; half--) {
@@ -1360,9 +1345,8 @@ static __nv_bfloat16* tiles_of(const pl_delta_shape* s, Mats* mats) {
 }
 static int2* table_of(const pl_delta_shape* s, Mats* mats) { return (int2*)((char*)tiles_of(s, mats) + tiles_bytes(s)); }
 static size_t states_bytes(const pl_delta_shape* s) {
-  return up256(heads_slots(s) * (s->dk > 64 ? 136 : 72) * round_up((long)s->dv, 64) * 4);
+  return up256(heads_slots(s) * (s->dk > 64 ? 128 : 64) * round_up((long)s->dv, 64) * 4);
 }
-static size_t rows_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * kLd * round_up((long)s->dv, 64) * 4); }
 static size_t lanes_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * kC * round_up((long)s->dv, 64) * 4); }
 static size_t sums_bytes(const pl_delta_shape* s) { return up256(heads_slots(s) * round_up((long)s->dv, 64) / 16 * kSums * 4); }
 
@@ -1406,7 +1390,7 @@ size_t pl_delta_saved(const pl_delta_shape* s) {
 }
 size_t pl_delta_ws(const pl_delta_shape* s, uint8_t grad) {
   if (!s || s->sequences == 0) return 0;
-  return grad ? pl::states_bytes(s) + 2 * pl::rows_bytes(s) + pl::sums_bytes(s) : pl::mats_bytes(s);
+  return grad ? pl::states_bytes(s) + pl::lanes_bytes(s) + pl::sums_bytes(s) : pl::mats_bytes(s);
 }
 
 int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g, const float* beta,
@@ -1437,7 +1421,7 @@ int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const vo
   }
   ScanArgs p = {a, mats, tiles_of(s, mats), state, (__nv_bfloat16*)o, final_state, nullptr, nullptr, nullptr};
   if (saved) {
-    p.kept = (__nv_bfloat16*)saved;
+    p.kept = (float*)saved;
     p.y = (float*)((char*)saved + states_bytes(s));
     p.out = (float*)((char*)saved + states_bytes(s) + lanes_bytes(s));
   }
@@ -1469,20 +1453,19 @@ int pl_delta_grad_dev(const pl_delta_shape* s, const void* dout, size_t do_token
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   const DeltaArgs a = delta_args(s, q, k, v, g, beta, offsets);
-  __nv_bfloat16 *ds = (__nv_bfloat16*)ws, *dr = (__nv_bfloat16*)((char*)ws + states_bytes(s));
+  float *ds = (float*)ws, *dr = (float*)((char*)ws + states_bytes(s)), *sums = (float*)((char*)dr + lanes_bytes(s));
+  const float *kept = (const float*)saved, *y = (const float*)((const char*)saved + states_bytes(s));
+  const float* out = (const float*)((const char*)y + lanes_bytes(s));
   const int align_o = row_align(dout, do_token, do_head);
-  __nv_bfloat16* y = (__nv_bfloat16*)((char*)dr + rows_bytes(s));
-  float* sums = (float*)((char*)y + rows_bytes(s));
-  float *yf = (float*)((char*)saved + states_bytes(s)), *out = (float*)((char*)yf + lanes_bytes(s));
   Mats* mats = (Mats*)((char*)out + lanes_bytes(s));
   const BackArgs b = {a, mats, tiles_of(s, mats), (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, dfinal,
-                      yf, out, (__nv_bfloat16*)dv, dstate, ds, dr, y, sums};
+                      kept, y, out, (__nv_bfloat16*)dv, dstate, ds, dr, sums};
   const dim3 grid((unsigned)(a.dvp / 64), (unsigned)a.hv, (unsigned)a.seqs);
   rc = a.dk > 64 ? launch_wide(delta_back_kernel<128>, grid, kChainThreads, sizeof(BackShared<128>), st, b)
                  : launch_wide(delta_back_kernel<64>, grid, kChainThreads, sizeof(BackShared<64>), st, b);
   if (rc || s->tokens == 0) return rc;
-  const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, (const __nv_bfloat16*)saved, y, ds, dr,
-                      sums, mats, tiles_of(s, mats), table_of(s, mats), (__nv_bfloat16*)dq, (__nv_bfloat16*)dk, dg, dbeta};
+  const GradArgs p = {a, (const __nv_bfloat16*)dout, (long)do_token, (long)do_head, align_o, kept, y, ds, dr, sums, mats,
+                      tiles_of(s, mats), table_of(s, mats), (__nv_bfloat16*)dq, (__nv_bfloat16*)dk, dg, dbeta};
   const dim3 chunks((unsigned)slot_count(a.n, a.seqs), (unsigned)a.hk);
   rc = a.dk > 64 ? launch_wide(delta_grad_kernel<128>, chunks, kGradThreads, sizeof(GradShared<128>), st, p)
                  : launch_wide(delta_grad_kernel<64>, chunks, kGradThreads, sizeof(GradShared<64>), st, p);
