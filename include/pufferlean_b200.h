@@ -597,13 +597,13 @@ int pl_sample_dev(const void* logits, size_t ld, size_t rows, size_t V, uint8_t 
  * All else has to be finite: 64 tokens are worked on at once, and a NaN or an infinity, one that an unstable rule has come to
  * included, reaches any token of its sequence in its 64 and behind them, whether a token between forgets or not; never
  * another sequence or a head that does not read it. What a sequence's first token forgets may be anything.
- * Products carry f32 operands, states among them, as two bf16 parts: f32 results are 5e-6 of their norm off as a rule, up to 1e-4
- * where terms cancel, bf16 ones by their own rounding. pl_delta_step_dev computes in f32.
+ * States, decays, gates' gradients and all sums are f32: f32 results are as near as f32 operations bring them, bf16 ones but for
+ * their own rounding.
  *
  * Sequences lie one behind the other: sequence s has tokens offsets[s] to offsets[s + 1] - 1 (int32 on the device,
  * not falling; NULL: `sequences` of equal length). Tokens in front of the first and behind the last belong to none: their outputs
  * are zero. state (NULL: zero) and final_state are [sequences][heads_v][dk][dv] f32. Either saved, for the gradient
- * (pl_delta_saved bytes: for 64 tokens of a head of 128 x 128 with a key head of its own 163 KB, three times what q, k and v
+ * (pl_delta_saved bytes: for 64 tokens of a head of 128 x 128 with a key head of its own 198 KB, four times what q, k and v
  * hold), or ws (pl_delta_ws bytes) is needed, 256-byte aligned. A wait for copies that ran out
  * (pl_device_check) leaves results that are not valid. */
 typedef struct {
@@ -616,7 +616,7 @@ size_t pl_delta_saved(const pl_delta_shape* s);
 int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g, const float* beta,
                  const int32_t* offsets, const float* state, void* o, float* final_state, void* saved, size_t saved_bytes,
                  void* ws, size_t ws_bytes, void* stream);
-/* Its gradient, from what the forward call saved: q, k, v, g and beta are checked as there, but their values are those that
+/* Its gradient, from v and what the forward call saved: q, k, g and beta are checked as there, but their values are those that
  * `saved` holds. dout [tokens][heads_v][dv] bf16 (strides in elements) and dfinal (of final_state; NULL: zero): dq, dk,
  * dv bf16, dg, dbeta f32 (zero dg at a token that forgets), dstate (of state; may be NULL). Sums go in a fixed order; what
  * heads of values add to the shared queries and keys is added in their order. */

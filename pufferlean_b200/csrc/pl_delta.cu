@@ -16,19 +16,17 @@
 //   dS = exp(G_last) dS' + scale (E Q)^T dO - (E K)^T dR
 //   dQ = scale (E dO S^T + (dO U^T * D) K)
 //   dK = -E dR S^T + F U dS'^T + scale (dO U^T * D)^T Q - (M + M^T) K,  M = strictly lower part of dR U^T times D
-//   dbeta_j = scale sum_i P_ij (dO_i . Y_j) + F_j K_j . (dS' Y_j) - sum_i N_ij (dR_i . Y_j)
-//   dg_t = sum over i >= t > j of W_ij, over i >= t of e_i and over j < t of f_j, and exp(G_last) <S, dS'>, with
-//          W = scale P * (dO U^T) - N * (dR U^T), e_i = E_i (scale q_i . S dO_i - k_i . S dR_i), f_j = F_j K_j . (dS' U_j)
+//   dbeta_t = Z_t . Y_t with dR = diag(beta) Z
+//   dg_t = sum over i >= t of (o_i . dO_i - v_i . dR_i), and <S', dS'> = exp(G_last) <S, dS'> + sum_j U_j . (F K dS')_j
 //
-// (up to the resets: what lies on two sides of one has no W, e or f). The sums for dg are taken as those over i >= t of
-// W's rows less W's columns: what is left out on both sides is the same number, so the products' errors cancel with it
-// (q . dq - v . dv is the same in exact arithmetic, and three times as far off).
+// (dg up to the next reset: behind one, neither tokens nor S' depend on g_t).
 //
 // X and P depend on q, k, g and beta alone: one kernel makes them for all chunks at once. What is left in the chain over a
 // sequence's chunks is a few products with the state, for each 64 columns of v on their own (columns do not mix), and
-// what the gradient needs beyond the two chains (S per chunk forward, dS' back) is again one kernel over all chunks.
-// f32 operands of products (S, Y, U, dR, X, P) go as two bf16 parts: with one, the states and gradients in f32 would be 2e-3
-// off, with two 5e-6.
+// what dq and dk need beyond the two chains (S per chunk forward, dS' back) is again one kernel over all chunks.
+// What f32 results come from is held in f32: states, Y, Z and the outputs between the kernels, and as operands of products
+// as three bf16 parts, which hold all 24 bits; f32 results are 1e-7 to 5e-7 off 64 bits, as with f32 operations. dq, dk and, without
+// a gradient, o are bf16 and nothing else: two parts, 3e-6 (the rounding: 1.7e-3; with one part they would be 2e-3 off).
 #include "pl_delta.cuh"
 #include "pl_runtime.h"
 
@@ -144,7 +142,7 @@ __global__ void __launch_bounds__(256) delta_step_kernel(const StepArgs p) {
 // Per slot and value head: X and P, triangular, as three bf16 parts each, and the decays; per slot and key head K and Q in
 // rows as they stand in shared memory, [2][64][dkp + 8], so that the other kernels get them by one bulk copy; per slot its
 // chunk's first token and length (0: none).
-// Measured: 8,192 chunks of a head, dk = 128, in 210 us, where their 730 MB would take 110: a block's dozen steps (search,
+// Measured: 8,192 chunks of a head, dk = 128, in 218 us, where their 820 MB would take 125: a block's dozen steps (search,
 // copies, decays, two products, the inverse in blocks of 16 and 32) wait for one another, four blocks to an SM.
 struct __align__(16) Mats {
   __nv_bfloat16 x[3][kTri], p[3][kTri];
@@ -472,14 +470,16 @@ __device__ __forceinline__ uint32_t across_at(const __nv_bfloat16* tile, int n) 
   return smem_u32(tile + (n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8) * kLd + ((lane >> 3) & 1) * 8);
 }
 
-// A block per sequence, value head and 64 columns of v. A warp of the chain keeps 16 columns of the state, transposed
-// [16][dk], in registers for the whole sequence, and everything that a chunk makes of it: an accumulator's layout is that
-// of a first operand, so K S, R, Y and F U go from one product into the next as they are, split into two bf16 parts. What the
-// next chunk's state does not wait for is another warp's, which gets the state's parts and Y through shared memory: Q S
-// and P U; a third one's is what goes from and to memory.
-// A chunk takes 3.9 us, 6,600 clocks. Its products are 316 and 188 of 16 x 8 x 16 for each scheduler, 8 clocks each: 4,032.
-// (All in one warp it took 5.5 us; with R, Y, U and the state's parts in shared memory, shared by 16 warps in four steps with
-// barriers, 5.6.) 4 x 8,192 tokens of 16 heads of 128 x 128: 500 us, 128 of 148 SMs with a chain of 128 chunks each.
+// A block per sequence, value head and 64 columns of v. A warp of the chain has 16 columns of the state, transposed [16][dk], and
+// everything that a chunk makes of it: an accumulator's layout is that of a first operand, so K S, R, Y and F U go from one product
+// into the next as they are, split into bf16 parts. The state is in shared memory, f32, as its lanes hold it (in registers,
+// as before there were sums of parts of their own, 390 bytes spilled: 880 us instead of 704); the sums of a chunk are added to it in f32. What
+// the next chunk's state does not wait for is another warp's, which reads the state and Y there: Q S and P U; a third one's is
+// what goes from and to memory.
+// A chunk takes 5.3 us, 9,900 clocks. Its products are 504 and, with or without a gradient, 312 or 188 of 16 x 8 x 16 for each
+// scheduler, 8 clocks each: 6,528 or 5,536. Without K S it would be 1.2 us less, without F U K 0.9, without X R 0.5. (With two parts
+// of each operand, 316 and 188 products, 3.9 us, and f32 results 3e-6 off.) 4 x 8,192 tokens of 16 heads of 128 x 128: 662 to
+// 678 us, 128 of 148 SMs with a chain of 128 chunks each.
 template <int DK, bool SAVE>
 __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const ScanArgs p) {
   grid_wait();
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
   long from, to;
   seq_bounds(a, seq, from, to);
   const long slot0 = from / kC + seq, chunks = (to - from + kC - 1) / kC;
-  const int s_read = 1 + warp, y_ready = 5 + warp;
+  const int s_read = 1 + warp, y_ready = 5 + warp, k_done = 9 + warp;
   if (threadIdx.x == 0) {
     tc::mbar_init(&sh.full[0], 1);
     tc::mbar_init(&sh.full[1], 1);
@@ -524,6 +524,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
         take(sh.s[warp], 2 * k + 1, s1);
         step<false, 4>(r, low, parts_of<3>(s0, s1), pk + k * 32, 32 * LD);
       }
+      meet_arrive<64>(k_done);
       join(r, low);
       const uint32_t px = smem_u32(in.x + warp * 16 + lane_a<true, kLd>());
 #pragma unroll
@@ -589,6 +590,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_scan_kernel(const Scan
       zero(o);
       zero(low);
       const uint32_t pq = smem_u32(in.q + lane_b<false, LD>());
+      meet<64>(k_done);  // K S goes first: beside Q S it takes 0.3 us longer
 #pragma unroll
       for (int k = 0; k < DK / 16; k++) {
         float s0[4], s1[4];
@@ -727,9 +729,11 @@ struct BackShared {
   uint4 f[4][8 * 32];       // F K dS'
   uint64_t full[2];
 };
-// As the chain forward, from the last chunk to the first. The helpers' products, of dO with P and Q, need nothing of the chain.
+// As the chain forward, from the last chunk to the first. The helpers' products, of dO with P and Q, need nothing of the chain; they add
+// theirs to dS' when the chain and memory have read it, the chain its own after that.
 // Memory's warps also make the gates' gradients of what passes through them, in f32: dbeta is Z . Y, token by token (X^T beta dU is
-// beta Z; where beta is zero, a tiny one stands in), and dg is sums of o . dO - v . dR.
+// beta Z; where beta is zero, a tiny one stands in), and dg is sums of o . dO - v . dR. 64 x 512 tokens of 8 heads of 128 x 128: 451 us,
+// where its 1.7 GB would take 260 (forward, with what the gradient needs written out: 392 to 402).
 template <int DK>
 __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const BackArgs p) {
   grid_wait();
@@ -1013,7 +1017,8 @@ struct GradShared {
   uint64_t full[2];  // S, dO, dR (and K, Q, the decays); dS', Y
 };
 // A tile [64 of dv][8 NT] in f32, as four warps' lanes hold it, that a block turns into two bf16 parts of it, [2][64][LD], at the same
-// place: read by all, a barrier, written.
+// place: read by all, a barrier, written. (What it is needed for, dq and dk, is rounded to bf16. Written as parts by the chains, four
+// bytes at a time, the three kernels took 1,480 us for 64 x 512 tokens of 8 heads; so they take 1,330.)
 template <int NT>
 struct F32Tile {
   static constexpr int N = NT * 128 / kGradThreads;
@@ -1035,7 +1040,7 @@ struct F32Tile {
 };
 // A block per chunk and key head, 16 warps: its value heads one after the other, so that what they add to dq and dk stays in
 // registers and is added in their order; of each, 64 columns of v after the other (a step). A step's loads are under
-// way during the one before it. 4,096 chunks of a head in 534 us: 35,000 clocks each, of which the products take 16,000.
+// way during the one before it. 4,096 chunks of a head in 474 us: 31,000 clocks each, of which the products take 15,000.
 template <int DK>
 __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs p) {
   grid_wait();

@@ -1,5 +1,5 @@
 // What the kernels of the gated delta rule share: the cut of packed sequences into chunks of 64 tokens, copies of tiles
-// into shared memory, and products of bf16 tiles whose f32 operands are carried as two bf16 parts.
+// into shared memory, and products of bf16 tiles whose f32 operands are carried as two or three bf16 parts.
 #pragma once
 #include <type_traits>
 

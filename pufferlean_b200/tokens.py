@@ -139,12 +139,11 @@ def delta_rule(q, k, v, g, beta, offsets=None, state=None, scale=None, save=Fals
     offsets[s] to offsets[s + 1]; None: as many sequences of one length as `state` has (one without a state). Rows outside all
     sequences get zeros. g = -inf forgets the (finite) state: an episode's first token. With keys of length one and beta below 2
     the rule is stable. `saved` (None without save) is what delta_rule_grad takes: for 64 tokens of a head of 128 x 128 with a
-    key head of its own 163 KB, three times what q, k and v hold.
+    key head of its own 198 KB, four times what q, k and v hold.
 
     All inputs but g have to be finite: 64 tokens are worked on at once, so a NaN or an infinity (one that an unstable rule has
     come to, too) reaches any token of its sequence in its 64 and behind them, past a g of -inf as well; other sequences and
-    heads stay clean, and a sequence's first token with g = -inf forgets any state. f32 results are 5e-6 of their norm off
-    as a rule, up to 1e-4 where terms cancel: products carry f32 operands, states among them, as two bf16 parts."""
+    heads stay clean, and a sequence's first token with g = -inf forgets any state."""
     if offsets is not None:
         sequences = offsets.shape[0] - 1
     else:
@@ -156,14 +155,13 @@ def delta_rule(q, k, v, g, beta, offsets=None, state=None, scale=None, save=Fals
 def delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved, scale=None):
     """(dq, dk, dv, dg, dbeta, dstate) of delta_rule from the gradients do [N, Hv, dv] bf16 of o and dstate of the final
     state (None: zero); the last of the results is that of the first state. The other arguments are the forward call's, `saved`
-    what it returned, with the values of q, k, v, g and beta that count (changed ones in between change nothing). dq, dk, dv
-    bf16, dg, dbeta, dstate f32."""
+    what it returned, with the values of q, k, g and beta that count; v is read again. dq, dk, dv bf16, dg, dbeta, dstate f32."""
     if saved is None:
         raise PufferError("delta_rule_grad: saved is needed (delta_rule with save=True)")
     return _ext.delta_rule_grad(q, k, v, g, beta, offsets, saved[1], do, dstate, _scale(q, scale), saved[0])
 
 
 def delta_rule_step(q, k, v, g, beta, state, scale=None, out=None):
-    """(o, state): delta_rule for one token of every row, in f32, state [N, Hv, dk, dv]. The new states go into `out`, which may
+    """(o, state): delta_rule for one token of every row, state [N, Hv, dk, dv] f32. The new states go into `out`, which may
     be `state` itself, or a new tensor. A g of -inf forgets any state, one that is not finite too."""
     return _ext.delta_rule_step(q, k, v, g, beta, state, _scale(q, scale), out)

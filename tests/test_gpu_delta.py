@@ -209,22 +209,44 @@ def test_long_sequence_and_offsets():
 
 @pytest.mark.parametrize("lengths", [[64], [300], [2500], [130, 64, 1, 700]])
 @pytest.mark.parametrize("dk,dv,reset", [(128, 64, 0.0), (64, 72, 0.01), (40, 130, 0.0)])
-def test_both_parts_of_every_operand(lengths, dk, dv, reset):
-    """f32 results by norm. An operand's two bf16 parts are at most 2^-18 of its value off, and so is the product of the second
-    parts, which is left out: 3 * 2^-18 in all for a product of two such operands, of signs that have nothing to do with each
-    other. A result passes through five to twelve products, whose errors add up by squares to sqrt(12) * 3 * 2^-18 at most, and
-    the rule contracts: 4e-5. A second part that is lost is 2^-9, fifty times as much, of its operand."""
+@pytest.mark.parametrize("decay", [1.0, 0.0])
+def test_f32_results(lengths, dk, dv, reset, decay):
+    """f32 results by norm, with decays and without any. Products of three bf16 parts hold all of an f32 operand; their sums are cut off
+    towards zero at each of their 4 to 8 steps of 16, by 2^-23 at most and half of it on average: 4 * 2^-23, and 2^-22 for the
+    decays' exponentials. A result passes through five to twelve products, whose errors add up by squares: sqrt(12) * 6 * 2^-23. Two
+    parts of an operand would be 2^-18 off."""
     q, k, v, g, beta, offsets, state, do, dstate = _inputs(lengths, 1, 2, dk, dv, dk + len(lengths), reset=reset)
+    g = torch.where(torch.isinf(g), g, g * decay)
     o, final, saved = tokens.delta_rule(q, k, v, g, beta, offsets, state, save=True)
     grads = tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved)
     _, rfinal, rgrads, _ = _ref(q, k, v, g, beta, offsets, state, dk ** -0.5, do, dstate)
-    tol = math.sqrt(12) * 3 * 2.0 ** -18
+    tol = math.sqrt(12) * 6 * 2.0 ** -23
     floor = 2.0 ** -23 * float((q.double().norm(dim=2) * rgrads[0].norm(dim=2)).norm()
                                + (k.double().norm(dim=2) * rgrads[1].norm(dim=2)).norm()) * 8
     _near(final, rfinal, tol, "final")
     _near(grads[3], rgrads[3], tol, "dg", floor)
     _near(grads[4], rgrads[4], tol, "dbeta")
     _near(grads[5], rgrads[5], tol, "dstate")
+
+
+def test_tokens_that_write_nothing():
+    """beta zero, or next to it: the token leaves the state as it is, has no dv, and still a dbeta."""
+    q, k, v, g, beta, offsets, state, do, dstate = _inputs([150, 70, 64], 2, 4, 64, 72, 23, reset=0.02)
+    beta[::3] = 0.0
+    beta[1::7] = 1e-20
+    beta[64:128] = 0.0  # a chunk's worth
+    o, final, saved = tokens.delta_rule(q, k, v, g, beta, offsets, state, save=True)
+    grads = tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved)
+    ro, rfinal, rgrads, _ = _ref(q, k, v, g, beta, offsets, state, 0.125, do, dstate)
+    assert (grads[2][beta == 0] == 0).all()
+    _near(o, ro, B, "o")
+    tol = math.sqrt(12) * 6 * 2.0 ** -23
+    floor = 2.0 ** -20 * float((q.double().norm(dim=2) * rgrads[0].norm(dim=2)).norm()
+                               + (k.double().norm(dim=2) * rgrads[1].norm(dim=2)).norm())
+    for name, x, r in zip(("final", "dq", "dk", "dv", "dg", "dbeta", "dstate"), (final,) + grads, [rfinal] + rgrads):
+        _near(x, r, B if x.dtype == BF16 else tol, name, floor if name == "dg" else 0.0)
+    zero = beta == 0
+    _near(grads[4][zero], rgrads[4][zero], tol, "dbeta where beta is zero")
 
 
 def _same(got, want):
@@ -270,7 +292,7 @@ def test_gradients_take_what_was_saved():
     q, k, v, g, beta, offsets, state, do, dstate = _inputs([130, 7], 2, 4, 32, 32, 6)
     _, _, saved = tokens.delta_rule(q, k, v, g, beta, offsets, state, save=True)
     want = tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved)
-    for t in (q, k, g, beta):  # (v is read again)
+    for t in (q, k, g, beta):  # (all but v)
         t.fill_(math.nan)
     assert _same(tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved), want)
 
