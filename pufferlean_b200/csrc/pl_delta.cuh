@@ -388,6 +388,11 @@ __device__ __forceinline__ float exp2_of(float x) {  // 2^-22 off; zero below 2^
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
   return e;
 }
+// The same of an f64 exponent: what its f32 leaves, up to 4e-6 of the result far below zero, is multiplied in.
+__device__ __forceinline__ float exp2_of(double x) {
+  const float hi = (float)x;
+  return exp2_of(hi) * __fmaf_rn((float)(x - (double)hi), 0.69314718f, 1.f);
+}
 struct Gates {
   float g[2], beta[2];  // of tokens lane and lane + 32, in the block's first warp
 };
@@ -438,8 +443,8 @@ __device__ __forceinline__ void chunk_decay(Decay& d, const Gates& r) {
       const float hi = (float)cum[half];
       d.cum[t] = make_float2(hi, (float)(cum[half] - (double)hi));
       d.era[t] = era[half];
-      d.since[t] = era[half] == 0 ? exp2_of(hi) : 0.f;
-      d.until[t] = era[half] == last ? exp2_of((float)(end - cum[half])) : 0.f;
+      d.since[t] = era[half] == 0 ? exp2_of(cum[half]) : 0.f;
+      d.until[t] = era[half] == last ? exp2_of(end - cum[half]) : 0.f;
     }
   }
 }

@@ -229,6 +229,18 @@ def test_f32_results(lengths, dk, dv, reset, decay):
     _near(grads[5], rgrads[5], tol, "dstate")
 
 
+@pytest.mark.parametrize("g0", [-0.5, -1.0, -1.9])
+def test_states_that_fade(g0):
+    """What reaches a state through 40 tokens that keep little of it is right relative to itself, though it is 2^-29 to 2^-110."""
+    q, k, v, g, beta, offsets, state, do, dstate = _inputs([40, 7], 2, 2, 64, 64, 29)
+    g = g0 + 0.1 * g
+    _, _, saved = tokens.delta_rule(q, k, v, g, beta, offsets, state, save=True)
+    grads = tokens.delta_rule_grad(torch.zeros_like(do), dstate, q, k, v, g, beta, offsets, saved)
+    _, _, rgrads, _ = _ref(q, k, v, g, beta, offsets, state, 0.125, torch.zeros_like(do), dstate)
+    for s in (0, 1):
+        _near(grads[5][s], rgrads[5][s], math.sqrt(12) * 6 * 2.0 ** -23, "dstate")
+
+
 def test_tokens_that_write_nothing():
     """beta zero, or next to it: the token leaves the state as it is, has no dv, and still a dbeta."""
     q, k, v, g, beta, offsets, state, do, dstate = _inputs([150, 70, 64], 2, 4, 64, 72, 23, reset=0.02)
