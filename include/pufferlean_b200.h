@@ -604,7 +604,7 @@ int pl_sample_dev(const void* logits, size_t ld, size_t rows, size_t V, uint8_t 
  * not falling; NULL: `sequences` of equal length). Tokens in front of the first and behind the last belong to none: their outputs
  * are zero. state (NULL: zero) and final_state are [sequences][heads_v][dk][dv] f32. Either saved, for the gradient
  * (pl_delta_saved bytes: for 64 tokens of a head of 128 x 128 with a key head of its own 198 KB, four times what q, k and v
- * hold), or ws (pl_delta_ws bytes) is needed, 256-byte aligned. A wait for copies that ran out
+ * hold), or ws (pl_delta_ws bytes; the gradient's, grad = 1, serve either call) is needed, 256-byte aligned. A wait for copies that ran out
  * (pl_device_check) leaves results that are not valid. */
 typedef struct {
   size_t tokens, sequences, heads_k, heads_v, dk, dv;

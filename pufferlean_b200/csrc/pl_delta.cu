@@ -472,8 +472,8 @@ __device__ __forceinline__ uint32_t across_at(const __nv_bfloat16* tile, int n) 
 
 // A block per sequence, value head and 64 columns of v. A warp of the chain has 16 columns of the state, transposed [16][dk], and
 // everything that a chunk makes of it: an accumulator's layout is that of a first operand, so K S, R, Y and F U go from one product
-// into the next as they are, split into bf16 parts. The state is in shared memory, f32, as its lanes hold it (in registers,
-// as before there were sums of parts of their own, 390 bytes spilled: 880 us instead of 704); the sums of a chunk are added to it in f32. What
+// into the next as they are, split into bf16 parts. The state is in shared memory, f32, as its lanes hold it (in registers, beside
+// sums of parts of their own, 390 bytes spilled: 880 us instead of 704); the sums of a chunk are added to it in f32. What
 // the next chunk's state does not wait for is another warp's, which reads the state and Y there: Q S and P U; a third one's is
 // what goes from and to memory.
 // A chunk takes 5.3 us, 9,900 clocks. Its products are 504 and, with or without a gradient, 312 or 188 of 16 x 8 x 16 for each
@@ -1395,7 +1395,8 @@ size_t pl_delta_saved(const pl_delta_shape* s) {
 }
 size_t pl_delta_ws(const pl_delta_shape* s, uint8_t grad) {
   if (!s || s->sequences == 0) return 0;
-  return grad ? pl::states_bytes(s) + pl::lanes_bytes(s) + pl::sums_bytes(s) : pl::mats_bytes(s);
+  const size_t forward = pl::mats_bytes(s), back = pl::states_bytes(s) + pl::lanes_bytes(s) + pl::sums_bytes(s);
+  return !grad ? forward : (back > forward ? back : forward) + 256;  // the gradient's serves the forward call, too
 }
 
 int pl_delta_dev(const pl_delta_shape* s, const void* q, const void* k, const void* v, const float* g, const float* beta,

@@ -103,7 +103,8 @@ def test_both_sides_of_a_split(n, v, dtype):
         a = tokens.sample(x, u, *(o.get(key, d) for key, d in (("temp", 1.0), ("k", 0), ("p", 1.0))))
         _check(x[:4], u[:4], **o)
         many = 70 if n < 70 else n
-        b = tokens.sample(x.repeat(-(-many // n), 1)[:many], u.repeat(-(-many // n))[:many],
+        times = -(-many // n)
+        b = tokens.sample(x.repeat(times, 1)[:many], u.repeat(times)[:many],
                           *(o.get(key, d) for key, d in (("temp", 1.0), ("k", 0), ("p", 1.0))))
         assert torch.equal(a[0], b[0][:n]) and (a[1] - b[1][:n]).abs().max() <= 2.0 ** -22 * a[1].abs().max()
 
