@@ -699,7 +699,8 @@ struct BackArgs {
   float *ds, *dr;               // dS' and dR of every slot
   float* sums;                  // sums_at
 };
-// Per slot, value head and 16 columns of v, sums over them: of every token Y . Z beta' and o . dO - v . dR, of the chunk <S', dS'>.
+// Per slot, value head and 16 columns of v, sums over them: of every token Y . Z beta' and o . dO - v . dR; of the chunk <S', dS'> and
+// <S, dS>, which is dg of its first token (zero, not nearly zero, without a state).
 constexpr int kSums = 2 * kC + 2;
 __device__ __forceinline__ long sums_at(const DeltaArgs& a, long slot, int h, int group) {
   return ((slot * a.hv + h) * (a.dvp / 16) + group) * kSums;
@@ -833,6 +834,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
         give(sh.s[warp], t, v);
       });
     }
+    if (chunks) meet<kChainThreads>(kAll);
 #pragma unroll
     for (int t = 0; t < NK; t++) take(sh.s[warp], t, s[t]);
     if (p.dstate) state_out(s, p.dstate + sbase, a.dk, a.dv, mine);
@@ -891,6 +893,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
       });
       meet_arrive<64>(q_ready);
     }
+    if (chunks) meet<kChainThreads>(kAll);
     return;
   }
   // memory
@@ -911,6 +914,28 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
   if (chunks) load(chunks - 1);
   cp_commit();
   zero_rows<128>(a, seq, p.dv + (long)h * a.dv + c0, (long)a.hv * a.dv, cols, tid);
+  float s[NK][4];  // S before a slot's chunk, and its product with the gradient in shared memory: this lane's part
+  auto load_s = [&](long slot) {
+    const uint4* from_s = states_at(a, p.kept, slot, h, slice, warp);
+#pragma unroll
+    for (int t = 0; t < NK; t++) take(from_s, t, s[t]);
+  };
+  auto inner = [&] {
+    float f = 0.f;
+#pragma unroll
+    for (int t = 0; t < NK; t++) {
+      float v[4];
+      take(sh.s[warp], t, v);
+#pragma unroll
+      for (int e = 0; e < 4; e++) f = __fmaf_rn(s[t][e], v[e], f);
+    }
+    return f;
+  };
+  auto warp_total = [](float f) {
+#pragma unroll
+    for (int w = 16; w; w >>= 1) f += __shfl_xor_sync(0xffffffffu, f, w);
+    return f;
+  };
   const bool vec_dv = a.dv % 8 == 0 && (uintptr_t)p.dv % 16 == 0;
   for (long c = chunks - 1; c >= 0; c--) {
     const long start = from + c * kC, slot = slot0 + c;
@@ -922,18 +947,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     cp_commit();
     if (c > 0) load(c - 1);
     cp_commit();
-    const uint4 *sf = states_at(a, p.kept, slot, h, slice, warp), *yf = lanes_at(a, p.y, slot, h, slice, warp);
-    const uint4* of = lanes_at(a, p.out, slot, h, slice, warp);
+    const uint4 *yf = lanes_at(a, p.y, slot, h, slice, warp), *of = lanes_at(a, p.out, slot, h, slice, warp);
+    load_s(slot);
     lanes_out(states_at(a, p.ds, slot, h, slice, warp), sh.s[warp], sizeof(sh.s[0]));
-    float fu = 0.f;  // <S, dS'> over 16 columns
-#pragma unroll
-    for (int t = 0; t < NK; t++) {
-      float u[4], v[4];
-      take(sf, t, u);
-      take(sh.s[warp], t, v);
-#pragma unroll
-      for (int e = 0; e < 4; e++) fu = __fmaf_rn(u[e], v[e], fu);
-    }
+    float fu = inner();
     meet_arrive<kChainThreads>(kRead);
     float y[8][4], o[8][4];
 #pragma unroll
@@ -982,11 +999,19 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const Back
     float* sums = p.sums + sums_at(a, slot, h, slice * 4 + warp);
     reinterpret_cast<float2*>(sums)[lane] = column_sums(zy);
     reinterpret_cast<float2*>(sums + kC)[lane] = column_sums(ov);
-#pragma unroll
-    for (int w = 16; w; w >>= 1) fu += __shfl_xor_sync(0xffffffffu, fu, w);
-    if (lane == 0) sums[2 * kC] = fu;
+    fu = warp_total(fu);
+    if (lane == 0) {
+      sums[2 * kC] = fu;
+      if (c + 1 < chunks) p.sums[sums_at(a, slot + 1, h, slice * 4 + warp) + 2 * kC + 1] = fu;
+    }
     __syncwarp();
     rows_out(in.x + warp * 16, p.dv + start * a.hv * a.dv + (long)h * a.dv + w0, (long)a.hv * a.dv, len, mine, vec_dv);
+  }
+  if (chunks) {
+    load_s(slot0);
+    meet<kChainThreads>(kAll);
+    const float f = warp_total(inner());
+    if (lane == 0) p.sums[sums_at(a, slot0, h, slice * 4 + warp) + 2 * kC + 1] = f;
   }
   tc::bulk_wait<0>();
 }
@@ -1012,7 +1037,7 @@ struct GradShared {
   __nv_bfloat16 o[2][kC * kLd], r[2][2][kC * kLd];  // by turns: the next step's are on their way
   __nv_bfloat16 s[2][kC * (DK + 8)], ds[2][kC * (DK + 8)], y[2][kC * kLd];  // transposed, as r
   __nv_bfloat16 p[2][kC * kLd], m[2][kC * kLd];     // scale dO U^T * D, -M
-  float gate[2 * kC + 1];
+  float gate[2 * kC + 2];
   Decay decay[2];  // by turns, a head's
   uint64_t full[2];  // S, dO, dR (and K, Q, the decays); dS', Y
 };
@@ -1109,10 +1134,20 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
         for (int g = 0; g < a.dvp / 16; g++) v += sums[g * kSums + tid];
         sh.gate[tid] = v;
       } else if (warp == 4) {
-        for (int g = lane; g < a.dvp / 16; g += 32) v += sums[g * kSums + 2 * kC];
+        float u = 0.f;
+        for (int g = lane; g < a.dvp / 16; g += 32) {
+          v += sums[g * kSums + 2 * kC];
+          u += sums[g * kSums + 2 * kC + 1];
+        }
 #pragma unroll
-        for (int w = 16; w; w >>= 1) v += __shfl_xor_sync(0xffffffffu, v, w);
-        if (lane == 0) sh.gate[2 * kC] = v;
+        for (int w = 16; w; w >>= 1) {
+          v += __shfl_xor_sync(0xffffffffu, v, w);
+          u += __shfl_xor_sync(0xffffffffu, u, w);
+        }
+        if (lane == 0) {
+          sh.gate[2 * kC] = v;
+          sh.gate[2 * kC + 1] = u;
+        }
       }
     }
     cp_wait<0>();
@@ -1228,7 +1263,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const GradArgs
         const int i = half * 32 + lane;
         const int before = __shfl_up_sync(0xffffffffu, era[half], 1), across = __shfl_sync(0xffffffffu, era[0], 31);
         const bool reset = era[half] != (lane ? before : half ? across : 0);
-        if (i < len) p.dg[(start + i) * a.hv + h] = reset ? 0.f : v;
+        if (i < len) p.dg[(start + i) * a.hv + h] = reset ? 0.f : i == 0 ? sh.gate[2 * kC + 1] : v;
         behind = __shfl_sync(0xffffffffu, v, 0);
         behind_era = __shfl_sync(0xffffffffu, era[half], 0);
       }

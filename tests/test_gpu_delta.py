@@ -229,6 +229,21 @@ def test_f32_results(lengths, dk, dv, reset, decay):
     _near(grads[5], rgrads[5], tol, "dstate")
 
 
+@pytest.mark.parametrize("state", [None, 0.0])
+def test_first_tokens_of_an_empty_memory(state):
+    """Nothing depends on what a first token keeps of no state: its dg is zero, not nearly; and right where there is a state."""
+    q, k, v, g, beta, offsets, st, do, dstate = _inputs([1, 1, 70, 1, 130], 2, 4, 72, 100, 37)
+    first = offsets[:-1].long()
+    given = None if state is None else torch.zeros_like(st)
+    _, _, saved = tokens.delta_rule(q, k, v, g, beta, offsets, given, save=True)
+    dg = tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved)[3]
+    assert (dg[first] == 0).all() and (dg[first[2] + 1] != 0).all()
+    _, _, saved = tokens.delta_rule(q, k, v, g, beta, offsets, st, save=True)
+    dg = tokens.delta_rule_grad(do, dstate, q, k, v, g, beta, offsets, saved)[3]
+    _, _, rgrads, _ = _ref(q, k, v, g, beta, offsets, st, 72 ** -0.5, do, dstate)
+    _near(dg[first], rgrads[3][first], math.sqrt(12) * 6 * 2.0 ** -23, "dg")
+
+
 @pytest.mark.parametrize("g0", [-0.5, -1.0, -1.9])
 def test_states_that_fade(g0):
     """What reaches a state through 40 tokens that keep little of it is right relative to itself, though it is 2^-29 to 2^-110."""
