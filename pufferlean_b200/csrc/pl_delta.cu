@@ -733,7 +733,7 @@ struct BackShared {
 // As the chain forward, from the last chunk to the first. The helpers' products, of dO with P and Q, need nothing of the chain; they add
 // theirs to dS' when the chain and memory have read it, the chain its own after that.
 // Memory's warps also make the gates' gradients of what passes through them, in f32: dbeta is Z . Y, token by token (X^T beta dU is
-// beta Z; where beta is zero, a tiny one stands in), and dg is sums of o . dO - v . dR. 64 x 512 tokens of 8 heads of 128 x 128: 451 us,
+// beta Z; where beta is zero, a tiny one stands in), and dg is sums of o . dO - v . dR. 64 x 512 tokens of 8 heads of 128 x 128: 465 us,
 // where its 1.7 GB would take 260 (forward, with what the gradient needs written out: 392 to 402).
 template <int DK>
 __global__ void __launch_bounds__(kChainThreads, 1) delta_back_kernel(const BackArgs p) {
@@ -1043,7 +1043,7 @@ struct GradShared {
 };
 // A tile [64 of dv][8 NT] in f32, as four warps' lanes hold it, that a block turns into two bf16 parts of it, [2][64][LD], at the same
 // place: read by all, a barrier, written. (What it is needed for, dq and dk, is rounded to bf16. Written as parts by the chains, four
-// bytes at a time, the three kernels took 1,480 us for 64 x 512 tokens of 8 heads; so they take 1,330.)
+// bytes at a time, the three kernels took 1,480 us for 64 x 512 tokens of 8 heads; so they take 1,340.)
 template <int NT>
 struct F32Tile {
   static constexpr int N = NT * 128 / kGradThreads;
